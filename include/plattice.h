@@ -45,7 +45,7 @@
 extern "C" {
 #endif
 
-#define PLATTICE_ABI_VERSION 5
+#define PLATTICE_ABI_VERSION 6
 
 /* status codes */
 #define PLATTICE_OK 0
@@ -281,6 +281,91 @@ int plattice_noalloc_status(int* status, int* m, void* stream);
 void plattice_profile_enable(int on);
 int plattice_profile_read(double* ms_total, int* launches, int n_stages);
 const char* plattice_profile_stage_name(int stage);
+
+/* Row operators (no reference counterpart): what a network needs on either
+ * side of the filter, where its features and values are learned.  A row is a
+ * pixel's channels; tensors are [rows][channels], contiguous, on the current
+ * device.  No call synchronises.
+ *
+ * Element types.  Parameters (gain, bias) and their gradients may be of any of
+ * the three types; all other tensors of a call share one. */
+#define PLATTICE_F32 0
+#define PLATTICE_BF16 1
+#define PLATTICE_F16 2
+
+/* Activations of plattice_linear: x, max(x, 0), x Phi(x), x / (1 + exp(-x)). */
+#define PLATTICE_ACT_NONE 0
+#define PLATTICE_ACT_RELU 1
+#define PLATTICE_ACT_GELU 2
+#define PLATTICE_ACT_SILU 3
+
+/* 8-bit rows of [rows][c]: codes q [rows][cp] (e4m3, cp = c rounded up to 32,
+ * zeros behind the last channel) and scale [rows][cp / 32]; channel i of a row
+ * stands for q[i] * 2^(scale[i / 32] - 127).  The power of two is the smallest
+ * with which the block's largest finite magnitude is at most 448 (the exponent
+ * is held in -110..120); a value that is not finite comes back as NaN and its
+ * neighbours are kept.  q is 16-byte aligned.  Rounding: at most 2^-4 of a
+ * value, or 2^-10 of the scale for small ones. */
+int plattice_rows_pack8(uint8_t* q, uint8_t* scale, const void* x, int dtype, long long rows, int c, void* stream);
+int plattice_rows_unpack8(void* y, int dtype, const uint8_t* q, const uint8_t* scale, long long rows, int c,
+                          void* stream);
+
+/* Root-mean-square norm of h = x + residual (residual NULL: h = x):
+ *   rstd[r] = 1 / sqrt(mean_c h[r][c]^2 + eps),  y = h * rstd * gain.
+ * h is stored in the rows' type unless NULL (may be x or residual itself: each
+ * row is read before it is written).  yscale non-NULL: y is 8-bit rows (codes
+ * in y, scales in yscale).  c <= PLATTICE_NORM_MAX_CHANNELS. */
+#define PLATTICE_NORM_MAX_CHANNELS 16384
+int plattice_rms_norm(void* y, uint8_t* yscale, void* h, float* rstd, const void* x, const void* residual,
+                      const void* gain, int dtype, int gain_dtype, float eps, long long rows, int c, void* stream);
+
+/* Its gradients, with n = h * rstd and gn = grad_y * gain:
+ *   grad_x = rstd (gn - n mean(gn n)) + grad_h   (of x and of the residual),
+ *   grad_gain = sum over the rows of grad_y n    (in the gain's type).
+ * grad_h (the gradient of h from elsewhere) may be NULL. */
+int plattice_rms_norm_backward_workspace_size(long long rows, int c, size_t* bytes);
+int plattice_rms_norm_backward(void* grad_x, void* grad_gain, const void* grad_y, const void* h, const float* rstd,
+                               const void* gain, const void* grad_h, void* workspace, size_t workspace_bytes,
+                               int dtype, int gain_dtype, long long rows, int c, void* stream);
+
+/* Linear map of rows: z = x w^T + bias, y = act(z) + residual, with x [rows][k],
+ * w [n][k].  dtype: the type of x and w (x_scale non-NULL: x is 8-bit rows and
+ * w is float32 or bfloat16).  out_dtype: of y, residual, a kept z and the
+ * incoming gradient: dtype or PLATTICE_F32.  split > 0: columns 0..split-1 go
+ * to y0 [rows][split] and the others to y1 [rows][n - split] (0 < split < n; no
+ * residual, no activation): the features and values of a filter call.
+ * z non-NULL (forward): the pre-activation is kept there, as 8-bit rows when
+ * z_scale is non-NULL, else in out_dtype.
+ *
+ * Backward, with gz = grad_y act'(z) (z as kept, or NULL without activation):
+ *   grad_x = gz w, grad_w = gz^T x (both in dtype), grad_bias = sum_r gz
+ * (bias_dtype); each output may be NULL.  gz is rounded to dtype before the
+ * two products.  Sums are held in float32 and added in a fixed order. */
+typedef struct plattice_linear_args {
+    const void* x;
+    const uint8_t* x_scale;
+    const void* w;
+    const void* bias;           /* forward: NULL for none */
+    const void* residual;       /* forward: NULL for none */
+    void* y0;                   /* forward */
+    void* y1;
+    void* z;                    /* forward: output; backward: input */
+    uint8_t* z_scale;
+    const void* grad0;          /* backward: gradient of y0 (and y1) */
+    const void* grad1;
+    void* grad_x;
+    void* grad_w;
+    void* grad_bias;
+    void* workspace;            /* 256-byte aligned */
+    size_t workspace_bytes;
+    long long rows;
+    int k, n, split;
+    int dtype, out_dtype, bias_dtype, act;
+} plattice_linear_args;
+int plattice_linear_workspace_size(const plattice_linear_args* args, size_t* bytes);
+int plattice_linear(const plattice_linear_args* args, void* stream);
+int plattice_linear_backward_workspace_size(const plattice_linear_args* args, size_t* bytes);
+int plattice_linear_backward(const plattice_linear_args* args, void* stream);
 
 #ifdef __cplusplus
 }

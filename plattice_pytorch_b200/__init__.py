@@ -5,9 +5,9 @@ module (forward / backward) and ``plattice_pytorch_b200.plattice`` its
 plattice.py (PermutoLatticeFunction, PermutoLattice).  The work is done by
 libplattice_b200.so through the C ABI of include/plattice.h.
 """
-from . import PLOO
+from . import PLOO, rows
 from .plattice import (LatticeFilterFunction, PermutoLattice, PermutoLatticeBatchFunction,
                        PermutoLatticeFeatureFunction, PermutoLatticeFunction)
 
-__all__ = ["PLOO", "PermutoLattice", "PermutoLatticeFunction", "PermutoLatticeBatchFunction",
+__all__ = ["PLOO", "rows", "PermutoLattice", "PermutoLatticeFunction", "PermutoLatticeBatchFunction",
            "PermutoLatticeFeatureFunction", "LatticeFilterFunction"]

@@ -13,7 +13,15 @@ LIB_PATH = os.path.join(HERE, "libplattice_b200.so")
 
 OK, ERR_INVALID, ERR_WORKSPACE, ERR_CUDA, ERR_DEVICE = 0, 1, 2, 3, 4
 DEV_TABLE_FULL, DEV_WAIT_LIMIT, DEV_ROUND_LIMIT = 2, 4, 8
-ABI_VERSION = 5
+ABI_VERSION = 6
+
+class LinearArgs(ctypes.Structure):
+    """plattice_linear_args of include/plattice.h."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "x_scale", "w", "bias", "residual", "y0", "y1", "z", "z_scale",
+                                               "grad0", "grad1", "grad_x", "grad_w", "grad_bias", "workspace")]
+                + [("workspace_bytes", ctypes.c_size_t), ("rows", ctypes.c_longlong)]
+                + [(n, ctypes.c_int) for n in ("k", "n", "split", "dtype", "out_dtype", "bias_dtype", "act")])
+
 
 _lock = threading.Lock()
 _lib = None
@@ -116,6 +124,22 @@ def lib():
         L.plattice_profile_read.argtypes = [ctypes.POINTER(ctypes.c_double), ctypes.POINTER(I), I]
         L.plattice_profile_stage_name.restype = ctypes.c_char_p
         L.plattice_profile_stage_name.argtypes = [I]
+        LL, A = ctypes.c_longlong, ctypes.POINTER(LinearArgs)
+        L.plattice_rows_pack8.restype = I
+        L.plattice_rows_pack8.argtypes = [P, P, P, I, LL, I, P]
+        L.plattice_rows_unpack8.restype = I
+        L.plattice_rows_unpack8.argtypes = [P, I, P, P, LL, I, P]
+        L.plattice_rms_norm.restype = I
+        L.plattice_rms_norm.argtypes = [P, P, P, P, P, P, P, I, I, ctypes.c_float, LL, I, P]
+        L.plattice_rms_norm_backward_workspace_size.restype = I
+        L.plattice_rms_norm_backward_workspace_size.argtypes = [LL, I, ctypes.POINTER(S)]
+        L.plattice_rms_norm_backward.restype = I
+        L.plattice_rms_norm_backward.argtypes = [P, P, P, P, P, P, P, P, S, I, I, LL, I, P]
+        for name in ("plattice_linear", "plattice_linear_backward"):
+            getattr(L, name).restype = I
+            getattr(L, name).argtypes = [A, P]
+            getattr(L, name + "_workspace_size").restype = I
+            getattr(L, name + "_workspace_size").argtypes = [A, ctypes.POINTER(S)]
         v = L.plattice_abi_version()
         if v != ABI_VERSION:
             raise ImportError(f"{LIB_PATH} has ABI version {v}, expected {ABI_VERSION}: rebuild it")

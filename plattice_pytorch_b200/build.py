@@ -1,8 +1,9 @@
 """Build libplattice_b200.so (sm_100a) in-tree with nvcc.
 
 The 16 feature dimensions are separate translation units (plattice_pd.cu with
--DPL_PD=n) compiled in parallel, plus the C-ABI unit; objects go to
-plattice_pytorch_b200/_build/, the library next to this file.  Rebuilds only
+-DPL_PD=n) compiled in parallel, plus the C-ABI unit and the row operators
+(rows_*.cu); objects go to plattice_pytorch_b200/_build/, the library next to
+this file.  Rebuilds only
 what is older than its sources.
 
     python -m plattice_pytorch_b200.build [--jobs N] [--verbose-ptxas]
@@ -32,10 +33,13 @@ def nvcc():
     raise RuntimeError("nvcc not found: the CUDA toolkit is required to build libplattice_b200.so")
 
 
-def _deps():
-    return sorted(glob.glob(os.path.join(CSRC, "*.cu")) + glob.glob(os.path.join(CSRC, "*.cuh"))
-                  + glob.glob(os.path.join(CSRC, "*.h")) + [os.path.join(ROOT, "include", "plattice.h"),
-                                                           os.path.abspath(__file__)])
+def _deps(unit):
+    """Sources that the objects of a unit ("plattice" or "rows") are made from:
+    its own files and the headers (the row operators' units include only
+    headers, the lattice's none of the rows_*.cuh)."""
+    files = glob.glob(os.path.join(CSRC, f"{unit}_*.cu")) + glob.glob(os.path.join(CSRC, f"{unit}_*.cuh"))
+    return sorted(files + glob.glob(os.path.join(CSRC, "*.h")) + [os.path.join(ROOT, "include", "plattice.h"),
+                                                                 os.path.abspath(__file__)])
 
 
 def _stale(target, deps):
@@ -53,17 +57,17 @@ def _run(cmd):
 def build(jobs=None, verbose_ptxas=False, force=False):
     """Compile and link; returns the library path."""
     os.makedirs(BUILD, exist_ok=True)
-    deps = _deps()
+    deps = {unit: _deps(unit) for unit in ("plattice", "rows")}
     extra = ["-Xptxas", "-v"] if verbose_ptxas else []
     units = []
     for pd in range(1, 17):
         obj = os.path.join(BUILD, f"plattice_pd{pd}.o")
         units.append((obj, [nvcc()] + NVCC_FLAGS + extra + [f"-DPL_PD={pd}", "-c",
                                                            os.path.join(CSRC, "plattice_pd.cu"), "-o", obj]))
-    for name in ("plattice_capi", "plattice_runtime", "plattice_noalloc"):
+    for name in ("plattice_capi", "plattice_runtime", "plattice_noalloc", "rows_norm", "rows_linear"):
         obj = os.path.join(BUILD, f"{name}.o")
         units.append((obj, [nvcc()] + NVCC_FLAGS + extra + ["-c", os.path.join(CSRC, f"{name}.cu"), "-o", obj]))
-    todo = [(o, c) for o, c in units if force or _stale(o, deps)]
+    todo = [(o, c) for o, c in units if force or _stale(o, deps[os.path.basename(o).split("_")[0]])]
     if todo:
         jobs = jobs or max(1, min(len(todo), os.cpu_count() or 4))
         with cf.ThreadPoolExecutor(jobs) as ex:

@@ -14,6 +14,7 @@
 #include "../../include/plattice.h"
 #include "plattice_impl.cuh"
 #include "plattice_runtime.h"
+#include "rows_host.h"
 
 namespace pl {
 #define PL_DECLARE_PD(N)                                                                    \
@@ -771,3 +772,11 @@ void plattice_graph_cache_stats(long long* captures, long long* replays) {
 }
 
 }  // extern "C"
+
+// ---------------------------------------------------------------- row operators
+
+namespace plr {
+int rows_status(cudaError_t e, const char* call) { return cuda_status(e, call); }
+int rows_poll(const char* call) { return poll_earlier(call); }
+int sm_count() { return sm_count_current(); }
+}  // namespace plr

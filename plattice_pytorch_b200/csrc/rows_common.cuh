@@ -1,0 +1,195 @@
+// rows_common.cuh -- what the row operators share: element types, loads and
+// stores of 8 consecutive channels, the 8-bit row format, the activations.
+//
+// 8-bit rows: a [rows][c] tensor as e4m3 codes [rows][cp], cp = c rounded up
+// to 32 (codes behind the last channel are 0), and one byte per 32 channels,
+// 127 + s: the codes stand for code * 2^s.  2^s is the smallest power of two
+// with amax <= 448 * 2^s (448: the largest e4m3 value), so nothing saturates
+// and a block's largest value keeps at least 3 mantissa bits.  A power of two
+// makes code * 2^s exact in bfloat16 and float32 (4 significant bits), so a
+// product of bfloat16 operands reads the checkpoint without a further
+// rounding.  s is clamped to [-110, 120]: the smallest non-zero value is then
+// 2^-119, a normal number in both types.  A value that is not finite becomes
+// the NaN code and does not enter amax, so its neighbours keep their values.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/plattice.h"
+
+namespace plr {
+
+constexpr int kBlock8 = 32;          // channels that share one scale
+constexpr int kScaleMin = -110, kScaleMax = 120;
+
+__host__ __device__ inline int64_t width8(int64_t c) { return (c + kBlock8 - 1) / kBlock8 * kBlock8; }
+
+// ------------------------------------------------------------- element types
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+
+// The value a parameter (gain, bias) of either type holds.
+__device__ __forceinline__ float load_param(const void* p, int dtype, int64_t i) {
+    if (dtype == PLATTICE_F32) return static_cast<const float*>(p)[i];
+    if (dtype == PLATTICE_BF16) return to_f32(static_cast<const __nv_bfloat16*>(p)[i]);
+    return to_f32(static_cast<const __half*>(p)[i]);
+}
+
+__device__ __forceinline__ void store_param(void* p, int dtype, int64_t i, float v) {
+    if (dtype == PLATTICE_F32) static_cast<float*>(p)[i] = v;
+    else if (dtype == PLATTICE_BF16) static_cast<__nv_bfloat16*>(p)[i] = from_f32<__nv_bfloat16>(v);
+    else static_cast<__half*>(p)[i] = from_f32<__half>(v);
+}
+
+// 8 consecutive elements; `vec`: 16-byte accesses are aligned and all 8 exist,
+// otherwise the first n (n <= 8, also <= 0) are accessed one by one and the
+// others read as 0.
+__device__ __forceinline__ void load8(float (&v)[8], const float* p, bool vec, int n) {
+    if (vec) {
+        const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : 0.f;
+    }
+}
+
+template <typename T> struct Pair;
+template <> struct Pair<__nv_bfloat16> { typedef __nv_bfloat162 type; };
+template <> struct Pair<__half> { typedef __half2 type; };
+__device__ __forceinline__ float2 pair_f32(__nv_bfloat162 v) { return __bfloat1622float2(v); }
+__device__ __forceinline__ float2 pair_f32(__half2 v) { return __half22float2(v); }
+__device__ __forceinline__ void pair_from(__nv_bfloat162& o, float a, float b) { o = __floats2bfloat162_rn(a, b); }
+__device__ __forceinline__ void pair_from(__half2& o, float a, float b) { o = __floats2half2_rn(a, b); }
+
+template <typename T>
+__device__ __forceinline__ void load8(float (&v)[8], const T* p, bool vec, int n) {
+    if (vec) {
+        union { uint4 u; typename Pair<T>::type h[4]; } r;
+        r.u = *reinterpret_cast<const uint4*>(p);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = pair_f32(r.h[i]);
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < n ? to_f32(p[i]) : 0.f;
+    }
+}
+
+__device__ __forceinline__ void store8(float* p, const float (&v)[8], bool vec, int n) {
+    if (vec) {
+        reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < n) p[i] = v[i];
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&v)[8], bool vec, int n) {
+    if (vec) {
+        union { uint4 u; typename Pair<T>::type h[4]; } r;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) pair_from(r.h[i], v[2 * i], v[2 * i + 1]);
+        *reinterpret_cast<uint4*>(p) = r.u;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < n) p[i] = from_f32<T>(v[i]);
+    }
+}
+
+// --------------------------------------------------------------- 8-bit rows
+
+// s of a block whose largest finite magnitude is amax: amax = 1.f * 2^e needs
+// 2^(e-8) when 1.f <= 1.75 (448 = 1.75 * 2^8), twice that otherwise.
+__device__ __forceinline__ int block_exponent(float amax) {
+    const int b = __float_as_int(amax);
+    const int s = (b >> 23) - 135 + ((b & 0x7fffff) > 0x600000);
+    return min(max(s, kScaleMin), kScaleMax);
+}
+
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }   // -126 <= e <= 127
+
+__device__ __forceinline__ float finite_abs(float v) {
+    const float a = fabsf(v);
+    return a <= 3.402823466e38f ? a : 0.f;
+}
+
+// Codes of 8 values times 2^-s (multiplying by a power of two is exact, so
+// the one rounding is the conversion's); not finite -> the NaN code.
+__device__ __forceinline__ uint2 codes8(const float (&v)[8], float inv) {
+    unsigned w[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        float t[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            t[j] = v[4 * i + j];
+            t[j] = fabsf(t[j]) <= 3.402823466e38f ? t[j] * inv : __int_as_float(0x7fffffff);
+        }
+        w[i] = __nv_cvt_float2_to_fp8x2(make_float2(t[0], t[1]), __NV_SATFINITE, __NV_E4M3) |
+               ((unsigned)__nv_cvt_float2_to_fp8x2(make_float2(t[2], t[3]), __NV_SATFINITE, __NV_E4M3) << 16);
+    }
+    return make_uint2(w[0], w[1]);
+}
+
+__device__ __forceinline__ void values4(float* v, unsigned codes, float scale) {
+    const __half2 a(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(codes & 0xffff), __NV_E4M3));
+    const __half2 b(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(codes >> 16), __NV_E4M3));
+    const float2 fa = __half22float2(a), fb = __half22float2(b);
+    v[0] = fa.x * scale; v[1] = fa.y * scale; v[2] = fb.x * scale; v[3] = fb.y * scale;
+}
+
+__device__ __forceinline__ void values8(float (&v)[8], uint2 codes, float scale) {
+    values4(v, codes.x, scale);
+    values4(v + 4, codes.y, scale);
+}
+
+__device__ __forceinline__ float scale_of(uint8_t byte) { return pow2((int)byte - 127); }
+
+// float16 ends at 65504; a block's largest value may round to the next code
+// above it, which stays the largest number rather than becoming infinite.
+template <typename T> __device__ __forceinline__ float within(float v) { return v; }
+template <> __device__ __forceinline__ float within<__half>(float v) {
+    return fabsf(v) <= 3.402823466e38f ? fminf(fmaxf(v, -65504.f), 65504.f) : v;
+}
+
+// -------------------------------------------------------------- activations
+
+__device__ __forceinline__ float act_value(float z, int act) {
+    if (act == PLATTICE_ACT_RELU) return z > 0.f ? z : (z != z ? z : 0.f);
+    if (act == PLATTICE_ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+    if (act == PLATTICE_ACT_SILU) return z / (1.f + __expf(-z));
+    return z;
+}
+
+// d act / d z
+__device__ __forceinline__ float act_slope(float z, int act) {
+    if (act == PLATTICE_ACT_RELU) return z > 0.f ? 1.f : (z != z ? z : 0.f);
+    if (act == PLATTICE_ACT_GELU)
+        return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * __expf(-0.5f * z * z) * 0.39894228040143268f;
+    if (act == PLATTICE_ACT_SILU) {
+        const float s = 1.f / (1.f + __expf(-z));
+        return s * (1.f + z * (1.f - s));
+    }
+    return 1.f;
+}
+
+}  // namespace plr

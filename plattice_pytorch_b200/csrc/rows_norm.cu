@@ -1,0 +1,482 @@
+// rows_norm.cu -- 8-bit rows (pack, unpack) and the root-mean-square norm of
+// rows with the residual's addition, forward and backward.  Formats and
+// element access: rows_common.cuh; C ABI: include/plattice.h.
+#include <limits.h>
+
+#include "plattice_runtime.h"
+#include "rows_common.cuh"
+#include "rows_host.h"
+
+namespace plr {
+
+// ------------------------------------------------------------ pack / unpack
+//
+// A thread takes 8 channels, 4 neighbouring lanes a block of 32.  Both kernels
+// move each byte once and are bound by HBM.  A CTA takes kUnits x 256 such
+// groups of 8, so that each thread has kUnits independent loads in flight.
+
+constexpr int kUnits = 4;
+
+// Splits the flat group index of (CTA base + offset) into row and group: one
+// 64-bit division per CTA, 32-bit ones per thread.
+struct GroupAt {
+    int64_t row0;
+    unsigned rem, groups;
+    __device__ __forceinline__ GroupAt(int64_t base, unsigned groups_) : groups(groups_) {
+        row0 = base / groups;
+        rem = (unsigned)(base - row0 * groups);
+    }
+    __device__ __forceinline__ void at(unsigned offset, int64_t& row, unsigned& g) const {
+        const unsigned t = rem + offset, r = t / groups;
+        row = row0 + r;
+        g = t - r * groups;
+    }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256) k_pack8(uint8_t* __restrict__ q, uint8_t* __restrict__ scale,
+                                               const T* __restrict__ x, int64_t rows, int c, unsigned groups, bool vec) {
+    const int64_t base = (int64_t)blockIdx.x * (256 * kUnits);
+    const GroupAt where(base, groups);
+    float v[kUnits][8];
+    int64_t row[kUnits];
+    unsigned g[kUnits];
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+        where.at(threadIdx.x + 256 * u, row[u], g[u]);
+        const int left = row[u] < rows ? c - (int)g[u] * 8 : 0;
+        load8(v[u], x + (left > 0 ? row[u] * c + (int64_t)g[u] * 8 : 0), vec && left >= 8, left);
+    }
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+        float amax = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) amax = fmaxf(amax, finite_abs(v[u][i]));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        const int s = block_exponent(amax);
+        if (row[u] >= rows) continue;
+        const uint2 w = codes8(v[u], pow2(-s));
+        const int64_t at = row[u] * groups + g[u];
+        reinterpret_cast<uint2*>(q)[at] = w;
+        if ((threadIdx.x & 3) == 0) scale[at >> 2] = (uint8_t)(s + 127);
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) k_unpack8(T* __restrict__ y, int64_t pitch, const uint8_t* __restrict__ q,
+                                                 const uint8_t* __restrict__ scale, int64_t rows, int c,
+                                                 unsigned groups, bool vec) {
+    const int64_t base = (int64_t)blockIdx.x * (256 * kUnits);
+    const GroupAt where(base, groups);
+    uint2 w[kUnits];
+    float sc[kUnits];
+    int64_t row[kUnits];
+    unsigned g[kUnits];
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+        where.at(threadIdx.x + 256 * u, row[u], g[u]);
+        const int64_t at = row[u] < rows ? row[u] * groups + g[u] : 0;
+        w[u] = reinterpret_cast<const uint2*>(q)[at];
+        sc[u] = scale_of(scale[at >> 2]);
+    }
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+        if (row[u] >= rows) continue;
+        float v[8];
+        values8(v, w[u], sc[u]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = within<T>(v[i]);
+        const int left = c - (int)g[u] * 8;
+        if (left > 0) store8(y + row[u] * pitch + (int64_t)g[u] * 8, v, vec && left >= 8, left);
+    }
+}
+
+// --------------------------------------------------------------- the norm
+//
+// L threads share a row (L <= 32: several rows per warp; L = 256 or 512: a CTA
+// per row); a thread holds kChunks groups of 8 channels in registers, so a row
+// is read once whatever its statistics need.  The mean of squares is summed in
+// float32.  h is rounded to the rows' type where it is stored; y is computed
+// from the unrounded sum, one rounding from its definition.
+
+template <int L>
+__device__ __forceinline__ float row_sum(float v, float* red) {
+    constexpr int kWarp = L < 32 ? L : 32;
+#pragma unroll
+    for (int o = kWarp / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (L > 32) {
+        __syncthreads();   // the previous row's sums have been read
+        if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+        __syncthreads();
+        v = 0.f;
+#pragma unroll
+        for (int i = 0; i < L / 32; ++i) v += red[i];
+    }
+    return v;
+}
+
+struct NormArgs {
+    void* y;
+    uint8_t* yscale;   // non-null: y is 8-bit rows
+    void* h;           // null: not stored
+    float* rstd;
+    const void* x;
+    const void* residual;   // null: none
+    const void* gain;
+    int gain_dtype;
+    float eps;
+    int64_t rows;
+    int c;
+    bool vec;
+};
+
+template <typename T, int L, int kChunks>
+__global__ void __launch_bounds__(L > 256 ? L : 256) k_rms_norm(const NormArgs a) {
+    constexpr int kThreads = L > 256 ? L : 256;
+    constexpr int kRows = kThreads / L;
+    __shared__ float red[L > 32 ? L / 32 : 1];
+    const int lane = threadIdx.x % L;
+    const int cp = (int)width8(a.c);
+    float gain[kChunks][8];
+#pragma unroll
+    for (int k = 0; k < kChunks; ++k)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int col = (k * L + lane) * 8 + i;
+            gain[k][i] = col < a.c ? load_param(a.gain, a.gain_dtype, col) : 0.f;
+        }
+    const float inv_c = 1.f / (float)a.c;
+    for (int64_t row0 = (int64_t)blockIdx.x * kRows; row0 < a.rows; row0 += (int64_t)gridDim.x * kRows) {
+        const int64_t row = row0 + threadIdx.x / L;
+        const bool live = row < a.rows;
+        float v[kChunks][8];
+        float ss = 0.f;
+#pragma unroll
+        for (int k = 0; k < kChunks; ++k) {
+            const int col = (k * L + lane) * 8;
+            const int left = live ? a.c - col : 0;
+            const int64_t at = left > 0 ? row * a.c + col : 0;
+            load8(v[k], static_cast<const T*>(a.x) + at, a.vec && left >= 8, left);
+            if (a.residual) {
+                float r[8];
+                load8(r, static_cast<const T*>(a.residual) + at, a.vec && left >= 8, left);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[k][i] += r[i];
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kChunks; ++k)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ss = fmaf(v[k][i], v[k][i], ss);
+        const float rstd = rsqrtf(row_sum<L>(ss, red) * inv_c + a.eps);
+        if (live && lane == 0) a.rstd[row] = rstd;
+#pragma unroll
+        for (int k = 0; k < kChunks; ++k) {
+            const int col = (k * L + lane) * 8;
+            const int left = live ? a.c - col : 0;
+            const bool vec = a.vec && left >= 8;
+            const int64_t at = left > 0 ? row * a.c + col : 0;
+            if (a.h) store8(static_cast<T*>(a.h) + at, v[k], vec, left);
+            float y[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = left > i ? v[k][i] * rstd * gain[k][i] : 0.f;
+            if (a.yscale) {
+                float amax = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) amax = fmaxf(amax, finite_abs(y[i]));
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+                const int s = block_exponent(amax);
+                if (live && col < cp) {
+                    const int64_t p = row * (cp / 8) + col / 8;
+                    reinterpret_cast<uint2*>(a.y)[p] = codes8(y, pow2(-s));
+                    if ((lane & 3) == 0) a.yscale[p >> 2] = (uint8_t)(s + 127);
+                }
+            } else {
+                store8(static_cast<T*>(a.y) + at, y, vec, left);
+            }
+        }
+    }
+}
+
+struct NormGradArgs {
+    void* grad_x;
+    float* partial;   // [gridDim.x][c]: each CTA's sum of grad_y * n
+    const void* grad_y;
+    const void* h;
+    const float* rstd;
+    const void* gain;
+    int gain_dtype;
+    const void* grad_h;   // null: none
+    int64_t rows;
+    int c;
+    bool vec;
+};
+
+// With n = h rstd and gn = grad_y gain:  grad_x = rstd (gn - n mean(gn n)) + grad_h.
+// A thread keeps its channels from row to row, so the gain's gradient is
+// summed in registers, then over the CTA's rows in shared memory, and one row
+// of sums per CTA goes to `partial`; k_column_sums adds those in a fixed order
+// (no atomics: the same input gives the same bits).
+template <typename T, int L, int kChunks>
+__global__ void __launch_bounds__(L > 256 ? L : 256) k_rms_norm_grad(const NormGradArgs a) {
+    constexpr int kThreads = L > 256 ? L : 256;
+    constexpr int kRows = kThreads / L;
+    __shared__ float red[L > 32 ? L / 32 : 1];
+    __shared__ float sums[kRows > 1 ? kThreads * 8 : 1];
+    const int lane = threadIdx.x % L;
+    float gain[kChunks][8], acc[kChunks][8];
+#pragma unroll
+    for (int k = 0; k < kChunks; ++k)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int col = (k * L + lane) * 8 + i;
+            gain[k][i] = col < a.c ? load_param(a.gain, a.gain_dtype, col) : 0.f;
+            acc[k][i] = 0.f;
+        }
+    const float inv_c = 1.f / (float)a.c;
+    for (int64_t row0 = (int64_t)blockIdx.x * kRows; row0 < a.rows; row0 += (int64_t)gridDim.x * kRows) {
+        const int64_t row = row0 + threadIdx.x / L;
+        const bool live = row < a.rows;
+        const float rstd = live ? a.rstd[row] : 0.f;
+        float n[kChunks][8], g[kChunks][8];
+        float dot = 0.f;
+#pragma unroll
+        for (int k = 0; k < kChunks; ++k) {
+            const int col = (k * L + lane) * 8;
+            const int left = live ? a.c - col : 0;
+            const int64_t at = left > 0 ? row * a.c + col : 0;
+            load8(n[k], static_cast<const T*>(a.h) + at, a.vec && left >= 8, left);
+            load8(g[k], static_cast<const T*>(a.grad_y) + at, a.vec && left >= 8, left);
+        }
+#pragma unroll
+        for (int k = 0; k < kChunks; ++k)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                n[k][i] *= rstd;
+                acc[k][i] = fmaf(g[k][i], n[k][i], acc[k][i]);
+                g[k][i] *= gain[k][i];
+                dot = fmaf(g[k][i], n[k][i], dot);
+            }
+        const float m = row_sum<L>(dot, red) * inv_c;
+#pragma unroll
+        for (int k = 0; k < kChunks; ++k) {
+            const int col = (k * L + lane) * 8;
+            const int left = live ? a.c - col : 0;
+            const bool vec = a.vec && left >= 8;
+            const int64_t at = left > 0 ? row * a.c + col : 0;
+            float o[8];
+            if (a.grad_h) load8(o, static_cast<const T*>(a.grad_h) + at, vec, left);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float d = rstd * (g[k][i] - n[k][i] * m);
+                o[i] = a.grad_h ? o[i] + d : d;
+            }
+            store8(static_cast<T*>(a.grad_x) + at, o, vec, left);
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < kChunks; ++k) {
+        if (kRows > 1) {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sums[i * kThreads + threadIdx.x] = acc[k][i];
+            __syncthreads();
+        }
+        for (int t = threadIdx.x; t < L * 8; t += kThreads) {
+            const int i = t / L, l = t % L, col = (k * L + l) * 8 + i;
+            float s = 0.f;
+            if (kRows > 1) {
+                for (int r = 0; r < kRows; ++r) s += sums[i * kThreads + r * L + l];
+                if (col < a.c) a.partial[(int64_t)blockIdx.x * a.c + col] = s;
+            }
+        }
+        if (kRows == 1) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int col = (k * L + lane) * 8 + i;
+                if (col < a.c) a.partial[(int64_t)blockIdx.x * a.c + col] = acc[k][i];
+            }
+        }
+    }
+}
+
+// out[col] = sum over the parts of partial[part][col]: a CTA takes 32 columns,
+// its 32 warps every 32nd part each.
+__global__ void __launch_bounds__(1024) k_column_sums(void* out, int dtype, const float* __restrict__ partial,
+                                                      int parts, int64_t c) {
+    __shared__ float s[32][33];
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int64_t col = (int64_t)blockIdx.x * 32 + lane;
+    float v = 0.f;
+    if (col < c)
+        for (int p = w; p < parts; p += 32) v += partial[(int64_t)p * c + col];
+    s[w][lane] = v;
+    __syncthreads();
+    v = s[lane][w];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    const int64_t mine = (int64_t)blockIdx.x * 32 + w;
+    if (lane == 0 && mine < c) store_param(out, dtype, mine, v);
+}
+
+cudaError_t column_sums(void* out, int dtype, const float* partial, int parts, int64_t c, cudaStream_t s) {
+    k_column_sums<<<(unsigned)((c + 31) / 32), 1024, 0, s>>>(out, dtype, partial, parts, c);
+    return cudaGetLastError();
+}
+
+// ------------------------------------------------------------------ launches
+
+template <typename T>
+cudaError_t launch_pack(uint8_t* q, uint8_t* scale, const void* x, int64_t rows, int c, cudaStream_t s) {
+    const unsigned groups = (unsigned)(width8(c) / 8);
+    const int64_t ctas = (rows * groups + 256 * kUnits - 1) / (256 * kUnits);
+    if (ctas > INT_MAX) return cudaErrorInvalidValue;
+    const bool vec = c % 8 == 0 && aligned16(x);
+    k_pack8<T><<<(unsigned)ctas, 256, 0, s>>>(q, scale, static_cast<const T*>(x), rows, c, groups, vec);
+    return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t launch_unpack(void* y, int64_t pitch, const uint8_t* q, const uint8_t* scale, int64_t rows, int c,
+                          cudaStream_t s) {
+    const unsigned groups = (unsigned)(width8(c) / 8);
+    const int64_t ctas = (rows * groups + 256 * kUnits - 1) / (256 * kUnits);
+    if (ctas > INT_MAX) return cudaErrorInvalidValue;
+    const bool vec = pitch % 8 == 0 && aligned16(y);
+    k_unpack8<T><<<(unsigned)ctas, 256, 0, s>>>(static_cast<T*>(y), pitch, q, scale, rows, c, groups, vec);
+    return cudaGetLastError();
+}
+
+cudaError_t unpack_rows(void* y, int dtype, int64_t pitch, const uint8_t* q, const uint8_t* scale, int64_t rows,
+                        int c, cudaStream_t s) {
+    if (dtype == PLATTICE_F32) return launch_unpack<float>(y, pitch, q, scale, rows, c, s);
+    if (dtype == PLATTICE_BF16) return launch_unpack<__nv_bfloat16>(y, pitch, q, scale, rows, c, s);
+    return launch_unpack<__half>(y, pitch, q, scale, rows, c, s);
+}
+
+// CTAs of a grid-stride launch: what the rows need, at most 4 per SM of the
+// current device (each then walks many rows and its loads of the gain and its
+// partial sums are paid once).
+static int norm_ctas(int64_t rows, int rows_per_cta) {
+    const int64_t need = (rows + rows_per_cta - 1) / rows_per_cta;
+    const int64_t most = 4 * (int64_t)sm_count();
+    return (int)(need < most ? need : most);
+}
+
+// Calls f<L, kChunks>() for the row width: L * 8 * kChunks >= channels.
+#define PLR_NORM_SHAPE(CHANNELS, F)                      \
+    do {                                                 \
+        const int n_ = (int)(((CHANNELS) + 7) / 8);      \
+        if (n_ <= 4) return F(4, 1);                     \
+        if (n_ <= 8) return F(8, 1);                     \
+        if (n_ <= 16) return F(16, 1);                   \
+        if (n_ <= 32) return F(32, 1);                   \
+        if (n_ <= 64) return F(32, 2);                   \
+        if (n_ <= 128) return F(32, 4);                  \
+        if (n_ <= 256) return F(256, 1);                 \
+        if (n_ <= 512) return F(512, 1);                 \
+        if (n_ <= 1024) return F(512, 2);                \
+        return F(512, 4);                                \
+    } while (0)
+
+template <typename T>
+cudaError_t launch_norm(const NormArgs& a, cudaStream_t s) {
+#define PLR_F(L, K)                                                                                      \
+    (k_rms_norm<T, L, K><<<norm_ctas(a.rows, (L > 256 ? L : 256) / L), L > 256 ? L : 256, 0, s>>>(a),     \
+     cudaGetLastError())
+    PLR_NORM_SHAPE(a.c, PLR_F);
+#undef PLR_F
+}
+
+static int norm_rows_per_cta(int c) {
+#define PLR_F(L, K) ((L > 256 ? L : 256) / L)
+    PLR_NORM_SHAPE(c, PLR_F);
+#undef PLR_F
+}
+
+template <typename T>
+cudaError_t launch_norm_grad(const NormGradArgs& a, int ctas, cudaStream_t s) {
+#define PLR_F(L, K) (k_rms_norm_grad<T, L, K><<<ctas, L > 256 ? L : 256, 0, s>>>(a), cudaGetLastError())
+    PLR_NORM_SHAPE(a.c, PLR_F);
+#undef PLR_F
+}
+
+}  // namespace plr
+
+using namespace plr;
+
+extern "C" {
+
+int plattice_rows_pack8(uint8_t* q, uint8_t* scale, const void* x, int dtype, long long rows, int c, void* stream) {
+    if (!dtype_ok(dtype) || rows < 0 || c < 1) return PLATTICE_ERR_INVALID;
+    if (rows == 0) return PLATTICE_OK;
+    if (!q || !scale || !x || !fits(rows, width8(c))) return PLATTICE_ERR_INVALID;
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const cudaError_t e = dtype == PLATTICE_F32    ? launch_pack<float>(q, scale, x, rows, c, s)
+                          : dtype == PLATTICE_BF16 ? launch_pack<__nv_bfloat16>(q, scale, x, rows, c, s)
+                                                   : launch_pack<__half>(q, scale, x, rows, c, s);
+    return rows_status(e, "plattice_rows_pack8");
+}
+
+int plattice_rows_unpack8(void* y, int dtype, const uint8_t* q, const uint8_t* scale, long long rows, int c,
+                          void* stream) {
+    if (!dtype_ok(dtype) || rows < 0 || c < 1) return PLATTICE_ERR_INVALID;
+    if (rows == 0) return PLATTICE_OK;
+    if (!q || !scale || !y || !fits(rows, width8(c))) return PLATTICE_ERR_INVALID;
+    return rows_status(unpack_rows(y, dtype, c, q, scale, rows, c, static_cast<cudaStream_t>(stream)),
+                       "plattice_rows_unpack8");
+}
+
+int plattice_rms_norm(void* y, uint8_t* yscale, void* h, float* rstd, const void* x, const void* residual,
+                      const void* gain, int dtype, int gain_dtype, float eps, long long rows, int c, void* stream) {
+    if (!dtype_ok(dtype) || !dtype_ok(gain_dtype) || rows < 0 || c < 1 || c > PLATTICE_NORM_MAX_CHANNELS)
+        return PLATTICE_ERR_INVALID;
+    if (rows == 0) return PLATTICE_OK;
+    if (!y || !rstd || !x || !gain || !fits(rows, width8(c))) return PLATTICE_ERR_INVALID;
+    NormArgs a{y, yscale, h, rstd, x, residual, gain, gain_dtype, eps, rows, c, false};
+    a.vec = c % 8 == 0 && aligned16(x) && (!residual || aligned16(residual)) && (!h || aligned16(h)) &&
+            (yscale || aligned16(y));
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const cudaError_t e = dtype == PLATTICE_F32    ? launch_norm<float>(a, s)
+                          : dtype == PLATTICE_BF16 ? launch_norm<__nv_bfloat16>(a, s)
+                                                   : launch_norm<__half>(a, s);
+    return rows_status(e, "plattice_rms_norm");
+}
+
+int plattice_rms_norm_backward_workspace_size(long long rows, int c, size_t* bytes) {
+    if (!bytes || rows < 0 || c < 1 || c > PLATTICE_NORM_MAX_CHANNELS) return PLATTICE_ERR_INVALID;
+    // one row of partial sums per CTA, whatever the device's SM count (<= 256)
+    const int64_t per = norm_rows_per_cta(c);
+    const int64_t need = (rows + per - 1) / per;
+    *bytes = (size_t)(need < 1024 ? (need < 1 ? 1 : need) : 1024) * c * sizeof(float);
+    return PLATTICE_OK;
+}
+
+int plattice_rms_norm_backward(void* grad_x, void* grad_gain, const void* grad_y, const void* h, const float* rstd,
+                               const void* gain, const void* grad_h, void* workspace, size_t workspace_bytes,
+                               int dtype, int gain_dtype, long long rows, int c, void* stream) {
+    if (!dtype_ok(dtype) || !dtype_ok(gain_dtype) || rows < 0 || c < 1 || c > PLATTICE_NORM_MAX_CHANNELS)
+        return PLATTICE_ERR_INVALID;
+    if (!grad_gain || !fits(rows, width8(c))) return PLATTICE_ERR_INVALID;
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (rows == 0)   // the sum over no rows
+        return rows_status(cudaMemsetAsync(grad_gain, 0, (size_t)c * dtype_size(gain_dtype), s),
+                           "plattice_rms_norm_backward");
+    if (!grad_x || !grad_y || !h || !rstd || !gain || !workspace) return PLATTICE_ERR_INVALID;
+    size_t need = 0;
+    plattice_rms_norm_backward_workspace_size(rows, c, &need);
+    if (workspace_bytes < need) return PLATTICE_ERR_WORKSPACE;
+    int ctas = norm_ctas(rows, norm_rows_per_cta(c));
+    if (ctas > 1024) ctas = 1024;
+    NormGradArgs a{grad_x, static_cast<float*>(workspace), grad_y, h, rstd, gain, gain_dtype, grad_h, rows, c, false};
+    a.vec = c % 8 == 0 && aligned16(grad_x) && aligned16(grad_y) && aligned16(h) && (!grad_h || aligned16(grad_h));
+    cudaError_t e = dtype == PLATTICE_F32    ? launch_norm_grad<float>(a, ctas, s)
+                    : dtype == PLATTICE_BF16 ? launch_norm_grad<__nv_bfloat16>(a, ctas, s)
+                                             : launch_norm_grad<__half>(a, ctas, s);
+    if (e == cudaSuccess) e = column_sums(grad_gain, gain_dtype, a.partial, ctas, c, s);
+    return rows_status(e, "plattice_rms_norm_backward");
+}
+
+}  // extern "C"
