@@ -140,6 +140,7 @@ cudaError_t symbol_address(const void* symbol, void** addr) {
 namespace {
 
 constexpr unsigned kRing = 4096;
+constexpr int kWaitGaveUp = 4;   // PLATTICE_DEV_WAIT_LIMIT
 
 struct Ring {
     std::mutex mu;
@@ -153,6 +154,9 @@ struct Ring {
     int fail_status = 0;
     const char* fail_name = nullptr;
     unsigned fail_seq = 0;
+    unsigned* fault_host = nullptr;
+    unsigned* fault_dev = nullptr;
+    bool fault_unavailable = false;
 };
 
 Ring& ring() {
@@ -221,6 +225,12 @@ int status_poll(const char** name, unsigned* seq) {
             }
         }
     }
+    if (r.fault_host && *reinterpret_cast<volatile unsigned*>(r.fault_host) != 0 && r.fail_status == 0) {
+        *reinterpret_cast<volatile unsigned*>(r.fault_host) = 0;
+        r.fail_status = kWaitGaveUp;
+        r.fail_name = "a row operator";
+        r.fail_seq = 0;
+    }
     const int st = r.fail_status;
     if (st) {
         if (name) *name = r.fail_name;
@@ -228,6 +238,25 @@ int status_poll(const char** name, unsigned* seq) {
         r.fail_status = 0;
     }
     return st;
+}
+
+unsigned* fault_word() {
+    Ring& r = ring();
+    std::lock_guard<std::mutex> lk(r.mu);
+    if (!r.fault_host && !r.fault_unavailable) {
+        void *p = nullptr, *d = nullptr;
+        if (cudaHostAlloc(&p, sizeof(unsigned), cudaHostAllocPortable | cudaHostAllocMapped) != cudaSuccess ||
+            cudaHostGetDevicePointer(&d, p, 0) != cudaSuccess || !d) {
+            cudaGetLastError();
+            if (p) cudaFreeHost(p);
+            r.fault_unavailable = true;
+        } else {
+            *static_cast<volatile unsigned*>(p) = 0;
+            r.fault_host = static_cast<unsigned*>(p);
+            r.fault_dev = static_cast<unsigned*>(d);
+        }
+    }
+    return r.fault_dev;
 }
 
 }  // namespace pl

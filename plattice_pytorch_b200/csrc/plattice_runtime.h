@@ -45,4 +45,9 @@ StatusTicket status_ticket(const char* call);
 // call's name and sequence number in name/seq.
 int status_poll(const char** name, unsigned* seq);
 
+// Device address of a pinned, mapped word that a kernel of a call without a
+// ticket sets to non-zero when a bounded wait of its own gives up (nullptr:
+// not available); status_poll reports and clears it.
+unsigned* fault_word();
+
 }  // namespace pl

@@ -173,21 +173,49 @@ template <> __device__ __forceinline__ float within<__half>(float v) {
 
 // -------------------------------------------------------------- activations
 
+// Phi(-|z|) and exp(-z^2 / 2), by the rational approximation of the error
+// function 7.1.26 of Abramowitz and Stegun, Handbook of Mathematical
+// Functions (off by at most 1.5e-7 of erf, about a float32 step of 1): a
+// reciprocal, an exponential and six multiply-adds.  The product's epilogue
+// computes it for every output on the way out, where a full-precision erf
+// would take longer than the matrix instructions it runs beside.
+__device__ __forceinline__ float tail(float z, float& e) {
+    const float x = fabsf(z) * 0.70710678118654752f;
+    const float t = __fdividef(1.f, fmaf(0.3275911f, x, 1.f));
+    e = __expf(-x * x);
+    float q = fmaf(1.061405429f, t, -1.453152027f);
+    q = fmaf(q, t, 1.421413741f);
+    q = fmaf(q, t, -0.284496736f);
+    q = fmaf(q, t, 0.254829592f);
+    return 0.5f * q * t * e;
+}
+
+__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
+
+// NaN stays NaN; the products with an infinite z are kept out of 0 x infinity.
 __device__ __forceinline__ float act_value(float z, int act) {
-    if (act == PLATTICE_ACT_RELU) return z > 0.f ? z : (z != z ? z : 0.f);
-    if (act == PLATTICE_ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
-    if (act == PLATTICE_ACT_SILU) return z / (1.f + __expf(-z));
+    if (act == PLATTICE_ACT_RELU) return z > 0.f ? z : (z == z ? 0.f : z);
+    if (act == PLATTICE_ACT_GELU) {   // z Phi(z) = max(z, 0) - |z| Phi(-|z|); beyond |z| = 16 the tail is 0
+        float e;
+        const float q = tail(z, e);
+        return fmaf(-fminf(fabsf(z), 16.f), q, z > 0.f ? z : z * 0.f);
+    }
+    if (act == PLATTICE_ACT_SILU) return z * sigmoid(z);
     return z;
 }
 
 // d act / d z
 __device__ __forceinline__ float act_slope(float z, int act) {
-    if (act == PLATTICE_ACT_RELU) return z > 0.f ? 1.f : (z != z ? z : 0.f);
-    if (act == PLATTICE_ACT_GELU)
-        return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * __expf(-0.5f * z * z) * 0.39894228040143268f;
+    if (act == PLATTICE_ACT_RELU) return z > 0.f ? 1.f : (z == z ? 0.f : z);
+    if (act == PLATTICE_ACT_GELU) {   // Phi(z) + z phi(z)
+        float e;
+        const float q = tail(z, e);
+        const float zc = z > 16.f ? 16.f : (z < -16.f ? -16.f : z);   // a NaN stays
+        return fmaf(zc * 0.39894228040143268f, e, z >= 0.f ? 1.f - q : q);
+    }
     if (act == PLATTICE_ACT_SILU) {
-        const float s = 1.f / (1.f + __expf(-z));
-        return s * (1.f + z * (1.f - s));
+        const float s = sigmoid(z);
+        return s * fmaf(z, 1.f - s, 1.f);
     }
     return 1.f;
 }

@@ -1,9 +1,12 @@
 // rows_linear.cu -- linear map of rows with bias, activation and residual,
 // and its backward pass, x plain or in 8-bit rows.  C ABI: include/plattice.h.
 #include <limits.h>
+#include <string.h>
 
+#include "plattice_runtime.h"
 #include "rows_common.cuh"
 #include "rows_host.h"
+#include "rows_mma.cuh"
 
 namespace plr {
 
@@ -134,6 +137,59 @@ __global__ void __launch_bounds__(256) k_finish(const FinishArgs a, unsigned gro
     }
 }
 
+// ----------------------------------------------------- operands for the MMAs
+
+// A float32 value as three bfloat16 whose sum it is: each takes the leading 8
+// significant bits of what is left (cut, not rounded, so that none overflows
+// and the remainders are exact).  What is not finite stays in the first part.
+__device__ __forceinline__ void split3(float v, __nv_bfloat16 (&o)[3]) {
+    const bool fine = fabsf(v) <= 3.402823466e38f;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        // cutting a NaN's low bits could leave an infinity: round those
+        const __nv_bfloat16 h = fine ? __ushort_as_bfloat16((unsigned short)(__float_as_uint(v) >> 16))
+                                     : __float2bfloat16_rn(i == 0 ? v : 0.f);
+        o[i] = h;
+        v = fine ? v - __bfloat162float(h) : v;
+    }
+}
+
+__device__ __forceinline__ void store_parts(__nv_bfloat16* p, int64_t stride, const float (&v)[8], bool vec, int n) {
+    union { uint4 u; __nv_bfloat16 h[8]; } o[3];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        __nv_bfloat16 t[3];
+        split3(v[i], t);
+        o[0].h[i] = t[0];
+        o[1].h[i] = t[1];
+        o[2].h[i] = t[2];
+    }
+#pragma unroll
+    for (int j = 0; j < 3; ++j) {
+        if (vec) *reinterpret_cast<uint4*>(p + j * stride) = o[j].u;
+        else
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i < n) p[j * stride + i] = o[j].h[i];
+    }
+}
+
+// Rows of c elements copied to rows of `pitch` (a multiple of 8): what TMA
+// needs when the rows do not lie on 16-byte boundaries; float32 becomes its
+// three parts.  Costs one read and one (float32: 1.5) write of the operand.
+template <typename T>
+__global__ void __launch_bounds__(256) k_repack(void* __restrict__ out, const T* __restrict__ x, int64_t rows, int c,
+                                                unsigned groups, bool vec) {
+    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t row = t / groups;
+    if (row >= rows) return;
+    const int col = (int)(t - row * groups) * 8, left = c - col;
+    float v[8];
+    load8(v, x + row * c + col, vec && left >= 8, left);
+    if (sizeof(T) == 4) store_parts(static_cast<__nv_bfloat16*>(out) + t * 8, rows * groups * 8, v, true, 8);
+    else store8(static_cast<T*>(out) + t * 8, v, true, 8);
+}
+
 // ------------------------------------------------- backward: gz and its sums
 
 struct GradArgs {
@@ -143,6 +199,7 @@ struct GradArgs {
     const uint8_t* z_scale;
     void* gz;           // [rows][pitch] in the operands' type; null: not stored
     int64_t pitch;
+    bool parts;         // float32: gz as three bfloat16 parts [3][rows][pitch]
     float* partial;     // [gridDim.y][n]; null: no bias gradient
     int64_t rows;
     int n, split, act;
@@ -188,7 +245,10 @@ __global__ void __launch_bounds__(256) k_grad_z(const GradArgs a) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) acc[i] += g[i];
         const int64_t wide = a.pitch - col;   // zeros up to the pitch
-        if (a.gz && wide > 0) store8(static_cast<T*>(a.gz) + row * a.pitch + col, g, false, (int)min(wide, (int64_t)8));
+        if (!a.gz || wide <= 0) continue;
+        const int64_t at = row * a.pitch + col;
+        if (sizeof(T) == 4 && a.parts) store_parts(static_cast<__nv_bfloat16*>(a.gz) + at, a.rows * a.pitch, g, wide >= 8, (int)min(wide, (int64_t)8));
+        else store8(static_cast<T*>(a.gz) + at, g, a.pitch % 8 == 0 && wide >= 8, (int)min(wide, (int64_t)8));
     }
     if (!a.partial) return;
 #pragma unroll
@@ -215,25 +275,34 @@ __global__ void __launch_bounds__(256) k_add_parts(T* __restrict__ out, const fl
 // ------------------------------------------------------------------ host side
 
 static int64_t up256(int64_t n) { return (n + 255) & ~255ll; }
+static int64_t up8(int64_t n) { return (n + 7) & ~7ll; }
+static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Parts of a sum over `len` terms whose result has `tiles` tiles: enough CTAs
-// for the device, none shorter than 512 terms.
-static int parts_of(int64_t tiles, int64_t len) {
-    const int64_t want = (2 * (int64_t)sm_count() + tiles - 1) / tiles;
-    const int64_t most = (len + 511) / 512;
-    int64_t p = want < most ? want : most;
-    if (p < 1) p = 1;
-    if (p > 512) p = 512;
-    return (int)p;
+// Buffers of a call, one after the other in its workspace.
+struct Carve {
+    int64_t at = 0;
+    int64_t take(int64_t bytes) {
+        const int64_t p = at;
+        at += up256(bytes);
+        return p;
+    }
+};
+
+static bool linear_shape_ok(const plattice_linear_args* a) {
+    if (!a || a->rows < 0 || a->k < 1 || a->n < 1 || a->split < 0 || a->split >= a->n) return false;
+    if (!dtype_ok(a->dtype) || !dtype_ok(a->out_dtype) || !dtype_ok(a->bias_dtype)) return false;
+    if (a->out_dtype != a->dtype && a->out_dtype != PLATTICE_F32) return false;
+    if (a->x_scale && a->dtype == PLATTICE_F16) return false;
+    if (a->act < PLATTICE_ACT_NONE || a->act > PLATTICE_ACT_SILU) return false;
+    if (a->split && a->act != PLATTICE_ACT_NONE) return false;
+    // TMA coordinates and tile numbers are 32-bit
+    if (a->rows > INT_MAX - 256 || a->k > (1 << 30) || a->n > (1 << 30)) return false;
+    return fits(a->rows, width8(a->k)) && fits(a->rows, width8(a->n)) && fits(a->k, a->n);
 }
 
-static int64_t tiles_of(int64_t n) { return (n + kTile - 1) / kTile; }
+// ---- products on the CUDA cores (float32 of few operations)
 
-static int grad_rows_parts(int64_t rows, int n) {
-    const int64_t strips = (n + 255) / 256, need = (rows + 7) / 8;
-    const int64_t most = (4 * (int64_t)sm_count() + strips - 1) / strips;
-    return (int)(need < most ? need : most);
-}
+static int64_t simt_tiles(int64_t n) { return ceil_div(n, kTile); }
 
 static View view_rows(const void* p, const uint8_t* scale, int64_t pitch, int dtype, bool along_rows) {
     if (scale) pitch = width8(pitch);
@@ -242,15 +311,24 @@ static View view_rows(const void* p, const uint8_t* scale, int64_t pitch, int dt
 
 static cudaError_t product(float* out, const View& a, const View& b, int64_t ni, int64_t nj, int64_t nr, int parts,
                            cudaStream_t s) {
-    if (tiles_of(ni) > INT_MAX || tiles_of(nj) > 65535) return cudaErrorInvalidValue;
-    const int64_t part = (nr + parts - 1) / parts;
-    k_product<<<dim3((unsigned)tiles_of(ni), (unsigned)tiles_of(nj), parts), 256, 0, s>>>(out, a, b, ni, nj, nr, part);
+    if (simt_tiles(ni) > INT_MAX || simt_tiles(nj) > 65535) return cudaErrorInvalidValue;
+    const int64_t part = ceil_div(nr, parts);
+    k_product<<<dim3((unsigned)simt_tiles(ni), (unsigned)simt_tiles(nj), parts), 256, 0, s>>>(out, a, b, ni, nj, nr,
+                                                                                           part);
     return cudaGetLastError();
+}
+
+// Parts of a sum over `len` terms whose result has `tiles` tiles: enough CTAs
+// for the device, none shorter than 512 terms.
+static int simt_parts(int64_t tiles, int64_t len) {
+    int64_t p = ceil_div(2 * (int64_t)sm_count(), tiles);
+    if (p > ceil_div(len, 512)) p = ceil_div(len, 512);
+    return (int)(p < 1 ? 1 : p > 512 ? 512 : p);
 }
 
 template <typename T>
 static cudaError_t add_parts(void* out, const float* partial, int parts, int64_t n, cudaStream_t s) {
-    k_add_parts<T><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(static_cast<T*>(out), partial, parts, n);
+    k_add_parts<T><<<(unsigned)ceil_div(n, 256), 256, 0, s>>>(static_cast<T*>(out), partial, parts, n);
     return cudaGetLastError();
 }
 
@@ -260,40 +338,359 @@ static cudaError_t add_parts_to(void* out, int dtype, const float* partial, int 
     return add_parts<__half>(out, partial, parts, n, s);
 }
 
-static bool linear_shape_ok(const plattice_linear_args* a) {
-    if (!a || a->rows < 0 || a->k < 1 || a->n < 1 || a->split < 0 || a->split >= a->n) return false;
-    if (!dtype_ok(a->dtype) || !dtype_ok(a->out_dtype) || !dtype_ok(a->bias_dtype)) return false;
-    if (a->out_dtype != a->dtype && a->out_dtype != PLATTICE_F32) return false;
-    if (a->x_scale && a->dtype == PLATTICE_F16) return false;
-    if (a->act < PLATTICE_ACT_NONE || a->act > PLATTICE_ACT_SILU) return false;
-    if (a->split && a->act != PLATTICE_ACT_NONE) return false;
-    return fits(a->rows, width8(a->k)) && fits(a->rows, width8(a->n)) && fits(a->k, a->n);
+// ---- products on the tensor cores
+
+// A 16-bit operand [parts][rows][pitch] of `width` columns.
+struct Operand {
+    const void* p = nullptr;
+    int64_t rows = 0, width = 0, pitch = 0;
+    int parts = 1;
+};
+
+// Whether TMA can read the rows where they are.
+static bool tma_ready(const void* p, int dtype, int64_t width) {
+    return dtype != PLATTICE_F32 && width % 8 == 0 && aligned16(p);
+}
+
+static int64_t repack_bytes(int dtype, int64_t rows, int64_t width) {
+    return rows * up8(width) * 2 * (dtype == PLATTICE_F32 ? 3 : 1);
+}
+
+// The operand where it is, or repacked into `ws`.
+static cudaError_t operand(Operand* o, const void* p, int dtype, int64_t rows, int64_t width, void* ws,
+                           cudaStream_t s) {
+    *o = Operand{p, rows, width, width, 1};
+    if (tma_ready(p, dtype, width)) return cudaSuccess;
+    o->p = ws;
+    o->pitch = up8(width);
+    o->parts = dtype == PLATTICE_F32 ? 3 : 1;
+    const unsigned groups = (unsigned)(o->pitch / 8);
+    const int64_t ctas = ceil_div(rows * groups, 256);
+    if (ctas > INT_MAX) return cudaErrorInvalidValue;
+    const bool vec = width % 8 == 0 && aligned16(p);
+    if (dtype == PLATTICE_F32)
+        k_repack<float><<<(unsigned)ctas, 256, 0, s>>>(ws, static_cast<const float*>(p), rows, (int)width, groups, vec);
+    else if (dtype == PLATTICE_BF16)
+        k_repack<__nv_bfloat16><<<(unsigned)ctas, 256, 0, s>>>(ws, static_cast<const __nv_bfloat16*>(p), rows, (int)width,
+                                                              groups, vec);
+    else
+        k_repack<__half><<<(unsigned)ctas, 256, 0, s>>>(ws, static_cast<const __half*>(p), rows, (int)width, groups, vec);
+    return cudaGetLastError();
+}
+
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static EncodeTiled encode_tiled() {
+    static EncodeTiled f = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess) {
+            cudaGetLastError();
+            return (EncodeTiled) nullptr;
+        }
+        return (EncodeTiled)p;
+    }();
+    return f;
+}
+
+// Boxes of 64 columns x `box_rows` rows, zeros outside the operand.
+static cudaError_t make_map(CUtensorMap* m, const Operand& o, int box_rows) {
+    const EncodeTiled enc = encode_tiled();
+    if (!enc) return cudaErrorNotSupported;
+    const cuuint64_t dims[3] = {(cuuint64_t)o.width, (cuuint64_t)o.rows, (cuuint64_t)o.parts};
+    const cuuint64_t strides[2] = {(cuuint64_t)o.pitch * 2, (cuuint64_t)(o.pitch * o.rows) * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1}, unit[3] = {1, 1, 1};
+    const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(o.p), dims, strides, box, unit,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+// Cycles of a 64-deep slice of a 128 x bn tile: the MMA itself (512 at 256
+// columns), or below that what staging the operands' slices takes.
+static double slice_cost(int bn) { return bn == 256 ? 512 : bn == 128 ? 300 : bn == 64 ? 220 : 200; }
+
+static int64_t mma_tiles(int64_t ni, int64_t nj, int bn) { return ceil_div(ni, kBM) * ceil_div(nj, bn); }
+
+// Columns of a tile: the cheapest number of rounds over the device's SMs
+// (wide tiles do more per byte staged, narrow ones fill the device when D is
+// small and waste less when it is narrow).
+static int choose_bn(int64_t ni, int64_t nj, int least) {
+    int best = least;
+    double cost = 1e300;
+    for (int bn = 256; bn >= least; bn /= 2) {
+        const double c = (double)ceil_div(mma_tiles(ni, nj, bn), sm_count()) * slice_cost(bn);
+        if (c < cost) cost = c, best = bn;
+    }
+    return best;
+}
+
+// Parts of kGradW's sum: the cheapest of rounds over the SMs, where a part
+// costs its slices and some 6 more for filling and emptying the accumulator,
+// plus writing and adding the partial results (8 bytes an element, about
+// 3 bytes a cycle and SM).
+static int choose_parts(int64_t ni, int64_t nj, int bn, int64_t steps) {
+    const int64_t tiles = mma_tiles(ni, nj, bn);
+    int best = 1;
+    double cost = 1e300;
+    for (int p = 1; p <= 256 && p <= steps; ++p) {
+        const double rounds = (double)ceil_div(tiles * p, sm_count());
+        double c = rounds * (double)(ceil_div(steps, p) + 6) * slice_cost(bn);
+        if (p > 1) c += (double)p * ni * nj * 8 / (3.0 * 8 * sm_count());
+        if (c < cost) cost = c, best = p;
+    }
+    return best;
+}
+
+template <int kKind, bool kX8, int kBN>
+static cudaError_t launch_mma(const Operand& a, const Operand& b, const MmaArgs& p, cudaStream_t s) {
+    int unused = 0;
+    cudaError_t e = pl::kernel_once(
+        reinterpret_cast<const void*>(k_mma<kKind, kX8, kBN>),
+        [](int*) {
+            return cudaFuncSetAttribute(k_mma<kKind, kX8, kBN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        smem_bytes(kKind, kBN));
+        },
+        &unused);
+    if (e != cudaSuccess) return e;
+    CUtensorMap ma, mb;
+    if (kX8) memset(&ma, 0, sizeof(ma));
+    else if ((e = make_map(&ma, a, a_mn(kKind) ? kBK : kBM)) != cudaSuccess) return e;
+    if ((e = make_map(&mb, b, b_mn(kKind) ? kBK : kBN)) != cudaSuccess) return e;
+    const int64_t tiles = mma_tiles(p.ni, p.nj, kBN) * p.parts;
+    if (tiles > INT_MAX) return cudaErrorInvalidValue;
+    const int ctas = (int)(tiles < sm_count() ? tiles : sm_count());
+    k_mma<kKind, kX8, kBN><<<ctas, kRoleThreads + (kX8 ? 32 * kConvertWarps : 0), smem_bytes(kKind, kBN), s>>>(
+        ma, mb, p, (unsigned)tiles);
+    return cudaGetLastError();
+}
+
+template <int kKind, bool kX8>
+static cudaError_t run_mma(int bn, const Operand& a, const Operand& b, const MmaArgs& p, cudaStream_t s) {
+    if (bn == 256) return launch_mma<kKind, kX8, 256>(a, b, p, s);
+    if (bn == 128) return launch_mma<kKind, kX8, 128>(a, b, p, s);
+    if (bn == 64) return launch_mma<kKind, kX8, 64>(a, b, p, s);
+    if constexpr (kKind != kGradX) return launch_mma<kKind, kX8, 32>(a, b, p, s);
+    return cudaErrorInvalidValue;
+}
+
+// The sum's side of the arguments: slices of r and the products of parts.
+static void sum_args(MmaArgs* p, int64_t nr, int parts, int parts_a, int parts_b) {
+    p->steps = (int)ceil_div(nr, kBK);
+    p->part_steps = (int)ceil_div(p->steps, parts);
+    p->parts = (int)ceil_div(p->steps, p->part_steps);   // none is empty
+    static const unsigned char pairs33[6][2] = {{0, 2}, {1, 1}, {2, 0}, {0, 1}, {1, 0}, {0, 0}};
+    p->pairs = 0;
+    p->pairs_a = p->pairs_b = 0;
+    for (const auto& c : pairs33) {
+        if (c[0] >= parts_a || c[1] >= parts_b) continue;
+        p->pairs_a |= (unsigned)c[0] << (2 * p->pairs);
+        p->pairs_b |= (unsigned)c[1] << (2 * p->pairs);
+        ++p->pairs;
+    }
+}
+
+static void x8_args(MmaArgs* p, const plattice_linear_args* a) {
+    if (!a->x_scale) return;
+    p->q = static_cast<const uint8_t*>(a->x);
+    p->q_scale = a->x_scale;
+    p->q_rows = a->rows;
+    p->q_width = width8(a->k);
+}
+
+// Which products run on the tensor cores: all of 16-bit operands; float32 (six
+// products of bfloat16 parts, three with an 8-bit x) from an amount of work on.
+static bool on_tensor_cores(const plattice_linear_args* a) {
+    return a->dtype != PLATTICE_F32 || (double)a->rows * a->k * a->n >= 64.0 * 1024 * 1024;
+}
+
+struct ForwardPlan {
+    bool mma;
+    int bn;
+    int64_t x, w, acc, bytes;
+};
+
+static ForwardPlan forward_plan(const plattice_linear_args* a) {
+    ForwardPlan p{};
+    Carve c;
+    p.mma = on_tensor_cores(a);
+    if (p.mma) {
+        p.bn = choose_bn(a->rows, a->n, 32);
+        p.x = a->x_scale || tma_ready(a->x, a->dtype, a->k) ? 0 : c.take(repack_bytes(a->dtype, a->rows, a->k));
+        p.w = tma_ready(a->w, a->dtype, a->k) ? 0 : c.take(repack_bytes(a->dtype, a->n, a->k));
+    } else {
+        p.acc = c.take(a->rows * a->n * 4);
+    }
+    p.bytes = c.at;
+    return p;
 }
 
 struct BackwardPlan {
-    int64_t gz, partial_b, partial_w, acc_x, bytes;
-    int parts_b, parts_w;
-    int64_t pitch;
+    bool mma, gz_needed;
+    int bn_x, bn_w, parts_b, parts_w;
+    int64_t gz, x, w, partial_b, partial_w, acc_x, pitch, bytes;
 };
 
 static BackwardPlan backward_plan(const plattice_linear_args* a) {
     BackwardPlan p{};
-    p.pitch = a->n;
-    p.parts_b = grad_rows_parts(a->rows, a->n);
-    p.parts_w = parts_of(tiles_of(a->n) * tiles_of(a->k), a->rows);
-    int64_t at = 0;
-    p.gz = at; at += up256(a->rows * p.pitch * (int64_t)dtype_size(a->dtype));
-    p.partial_b = at; at += up256((int64_t)p.parts_b * a->n * 4);
-    p.partial_w = at; at += up256((int64_t)p.parts_w * a->n * a->k * 4);
-    p.acc_x = at; at += up256(a->rows * a->k * 4);
-    p.bytes = at;
+    Carve c;
+    p.mma = on_tensor_cores(a);
+    const int64_t strips = ceil_div(a->n, 256), need = ceil_div(a->rows, 8);
+    const int64_t most = ceil_div(4 * (int64_t)sm_count(), strips);
+    p.parts_b = (int)(need < most ? need : most);
+    if (p.parts_b < 1) p.parts_b = 1;
+    p.partial_b = c.take((int64_t)p.parts_b * a->n * 4);
+    // the incoming gradient itself serves where it is already what TMA reads
+    p.gz_needed = !(p.mma && a->act == PLATTICE_ACT_NONE && !a->split && a->out_dtype == a->dtype &&
+                    tma_ready(a->grad0, a->dtype, a->n));
+    if (p.mma) {
+        p.pitch = up8(a->n);
+        if (p.gz_needed) p.gz = c.take(repack_bytes(a->dtype, a->rows, a->n));
+        p.bn_x = choose_bn(a->rows, a->k, 64);
+        p.bn_w = a->n > 128 ? 256 : a->n > 64 ? 128 : a->n > 32 ? 64 : 32;
+        p.parts_w = choose_parts(a->k, a->n, p.bn_w, ceil_div(a->rows, kBK));
+        if (a->grad_x && !tma_ready(a->w, a->dtype, a->k)) p.w = c.take(repack_bytes(a->dtype, a->n, a->k));
+        if (a->grad_w && !a->x_scale && !tma_ready(a->x, a->dtype, a->k))
+            p.x = c.take(repack_bytes(a->dtype, a->rows, a->k));
+        if (a->grad_w && p.parts_w > 1) p.partial_w = c.take((int64_t)p.parts_w * a->n * a->k * 4);
+    } else {
+        p.pitch = a->n;
+        p.gz = c.take(a->rows * p.pitch * (int64_t)dtype_size(a->dtype));
+        p.parts_w = simt_parts(simt_tiles(a->n) * simt_tiles(a->k), a->rows);
+        if (a->grad_w) p.partial_w = c.take((int64_t)p.parts_w * a->n * a->k * 4);
+        if (a->grad_x) p.acc_x = c.take(a->rows * a->k * 4);
+    }
+    p.bytes = c.at;
     return p;
 }
 
 template <typename TG, typename T>
 static cudaError_t launch_grad_z(const GradArgs& g, int parts, cudaStream_t s) {
-    k_grad_z<TG, T><<<dim3((g.n + 255) / 256, parts), 256, 0, s>>>(g);
+    k_grad_z<TG, T><<<dim3((unsigned)ceil_div(g.n, 256), parts), 256, 0, s>>>(g);
     return cudaGetLastError();
+}
+
+static cudaError_t forward_simt(const plattice_linear_args* a, const ForwardPlan& p, cudaStream_t s) {
+    float* acc = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + p.acc);
+    const cudaError_t e = product(acc, view_rows(a->x, a->x_scale, a->k, a->dtype, false),
+                                  view_rows(a->w, nullptr, a->k, a->dtype, false), a->rows, a->n, a->k, 1, s);
+    if (e != cudaSuccess) return e;
+    const FinishArgs f{acc, a->bias, a->bias_dtype, a->residual, a->y0, a->y1, a->z, a->z_scale, a->rows,
+                       a->n, a->split, a->act, a->out_dtype};
+    const unsigned groups = (unsigned)(width8(a->n) / 8);
+    const int64_t ctas = ceil_div(a->rows * groups, 256);
+    if (ctas > INT_MAX) return cudaErrorInvalidValue;
+    k_finish<float><<<(unsigned)ctas, 256, 0, s>>>(f, groups);
+    return cudaGetLastError();
+}
+
+static cudaError_t forward_mma(const plattice_linear_args* a, const ForwardPlan& p, cudaStream_t s) {
+    char* ws = static_cast<char*>(a->workspace);
+    Operand x, w;
+    cudaError_t e = cudaSuccess;
+    if (!a->x_scale) e = operand(&x, a->x, a->dtype, a->rows, a->k, ws + p.x, s);
+    if (e == cudaSuccess) e = operand(&w, a->w, a->dtype, a->n, a->k, ws + p.w, s);
+    if (e != cudaSuccess) return e;
+    MmaArgs m{};
+    m.y0 = a->y0;
+    m.y1 = a->y1;
+    m.bias = a->bias;
+    m.residual = a->residual;
+    m.z = a->z;
+    m.z_scale = a->z_scale;
+    m.ni = a->rows;
+    m.nj = a->n;
+    m.bias_dtype = a->bias_dtype;
+    m.out_dtype = a->out_dtype;
+    m.act = a->act;
+    m.split = a->split;
+    m.vec = a->n % 8 == 0 && aligned16(a->y0) && (!a->residual || aligned16(a->residual)) &&
+            (!a->z || a->z_scale || aligned16(a->z));
+    m.half = a->dtype == PLATTICE_F16;
+    m.fault = pl::fault_word();
+    sum_args(&m, a->k, 1, x.parts, w.parts);
+    x8_args(&m, a);
+    return a->x_scale ? run_mma<kForward, true>(p.bn, x, w, m, s) : run_mma<kForward, false>(p.bn, x, w, m, s);
+}
+
+static cudaError_t grad_z(const plattice_linear_args* a, const BackwardPlan& p, cudaStream_t s) {
+    char* ws = static_cast<char*>(a->workspace);
+    const bool store = p.gz_needed && (a->grad_x || a->grad_w);
+    if (!store && !a->grad_bias) return cudaSuccess;
+    const GradArgs g{a->grad0, a->grad1, a->z, a->z_scale, store ? ws + p.gz : nullptr, p.pitch, p.mma,
+                     a->grad_bias ? reinterpret_cast<float*>(ws + p.partial_b) : nullptr, a->rows, a->n, a->split,
+                     a->act};
+    cudaError_t e;
+    if (a->out_dtype == PLATTICE_F32)
+        e = a->dtype == PLATTICE_F32    ? launch_grad_z<float, float>(g, p.parts_b, s)
+            : a->dtype == PLATTICE_BF16 ? launch_grad_z<float, __nv_bfloat16>(g, p.parts_b, s)
+                                        : launch_grad_z<float, __half>(g, p.parts_b, s);
+    else
+        e = a->dtype == PLATTICE_BF16 ? launch_grad_z<__nv_bfloat16, __nv_bfloat16>(g, p.parts_b, s)
+                                      : launch_grad_z<__half, __half>(g, p.parts_b, s);
+    if (e == cudaSuccess && a->grad_bias) e = column_sums(a->grad_bias, a->bias_dtype, g.partial, p.parts_b, a->n, s);
+    return e;
+}
+
+static cudaError_t backward_simt(const plattice_linear_args* a, const BackwardPlan& p, cudaStream_t s) {
+    char* ws = static_cast<char*>(a->workspace);
+    cudaError_t e = cudaSuccess;
+    if (a->grad_x) {
+        float* acc = reinterpret_cast<float*>(ws + p.acc_x);
+        e = product(acc, view_rows(ws + p.gz, nullptr, p.pitch, a->dtype, false),
+                    view_rows(a->w, nullptr, a->k, a->dtype, true), a->rows, a->k, a->n, 1, s);
+        if (e == cudaSuccess) e = add_parts_to(a->grad_x, a->dtype, acc, 1, a->rows * a->k, s);
+    }
+    if (e == cudaSuccess && a->grad_w) {
+        float* part = reinterpret_cast<float*>(ws + p.partial_w);
+        e = product(part, view_rows(ws + p.gz, nullptr, p.pitch, a->dtype, true),
+                    view_rows(a->x, a->x_scale, a->k, a->dtype, true), a->n, a->k, a->rows, p.parts_w, s);
+        if (e == cudaSuccess) e = add_parts_to(a->grad_w, a->dtype, part, p.parts_w, (int64_t)a->n * a->k, s);
+    }
+    return e;
+}
+
+static cudaError_t backward_mma(const plattice_linear_args* a, const BackwardPlan& p, cudaStream_t s) {
+    char* ws = static_cast<char*>(a->workspace);
+    Operand gz{p.gz_needed ? ws + p.gz : a->grad0, a->rows, a->n, p.gz_needed ? p.pitch : a->n,
+               a->dtype == PLATTICE_F32 ? 3 : 1};
+    cudaError_t e = cudaSuccess;
+    MmaArgs m{};
+    m.half = a->dtype == PLATTICE_F16;
+    m.fault = pl::fault_word();
+    if (a->grad_x) {
+        Operand w;
+        e = operand(&w, a->w, a->dtype, a->n, a->k, ws + p.w, s);
+        if (e != cudaSuccess) return e;
+        m.y0 = a->grad_x;
+        m.ni = a->rows;
+        m.nj = a->k;
+        m.out_dtype = a->dtype;
+        m.vec = a->k % 8 == 0 && aligned16(a->grad_x);
+        sum_args(&m, a->n, 1, gz.parts, w.parts);
+        e = run_mma<kGradX, false>(p.bn_x, gz, w, m, s);
+        if (e != cudaSuccess) return e;
+    }
+    if (a->grad_w) {
+        Operand x;
+        if (!a->x_scale) e = operand(&x, a->x, a->dtype, a->rows, a->k, ws + p.x, s);
+        if (e != cudaSuccess) return e;
+        m.ni = a->k;
+        m.nj = a->n;
+        sum_args(&m, a->rows, p.parts_w, x.parts, gz.parts);
+        const bool direct = p.parts_w == 1;
+        m.y0 = direct ? a->grad_w : ws + p.partial_w;
+        m.out_dtype = direct ? a->dtype : PLATTICE_F32;
+        x8_args(&m, a);
+        e = a->x_scale ? run_mma<kGradW, true>(p.bn_w, x, gz, m, s) : run_mma<kGradW, false>(p.bn_w, x, gz, m, s);
+        if (e == cudaSuccess && !direct)
+            e = add_parts_to(a->grad_w, a->dtype, reinterpret_cast<const float*>(ws + p.partial_w), m.parts,
+                             (int64_t)a->n * a->k, s);
+    }
+    return e;
 }
 
 }  // namespace plr
@@ -304,7 +701,7 @@ extern "C" {
 
 int plattice_linear_workspace_size(const plattice_linear_args* a, size_t* bytes) {
     if (!bytes || !linear_shape_ok(a)) return PLATTICE_ERR_INVALID;
-    *bytes = (size_t)up256(a->rows * a->n * 4);
+    *bytes = (size_t)forward_plan(a).bytes;
     return PLATTICE_OK;
 }
 
@@ -313,25 +710,12 @@ int plattice_linear(const plattice_linear_args* a, void* stream) {
     if (a->rows == 0) return PLATTICE_OK;
     if (!a->x || !a->w || !a->y0 || (a->split && !a->y1) || (a->z_scale && !a->z)) return PLATTICE_ERR_INVALID;
     if (a->split && a->residual) return PLATTICE_ERR_INVALID;
-    size_t need = 0;
-    plattice_linear_workspace_size(a, &need);
-    if (!a->workspace || a->workspace_bytes < need) return PLATTICE_ERR_WORKSPACE;
+    const ForwardPlan p = forward_plan(a);
+    if (p.bytes && (!a->workspace || a->workspace_bytes < (size_t)p.bytes)) return PLATTICE_ERR_WORKSPACE;
+    const int rc = rows_poll("plattice_linear");
+    if (rc != PLATTICE_OK) return rc;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    float* acc = static_cast<float*>(a->workspace);
-    cudaError_t e = product(acc, view_rows(a->x, a->x_scale, a->k, a->dtype, false),
-                            view_rows(a->w, nullptr, a->k, a->dtype, false), a->rows, a->n, a->k, 1, s);
-    if (e == cudaSuccess) {
-        const FinishArgs f{acc, a->bias, a->bias_dtype, a->residual, a->y0, a->y1, a->z, a->z_scale, a->rows,
-                           a->n, a->split, a->act, a->out_dtype};
-        const unsigned groups = (unsigned)(width8(a->n) / 8);
-        const int64_t ctas = (a->rows * groups + 255) / 256;
-        if (ctas > INT_MAX) return PLATTICE_ERR_INVALID;
-        if (a->out_dtype == PLATTICE_F32) k_finish<float><<<(unsigned)ctas, 256, 0, s>>>(f, groups);
-        else if (a->out_dtype == PLATTICE_BF16) k_finish<__nv_bfloat16><<<(unsigned)ctas, 256, 0, s>>>(f, groups);
-        else k_finish<__half><<<(unsigned)ctas, 256, 0, s>>>(f, groups);
-        e = cudaGetLastError();
-    }
-    return rows_status(e, "plattice_linear");
+    return rows_status(p.mma ? forward_mma(a, p, s) : forward_simt(a, p, s), "plattice_linear");
 }
 
 int plattice_linear_backward_workspace_size(const plattice_linear_args* a, size_t* bytes) {
@@ -355,30 +739,10 @@ int plattice_linear_backward(const plattice_linear_args* a, void* stream) {
         return PLATTICE_ERR_INVALID;
     const BackwardPlan p = backward_plan(a);
     if (!a->workspace || a->workspace_bytes < (size_t)p.bytes) return PLATTICE_ERR_WORKSPACE;
-    char* ws = static_cast<char*>(a->workspace);
-    GradArgs g{a->grad0, a->grad1, a->z, a->z_scale, ws + p.gz, p.pitch,
-               a->grad_bias ? reinterpret_cast<float*>(ws + p.partial_b) : nullptr, a->rows, a->n, a->split, a->act};
-    if (a->out_dtype == PLATTICE_F32) {
-        e = a->dtype == PLATTICE_F32    ? launch_grad_z<float, float>(g, p.parts_b, s)
-            : a->dtype == PLATTICE_BF16 ? launch_grad_z<float, __nv_bfloat16>(g, p.parts_b, s)
-                                        : launch_grad_z<float, __half>(g, p.parts_b, s);
-    } else {
-        e = a->dtype == PLATTICE_BF16 ? launch_grad_z<__nv_bfloat16, __nv_bfloat16>(g, p.parts_b, s)
-                                      : launch_grad_z<__half, __half>(g, p.parts_b, s);
-    }
-    if (e == cudaSuccess && a->grad_bias) e = column_sums(a->grad_bias, a->bias_dtype, g.partial, p.parts_b, a->n, s);
-    if (e == cudaSuccess && a->grad_x) {
-        float* acc = reinterpret_cast<float*>(ws + p.acc_x);
-        e = product(acc, view_rows(g.gz, nullptr, p.pitch, a->dtype, false),
-                    view_rows(a->w, nullptr, a->k, a->dtype, true), a->rows, a->k, a->n, 1, s);
-        if (e == cudaSuccess) e = add_parts_to(a->grad_x, a->dtype, acc, 1, a->rows * a->k, s);
-    }
-    if (e == cudaSuccess && a->grad_w) {
-        float* part = reinterpret_cast<float*>(ws + p.partial_w);
-        e = product(part, view_rows(g.gz, nullptr, p.pitch, a->dtype, true),
-                    view_rows(a->x, a->x_scale, a->k, a->dtype, true), a->n, a->k, a->rows, p.parts_w, s);
-        if (e == cudaSuccess) e = add_parts_to(a->grad_w, a->dtype, part, p.parts_w, (int64_t)a->n * a->k, s);
-    }
+    const int rc = rows_poll("plattice_linear_backward");
+    if (rc != PLATTICE_OK) return rc;
+    e = grad_z(a, p, s);
+    if (e == cudaSuccess) e = p.mma ? backward_mma(a, p, s) : backward_simt(a, p, s);
     return rows_status(e, "plattice_linear_backward");
 }
 

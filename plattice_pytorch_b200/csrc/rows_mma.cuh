@@ -1,0 +1,616 @@
+// rows_mma.cuh -- the products of the linear map on the tensor cores
+// (tcgen05, operands by TMA, accumulators in tensor memory).
+//
+//   D[i][j] = sum over r of A(i, r) B(j, r)
+//
+// in three kinds, by what i, j, r are and along which index each operand is
+// contiguous ("K-major": along the sum; "MN-major": along the result):
+//   kForward   i row, j output channel, r input channel   A = x   K   B = w   K
+//   kGradX     i row, j input channel,  r output channel  A = gz  K   B = w   MN
+//   kGradW     i input channel, j output channel, r row   A = x   MN  B = gz  MN
+// so no operand is ever transposed in memory.
+//
+// Operands are 16-bit.  float32 operands come as three bfloat16 parts whose
+// sum is the value (8 + 8 + 8 significant bits); the six products of parts
+// down to 2^-16 of the largest are added, the small ones first.  An 8-bit x
+// is widened to bfloat16 (exact) on its way to shared memory by warps of its
+// own, so HBM carries one byte a value.
+//
+// One CTA per SM walks over 128 x kBN tiles of D (times parts of the sum for
+// kGradW): one thread issues TMA copies of 64-deep slices into a ring of
+// stages, one issues the MMAs, eight warps empty the other of two
+// accumulators (activation, residual, stores) meanwhile.  Every wait is
+// bounded: a wait that gives up ends all roles, copies and MMAs in flight are
+// waited for, tensor memory is freed and the call's failure is reported.
+#pragma once
+#include <cuda.h>
+
+#include "rows_common.cuh"
+
+namespace plr {
+
+enum Kind { kForward = 0, kGradX = 1, kGradW = 2 };
+
+constexpr int kBM = 128, kBK = 64;
+constexpr int kEpilogueWarps = 8, kConvertWarps = 8;
+constexpr int kRoleThreads = 128 + 32 * kEpilogueWarps;
+constexpr int kStageA = kBM * kBK * 2;
+constexpr int kMaxSmem = 232448;   // shared memory a CTA can have
+
+__host__ __device__ constexpr bool a_mn(int kind) { return kind == kGradW; }
+__host__ __device__ constexpr bool b_mn(int kind) { return kind != kForward; }
+// MN-major slices come in groups of 64 columns
+__host__ __device__ constexpr int b_columns(int kind, int bn) { return b_mn(kind) && bn < 64 ? 64 : bn; }
+__host__ __device__ constexpr int stage_bytes(int kind, int bn) { return kStageA + b_columns(kind, bn) * kBK * 2; }
+constexpr int kWarpStaging = 32 * 32 * 4 + 32 * 4;   // a 32 x 32 float tile and 32 biases
+constexpr int kFixedSmem = 1024 + kEpilogueWarps * kWarpStaging + 512;
+__host__ __device__ constexpr int stages(int kind, int bn) {
+    const int n = (kMaxSmem - kFixedSmem) / stage_bytes(kind, bn);
+    return n > 8 ? 8 : n;
+}
+__host__ __device__ constexpr int smem_bytes(int kind, int bn) {
+    return kFixedSmem + stages(kind, bn) * stage_bytes(kind, bn);
+}
+
+struct MmaArgs {
+    // result
+    void* y0;
+    void* y1;             // split: columns split.. of D
+    const void* bias;     // null: none
+    const void* residual;
+    void* z;              // kept pre-activation (null: none)
+    uint8_t* z_scale;
+    int64_t ni, nj;       // D is ni x nj
+    int bias_dtype, out_dtype, act, split;
+    bool vec;             // rows of y0, residual and z allow 16-byte accesses
+    // sum
+    int steps;            // 64-deep slices of r
+    int part_steps;       // of a part (kGradW); parts are numbered tile-slowest
+    int parts;
+    unsigned pairs_a, pairs_b;   // parts of A and B of each product, 2 bits each
+    int pairs;
+    bool half;            // operands are float16 (else bfloat16)
+    // 8-bit A
+    const uint8_t* q;
+    const uint8_t* q_scale;
+    int64_t q_rows;
+    int64_t q_width;
+    unsigned* fault;      // host-mapped word that reports a wait that gave up (may be null)
+};
+
+// ------------------------------------------------------------- PTX wrappers
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ void bar_init(uint32_t bar, int count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint32_t bar, int bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.release.cta.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint32_t bar, int parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n.reg .pred p;\n"
+        "mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n"
+        "selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return done != 0;
+}
+
+// Waits for the phase; false when another role has given up or the wait
+// itself does, after about two seconds of clock cycles.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, int parity, volatile int* dead) {
+    if (bar_try(bar, parity)) return true;
+    const long long begin = clock64();
+    for (int i = 0; i < (1 << 26); ++i) {
+        if (bar_try(bar, parity)) return true;
+        if ((i & 15) == 15 && (*dead || clock64() - begin > 4000000000ll)) break;
+    }
+    *dead = 1;
+    return false;
+}
+
+// The same for all lanes of a warp, with one answer.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, int parity, volatile int* dead) {
+    return __all_sync(0xffffffffu, bar_wait(bar, parity, dead));
+}
+
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+        : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+__device__ __forceinline__ void tmem_load32(float (&v)[32], uint32_t addr) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr)
+        : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// Shared-memory operand descriptor of a slice in the 128-byte swizzle: 8-row
+// groups of 128 bytes lie 1024 bytes apart (along i for K-major, along r for
+// MN-major slices); MN-major groups of 64 columns lie 64 rows = 8192 bytes apart.
+__device__ __forceinline__ uint64_t operand_desc(uint32_t addr, bool mn) {
+    const uint64_t lead = mn ? 8192 >> 4 : 1;
+    return (uint64_t)((addr & 0x3ffff) >> 4) | (lead << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// ------------------------------------------------------------------- tiles
+
+struct Tile {
+    int64_t i0, j0;
+    int part, begin, end;   // slices [begin, end) of the sum
+};
+
+// Tiles are numbered along j first, then i, then the parts of the sum.
+template <int kBN>
+__device__ __forceinline__ Tile tile_at(const MmaArgs& p, unsigned t) {
+    const unsigned nj = (unsigned)((p.nj + kBN - 1) / kBN), ni = (unsigned)((p.ni + kBM - 1) / kBM);
+    Tile r;
+    const unsigned u = t / nj;
+    r.j0 = (int64_t)(t - u * nj) * kBN;
+    r.part = (int)(u / ni);
+    r.i0 = (int64_t)(u - r.part * ni) * kBM;
+    r.begin = r.part * p.part_steps;
+    r.end = min(p.steps, r.begin + p.part_steps);
+    return r;
+}
+
+// ---------------------------------------------------------------- epilogue
+
+__device__ __forceinline__ void store8_as(void* p, int dtype, int64_t at, const float (&v)[8], bool vec, int n) {
+    if (dtype == PLATTICE_F32) store8(static_cast<float*>(p) + at, v, vec, n);
+    else if (dtype == PLATTICE_BF16) store8(static_cast<__nv_bfloat16*>(p) + at, v, vec, n);
+    else store8(static_cast<__half*>(p) + at, v, vec, n);
+}
+__device__ __forceinline__ void load8_as(float (&v)[8], const void* p, int dtype, int64_t at, bool vec, int n) {
+    if (dtype == PLATTICE_F32) load8(v, static_cast<const float*>(p) + at, vec, n);
+    else if (dtype == PLATTICE_BF16) load8(v, static_cast<const __nv_bfloat16*>(p) + at, vec, n);
+    else load8(v, static_cast<const __half*>(p) + at, vec, n);
+}
+
+// A warp's 32 x 32 tile in shared memory: float4 c of row r at slot c ^ (r & 7),
+// free of bank conflicts both a row per lane and 4 lanes a row.
+__device__ __forceinline__ float4* staged(float* s, int row, int c4) {
+    return reinterpret_cast<float4*>(s) + row * 8 + (c4 ^ (row & 7));
+}
+__device__ __forceinline__ float staged_at(const float* s, int row, int c) {
+    return s[row * 32 + (((c >> 2) ^ (row & 7)) << 2) + (c & 3)];
+}
+
+__device__ __forceinline__ void stage_rows(float* s, const float (&v)[32], int lane) {
+    __syncwarp();
+#pragma unroll
+    for (int c = 0; c < 8; ++c) *staged(s, lane, c) = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+    __syncwarp();
+}
+
+// Stores columns [c0, c0 + w) of the staged rows to a tensor of w columns whose
+// rows all lie in this tile: one run of 32 w elements, lane by lane.
+__device__ __forceinline__ void store_run(const float* s, void* dst, int dtype, int64_t row0, int rows, int c0, int w,
+                                          const void* add, int lane) {
+    const unsigned inv = 65536u / (unsigned)w + 1;   // t / w for t < 1024, w <= 32
+    for (int t = lane; t < rows * w; t += 32) {
+        const int r = (int)((t * inv) >> 16), c = t - r * w;
+        float v = staged_at(s, r, c0 + c);
+        if (add) v += load_param(add, dtype, row0 * w + t);
+        store_param(dst, dtype, row0 * w + t, v);
+    }
+}
+
+// The staged 32 x 32 tile at (row0, col0) of an [ni][nj] tensor, `add` (the
+// residual, same layout) added: 4 lanes a row, 8 columns each.
+__device__ __forceinline__ void store_tile(const float* s, void* dst, const MmaArgs& p, int64_t row0, int64_t col0,
+                                           const void* add, int lane) {
+    const int rows = (int)min((int64_t)32, p.ni - row0), left = (int)min((int64_t)32, p.nj - col0);
+    if (p.nj <= 32 && !(p.vec && left == 32)) {
+        store_run(s, dst, p.out_dtype, row0, rows, 0, left, add, lane);
+        return;
+    }
+    const int c = (lane & 3) * 8, n = left - c;
+#pragma unroll
+    for (int it = 0; it < 4; ++it) {
+        const int r = it * 8 + (lane >> 2);
+        if (r >= rows || n <= 0) continue;
+        const bool vec = p.vec && n >= 8;
+        const int64_t at = (row0 + r) * p.nj + col0 + c;
+        const float4 a = *staged(const_cast<float*>(s), r, c >> 2), b = *staged(const_cast<float*>(s), r, (c >> 2) + 1);
+        float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        if (add) {
+            float q[8];
+            load8_as(q, add, p.out_dtype, at, vec, n);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] += q[i];
+        }
+        store8_as(dst, p.out_dtype, at, v, vec, n);
+    }
+}
+
+// Two tensors of a split: columns below `split` and the others.
+__device__ __forceinline__ void store_split(const float* s, const MmaArgs& p, int64_t row0, int64_t col0, int lane) {
+    const int rows = (int)min((int64_t)32, p.ni - row0), left = (int)min((int64_t)32, p.nj - col0);
+    if (p.nj <= 32) {
+        store_run(s, p.y0, p.out_dtype, row0, rows, 0, p.split, nullptr, lane);
+        store_run(s, p.y1, p.out_dtype, row0, rows, p.split, (int)p.nj - p.split, nullptr, lane);
+        return;
+    }
+    const int64_t col = col0 + lane;
+    if (lane >= left) return;
+    for (int r = 0; r < rows; ++r) {
+        const float v = staged_at(s, r, lane);
+        if (col < p.split) store_param(p.y0, p.out_dtype, (row0 + r) * p.split + col, v);
+        else store_param(p.y1, p.out_dtype, (row0 + r) * (p.nj - p.split) + col - p.split, v);
+    }
+}
+
+template <int kAct> __device__ __forceinline__ void apply32(float (&v)[32]) {
+#pragma unroll
+    for (int c = 0; c < 32; ++c) v[c] = act_value(v[c], kAct);
+}
+
+// 32 columns of 32 rows, a row per lane.
+template <int kKind>
+__device__ __forceinline__ void finish32(float (&v)[32], const MmaArgs& p, const Tile& t, int64_t row0, int64_t col0,
+                                         float* s, int lane) {
+    if (col0 >= p.nj || row0 >= p.ni) return;
+    if (kKind == kGradW) {
+        // D is [input channel][output channel], its result [output channel]
+        // [input channel]: a lane per input channel stores whole lines
+        const int64_t i = row0 + lane;
+        if (i >= p.ni) return;
+        const int left = (int)min((int64_t)32, p.nj - col0);
+        const int64_t at = ((int64_t)t.part * p.nj + col0) * p.ni + i;
+#pragma unroll
+        for (int c = 0; c < 32; ++c)
+            if (c < left) store_param(p.y0, p.out_dtype, at + (int64_t)c * p.ni, v[c]);
+        return;
+    }
+    if (kKind == kForward) {
+        float* sb = s + 32 * 32;
+        if (p.bias) {
+            sb[lane] = col0 + lane < p.nj ? load_param(p.bias, p.bias_dtype, col0 + lane) : 0.f;
+            __syncwarp();
+#pragma unroll
+            for (int c = 0; c < 32; c += 4) {
+                const float4 b = *reinterpret_cast<const float4*>(sb + c);
+                v[c] += b.x; v[c + 1] += b.y; v[c + 2] += b.z; v[c + 3] += b.w;
+            }
+        }
+        if (p.z) {
+            if (p.z_scale) {   // 32 columns are one block of the 8-bit rows
+                float amax = 0.f;
+#pragma unroll
+                for (int c = 0; c < 32; ++c) amax = fmaxf(amax, finite_abs(v[c]));
+                const int e = block_exponent(amax);
+                if (row0 + lane < p.ni) {
+                    const int64_t blocks = (p.nj + 31) / 32, at = (row0 + lane) * blocks + col0 / 32;
+                    uint4* q = reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.z) + at * 32);
+                    const float inv = pow2(-e);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float a[8], b[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) a[i] = v[16 * h + i], b[i] = v[16 * h + 8 + i];
+                        const uint2 x = codes8(a, inv), y = codes8(b, inv);
+                        q[h] = make_uint4(x.x, x.y, y.x, y.y);
+                    }
+                    p.z_scale[at] = (uint8_t)(e + 127);
+                }
+            } else {
+                stage_rows(s, v, lane);
+                store_tile(s, p.z, p, row0, col0, nullptr, lane);
+            }
+        }
+        if (p.act == PLATTICE_ACT_RELU) apply32<PLATTICE_ACT_RELU>(v);
+        else if (p.act == PLATTICE_ACT_GELU) apply32<PLATTICE_ACT_GELU>(v);
+        else if (p.act == PLATTICE_ACT_SILU) apply32<PLATTICE_ACT_SILU>(v);
+    }
+    stage_rows(s, v, lane);
+    if (kKind == kForward && p.split) store_split(s, p, row0, col0, lane);
+    else store_tile(s, p.y0, p, row0, col0, kKind == kForward ? p.residual : nullptr, lane);
+}
+
+// ------------------------------------------------- widening an 8-bit operand
+
+constexpr int kAhead = 4;   // slices whose codes are in flight per thread
+
+struct Codes {
+    uint4 c[2];
+    uint8_t scale;
+};
+
+// 32 codes of one scale per thread and slice.  K-major: 128 rows x 64
+// channels, two threads a row; MN-major: 64 rows x 128 channels, neighbouring
+// lanes on neighbouring rows, so that the 8 lanes of a shared-memory phase
+// write 8 different 16-byte columns of the swizzle.
+template <bool kMN>
+__device__ __forceinline__ void convert_place(int t, int& row, int& channel) {
+    row = kMN ? t & 63 : t >> 1;
+    channel = kMN ? (t >> 6) * 32 : (t & 1) * 32;
+}
+
+template <bool kMN>
+__device__ __forceinline__ Codes load_codes(const MmaArgs& p, const Tile& t, int step, int thread) {
+    int row, ch;
+    convert_place<kMN>(thread, row, ch);
+    const int64_t m = (kMN ? (int64_t)step * kBK : t.i0) + row;
+    const int64_t c = (kMN ? t.i0 : (int64_t)step * kBK) + ch;
+    Codes r;
+    r.c[0] = r.c[1] = make_uint4(0, 0, 0, 0);
+    r.scale = 127;
+    if (m < p.q_rows && c < p.q_width) {
+        const int64_t at = m * p.q_width + c;
+        const uint4* src = reinterpret_cast<const uint4*>(p.q + at);
+        r.c[0] = src[0];
+        r.c[1] = src[1];
+        r.scale = p.q_scale[at >> 5];
+    }
+    return r;
+}
+
+template <bool kMN>
+__device__ __forceinline__ void store_codes(uint32_t slice, const Codes& k, int thread) {
+    int row, ch;
+    convert_place<kMN>(thread, row, ch);
+    const uint32_t base = slice + (kMN ? (ch >> 6) * 8192 : 0) + row * 128;
+    const int chunk = (ch & 63) >> 3;
+    const float scale = scale_of(k.scale);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint4& q = k.c[i >> 1];
+        const uint2 w = i & 1 ? make_uint2(q.z, q.w) : make_uint2(q.x, q.y);
+        float f[8];
+        values8(f, w, scale);
+        union { uint4 u; __nv_bfloat162 h[4]; } o;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o.h[j] = __floats2bfloat162_rn(f[2 * j], f[2 * j + 1]);   // exact
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(base + (((chunk + i) ^ (row & 7)) << 4)),
+                     "r"(o.u.x), "r"(o.u.y), "r"(o.u.z), "r"(o.u.w)
+                     : "memory");
+    }
+}
+
+// -------------------------------------------------------------- the kernel
+
+template <int kKind, bool kX8, int kBN>
+__global__ void __launch_bounds__(kRoleThreads + (kX8 ? 32 * kConvertWarps : 0), 1)
+    k_mma(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const MmaArgs p,
+          unsigned tiles) {
+    constexpr int kStages = stages(kKind, kBN);
+    constexpr int kStage = stage_bytes(kKind, kBN);
+    constexpr int kColumns = 2 * kBN;   // tensor memory: two accumulators
+    extern __shared__ char smem_raw[];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int dead_flag;
+    volatile int* dead = &dead_flag;
+
+    char* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
+    const uint32_t ring = smem_addr(smem);
+    float* staging = reinterpret_cast<float*>(smem + kStages * kStage);
+    const uint32_t bars = smem_addr(smem + kStages * kStage + kEpilogueWarps * kWarpStaging);
+    auto full = [&](int s) { return bars + 8 * s; };
+    auto empty = [&](int s) { return bars + 8 * (kStages + s); };
+    auto acc_full = [&](int b) { return bars + 8 * (2 * kStages + b); };
+    auto acc_empty = [&](int b) { return bars + 8 * (2 * kStages + 2 + b); };
+    const uint32_t drained = bars + 8 * (2 * kStages + 4);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        dead_flag = 0;
+        for (int s = 0; s < kStages; ++s) {
+            bar_init(full(s), 1 + (kX8 ? kConvertWarps : 0));
+            bar_init(empty(s), 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            bar_init(acc_full(b), 1);
+            bar_init(acc_empty(b), kEpilogueWarps);
+        }
+        bar_init(drained, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 2) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_slot)),
+                     "r"(kColumns)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = tmem_slot;
+
+    if (warp == 0) {
+        // ---- TMA copies
+        if (lane == 0) {
+            int s = 0, phase = 0, issued = 0;
+            for (unsigned t = blockIdx.x; t < tiles && !*dead; t += gridDim.x) {
+                const Tile tile = tile_at<kBN>(p, t);
+                for (int pair = 0; pair < p.pairs; ++pair) {
+                    const int za = (p.pairs_a >> (2 * pair)) & 3, zb = (p.pairs_b >> (2 * pair)) & 3;
+                    for (int k = tile.begin; k < tile.end; ++k) {
+                        if (!bar_wait(empty(s), phase ^ 1, dead)) goto copies_done;
+                        const uint32_t a = ring + s * kStage, b = a + kStageA;
+                        bar_expect(full(s), (kX8 ? 0 : kStageA) + b_columns(kKind, kBN) * kBK * 2);
+                        if (!kX8) {
+                            if (a_mn(kKind)) {
+                                for (int g = 0; g < kBM / 64; ++g)
+                                    tma_load(a + g * 8192, &map_a, full(s), (int)tile.i0 + g * 64, k * kBK, za);
+                            } else {
+                                tma_load(a, &map_a, full(s), k * kBK, (int)tile.i0, za);
+                            }
+                        }
+                        if (b_mn(kKind)) {
+                            for (int g = 0; g < b_columns(kKind, kBN) / 64; ++g)
+                                tma_load(b + g * 8192, &map_b, full(s), (int)tile.j0 + g * 64, k * kBK, zb);
+                        } else {
+                            tma_load(b, &map_b, full(s), k * kBK, (int)tile.j0, zb);
+                        }
+                        ++issued;
+                        if (++s == kStages) s = 0, phase ^= 1;
+                    }
+                }
+            }
+        copies_done:
+            if (*dead) {   // no thread leaves while a copy may still write here
+                for (int b = issued < kStages ? issued : kStages; b > 0; --b) {
+                    const int n = issued - b, at = n % kStages, par = (n / kStages) & 1;
+                    const long long begin = clock64();
+                    while (!bar_try(full(at), par) && clock64() - begin < 200000000ll) {}
+                }
+            }
+        }
+    } else if (warp == 1) {
+        // ---- MMAs
+        if (lane == 0) {
+            const uint32_t fmt = p.half ? 0u : 1u;
+            const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)a_mn(kKind) << 15) |
+                                   ((uint32_t)b_mn(kKind) << 16) | ((uint32_t)(kBN >> 3) << 17) |
+                                   ((uint32_t)(kBM >> 4) << 24);
+            constexpr int kStepA = (a_mn(kKind) ? 2048 : 32) >> 4, kStepB = (b_mn(kKind) ? 2048 : 32) >> 4;
+            int s = 0, phase = 0, n = 0;
+            for (unsigned t = blockIdx.x; t < tiles; t += gridDim.x, ++n) {
+                const Tile tile = tile_at<kBN>(p, t);
+                const int buf = n & 1;
+                if (!bar_wait(acc_empty(buf), ((n >> 1) & 1) ^ 1, dead)) break;
+                fence_after();
+                const uint32_t d = tmem + buf * kBN;
+                const int count = p.pairs * (tile.end - tile.begin);
+                int k = 0;
+                for (; k < count; ++k) {
+                    if (!bar_wait(full(s), phase, dead)) break;
+                    fence_after();
+                    const uint64_t a = operand_desc(ring + s * kStage, a_mn(kKind));
+                    const uint64_t b = operand_desc(ring + s * kStage + kStageA, b_mn(kKind));
+#pragma unroll
+                    for (int u = 0; u < kBK / 16; ++u)
+                        mma_f16(d, a + u * kStepA, b + u * kStepB, idesc, k > 0 || u > 0);
+                    mma_commit(empty(s));
+                    if (++s == kStages) s = 0, phase ^= 1;
+                }
+                if (k < count) break;
+                mma_commit(acc_full(buf));
+            }
+            if (*dead) {   // MMAs in flight end before the shared memory they read goes
+                mma_commit(drained);
+                const long long begin = clock64();
+                while (!bar_try(drained, 0) && clock64() - begin < 200000000ll) {}
+            }
+        }
+    } else if (warp >= 4 && warp < 4 + kEpilogueWarps) {
+        // ---- epilogue: warp w reads the 32 accumulator rows 32 (w % 4)..,
+        // the two warps of a quarter alternate over its 32-column pieces
+        const int quarter = warp & 3, half = (warp - 4) >> 2;
+        float* s = staging + (warp - 4) * (kWarpStaging / 4);
+        int n = 0;
+        for (unsigned t = blockIdx.x; t < tiles; t += gridDim.x, ++n) {
+            const Tile tile = tile_at<kBN>(p, t);
+            const int buf = n & 1;
+            if (!warp_wait(acc_full(buf), (n >> 1) & 1, dead)) break;
+            fence_after();
+            const uint32_t base = tmem + buf * kBN + ((uint32_t)(quarter * 32) << 16);
+            constexpr int kPieces = kBN / 32;
+#pragma unroll 1
+            for (int c = half; c < kPieces; c += 2) {
+                float v[32];
+                __syncwarp();
+                tmem_load32(v, base + c * 32);
+                if (c + 2 >= kPieces) {
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(acc_empty(buf));
+                }
+                finish32<kKind>(v, p, tile, tile.i0 + quarter * 32, tile.j0 + c * 32, s, lane);
+            }
+            if (half >= kPieces && lane == 0) bar_arrive(acc_empty(buf));
+        }
+    } else if (kX8 && warp >= 4 + kEpilogueWarps) {
+        // ---- widening 8-bit rows
+        const int thread = threadIdx.x - kRoleThreads;
+        constexpr bool kMN = a_mn(kKind);
+        Codes ahead[kAhead];
+        // cursor of the next slice to load
+        unsigned lt = blockIdx.x;
+        Tile ltile = lt < tiles ? tile_at<kBN>(p, lt) : Tile{};
+        int lpair = 0, lk = ltile.begin;
+        auto load_next = [&](Codes& c) {
+            if (lt >= tiles) return false;
+            c = load_codes<kMN>(p, ltile, lk, thread);
+            if (++lk == ltile.end) {
+                lk = ltile.begin;
+                if (++lpair == p.pairs) {
+                    lpair = 0;
+                    lt += gridDim.x;
+                    if (lt < tiles) {
+                        ltile = tile_at<kBN>(p, lt);
+                        lk = ltile.begin;
+                    }
+                }
+            }
+            return true;
+        };
+        bool have[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) have[u] = load_next(ahead[u]);
+        int s = 0, phase = 0;
+        bool more = true;
+        while (more) {
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                if (!more || !have[u]) {
+                    more = false;
+                    continue;
+                }
+                if (!warp_wait(empty(s), phase ^ 1, dead)) {
+                    more = false;
+                    continue;
+                }
+                store_codes<kMN>(ring + s * kStage, ahead[u], thread);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the MMA reads what was written
+                __syncwarp();
+                if (lane == 0) bar_arrive(full(s));
+                if (++s == kStages) s = 0, phase ^= 1;
+                have[u] = load_next(ahead[u]);
+            }
+        }
+    }
+    __syncwarp();
+    fence_before();
+    __syncthreads();
+    fence_after();
+    if (warp == 2)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kColumns) : "memory");
+    if (threadIdx.x == 0 && dead_flag && p.fault) *reinterpret_cast<volatile unsigned*>(p.fault) = 1;
+}
+
+}  // namespace plr
