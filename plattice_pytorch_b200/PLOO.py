@@ -38,7 +38,7 @@ __all__ = ["forward", "backward", "Lattice", "lattice_forward", "lattice_backwar
            "lattice_filter", "lattice_filter_backward", "feature_grad", "BatchLattice", "batch_forward",
            "batch_backward", "forward_batch", "backward_batch", "lattice_info", "vertex_keys",
            "check_device_status", "prepare", "set_graph_cache", "graph_cache_stats", "set_keep_lattice",
-           "get_keep_lattice"]
+           "get_keep_lattice", "set_checkpoint_precision", "get_checkpoint_precision"]
 
 _CHECK = os.environ.get("PLATTICE_CHECK", "0") not in ("", "0")
 
@@ -50,6 +50,10 @@ _CHECK = os.environ.get("PLATTICE_CHECK", "0") not in ("", "0")
 # its outputs, and the backward allocates the full lattice and scratch for its
 # duration.  PLATTICE_KEEP_LATTICE=0 or set_keep_lattice(False).
 _KEEP = os.environ.get("PLATTICE_KEEP_LATTICE", "1") not in ("", "0")
+
+# Whether PermutoLatticeFeatureFunction keeps values and out in 8 bits for its
+# backward; set_checkpoint_precision.
+_CHECKPOINT8 = False
 
 _F32 = torch.float32
 _cur_dev = torch._C._cuda_getDevice
@@ -573,6 +577,24 @@ def set_keep_lattice(keep):
 def get_keep_lattice():
     """The setting of :func:`set_keep_lattice`."""
     return _KEEP
+
+
+def set_checkpoint_precision(precision):
+    """How PermutoLatticeFeatureFunction keeps the filter's values and results
+    from forward to backward, where the feature gradient reads them again:
+    ``"fp32"`` (default, as they are) or ``"8bit"`` (``rows.pack8``: 1.03 bytes a
+    value; each is off by at most 2^-4 of itself in the feature gradient, the
+    forward and the value gradient do not change).  Applies to the forwards
+    made after it.  No counterpart in the reference, which has no feature
+    gradient (plattice.py:19)."""
+    global _CHECKPOINT8
+    _require(precision in ("fp32", "8bit"), f"checkpoint precision must be 'fp32' or '8bit', got {precision!r}")
+    _CHECKPOINT8 = precision == "8bit"
+
+
+def get_checkpoint_precision():
+    """The setting of :func:`set_checkpoint_precision`."""
+    return "8bit" if _CHECKPOINT8 else "fp32"
 
 
 def get_lattice_precision():

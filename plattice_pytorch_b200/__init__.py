@@ -7,7 +7,9 @@ libplattice_b200.so through the C ABI of include/plattice.h.
 """
 from . import PLOO, rows
 from .plattice import (LatticeFilterFunction, PermutoLattice, PermutoLatticeBatchFunction,
-                       PermutoLatticeFeatureFunction, PermutoLatticeFunction)
+                       PermutoLatticeFeatureFunction, PermutoLatticeFunction, PermutoLatticeLayer,
+                       RowLinearFunction, RowNormLinearFunction)
 
 __all__ = ["PLOO", "rows", "PermutoLattice", "PermutoLatticeFunction", "PermutoLatticeBatchFunction",
-           "PermutoLatticeFeatureFunction", "LatticeFilterFunction"]
+           "PermutoLatticeFeatureFunction", "LatticeFilterFunction", "PermutoLatticeLayer", "RowLinearFunction",
+           "RowNormLinearFunction"]

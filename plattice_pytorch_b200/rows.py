@@ -195,8 +195,9 @@ def rms_norm_backward(grad_y, h, rstd, gain, grad_h=None):
 
 # ---------------------------------------------------------------- the linear map
 
-def _linear_common(x, weight, act, out_dtype):
-    """Checked (args struct, shape before the channels, out dtype, device) of a linear call."""
+def _linear_common(x, weight, act, out_dtype, lead=None):
+    """Checked (args struct, shape before the channels, out dtype, device) of a
+    linear call; ``lead`` is that shape where ``x`` is None."""
     _check_input(weight, "weight")
     _require(weight.dtype in _DTYPES, "weight must be float32, bfloat16 or float16")
     _require(weight.dim() == 2 and weight.shape[0] >= 1 and weight.shape[1] >= 1, "weight must be [n, k]")
@@ -204,20 +205,22 @@ def _linear_common(x, weight, act, out_dtype):
     if isinstance(x, Rows8):
         _require(weight.dtype != torch.float16, "weight must be float32 or bfloat16 for 8-bit rows")
         _require(x.shape[-1] == k, f"x must have {k} channels")
-    else:
+    elif x is not None:
         _check_rows(x, "x", k)
         _require(x.dtype == weight.dtype, "x and weight must have the same type")
-    _require(weight.device == x.device, "x and weight must be on the same device")
+    dev = weight.device
+    _require(x is None or x.device == dev, "x and weight must be on the same device")
     _require(act in ACTIVATIONS, f"act must be one of {', '.join(ACTIVATIONS)}")
     out_dtype = weight.dtype if out_dtype is None else out_dtype
     _require(out_dtype in (weight.dtype, torch.float32), "out_dtype must be float32 or the weight's type")
     a = _lib.LinearArgs()
-    a.x, a.x_scale = (x.q.data_ptr(), x.scale.data_ptr()) if isinstance(x, Rows8) else (x.data_ptr(), None)
+    a.x, a.x_scale = (x.q.data_ptr(), x.scale.data_ptr()) if isinstance(x, Rows8) else (_ptr(x), None)
     a.w = weight.data_ptr()
-    a.rows, a.k, a.n, a.act = _rows_of(x.shape), k, n, ACTIVATIONS[act]
+    lead = tuple(x.shape[:-1]) if lead is None else lead
+    a.rows, a.k, a.n, a.act = _rows_of(lead + (k,)), k, n, ACTIVATIONS[act]
     a.dtype = a.bias_dtype = _DTYPES[weight.dtype]
     a.out_dtype = _DTYPES[out_dtype]
-    return a, tuple(x.shape[:-1]), out_dtype, x.device
+    return a, lead, out_dtype, dev
 
 
 def _linear_call(name, a, dev):
@@ -281,12 +284,14 @@ def linear_backward(grad_y, x, weight, z=None, act="none", bias_dtype=None, need
 
     ``grad_y`` as the forward's ``y`` (a pair after a split); ``x`` and ``z`` what
     the forward read and kept, tensors or :class:`Rows8` (``z`` only with an
-    activation).  The gradient of the residual is ``grad_y`` itself."""
+    activation; ``x`` may be None when ``grad_weight`` is not wanted).  The
+    gradient of the residual is ``grad_y`` itself."""
     pair = isinstance(grad_y, (tuple, list))
     _require(not pair or len(grad_y) == 2, "grad_y must be a tensor or a pair of tensors")
     first = grad_y[0] if pair else grad_y
     _check_rows(first, "grad_y")
-    a, lead, out_dtype, dev = _linear_common(x, weight, act, first.dtype)
+    _require(x is not None or not need[1], "x is needed for grad_weight")
+    a, lead, out_dtype, dev = _linear_common(x, weight, act, first.dtype, tuple(first.shape[:-1]) if x is None else None)
     n = a.n
     if pair:
         a.split = int(first.shape[-1])
