@@ -127,26 +127,36 @@ __device__ __forceinline__ int block_exponent(float amax) {
 
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }   // -126 <= e <= 127
 
-__device__ __forceinline__ float finite_abs(float v) {
-    const float a = fabsf(v);
-    return a <= 3.402823466e38f ? a : 0.f;
+__device__ __forceinline__ bool is_infinite(float a) { return a > 3.402823466e38f; }   // of a magnitude
+
+// Largest finite magnitude of v (fmaxf passes over NaN by itself).  Infinities
+// become NaN on the way, which is the code they get.
+template <int N>
+__device__ __forceinline__ float finite_amax(float (&v)[N]) {
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) amax = fmaxf(amax, fabsf(v[i]));
+    if (is_infinite(amax)) {   // rare: look at each
+        amax = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (is_infinite(fabsf(v[i]))) v[i] = __int_as_float(0x7fffffff);
+            amax = fmaxf(amax, fabsf(v[i]));
+        }
+    }
+    return amax;
 }
 
-// Codes of 8 values times 2^-s (multiplying by a power of two is exact, so
-// the one rounding is the conversion's); not finite -> the NaN code.
-__device__ __forceinline__ uint2 codes8(const float (&v)[8], float inv) {
+// Codes of 8 values, finite or NaN, times 2^-s (multiplying by a power of two
+// is exact, so the one rounding is the conversion's).
+__device__ __forceinline__ uint2 codes8(const float* v, float inv) {
     unsigned w[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        float t[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            t[j] = v[4 * i + j];
-            t[j] = fabsf(t[j]) <= 3.402823466e38f ? t[j] * inv : __int_as_float(0x7fffffff);
-        }
-        w[i] = __nv_cvt_float2_to_fp8x2(make_float2(t[0], t[1]), __NV_SATFINITE, __NV_E4M3) |
-               ((unsigned)__nv_cvt_float2_to_fp8x2(make_float2(t[2], t[3]), __NV_SATFINITE, __NV_E4M3) << 16);
-    }
+    for (int i = 0; i < 2; ++i)
+        w[i] = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * i] * inv, v[4 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3) |
+               ((unsigned)__nv_cvt_float2_to_fp8x2(make_float2(v[4 * i + 2] * inv, v[4 * i + 3] * inv), __NV_SATFINITE,
+                                                   __NV_E4M3)
+                << 16);
     return make_uint2(w[0], w[1]);
 }
 
@@ -179,18 +189,30 @@ template <> __device__ __forceinline__ float within<__half>(float v) {
 // reciprocal, an exponential and six multiply-adds.  The product's epilogue
 // computes it for every output on the way out, where a full-precision erf
 // would take longer than the matrix instructions it runs beside.
-__device__ __forceinline__ float tail(float z, float& e) {
-    const float x = fabsf(z) * 0.70710678118654752f;
-    const float t = __fdividef(1.f, fmaf(0.3275911f, x, 1.f));
-    e = __expf(-x * x);
-    float q = fmaf(1.061405429f, t, -1.453152027f);
-    q = fmaf(q, t, 1.421413741f);
-    q = fmaf(q, t, -0.284496736f);
-    q = fmaf(q, t, 0.254829592f);
-    return 0.5f * q * t * e;
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float reciprocal_fast(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
-__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
+__device__ __forceinline__ float tail(float z, float& e) {
+    const float t = reciprocal_fast(fmaf(0.3275911f * 0.70710678118654752f, fabsf(z), 1.f));
+    e = exp2_fast(z * z * -0.72134752044448170f);   // log2(e) / 2
+    float q = fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
+    q = fmaf(q, t, 0.5f * 1.421413741f);
+    q = fmaf(q, t, 0.5f * -0.284496736f);
+    q = fmaf(q, t, 0.5f * 0.254829592f);
+    return q * t * e;
+}
+
+__device__ __forceinline__ float sigmoid(float z) {
+    return reciprocal_fast(1.f + exp2_fast(z * -1.4426950408889634f));
+}
 
 // NaN stays NaN; the products with an infinite z are kept out of 0 x infinity.
 __device__ __forceinline__ float act_value(float z, int act) {

@@ -114,9 +114,7 @@ __global__ void __launch_bounds__(256) k_finish(const FinishArgs a, unsigned gro
         for (int i = 0; i < 8; ++i) y[i] += r[i];
     }
     if (a.z_scale) {
-        float amax = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) amax = fmaxf(amax, finite_abs(z[i]));
+        float amax = finite_amax(z);
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
         const int s = block_exponent(amax);
@@ -203,61 +201,74 @@ struct GradArgs {
     float* partial;     // [gridDim.y][n]; null: no bias gradient
     int64_t rows;
     int n, split, act;
+    int shift;          // log2 of the threads that share a row
+    bool vec;           // rows of grad_y and z allow 16-byte accesses
 };
+
+template <int kAct>
+__device__ __forceinline__ void times_slope(float (&g)[8], const float (&z)[8], int left) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (i < left) g[i] *= act_slope(z[i], kAct);
+}
 
 // gz = grad_y act'(z), rounded to the operands' type for the two products (a
 // tensor core takes no wider operand; one rounding, as a stored gradient has),
-// and the sums of the unrounded gz over a CTA's rows.  32 lanes of 8 columns,
-// 8 rows at a time; gridDim.x strips of 256 columns, gridDim.y parts of rows.
+// and the sums of the unrounded gz over a CTA's rows.  2^shift threads of 8
+// columns share a row; gridDim.x strips of columns, gridDim.y parts of rows.
 template <typename TG, typename T>
-__global__ void __launch_bounds__(256) k_grad_z(const GradArgs a) {
-    __shared__ float sums[8][256];
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const int col = blockIdx.x * 256 + lane * 8;
+__global__ void __launch_bounds__(256, 4) k_grad_z(const GradArgs a) {
+    __shared__ float sums[8 * 256];
+    const int lane = threadIdx.x & ((1 << a.shift) - 1), rows = 256 >> a.shift;
+    const int col = ((int)blockIdx.x << (a.shift + 3)) + lane * 8;
+    const int left = a.n - col, wide = (int)min(a.pitch - col, (int64_t)8);
+    const bool vec = a.vec && left >= 8;
     float acc[8] = {};
-    for (int64_t row = (int64_t)blockIdx.y * 8 + w; row < a.rows; row += (int64_t)gridDim.y * 8) {
-        const int left = a.n - col;
-        float g[8], z[8];
-        if (a.split == 0) {
-            load8(g, static_cast<const TG*>(a.g0) + (left > 0 ? row * a.n + col : 0), false, left);
-        } else {
+    if (left > 0) {
+        for (int64_t row = (int64_t)blockIdx.y * rows + (threadIdx.x >> a.shift); row < a.rows;
+             row += (int64_t)gridDim.y * rows) {
+            float g[8], z[8];
+            if (a.split == 0) {
+                load8(g, static_cast<const TG*>(a.g0) + row * a.n + col, vec, left);
+            } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int c = col + i;
-                g[i] = i >= left ? 0.f
-                       : c < a.split ? to_f32(static_cast<const TG*>(a.g0)[row * a.split + c])
-                                     : to_f32(static_cast<const TG*>(a.g1)[row * (a.n - a.split) + c - a.split]);
+                for (int i = 0; i < 8; ++i) {
+                    const int c = col + i;
+                    g[i] = i >= left ? 0.f
+                           : c < a.split ? to_f32(static_cast<const TG*>(a.g0)[row * a.split + c])
+                                         : to_f32(static_cast<const TG*>(a.g1)[row * (a.n - a.split) + c - a.split]);
+                }
             }
-        }
-        if (a.act != PLATTICE_ACT_NONE) {
-            if (a.z_scale) {
-                if (left > 0) {
+            if (a.act != PLATTICE_ACT_NONE) {
+                if (a.z_scale) {
                     const int64_t at = row * (width8(a.n) / 8) + col / 8;
                     values8(z, reinterpret_cast<const uint2*>(a.z)[at], scale_of(a.z_scale[at >> 2]));
+                } else {
+                    load8(z, static_cast<const TG*>(a.z) + row * a.n + col, vec, left);
                 }
-            } else {
-                load8(z, static_cast<const TG*>(a.z) + (left > 0 ? row * a.n + col : 0), false, left);
+                if (a.act == PLATTICE_ACT_RELU) times_slope<PLATTICE_ACT_RELU>(g, z, left);
+                else if (a.act == PLATTICE_ACT_GELU) times_slope<PLATTICE_ACT_GELU>(g, z, left);
+                else times_slope<PLATTICE_ACT_SILU>(g, z, left);
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (i < left) g[i] *= act_slope(z[i], a.act);
+            for (int i = 0; i < 8; ++i) acc[i] += g[i];
+            if (!a.gz) continue;
+            const int64_t at = row * a.pitch + col;   // zeros up to the pitch
+            if (sizeof(T) == 4 && a.parts)
+                store_parts(static_cast<__nv_bfloat16*>(a.gz) + at, a.rows * a.pitch, g, wide == 8, wide);
+            else
+                store8(static_cast<T*>(a.gz) + at, g, a.pitch % 8 == 0 && wide == 8, wide);
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) acc[i] += g[i];
-        const int64_t wide = a.pitch - col;   // zeros up to the pitch
-        if (!a.gz || wide <= 0) continue;
-        const int64_t at = row * a.pitch + col;
-        if (sizeof(T) == 4 && a.parts) store_parts(static_cast<__nv_bfloat16*>(a.gz) + at, a.rows * a.pitch, g, wide >= 8, (int)min(wide, (int64_t)8));
-        else store8(static_cast<T*>(a.gz) + at, g, a.pitch % 8 == 0 && wide >= 8, (int)min(wide, (int64_t)8));
     }
     if (!a.partial) return;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sums[w][lane * 8 + i] = acc[i];
+    for (int i = 0; i < 8; ++i) sums[i * 256 + threadIdx.x] = acc[i];
     __syncthreads();
-    const int c = blockIdx.x * 256 + threadIdx.x;
+    if (threadIdx.x >> (a.shift + 3)) return;
+    const int l = threadIdx.x & ((1 << a.shift) - 1), i = threadIdx.x >> a.shift;
+    const int c = ((int)blockIdx.x << (a.shift + 3)) + l * 8 + i;
     float s = 0.f;
-#pragma unroll
-    for (int r = 0; r < 8; ++r) s += sums[r][threadIdx.x];
+    for (int r = 0; r < rows; ++r) s += sums[i * 256 + (r << a.shift) + l];
     if (c < a.n) a.partial[(int64_t)blockIdx.y * a.n + c] = s;
 }
 
@@ -493,8 +504,13 @@ static void sum_args(MmaArgs* p, int64_t nr, int parts, int parts_a, int parts_b
     }
 }
 
+// The 8-bit x as a bfloat16 operand in `ws`.
+static cudaError_t unpacked(Operand* o, const plattice_linear_args* a, void* ws, cudaStream_t s) {
+    *o = Operand{ws, a->rows, a->k, up8(a->k), 1};
+    return unpack_rows(ws, PLATTICE_BF16, o->pitch, static_cast<const uint8_t*>(a->x), a->x_scale, a->rows, a->k, s);
+}
+
 static void x8_args(MmaArgs* p, const plattice_linear_args* a) {
-    if (!a->x_scale) return;
     p->q = static_cast<const uint8_t*>(a->x);
     p->q_scale = a->x_scale;
     p->q_rows = a->rows;
@@ -507,8 +523,15 @@ static bool on_tensor_cores(const plattice_linear_args* a) {
     return a->dtype != PLATTICE_F32 || (double)a->rows * a->k * a->n >= 64.0 * 1024 * 1024;
 }
 
+// Whether an 8-bit x is unpacked to bfloat16 before the product rather than on
+// its way through it: when several tiles along j would each widen the same
+// slice (the widening and the MMA share the shared memory's bandwidth, so a
+// 256-wide tile then runs at a third of its rate), one pass over x, 5 bytes a
+// value, costs less.
+static bool unpack_first(int n, int bn) { return n > bn; }
+
 struct ForwardPlan {
-    bool mma;
+    bool mma, unpack;
     int bn;
     int64_t x, w, acc, bytes;
 };
@@ -519,7 +542,9 @@ static ForwardPlan forward_plan(const plattice_linear_args* a) {
     p.mma = on_tensor_cores(a);
     if (p.mma) {
         p.bn = choose_bn(a->rows, a->n, 32);
-        p.x = a->x_scale || tma_ready(a->x, a->dtype, a->k) ? 0 : c.take(repack_bytes(a->dtype, a->rows, a->k));
+        p.unpack = a->x_scale && unpack_first(a->n, p.bn);
+        if (p.unpack) p.x = c.take(a->rows * up8(a->k) * 2);
+        else if (!a->x_scale && !tma_ready(a->x, a->dtype, a->k)) p.x = c.take(repack_bytes(a->dtype, a->rows, a->k));
         p.w = tma_ready(a->w, a->dtype, a->k) ? 0 : c.take(repack_bytes(a->dtype, a->n, a->k));
     } else {
         p.acc = c.take(a->rows * a->n * 4);
@@ -529,7 +554,8 @@ static ForwardPlan forward_plan(const plattice_linear_args* a) {
 }
 
 struct BackwardPlan {
-    bool mma, gz_needed;
+    bool mma, gz_needed, unpack;
+    int shift, strips;
     int bn_x, bn_w, parts_b, parts_w;
     int64_t gz, x, w, partial_b, partial_w, acc_x, pitch, bytes;
 };
@@ -538,8 +564,9 @@ static BackwardPlan backward_plan(const plattice_linear_args* a) {
     BackwardPlan p{};
     Carve c;
     p.mma = on_tensor_cores(a);
-    const int64_t strips = ceil_div(a->n, 256), need = ceil_div(a->rows, 8);
-    const int64_t most = ceil_div(4 * (int64_t)sm_count(), strips);
+    while (p.shift < 5 && (8 << p.shift) < a->n) ++p.shift;   // a row's columns / 8, at most a warp
+    p.strips = (int)ceil_div(a->n, 8 << p.shift);
+    const int64_t need = ceil_div(a->rows, 256 >> p.shift), most = ceil_div(8 * (int64_t)sm_count(), p.strips);
     p.parts_b = (int)(need < most ? need : most);
     if (p.parts_b < 1) p.parts_b = 1;
     p.partial_b = c.take((int64_t)p.parts_b * a->n * 4);
@@ -553,6 +580,8 @@ static BackwardPlan backward_plan(const plattice_linear_args* a) {
         p.bn_w = a->n > 128 ? 256 : a->n > 64 ? 128 : a->n > 32 ? 64 : 32;
         p.parts_w = choose_parts(a->k, a->n, p.bn_w, ceil_div(a->rows, kBK));
         if (a->grad_x && !tma_ready(a->w, a->dtype, a->k)) p.w = c.take(repack_bytes(a->dtype, a->n, a->k));
+        p.unpack = a->x_scale && unpack_first(a->n, p.bn_w);
+        if (a->grad_w && p.unpack) p.x = c.take(a->rows * up8(a->k) * 2);
         if (a->grad_w && !a->x_scale && !tma_ready(a->x, a->dtype, a->k))
             p.x = c.take(repack_bytes(a->dtype, a->rows, a->k));
         if (a->grad_w && p.parts_w > 1) p.partial_w = c.take((int64_t)p.parts_w * a->n * a->k * 4);
@@ -568,8 +597,8 @@ static BackwardPlan backward_plan(const plattice_linear_args* a) {
 }
 
 template <typename TG, typename T>
-static cudaError_t launch_grad_z(const GradArgs& g, int parts, cudaStream_t s) {
-    k_grad_z<TG, T><<<dim3((unsigned)ceil_div(g.n, 256), parts), 256, 0, s>>>(g);
+static cudaError_t launch_grad_z(const GradArgs& g, const BackwardPlan& p, cudaStream_t s) {
+    k_grad_z<TG, T><<<dim3(p.strips, p.parts_b), 256, 0, s>>>(g);
     return cudaGetLastError();
 }
 
@@ -591,7 +620,8 @@ static cudaError_t forward_mma(const plattice_linear_args* a, const ForwardPlan&
     char* ws = static_cast<char*>(a->workspace);
     Operand x, w;
     cudaError_t e = cudaSuccess;
-    if (!a->x_scale) e = operand(&x, a->x, a->dtype, a->rows, a->k, ws + p.x, s);
+    if (p.unpack) e = unpacked(&x, a, ws + p.x, s);
+    else if (!a->x_scale) e = operand(&x, a->x, a->dtype, a->rows, a->k, ws + p.x, s);
     if (e == cudaSuccess) e = operand(&w, a->w, a->dtype, a->n, a->k, ws + p.w, s);
     if (e != cudaSuccess) return e;
     MmaArgs m{};
@@ -612,8 +642,9 @@ static cudaError_t forward_mma(const plattice_linear_args* a, const ForwardPlan&
     m.half = a->dtype == PLATTICE_F16;
     m.fault = pl::fault_word();
     sum_args(&m, a->k, 1, x.parts, w.parts);
+    if (!a->x_scale || p.unpack) return run_mma<kForward, false>(p.bn, x, w, m, s);
     x8_args(&m, a);
-    return a->x_scale ? run_mma<kForward, true>(p.bn, x, w, m, s) : run_mma<kForward, false>(p.bn, x, w, m, s);
+    return run_mma<kForward, true>(p.bn, x, w, m, s);
 }
 
 static cudaError_t grad_z(const plattice_linear_args* a, const BackwardPlan& p, cudaStream_t s) {
@@ -622,15 +653,16 @@ static cudaError_t grad_z(const plattice_linear_args* a, const BackwardPlan& p, 
     if (!store && !a->grad_bias) return cudaSuccess;
     const GradArgs g{a->grad0, a->grad1, a->z, a->z_scale, store ? ws + p.gz : nullptr, p.pitch, p.mma,
                      a->grad_bias ? reinterpret_cast<float*>(ws + p.partial_b) : nullptr, a->rows, a->n, a->split,
-                     a->act};
+                     a->act, p.shift,
+                     a->n % 8 == 0 && aligned16(a->grad0) && (!a->z || a->z_scale || aligned16(a->z))};
     cudaError_t e;
     if (a->out_dtype == PLATTICE_F32)
-        e = a->dtype == PLATTICE_F32    ? launch_grad_z<float, float>(g, p.parts_b, s)
-            : a->dtype == PLATTICE_BF16 ? launch_grad_z<float, __nv_bfloat16>(g, p.parts_b, s)
-                                        : launch_grad_z<float, __half>(g, p.parts_b, s);
+        e = a->dtype == PLATTICE_F32    ? launch_grad_z<float, float>(g, p, s)
+            : a->dtype == PLATTICE_BF16 ? launch_grad_z<float, __nv_bfloat16>(g, p, s)
+                                        : launch_grad_z<float, __half>(g, p, s);
     else
-        e = a->dtype == PLATTICE_BF16 ? launch_grad_z<__nv_bfloat16, __nv_bfloat16>(g, p.parts_b, s)
-                                      : launch_grad_z<__half, __half>(g, p.parts_b, s);
+        e = a->dtype == PLATTICE_BF16 ? launch_grad_z<__nv_bfloat16, __nv_bfloat16>(g, p, s)
+                                      : launch_grad_z<__half, __half>(g, p, s);
     if (e == cudaSuccess && a->grad_bias) e = column_sums(a->grad_bias, a->bias_dtype, g.partial, p.parts_b, a->n, s);
     return e;
 }
@@ -676,7 +708,8 @@ static cudaError_t backward_mma(const plattice_linear_args* a, const BackwardPla
     }
     if (a->grad_w) {
         Operand x;
-        if (!a->x_scale) e = operand(&x, a->x, a->dtype, a->rows, a->k, ws + p.x, s);
+        if (p.unpack) e = unpacked(&x, a, ws + p.x, s);
+        else if (!a->x_scale) e = operand(&x, a->x, a->dtype, a->rows, a->k, ws + p.x, s);
         if (e != cudaSuccess) return e;
         m.ni = a->k;
         m.nj = a->n;
@@ -684,8 +717,12 @@ static cudaError_t backward_mma(const plattice_linear_args* a, const BackwardPla
         const bool direct = p.parts_w == 1;
         m.y0 = direct ? a->grad_w : ws + p.partial_w;
         m.out_dtype = direct ? a->dtype : PLATTICE_F32;
-        x8_args(&m, a);
-        e = a->x_scale ? run_mma<kGradW, true>(p.bn_w, x, gz, m, s) : run_mma<kGradW, false>(p.bn_w, x, gz, m, s);
+        if (!a->x_scale || p.unpack) {
+            e = run_mma<kGradW, false>(p.bn_w, x, gz, m, s);
+        } else {
+            x8_args(&m, a);
+            e = run_mma<kGradW, true>(p.bn_w, x, gz, m, s);
+        }
         if (e == cudaSuccess && !direct)
             e = add_parts_to(a->grad_w, a->dtype, reinterpret_cast<const float*>(ws + p.partial_w), m.parts,
                              (int64_t)a->n * a->k, s);

@@ -229,10 +229,59 @@ __device__ __forceinline__ void store_run(const float* s, void* dst, int dtype, 
     }
 }
 
+// 32 x 32 of the residual as store_tile's lanes take them, loaded a piece
+// ahead: a load waited for at each store would cost a trip to HBM four times a
+// piece (652 us against 2xx at 32768 x 1024 -> 4096, gelu, residual, kept z).
+struct Ahead {
+    uint4 r[8];   // 4 rows of 8 columns; 16-bit types use the first 4
+    bool have;
+};
+
+__device__ __forceinline__ void load_ahead(Ahead& a, const MmaArgs& p, int64_t row0, int64_t col0, int lane) {
+    a.have = p.residual && p.vec && col0 + 32 <= p.nj && row0 + 32 <= p.ni;
+    if (!a.have) return;
+#pragma unroll
+    for (int it = 0; it < 4; ++it) {
+        const int64_t at = (row0 + it * 8 + (lane >> 2)) * p.nj + col0 + (lane & 3) * 8;
+        if (p.out_dtype == PLATTICE_F32) {
+            const uint4* src = reinterpret_cast<const uint4*>(static_cast<const float*>(p.residual) + at);
+            a.r[2 * it] = src[0];
+            a.r[2 * it + 1] = src[1];
+        } else {
+            a.r[it] = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.residual) + at);
+        }
+    }
+}
+
+template <typename T> __device__ __forceinline__ void add_pairs(float (&v)[8], const uint4& r) {
+    union { uint4 u; typename Pair<T>::type h[4]; } x;
+    x.u = r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = pair_f32(x.h[i]);
+        v[2 * i] += f.x;
+        v[2 * i + 1] += f.y;
+    }
+}
+
+__device__ __forceinline__ void add_ahead(float (&v)[8], const Ahead& a, int it, int dtype) {
+    if (dtype == PLATTICE_F32) {
+        const uint4 x = a.r[2 * it], y = a.r[2 * it + 1];
+        v[0] += __uint_as_float(x.x); v[1] += __uint_as_float(x.y);
+        v[2] += __uint_as_float(x.z); v[3] += __uint_as_float(x.w);
+        v[4] += __uint_as_float(y.x); v[5] += __uint_as_float(y.y);
+        v[6] += __uint_as_float(y.z); v[7] += __uint_as_float(y.w);
+    } else if (dtype == PLATTICE_BF16) {
+        add_pairs<__nv_bfloat16>(v, a.r[it]);
+    } else {
+        add_pairs<__half>(v, a.r[it]);
+    }
+}
+
 // The staged 32 x 32 tile at (row0, col0) of an [ni][nj] tensor, `add` (the
 // residual, same layout) added: 4 lanes a row, 8 columns each.
 __device__ __forceinline__ void store_tile(const float* s, void* dst, const MmaArgs& p, int64_t row0, int64_t col0,
-                                           const void* add, int lane) {
+                                           const void* add, const Ahead& ahead, int lane) {
     const int rows = (int)min((int64_t)32, p.ni - row0), left = (int)min((int64_t)32, p.nj - col0);
     if (p.nj <= 32 && !(p.vec && left == 32)) {
         store_run(s, dst, p.out_dtype, row0, rows, 0, left, add, lane);
@@ -247,7 +296,9 @@ __device__ __forceinline__ void store_tile(const float* s, void* dst, const MmaA
         const int64_t at = (row0 + r) * p.nj + col0 + c;
         const float4 a = *staged(const_cast<float*>(s), r, c >> 2), b = *staged(const_cast<float*>(s), r, (c >> 2) + 1);
         float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-        if (add) {
+        if (add && ahead.have) {
+            add_ahead(v, ahead, it, p.out_dtype);
+        } else if (add) {
             float q[8];
             load8_as(q, add, p.out_dtype, at, vec, n);
 #pragma unroll
@@ -282,7 +333,7 @@ template <int kAct> __device__ __forceinline__ void apply32(float (&v)[32]) {
 // 32 columns of 32 rows, a row per lane.
 template <int kKind>
 __device__ __forceinline__ void finish32(float (&v)[32], const MmaArgs& p, const Tile& t, int64_t row0, int64_t col0,
-                                         float* s, int lane) {
+                                         float* s, const Ahead& ahead, float bias, int lane) {
     if (col0 >= p.nj || row0 >= p.ni) return;
     if (kKind == kGradW) {
         // D is [input channel][output channel], its result [output channel]
@@ -299,7 +350,7 @@ __device__ __forceinline__ void finish32(float (&v)[32], const MmaArgs& p, const
     if (kKind == kForward) {
         float* sb = s + 32 * 32;
         if (p.bias) {
-            sb[lane] = col0 + lane < p.nj ? load_param(p.bias, p.bias_dtype, col0 + lane) : 0.f;
+            sb[lane] = bias;
             __syncwarp();
 #pragma unroll
             for (int c = 0; c < 32; c += 4) {
@@ -309,27 +360,24 @@ __device__ __forceinline__ void finish32(float (&v)[32], const MmaArgs& p, const
         }
         if (p.z) {
             if (p.z_scale) {   // 32 columns are one block of the 8-bit rows
-                float amax = 0.f;
+                float u[32];   // v itself keeps its infinities for the activation
 #pragma unroll
-                for (int c = 0; c < 32; ++c) amax = fmaxf(amax, finite_abs(v[c]));
-                const int e = block_exponent(amax);
+                for (int c = 0; c < 32; ++c) u[c] = v[c];
+                const int e = block_exponent(finite_amax(u));
                 if (row0 + lane < p.ni) {
                     const int64_t blocks = (p.nj + 31) / 32, at = (row0 + lane) * blocks + col0 / 32;
                     uint4* q = reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.z) + at * 32);
                     const float inv = pow2(-e);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        float a[8], b[8];
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) a[i] = v[16 * h + i], b[i] = v[16 * h + 8 + i];
-                        const uint2 x = codes8(a, inv), y = codes8(b, inv);
+                        const uint2 x = codes8(u + 16 * h, inv), y = codes8(u + 16 * h + 8, inv);
                         q[h] = make_uint4(x.x, x.y, y.x, y.y);
                     }
                     p.z_scale[at] = (uint8_t)(e + 127);
                 }
             } else {
                 stage_rows(s, v, lane);
-                store_tile(s, p.z, p, row0, col0, nullptr, lane);
+                store_tile(s, p.z, p, row0, col0, nullptr, ahead, lane);
             }
         }
         if (p.act == PLATTICE_ACT_RELU) apply32<PLATTICE_ACT_RELU>(v);
@@ -338,7 +386,7 @@ __device__ __forceinline__ void finish32(float (&v)[32], const MmaArgs& p, const
     }
     stage_rows(s, v, lane);
     if (kKind == kForward && p.split) store_split(s, p, row0, col0, lane);
-    else store_tile(s, p.y0, p, row0, col0, kKind == kForward ? p.residual : nullptr, lane);
+    else store_tile(s, p.y0, p, row0, col0, kKind == kForward ? p.residual : nullptr, ahead, lane);
 }
 
 // ------------------------------------------------- widening an 8-bit operand
@@ -536,6 +584,17 @@ __global__ void __launch_bounds__(kRoleThreads + (kX8 ? 32 * kConvertWarps : 0),
         for (unsigned t = blockIdx.x; t < tiles; t += gridDim.x, ++n) {
             const Tile tile = tile_at<kBN>(p, t);
             const int buf = n & 1;
+            const int64_t row0 = tile.i0 + quarter * 32;
+            Ahead ahead;
+            float bias = 0.f;
+            auto look_ahead = [&](int c) {
+                const int64_t col0 = tile.j0 + c * 32;
+                if (kKind != kForward) return;
+                load_ahead(ahead, p, row0, col0, lane);
+                if (p.bias && col0 + lane < p.nj) bias = load_param(p.bias, p.bias_dtype, col0 + lane);
+                else bias = 0.f;
+            };
+            look_ahead(half);
             if (!warp_wait(acc_full(buf), (n >> 1) & 1, dead)) break;
             fence_after();
             const uint32_t base = tmem + buf * kBN + ((uint32_t)(quarter * 32) << 16);
@@ -550,7 +609,8 @@ __global__ void __launch_bounds__(kRoleThreads + (kX8 ? 32 * kConvertWarps : 0),
                     __syncwarp();
                     if (lane == 0) bar_arrive(acc_empty(buf));
                 }
-                finish32<kKind>(v, p, tile, tile.i0 + quarter * 32, tile.j0 + c * 32, s, lane);
+                finish32<kKind>(v, p, tile, row0, tile.j0 + c * 32, s, ahead, bias, lane);
+                if (c + 2 < kPieces) look_ahead(c + 2);
             }
             if (half >= kPieces && lane == 0) bar_arrive(acc_empty(buf));
         }

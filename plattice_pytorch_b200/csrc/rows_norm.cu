@@ -33,32 +33,36 @@ struct GroupAt {
     }
 };
 
-template <typename T>
+// kFlat: rows without padding and aligned (c a multiple of 32), so that group g
+// is elements 8 g.. whatever its row: no division.
+template <typename T, bool kFlat>
 __global__ void __launch_bounds__(256) k_pack8(uint8_t* __restrict__ q, uint8_t* __restrict__ scale,
                                                const T* __restrict__ x, int64_t rows, int c, unsigned groups, bool vec) {
-    const int64_t base = (int64_t)blockIdx.x * (256 * kUnits);
-    const GroupAt where(base, groups);
+    const int64_t base = (int64_t)blockIdx.x * (256 * kUnits), all = rows * groups;
+    const GroupAt where(kFlat ? 0 : base, kFlat ? 1 : groups);
     float v[kUnits][8];
-    int64_t row[kUnits];
-    unsigned g[kUnits];
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {
-        where.at(threadIdx.x + 256 * u, row[u], g[u]);
-        const int left = row[u] < rows ? c - (int)g[u] * 8 : 0;
-        load8(v[u], x + (left > 0 ? row[u] * c + (int64_t)g[u] * 8 : 0), vec && left >= 8, left);
+        const int64_t at = base + threadIdx.x + 256 * u;
+        if (kFlat) {
+            load8(v[u], x + (at < all ? at : 0) * 8, true, 8);
+        } else {
+            int64_t row;
+            unsigned g;
+            where.at(threadIdx.x + 256 * u, row, g);
+            const int left = at < all ? c - (int)g * 8 : 0;
+            load8(v[u], x + (left > 0 ? row * c + (int64_t)g * 8 : 0), vec && left >= 8, left);
+        }
     }
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {
-        float amax = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) amax = fmaxf(amax, finite_abs(v[u][i]));
+        const int64_t at = base + threadIdx.x + 256 * u;
+        float amax = finite_amax(v[u]);
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
         const int s = block_exponent(amax);
-        if (row[u] >= rows) continue;
-        const uint2 w = codes8(v[u], pow2(-s));
-        const int64_t at = row[u] * groups + g[u];
-        reinterpret_cast<uint2*>(q)[at] = w;
+        if (at >= all) continue;
+        reinterpret_cast<uint2*>(q)[at] = codes8(v[u], pow2(-s));
         if ((threadIdx.x & 3) == 0) scale[at >> 2] = (uint8_t)(s + 127);
     }
 }
@@ -182,9 +186,7 @@ __global__ void __launch_bounds__(L > 256 ? L : 256) k_rms_norm(const NormArgs a
 #pragma unroll
             for (int i = 0; i < 8; ++i) y[i] = left > i ? v[k][i] * rstd * gain[k][i] : 0.f;
             if (a.yscale) {
-                float amax = 0.f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) amax = fmaxf(amax, finite_abs(y[i]));
+                float amax = finite_amax(y);
                 amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
                 amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
                 const int s = block_exponent(amax);
@@ -334,7 +336,10 @@ cudaError_t launch_pack(uint8_t* q, uint8_t* scale, const void* x, int64_t rows,
     const int64_t ctas = (rows * groups + 256 * kUnits - 1) / (256 * kUnits);
     if (ctas > INT_MAX) return cudaErrorInvalidValue;
     const bool vec = c % 8 == 0 && aligned16(x);
-    k_pack8<T><<<(unsigned)ctas, 256, 0, s>>>(q, scale, static_cast<const T*>(x), rows, c, groups, vec);
+    if (vec && c % kBlock8 == 0)
+        k_pack8<T, true><<<(unsigned)ctas, 256, 0, s>>>(q, scale, static_cast<const T*>(x), rows, c, groups, vec);
+    else
+        k_pack8<T, false><<<(unsigned)ctas, 256, 0, s>>>(q, scale, static_cast<const T*>(x), rows, c, groups, vec);
     return cudaGetLastError();
 }
 
@@ -356,12 +361,13 @@ cudaError_t unpack_rows(void* y, int dtype, int64_t pitch, const uint8_t* q, con
     return launch_unpack<__half>(y, pitch, q, scale, rows, c, s);
 }
 
-// CTAs of a grid-stride launch: what the rows need, at most 4 per SM of the
+// CTAs of a grid-stride launch: what the rows need, at most 8 per SM of the
 // current device (each then walks many rows and its loads of the gain and its
 // partial sums are paid once).
+constexpr int kNormCtas = 8;
 static int norm_ctas(int64_t rows, int rows_per_cta) {
     const int64_t need = (rows + rows_per_cta - 1) / rows_per_cta;
-    const int64_t most = 4 * (int64_t)sm_count();
+    const int64_t most = kNormCtas * (int64_t)sm_count();
     return (int)(need < most ? need : most);
 }
 
@@ -450,7 +456,7 @@ int plattice_rms_norm_backward_workspace_size(long long rows, int c, size_t* byt
     // one row of partial sums per CTA, whatever the device's SM count (<= 256)
     const int64_t per = norm_rows_per_cta(c);
     const int64_t need = (rows + per - 1) / per;
-    *bytes = (size_t)(need < 1024 ? (need < 1 ? 1 : need) : 1024) * c * sizeof(float);
+    *bytes = (size_t)(need < 2048 ? (need < 1 ? 1 : need) : 2048) * c * sizeof(float);
     return PLATTICE_OK;
 }
 
@@ -469,7 +475,7 @@ int plattice_rms_norm_backward(void* grad_x, void* grad_gain, const void* grad_y
     plattice_rms_norm_backward_workspace_size(rows, c, &need);
     if (workspace_bytes < need) return PLATTICE_ERR_WORKSPACE;
     int ctas = norm_ctas(rows, norm_rows_per_cta(c));
-    if (ctas > 1024) ctas = 1024;
+    if (ctas > 2048) ctas = 2048;
     NormGradArgs a{grad_x, static_cast<float*>(workspace), grad_y, h, rstd, gain, gain_dtype, grad_h, rows, c, false};
     a.vec = c % 8 == 0 && aligned16(grad_x) && aligned16(grad_y) && aligned16(h) && (!grad_h || aligned16(grad_h));
     cudaError_t e = dtype == PLATTICE_F32    ? launch_norm_grad<float>(a, ctas, s)
