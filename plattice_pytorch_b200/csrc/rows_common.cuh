@@ -115,6 +115,72 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8], bool vec, int 
     }
 }
 
+// ------------------------------------------------------ pairs of float32 values
+
+// Two multiply-adds in one instruction (f32x2).
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void pair_to(uint64_t p, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t both(float a) { return pair_of(a, a); }
+__device__ __forceinline__ void mul2(float& a, float& b, float x, float y) { pair_to(mul2(pair_of(a, b), pair_of(x, y)), a, b); }
+__device__ __forceinline__ void add2(float& a, float& b, float x, float y) { pair_to(add2(pair_of(a, b), pair_of(x, y)), a, b); }
+
+// 8 elements as loaded, to be widened when they are used: what a kernel holds
+// while the loads of its next row are in flight.
+template <typename T> struct Raw8 {
+    uint4 u;
+    __device__ __forceinline__ void load(const T* p, bool vec, int n) {
+        if (vec) {
+            u = *reinterpret_cast<const uint4*>(p);
+        } else {
+            union { uint4 w; T h[8]; } r;
+            r.w = make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i < n) r.h[i] = p[i];
+            u = r.w;
+        }
+    }
+    __device__ __forceinline__ void widen(float (&v)[8]) const {
+        union { uint4 w; typename Pair<T>::type h[4]; } r;
+        r.w = u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = pair_f32(r.h[i]);
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
+        }
+    }
+};
+template <> struct Raw8<float> {
+    float v8[8];
+    __device__ __forceinline__ void load(const float* p, bool vec, int n) { load8(v8, p, vec, n); }
+    __device__ __forceinline__ void widen(float (&v)[8]) const {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = v8[i];
+    }
+};
+
 // --------------------------------------------------------------- 8-bit rows
 
 // s of a block whose largest finite magnitude is amax: amax = 1.f * 2^e needs
@@ -147,17 +213,44 @@ __device__ __forceinline__ float finite_amax(float (&v)[N]) {
     return amax;
 }
 
+// The same of values that must stay: infinities are passed over in amax and
+// codes8_of gives them the NaN code.
+template <int N>
+__device__ __forceinline__ float finite_amax_of(const float (&v)[N], bool& infinite) {
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) amax = fmaxf(amax, fabsf(v[i]));
+    infinite = is_infinite(amax);
+    if (infinite) {
+        amax = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) amax = is_infinite(fabsf(v[i])) ? amax : fmaxf(amax, fabsf(v[i]));
+    }
+    return amax;
+}
+
 // Codes of 8 values, finite or NaN, times 2^-s (multiplying by a power of two
 // is exact, so the one rounding is the conversion's).
 __device__ __forceinline__ uint2 codes8(const float* v, float inv) {
     unsigned w[2];
+    const uint64_t m = both(inv);
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-        w[i] = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * i] * inv, v[4 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3) |
-               ((unsigned)__nv_cvt_float2_to_fp8x2(make_float2(v[4 * i + 2] * inv, v[4 * i + 3] * inv), __NV_SATFINITE,
-                                                   __NV_E4M3)
-                << 16);
+    for (int i = 0; i < 2; ++i) {
+        float2 lo, hi;
+        pair_to(mul2(pair_of(v[4 * i], v[4 * i + 1]), m), lo.x, lo.y);
+        pair_to(mul2(pair_of(v[4 * i + 2], v[4 * i + 3]), m), hi.x, hi.y);
+        w[i] = __nv_cvt_float2_to_fp8x2(lo, __NV_SATFINITE, __NV_E4M3) |
+               ((unsigned)__nv_cvt_float2_to_fp8x2(hi, __NV_SATFINITE, __NV_E4M3) << 16);
+    }
     return make_uint2(w[0], w[1]);
+}
+
+__device__ __forceinline__ uint2 codes8_of(const float* v, float inv, bool infinite) {
+    if (!infinite) return codes8(v, inv);
+    float t[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = is_infinite(fabsf(v[i])) ? __int_as_float(0x7fffffff) : v[i];
+    return codes8(t, inv);
 }
 
 __device__ __forceinline__ void values4(float* v, unsigned codes, float scale) {
@@ -183,12 +276,6 @@ template <> __device__ __forceinline__ float within<__half>(float v) {
 
 // -------------------------------------------------------------- activations
 
-// Phi(-|z|) and exp(-z^2 / 2), by the rational approximation of the error
-// function 7.1.26 of Abramowitz and Stegun, Handbook of Mathematical
-// Functions (off by at most 1.5e-7 of erf, about a float32 step of 1): a
-// reciprocal, an exponential and six multiply-adds.  The product's epilogue
-// computes it for every output on the way out, where a full-precision erf
-// would take longer than the matrix instructions it runs beside.
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -199,47 +286,95 @@ __device__ __forceinline__ float reciprocal_fast(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-
-__device__ __forceinline__ float tail(float z, float& e) {
-    const float t = reciprocal_fast(fmaf(0.3275911f * 0.70710678118654752f, fabsf(z), 1.f));
-    e = exp2_fast(z * z * -0.72134752044448170f);   // log2(e) / 2
-    float q = fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
-    q = fmaf(q, t, 0.5f * 1.421413741f);
-    q = fmaf(q, t, 0.5f * -0.284496736f);
-    q = fmaf(q, t, 0.5f * 0.254829592f);
-    return q * t * e;
+// NaN stays NaN in both
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float y;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
 }
 
-__device__ __forceinline__ float sigmoid(float z) {
-    return reciprocal_fast(1.f + exp2_fast(z * -1.4426950408889634f));
+// Phi(-|z|) and exp(-z^2 / 2), by the rational approximation of the error
+// function 7.1.26 of Abramowitz and Stegun, Handbook of Mathematical
+// Functions (off by at most 1.5e-7 of erf, about a float32 step of 1): a
+// reciprocal, an exponential and six multiply-adds.  The product's epilogue
+// computes it for every output on the way out, where a full-precision erf
+// would take longer than the matrix instructions it runs beside.
+__device__ __forceinline__ uint64_t tail2(float z0, float z1, uint64_t& e) {
+    constexpr float kP = 0.3275911f * 0.70710678118654752f;
+    const uint64_t t = pair_of(reciprocal_fast(fmaf(kP, fabsf(z0), 1.f)), reciprocal_fast(fmaf(kP, fabsf(z1), 1.f)));
+    const uint64_t z = pair_of(z0, z1);
+    float x0, x1;
+    pair_to(mul2(mul2(z, both(-0.72134752044448170f)), z), x0, x1);   // log2(e) / 2
+    e = pair_of(exp2_fast(x0), exp2_fast(x1));
+    uint64_t q = fma2(both(0.5f * 1.061405429f), t, both(0.5f * -1.453152027f));
+    q = fma2(q, t, both(0.5f * 1.421413741f));
+    q = fma2(q, t, both(0.5f * -0.284496736f));
+    q = fma2(q, t, both(0.5f * 0.254829592f));
+    return mul2(mul2(q, t), e);
 }
 
-// NaN stays NaN; the products with an infinite z are kept out of 0 x infinity.
-__device__ __forceinline__ float act_value(float z, int act) {
-    if (act == PLATTICE_ACT_RELU) return z > 0.f ? z : (z == z ? 0.f : z);
-    if (act == PLATTICE_ACT_GELU) {   // z Phi(z) = max(z, 0) - |z| Phi(-|z|); beyond |z| = 16 the tail is 0
-        float e;
-        const float q = tail(z, e);
-        return fmaf(-fminf(fabsf(z), 16.f), q, z > 0.f ? z : z * 0.f);
+// The activation of a pair.  gelu: z Phi(z) = max(z, 0) - |z| Phi(-|z|), with
+// |z| held at 16, where the tail is 0, so that an infinite z has its limit.
+template <int kAct> __device__ __forceinline__ void act2(float& a, float& b) {
+    if (kAct == PLATTICE_ACT_RELU) {
+        a = max_nan(a, 0.f);
+        b = max_nan(b, 0.f);
+    } else if (kAct == PLATTICE_ACT_GELU) {
+        uint64_t e;
+        const uint64_t q = tail2(a, b, e);
+        pair_to(fma2(pair_of(-min_nan(fabsf(a), 16.f), -min_nan(fabsf(b), 16.f)), q,
+                     pair_of(fmaxf(a, 0.f), fmaxf(b, 0.f))),
+                a, b);
+    } else if (kAct == PLATTICE_ACT_SILU) {
+        float x, y;
+        pair_to(mul2(pair_of(a, b), both(-1.4426950408889634f)), x, y);
+        pair_to(add2(pair_of(exp2_fast(x), exp2_fast(y)), both(1.f)), x, y);
+        mul2(a, b, reciprocal_fast(x), reciprocal_fast(y));
     }
-    if (act == PLATTICE_ACT_SILU) return z * sigmoid(z);
-    return z;
 }
 
-// d act / d z
-__device__ __forceinline__ float act_slope(float z, int act) {
-    if (act == PLATTICE_ACT_RELU) return z > 0.f ? 1.f : (z == z ? 0.f : z);
-    if (act == PLATTICE_ACT_GELU) {   // Phi(z) + z phi(z)
-        float e;
-        const float q = tail(z, e);
-        const float zc = z > 16.f ? 16.f : (z < -16.f ? -16.f : z);   // a NaN stays
-        return fmaf(zc * 0.39894228040143268f, e, z >= 0.f ? 1.f - q : q);
+// d act / d z of a pair.  gelu: Phi(z) + z phi(z), z held in -16..16 (there
+// both have reached their limits).
+template <int kAct> __device__ __forceinline__ void slope2(float& a, float& b) {
+    if (kAct == PLATTICE_ACT_RELU) {
+        a = a > 0.f ? 1.f : (a == a ? 0.f : a);
+        b = b > 0.f ? 1.f : (b == b ? 0.f : b);
+    } else if (kAct == PLATTICE_ACT_GELU) {
+        const float x = max_nan(min_nan(a, 16.f), -16.f), y = max_nan(min_nan(b, 16.f), -16.f);
+        uint64_t e;
+        const uint64_t q = tail2(x, y, e);
+        float u, v;
+        pair_to(fma2(q, both(-1.f), both(0.5f)), u, v);   // 1/2 - Phi(-|z|), with the sign of z: Phi(z) - 1/2
+        const uint64_t p = add2(pair_of(copysignf(u, x), copysignf(v, y)), both(0.5f));
+        pair_to(fma2(mul2(pair_of(x, y), both(0.39894228040143268f)), e, p), a, b);
+    } else if (kAct == PLATTICE_ACT_SILU) {
+        float x, y;
+        const uint64_t z = pair_of(a, b);
+        pair_to(mul2(z, both(-1.4426950408889634f)), x, y);
+        pair_to(add2(pair_of(exp2_fast(x), exp2_fast(y)), both(1.f)), x, y);
+        const uint64_t s = pair_of(reciprocal_fast(x), reciprocal_fast(y));
+        // s (1 + z (1 - s))
+        pair_to(mul2(s, fma2(z, fma2(s, both(-1.f), both(1.f)), both(1.f))), a, b);
     }
-    if (act == PLATTICE_ACT_SILU) {
-        const float s = sigmoid(z);
-        return s * fmaf(z, 1.f - s, 1.f);
-    }
-    return 1.f;
+}
+
+template <int kAct, int N> __device__ __forceinline__ void activations(float (&v)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) act2<kAct>(v[i], v[i + 1]);
+}
+template <int kAct, int N> __device__ __forceinline__ void slopes(float (&v)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) slope2<kAct>(v[i], v[i + 1]);
+}
+template <int N> __device__ __forceinline__ void activate(float (&v)[N], int act) {
+    if (act == PLATTICE_ACT_RELU) activations<PLATTICE_ACT_RELU>(v);
+    else if (act == PLATTICE_ACT_GELU) activations<PLATTICE_ACT_GELU>(v);
+    else if (act == PLATTICE_ACT_SILU) activations<PLATTICE_ACT_SILU>(v);
 }
 
 }  // namespace plr

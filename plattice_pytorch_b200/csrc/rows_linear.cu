@@ -105,8 +105,9 @@ __global__ void __launch_bounds__(256) k_finish(const FinishArgs a, unsigned gro
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         if (a.bias && i < left) z[i] += load_param(a.bias, a.bias_dtype, col + i);
-        y[i] = act_value(z[i], a.act);
+        y[i] = z[i];
     }
+    activate(y, a.act);
     if (a.residual) {
         float r[8];
         load8(r, static_cast<const T*>(a.residual) + (left > 0 ? row * a.n + col : 0), false, left);
@@ -205,11 +206,12 @@ struct GradArgs {
     bool vec;           // rows of grad_y and z allow 16-byte accesses
 };
 
+// g *= slope(z); what lies behind the last column is 0 in both
 template <int kAct>
-__device__ __forceinline__ void times_slope(float (&g)[8], const float (&z)[8], int left) {
+__device__ __forceinline__ void times_slope(float (&g)[8], float (&z)[8]) {
+    slopes<kAct>(z);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (i < left) g[i] *= act_slope(z[i], kAct);
+    for (int i = 0; i < 8; i += 2) mul2(g[i], g[i + 1], z[i], z[i + 1]);
 }
 
 // gz = grad_y act'(z), rounded to the operands' type for the two products (a
@@ -246,9 +248,9 @@ __global__ void __launch_bounds__(256, 4) k_grad_z(const GradArgs a) {
                 } else {
                     load8(z, static_cast<const TG*>(a.z) + row * a.n + col, vec, left);
                 }
-                if (a.act == PLATTICE_ACT_RELU) times_slope<PLATTICE_ACT_RELU>(g, z, left);
-                else if (a.act == PLATTICE_ACT_GELU) times_slope<PLATTICE_ACT_GELU>(g, z, left);
-                else times_slope<PLATTICE_ACT_SILU>(g, z, left);
+                if (a.act == PLATTICE_ACT_RELU) times_slope<PLATTICE_ACT_RELU>(g, z);
+                else if (a.act == PLATTICE_ACT_GELU) times_slope<PLATTICE_ACT_GELU>(g, z);
+                else times_slope<PLATTICE_ACT_SILU>(g, z);
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) acc[i] += g[i];
@@ -463,7 +465,7 @@ static cudaError_t launch_mma(const Operand& a, const Operand& b, const MmaArgs&
         reinterpret_cast<const void*>(k_mma<kKind, kX8, kBN>),
         [](int*) {
             return cudaFuncSetAttribute(k_mma<kKind, kX8, kBN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        smem_bytes(kKind, kBN));
+                                        smem_bytes(kKind, kX8, kBN));
         },
         &unused);
     if (e != cudaSuccess) return e;
@@ -474,7 +476,7 @@ static cudaError_t launch_mma(const Operand& a, const Operand& b, const MmaArgs&
     const int64_t tiles = mma_tiles(p.ni, p.nj, kBN) * p.parts;
     if (tiles > INT_MAX) return cudaErrorInvalidValue;
     const int ctas = (int)(tiles < sm_count() ? tiles : sm_count());
-    k_mma<kKind, kX8, kBN><<<ctas, kRoleThreads + (kX8 ? 32 * kConvertWarps : 0), smem_bytes(kKind, kBN), s>>>(
+    k_mma<kKind, kX8, kBN><<<ctas, role_threads(kKind, kX8) + (kX8 ? 32 * kConvertWarps : 0), smem_bytes(kKind, kX8, kBN), s>>>(
         ma, mb, p, (unsigned)tiles);
     return cudaGetLastError();
 }

@@ -32,8 +32,13 @@ namespace plr {
 enum Kind { kForward = 0, kGradX = 1, kGradW = 2 };
 
 constexpr int kBM = 128, kBK = 64;
-constexpr int kEpilogueWarps = 8, kConvertWarps = 8;
-constexpr int kRoleThreads = 128 + 32 * kEpilogueWarps;
+constexpr int kConvertWarps = 8;
+// Warps that empty accumulators.  The forward's work per output (activation,
+// residual, 8-bit codes) waits more than it issues: 16 warps hide what 8 do
+// not (422 -> 2xx us at 32768 x 1024 -> 4096, gelu, residual, kept z).
+// Beside converting warps, and for the plain stores of the gradients, 8 do.
+__host__ __device__ constexpr int epilogue_warps(int kind, bool x8) { return kind == 0 && !x8 ? 16 : 8; }
+__host__ __device__ constexpr int role_threads(int kind, bool x8) { return 128 + 32 * epilogue_warps(kind, x8); }
 constexpr int kStageA = kBM * kBK * 2;
 constexpr int kMaxSmem = 232448;   // shared memory a CTA can have
 
@@ -42,14 +47,16 @@ __host__ __device__ constexpr bool b_mn(int kind) { return kind != kForward; }
 // MN-major slices come in groups of 64 columns
 __host__ __device__ constexpr int b_columns(int kind, int bn) { return b_mn(kind) && bn < 64 ? 64 : bn; }
 __host__ __device__ constexpr int stage_bytes(int kind, int bn) { return kStageA + b_columns(kind, bn) * kBK * 2; }
-constexpr int kWarpStaging = 32 * 32 * 4 + 32 * 4;   // a 32 x 32 float tile and 32 biases
-constexpr int kFixedSmem = 1024 + kEpilogueWarps * kWarpStaging + 512;
-__host__ __device__ constexpr int stages(int kind, int bn) {
-    const int n = (kMaxSmem - kFixedSmem) / stage_bytes(kind, bn);
+constexpr int kWarpStaging = 32 * 16 * 4 + 32 * 4;   // a 32 x 16 float tile and 32 biases
+__host__ __device__ constexpr int fixed_smem(int kind, bool x8) {
+    return 1024 + epilogue_warps(kind, x8) * kWarpStaging + 256;
+}
+__host__ __device__ constexpr int stages(int kind, bool x8, int bn) {
+    const int n = (kMaxSmem - 16 - fixed_smem(kind, x8)) / stage_bytes(kind, bn);
     return n > 8 ? 8 : n;
 }
-__host__ __device__ constexpr int smem_bytes(int kind, int bn) {
-    return kFixedSmem + stages(kind, bn) * stage_bytes(kind, bn);
+__host__ __device__ constexpr int smem_bytes(int kind, bool x8, int bn) {
+    return fixed_smem(kind, x8) + stages(kind, x8, bn) * stage_bytes(kind, bn);
 }
 
 struct MmaArgs {
@@ -200,56 +207,38 @@ __device__ __forceinline__ void load8_as(float (&v)[8], const void* p, int dtype
     else load8(v, static_cast<const __half*>(p) + at, vec, n);
 }
 
-// A warp's 32 x 32 tile in shared memory: float4 c of row r at slot c ^ (r & 7),
-// free of bank conflicts both a row per lane and 4 lanes a row.
+// Half a warp's 32 x 32 tile in shared memory, 16 columns: float4 c of row r at
+// slot c ^ ((r >> 1) & 3), free of bank conflicts both a row per lane and two
+// lanes a row.
 __device__ __forceinline__ float4* staged(float* s, int row, int c4) {
-    return reinterpret_cast<float4*>(s) + row * 8 + (c4 ^ (row & 7));
+    return reinterpret_cast<float4*>(s) + row * 4 + (c4 ^ ((row >> 1) & 3));
 }
 __device__ __forceinline__ float staged_at(const float* s, int row, int c) {
-    return s[row * 32 + (((c >> 2) ^ (row & 7)) << 2) + (c & 3)];
+    return s[row * 16 + (((c >> 2) ^ ((row >> 1) & 3)) << 2) + (c & 3)];
 }
 
-__device__ __forceinline__ void stage_rows(float* s, const float (&v)[32], int lane) {
+__device__ __forceinline__ void stage_rows(float* s, const float* v, int lane) {
     __syncwarp();
 #pragma unroll
-    for (int c = 0; c < 8; ++c) *staged(s, lane, c) = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+    for (int c = 0; c < 4; ++c) *staged(s, lane, c) = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
     __syncwarp();
 }
 
-// Stores columns [c0, c0 + w) of the staged rows to a tensor of w columns whose
-// rows all lie in this tile: one run of 32 w elements, lane by lane.
-__device__ __forceinline__ void store_run(const float* s, void* dst, int dtype, int64_t row0, int rows, int c0, int w,
-                                          const void* add, int lane) {
-    const unsigned inv = 65536u / (unsigned)w + 1;   // t / w for t < 1024, w <= 32
-    for (int t = lane; t < rows * w; t += 32) {
-        const int r = (int)((t * inv) >> 16), c = t - r * w;
-        float v = staged_at(s, r, c0 + c);
-        if (add) v += load_param(add, dtype, row0 * w + t);
-        store_param(dst, dtype, row0 * w + t, v);
-    }
-}
-
-// 32 x 32 of the residual as store_tile's lanes take them, loaded a piece
+// 32 x 32 of the residual as store_half's lanes take them, loaded a piece
 // ahead: a load waited for at each store would cost a trip to HBM four times a
-// piece (652 us against 2xx at 32768 x 1024 -> 4096, gelu, residual, kept z).
+// piece (652 us against 422 at 32768 x 1024 -> 4096, gelu, residual, kept z).
 struct Ahead {
-    uint4 r[8];   // 4 rows of 8 columns; 16-bit types use the first 4
+    uint4 r[4];   // 4 times 8 columns of a 16-bit type (float32 would take 32 registers: loaded at the store)
     bool have;
 };
 
 __device__ __forceinline__ void load_ahead(Ahead& a, const MmaArgs& p, int64_t row0, int64_t col0, int lane) {
-    a.have = p.residual && p.vec && col0 + 32 <= p.nj && row0 + 32 <= p.ni;
+    a.have = p.residual && p.out_dtype != PLATTICE_F32 && p.vec && col0 + 32 <= p.nj && row0 + 32 <= p.ni;
     if (!a.have) return;
 #pragma unroll
-    for (int it = 0; it < 4; ++it) {
-        const int64_t at = (row0 + it * 8 + (lane >> 2)) * p.nj + col0 + (lane & 3) * 8;
-        if (p.out_dtype == PLATTICE_F32) {
-            const uint4* src = reinterpret_cast<const uint4*>(static_cast<const float*>(p.residual) + at);
-            a.r[2 * it] = src[0];
-            a.r[2 * it + 1] = src[1];
-        } else {
-            a.r[it] = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.residual) + at);
-        }
+    for (int it = 0; it < 4; ++it) {   // half it / 2, rows 16 (it % 2)..
+        const int64_t at = (row0 + (it & 1) * 16 + (lane >> 1)) * p.nj + col0 + (it >> 1) * 16 + (lane & 1) * 8;
+        a.r[it] = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.residual) + at);
     }
 }
 
@@ -259,45 +248,35 @@ template <typename T> __device__ __forceinline__ void add_pairs(float (&v)[8], c
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float2 f = pair_f32(x.h[i]);
-        v[2 * i] += f.x;
-        v[2 * i + 1] += f.y;
+        add2(v[2 * i], v[2 * i + 1], f.x, f.y);
     }
 }
 
 __device__ __forceinline__ void add_ahead(float (&v)[8], const Ahead& a, int it, int dtype) {
-    if (dtype == PLATTICE_F32) {
-        const uint4 x = a.r[2 * it], y = a.r[2 * it + 1];
-        v[0] += __uint_as_float(x.x); v[1] += __uint_as_float(x.y);
-        v[2] += __uint_as_float(x.z); v[3] += __uint_as_float(x.w);
-        v[4] += __uint_as_float(y.x); v[5] += __uint_as_float(y.y);
-        v[6] += __uint_as_float(y.z); v[7] += __uint_as_float(y.w);
-    } else if (dtype == PLATTICE_BF16) {
+    if (dtype == PLATTICE_BF16) {
         add_pairs<__nv_bfloat16>(v, a.r[it]);
     } else {
         add_pairs<__half>(v, a.r[it]);
     }
 }
 
-// The staged 32 x 32 tile at (row0, col0) of an [ni][nj] tensor, `add` (the
-// residual, same layout) added: 4 lanes a row, 8 columns each.
-__device__ __forceinline__ void store_tile(const float* s, void* dst, const MmaArgs& p, int64_t row0, int64_t col0,
+// Half kHalf of a 32 x 32 tile at (row0, col0) of an [ni][nj] tensor, staged,
+// `add` (the residual, same layout) added: two lanes a row, 8 columns each.
+template <int kHalf>
+__device__ __forceinline__ void store_half(float* s, void* dst, const MmaArgs& p, int64_t row0, int64_t col0,
                                            const void* add, const Ahead& ahead, int lane) {
-    const int rows = (int)min((int64_t)32, p.ni - row0), left = (int)min((int64_t)32, p.nj - col0);
-    if (p.nj <= 32 && !(p.vec && left == 32)) {
-        store_run(s, dst, p.out_dtype, row0, rows, 0, left, add, lane);
-        return;
-    }
-    const int c = (lane & 3) * 8, n = left - c;
+    const int rows = (int)min((int64_t)32, p.ni - row0);
+    const int c = (lane & 1) * 8, n = (int)min((int64_t)32, p.nj - col0) - kHalf * 16 - c;
+    const bool vec = p.vec && n >= 8;
 #pragma unroll
-    for (int it = 0; it < 4; ++it) {
-        const int r = it * 8 + (lane >> 2);
+    for (int it = 0; it < 2; ++it) {
+        const int r = it * 16 + (lane >> 1);
         if (r >= rows || n <= 0) continue;
-        const bool vec = p.vec && n >= 8;
-        const int64_t at = (row0 + r) * p.nj + col0 + c;
-        const float4 a = *staged(const_cast<float*>(s), r, c >> 2), b = *staged(const_cast<float*>(s), r, (c >> 2) + 1);
+        const int64_t at = (row0 + r) * p.nj + col0 + kHalf * 16 + c;
+        const float4 a = *staged(s, r, c >> 2), b = *staged(s, r, (c >> 2) + 1);
         float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
         if (add && ahead.have) {
-            add_ahead(v, ahead, it, p.out_dtype);
+            add_ahead(v, ahead, kHalf * 2 + it, p.out_dtype);
         } else if (add) {
             float q[8];
             load8_as(q, add, p.out_dtype, at, vec, n);
@@ -308,26 +287,29 @@ __device__ __forceinline__ void store_tile(const float* s, void* dst, const MmaA
     }
 }
 
-// Two tensors of a split: columns below `split` and the others.
-__device__ __forceinline__ void store_split(const float* s, const MmaArgs& p, int64_t row0, int64_t col0, int lane) {
-    const int rows = (int)min((int64_t)32, p.ni - row0), left = (int)min((int64_t)32, p.nj - col0);
-    if (p.nj <= 32) {
-        store_run(s, p.y0, p.out_dtype, row0, rows, 0, p.split, nullptr, lane);
-        store_run(s, p.y1, p.out_dtype, row0, rows, p.split, (int)p.nj - p.split, nullptr, lane);
-        return;
-    }
-    const int64_t col = col0 + lane;
-    if (lane >= left) return;
-    for (int r = 0; r < rows; ++r) {
-        const float v = staged_at(s, r, lane);
-        if (col < p.split) store_param(p.y0, p.out_dtype, (row0 + r) * p.split + col, v);
-        else store_param(p.y1, p.out_dtype, (row0 + r) * (p.nj - p.split) + col - p.split, v);
-    }
+__device__ __forceinline__ void store_tile(float* s, const float (&v)[32], void* dst, const MmaArgs& p, int64_t row0,
+                                           int64_t col0, const void* add, const Ahead& ahead, int lane) {
+    stage_rows(s, v, lane);
+    store_half<0>(s, dst, p, row0, col0, add, ahead, lane);
+    stage_rows(s, v + 16, lane);
+    store_half<1>(s, dst, p, row0, col0, add, ahead, lane);
 }
 
-template <int kAct> __device__ __forceinline__ void apply32(float (&v)[32]) {
-#pragma unroll
-    for (int c = 0; c < 32; ++c) v[c] = act_value(v[c], kAct);
+// Two tensors of a split: columns below `split` and the others.
+__device__ __forceinline__ void store_split(float* s, const float (&v)[32], const MmaArgs& p, int64_t row0,
+                                            int64_t col0, int lane) {
+    const int rows = (int)min((int64_t)32, p.ni - row0), c = lane & 15;
+    for (int half = 0; half < 2; ++half) {
+        if (half) stage_rows(s, v + 16, lane);
+        else stage_rows(s, v, lane);
+        const int64_t col = col0 + half * 16 + c;
+        if (col >= p.nj) continue;
+        for (int r = lane >> 4; r < rows; r += 2) {
+            const float x = staged_at(s, r, c);
+            if (col < p.split) store_param(p.y0, p.out_dtype, (row0 + r) * p.split + col, x);
+            else store_param(p.y1, p.out_dtype, (row0 + r) * (p.nj - p.split) + col - p.split, x);
+        }
+    }
 }
 
 // 32 columns of 32 rows, a row per lane.
@@ -348,45 +330,40 @@ __device__ __forceinline__ void finish32(float (&v)[32], const MmaArgs& p, const
         return;
     }
     if (kKind == kForward) {
-        float* sb = s + 32 * 32;
+        float* sb = s + 32 * 16;
         if (p.bias) {
             sb[lane] = bias;
             __syncwarp();
 #pragma unroll
             for (int c = 0; c < 32; c += 4) {
                 const float4 b = *reinterpret_cast<const float4*>(sb + c);
-                v[c] += b.x; v[c + 1] += b.y; v[c + 2] += b.z; v[c + 3] += b.w;
+                add2(v[c], v[c + 1], b.x, b.y);
+                add2(v[c + 2], v[c + 3], b.z, b.w);
             }
         }
         if (p.z) {
             if (p.z_scale) {   // 32 columns are one block of the 8-bit rows
-                float u[32];   // v itself keeps its infinities for the activation
-#pragma unroll
-                for (int c = 0; c < 32; ++c) u[c] = v[c];
-                const int e = block_exponent(finite_amax(u));
+                bool infinite;
+                const int e = block_exponent(finite_amax_of(v, infinite));
                 if (row0 + lane < p.ni) {
                     const int64_t blocks = (p.nj + 31) / 32, at = (row0 + lane) * blocks + col0 / 32;
                     uint4* q = reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.z) + at * 32);
                     const float inv = pow2(-e);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const uint2 x = codes8(u + 16 * h, inv), y = codes8(u + 16 * h + 8, inv);
+                        const uint2 x = codes8_of(v + 16 * h, inv, infinite), y = codes8_of(v + 16 * h + 8, inv, infinite);
                         q[h] = make_uint4(x.x, x.y, y.x, y.y);
                     }
                     p.z_scale[at] = (uint8_t)(e + 127);
                 }
             } else {
-                stage_rows(s, v, lane);
-                store_tile(s, p.z, p, row0, col0, nullptr, ahead, lane);
+                store_tile(s, v, p.z, p, row0, col0, nullptr, ahead, lane);
             }
         }
-        if (p.act == PLATTICE_ACT_RELU) apply32<PLATTICE_ACT_RELU>(v);
-        else if (p.act == PLATTICE_ACT_GELU) apply32<PLATTICE_ACT_GELU>(v);
-        else if (p.act == PLATTICE_ACT_SILU) apply32<PLATTICE_ACT_SILU>(v);
+        activate(v, p.act);
     }
-    stage_rows(s, v, lane);
-    if (kKind == kForward && p.split) store_split(s, p, row0, col0, lane);
-    else store_tile(s, p.y0, p, row0, col0, kKind == kForward ? p.residual : nullptr, ahead, lane);
+    if (kKind == kForward && p.split) store_split(s, v, p, row0, col0, lane);
+    else store_tile(s, v, p.y0, p, row0, col0, kKind == kForward ? p.residual : nullptr, ahead, lane);
 }
 
 // ------------------------------------------------- widening an 8-bit operand
@@ -452,10 +429,11 @@ __device__ __forceinline__ void store_codes(uint32_t slice, const Codes& k, int 
 // -------------------------------------------------------------- the kernel
 
 template <int kKind, bool kX8, int kBN>
-__global__ void __launch_bounds__(kRoleThreads + (kX8 ? 32 * kConvertWarps : 0), 1)
+__global__ void __launch_bounds__(role_threads(kKind, kX8) + (kX8 ? 32 * kConvertWarps : 0), 1)
     k_mma(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const MmaArgs p,
           unsigned tiles) {
-    constexpr int kStages = stages(kKind, kBN);
+    constexpr int kStages = stages(kKind, kX8, kBN), kEpilogueWarps = epilogue_warps(kKind, kX8);
+    constexpr int kGroups = kEpilogueWarps / 4;   // warps that share 32 accumulator rows
     constexpr int kStage = stage_bytes(kKind, kBN);
     constexpr int kColumns = 2 * kBN;   // tensor memory: two accumulators
     extern __shared__ char smem_raw[];
@@ -577,8 +555,8 @@ __global__ void __launch_bounds__(kRoleThreads + (kX8 ? 32 * kConvertWarps : 0),
         }
     } else if (warp >= 4 && warp < 4 + kEpilogueWarps) {
         // ---- epilogue: warp w reads the 32 accumulator rows 32 (w % 4)..,
-        // the two warps of a quarter alternate over its 32-column pieces
-        const int quarter = warp & 3, half = (warp - 4) >> 2;
+        // the warps of a quarter take turns over its 32-column pieces
+        const int quarter = warp & 3, group = (warp - 4) >> 2;
         float* s = staging + (warp - 4) * (kWarpStaging / 4);
         int n = 0;
         for (unsigned t = blockIdx.x; t < tiles; t += gridDim.x, ++n) {
@@ -594,29 +572,29 @@ __global__ void __launch_bounds__(kRoleThreads + (kX8 ? 32 * kConvertWarps : 0),
                 if (p.bias && col0 + lane < p.nj) bias = load_param(p.bias, p.bias_dtype, col0 + lane);
                 else bias = 0.f;
             };
-            look_ahead(half);
+            look_ahead(group);
             if (!warp_wait(acc_full(buf), (n >> 1) & 1, dead)) break;
             fence_after();
             const uint32_t base = tmem + buf * kBN + ((uint32_t)(quarter * 32) << 16);
             constexpr int kPieces = kBN / 32;
 #pragma unroll 1
-            for (int c = half; c < kPieces; c += 2) {
+            for (int c = group; c < kPieces; c += kGroups) {
                 float v[32];
                 __syncwarp();
                 tmem_load32(v, base + c * 32);
-                if (c + 2 >= kPieces) {
+                if (c + kGroups >= kPieces) {
                     fence_before();
                     __syncwarp();
                     if (lane == 0) bar_arrive(acc_empty(buf));
                 }
                 finish32<kKind>(v, p, tile, row0, tile.j0 + c * 32, s, ahead, bias, lane);
-                if (c + 2 < kPieces) look_ahead(c + 2);
+                if (c + kGroups < kPieces) look_ahead(c + kGroups);
             }
-            if (half >= kPieces && lane == 0) bar_arrive(acc_empty(buf));
+            if (group >= kPieces && lane == 0) bar_arrive(acc_empty(buf));
         }
     } else if (kX8 && warp >= 4 + kEpilogueWarps) {
         // ---- widening 8-bit rows
-        const int thread = threadIdx.x - kRoleThreads;
+        const int thread = threadIdx.x - role_threads(kKind, kX8);
         constexpr bool kMN = a_mn(kKind);
         Codes ahead[kAhead];
         // cursor of the next slice to load

@@ -151,6 +151,18 @@ __global__ void __launch_bounds__(L > 256 ? L : 256) k_rms_norm(const NormArgs a
             gain[k][i] = col < a.c ? load_param(a.gain, a.gain_dtype, col) : 0.f;
         }
     const float inv_c = 1.f / (float)a.c;
+    Raw8<T> x[kChunks], r[kChunks];
+    auto load_row = [&](int64_t row) {
+#pragma unroll
+        for (int k = 0; k < kChunks; ++k) {
+            const int col = (k * L + lane) * 8;
+            const int left = row < a.rows ? a.c - col : 0;
+            const int64_t at = left > 0 ? row * a.c + col : 0;
+            x[k].load(static_cast<const T*>(a.x) + at, a.vec && left >= 8, left);
+            if (a.residual) r[k].load(static_cast<const T*>(a.residual) + at, a.vec && left >= 8, left);
+        }
+    };
+    load_row((int64_t)blockIdx.x * kRows + threadIdx.x / L);
     for (int64_t row0 = (int64_t)blockIdx.x * kRows; row0 < a.rows; row0 += (int64_t)gridDim.x * kRows) {
         const int64_t row = row0 + threadIdx.x / L;
         const bool live = row < a.rows;
@@ -158,17 +170,15 @@ __global__ void __launch_bounds__(L > 256 ? L : 256) k_rms_norm(const NormArgs a
         float ss = 0.f;
 #pragma unroll
         for (int k = 0; k < kChunks; ++k) {
-            const int col = (k * L + lane) * 8;
-            const int left = live ? a.c - col : 0;
-            const int64_t at = left > 0 ? row * a.c + col : 0;
-            load8(v[k], static_cast<const T*>(a.x) + at, a.vec && left >= 8, left);
+            x[k].widen(v[k]);
             if (a.residual) {
-                float r[8];
-                load8(r, static_cast<const T*>(a.residual) + at, a.vec && left >= 8, left);
+                float t[8];
+                r[k].widen(t);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[k][i] += r[i];
+                for (int i = 0; i < 8; ++i) v[k][i] += t[i];
             }
         }
+        load_row(row + (int64_t)gridDim.x * kRows);   // the next row's, while this one is worked on
 #pragma unroll
         for (int k = 0; k < kChunks; ++k)
 #pragma unroll
