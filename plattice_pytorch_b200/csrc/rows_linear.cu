@@ -7,151 +7,11 @@
 #include "rows_common.cuh"
 #include "rows_host.h"
 #include "rows_mma.cuh"
+#include "rows_narrow.cuh"
 
 namespace plr {
 
-// ------------------------------------------------------------------- operands
-
-// An operand of the products, seen as element (i, r): i along the result, r
-// along the sum.  One of the two strides is 1.  8-bit rows: `scale` non-null;
-// their pitch is a multiple of 32, so element e of the buffer has scale e / 32.
-struct View {
-    const void* p;
-    const uint8_t* scale;
-    int64_t si, sr;
-    int dtype;
-};
-
-__device__ __forceinline__ float view_at(const View& v, int64_t i, int64_t r) {
-    const int64_t e = i * v.si + r * v.sr;
-    if (v.scale) {
-        float t[4];
-        values4(t, static_cast<const uint8_t*>(v.p)[e], scale_of(v.scale[e >> 5]));
-        return t[0];
-    }
-    return load_param(v.p, v.dtype, e);
-}
-
-// ------------------------------------------------- product on the CUDA cores
-
-// out[z][i][j] = sum over r in part z of a(i, r) b(j, r), float32.
-constexpr int kTile = 64, kStep = 16;
-
-__global__ void __launch_bounds__(256) k_product(float* __restrict__ out, const View a, const View b, int64_t ni,
-                                                 int64_t nj, int64_t nr, int64_t part) {
-    __shared__ float sa[kStep][kTile + 4], sb[kStep][kTile + 4];
-    const int64_t i0 = (int64_t)blockIdx.x * kTile, j0 = (int64_t)blockIdx.y * kTile;
-    const int64_t r0 = (int64_t)blockIdx.z * part, r1 = min(nr, r0 + part);
-    const int ti = threadIdx.x & 15, tj = threadIdx.x >> 4;
-    float acc[4][4] = {};
-    for (int64_t rb = r0; rb < r1; rb += kStep) {
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int t = threadIdx.x + 256 * u;
-            // neighbouring threads along the contiguous direction
-            const int ia = a.sr == 1 ? t / kStep : t % kTile, ra = a.sr == 1 ? t % kStep : t / kTile;
-            const int jb = b.sr == 1 ? t / kStep : t % kTile, rr = b.sr == 1 ? t % kStep : t / kTile;
-            sa[ra][ia] = i0 + ia < ni && rb + ra < r1 ? view_at(a, i0 + ia, rb + ra) : 0.f;
-            sb[rr][jb] = j0 + jb < nj && rb + rr < r1 ? view_at(b, j0 + jb, rb + rr) : 0.f;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int r = 0; r < kStep; ++r) {
-            const float4 x = *reinterpret_cast<const float4*>(&sa[r][ti * 4]);
-            const float4 y = *reinterpret_cast<const float4*>(&sb[r][tj * 4]);
-            const float xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-            for (int m = 0; m < 4; ++m)
-#pragma unroll
-                for (int n = 0; n < 4; ++n) acc[m][n] = fmaf(xs[m], ys[n], acc[m][n]);
-        }
-        __syncthreads();
-    }
-    float* o = out + (int64_t)blockIdx.z * ni * nj;
-#pragma unroll
-    for (int m = 0; m < 4; ++m)
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-            const int64_t i = i0 + ti * 4 + m, j = j0 + tj * 4 + n;
-            if (i < ni && j < nj) o[i * nj + j] = acc[m][n];
-        }
-}
-
-// ------------------------------------------------------------------ epilogue
-
-struct FinishArgs {
-    const float* acc;   // [rows][n]
-    const void* bias;
-    int bias_dtype;
-    const void* residual;
-    void* y0;
-    void* y1;
-    void* z;
-    uint8_t* z_scale;
-    int64_t rows;
-    int n, split, act, out_dtype;
-};
-
-// A thread takes 8 columns of a row, 4 neighbouring lanes a block of 32 (the
-// blocks of the kept 8-bit pre-activation).
-template <typename T>
-__global__ void __launch_bounds__(256) k_finish(const FinishArgs a, unsigned groups) {
-    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t row = t / groups;
-    const int col = (int)(t - row * groups) * 8;
-    const int left = row < a.rows ? a.n - col : 0;
-    float z[8], y[8];
-    load8(z, a.acc + (left > 0 ? row * a.n + col : 0), false, left);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        if (a.bias && i < left) z[i] += load_param(a.bias, a.bias_dtype, col + i);
-        y[i] = z[i];
-    }
-    activate(y, a.act);
-    if (a.residual) {
-        float r[8];
-        load8(r, static_cast<const T*>(a.residual) + (left > 0 ? row * a.n + col : 0), false, left);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] += r[i];
-    }
-    if (a.z_scale) {
-        float amax = finite_amax(z);
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-        const int s = block_exponent(amax);
-        if (row < a.rows) {
-            reinterpret_cast<uint2*>(a.z)[t] = codes8(z, pow2(-s));
-            if ((threadIdx.x & 3) == 0) a.z_scale[t >> 2] = (uint8_t)(s + 127);
-        }
-    } else if (a.z) {
-        store8(static_cast<T*>(a.z) + (left > 0 ? row * a.n + col : 0), z, false, left);
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        if (i >= left) continue;
-        const int c = col + i;
-        if (c < a.split) static_cast<T*>(a.y0)[row * a.split + c] = from_f32<T>(y[i]);
-        else if (a.split) static_cast<T*>(a.y1)[row * (a.n - a.split) + c - a.split] = from_f32<T>(y[i]);
-        else static_cast<T*>(a.y0)[row * a.n + c] = from_f32<T>(y[i]);
-    }
-}
-
 // ----------------------------------------------------- operands for the MMAs
-
-// A float32 value as three bfloat16 whose sum it is: each takes the leading 8
-// significant bits of what is left (cut, not rounded, so that none overflows
-// and the remainders are exact).  What is not finite stays in the first part.
-__device__ __forceinline__ void split3(float v, __nv_bfloat16 (&o)[3]) {
-    const bool fine = fabsf(v) <= 3.402823466e38f;
-#pragma unroll
-    for (int i = 0; i < 3; ++i) {
-        // cutting a NaN's low bits could leave an infinity: round those
-        const __nv_bfloat16 h = fine ? __ushort_as_bfloat16((unsigned short)(__float_as_uint(v) >> 16))
-                                     : __float2bfloat16_rn(i == 0 ? v : 0.f);
-        o[i] = h;
-        v = fine ? v - __bfloat162float(h) : v;
-    }
-}
 
 __device__ __forceinline__ void store_parts(__nv_bfloat16* p, int64_t stride, const float (&v)[8], bool vec, int n) {
     union { uint4 u; __nv_bfloat16 h[8]; } o[3];
@@ -196,9 +56,8 @@ struct GradArgs {
     const void* g1;
     const void* z;
     const uint8_t* z_scale;
-    void* gz;           // [rows][pitch] in the operands' type; null: not stored
+    void* gz;           // [rows][pitch] in the operands' type, float32 as three bfloat16 parts; null: not stored
     int64_t pitch;
-    bool parts;         // float32: gz as three bfloat16 parts [3][rows][pitch]
     float* partial;     // [gridDim.y][n]; null: no bias gradient
     int64_t rows;
     int n, split, act;
@@ -214,21 +73,70 @@ __device__ __forceinline__ void times_slope(float (&g)[8], float (&z)[8]) {
     for (int i = 0; i < 8; i += 2) mul2(g[i], g[i + 1], z[i], z[i + 1]);
 }
 
+constexpr int kTogether = 2;
+
 // gz = grad_y act'(z), rounded to the operands' type for the two products (a
 // tensor core takes no wider operand; one rounding, as a stored gradient has),
 // and the sums of the unrounded gz over a CTA's rows.  2^shift threads of 8
 // columns share a row; gridDim.x strips of columns, gridDim.y parts of rows.
-template <typename TG, typename T>
-__global__ void __launch_bounds__(256, 4) k_grad_z(const GradArgs a) {
+template <typename TG, typename T, bool kFast>
+__global__ void __launch_bounds__(256, 3) k_grad_z(const GradArgs a) {
     __shared__ float sums[8 * 256];
     const int lane = threadIdx.x & ((1 << a.shift) - 1), rows = 256 >> a.shift;
     const int col = ((int)blockIdx.x << (a.shift + 3)) + lane * 8;
     const int left = a.n - col, wide = (int)min(a.pitch - col, (int64_t)8);
-    const bool vec = a.vec && left >= 8;
+    const int zgroups = (a.n + 31) / 32 * 4;
     float acc[8] = {};
-    if (left > 0) {
-        for (int64_t row = (int64_t)blockIdx.y * rows + (threadIdx.x >> a.shift); row < a.rows;
-             row += (int64_t)gridDim.y * rows) {
+    auto finish = [&](float (&g)[8], float (&z)[8], int64_t row) {
+        if (a.act == PLATTICE_ACT_RELU) times_slope<PLATTICE_ACT_RELU>(g, z);
+        else if (a.act == PLATTICE_ACT_GELU) times_slope<PLATTICE_ACT_GELU>(g, z);
+        else if (a.act == PLATTICE_ACT_SILU) times_slope<PLATTICE_ACT_SILU>(g, z);
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) add2(acc[i], acc[i + 1], g[i], g[i + 1]);
+        if (!a.gz) return;
+        const int64_t at = row * a.pitch + col;   // zeros up to the pitch
+        if constexpr (sizeof(T) == 4)
+            store_parts(static_cast<__nv_bfloat16*>(a.gz) + at, a.rows * a.pitch, g, kFast || wide == 8, wide);
+        else
+            store8(static_cast<T*>(a.gz) + at, g, kFast || (a.pitch % 8 == 0 && wide == 8), wide);
+    };
+    const int64_t stride = (int64_t)gridDim.y * rows;
+    int64_t row = (int64_t)blockIdx.y * rows + (threadIdx.x >> a.shift);
+    if (kFast) {
+        // whole groups of 8 on 16-byte boundaries, gradient in one tensor:
+        // kTogether rows' loads are issued before the first is used
+        if (left > 0) {
+            const TG* g0 = static_cast<const TG*>(a.g0) + col;
+            for (; row < a.rows; row += stride * kTogether) {
+                Raw8<TG> g[kTogether], z[kTogether];
+                uint2 codes[kTogether];
+                uint8_t scale[kTogether];
+#pragma unroll
+                for (int u = 0; u < kTogether; ++u) {
+                    const int64_t r = min(row + u * stride, a.rows - 1);
+                    g[u].load(g0 + r * a.n, true, 8);
+                    if (a.z_scale) {
+                        const int64_t at = r * zgroups + (col >> 3);
+                        codes[u] = reinterpret_cast<const uint2*>(a.z)[at];
+                        scale[u] = a.z_scale[at >> 2];
+                    } else if (a.z) {
+                        z[u].load(static_cast<const TG*>(a.z) + r * a.n + col, true, 8);
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < kTogether; ++u) {
+                    if (row + u * stride >= a.rows) break;
+                    float gv[8], zv[8];
+                    g[u].widen(gv);
+                    if (a.z_scale) values8(zv, codes[u], scale_of(scale[u]));
+                    else if (a.z) z[u].widen(zv);
+                    finish(gv, zv, row + u * stride);
+                }
+            }
+        }
+    } else if (left > 0) {
+        const bool vec = a.vec && left >= 8;
+        for (; row < a.rows; row += stride) {
             float g[8], z[8];
             if (a.split == 0) {
                 load8(g, static_cast<const TG*>(a.g0) + row * a.n + col, vec, left);
@@ -241,25 +149,13 @@ __global__ void __launch_bounds__(256, 4) k_grad_z(const GradArgs a) {
                                          : to_f32(static_cast<const TG*>(a.g1)[row * (a.n - a.split) + c - a.split]);
                 }
             }
-            if (a.act != PLATTICE_ACT_NONE) {
-                if (a.z_scale) {
-                    const int64_t at = row * (width8(a.n) / 8) + col / 8;
-                    values8(z, reinterpret_cast<const uint2*>(a.z)[at], scale_of(a.z_scale[at >> 2]));
-                } else {
-                    load8(z, static_cast<const TG*>(a.z) + row * a.n + col, vec, left);
-                }
-                if (a.act == PLATTICE_ACT_RELU) times_slope<PLATTICE_ACT_RELU>(g, z);
-                else if (a.act == PLATTICE_ACT_GELU) times_slope<PLATTICE_ACT_GELU>(g, z);
-                else times_slope<PLATTICE_ACT_SILU>(g, z);
+            if (a.z_scale) {
+                const int64_t at = row * zgroups + col / 8;
+                values8(z, reinterpret_cast<const uint2*>(a.z)[at], scale_of(a.z_scale[at >> 2]));
+            } else if (a.z) {
+                load8(z, static_cast<const TG*>(a.z) + row * a.n + col, vec, left);
             }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) acc[i] += g[i];
-            if (!a.gz) continue;
-            const int64_t at = row * a.pitch + col;   // zeros up to the pitch
-            if (sizeof(T) == 4 && a.parts)
-                store_parts(static_cast<__nv_bfloat16*>(a.gz) + at, a.rows * a.pitch, g, wide == 8, wide);
-            else
-                store8(static_cast<T*>(a.gz) + at, g, a.pitch % 8 == 0 && wide == 8, wide);
+            finish(g, z, row);
         }
     }
     if (!a.partial) return;
@@ -311,32 +207,6 @@ static bool linear_shape_ok(const plattice_linear_args* a) {
     // TMA coordinates and tile numbers are 32-bit
     if (a->rows > INT_MAX - 256 || a->k > (1 << 30) || a->n > (1 << 30)) return false;
     return fits(a->rows, width8(a->k)) && fits(a->rows, width8(a->n)) && fits(a->k, a->n);
-}
-
-// ---- products on the CUDA cores (float32 of few operations)
-
-static int64_t simt_tiles(int64_t n) { return ceil_div(n, kTile); }
-
-static View view_rows(const void* p, const uint8_t* scale, int64_t pitch, int dtype, bool along_rows) {
-    if (scale) pitch = width8(pitch);
-    return along_rows ? View{p, scale, 1, pitch, dtype} : View{p, scale, pitch, 1, dtype};
-}
-
-static cudaError_t product(float* out, const View& a, const View& b, int64_t ni, int64_t nj, int64_t nr, int parts,
-                           cudaStream_t s) {
-    if (simt_tiles(ni) > INT_MAX || simt_tiles(nj) > 65535) return cudaErrorInvalidValue;
-    const int64_t part = ceil_div(nr, parts);
-    k_product<<<dim3((unsigned)simt_tiles(ni), (unsigned)simt_tiles(nj), parts), 256, 0, s>>>(out, a, b, ni, nj, nr,
-                                                                                           part);
-    return cudaGetLastError();
-}
-
-// Parts of a sum over `len` terms whose result has `tiles` tiles: enough CTAs
-// for the device, none shorter than 512 terms.
-static int simt_parts(int64_t tiles, int64_t len) {
-    int64_t p = ceil_div(2 * (int64_t)sm_count(), tiles);
-    if (p > ceil_div(len, 512)) p = ceil_div(len, 512);
-    return (int)(p < 1 ? 1 : p > 512 ? 512 : p);
 }
 
 template <typename T>
@@ -519,12 +389,6 @@ static void x8_args(MmaArgs* p, const plattice_linear_args* a) {
     p->q_width = width8(a->k);
 }
 
-// Which products run on the tensor cores: all of 16-bit operands; float32 (six
-// products of bfloat16 parts, three with an 8-bit x) from an amount of work on.
-static bool on_tensor_cores(const plattice_linear_args* a) {
-    return a->dtype != PLATTICE_F32 || (double)a->rows * a->k * a->n >= 64.0 * 1024 * 1024;
-}
-
 // Whether an 8-bit x is unpacked to bfloat16 before the product rather than on
 // its way through it: when several tiles along j would each widen the same
 // slice (the widening and the MMA share the shared memory's bandwidth, so a
@@ -532,40 +396,51 @@ static bool on_tensor_cores(const plattice_linear_args* a) {
 // value, costs less.
 static bool unpack_first(int n, int bn) { return n > bn; }
 
+// How a forward runs: few rows a warp per output channel, few output channels
+// a warp per rows with the weights in shared memory, else the tiled product.
+// Measured at their borders: see k_few and k_narrow.
+enum Way { kWayFew, kWayNarrow, kWayTiles };
+
+constexpr int kFewRows = 8;
+
+static Way forward_way(const plattice_linear_args* a) {
+    const int parts = a->dtype == PLATTICE_F32 ? 3 : 1;
+    if (a->n <= 32 && narrow_fragments(a->k, (int)ceil_div(a->n, 8), parts) <= kNarrowMost) return kWayNarrow;
+    return a->rows <= kFewRows ? kWayFew : kWayTiles;
+}
+
 struct ForwardPlan {
-    bool mma, unpack;
+    Way way;
+    bool unpack;
     int bn;
-    int64_t x, w, acc, bytes;
+    int64_t x, w, bytes;
 };
 
 static ForwardPlan forward_plan(const plattice_linear_args* a) {
     ForwardPlan p{};
     Carve c;
-    p.mma = on_tensor_cores(a);
-    if (p.mma) {
+    p.way = forward_way(a);
+    if (p.way == kWayTiles) {
         p.bn = choose_bn(a->rows, a->n, 32);
         p.unpack = a->x_scale && unpack_first(a->n, p.bn);
         if (p.unpack) p.x = c.take(a->rows * up8(a->k) * 2);
         else if (!a->x_scale && !tma_ready(a->x, a->dtype, a->k)) p.x = c.take(repack_bytes(a->dtype, a->rows, a->k));
         p.w = tma_ready(a->w, a->dtype, a->k) ? 0 : c.take(repack_bytes(a->dtype, a->n, a->k));
-    } else {
-        p.acc = c.take(a->rows * a->n * 4);
     }
     p.bytes = c.at;
     return p;
 }
 
 struct BackwardPlan {
-    bool mma, gz_needed, unpack;
+    bool gz_needed, unpack;
     int shift, strips;
     int bn_x, bn_w, parts_b, parts_w;
-    int64_t gz, x, w, partial_b, partial_w, acc_x, pitch, bytes;
+    int64_t gz, x, w, partial_b, partial_w, pitch, bytes;
 };
 
 static BackwardPlan backward_plan(const plattice_linear_args* a) {
     BackwardPlan p{};
     Carve c;
-    p.mma = on_tensor_cores(a);
     while (p.shift < 5 && (8 << p.shift) < a->n) ++p.shift;   // a row's columns / 8, at most a warp
     p.strips = (int)ceil_div(a->n, 8 << p.shift);
     const int64_t need = ceil_div(a->rows, 256 >> p.shift), most = ceil_div(8 * (int64_t)sm_count(), p.strips);
@@ -573,49 +448,84 @@ static BackwardPlan backward_plan(const plattice_linear_args* a) {
     if (p.parts_b < 1) p.parts_b = 1;
     p.partial_b = c.take((int64_t)p.parts_b * a->n * 4);
     // the incoming gradient itself serves where it is already what TMA reads
-    p.gz_needed = !(p.mma && a->act == PLATTICE_ACT_NONE && !a->split && a->out_dtype == a->dtype &&
+    p.gz_needed = !(a->act == PLATTICE_ACT_NONE && !a->split && a->out_dtype == a->dtype &&
                     tma_ready(a->grad0, a->dtype, a->n));
-    if (p.mma) {
-        p.pitch = up8(a->n);
-        if (p.gz_needed) p.gz = c.take(repack_bytes(a->dtype, a->rows, a->n));
-        p.bn_x = choose_bn(a->rows, a->k, 64);
-        p.bn_w = a->n > 128 ? 256 : a->n > 64 ? 128 : a->n > 32 ? 64 : 32;
-        p.parts_w = choose_parts(a->k, a->n, p.bn_w, ceil_div(a->rows, kBK));
-        if (a->grad_x && !tma_ready(a->w, a->dtype, a->k)) p.w = c.take(repack_bytes(a->dtype, a->n, a->k));
-        p.unpack = a->x_scale && unpack_first(a->n, p.bn_w);
-        if (a->grad_w && p.unpack) p.x = c.take(a->rows * up8(a->k) * 2);
-        if (a->grad_w && !a->x_scale && !tma_ready(a->x, a->dtype, a->k))
-            p.x = c.take(repack_bytes(a->dtype, a->rows, a->k));
-        if (a->grad_w && p.parts_w > 1) p.partial_w = c.take((int64_t)p.parts_w * a->n * a->k * 4);
-    } else {
-        p.pitch = a->n;
-        p.gz = c.take(a->rows * p.pitch * (int64_t)dtype_size(a->dtype));
-        p.parts_w = simt_parts(simt_tiles(a->n) * simt_tiles(a->k), a->rows);
-        if (a->grad_w) p.partial_w = c.take((int64_t)p.parts_w * a->n * a->k * 4);
-        if (a->grad_x) p.acc_x = c.take(a->rows * a->k * 4);
-    }
+    p.pitch = up8(a->n);
+    if (p.gz_needed) p.gz = c.take(repack_bytes(a->dtype, a->rows, a->n));
+    p.bn_x = choose_bn(a->rows, a->k, 64);
+    p.bn_w = a->n > 128 ? 256 : a->n > 64 ? 128 : a->n > 32 ? 64 : 32;
+    p.parts_w = choose_parts(a->k, a->n, p.bn_w, ceil_div(a->rows, kBK));
+    if (a->grad_x && !tma_ready(a->w, a->dtype, a->k)) p.w = c.take(repack_bytes(a->dtype, a->n, a->k));
+    p.unpack = a->x_scale && unpack_first(a->n, p.bn_w);
+    if (a->grad_w && p.unpack) p.x = c.take(a->rows * up8(a->k) * 2);
+    if (a->grad_w && !a->x_scale && !tma_ready(a->x, a->dtype, a->k))
+        p.x = c.take(repack_bytes(a->dtype, a->rows, a->k));
+    if (a->grad_w && p.parts_w > 1) p.partial_w = c.take((int64_t)p.parts_w * a->n * a->k * 4);
     p.bytes = c.at;
     return p;
 }
 
 template <typename TG, typename T>
 static cudaError_t launch_grad_z(const GradArgs& g, const BackwardPlan& p, cudaStream_t s) {
-    k_grad_z<TG, T><<<dim3(p.strips, p.parts_b), 256, 0, s>>>(g);
+    if (g.vec && !g.split && g.pitch % 8 == 0) k_grad_z<TG, T, true><<<dim3(p.strips, p.parts_b), 256, 0, s>>>(g);
+    else k_grad_z<TG, T, false><<<dim3(p.strips, p.parts_b), 256, 0, s>>>(g);
     return cudaGetLastError();
 }
 
-static cudaError_t forward_simt(const plattice_linear_args* a, const ForwardPlan& p, cudaStream_t s) {
-    float* acc = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + p.acc);
-    const cudaError_t e = product(acc, view_rows(a->x, a->x_scale, a->k, a->dtype, false),
-                                  view_rows(a->w, nullptr, a->k, a->dtype, false), a->rows, a->n, a->k, 1, s);
+template <int kXT, int kNF, bool kW3, bool kSplit>
+static cudaError_t launch_narrow(const SmallArgs& a, int64_t blocks, cudaStream_t s) {
+    const int64_t smem = narrow_fragments(a.k, kNF, kW3 ? 3 : 1) + narrow_staging(NarrowShape<kXT>::kM);
+    int unused = 0;
+    const cudaError_t e = pl::kernel_once(
+        reinterpret_cast<const void*>(k_narrow<kXT, kNF, kW3, kSplit>),
+        [](int*) {
+            return cudaFuncSetAttribute(k_narrow<kXT, kNF, kW3, kSplit>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        (int)(kNarrowMost + narrow_staging(2)));
+        },
+        &unused);
     if (e != cudaSuccess) return e;
-    const FinishArgs f{acc, a->bias, a->bias_dtype, a->residual, a->y0, a->y1, a->z, a->z_scale, a->rows,
-                       a->n, a->split, a->act, a->out_dtype};
-    const unsigned groups = (unsigned)(width8(a->n) / 8);
-    const int64_t ctas = ceil_div(a->rows * groups, 256);
-    if (ctas > INT_MAX) return cudaErrorInvalidValue;
-    k_finish<float><<<(unsigned)ctas, 256, 0, s>>>(f, groups);
+    const int64_t need = kSplit ? blocks : ceil_div(blocks, kNarrowWarps), most = 4 * (int64_t)sm_count();
+    k_narrow<kXT, kNF, kW3, kSplit><<<(unsigned)(need < most ? need : most), 32 * kNarrowWarps, smem, s>>>(a);
     return cudaGetLastError();
+}
+
+template <int kXT, bool kW3>
+static cudaError_t run_narrow(const SmallArgs& a, cudaStream_t s) {
+    const int64_t blocks = ceil_div(a.rows, 16 * NarrowShape<kXT>::kM);
+    // fewer blocks of rows than a warp on each SM would take: the warps of a
+    // CTA share a block instead (at least two chunks of channels to share)
+    const bool split = blocks <= 2 * (int64_t)sm_count() && a.k > 64;
+    switch ((a.n + 7) / 8) {
+        case 1: return split ? launch_narrow<kXT, 1, kW3, true>(a, blocks, s) : launch_narrow<kXT, 1, kW3, false>(a, blocks, s);
+        case 2: return split ? launch_narrow<kXT, 2, kW3, true>(a, blocks, s) : launch_narrow<kXT, 2, kW3, false>(a, blocks, s);
+        case 3: return split ? launch_narrow<kXT, 3, kW3, true>(a, blocks, s) : launch_narrow<kXT, 3, kW3, false>(a, blocks, s);
+        default: return split ? launch_narrow<kXT, 4, kW3, true>(a, blocks, s) : launch_narrow<kXT, 4, kW3, false>(a, blocks, s);
+    }
+}
+
+template <typename TW>
+static cudaError_t run_few(const SmallArgs& a, cudaStream_t s) {
+    const unsigned ctas = (unsigned)ceil_div(a.n, 32);
+    if (a.rows == 1) k_few<TW, 1><<<ctas, 32 * kFewWarps, 0, s>>>(a);
+    else if (a.rows == 2) k_few<TW, 2><<<ctas, 32 * kFewWarps, 0, s>>>(a);
+    else if (a.rows <= 4) k_few<TW, 4><<<ctas, 32 * kFewWarps, 0, s>>>(a);
+    else k_few<TW, 8><<<ctas, 32 * kFewWarps, 0, s>>>(a);
+    return cudaGetLastError();
+}
+
+static cudaError_t forward_small(const plattice_linear_args* a, Way way, cudaStream_t s) {
+    const int e = a->dtype == PLATTICE_F32 ? 4 : 8;   // elements of 16 bytes
+    const SmallArgs p{a->x, a->x_scale, a->w, a->bias, a->residual, a->y0, a->y1, a->z, a->z_scale, a->rows,
+                      a->k, a->n, a->split, a->act, a->dtype, a->out_dtype, a->bias_dtype,
+                      a->k % e == 0 && aligned16(a->x), a->k % 8 == 0 && aligned16(a->w)};
+    if (way == kWayFew)
+        return a->dtype == PLATTICE_F32    ? run_few<float>(p, s)
+               : a->dtype == PLATTICE_BF16 ? run_few<__nv_bfloat16>(p, s)
+                                           : run_few<__half>(p, s);
+    if (a->x_scale) return a->dtype == PLATTICE_F32 ? run_narrow<kX8, true>(p, s) : run_narrow<kX8, false>(p, s);
+    return a->dtype == PLATTICE_F32    ? run_narrow<kXFloat, true>(p, s)
+           : a->dtype == PLATTICE_BF16 ? run_narrow<kXBf16, false>(p, s)
+                                       : run_narrow<kXHalf, false>(p, s);
 }
 
 static cudaError_t forward_mma(const plattice_linear_args* a, const ForwardPlan& p, cudaStream_t s) {
@@ -651,12 +561,13 @@ static cudaError_t forward_mma(const plattice_linear_args* a, const ForwardPlan&
 
 static cudaError_t grad_z(const plattice_linear_args* a, const BackwardPlan& p, cudaStream_t s) {
     char* ws = static_cast<char*>(a->workspace);
+    const bool slope = a->act != PLATTICE_ACT_NONE;
     const bool store = p.gz_needed && (a->grad_x || a->grad_w);
     if (!store && !a->grad_bias) return cudaSuccess;
-    const GradArgs g{a->grad0, a->grad1, a->z, a->z_scale, store ? ws + p.gz : nullptr, p.pitch, p.mma,
+    const GradArgs g{a->grad0, a->grad1, slope ? a->z : nullptr, slope ? a->z_scale : nullptr, store ? ws + p.gz : nullptr, p.pitch,
                      a->grad_bias ? reinterpret_cast<float*>(ws + p.partial_b) : nullptr, a->rows, a->n, a->split,
                      a->act, p.shift,
-                     a->n % 8 == 0 && aligned16(a->grad0) && (!a->z || a->z_scale || aligned16(a->z))};
+                     a->n % 8 == 0 && aligned16(a->grad0) && (!slope || a->z_scale || aligned16(a->z))};
     cudaError_t e;
     if (a->out_dtype == PLATTICE_F32)
         e = a->dtype == PLATTICE_F32    ? launch_grad_z<float, float>(g, p, s)
@@ -666,24 +577,6 @@ static cudaError_t grad_z(const plattice_linear_args* a, const BackwardPlan& p, 
         e = a->dtype == PLATTICE_BF16 ? launch_grad_z<__nv_bfloat16, __nv_bfloat16>(g, p, s)
                                       : launch_grad_z<__half, __half>(g, p, s);
     if (e == cudaSuccess && a->grad_bias) e = column_sums(a->grad_bias, a->bias_dtype, g.partial, p.parts_b, a->n, s);
-    return e;
-}
-
-static cudaError_t backward_simt(const plattice_linear_args* a, const BackwardPlan& p, cudaStream_t s) {
-    char* ws = static_cast<char*>(a->workspace);
-    cudaError_t e = cudaSuccess;
-    if (a->grad_x) {
-        float* acc = reinterpret_cast<float*>(ws + p.acc_x);
-        e = product(acc, view_rows(ws + p.gz, nullptr, p.pitch, a->dtype, false),
-                    view_rows(a->w, nullptr, a->k, a->dtype, true), a->rows, a->k, a->n, 1, s);
-        if (e == cudaSuccess) e = add_parts_to(a->grad_x, a->dtype, acc, 1, a->rows * a->k, s);
-    }
-    if (e == cudaSuccess && a->grad_w) {
-        float* part = reinterpret_cast<float*>(ws + p.partial_w);
-        e = product(part, view_rows(ws + p.gz, nullptr, p.pitch, a->dtype, true),
-                    view_rows(a->x, a->x_scale, a->k, a->dtype, true), a->n, a->k, a->rows, p.parts_w, s);
-        if (e == cudaSuccess) e = add_parts_to(a->grad_w, a->dtype, part, p.parts_w, (int64_t)a->n * a->k, s);
-    }
     return e;
 }
 
@@ -749,12 +642,14 @@ int plattice_linear(const plattice_linear_args* a, void* stream) {
     if (a->rows == 0) return PLATTICE_OK;
     if (!a->x || !a->w || !a->y0 || (a->split && !a->y1) || (a->z_scale && !a->z)) return PLATTICE_ERR_INVALID;
     if (a->split && a->residual) return PLATTICE_ERR_INVALID;
+    if (a->z_scale && ((uintptr_t)a->z & 31)) return PLATTICE_ERR_INVALID;   // codes leave 32 bytes at a time
+    if (a->x_scale && !aligned16(a->x)) return PLATTICE_ERR_INVALID;
     const ForwardPlan p = forward_plan(a);
     if (p.bytes && (!a->workspace || a->workspace_bytes < (size_t)p.bytes)) return PLATTICE_ERR_WORKSPACE;
     const int rc = rows_poll("plattice_linear");
     if (rc != PLATTICE_OK) return rc;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return rows_status(p.mma ? forward_mma(a, p, s) : forward_simt(a, p, s), "plattice_linear");
+    return rows_status(p.way == kWayTiles ? forward_mma(a, p, s) : forward_small(a, p.way, s), "plattice_linear");
 }
 
 int plattice_linear_backward_workspace_size(const plattice_linear_args* a, size_t* bytes) {
@@ -776,12 +671,13 @@ int plattice_linear_backward(const plattice_linear_args* a, void* stream) {
     if (!a->grad0 || (a->split && !a->grad1) || (a->grad_x && !a->w) || (a->grad_w && !a->x) ||
         (a->act != PLATTICE_ACT_NONE && !a->z))
         return PLATTICE_ERR_INVALID;
+    if (a->x_scale && !aligned16(a->x)) return PLATTICE_ERR_INVALID;
     const BackwardPlan p = backward_plan(a);
     if (!a->workspace || a->workspace_bytes < (size_t)p.bytes) return PLATTICE_ERR_WORKSPACE;
     const int rc = rows_poll("plattice_linear_backward");
     if (rc != PLATTICE_OK) return rc;
     e = grad_z(a, p, s);
-    if (e == cudaSuccess) e = p.mma ? backward_mma(a, p, s) : backward_simt(a, p, s);
+    if (e == cudaSuccess) e = backward_mma(a, p, s);
     return rows_status(e, "plattice_linear_backward");
 }
 

@@ -148,21 +148,18 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-__device__ __forceinline__ void tmem_load32(float (&v)[32], uint32_t addr) {
-    uint32_t r[32];
+__device__ __forceinline__ void tmem_load16(float (&v)[16], uint32_t addr) {
+    uint32_t r[16];
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(addr)
         : "memory");
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
 // Shared-memory operand descriptor of a slice in the 128-byte swizzle: 8-row
@@ -260,110 +257,106 @@ __device__ __forceinline__ void add_ahead(float (&v)[8], const Ahead& a, int it,
     }
 }
 
-// Half kHalf of a 32 x 32 tile at (row0, col0) of an [ni][nj] tensor, staged,
-// `add` (the residual, same layout) added: two lanes a row, 8 columns each.
+// 16 columns of 32 rows (a row per lane) to (row0, col0) of an [ni][nj] tensor,
+// `add` (the residual, same layout) added: through the staging to two lanes a
+// row, 8 columns each.
 template <int kHalf>
-__device__ __forceinline__ void store_half(float* s, void* dst, const MmaArgs& p, int64_t row0, int64_t col0,
-                                           const void* add, const Ahead& ahead, int lane) {
+__device__ __forceinline__ void store_half(float* s, const float (&v)[16], void* dst, const MmaArgs& p, int64_t row0,
+                                           int64_t col0, const void* add, const Ahead& ahead, int lane) {
+    stage_rows(s, v, lane);
     const int rows = (int)min((int64_t)32, p.ni - row0);
-    const int c = (lane & 1) * 8, n = (int)min((int64_t)32, p.nj - col0) - kHalf * 16 - c;
+    const int c = (lane & 1) * 8, n = (int)min((int64_t)16, p.nj - col0) - c;
     const bool vec = p.vec && n >= 8;
 #pragma unroll
     for (int it = 0; it < 2; ++it) {
         const int r = it * 16 + (lane >> 1);
         if (r >= rows || n <= 0) continue;
-        const int64_t at = (row0 + r) * p.nj + col0 + kHalf * 16 + c;
+        const int64_t at = (row0 + r) * p.nj + col0 + c;
         const float4 a = *staged(s, r, c >> 2), b = *staged(s, r, (c >> 2) + 1);
-        float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        float o[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
         if (add && ahead.have) {
-            add_ahead(v, ahead, kHalf * 2 + it, p.out_dtype);
+            add_ahead(o, ahead, kHalf * 2 + it, p.out_dtype);
         } else if (add) {
             float q[8];
             load8_as(q, add, p.out_dtype, at, vec, n);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] += q[i];
+            for (int i = 0; i < 8; ++i) o[i] += q[i];
         }
-        store8_as(dst, p.out_dtype, at, v, vec, n);
+        store8_as(dst, p.out_dtype, at, o, vec, n);
     }
-}
-
-__device__ __forceinline__ void store_tile(float* s, const float (&v)[32], void* dst, const MmaArgs& p, int64_t row0,
-                                           int64_t col0, const void* add, const Ahead& ahead, int lane) {
-    stage_rows(s, v, lane);
-    store_half<0>(s, dst, p, row0, col0, add, ahead, lane);
-    stage_rows(s, v + 16, lane);
-    store_half<1>(s, dst, p, row0, col0, add, ahead, lane);
 }
 
 // Two tensors of a split: columns below `split` and the others.
-__device__ __forceinline__ void store_split(float* s, const float (&v)[32], const MmaArgs& p, int64_t row0,
+__device__ __forceinline__ void store_split(float* s, const float (&v)[16], const MmaArgs& p, int64_t row0,
                                             int64_t col0, int lane) {
+    stage_rows(s, v, lane);
     const int rows = (int)min((int64_t)32, p.ni - row0), c = lane & 15;
-    for (int half = 0; half < 2; ++half) {
-        if (half) stage_rows(s, v + 16, lane);
-        else stage_rows(s, v, lane);
-        const int64_t col = col0 + half * 16 + c;
-        if (col >= p.nj) continue;
-        for (int r = lane >> 4; r < rows; r += 2) {
-            const float x = staged_at(s, r, c);
-            if (col < p.split) store_param(p.y0, p.out_dtype, (row0 + r) * p.split + col, x);
-            else store_param(p.y1, p.out_dtype, (row0 + r) * (p.nj - p.split) + col - p.split, x);
-        }
+    const int64_t col = col0 + c;
+    if (col >= p.nj) return;
+    for (int r = lane >> 4; r < rows; r += 2) {
+        const float x = staged_at(s, r, c);
+        if (col < p.split) store_param(p.y0, p.out_dtype, (row0 + r) * p.split + col, x);
+        else store_param(p.y1, p.out_dtype, (row0 + r) * (p.nj - p.split) + col - p.split, x);
     }
 }
 
-// 32 columns of 32 rows, a row per lane.
-template <int kKind>
-__device__ __forceinline__ void finish32(float (&v)[32], const MmaArgs& p, const Tile& t, int64_t row0, int64_t col0,
-                                         float* s, const Ahead& ahead, float bias, int lane) {
-    if (col0 >= p.nj || row0 >= p.ni) return;
+__device__ __forceinline__ void add_bias(float (&v)[16], const float* sb) {
+#pragma unroll
+    for (int c = 0; c < 16; c += 4) {
+        const float4 b = *reinterpret_cast<const float4*>(sb + c);
+        add2(v[c], v[c + 1], b.x, b.y);
+        add2(v[c + 2], v[c + 3], b.z, b.w);
+    }
+}
+
+// Scale of the kept 8-bit rows: 32 columns are one block.
+struct Block8 {
+    int exponent;
+    bool infinite;
+    uint4 first;   // codes of the first half, stored together with the second's
+};
+
+// Half kHalf (16 columns from col0) of a 32-column piece, a row per lane.
+template <int kKind, int kHalf>
+__device__ __forceinline__ void finish16(float (&v)[16], const MmaArgs& p, const Tile& t, int64_t row0, int64_t col0,
+                                         float* s, const Ahead& ahead, Block8& block, int lane) {
     if (kKind == kGradW) {
         // D is [input channel][output channel], its result [output channel]
         // [input channel]: a lane per input channel stores whole lines
         const int64_t i = row0 + lane;
         if (i >= p.ni) return;
-        const int left = (int)min((int64_t)32, p.nj - col0);
+        const int left = (int)min((int64_t)16, p.nj - col0);
         const int64_t at = ((int64_t)t.part * p.nj + col0) * p.ni + i;
 #pragma unroll
-        for (int c = 0; c < 32; ++c)
+        for (int c = 0; c < 16; ++c)
             if (c < left) store_param(p.y0, p.out_dtype, at + (int64_t)c * p.ni, v[c]);
         return;
     }
-    if (kKind == kForward) {
-        float* sb = s + 32 * 16;
-        if (p.bias) {
-            sb[lane] = bias;
-            __syncwarp();
-#pragma unroll
-            for (int c = 0; c < 32; c += 4) {
-                const float4 b = *reinterpret_cast<const float4*>(sb + c);
-                add2(v[c], v[c + 1], b.x, b.y);
-                add2(v[c + 2], v[c + 3], b.z, b.w);
-            }
-        }
-        if (p.z) {
-            if (p.z_scale) {   // 32 columns are one block of the 8-bit rows
-                bool infinite;
-                const int e = block_exponent(finite_amax_of(v, infinite));
-                if (row0 + lane < p.ni) {
-                    const int64_t blocks = (p.nj + 31) / 32, at = (row0 + lane) * blocks + col0 / 32;
-                    uint4* q = reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.z) + at * 32);
-                    const float inv = pow2(-e);
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const uint2 x = codes8_of(v + 16 * h, inv, infinite), y = codes8_of(v + 16 * h + 8, inv, infinite);
-                        q[h] = make_uint4(x.x, x.y, y.x, y.y);
-                    }
-                    p.z_scale[at] = (uint8_t)(e + 127);
-                }
-            } else {
-                store_tile(s, v, p.z, p, row0, col0, nullptr, ahead, lane);
-            }
-        }
-        activate(v, p.act);
+    if (kKind == kGradX) {
+        store_half<kHalf>(s, v, p.y0, p, row0, col0, nullptr, ahead, lane);
+        return;
     }
-    if (kKind == kForward && p.split) store_split(s, v, p, row0, col0, lane);
-    else store_tile(s, v, p.y0, p, row0, col0, kKind == kForward ? p.residual : nullptr, ahead, lane);
+    if (p.bias) add_bias(v, s + 32 * 16 + kHalf * 16);
+    if (p.z_scale) {
+        const float inv = pow2(-block.exponent);
+        const uint2 x = codes8_of(v, inv, block.infinite), y = codes8_of(v + 8, inv, block.infinite);
+        if (kHalf == 0) {
+            block.first = make_uint4(x.x, x.y, y.x, y.y);
+        } else if (row0 + lane < p.ni) {   // a lane's 32 bytes in one store: whole sectors
+            const int64_t at = (row0 + lane) * ((p.nj + 31) / 32) + (col0 >> 5);
+            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(static_cast<uint8_t*>(p.z) + at * 32),
+                         "r"(block.first.x), "r"(block.first.y), "r"(block.first.z), "r"(block.first.w), "r"(x.x),
+                         "r"(x.y), "r"(y.x), "r"(y.y)
+                         : "memory");
+            p.z_scale[at] = (uint8_t)(block.exponent + 127);
+        }
+    } else if (p.z) {
+        if (col0 < p.nj) store_half<kHalf>(s, v, p.z, p, row0, col0, nullptr, ahead, lane);
+    }
+    if (col0 >= p.nj) return;
+    activate(v, p.act);
+    if (p.split) store_split(s, v, p, row0, col0, lane);
+    else store_half<kHalf>(s, v, p.y0, p, row0, col0, p.residual, ahead, lane);
 }
 
 // ------------------------------------------------- widening an 8-bit operand
@@ -579,15 +572,37 @@ __global__ void __launch_bounds__(role_threads(kKind, kX8) + (kX8 ? 32 * kConver
             constexpr int kPieces = kBN / 32;
 #pragma unroll 1
             for (int c = group; c < kPieces; c += kGroups) {
-                float v[32];
+                const int64_t col0 = tile.j0 + c * 32;
+                const bool live = col0 < p.nj && row0 < p.ni;
+                float v[16];
+                Block8 block{0, false, {}};
                 __syncwarp();
-                tmem_load32(v, base + c * 32);
+                if (kKind == kForward && live && p.bias) {
+                    s[32 * 16 + lane] = bias;
+                    __syncwarp();
+                }
+                if (kKind == kForward && live && p.z_scale) {
+                    float amax = 0.f;   // of both halves, which are read again below
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        tmem_load16(v, base + c * 32 + h * 16);
+                        if (p.bias) add_bias(v, s + 32 * 16 + h * 16);
+                        bool infinite;
+                        amax = fmaxf(amax, finite_amax_of(v, infinite));
+                        block.infinite |= infinite;
+                    }
+                    block.exponent = block_exponent(amax);
+                }
+                tmem_load16(v, base + c * 32);
+                if (live) finish16<kKind, 0>(v, p, tile, row0, col0, s, ahead, block, lane);
+                __syncwarp();
+                tmem_load16(v, base + c * 32 + 16);
                 if (c + kGroups >= kPieces) {
                     fence_before();
                     __syncwarp();
                     if (lane == 0) bar_arrive(acc_empty(buf));
                 }
-                finish32<kKind>(v, p, tile, row0, tile.j0 + c * 32, s, ahead, bias, lane);
+                if (live) finish16<kKind, 1>(v, p, tile, row0, col0 + 16, s, ahead, block, lane);
                 if (c + kGroups < kPieces) look_ahead(c + kGroups);
             }
             if (group >= kPieces && lane == 0) bar_arrive(acc_empty(buf));
