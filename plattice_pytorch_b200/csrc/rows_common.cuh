@@ -260,6 +260,10 @@ __device__ __forceinline__ void values4(float* v, unsigned codes, float scale) {
     v[0] = fa.x * scale; v[1] = fa.y * scale; v[2] = fb.x * scale; v[3] = fb.y * scale;
 }
 
+__device__ __forceinline__ float value1(uint8_t code, float scale) {
+    return __half2float(__half(__nv_cvt_fp8_to_halfraw(code, __NV_E4M3))) * scale;
+}
+
 __device__ __forceinline__ void values8(float (&v)[8], uint2 codes, float scale) {
     values4(v, codes.x, scale);
     values4(v + 4, codes.y, scale);

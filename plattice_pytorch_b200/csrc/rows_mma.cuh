@@ -221,22 +221,21 @@ __device__ __forceinline__ void stage_rows(float* s, const float* v, int lane) {
     __syncwarp();
 }
 
-// 32 x 32 of the residual as store_half's lanes take them, loaded a piece
-// ahead: a load waited for at each store would cost a trip to HBM four times a
-// piece (652 us against 422 at 32768 x 1024 -> 4096, gelu, residual, kept z).
+// 32 x 16 of the residual as store_half's lanes take them, loaded a half piece
+// ahead: a load waited for at each store would cost a trip to HBM twice a half
+// (652 us against 422 at 32768 x 1024 -> 4096, gelu, residual, kept z).
 struct Ahead {
-    uint4 r[4];   // 4 times 8 columns of a 16-bit type (float32 would take 32 registers: loaded at the store)
+    uint4 r[2];   // twice 8 columns of a 16-bit type (float32 is loaded at the store)
     bool have;
 };
 
 __device__ __forceinline__ void load_ahead(Ahead& a, const MmaArgs& p, int64_t row0, int64_t col0, int lane) {
-    a.have = p.residual && p.out_dtype != PLATTICE_F32 && p.vec && col0 + 32 <= p.nj && row0 + 32 <= p.ni;
+    a.have = p.residual && p.out_dtype != PLATTICE_F32 && p.vec && col0 + 16 <= p.nj && row0 + 32 <= p.ni;
     if (!a.have) return;
 #pragma unroll
-    for (int it = 0; it < 4; ++it) {   // half it / 2, rows 16 (it % 2)..
-        const int64_t at = (row0 + (it & 1) * 16 + (lane >> 1)) * p.nj + col0 + (it >> 1) * 16 + (lane & 1) * 8;
-        a.r[it] = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.residual) + at);
-    }
+    for (int it = 0; it < 2; ++it)
+        a.r[it] = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.residual) +
+                                                  (row0 + it * 16 + (lane >> 1)) * p.nj + col0 + (lane & 1) * 8);
 }
 
 template <typename T> __device__ __forceinline__ void add_pairs(float (&v)[8], const uint4& r) {
@@ -260,13 +259,28 @@ __device__ __forceinline__ void add_ahead(float (&v)[8], const Ahead& a, int it,
 // 16 columns of 32 rows (a row per lane) to (row0, col0) of an [ni][nj] tensor,
 // `add` (the residual, same layout) added: through the staging to two lanes a
 // row, 8 columns each.
-template <int kHalf>
 __device__ __forceinline__ void store_half(float* s, const float (&v)[16], void* dst, const MmaArgs& p, int64_t row0,
                                            int64_t col0, const void* add, const Ahead& ahead, int lane) {
     stage_rows(s, v, lane);
     const int rows = (int)min((int64_t)32, p.ni - row0);
+    if (!p.vec) {   // rows on no 16-byte boundaries: a lane per column, two rows at a time
+        const int64_t col = col0 + (lane & 15);
+        if (col >= p.nj) return;
+        float x[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {   // all of the residual's loads before the first store
+            const int r = (lane >> 4) + 2 * i;
+            x[i] = add && r < rows ? load_param(add, p.out_dtype, (row0 + r) * p.nj + col) : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int r = (lane >> 4) + 2 * i;
+            if (r < rows) store_param(dst, p.out_dtype, (row0 + r) * p.nj + col, x[i] + staged_at(s, r, lane & 15));
+        }
+        return;
+    }
     const int c = (lane & 1) * 8, n = (int)min((int64_t)16, p.nj - col0) - c;
-    const bool vec = p.vec && n >= 8;
+    const bool vec = n >= 8;
 #pragma unroll
     for (int it = 0; it < 2; ++it) {
         const int r = it * 16 + (lane >> 1);
@@ -275,7 +289,7 @@ __device__ __forceinline__ void store_half(float* s, const float (&v)[16], void*
         const float4 a = *staged(s, r, c >> 2), b = *staged(s, r, (c >> 2) + 1);
         float o[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
         if (add && ahead.have) {
-            add_ahead(o, ahead, kHalf * 2 + it, p.out_dtype);
+            add_ahead(o, ahead, it, p.out_dtype);
         } else if (add) {
             float q[8];
             load8_as(q, add, p.out_dtype, at, vec, n);
@@ -316,10 +330,10 @@ struct Block8 {
     uint4 first;   // codes of the first half, stored together with the second's
 };
 
-// Half kHalf (16 columns from col0) of a 32-column piece, a row per lane.
-template <int kKind, int kHalf>
+// Half a 32-column piece (16 columns from col0), a row per lane.
+template <int kKind>
 __device__ __forceinline__ void finish16(float (&v)[16], const MmaArgs& p, const Tile& t, int64_t row0, int64_t col0,
-                                         float* s, const Ahead& ahead, Block8& block, int lane) {
+                                         float* s, Ahead& ahead, Block8& block, int half, int lane) {
     if (kKind == kGradW) {
         // D is [input channel][output channel], its result [output channel]
         // [input channel]: a lane per input channel stores whole lines
@@ -333,14 +347,14 @@ __device__ __forceinline__ void finish16(float (&v)[16], const MmaArgs& p, const
         return;
     }
     if (kKind == kGradX) {
-        store_half<kHalf>(s, v, p.y0, p, row0, col0, nullptr, ahead, lane);
+        store_half(s, v, p.y0, p, row0, col0, nullptr, ahead, lane);
         return;
     }
-    if (p.bias) add_bias(v, s + 32 * 16 + kHalf * 16);
+    if (p.bias) add_bias(v, s + 32 * 16 + half * 16);
     if (p.z_scale) {
         const float inv = pow2(-block.exponent);
         const uint2 x = codes8_of(v, inv, block.infinite), y = codes8_of(v + 8, inv, block.infinite);
-        if (kHalf == 0) {
+        if (half == 0) {
             block.first = make_uint4(x.x, x.y, y.x, y.y);
         } else if (row0 + lane < p.ni) {   // a lane's 32 bytes in one store: whole sectors
             const int64_t at = (row0 + lane) * ((p.nj + 31) / 32) + (col0 >> 5);
@@ -351,12 +365,12 @@ __device__ __forceinline__ void finish16(float (&v)[16], const MmaArgs& p, const
             p.z_scale[at] = (uint8_t)(block.exponent + 127);
         }
     } else if (p.z) {
-        if (col0 < p.nj) store_half<kHalf>(s, v, p.z, p, row0, col0, nullptr, ahead, lane);
+        if (col0 < p.nj) store_half(s, v, p.z, p, row0, col0, nullptr, ahead, lane);
     }
     if (col0 >= p.nj) return;
     activate(v, p.act);
     if (p.split) store_split(s, v, p, row0, col0, lane);
-    else store_half<kHalf>(s, v, p.y0, p, row0, col0, p.residual, ahead, lane);
+    else store_half(s, v, p.y0, p, row0, col0, p.residual, ahead, lane);
 }
 
 // ------------------------------------------------- widening an 8-bit operand
@@ -554,22 +568,21 @@ __global__ void __launch_bounds__(role_threads(kKind, kX8) + (kX8 ? 32 * kConver
         int n = 0;
         for (unsigned t = blockIdx.x; t < tiles; t += gridDim.x, ++n) {
             const Tile tile = tile_at<kBN>(p, t);
+            constexpr int kPieces = kBN / 32;
             const int buf = n & 1;
             const int64_t row0 = tile.i0 + quarter * 32;
             Ahead ahead;
             float bias = 0.f;
-            auto look_ahead = [&](int c) {
-                const int64_t col0 = tile.j0 + c * 32;
-                if (kKind != kForward) return;
-                load_ahead(ahead, p, row0, col0, lane);
-                if (p.bias && col0 + lane < p.nj) bias = load_param(p.bias, p.bias_dtype, col0 + lane);
-                else bias = 0.f;
+            auto bias_ahead = [&](int c) {
+                const int64_t col = tile.j0 + c * 32 + lane;
+                bias = kKind == kForward && p.bias && c < kPieces && col < p.nj ? load_param(p.bias, p.bias_dtype, col) : 0.f;
             };
-            look_ahead(group);
+            ahead.have = false;
+            bias_ahead(group);
+            if (kKind == kForward && group < kPieces) load_ahead(ahead, p, row0, tile.j0 + group * 32, lane);
             if (!warp_wait(acc_full(buf), (n >> 1) & 1, dead)) break;
             fence_after();
             const uint32_t base = tmem + buf * kBN + ((uint32_t)(quarter * 32) << 16);
-            constexpr int kPieces = kBN / 32;
 #pragma unroll 1
             for (int c = group; c < kPieces; c += kGroups) {
                 const int64_t col0 = tile.j0 + c * 32;
@@ -581,9 +594,10 @@ __global__ void __launch_bounds__(role_threads(kKind, kX8) + (kX8 ? 32 * kConver
                     s[32 * 16 + lane] = bias;
                     __syncwarp();
                 }
+                bias_ahead(c + kGroups);
                 if (kKind == kForward && live && p.z_scale) {
                     float amax = 0.f;   // of both halves, which are read again below
-#pragma unroll
+#pragma unroll 1
                     for (int h = 0; h < 2; ++h) {
                         tmem_load16(v, base + c * 32 + h * 16);
                         if (p.bias) add_bias(v, s + 32 * 16 + h * 16);
@@ -593,17 +607,19 @@ __global__ void __launch_bounds__(role_threads(kKind, kX8) + (kX8 ? 32 * kConver
                     }
                     block.exponent = block_exponent(amax);
                 }
-                tmem_load16(v, base + c * 32);
-                if (live) finish16<kKind, 0>(v, p, tile, row0, col0, s, ahead, block, lane);
-                __syncwarp();
-                tmem_load16(v, base + c * 32 + 16);
-                if (c + kGroups >= kPieces) {
-                    fence_before();
+#pragma unroll 1
+                for (int h = 0; h < 2; ++h) {
                     __syncwarp();
-                    if (lane == 0) bar_arrive(acc_empty(buf));
+                    tmem_load16(v, base + c * 32 + h * 16);
+                    if (h == 1 && c + kGroups >= kPieces) {
+                        fence_before();
+                        __syncwarp();
+                        if (lane == 0) bar_arrive(acc_empty(buf));
+                    }
+                    if (live) finish16<kKind>(v, p, tile, row0, col0 + h * 16, s, ahead, block, h, lane);
+                    const int64_t next = h == 0 ? col0 + 16 : col0 + kGroups * 32;
+                    if (kKind == kForward && (h == 0 || c + kGroups < kPieces)) load_ahead(ahead, p, row0, next, lane);
                 }
-                if (live) finish16<kKind, 1>(v, p, tile, row0, col0 + 16, s, ahead, block, lane);
-                if (c + kGroups < kPieces) look_ahead(c + kGroups);
             }
             if (group >= kPieces && lane == 0) bar_arrive(acc_empty(buf));
         }

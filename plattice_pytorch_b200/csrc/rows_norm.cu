@@ -18,16 +18,21 @@ namespace plr {
 constexpr int kUnits = 4;
 
 // Splits the flat group index of (CTA base + offset) into row and group: one
-// 64-bit division per CTA, 32-bit ones per thread.
+// 64-bit division per CTA, a multiplication and its correction per thread.
 struct GroupAt {
     int64_t row0;
     unsigned rem, groups;
+    float inv;
     __device__ __forceinline__ GroupAt(int64_t base, unsigned groups_) : groups(groups_) {
         row0 = base / groups;
         rem = (unsigned)(base - row0 * groups);
+        inv = 1.f / (float)groups;
     }
     __device__ __forceinline__ void at(unsigned offset, int64_t& row, unsigned& g) const {
-        const unsigned t = rem + offset, r = t / groups;
+        const unsigned t = rem + offset;
+        unsigned r = (unsigned)((float)t * inv);   // at most offset / groups + 1: off by one at most
+        if (r * groups > t) --r;
+        if (t - r * groups >= groups) ++r;
         row = row0 + r;
         g = t - r * groups;
     }
@@ -96,6 +101,25 @@ __global__ void __launch_bounds__(256) k_unpack8(T* __restrict__ y, int64_t pitc
     }
 }
 
+// Rows that lie on no 16-byte boundaries: a thread takes single values 256
+// apart, so that a warp's stores are whole lines.
+template <typename T>
+__global__ void __launch_bounds__(256) k_unpack8_any(T* __restrict__ y, int64_t pitch, const uint8_t* __restrict__ q,
+                                                     const uint8_t* __restrict__ scale, int64_t rows, int c) {
+    const int64_t base = (int64_t)blockIdx.x * (256 * 8);
+    const GroupAt where(base, (unsigned)c);
+    const int64_t width = (c + kBlock8 - 1) / kBlock8 * kBlock8;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+        int64_t row;
+        unsigned col;
+        where.at(threadIdx.x + 256 * u, row, col);
+        if (row >= rows) return;
+        const int64_t at = row * width + col;
+        y[row * pitch + col] = from_f32<T>(within<T>(value1(q[at], scale_of(scale[at >> 5]))));
+    }
+}
+
 // --------------------------------------------------------------- the norm
 //
 // L threads share a row (L <= 32: several rows per warp; L = 256 or 512: a CTA
@@ -120,6 +144,28 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
     return v;
 }
 
+// Stores what the lanes of a warp hold, 8 channels each (lane l of the warp:
+// row row0 + l / L, channels first + 8 (l % L)..), where rows lie on no 16-byte
+// boundaries: through shared memory, so that neighbouring lanes store
+// neighbouring channels.
+template <typename T, int L>
+__device__ __forceinline__ void warp_store8(T* p, const float (&v)[8], float* s, int64_t row0, int first, int64_t rows,
+                                            int c) {
+    constexpr int kW = L < 32 ? L : 32;
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
+    reinterpret_cast<float4*>(s)[lane * 2] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4*>(s)[lane * 2 + 1] = make_float4(v[4], v[5], v[6], v[7]);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int e = i * 32 + lane;
+        const int64_t row = row0 + e / (8 * kW);
+        const int col = first + e % (8 * kW);
+        if (row < rows && col < c) p[row * c + col] = from_f32<T>(s[e]);
+    }
+}
+
 struct NormArgs {
     void* y;
     uint8_t* yscale;   // non-null: y is 8-bit rows
@@ -135,11 +181,13 @@ struct NormArgs {
     bool vec;
 };
 
-template <typename T, int L, int kChunks>
+template <typename T, int L, int kChunks, bool kVec>
 __global__ void __launch_bounds__(L > 256 ? L : 256) k_rms_norm(const NormArgs a) {
     constexpr int kThreads = L > 256 ? L : 256;
     constexpr int kRows = kThreads / L;
     __shared__ float red[L > 32 ? L / 32 : 1];
+    __shared__ __align__(16) float turn[kVec ? 4 : kThreads * 8];
+    float* mine = turn + (kVec ? 0 : (threadIdx.x >> 5) * 256);
     const int lane = threadIdx.x % L;
     const int cp = (int)width8(a.c);
     float gain[kChunks][8];
@@ -158,8 +206,8 @@ __global__ void __launch_bounds__(L > 256 ? L : 256) k_rms_norm(const NormArgs a
             const int col = (k * L + lane) * 8;
             const int left = row < a.rows ? a.c - col : 0;
             const int64_t at = left > 0 ? row * a.c + col : 0;
-            x[k].load(static_cast<const T*>(a.x) + at, a.vec && left >= 8, left);
-            if (a.residual) r[k].load(static_cast<const T*>(a.residual) + at, a.vec && left >= 8, left);
+            x[k].load(static_cast<const T*>(a.x) + at, kVec && left >= 8, left);
+            if (a.residual) r[k].load(static_cast<const T*>(a.residual) + at, kVec && left >= 8, left);
         }
     };
     load_row((int64_t)blockIdx.x * kRows + threadIdx.x / L);
@@ -189,9 +237,12 @@ __global__ void __launch_bounds__(L > 256 ? L : 256) k_rms_norm(const NormArgs a
         for (int k = 0; k < kChunks; ++k) {
             const int col = (k * L + lane) * 8;
             const int left = live ? a.c - col : 0;
-            const bool vec = a.vec && left >= 8;
+            const bool vec = kVec && left >= 8;
             const int64_t at = left > 0 ? row * a.c + col : 0;
-            if (a.h) store8(static_cast<T*>(a.h) + at, v[k], vec, left);
+            const int64_t warp_row = row0 + (threadIdx.x & ~31) / L;
+            const int warp_col = (k * L + (L > 32 ? lane & ~31 : 0)) * 8;
+            if (a.h && kVec) store8(static_cast<T*>(a.h) + at, v[k], vec, left);
+            else if (a.h) warp_store8<T, L>(static_cast<T*>(a.h), v[k], mine, warp_row, warp_col, a.rows, a.c);
             float y[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) y[i] = left > i ? v[k][i] * rstd * gain[k][i] : 0.f;
@@ -205,8 +256,10 @@ __global__ void __launch_bounds__(L > 256 ? L : 256) k_rms_norm(const NormArgs a
                     reinterpret_cast<uint2*>(a.y)[p] = codes8(y, pow2(-s));
                     if ((lane & 3) == 0) a.yscale[p >> 2] = (uint8_t)(s + 127);
                 }
-            } else {
+            } else if (kVec) {
                 store8(static_cast<T*>(a.y) + at, y, vec, left);
+            } else {
+                warp_store8<T, L>(static_cast<T*>(a.y), y, mine, warp_row, warp_col, a.rows, a.c);
             }
         }
     }
@@ -231,12 +284,12 @@ struct NormGradArgs {
 // summed in registers, then over the CTA's rows in shared memory, and one row
 // of sums per CTA goes to `partial`; k_column_sums adds those in a fixed order
 // (no atomics: the same input gives the same bits).
-template <typename T, int L, int kChunks>
+template <typename T, int L, int kChunks, bool kVec>
 __global__ void __launch_bounds__(L > 256 ? L : 256) k_rms_norm_grad(const NormGradArgs a) {
     constexpr int kThreads = L > 256 ? L : 256;
     constexpr int kRows = kThreads / L;
     __shared__ float red[L > 32 ? L / 32 : 1];
-    __shared__ float sums[kRows > 1 ? kThreads * 8 : 1];
+    __shared__ __align__(16) float sums[kRows > 1 || !kVec ? kThreads * 8 : 4];
     const int lane = threadIdx.x % L;
     float gain[kChunks][8], acc[kChunks][8];
 #pragma unroll
@@ -259,8 +312,8 @@ __global__ void __launch_bounds__(L > 256 ? L : 256) k_rms_norm_grad(const NormG
             const int col = (k * L + lane) * 8;
             const int left = live ? a.c - col : 0;
             const int64_t at = left > 0 ? row * a.c + col : 0;
-            load8(n[k], static_cast<const T*>(a.h) + at, a.vec && left >= 8, left);
-            load8(g[k], static_cast<const T*>(a.grad_y) + at, a.vec && left >= 8, left);
+            load8(n[k], static_cast<const T*>(a.h) + at, kVec && left >= 8, left);
+            load8(g[k], static_cast<const T*>(a.grad_y) + at, kVec && left >= 8, left);
         }
 #pragma unroll
         for (int k = 0; k < kChunks; ++k)
@@ -276,7 +329,7 @@ __global__ void __launch_bounds__(L > 256 ? L : 256) k_rms_norm_grad(const NormG
         for (int k = 0; k < kChunks; ++k) {
             const int col = (k * L + lane) * 8;
             const int left = live ? a.c - col : 0;
-            const bool vec = a.vec && left >= 8;
+            const bool vec = kVec && left >= 8;
             const int64_t at = left > 0 ? row * a.c + col : 0;
             float o[8];
             if (a.grad_h) load8(o, static_cast<const T*>(a.grad_h) + at, vec, left);
@@ -285,7 +338,9 @@ __global__ void __launch_bounds__(L > 256 ? L : 256) k_rms_norm_grad(const NormG
                 const float d = rstd * (g[k][i] - n[k][i] * m);
                 o[i] = a.grad_h ? o[i] + d : d;
             }
-            store8(static_cast<T*>(a.grad_x) + at, o, vec, left);
+            if (kVec) store8(static_cast<T*>(a.grad_x) + at, o, vec, left);
+            else warp_store8<T, L>(static_cast<T*>(a.grad_x), o, sums + (threadIdx.x >> 5) * 256,
+                                   row0 + (threadIdx.x & ~31) / L, (k * L + (L > 32 ? lane & ~31 : 0)) * 8, a.rows, a.c);
         }
     }
 #pragma unroll
@@ -360,6 +415,12 @@ cudaError_t launch_unpack(void* y, int64_t pitch, const uint8_t* q, const uint8_
     const int64_t ctas = (rows * groups + 256 * kUnits - 1) / (256 * kUnits);
     if (ctas > INT_MAX) return cudaErrorInvalidValue;
     const bool vec = pitch % 8 == 0 && aligned16(y);
+    if (!vec && c >= 8) {
+        const int64_t n = (rows * c + 256 * 8 - 1) / (256 * 8);
+        if (n > INT_MAX) return cudaErrorInvalidValue;
+        k_unpack8_any<T><<<(unsigned)n, 256, 0, s>>>(static_cast<T*>(y), pitch, q, scale, rows, c);
+        return cudaGetLastError();
+    }
     k_unpack8<T><<<(unsigned)ctas, 256, 0, s>>>(static_cast<T*>(y), pitch, q, scale, rows, c, groups, vec);
     return cudaGetLastError();
 }
@@ -399,8 +460,9 @@ static int norm_ctas(int64_t rows, int rows_per_cta) {
 
 template <typename T>
 cudaError_t launch_norm(const NormArgs& a, cudaStream_t s) {
-#define PLR_F(L, K)                                                                                      \
-    (k_rms_norm<T, L, K><<<norm_ctas(a.rows, (L > 256 ? L : 256) / L), L > 256 ? L : 256, 0, s>>>(a),     \
+#define PLR_F(L, K)                                                                                            \
+    (a.vec ? k_rms_norm<T, L, K, true><<<norm_ctas(a.rows, (L > 256 ? L : 256) / L), L > 256 ? L : 256, 0, s>>>(a)   \
+           : k_rms_norm<T, L, K, false><<<norm_ctas(a.rows, (L > 256 ? L : 256) / L), L > 256 ? L : 256, 0, s>>>(a), \
      cudaGetLastError())
     PLR_NORM_SHAPE(a.c, PLR_F);
 #undef PLR_F
@@ -414,7 +476,10 @@ static int norm_rows_per_cta(int c) {
 
 template <typename T>
 cudaError_t launch_norm_grad(const NormGradArgs& a, int ctas, cudaStream_t s) {
-#define PLR_F(L, K) (k_rms_norm_grad<T, L, K><<<ctas, L > 256 ? L : 256, 0, s>>>(a), cudaGetLastError())
+#define PLR_F(L, K)                                                                \
+    (a.vec ? k_rms_norm_grad<T, L, K, true><<<ctas, L > 256 ? L : 256, 0, s>>>(a)   \
+           : k_rms_norm_grad<T, L, K, false><<<ctas, L > 256 ? L : 256, 0, s>>>(a), \
+     cudaGetLastError())
     PLR_NORM_SHAPE(a.c, PLR_F);
 #undef PLR_F
 }
