@@ -89,16 +89,17 @@ TORCH_EXT = os.path.join(HERE, "_plattice_torch.so")
 
 
 def build_torch_extension(force=False):
-    """Compile csrc/plattice_torch.cpp (PermutoLatticeFunction in C++) as the
-    torch extension module _plattice_torch, next to this file; returns its path."""
-    src = os.path.join(CSRC, "plattice_torch.cpp")
-    deps = [src, os.path.join(ROOT, "include", "plattice.h"), os.path.abspath(__file__)]
+    """Compile csrc/plattice_torch.cpp (PermutoLatticeFunction in C++) and
+    csrc/rows_torch.cpp (the row operators' calls) as the torch extension module
+    _plattice_torch, next to this file; returns its path."""
+    srcs = [os.path.join(CSRC, "plattice_torch.cpp"), os.path.join(CSRC, "rows_torch.cpp")]
+    deps = srcs + [os.path.join(ROOT, "include", "plattice.h"), os.path.abspath(__file__)]
     if not force and not _stale(TORCH_EXT, deps):
         return TORCH_EXT
     from torch.utils.cpp_extension import load
     bdir = os.path.join(BUILD, "torch_ext")
     os.makedirs(bdir, exist_ok=True)
-    load(name="_plattice_torch", sources=[src], build_directory=bdir, extra_cflags=["-O3"],
+    load(name="_plattice_torch", sources=srcs, build_directory=bdir, extra_cflags=["-O3"],
          extra_include_paths=[os.path.join(ROOT, "include")], with_cuda=True, verbose=False)
     built = os.path.join(bdir, "_plattice_torch.so")
     shutil.copyfile(built, TORCH_EXT + ".tmp")

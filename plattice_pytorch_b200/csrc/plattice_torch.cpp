@@ -185,6 +185,8 @@ at::Tensor permuto_lattice(const at::Tensor& features, const at::Tensor& values,
 
 }  // namespace
 
+void register_rows(py::module_& m);   // rows_torch.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.doc() = "PermutoLatticeFunction as a C++ autograd Function over libplattice_b200.so";
     m.def("set_entry_points", &set_entry_points,
@@ -194,4 +196,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           "forward of PermutoLatticeFunction (out); backward by autograd, on the kept lattice (keep) or on one "
           "rebuilt there",
           py::arg("features"), py::arg("values"), py::arg("keep") = true, py::call_guard<py::gil_scoped_release>());
+    register_rows(m);
 }

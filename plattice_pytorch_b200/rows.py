@@ -33,6 +33,7 @@ __all__ = ["Rows8", "pack8", "unpack8", "rms_norm", "rms_norm_backward", "linear
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
+_KEEP = {None: 0, "8bit": 1, "full": 2}
 _MAX_NORM = 16384
 
 
@@ -75,11 +76,8 @@ def _rows_of(shape):
 
 def _empty8(shape, device):
     rows, width = _rows_of(shape), _width8(int(shape[-1]))
-    r = Rows8.__new__(Rows8)   # made here to the format: nothing to check
-    r.q = torch.empty((rows, width), dtype=torch.uint8, device=device)
-    r.scale = torch.empty((rows, width // 32), dtype=torch.uint8, device=device)
-    r.shape = tuple(int(s) for s in shape)
-    return r
+    return _made8(torch.empty((rows, width), dtype=torch.uint8, device=device),
+                  torch.empty((rows, width // 32), dtype=torch.uint8, device=device), tuple(int(s) for s in shape))
 
 
 def _check_rows(t, name, channels=None):
@@ -107,11 +105,45 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+_UNSET = object()
+_EXT = _UNSET
+_CALLS = ("plattice_rows_pack8", "plattice_rows_unpack8", "plattice_rms_norm",
+          "plattice_rms_norm_backward_workspace_size", "plattice_rms_norm_backward", "plattice_linear_workspace_size",
+          "plattice_linear", "plattice_linear_backward_workspace_size", "plattice_linear_backward")
+
+
+def _cpp():
+    """The torch extension's forms of the calls below (the same tests,
+    allocations and library calls in one step), pointed at the loaded library;
+    None when the extension is not built.  They answer None to arguments that
+    fail a test: the Python form then finds which and raises its message."""
+    global _EXT
+    if _EXT is _UNSET:
+        try:
+            from . import _plattice_torch as m
+            m.set_rows_entry_points([ctypes.cast(getattr(_lib.lib(), n), ctypes.c_void_p).value for n in _CALLS])
+            _EXT = m
+        except ImportError:
+            _EXT = None
+    return _EXT
+
+
+def _made8(q, scale, shape):
+    r = Rows8.__new__(Rows8)   # made by the library to the format: nothing to check
+    r.q, r.scale, r.shape = q, scale, shape
+    return r
+
+
 # ---------------------------------------------------------------- 8-bit rows
 
 def pack8(x):
     """``x [..., c]`` in 8 bits, as :class:`Rows8`.  What is not finite comes
     back as NaN; its neighbours keep their values."""
+    cpp = _cpp()
+    if cpp is not None and (got := cpp.rows_pack8(x)) is not None:
+        if type(got) is int:
+            _raise("plattice_rows_pack8", got, f"shape={tuple(x.shape)}")
+        return _made8(*got, tuple(x.shape))
     _check_rows(x, "x")
     r = _empty8(x.shape, x.device)
     rc = _call(x.device.index, _lib_h().plattice_rows_pack8, r.q.data_ptr(), r.scale.data_ptr(), x.data_ptr(),
@@ -126,6 +158,11 @@ def unpack8(r, dtype=torch.float32):
     bfloat16; in float16 rounded, and at most 65504)."""
     _require(isinstance(r, Rows8), "r must be Rows8")
     _require(dtype in _DTYPES, "dtype must be float32, bfloat16 or float16")
+    cpp = _cpp()
+    if cpp is not None and (got := cpp.rows_unpack8(r.q, r.scale, r.shape, _DTYPES[dtype])) is not None:
+        if type(got) is int:
+            _raise("plattice_rows_unpack8", got, f"shape={r.shape}")
+        return got
     y = torch.empty(r.shape, dtype=dtype, device=r.device)
     rc = _call(r.device.index, _lib_h().plattice_rows_unpack8, y.data_ptr(), _DTYPES[dtype], r.q.data_ptr(),
                r.scale.data_ptr(), r.q.shape[0], r.shape[-1], _raw_stream(r.device.index))
@@ -141,6 +178,11 @@ def rms_norm(x, gain, residual=None, eps=1e-6, pack=False):
     ``rstd [...] = (mean h^2 + eps)^-1/2`` (float32) and ``y = h rstd gain``, in
     the type of ``x`` or, with ``pack``, as :class:`Rows8`.  ``h`` is ``x``
     itself without a residual.  ``gain [c]`` of any of the three types."""
+    cpp = _cpp()
+    if cpp is not None and (got := cpp.rows_rms_norm(x, gain, residual, eps, pack)) is not None:
+        if type(got) is int:
+            _raise("plattice_rms_norm", got, f"shape={tuple(x.shape)}")
+        return (_made8(*got[0], tuple(x.shape)), got[1], got[2]) if pack else got
     _check_rows(x, "x")
     c, dev = int(x.shape[-1]), x.device
     _require(c <= _MAX_NORM, f"x must have at most {_MAX_NORM} channels")
@@ -166,6 +208,11 @@ def rms_norm_backward(grad_y, h, rstd, gain, grad_h=None):
     """Gradients of :func:`rms_norm` from its ``h`` and ``rstd``: ``(grad_x,
     grad_gain)``; ``grad_x`` is the gradient of ``x`` and of the residual, with
     ``grad_h`` (the gradient that reaches ``h`` from elsewhere) added."""
+    cpp = _cpp()
+    if cpp is not None and (got := cpp.rows_rms_norm_backward(grad_y, h, rstd, gain, grad_h)) is not None:
+        if type(got) is int:
+            _raise("plattice_rms_norm_backward", got, f"shape={tuple(h.shape)}")
+        return got
     _check_rows(h, "h")
     c, dev = int(h.shape[-1]), h.device
     _require(c <= _MAX_NORM, f"h must have at most {_MAX_NORM} channels")
@@ -247,6 +294,20 @@ def linear(x, weight, bias=None, act="none", residual=None, split=0, out_dtype=N
     split])``, such as the features and values of a filter call.  ``keep``:
     the pre-activation ``z`` for the backward of an activation, "8bit" as Rows8
     or "full" in the output's type (None: ``z`` is None)."""
+    cpp = _cpp()
+    if (cpp is not None and act in ACTIVATIONS and keep in _KEEP and type(split) is int and isinstance(weight, torch.Tensor)
+            and (out_dtype is None or out_dtype is torch.float32 or out_dtype is weight.dtype)):
+        eight = type(x) is Rows8
+        got = cpp.rows_linear(x.q if eight else x, x.scale if eight else None, x.shape if eight else None, weight, bias,
+                              ACTIVATIONS[act], residual, split,
+                              out_dtype is torch.float32 or weight.dtype is torch.float32, _KEEP[keep])
+        if got is not None:
+            if type(got) is int:
+                _raise("plattice_linear", got, f"x={tuple(x.shape)} weight={tuple(weight.shape)} split={split}")
+            y0, y1, z, z_scale = got
+            if z_scale is not None:
+                z = _made8(z, z_scale, (*x.shape[:-1], weight.shape[0]))
+            return (y0 if y1 is None else (y0, y1)), z
     a, lead, out_dtype, dev = _linear_common(x, weight, act, out_dtype)
     n, split = a.n, int(split)
     _require(0 <= split < n, "split must be in [0, n)")
@@ -287,6 +348,18 @@ def linear_backward(grad_y, x, weight, z=None, act="none", bias_dtype=None, need
     activation; ``x`` may be None when ``grad_weight`` is not wanted).  The
     gradient of the residual is ``grad_y`` itself."""
     pair = isinstance(grad_y, (tuple, list))
+    cpp = _cpp()
+    if cpp is not None and act in ACTIVATIONS and x is not None and (not pair or len(grad_y) == 2):
+        eight, z8 = type(x) is Rows8, type(z) is Rows8
+        got = cpp.rows_linear_backward(
+            *(grad_y if pair else (grad_y, None)), x.q if eight else x, x.scale if eight else None,
+            x.shape if eight else None, weight, z.q if z8 else z, z.scale if z8 else None, z.shape if z8 else None,
+            ACTIVATIONS[act], _DTYPES.get(getattr(weight, "dtype", None) if bias_dtype is None else bias_dtype, -1),
+            bool(need[0]), bool(need[1]), bool(need[2]))
+        if got is not None:
+            if type(got) is int:
+                _raise("plattice_linear_backward", got, f"x={tuple(x.shape)} weight={tuple(weight.shape)}")
+            return got
     _require(not pair or len(grad_y) == 2, "grad_y must be a tensor or a pair of tensors")
     first = grad_y[0] if pair else grad_y
     _check_rows(first, "grad_y")

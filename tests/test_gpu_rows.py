@@ -418,3 +418,47 @@ def test_rows_of_not_finite_values_stay_in_their_rows(dev, R):
         bad[5] = bad[130] = True
         assert torch.equal(y.cpu()[~bad], clean.cpu()[~bad])
         assert not torch.isfinite(y[5]).any() and not torch.isfinite(y[130]).any()
+
+
+def test_python_and_extension_calls_agree(dev, R, monkeypatch):
+    """The calls through the torch extension and through ctypes give the same
+    bits, shapes and types."""
+    def collect():
+        out = list(_calls(R, dev)()) + list(_calls(R, dev, 5, 40, 72, torch.float32)())
+        x, w, b = _randn((9, 33), 70).to(dev), _randn((12, 33), 71).to(dev), _randn((12,), 72).to(dev)
+        (f, v), z = R.linear(x, w, b, split=5)
+        out += [f, v, *R.linear_backward((f, v), x, w)]
+        out += [R.linear(x.bfloat16(), w.bfloat16(), act="relu", keep="full", out_dtype=torch.float32)[i] for i in (0, 1)]
+        y, h, rstd = R.rms_norm(x, x[0].contiguous())
+        out += [y, h, rstd, *R.rms_norm_backward(y, h, rstd, x[0].contiguous())]
+        return out
+    fast = collect()
+    assert R._cpp() is not None
+    monkeypatch.setattr(R, "_EXT", None)
+    slow = collect()
+    for a, b in zip(fast, slow):
+        assert a.dtype == b.dtype and torch.equal(a, b)
+
+
+def test_refusals_on_the_device(dev, R):
+    x, w, g = torch.zeros(4, 8, device=dev), torch.zeros(3, 8, device=dev), torch.zeros(8, device=dev)
+    for call, text in [
+            (lambda: R.pack8(x.double()), "float32, bfloat16 or float16"),
+            (lambda: R.pack8(x.t()), "contiguous"),
+            (lambda: R.pack8(x.cpu()), "CUDA"),
+            (lambda: R.rms_norm(x, g.cpu()), "CUDA"),
+            (lambda: R.rms_norm(x, g, x.half()), "residual"),
+            (lambda: R.rms_norm_backward(x, x, g, g), "rstd"),
+            (lambda: R.linear(x, w.half()), "same type"),
+            (lambda: R.linear(x, w, residual=x), "residual"),
+            (lambda: R.linear(x, w, split=1, act="relu"), "split"),
+            (lambda: R.linear(R.pack8(x), w.half()), "8-bit"),
+            (lambda: R.linear(x, w, act="tanh"), "act"),
+            (lambda: R.linear_backward(x, x, w), "grad_y"),
+            (lambda: R.linear_backward(torch.zeros(4, 3, device=dev), x, w, act="gelu"), "z is needed"),
+            (lambda: R.linear_backward(torch.zeros(4, 3, device=dev), x, w, R.pack8(x), act="gelu"), "z must be"),
+            (lambda: R.linear_backward(torch.zeros(4, 3, device=dev), None, w), "x is needed")]:
+        with pytest.raises(RuntimeError, match=text):
+            call()
+    got = R.linear_backward(torch.ones(4, 3, device=dev), None, w, need=(True, False, True))
+    assert got[0].shape == (4, 8) and got[1] is None and got[2].tolist() == [4.0, 4.0, 4.0]
