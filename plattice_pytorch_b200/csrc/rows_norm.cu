@@ -38,26 +38,17 @@ struct GroupAt {
     }
 };
 
-// kFlat: rows without padding and aligned (c a multiple of 32), so that group g
-// is elements 8 g.. whatever its row: no division.
-template <typename T, bool kFlat>
+// Rows without padding and aligned (c a multiple of 32): group g is elements
+// 8 g.. whatever its row.
+template <typename T>
 __global__ void __launch_bounds__(256) k_pack8(uint8_t* __restrict__ q, uint8_t* __restrict__ scale,
-                                               const T* __restrict__ x, int64_t rows, int c, unsigned groups, bool vec) {
-    const int64_t base = (int64_t)blockIdx.x * (256 * kUnits), all = rows * groups;
-    const GroupAt where(kFlat ? 0 : base, kFlat ? 1 : groups);
+                                               const T* __restrict__ x, int64_t all) {
+    const int64_t base = (int64_t)blockIdx.x * (256 * kUnits);
     float v[kUnits][8];
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {
         const int64_t at = base + threadIdx.x + 256 * u;
-        if (kFlat) {
-            load8(v[u], x + (at < all ? at : 0) * 8, true, 8);
-        } else {
-            int64_t row;
-            unsigned g;
-            where.at(threadIdx.x + 256 * u, row, g);
-            const int left = at < all ? c - (int)g * 8 : 0;
-            load8(v[u], x + (left > 0 ? row * c + (int64_t)g * 8 : 0), vec && left >= 8, left);
-        }
+        load8(v[u], x + (at < all ? at : 0) * 8, true, 8);
     }
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {
@@ -69,6 +60,44 @@ __global__ void __launch_bounds__(256) k_pack8(uint8_t* __restrict__ q, uint8_t*
         if (at >= all) continue;
         reinterpret_cast<uint2*>(q)[at] = codes8(v[u], pow2(-s));
         if ((threadIdx.x & 3) == 0) scale[at >> 2] = (uint8_t)(s + 127);
+    }
+}
+
+// Other rows: a warp takes kBlocks blocks of 32, a lane per channel, so that
+// its loads are whole lines wherever the rows begin.
+constexpr int kBlocks = 8;
+
+__device__ __forceinline__ uint8_t code1(float v, float inv) {
+    return (uint8_t)__nv_cvt_float_to_fp8(is_infinite(fabsf(v)) ? __int_as_float(0x7fffffff) : v * inv, __NV_SATFINITE,
+                                          __NV_E4M3);
+}
+
+__device__ __forceinline__ float lane_magnitude(float v) { return is_infinite(fabsf(v)) ? 0.f : fmaxf(fabsf(v), 0.f); }
+
+template <typename T>
+__global__ void __launch_bounds__(256) k_pack8_any(uint8_t* __restrict__ q, uint8_t* __restrict__ scale,
+                                                   const T* __restrict__ x, int64_t rows, int c, unsigned blocks) {
+    const int lane = threadIdx.x & 31;
+    const GroupAt where(((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * kBlocks, blocks);
+    float v[kBlocks];
+    int64_t row[kBlocks];
+    unsigned b[kBlocks];
+#pragma unroll
+    for (int u = 0; u < kBlocks; ++u) {
+        where.at(u, row[u], b[u]);
+        const int col = (int)b[u] * 32 + lane;
+        v[u] = row[u] < rows && col < c ? to_f32(x[row[u] * c + col]) : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < kBlocks; ++u) {
+        if (row[u] >= rows) return;   // the same for all lanes
+        float amax = lane_magnitude(v[u]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        const int s = block_exponent(amax);
+        const int64_t at = row[u] * blocks + b[u];
+        q[at * 32 + lane] = code1(v[u], pow2(-s));
+        if (lane == 0) scale[at] = (uint8_t)(s + 127);
     }
 }
 
@@ -144,25 +173,75 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
     return v;
 }
 
-// Stores what the lanes of a warp hold, 8 channels each (lane l of the warp:
-// row row0 + l / L, channels first + 8 (l % L)..), where rows lie on no 16-byte
-// boundaries: through shared memory, so that neighbouring lanes store
-// neighbouring channels.
-template <typename T, int L>
-__device__ __forceinline__ void warp_store8(T* p, const float (&v)[8], float* s, int64_t row0, int first, int64_t rows,
-                                            int c) {
+// Channel i of a thread's group k.  Aligned rows: 8 neighbouring channels.
+// Others: the warp's lanes on neighbouring channels, 8 times, so that each
+// access of a warp is one run wherever the row begins (32 of them are then one
+// block of the 8-bit rows, across the lanes).
+template <int L, bool kVec> __device__ __forceinline__ int channel_of(int lane, int k, int i) {
     constexpr int kW = L < 32 ? L : 32;
-    const int lane = threadIdx.x & 31;
-    __syncwarp();
-    reinterpret_cast<float4*>(s)[lane * 2] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4*>(s)[lane * 2 + 1] = make_float4(v[4], v[5], v[6], v[7]);
-    __syncwarp();
+    if (kVec) return (k * L + lane) * 8 + i;
+    return (k * L + lane / kW * kW) * 8 + i * kW + lane % kW;
+}
+
+template <typename T, int L, bool kVec>
+__device__ __forceinline__ void load_group(float (&v)[8], const T* row, int lane, int k, int c) {
+    if (kVec) {
+        const int col = channel_of<L, true>(lane, k, 0);
+        load8(v, row + (col < c ? col : 0), col < c, 0);
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const int e = i * 32 + lane;
-        const int64_t row = row0 + e / (8 * kW);
-        const int col = first + e % (8 * kW);
-        if (row < rows && col < c) p[row * c + col] = from_f32<T>(s[e]);
+        const int col = channel_of<L, false>(lane, k, i);
+        v[i] = col < c ? to_f32(row[col]) : 0.f;
+    }
+}
+
+template <typename T, int L, bool kVec>
+__device__ __forceinline__ void store_group(T* row, const float (&v)[8], int lane, int k, int c) {
+    if (kVec) {
+        const int col = channel_of<L, true>(lane, k, 0);
+        if (col < c) store8(row + col, v, true, 8);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int col = channel_of<L, false>(lane, k, i);
+        if (col < c) row[col] = from_f32<T>(v[i]);
+    }
+}
+
+// Group k of a row as 8-bit rows; q and scale are the row's.  All lanes call.
+template <int L, bool kVec>
+__device__ __forceinline__ void store_group8(uint8_t* q, uint8_t* scale, float (&y)[8], int lane, int k, int width,
+                                             bool live) {
+    if (kVec) {
+        float amax = finite_amax(y);
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        const int s = block_exponent(amax), col = channel_of<L, true>(lane, k, 0);
+        if (live && col < width) {
+            *reinterpret_cast<uint2*>(q + col) = codes8(y, pow2(-s));
+            if ((lane & 3) == 0) scale[col >> 5] = (uint8_t)(s + 127);
+        }
+        return;
+    }
+    constexpr int kW = L < 32 ? L : 32, kPer = 32 / kW;   // a block is kPer of a thread's values, kW lanes
+#pragma unroll
+    for (int b = 0; b < 8 / kPer; ++b) {
+        float amax = 0.f;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) amax = fmaxf(amax, lane_magnitude(y[b * kPer + j]));
+#pragma unroll
+        for (int o = kW / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        const int s = block_exponent(amax);
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            const int col = channel_of<L, false>(lane, k, b * kPer + j);
+            if (!live || col >= width) continue;
+            q[col] = code1(y[b * kPer + j], pow2(-s));
+            if (lane % kW == 0 && j == 0) scale[col >> 5] = (uint8_t)(s + 127);
+        }
     }
 }
 
@@ -186,47 +265,52 @@ __global__ void __launch_bounds__(L > 256 ? L : 256) k_rms_norm(const NormArgs a
     constexpr int kThreads = L > 256 ? L : 256;
     constexpr int kRows = kThreads / L;
     __shared__ float red[L > 32 ? L / 32 : 1];
-    __shared__ __align__(16) float turn[kVec ? 4 : kThreads * 8];
-    float* mine = turn + (kVec ? 0 : (threadIdx.x >> 5) * 256);
     const int lane = threadIdx.x % L;
-    const int cp = (int)width8(a.c);
+    const int width = (int)width8(a.c);
     float gain[kChunks][8];
 #pragma unroll
     for (int k = 0; k < kChunks; ++k)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const int col = (k * L + lane) * 8 + i;
+            const int col = channel_of<L, kVec>(lane, k, i);
             gain[k][i] = col < a.c ? load_param(a.gain, a.gain_dtype, col) : 0.f;
         }
     const float inv_c = 1.f / (float)a.c;
-    Raw8<T> x[kChunks], r[kChunks];
+    const int64_t stride = (int64_t)gridDim.x * kRows;
+    Raw8<T> x[kChunks], r[kChunks];   // aligned rows: the next row's, loaded while this one is worked on
     auto load_row = [&](int64_t row) {
 #pragma unroll
         for (int k = 0; k < kChunks; ++k) {
-            const int col = (k * L + lane) * 8;
-            const int left = row < a.rows ? a.c - col : 0;
-            const int64_t at = left > 0 ? row * a.c + col : 0;
-            x[k].load(static_cast<const T*>(a.x) + at, kVec && left >= 8, left);
-            if (a.residual) r[k].load(static_cast<const T*>(a.residual) + at, kVec && left >= 8, left);
+            const int col = channel_of<L, true>(lane, k, 0);
+            const bool have = row < a.rows && col < a.c;
+            const int64_t at = have ? row * a.c + col : 0;
+            x[k].load(static_cast<const T*>(a.x) + at, have, 0);
+            if (a.residual) r[k].load(static_cast<const T*>(a.residual) + at, have, 0);
         }
     };
-    load_row((int64_t)blockIdx.x * kRows + threadIdx.x / L);
-    for (int64_t row0 = (int64_t)blockIdx.x * kRows; row0 < a.rows; row0 += (int64_t)gridDim.x * kRows) {
+    if (kVec) load_row((int64_t)blockIdx.x * kRows + threadIdx.x / L);
+    for (int64_t row0 = (int64_t)blockIdx.x * kRows; row0 < a.rows; row0 += stride) {
         const int64_t row = row0 + threadIdx.x / L;
         const bool live = row < a.rows;
+        const int64_t at = live ? row * a.c : 0;
         float v[kChunks][8];
         float ss = 0.f;
 #pragma unroll
         for (int k = 0; k < kChunks; ++k) {
-            x[k].widen(v[k]);
+            float t[8];
+            if (kVec) {
+                x[k].widen(v[k]);
+                if (a.residual) r[k].widen(t);
+            } else {
+                load_group<T, L, false>(v[k], static_cast<const T*>(a.x) + at, lane, k, live ? a.c : 0);
+                if (a.residual) load_group<T, L, false>(t, static_cast<const T*>(a.residual) + at, lane, k, live ? a.c : 0);
+            }
             if (a.residual) {
-                float t[8];
-                r[k].widen(t);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[k][i] += t[i];
             }
         }
-        load_row(row + (int64_t)gridDim.x * kRows);   // the next row's, while this one is worked on
+        if (kVec) load_row(row + stride);
 #pragma unroll
         for (int k = 0; k < kChunks; ++k)
 #pragma unroll
@@ -235,32 +319,15 @@ __global__ void __launch_bounds__(L > 256 ? L : 256) k_rms_norm(const NormArgs a
         if (live && lane == 0) a.rstd[row] = rstd;
 #pragma unroll
         for (int k = 0; k < kChunks; ++k) {
-            const int col = (k * L + lane) * 8;
-            const int left = live ? a.c - col : 0;
-            const bool vec = kVec && left >= 8;
-            const int64_t at = left > 0 ? row * a.c + col : 0;
-            const int64_t warp_row = row0 + (threadIdx.x & ~31) / L;
-            const int warp_col = (k * L + (L > 32 ? lane & ~31 : 0)) * 8;
-            if (a.h && kVec) store8(static_cast<T*>(a.h) + at, v[k], vec, left);
-            else if (a.h) warp_store8<T, L>(static_cast<T*>(a.h), v[k], mine, warp_row, warp_col, a.rows, a.c);
-            float y[8];
+            if (a.h && live) store_group<T, L, kVec>(static_cast<T*>(a.h) + at, v[k], lane, k, a.c);
+            float y[8];   // the gain is 0 behind the last channel
 #pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = left > i ? v[k][i] * rstd * gain[k][i] : 0.f;
-            if (a.yscale) {
-                float amax = finite_amax(y);
-                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-                const int s = block_exponent(amax);
-                if (live && col < cp) {
-                    const int64_t p = row * (cp / 8) + col / 8;
-                    reinterpret_cast<uint2*>(a.y)[p] = codes8(y, pow2(-s));
-                    if ((lane & 3) == 0) a.yscale[p >> 2] = (uint8_t)(s + 127);
-                }
-            } else if (kVec) {
-                store8(static_cast<T*>(a.y) + at, y, vec, left);
-            } else {
-                warp_store8<T, L>(static_cast<T*>(a.y), y, mine, warp_row, warp_col, a.rows, a.c);
-            }
+            for (int i = 0; i < 8; ++i) y[i] = v[k][i] * rstd * gain[k][i];
+            if (a.yscale)
+                store_group8<L, kVec>(static_cast<uint8_t*>(a.y) + row * width, a.yscale + row * (width / 32), y, lane, k,
+                                      width, live);
+            else if (live)
+                store_group<T, L, kVec>(static_cast<T*>(a.y) + at, y, lane, k, a.c);
         }
     }
 }
@@ -289,14 +356,14 @@ __global__ void __launch_bounds__(L > 256 ? L : 256) k_rms_norm_grad(const NormG
     constexpr int kThreads = L > 256 ? L : 256;
     constexpr int kRows = kThreads / L;
     __shared__ float red[L > 32 ? L / 32 : 1];
-    __shared__ __align__(16) float sums[kRows > 1 || !kVec ? kThreads * 8 : 4];
+    __shared__ float sums[kRows > 1 ? kThreads * 8 : 1];
     const int lane = threadIdx.x % L;
     float gain[kChunks][8], acc[kChunks][8];
 #pragma unroll
     for (int k = 0; k < kChunks; ++k)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const int col = (k * L + lane) * 8 + i;
+            const int col = channel_of<L, kVec>(lane, k, i);
             gain[k][i] = col < a.c ? load_param(a.gain, a.gain_dtype, col) : 0.f;
             acc[k][i] = 0.f;
         }
@@ -304,16 +371,15 @@ __global__ void __launch_bounds__(L > 256 ? L : 256) k_rms_norm_grad(const NormG
     for (int64_t row0 = (int64_t)blockIdx.x * kRows; row0 < a.rows; row0 += (int64_t)gridDim.x * kRows) {
         const int64_t row = row0 + threadIdx.x / L;
         const bool live = row < a.rows;
+        const int c = live ? a.c : 0;
+        const int64_t at = live ? row * a.c : 0;
         const float rstd = live ? a.rstd[row] : 0.f;
         float n[kChunks][8], g[kChunks][8];
         float dot = 0.f;
 #pragma unroll
         for (int k = 0; k < kChunks; ++k) {
-            const int col = (k * L + lane) * 8;
-            const int left = live ? a.c - col : 0;
-            const int64_t at = left > 0 ? row * a.c + col : 0;
-            load8(n[k], static_cast<const T*>(a.h) + at, kVec && left >= 8, left);
-            load8(g[k], static_cast<const T*>(a.grad_y) + at, kVec && left >= 8, left);
+            load_group<T, L, kVec>(n[k], static_cast<const T*>(a.h) + at, lane, k, c);
+            load_group<T, L, kVec>(g[k], static_cast<const T*>(a.grad_y) + at, lane, k, c);
         }
 #pragma unroll
         for (int k = 0; k < kChunks; ++k)
@@ -325,46 +391,38 @@ __global__ void __launch_bounds__(L > 256 ? L : 256) k_rms_norm_grad(const NormG
                 dot = fmaf(g[k][i], n[k][i], dot);
             }
         const float m = row_sum<L>(dot, red) * inv_c;
+        if (!live) continue;
 #pragma unroll
         for (int k = 0; k < kChunks; ++k) {
-            const int col = (k * L + lane) * 8;
-            const int left = live ? a.c - col : 0;
-            const bool vec = kVec && left >= 8;
-            const int64_t at = left > 0 ? row * a.c + col : 0;
             float o[8];
-            if (a.grad_h) load8(o, static_cast<const T*>(a.grad_h) + at, vec, left);
+            if (a.grad_h) load_group<T, L, kVec>(o, static_cast<const T*>(a.grad_h) + at, lane, k, c);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float d = rstd * (g[k][i] - n[k][i] * m);
                 o[i] = a.grad_h ? o[i] + d : d;
             }
-            if (kVec) store8(static_cast<T*>(a.grad_x) + at, o, vec, left);
-            else warp_store8<T, L>(static_cast<T*>(a.grad_x), o, sums + (threadIdx.x >> 5) * 256,
-                                   row0 + (threadIdx.x & ~31) / L, (k * L + (L > 32 ? lane & ~31 : 0)) * 8, a.rows, a.c);
+            store_group<T, L, kVec>(static_cast<T*>(a.grad_x) + at, o, lane, k, a.c);
         }
     }
 #pragma unroll
     for (int k = 0; k < kChunks; ++k) {
-        if (kRows > 1) {
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < 8; ++i) sums[i * kThreads + threadIdx.x] = acc[k][i];
-            __syncthreads();
-        }
-        for (int t = threadIdx.x; t < L * 8; t += kThreads) {
-            const int i = t / L, l = t % L, col = (k * L + l) * 8 + i;
-            float s = 0.f;
-            if (kRows > 1) {
-                for (int r = 0; r < kRows; ++r) s += sums[i * kThreads + r * L + l];
-                if (col < a.c) a.partial[(int64_t)blockIdx.x * a.c + col] = s;
-            }
-        }
         if (kRows == 1) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int col = (k * L + lane) * 8 + i;
+                const int col = channel_of<L, kVec>(lane, k, i);
                 if (col < a.c) a.partial[(int64_t)blockIdx.x * a.c + col] = acc[k][i];
             }
+            continue;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sums[i * kThreads + threadIdx.x] = acc[k][i];
+        __syncthreads();
+        for (int t = threadIdx.x; t < L * 8; t += kThreads) {
+            const int i = t / L, l = t % L, col = channel_of<L, kVec>(l, k, i);
+            float s = 0.f;
+            for (int r = 0; r < kRows; ++r) s += sums[i * kThreads + r * L + l];
+            if (col < a.c) a.partial[(int64_t)blockIdx.x * a.c + col] = s;
         }
     }
 }
@@ -397,14 +455,12 @@ cudaError_t column_sums(void* out, int dtype, const float* partial, int parts, i
 
 template <typename T>
 cudaError_t launch_pack(uint8_t* q, uint8_t* scale, const void* x, int64_t rows, int c, cudaStream_t s) {
-    const unsigned groups = (unsigned)(width8(c) / 8);
-    const int64_t ctas = (rows * groups + 256 * kUnits - 1) / (256 * kUnits);
+    const int64_t blocks = width8(c) / kBlock8;
+    const bool flat = c % kBlock8 == 0 && aligned16(x);
+    const int64_t per = flat ? 256 * kUnits / 4 : 8 * kBlocks, ctas = (rows * blocks + per - 1) / per;
     if (ctas > INT_MAX) return cudaErrorInvalidValue;
-    const bool vec = c % 8 == 0 && aligned16(x);
-    if (vec && c % kBlock8 == 0)
-        k_pack8<T, true><<<(unsigned)ctas, 256, 0, s>>>(q, scale, static_cast<const T*>(x), rows, c, groups, vec);
-    else
-        k_pack8<T, false><<<(unsigned)ctas, 256, 0, s>>>(q, scale, static_cast<const T*>(x), rows, c, groups, vec);
+    if (flat) k_pack8<T><<<(unsigned)ctas, 256, 0, s>>>(q, scale, static_cast<const T*>(x), rows * blocks * 4);
+    else k_pack8_any<T><<<(unsigned)ctas, 256, 0, s>>>(q, scale, static_cast<const T*>(x), rows, c, (unsigned)blocks);
     return cudaGetLastError();
 }
 
@@ -451,6 +507,7 @@ static int norm_ctas(int64_t rows, int rows_per_cta) {
         if (n_ <= 16) return F(16, 1);                   \
         if (n_ <= 32) return F(32, 1);                   \
         if (n_ <= 64) return F(32, 2);                   \
+        if (n_ <= 96) return F(32, 3);                   \
         if (n_ <= 128) return F(32, 4);                  \
         if (n_ <= 256) return F(256, 1);                 \
         if (n_ <= 512) return F(512, 1);                 \

@@ -370,12 +370,22 @@ def test_storage_that_is_not_aligned(dev, R):
         gain, res = _randn((k,), 52, dtype).to(dev), _randn((rows, k), 53, dtype).to(dev)
         gy, rn = _randn((rows, n), 54, dtype).to(dev), _randn((rows, n), 55, dtype).to(dev)
         assert torch.equal(R.pack8(x).q, R.pack8(shifted(x)).q)
-        for a, b in zip(R.rms_norm(x, gain, res), R.rms_norm(shifted(x), shifted(gain), shifted(res))):
-            assert torch.equal(a, b)
-        _, h, rstd = R.rms_norm(x, gain, res)
-        for a, b in zip(R.rms_norm_backward(x, h, rstd, gain),
-                        R.rms_norm_backward(shifted(x), shifted(h), shifted(rstd), shifted(gain))):
-            assert torch.equal(a, b)
+        # the lanes of an unaligned row hold other channels, so its sums are added in another order.  Each
+        # result is within its bound of the definition (the tests above: (h + 64 u) |y|, 64 u rstd, and
+        # h |g| + 64 u size for a gradient), so two of them differ by at most twice that
+        close = lambda a, b, t: worst(f64(a), f64(b), t) <= 1  # noqa: E731
+        hs = half_step(dtype)
+        y, h, rstd = R.rms_norm(x, gain, res)
+        ys, h2, rs = R.rms_norm(shifted(x), shifted(gain), shifted(res))
+        tiny = 2.0 ** -24 if dtype is torch.float16 else 1e-30
+        assert torch.equal(h, h2)
+        assert close(y, ys, 2.01 * (hs + 64 * U) * np.abs(f64(y)) + tiny) and close(rs, rstd, 128 * U * f64(rstd))
+        gx, gg = R.rms_norm_backward(x, h, rstd, gain)
+        gx2, gg2 = R.rms_norm_backward(shifted(x), shifted(h), shifted(rstd), shifted(gain))
+        nn, gn = np.abs(f64(h) * f64(rstd)[:, None]), np.abs(f64(x) * f64(gain))
+        size = f64(rstd)[:, None] * (gn + nn * (gn * nn).mean(-1, keepdims=True))
+        assert close(gx, gx2, 2.01 * hs * np.abs(f64(gx)) + 128 * U * size + tiny)
+        assert close(gg, gg2, 2.01 * hs * np.abs(f64(gg)) + 2 * (rows + 8) * U * np.abs(f64(x) * nn).sum(0) + tiny)
         ye, _ = R.linear(x, w, residual=rn)
         yg, _ = R.linear(shifted(x), shifted(w), residual=shifted(rn))
         assert torch.equal(ye, yg)
