@@ -375,6 +375,11 @@ template <int kAct, int N> __device__ __forceinline__ void slopes(float (&v)[N])
 #pragma unroll
     for (int i = 0; i < N; i += 2) slope2<kAct>(v[i], v[i + 1]);
 }
+__device__ __forceinline__ void slope16(float (&v)[16], int act) {
+    if (act == PLATTICE_ACT_RELU) slopes<PLATTICE_ACT_RELU>(v);
+    else if (act == PLATTICE_ACT_GELU) slopes<PLATTICE_ACT_GELU>(v);
+    else slopes<PLATTICE_ACT_SILU>(v);
+}
 template <int N> __device__ __forceinline__ void activate(float (&v)[N], int act) {
     if (act == PLATTICE_ACT_RELU) activations<PLATTICE_ACT_RELU>(v);
     else if (act == PLATTICE_ACT_GELU) activations<PLATTICE_ACT_GELU>(v);

@@ -170,6 +170,30 @@ __global__ void __launch_bounds__(256, 3) k_grad_z(const GradArgs a) {
     if (c < a.n) a.partial[(int64_t)blockIdx.y * a.n + c] = s;
 }
 
+// Lines of nw + nb sums added in order into two tensors (either may be null);
+// a CTA takes 32 columns, its 32 warps every 32nd line each.
+__global__ void __launch_bounds__(1024) k_sum_lines(void* out_w, int dtype_w, int64_t nw, void* out_b, int dtype_b, int nb,
+                                                    const float* __restrict__ partial, int lines) {
+    __shared__ float s[32][33];
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int64_t all = nw + nb, col = (int64_t)blockIdx.x * 32 + lane;
+    float v = 0.f;
+    if (col < all && (col < nw ? out_w != nullptr : out_b != nullptr))
+        for (int p = w; p < lines; p += 32) v += partial[(int64_t)p * all + col];
+    s[w][lane] = v;
+    __syncthreads();
+    v = s[lane][w];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    const int64_t mine = (int64_t)blockIdx.x * 32 + w;
+    if (lane != 0 || mine >= all) return;
+    if (mine < nw) {
+        if (out_w) store_param(out_w, dtype_w, mine, v);
+    } else if (out_b) {
+        store_param(out_b, dtype_b, mine - nw, v);
+    }
+}
+
 // out[e] = sum over the parts of partial[part][e], in order.
 template <typename T>
 __global__ void __launch_bounds__(256) k_add_parts(T* __restrict__ out, const float* __restrict__ partial, int parts,
@@ -432,6 +456,9 @@ static ForwardPlan forward_plan(const plattice_linear_args* a) {
 }
 
 struct BackwardPlan {
+    bool narrow;
+    int lines;       // narrow: CTAs along the rows
+    int64_t line_bytes;
     bool gz_needed, unpack;
     int shift, strips;
     int bn_x, bn_w, parts_b, parts_w;
@@ -441,6 +468,16 @@ struct BackwardPlan {
 static BackwardPlan backward_plan(const plattice_linear_args* a) {
     BackwardPlan p{};
     Carve c;
+    p.narrow = a->n <= 32;
+    if (p.narrow) {
+        // three CTAs of 4 warps an SM over the slices of 64 channels
+        const int64_t slices = ceil_div(a->k, 64), need = ceil_div(ceil_div(a->rows, 16), kGradWarps);
+        const int64_t most = ceil_div(3 * (int64_t)sm_count(), slices);
+        p.lines = (int)(need < most ? (need < 1 ? 1 : need) : most);
+        p.partial_w = c.take((int64_t)p.lines * ((int64_t)a->n * a->k + a->n) * 4);
+        p.bytes = c.at;
+        return p;
+    }
     while (p.shift < 5 && (8 << p.shift) < a->n) ++p.shift;   // a row's columns / 8, at most a warp
     p.strips = (int)ceil_div(a->n, 8 << p.shift);
     const int64_t need = ceil_div(a->rows, 256 >> p.shift), most = ceil_div(8 * (int64_t)sm_count(), p.strips);
@@ -557,6 +594,76 @@ static cudaError_t forward_mma(const plattice_linear_args* a, const ForwardPlan&
     if (!a->x_scale || p.unpack) return run_mma<kForward, false>(p.bn, x, w, m, s);
     x8_args(&m, a);
     return run_mma<kForward, true>(p.bn, x, w, m, s);
+}
+
+template <int kXT, int kParts, int kNF>
+static cudaError_t launch_narrow_grad(const SmallGradArgs& a, int lines, cudaStream_t s) {
+    int unused = 0;
+    const cudaError_t e = pl::kernel_once(
+        reinterpret_cast<const void*>(k_narrow_grad<kXT, kParts, kNF>),
+        [](int*) {
+            return cudaFuncSetAttribute(k_narrow_grad<kXT, kParts, kNF>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        NarrowGradShape<kXT, kParts>::kBytes);
+        },
+        &unused);
+    if (e != cudaSuccess) return e;
+    const int64_t slices = ceil_div(a.s.k, 64);
+    if (slices > 65535) return cudaErrorInvalidValue;
+    k_narrow_grad<kXT, kParts, kNF><<<dim3(lines, (unsigned)slices), 32 * kGradWarps,
+                                      NarrowGradShape<kXT, kParts>::kBytes, s>>>(a);
+    return cudaGetLastError();
+}
+
+template <int kXT, int kParts>
+static cudaError_t run_narrow_grad(const SmallGradArgs& a, int lines, cudaStream_t s) {
+    switch ((a.s.n + 7) / 8) {
+        case 1: return launch_narrow_grad<kXT, kParts, 1>(a, lines, s);
+        case 2: return launch_narrow_grad<kXT, kParts, 2>(a, lines, s);
+        case 3: return launch_narrow_grad<kXT, kParts, 3>(a, lines, s);
+        default: return launch_narrow_grad<kXT, kParts, 4>(a, lines, s);
+    }
+}
+
+static cudaError_t backward_narrow(const plattice_linear_args* a, const BackwardPlan& p, cudaStream_t s) {
+    const bool slope = a->act != PLATTICE_ACT_NONE;
+    float* partial = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + p.partial_w);
+    const int per = a->dtype == PLATTICE_F32 ? 4 : 8;   // elements of 16 bytes
+    SmallGradArgs g{};
+    g.s.x = a->x;
+    g.s.x_scale = a->x_scale;
+    g.s.w = a->w;
+    g.s.z = slope ? a->z : nullptr;
+    g.s.z_scale = slope ? a->z_scale : nullptr;
+    g.s.rows = a->rows;
+    g.s.k = a->k;
+    g.s.n = a->n;
+    g.s.split = a->split;
+    g.s.act = a->act;
+    g.s.w_dtype = a->dtype;
+    g.s.out_dtype = a->out_dtype;
+    g.s.vec_x = a->k % per == 0 && aligned16(a->x);
+    g.g0 = a->grad0;
+    g.g1 = a->grad1;
+    g.grad_x = a->grad_x;
+    g.partial = partial;
+    g.need_x = a->grad_x != nullptr;
+    g.need_w = a->grad_w != nullptr;
+    g.need_b = a->grad_bias != nullptr;
+    g.vec_gx = a->k % 8 == 0 && aligned16(a->grad_x);
+    cudaError_t e;
+    if (a->x_scale || !a->x)   // without x (no weight gradient) its type does not matter
+        e = a->dtype == PLATTICE_F32    ? run_narrow_grad<kX8, 3>(g, p.lines, s)
+            : a->dtype == PLATTICE_BF16 ? run_narrow_grad<kX8, 1>(g, p.lines, s)
+                                        : run_narrow_grad<kXHalf, 1>(g, p.lines, s);
+    else
+        e = a->dtype == PLATTICE_F32    ? run_narrow_grad<kXFloat, 3>(g, p.lines, s)
+            : a->dtype == PLATTICE_BF16 ? run_narrow_grad<kXBf16, 1>(g, p.lines, s)
+                                        : run_narrow_grad<kXHalf, 1>(g, p.lines, s);
+    if (e != cudaSuccess || !(a->grad_w || a->grad_bias)) return e;
+    const int64_t nw = (int64_t)a->n * a->k, columns = nw + a->n;
+    k_sum_lines<<<(unsigned)ceil_div(columns, 32), 1024, 0, s>>>(a->grad_w, a->dtype, nw, a->grad_bias, a->bias_dtype, a->n,
+                                                               partial, p.lines);
+    return cudaGetLastError();
 }
 
 static cudaError_t grad_z(const plattice_linear_args* a, const BackwardPlan& p, cudaStream_t s) {
@@ -676,6 +783,7 @@ int plattice_linear_backward(const plattice_linear_args* a, void* stream) {
     if (!a->workspace || a->workspace_bytes < (size_t)p.bytes) return PLATTICE_ERR_WORKSPACE;
     const int rc = rows_poll("plattice_linear_backward");
     if (rc != PLATTICE_OK) return rc;
+    if (p.narrow) return rows_status(backward_narrow(a, p, s), "plattice_linear_backward");
     e = grad_z(a, p, s);
     if (e == cudaSuccess) e = backward_mma(a, p, s);
     return rows_status(e, "plattice_linear_backward");

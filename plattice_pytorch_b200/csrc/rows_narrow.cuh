@@ -95,11 +95,11 @@ template <int kXT> struct NarrowRaw {
     uint8_t scale[NarrowShape<kXT>::kM][2];
 };
 
-template <int kXT>
+template <int kXT, int kFragments = NarrowShape<kXT>::kM>
 __device__ __forceinline__ void narrow_load(NarrowRaw<kXT>& r, const SmallArgs& a, int64_t row0, int chunk, int lane) {
     const int g = lane >> 2, ch = chunk * 64 + (lane & 3) * 16;
 #pragma unroll
-    for (int m = 0; m < NarrowShape<kXT>::kM; ++m)
+    for (int m = 0; m < kFragments; ++m)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int64_t row = row0 + m * 16 + h * 8 + g;
@@ -341,6 +341,361 @@ __global__ void __launch_bounds__(32 * kNarrowWarps, 2) k_narrow(const SmallArgs
             } else {
                 narrow_run(st, a.y0, a.out_dtype, row0, rows, 0, a.n, a.residual, lane);
             }
+        }
+    }
+}
+
+// ------------------------------------ backward, at most 32 output channels
+//
+// One pass: a warp takes 16 rows and a slice of 64 input channels, makes gz
+// (grad_y act'(z), rounded to the operands' type) once in shared memory, and
+// from it the rows' grad_x (gz w) and its share of grad_w (x^T gz, kept in
+// registers over all of the warp's rows) and grad_bias.  What a CTA gathered
+// goes to `partial`, one line of n k + n sums per CTA of a slice's column;
+// k_sum_lines adds those in order.  Read once: grad_y and z per slice, x;
+// written once: grad_x.
+struct SmallGradArgs {
+    SmallArgs s;          // x, x_scale, w, z, z_scale, rows, k, n, split, act, types, alignments
+    const void* g0;
+    const void* g1;
+    void* grad_x;
+    float* partial;       // [gridDim.x][n k + n]: grad_w [n][k], then grad_bias [n]
+    bool need_x, need_w, need_b;
+    bool vec_gx;          // 16-byte accesses to grad_x's rows
+};
+
+constexpr int kGradWarps = 4;
+constexpr int kTilePitch = 72;   // 16-bit elements: rows 144 bytes apart, no bank conflicts for ldmatrix
+
+template <int kXT, int kParts> struct NarrowGradShape {
+    static constexpr int kPX = kXT == kXFloat ? 3 : 1;
+    static constexpr int kFragBytes = kParts * 2 * 8 * 32 * 8;                        // weights of the slice
+    static constexpr int kWarpBytes = 16 * kNarrowPitch * 4 + kPX * 16 * kTilePitch * 2;
+    static constexpr int kBytes = kFragBytes + kGradWarps * kWarpBytes + 64 * 33 * 4;
+};
+
+template <int kP>
+__device__ __forceinline__ void to_parts(float a, float b, bool half, uint32_t (&o)[kP]) {
+    if (kP == 3) {
+        uint32_t t[3];
+        split3_pair(a, b, t);
+#pragma unroll
+        for (int i = 0; i < kP; ++i) o[i] = t[i];
+    } else if (half) {
+        union { __half2 h; uint32_t u; } x;
+        x.h = __floats2half2_rn(a, b);
+        o[0] = x.u;
+    } else {
+        union { __nv_bfloat162 h; uint32_t u; } x;
+        x.h = __floats2bfloat162_rn(a, b);
+        o[0] = x.u;
+    }
+}
+
+// Element e of the 16 rows' gradients, g0's run first, then g1's: its place
+// (row, column) and value.
+struct GradRun {
+    const void *g0, *g1;
+    int dtype, w0, w1, rows;
+    unsigned inv0, inv1;
+    int64_t row0;
+    __device__ __forceinline__ GradRun(const SmallGradArgs& a, int64_t row0_)
+        : g0(a.g0), g1(a.g1), dtype(a.s.out_dtype), w0(a.s.split ? a.s.split : a.s.n), w1(a.s.split ? a.s.n - a.s.split : 1),
+          rows((int)min((int64_t)16, a.s.rows - row0_)), row0(row0_) {
+        inv0 = 65536u / (unsigned)w0 + 1;   // t / w for t < 1024, w <= 32
+        inv1 = 65536u / (unsigned)w1 + 1;
+        if (!a.s.split) w1 = 0;
+    }
+    __device__ __forceinline__ float value(int e) const {
+        if (e < rows * w0) return load_param(g0, dtype, row0 * w0 + e);
+        e -= rows * w0;
+        return e < rows * w1 ? load_param(g1, dtype, row0 * w1 + e) : 0.f;
+    }
+    // offset in the staged rows, -1 behind the end
+    __device__ __forceinline__ int place(int e) const {
+        if (e < rows * w0) {
+            const int r = (int)((e * inv0) >> 16);
+            return r * kNarrowPitch + e - r * w0;
+        }
+        e -= rows * w0;
+        if (e >= rows * w1) return -1;
+        const int r = (int)((e * inv1) >> 16);
+        return r * kNarrowPitch + w0 + e - r * w1;
+    }
+};
+
+// kXT: the type of x (and, for 16-bit ones, of everything); kParts: 3 with
+// float32 weights; kNF: output channels / 8.
+template <int kXT, int kParts, int kNF>
+__global__ void __launch_bounds__(32 * kGradWarps, kParts == 3 ? 2 : 3) k_narrow_grad(const SmallGradArgs a) {
+    typedef NarrowGradShape<kXT, kParts> Shape;
+    constexpr int kPX = Shape::kPX, kKS = kNF > 2 ? 2 : 1;   // steps of 16 output channels in grad_x's sum
+    constexpr bool kHalf = kXT == kXHalf;
+    extern __shared__ __align__(16) char smem_raw[];
+    uint2* frag = reinterpret_cast<uint2*>(smem_raw);   // [kParts][kKS][8][32]
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    char* mine = smem_raw + Shape::kFragBytes + warp * Shape::kWarpBytes;
+    float* st = reinterpret_cast<float*>(mine);                                       // gz, 16 x 33
+    uint16_t* tile = reinterpret_cast<uint16_t*>(mine + 16 * kNarrowPitch * 4);       // x, [kPX][16][72]
+    float* gather = reinterpret_cast<float*>(smem_raw + Shape::kFragBytes + kGradWarps * Shape::kWarpBytes);
+    const int ch0 = blockIdx.y * 64, n = a.s.n, k = a.s.k;
+    const int cols_per_lane = kKS * 4;   // output channels of lane t in grad_x's sum: t cols_per_lane..
+
+    // fragment f, column c of the weights is channel (c >> 1) 16 + 2 f + (c & 1)
+    // of the slice, so that a lane ends up with 16 neighbouring channels
+    if (a.need_x) {
+        for (int i = threadIdx.x; i < kKS * 8 * 32; i += blockDim.x) {
+            const int l = i & 31, f = (i >> 5) & 7, s = i >> 8;
+            const int ch = ch0 + (l >> 3) * 16 + 2 * f + ((l >> 2) & 1), o = (l & 3) * cols_per_lane + s * 4;
+            float v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                v[j] = o + j < n && ch < k ? load_param(a.s.w, a.s.w_dtype, (int64_t)(o + j) * k + ch) : 0.f;
+            uint32_t lo[kParts], hi[kParts];
+            to_parts<kParts>(v[0], v[1], kHalf, lo);
+            to_parts<kParts>(v[2], v[3], kHalf, hi);
+#pragma unroll
+            for (int p = 0; p < kParts; ++p) frag[p * kKS * 256 + i] = make_uint2(lo[p], hi[p]);
+        }
+    }
+    for (int i = lane; i < 16 * kNarrowPitch; i += 32) st[i] = 0.f;   // columns behind n stay 0
+    __syncthreads();
+
+    float dw[4][kNF][4];
+#pragma unroll
+    for (int m = 0; m < 4; ++m)
+#pragma unroll
+        for (int f = 0; f < kNF; ++f)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) dw[m][f][i] = 0.f;
+    float db = 0.f;
+
+    const int64_t blocks = (a.s.rows + 15) / 16, stride = (int64_t)gridDim.x * kGradWarps;
+    int64_t block = (int64_t)blockIdx.x * kGradWarps + warp;
+    constexpr int kRun = kNF * 4;   // 16 rows x 8 kNF columns / 32 lanes
+    float gn[kRun];                 // the next rows' gradients, x and z, loaded ahead
+    uint4 xn[2][NarrowShape<kXT>::kRaw];
+    uint8_t xs[2];
+    uint4 zn = make_uint4(0, 0, 0, 0);
+    uint8_t zs = 127;
+    auto load_rows = [&](int64_t b) {
+        const GradRun run(a, b * 16);
+#pragma unroll
+        for (int i = 0; i < kRun; ++i) gn[i] = run.value(i * 32 + lane);
+        if (a.s.z_scale) {   // a lane per half row
+            const int64_t row = b * 16 + (lane >> 1);
+            const bool live = row < a.s.rows;
+            zn = live ? reinterpret_cast<const uint4*>(a.s.z)[row * 2 + (lane & 1)] : make_uint4(0, 0, 0, 0);
+            zs = live ? a.s.z_scale[row] : 127;
+        }
+        if (!a.need_w) return;
+        NarrowRaw<kXT> r;
+        narrow_load<kXT, 1>(r, a.s, b * 16, blockIdx.y, lane);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int i = 0; i < NarrowShape<kXT>::kRaw; ++i) xn[h][i] = r.v[0][h][i];
+            if (kXT == kX8) xs[h] = r.scale[0][h];
+        }
+    };
+    if (block < blocks) load_rows(block);
+    for (; block < blocks; block += stride) {
+        const int64_t row0 = block * 16;
+        const int rows = (int)min((int64_t)16, a.s.rows - row0);
+        __syncwarp();
+        {
+            const GradRun run(a, row0);
+#pragma unroll
+            for (int i = 0; i < kRun; ++i) {
+                const int at = run.place(i * 32 + lane);
+                if (at >= 0) st[at] = gn[i];
+            }
+        }
+        if (rows < 16)
+            for (int i = rows * kNarrowPitch + lane; i < 16 * kNarrowPitch; i += 32) st[i] = 0.f;
+        if (a.need_w) {   // x, widened, into the tile
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint16_t* row = tile + (g + 8 * h) * kTilePitch + t * 16;
+                if (kXT == kX8) {
+                    float v[16];
+                    const float sc = scale_of(xs[h]);
+                    values4(v, xn[h][0].x, sc);
+                    values4(v + 4, xn[h][0].y, sc);
+                    values4(v + 8, xn[h][0].z, sc);
+                    values4(v + 12, xn[h][0].w, sc);
+                    union { uint4 u[2]; __nv_bfloat162 b[8]; } o;   // exact
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) o.b[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+                    reinterpret_cast<uint4*>(row)[0] = o.u[0];
+                    reinterpret_cast<uint4*>(row)[1] = o.u[1];
+                } else if (kXT == kXFloat) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint4& q = xn[h][i % NarrowShape<kXT>::kRaw];
+                        uint32_t lo[3], hi[3];
+                        split3_pair(__uint_as_float(q.x), __uint_as_float(q.y), lo);
+                        split3_pair(__uint_as_float(q.z), __uint_as_float(q.w), hi);
+#pragma unroll
+                        for (int p = 0; p < 3; ++p)
+                            *reinterpret_cast<uint2*>(row + (p % kPX) * 16 * kTilePitch + i * 4) = make_uint2(lo[p], hi[p]);
+                    }
+                } else {
+                    reinterpret_cast<uint4*>(row)[0] = xn[h][0];
+                    reinterpret_cast<uint4*>(row)[1] = xn[h][1 % NarrowShape<kXT>::kRaw];
+                }
+            }
+        }
+        const uint4 zc = zn;
+        const float zscale = scale_of(zs);
+        if (block + stride < blocks) load_rows(block + stride);
+        __syncwarp();
+        if (a.s.z_scale) {
+            float v[16];
+            values4(v, zc.x, zscale);
+            values4(v + 4, zc.y, zscale);
+            values4(v + 8, zc.z, zscale);
+            values4(v + 12, zc.w, zscale);
+            slope16(v, a.s.act);
+            float* row = st + (lane >> 1) * kNarrowPitch + (lane & 1) * 16;
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if ((lane & 1) * 16 + i < n) row[i] *= v[i];
+            __syncwarp();
+        } else if (a.s.z) {
+            const unsigned inv = 65536u / (unsigned)n + 1;
+            for (int e = lane; e < rows * n; e += 32) {
+                const int r = (int)((e * inv) >> 16);
+                float v[16] = {load_param(a.s.z, a.s.out_dtype, row0 * n + e)};
+                slope16(v, a.s.act);
+                st[r * kNarrowPitch + e - r * n] *= v[0];
+            }
+            __syncwarp();
+        }
+        if (a.need_b) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) db += st[r * kNarrowPitch + lane];
+        }
+        if (a.need_x) {
+            uint32_t o[kKS][kParts][4];
+#pragma unroll
+            for (int s = 0; s < kKS; ++s)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float* p = st + (g + 8 * h) * kNarrowPitch + t * cols_per_lane + s * 4;
+                    uint32_t lo[kParts], hi[kParts];
+                    to_parts<kParts>(p[0], p[1], kHalf, lo);
+                    to_parts<kParts>(p[2], p[3], kHalf, hi);
+#pragma unroll
+                    for (int q = 0; q < kParts; ++q) {
+                        o[s][q][h] = lo[q];
+                        o[s][q][2 + h] = hi[q];
+                    }
+                }
+            float dx[8][4];
+#pragma unroll
+            for (int f = 0; f < 8; ++f) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) dx[f][i] = 0.f;
+#pragma unroll
+                for (int sum = 2; sum >= 0; --sum)   // small products first
+#pragma unroll
+                    for (int pa = 0; pa < kParts; ++pa) {
+                        const int pb = sum - pa;
+                        if (pb < 0 || pb >= kParts) continue;
+#pragma unroll
+                        for (int s = 0; s < kKS; ++s)
+                            mma16816<kHalf>(dx[f], o[s][pa][0], o[s][pa][1], o[s][pa][2], o[s][pa][3],
+                                            frag[((pb * kKS + s) * 8 + f) * 32 + lane]);
+                    }
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {   // 16 neighbouring channels of rows g and g + 8
+                if (g + 8 * h >= rows) continue;
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    const int ch = ch0 + t * 16 + q * 8, left = k - ch;
+                    if (left <= 0) continue;
+                    float v[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] = dx[q * 4 + (i >> 1)][h * 2 + (i & 1)];
+                    const int64_t at = (row0 + g + 8 * h) * k + ch;
+                    const bool vec = a.vec_gx && left >= 8;
+                    if (kXT == kXHalf) store8(static_cast<__half*>(a.grad_x) + at, v, vec, left);
+                    else if (kParts == 3) store8(static_cast<float*>(a.grad_x) + at, v, vec, left);
+                    else store8(static_cast<__nv_bfloat16*>(a.grad_x) + at, v, vec, left);
+                }
+            }
+        }
+        if (a.need_w) {
+            uint32_t b[kParts][kNF][2];
+#pragma unroll
+            for (int f = 0; f < kNF; ++f)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float* p = st + (2 * t + 8 * h) * kNarrowPitch + f * 8 + g;
+                    uint32_t o[kParts];
+                    to_parts<kParts>(p[0], p[kNarrowPitch], kHalf, o);
+#pragma unroll
+                    for (int q = 0; q < kParts; ++q) b[q][f][h] = o[q];
+                }
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                uint32_t x[kPX][4];
+#pragma unroll
+                for (int q = 0; q < kPX; ++q) {
+                    const uint16_t* src = tile + q * 16 * kTilePitch + ((lane >> 4) * 8 + (lane & 7)) * kTilePitch +
+                                          m * 16 + ((lane >> 3) & 1) * 8;
+                    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                                 : "=r"(x[q][0]), "=r"(x[q][1]), "=r"(x[q][2]), "=r"(x[q][3])
+                                 : "r"((uint32_t)__cvta_generic_to_shared(src))
+                                 : "memory");
+                }
+#pragma unroll
+                for (int sum = 2; sum >= 0; --sum)
+#pragma unroll
+                    for (int px = 0; px < kPX; ++px) {
+                        const int pb = sum - px;
+                        if (pb < 0 || pb >= kParts) continue;
+#pragma unroll
+                        for (int f = 0; f < kNF; ++f)
+                            mma16816<kHalf>(dw[m][f], x[px][0], x[px][1], x[px][2], x[px][3],
+                                            make_uint2(b[pb][f][0], b[pb][f][1]));
+                    }
+            }
+        }
+    }
+
+    // the CTA's sums, warp after warp
+    float* line = a.partial + (int64_t)blockIdx.x * ((int64_t)n * k + n);
+    if (a.need_w) {
+        for (int w = 0; w < kGradWarps; ++w) {
+            __syncthreads();
+            if (warp != w) continue;
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
+#pragma unroll
+                for (int f = 0; f < kNF; ++f)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float* p = gather + (m * 16 + (i >> 1) * 8 + g) * 33 + f * 8 + t * 2 + (i & 1);
+                        *p = w ? *p + dw[m][f][i] : dw[m][f][i];
+                    }
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < 64 * n; i += blockDim.x) {
+            const int col = i >> 6, ch = i & 63;
+            if (ch0 + ch < k) line[(int64_t)col * k + ch0 + ch] = gather[ch * 33 + col];
+        }
+    }
+    if (a.need_b && blockIdx.y == 0) {
+        __syncthreads();
+        gather[warp * 32 + lane] = db;
+        __syncthreads();
+        if (threadIdx.x < n) {
+            float v = 0.f;
+            for (int w = 0; w < kGradWarps; ++w) v += gather[w * 32 + threadIdx.x];
+            line[(int64_t)n * k + threadIdx.x] = v;
         }
     }
 }
