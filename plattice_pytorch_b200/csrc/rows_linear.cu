@@ -470,9 +470,9 @@ static BackwardPlan backward_plan(const plattice_linear_args* a) {
     Carve c;
     p.narrow = a->n <= 32;
     if (p.narrow) {
-        // three CTAs of 4 warps an SM over the slices of 64 channels
+        // one round of CTAs over the slices of 64 channels
         const int64_t slices = ceil_div(a->k, 64), need = ceil_div(ceil_div(a->rows, 16), kGradWarps);
-        const int64_t most = ceil_div(3 * (int64_t)sm_count(), slices);
+        const int64_t most = ceil_div(narrow_grad_ctas(a->dtype == PLATTICE_F32 ? 3 : 1, (a->n + 7) / 8) * (int64_t)sm_count(), slices);
         p.lines = (int)(need < most ? (need < 1 ? 1 : need) : most);
         p.partial_w = c.take((int64_t)p.lines * ((int64_t)a->n * a->k + a->n) * 4);
         p.bytes = c.at;
@@ -509,34 +509,44 @@ static cudaError_t launch_grad_z(const GradArgs& g, const BackwardPlan& p, cudaS
     return cudaGetLastError();
 }
 
-template <int kXT, int kNF, bool kW3, bool kSplit>
+template <int kXT, int kNF, bool kW3, bool kSplit, bool kPlain>
 static cudaError_t launch_narrow(const SmallArgs& a, int64_t blocks, cudaStream_t s) {
     const int64_t smem = narrow_fragments(a.k, kNF, kW3 ? 3 : 1) + narrow_staging(NarrowShape<kXT>::kM);
     int unused = 0;
     const cudaError_t e = pl::kernel_once(
-        reinterpret_cast<const void*>(k_narrow<kXT, kNF, kW3, kSplit>),
+        reinterpret_cast<const void*>(k_narrow<kXT, kNF, kW3, kSplit, kPlain>),
         [](int*) {
-            return cudaFuncSetAttribute(k_narrow<kXT, kNF, kW3, kSplit>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+            return cudaFuncSetAttribute(k_narrow<kXT, kNF, kW3, kSplit, kPlain>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                         (int)(kNarrowMost + narrow_staging(2)));
         },
         &unused);
     if (e != cudaSuccess) return e;
-    const int64_t need = kSplit ? blocks : ceil_div(blocks, kNarrowWarps), most = 4 * (int64_t)sm_count();
-    k_narrow<kXT, kNF, kW3, kSplit><<<(unsigned)(need < most ? need : most), 32 * kNarrowWarps, smem, s>>>(a);
+    // one round of CTAs: as many as are resident at a time
+    const int64_t need = kSplit ? blocks : ceil_div(blocks, kNarrowWarps);
+    const int64_t fit = kMaxSmem / (smem + 1024), ctas = narrow_ctas(kXT, kNF);
+    const int64_t most = (fit < ctas ? fit : ctas) * sm_count();
+    k_narrow<kXT, kNF, kW3, kSplit, kPlain><<<(unsigned)(need < most ? need : most), 32 * kNarrowWarps, smem, s>>>(a);
     return cudaGetLastError();
+}
+
+template <int kXT, bool kW3, int kNF>
+static cudaError_t run_narrow_as(const SmallArgs& a, cudaStream_t s) {
+    const int64_t blocks = ceil_div(a.rows, 16 * NarrowShape<kXT>::kM);
+    // fewer blocks of rows than a warp on each SM would take: the warps of a
+    // CTA share a block instead (at least two chunks of channels to share)
+    if (blocks <= 2 * (int64_t)sm_count() && a.k > 64) return launch_narrow<kXT, kNF, kW3, true, false>(a, blocks, s);
+    if (a.out_dtype == PLATTICE_F32 && a.act == PLATTICE_ACT_NONE && !a.residual && !a.z)
+        return launch_narrow<kXT, kNF, kW3, false, true>(a, blocks, s);
+    return launch_narrow<kXT, kNF, kW3, false, false>(a, blocks, s);
 }
 
 template <int kXT, bool kW3>
 static cudaError_t run_narrow(const SmallArgs& a, cudaStream_t s) {
-    const int64_t blocks = ceil_div(a.rows, 16 * NarrowShape<kXT>::kM);
-    // fewer blocks of rows than a warp on each SM would take: the warps of a
-    // CTA share a block instead (at least two chunks of channels to share)
-    const bool split = blocks <= 2 * (int64_t)sm_count() && a.k > 64;
     switch ((a.n + 7) / 8) {
-        case 1: return split ? launch_narrow<kXT, 1, kW3, true>(a, blocks, s) : launch_narrow<kXT, 1, kW3, false>(a, blocks, s);
-        case 2: return split ? launch_narrow<kXT, 2, kW3, true>(a, blocks, s) : launch_narrow<kXT, 2, kW3, false>(a, blocks, s);
-        case 3: return split ? launch_narrow<kXT, 3, kW3, true>(a, blocks, s) : launch_narrow<kXT, 3, kW3, false>(a, blocks, s);
-        default: return split ? launch_narrow<kXT, 4, kW3, true>(a, blocks, s) : launch_narrow<kXT, 4, kW3, false>(a, blocks, s);
+        case 1: return run_narrow_as<kXT, kW3, 1>(a, s);
+        case 2: return run_narrow_as<kXT, kW3, 2>(a, s);
+        case 3: return run_narrow_as<kXT, kW3, 3>(a, s);
+        default: return run_narrow_as<kXT, kW3, 4>(a, s);
     }
 }
 
@@ -554,7 +564,9 @@ static cudaError_t forward_small(const plattice_linear_args* a, Way way, cudaStr
     const int e = a->dtype == PLATTICE_F32 ? 4 : 8;   // elements of 16 bytes
     const SmallArgs p{a->x, a->x_scale, a->w, a->bias, a->residual, a->y0, a->y1, a->z, a->z_scale, a->rows,
                       a->k, a->n, a->split, a->act, a->dtype, a->out_dtype, a->bias_dtype,
-                      a->k % e == 0 && aligned16(a->x), a->k % 8 == 0 && aligned16(a->w)};
+                      a->k % e == 0 && aligned16(a->x), a->k % 8 == 0 && aligned16(a->w),
+                      aligned16(a->y0) && (!a->y1 || aligned16(a->y1)) && (!a->residual || aligned16(a->residual)) &&
+                          (!a->z || aligned16(a->z))};
     if (way == kWayFew)
         return a->dtype == PLATTICE_F32    ? run_few<float>(p, s)
                : a->dtype == PLATTICE_BF16 ? run_few<__nv_bfloat16>(p, s)
@@ -596,32 +608,39 @@ static cudaError_t forward_mma(const plattice_linear_args* a, const ForwardPlan&
     return run_mma<kForward, true>(p.bn, x, w, m, s);
 }
 
-template <int kXT, int kParts, int kNF>
+template <int kXT, int kParts, int kNF, bool kG32>
 static cudaError_t launch_narrow_grad(const SmallGradArgs& a, int lines, cudaStream_t s) {
     int unused = 0;
     const cudaError_t e = pl::kernel_once(
-        reinterpret_cast<const void*>(k_narrow_grad<kXT, kParts, kNF>),
+        reinterpret_cast<const void*>(k_narrow_grad<kXT, kParts, kNF, kG32>),
         [](int*) {
-            return cudaFuncSetAttribute(k_narrow_grad<kXT, kParts, kNF>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+            return cudaFuncSetAttribute(k_narrow_grad<kXT, kParts, kNF, kG32>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                         NarrowGradShape<kXT, kParts>::kBytes);
         },
         &unused);
     if (e != cudaSuccess) return e;
     const int64_t slices = ceil_div(a.s.k, 64);
     if (slices > 65535) return cudaErrorInvalidValue;
-    k_narrow_grad<kXT, kParts, kNF><<<dim3(lines, (unsigned)slices), 32 * kGradWarps,
-                                      NarrowGradShape<kXT, kParts>::kBytes, s>>>(a);
+    k_narrow_grad<kXT, kParts, kNF, kG32><<<dim3(lines, (unsigned)slices), 32 * kGradWarps,
+                                            NarrowGradShape<kXT, kParts>::kBytes, s>>>(a);
     return cudaGetLastError();
+}
+
+template <int kXT, int kParts, bool kG32>
+static cudaError_t run_narrow_grad_as(const SmallGradArgs& a, int lines, cudaStream_t s) {
+    switch ((a.s.n + 7) / 8) {
+        case 1: return launch_narrow_grad<kXT, kParts, 1, kG32>(a, lines, s);
+        case 2: return launch_narrow_grad<kXT, kParts, 2, kG32>(a, lines, s);
+        case 3: return launch_narrow_grad<kXT, kParts, 3, kG32>(a, lines, s);
+        default: return launch_narrow_grad<kXT, kParts, 4, kG32>(a, lines, s);
+    }
 }
 
 template <int kXT, int kParts>
 static cudaError_t run_narrow_grad(const SmallGradArgs& a, int lines, cudaStream_t s) {
-    switch ((a.s.n + 7) / 8) {
-        case 1: return launch_narrow_grad<kXT, kParts, 1>(a, lines, s);
-        case 2: return launch_narrow_grad<kXT, kParts, 2>(a, lines, s);
-        case 3: return launch_narrow_grad<kXT, kParts, 3>(a, lines, s);
-        default: return launch_narrow_grad<kXT, kParts, 4>(a, lines, s);
-    }
+    if constexpr (kParts == 1)
+        if (a.s.out_dtype != PLATTICE_F32) return run_narrow_grad_as<kXT, kParts, false>(a, lines, s);
+    return run_narrow_grad_as<kXT, kParts, true>(a, lines, s);
 }
 
 static cudaError_t backward_narrow(const plattice_linear_args* a, const BackwardPlan& p, cudaStream_t s) {

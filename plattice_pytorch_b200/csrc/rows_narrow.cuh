@@ -25,6 +25,7 @@ struct SmallArgs {
     int w_dtype, out_dtype, bias_dtype;
     bool vec_x;    // 16-byte accesses to x's rows
     bool vec_w;    // the same for w's
+    bool vec_y;    // the outputs and the residual begin on 16-byte boundaries
 };
 
 // A float32 value as three bfloat16 whose sum it is: each takes the leading 8
@@ -64,6 +65,16 @@ __device__ __forceinline__ void split3_pair(float a, float b, uint32_t (&o)[3]) 
 // per row and load, straight into the operand's registers.
 //
 // float32 runs as three bfloat16 parts (split3), six products, small first.
+//
+// 8-bit rows go in as float16, one conversion a pair of codes and exact, with
+// their scales left out: a step then stays within a block of 32 channels (lane
+// t holds t 8.. of each), whose sum is multiplied by the row's scale.  The
+// weights are float16 too, each output channel's times the power of two that
+// takes its largest to 2^14: 11 significant bits hold a bfloat16 weight down
+// to 2^-28 of that largest, and below lose at most 2^-39 of it; a float32
+// weight takes three parts.  (Widening codes to bfloat16 instead, scales
+// included, took five instructions a pair: 38 against 2x us for 1048576 rows,
+// 64 -> 8.)
 
 template <int kXT> struct NarrowShape {
     static constexpr int kM = kXT == kX8 ? 2 : 1;                               // 16-row fragments
@@ -76,6 +87,9 @@ constexpr int kNarrowWarps = 8;
 constexpr int kNarrowPitch = 33;
 __host__ inline int64_t narrow_staging(int m) { return (int64_t)kNarrowWarps * 16 * m * kNarrowPitch * 4; }
 constexpr int64_t kNarrowMost = 64 * 1024;   // bytes of weights: two CTAs then share an SM
+
+// CTAs that the registers let share an SM (more would spill).
+__host__ __device__ constexpr int narrow_ctas(int xt, int nf) { return xt == kXFloat || (xt == kX8 && nf > 1) ? 2 : 3; }
 
 template <bool kHalf>
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint2 b) {
@@ -95,49 +109,116 @@ template <int kXT> struct NarrowRaw {
     uint8_t scale[NarrowShape<kXT>::kM][2];
 };
 
+// The same of 8-bit rows for k_narrow: 8 channels of each of the two blocks.
+struct NarrowCodes {
+    uint2 v[2][2][2];   // fragment, row, block
+    uint8_t scale[2][2][2];
+};
+
+// Rows behind the last read the last one again (what they give is not stored),
+// a missing second block reads the first: no load hangs on a branch.
+__device__ __forceinline__ void narrow_load(NarrowCodes& r, const SmallArgs& a, int64_t row0, int chunk, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+    const int width = (a.k + 31) & ~31, blocks = width >> 5;
+    const int last = (int)min((int64_t)31, a.rows - 1 - row0);
+    const int second = chunk * 64 + 32 < width ? 1 : 0;
+    const uint8_t* src = static_cast<const uint8_t*>(a.x) + row0 * width + chunk * 64 + t * 8;
+    const uint8_t* scale = a.x_scale + row0 * blocks + chunk * 2;
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int row = min(m * 16 + h * 8 + g, last);
+            const uint8_t *p = src + row * width, *q = scale + row * blocks;
+            r.v[m][h][0] = *reinterpret_cast<const uint2*>(p);
+            r.v[m][h][1] = *reinterpret_cast<const uint2*>(p + second * 32);
+            r.scale[m][h][0] = q[0];
+            r.scale[m][h][1] = q[second];
+        }
+}
+
+// 4 codes as two pairs of float16
+__device__ __forceinline__ void codes_to_half(uint32_t codes, uint32_t& lo, uint32_t& hi) {
+    asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %2;\ncvt.rn.f16x2.e4m3x2 %0, a;\ncvt.rn.f16x2.e4m3x2 %1, b;\n}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(codes));
+}
+
+// Three float16 parts of a pair, rounded: 11 + 11 + 2 and more bits.
+__device__ __forceinline__ void half_parts(float a, float b, uint32_t (&o)[3]) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        union { __half2 h; uint32_t u; } x;
+        x.h = __floats2half2_rn(a, b);
+        o[i] = x.u;
+        a -= __low2float(x.h);
+        b -= __high2float(x.h);
+    }
+}
+
 template <int kXT, int kFragments = NarrowShape<kXT>::kM>
 __device__ __forceinline__ void narrow_load(NarrowRaw<kXT>& r, const SmallArgs& a, int64_t row0, int chunk, int lane) {
     const int g = lane >> 2, ch = chunk * 64 + (lane & 3) * 16;
+    const int pitch = kXT == kX8 ? (a.k + 31) & ~31 : a.k;
+    const int last = (int)min((int64_t)(16 * kFragments - 1), a.rows - 1 - row0);
+    constexpr int kSize = kXT == kX8 ? 1 : kXT == kXFloat ? 4 : 2;
+    constexpr int kPer = 16 / kSize;   // elements of a 16-byte load
+    const char* src = static_cast<const char*>(a.x) + row0 * pitch * kSize;
 #pragma unroll
     for (int m = 0; m < kFragments; ++m)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const int64_t row = row0 + m * 16 + h * 8 + g;
-            const bool live = row < a.rows;
-#pragma unroll
-            for (int i = 0; i < NarrowShape<kXT>::kRaw; ++i) r.v[m][h][i] = make_uint4(0, 0, 0, 0);
+            const int row = min(m * 16 + h * 8 + g, last);
+            const char* p = src + (int64_t)row * pitch * kSize;
             if (kXT == kX8) {
-                const int width = (a.k + 31) / 32 * 32;
-                r.scale[m][h] = 127;
-                if (live && ch < width) {
-                    const int64_t at = row * width + ch;
-                    r.v[m][h][0] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.x) + at);
-                    r.scale[m][h] = a.x_scale[at >> 5];
+                const int c = ch < pitch ? ch : 0;
+                r.v[m][h][0] = *reinterpret_cast<const uint4*>(p + c);
+                r.scale[m][h] = a.x_scale[(row0 + row) * (pitch >> 5) + (c >> 5)];
+            } else if (a.vec_x) {
+#pragma unroll
+                for (int i = 0; i < NarrowShape<kXT>::kRaw; ++i) {
+                    const int c = ch + i * kPer;
+                    r.v[m][h][i] = *reinterpret_cast<const uint4*>(p + (c < a.k ? c : 0) * kSize);
                 }
-                continue;
-            }
-            constexpr int kPer = kXT == kXFloat ? 4 : 8;   // elements of a 16-byte load
+            } else {
 #pragma unroll
-            for (int i = 0; i < NarrowShape<kXT>::kRaw; ++i) {
-                const int c = ch + i * kPer;
-                if (!live || c >= a.k) continue;
-                if (a.vec_x) {
-                    r.v[m][h][i] = kXT == kXFloat
-                        ? *reinterpret_cast<const uint4*>(static_cast<const float*>(a.x) + row * a.k + c)
-                        : *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.x) + row * a.k + c);
-                } else if (kXT == kXFloat) {
-                    union { uint4 u; float f[4]; } o;
+                for (int i = 0; i < NarrowShape<kXT>::kRaw; ++i) {
+                    union { uint4 u; uint32_t w[4]; uint16_t f[8]; } o;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) o.f[j] = c + j < a.k ? static_cast<const float*>(a.x)[row * a.k + c + j] : 0.f;
-                    r.v[m][h][i] = o.u;
-                } else {
-                    union { uint4 u; uint16_t f[8]; } o;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) o.f[j] = c + j < a.k ? static_cast<const uint16_t*>(a.x)[row * a.k + c + j] : 0;
+                    for (int j = 0; j < kPer; ++j) {
+                        const int c = ch + i * kPer + j, at = c < a.k ? c : 0;
+                        if (kXT == kXFloat) o.w[j & 3] = reinterpret_cast<const uint32_t*>(p)[at];
+                        else o.f[j & 7] = reinterpret_cast<const uint16_t*>(p)[at];
+                    }
                     r.v[m][h][i] = o.u;
                 }
             }
         }
+}
+
+// Zeros in place of what lies behind the last channel (narrow_load reads
+// channel 0 there): when the values are used, so that no load is waited for.
+template <int kXT, int kFragments = NarrowShape<kXT>::kM>
+__device__ __forceinline__ void narrow_mask(NarrowRaw<kXT>& r, int k, int chunk, int lane) {
+    if (chunk * 64 + 64 <= k) return;
+    const int left = k - chunk * 64 - (lane & 3) * 16;
+#pragma unroll
+    for (int m = 0; m < kFragments; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < NarrowShape<kXT>::kRaw; ++i) {
+                union { uint4 u; uint32_t w[4]; } o;
+                o.u = r.v[m][h][i];
+                constexpr int kPer = kXT == kX8 ? 4 : kXT == kXFloat ? 1 : 2;   // elements of a word
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int n = left - (i * 4 + j) * kPer;   // that are there
+                    if (n <= 0) o.w[j] = 0;
+                    else if (kPer == 2 && n == 1) o.w[j] &= 0xffff;   // 8-bit rows hold zeros there
+                }
+                r.v[m][h][i] = o.u;
+            }
 }
 
 // The operand registers of step s (4 of the lane's 16 channels), part p of kPA.
@@ -145,16 +226,7 @@ template <int kXT, int kPA>
 __device__ __forceinline__ void narrow_operand(const NarrowRaw<kXT>& r, int m, int s, uint32_t (&o)[kPA][4]) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        if (kXT == kX8) {
-            const uint4& q = r.v[m][h][0];
-            float f[4];
-            values4(f, s == 0 ? q.x : s == 1 ? q.y : s == 2 ? q.z : q.w, scale_of(r.scale[m][h]));
-            union { __nv_bfloat162 b; uint32_t u; } lo, hi;   // exact
-            lo.b = __floats2bfloat162_rn(f[0], f[1]);
-            hi.b = __floats2bfloat162_rn(f[2], f[3]);
-            o[0][h] = lo.u;
-            o[0][2 + h] = hi.u;
-        } else if (kXT == kXFloat) {
+        if (kXT == kXFloat) {
             const uint4& q = r.v[m][h][s];
             uint32_t lo[3], hi[3];
             split3_pair(__uint_as_float(q.x), __uint_as_float(q.y), lo);
@@ -172,26 +244,66 @@ __device__ __forceinline__ void narrow_operand(const NarrowRaw<kXT>& r, int m, i
     }
 }
 
-// Stores columns [c0, c0 + w) of `rows` staged rows to a tensor of w columns
-// whose rows they are: one run of rows x w elements.
-__device__ __forceinline__ void narrow_run(const float* st, void* dst, int dtype, int64_t row0, int rows, int c0, int w,
-                                           const void* add, int lane) {
-    const unsigned inv = 65536u / (unsigned)w + 1;   // t / w for t < 1024, w <= 32
-    for (int t = lane; t < rows * w; t += 32) {
-        const int r = (int)((t * inv) >> 16), c = t - r * w;
-        float v = st[r * kNarrowPitch + c0 + c];
-        if (add) v += load_param(add, dtype, row0 * w + t);
-        store_param(dst, dtype, row0 * w + t, v);
+// Copies a run of `count` staged values to elements at.. of a tensor, `add`'s
+// elements added: 16 bytes a lane where the run starts on a 16-byte boundary.
+template <typename T>
+__device__ __forceinline__ void narrow_copy_as(const float* st, T* dst, int count, const T* add, bool vec, int lane) {
+    constexpr int kPer = 16 / sizeof(T);
+    int done = 0;
+    if (vec) {
+        for (int t = lane * kPer; t + kPer <= count; t += 32 * kPer) {
+            float v[kPer];
+#pragma unroll
+            for (int i = 0; i < kPer; i += 4) *reinterpret_cast<float4*>(v + i) = *reinterpret_cast<const float4*>(st + t + i);
+            union { uint4 u; T e[kPer]; } o;
+            if (add) {
+                o.u = *reinterpret_cast<const uint4*>(add + t);
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) v[i] += to_f32(o.e[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) o.e[i] = from_f32<T>(v[i]);
+            *reinterpret_cast<uint4*>(dst + t) = o.u;
+        }
+        done = count / kPer * kPer;
     }
+    for (int t = done + lane; t < count; t += 32) dst[t] = from_f32<T>(st[t] + (add ? to_f32(add[t]) : 0.f));
 }
+
+__device__ __forceinline__ void narrow_copy(const float* st, void* dst, int dtype, int64_t at, int count, const void* add,
+                                            bool vec, int lane) {
+    if (dtype == PLATTICE_F32)
+        narrow_copy_as(st, static_cast<float*>(dst) + at, count, add ? static_cast<const float*>(add) + at : nullptr, vec, lane);
+    else if (dtype == PLATTICE_BF16)
+        narrow_copy_as(st, static_cast<__nv_bfloat16*>(dst) + at, count,
+                       add ? static_cast<const __nv_bfloat16*>(add) + at : nullptr, vec, lane);
+    else
+        narrow_copy_as(st, static_cast<__half*>(dst) + at, count, add ? static_cast<const __half*>(add) + at : nullptr, vec,
+                       lane);
+}
+
+template <int kXT> struct NarrowLoad { typedef NarrowRaw<kXT> type; };
+template <> struct NarrowLoad<kX8> { typedef NarrowCodes type; };
+template <int kXT>
+__device__ __forceinline__ void narrow_fetch(NarrowRaw<kXT>& r, const SmallArgs& a, int64_t row0, int chunk, int lane) {
+    narrow_load<kXT>(r, a, row0, chunk, lane);
+}
+__device__ __forceinline__ void narrow_fetch(NarrowCodes& r, const SmallArgs& a, int64_t row0, int chunk, int lane) {
+    narrow_load(r, a, row0, chunk, lane);
+}
+__device__ __forceinline__ float lane_finite(float v) { return is_infinite(fabsf(v)) ? 0.f : fmaxf(fabsf(v), 0.f); }
 
 // kSplit: few rows and many channels: the CTA's warps take turns over the
 // channels of the same rows and their sums are added in shared memory, in order.
-template <int kXT, int kNF, bool kW3, bool kSplit>
-__global__ void __launch_bounds__(32 * kNarrowWarps, 2) k_narrow(const SmallArgs a) {
+// kPlain: float32 results without activation, residual and kept z, as the
+// filter takes them: none of those is asked for at every block of rows.
+template <int kXT, int kNF, bool kW3, bool kSplit, bool kPlain>
+__global__ void __launch_bounds__(32 * kNarrowWarps, narrow_ctas(kXT, kNF)) k_narrow(const SmallArgs a) {
     constexpr int kM = NarrowShape<kXT>::kM, kPA = kXT == kXFloat ? 3 : 1, kPB = kW3 ? 3 : 1;
     extern __shared__ __align__(16) char smem_raw[];
     __shared__ float sbias[32];
+    __shared__ float column[32];   // 8-bit rows: the power of two that undoes a channel's
+    typedef typename NarrowLoad<kXT>::type Raw;
     const int steps = narrow_steps(a.k), chunks = steps / 4;
     uint2* frag = reinterpret_cast<uint2*>(smem_raw);   // [kPB][steps][kNF][32]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -199,15 +311,34 @@ __global__ void __launch_bounds__(32 * kNarrowWarps, 2) k_narrow(const SmallArgs
 
     if (threadIdx.x < 32)
         sbias[threadIdx.x] = a.bias && (int)threadIdx.x < a.n ? load_param(a.bias, a.bias_dtype, threadIdx.x) : 0.f;
+    if (kXT == kX8) {
+        for (int c = warp; c < 32; c += kNarrowWarps) {
+            float most = 0.f;
+            if (c < a.n)
+                for (int ch = lane; ch < a.k; ch += 32) most = fmaxf(most, lane_finite(load_param(a.w, a.w_dtype, (int64_t)c * a.k + ch)));
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+            const int e = min(max((__float_as_int(most) >> 23) - 127 - 14, -120), 120);
+            if (lane == 0) column[c] = pow2(e);
+        }
+        __syncthreads();
+    }
     for (int i = threadIdx.x; i < steps * kNF * 32; i += blockDim.x) {
         const int l = i & 31, f = (i >> 5) % kNF, s = (i >> 5) / kNF;
-        const int col = f * 8 + (l >> 2), ch = (s >> 2) * 64 + (l & 3) * 16 + (s & 3) * 4;
+        const int col = f * 8 + (l >> 2);
+        const int ch = (s >> 2) * 64 + (kXT == kX8 ? ((s >> 1) & 1) * 32 + (l & 3) * 8 + (s & 1) * 4 : (l & 3) * 16 + (s & 3) * 4);
         float v[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             v[j] = col < a.n && ch + j < a.k ? load_param(a.w, a.w_dtype, (int64_t)col * a.k + ch + j) : 0.f;
         uint32_t lo[3], hi[3];
-        if (kW3) {
+        if (kXT == kX8) {
+            const float up = 1.f / column[col];   // a power of two
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] *= up;
+            half_parts(v[0], v[1], lo);
+            half_parts(v[2], v[3], hi);
+        } else if (kW3) {
             split3_pair(v[0], v[1], lo);
             split3_pair(v[2], v[3], hi);
         } else if (kXT == kXHalf) {
@@ -233,8 +364,24 @@ __global__ void __launch_bounds__(32 * kNarrowWarps, 2) k_narrow(const SmallArgs
     int64_t block = kSplit ? blockIdx.x : (int64_t)blockIdx.x * kNarrowWarps + warp;
     const int chunk0 = kSplit ? warp : 0, chunk_step = kSplit ? kNarrowWarps : 1;
 
-    NarrowRaw<kXT> next;
-    if (block < blocks && chunk0 < chunks) narrow_load<kXT>(next, a, block * (16 * kM), chunk0, lane);
+    // where a lane's columns go in the staged output: the rows of y0 one after
+    // the other, then y1's (a split), each as it will lie in memory
+    const int w0 = a.split ? a.split : a.n, w1 = a.n - w0;
+    int put[kNF][2], width[kNF][2];
+#pragma unroll
+    for (int f = 0; f < kNF; ++f)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int c = f * 8 + t * 2 + i;
+            width[f][i] = c < w0 ? w0 : w1;
+            put[f][i] = c < w0 ? c : c < a.n ? 16 * kM * w0 + c - w0 : -1;
+        }
+    uint64_t undo[kNF];
+#pragma unroll
+    for (int f = 0; f < kNF; ++f) undo[f] = kXT == kX8 ? pair_of(column[f * 8 + t * 2], column[f * 8 + t * 2 + 1]) : 0;
+
+    Raw next;
+    if (block < blocks && chunk0 < chunks) narrow_fetch(next, a, block * (16 * kM), chunk0, lane);
     for (; block < blocks; block += stride) {
         const int64_t row0 = block * (16 * kM);
         float acc[kM][kNF][4];
@@ -245,9 +392,55 @@ __global__ void __launch_bounds__(32 * kNarrowWarps, 2) k_narrow(const SmallArgs
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc[m][f][i] = 0.f;
         for (int c = chunk0; c < chunks; c += chunk_step) {
-            const NarrowRaw<kXT> raw = next;
-            if (c + chunk_step < chunks) narrow_load<kXT>(next, a, row0, c + chunk_step, lane);
-            else if (block + stride < blocks) narrow_load<kXT>(next, a, row0 + stride * (16 * kM), chunk0, lane);
+            Raw raw = next;
+            const bool more = c + chunk_step < chunks;   // of this block; else the next block's first
+            if (more || block + stride < blocks)
+                narrow_fetch(next, a, more ? row0 : row0 + stride * (16 * kM), more ? c + chunk_step : chunk0, lane);
+            if constexpr (kXT == kX8) {
+#pragma unroll
+                for (int blk = 0; blk < 2; ++blk) {
+                    if (blk && c * 64 + 32 >= a.k) break;   // no second block of 32 channels here
+                    float sum[kM][kNF][4];
+#pragma unroll
+                    for (int m = 0; m < kM; ++m)
+#pragma unroll
+                        for (int f = 0; f < kNF; ++f)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) sum[m][f][i] = 0.f;
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) {
+                        uint32_t o[kM][4];
+#pragma unroll
+                        for (int m = 0; m < kM; ++m)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h)
+                                codes_to_half(s ? raw.v[m][h][blk].y : raw.v[m][h][blk].x, o[m][h], o[m][2 + h]);
+#pragma unroll
+                        for (int p = kPB - 1; p >= 0; --p)   // small parts first
+#pragma unroll
+                            for (int f = 0; f < kNF; ++f) {
+                                const uint2 b = frag[((p * steps + c * 4 + blk * 2 + s) * kNF + f) * 32 + lane];
+#pragma unroll
+                                for (int m = 0; m < kM; ++m) mma16816<true>(sum[m][f], o[m][0], o[m][1], o[m][2], o[m][3], b);
+                            }
+                    }
+#pragma unroll
+                    for (int m = 0; m < kM; ++m)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const uint64_t sc = both(scale_of(raw.scale[m][h][blk]));
+#pragma unroll
+                            for (int f = 0; f < kNF; ++f) {
+                                // the channel's power first: neither product leaves float32's range by itself
+                                const uint64_t v = mul2(pair_of(sum[m][f][2 * h], sum[m][f][2 * h + 1]), undo[f]);
+                                pair_to(fma2(v, sc, pair_of(acc[m][f][2 * h], acc[m][f][2 * h + 1])), acc[m][f][2 * h],
+                                        acc[m][f][2 * h + 1]);
+                            }
+                        }
+                }
+                continue;
+            } else {
+            narrow_mask<kXT>(raw, a.k, c, lane);
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
                 uint2 b[kPB][kNF];
@@ -270,6 +463,7 @@ __global__ void __launch_bounds__(32 * kNarrowWarps, 2) k_narrow(const SmallArgs
                                 mma16816<kXT == kXHalf>(acc[m][f], o[pa][0], o[pa][1], o[pa][2], o[pa][3], b[pb][f]);
                         }
                 }
+            }
             }
         }
         const int rows = (int)min((int64_t)(16 * kM), a.rows - row0);
@@ -297,49 +491,63 @@ __global__ void __launch_bounds__(32 * kNarrowWarps, 2) k_narrow(const SmallArgs
                         acc[m][f][i] = v;
                     }
         }
-        const bool keep = a.z != nullptr;
-        for (int pass = keep ? 0 : 1; pass < 2; ++pass) {   // z, then y
+#pragma unroll
+        for (int m = 0; m < kM; ++m)
+#pragma unroll
+            for (int f = 0; f < kNF; ++f)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[m][f][i] += sbias[f * 8 + t * 2 + (i & 1)];
+        if (!kPlain && a.z_scale) {   // the whole row is one block; 16 columns a lane
+            __syncwarp();
+#pragma unroll
+            for (int m = 0; m < kM; ++m)
+#pragma unroll
+                for (int f = 0; f < kNF; ++f)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        st[(m * 16 + (i >> 1) * 8 + g) * kNarrowPitch + f * 8 + t * 2 + (i & 1)] = acc[m][f][i];
+            __syncwarp();
+#pragma unroll
+            for (int m = 0; m < kM; ++m) {
+                const int r = m * 16 + (lane >> 1), c0 = (lane & 1) * 16;
+                float v[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) v[i] = c0 + i < kNF * 8 ? st[r * kNarrowPitch + c0 + i] : 0.f;
+                bool infinite;
+                float amax = finite_amax_of(v, infinite);
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+                const int e = block_exponent(amax);
+                if (r < rows) {
+                    const float inv = pow2(-e);
+                    const uint2 x = codes8_of(v, inv, infinite), y = codes8_of(v + 8, inv, infinite);
+                    reinterpret_cast<uint4*>(a.z)[(row0 + r) * 2 + (lane & 1)] = make_uint4(x.x, x.y, y.x, y.y);
+                    if ((lane & 1) == 0) a.z_scale[row0 + r] = (uint8_t)(e + 127);
+                }
+            }
+        }
+        const bool full_z = !kPlain && a.z && !a.z_scale;
+        for (int pass = full_z ? 0 : 1; pass < 2; ++pass) {   // a kept z, then y
             __syncwarp();
 #pragma unroll
             for (int m = 0; m < kM; ++m)
 #pragma unroll
                 for (int f = 0; f < kNF; ++f) {
-                    if (pass == 0 || !keep) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) acc[m][f][i] += sbias[f * 8 + t * 2 + (i & 1)];
-                    }
-                    if (pass == 1) activate(acc[m][f], a.act);
+                    if (!kPlain && pass == 1) activate(acc[m][f], a.act);
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        st[(m * 16 + (i >> 1) * 8 + g) * kNarrowPitch + f * 8 + t * 2 + (i & 1)] = acc[m][f][i];
+                        if (put[f][i & 1] >= 0) st[(m * 16 + (i >> 1) * 8 + g) * width[f][i & 1] + put[f][i & 1]] = acc[m][f][i];
                 }
             __syncwarp();
-            if (pass == 0 && a.z_scale) {   // the whole row is one block; 16 columns a lane
-#pragma unroll
-                for (int m = 0; m < kM; ++m) {
-                    const int r = m * 16 + (lane >> 1), c0 = (lane & 1) * 16;
-                    float v[16];
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        v[i] = c0 + i < kNF * 8 ? st[r * kNarrowPitch + c0 + i] : 0.f;
-                    bool infinite;
-                    float amax = finite_amax_of(v, infinite);
-                    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-                    const int e = block_exponent(amax);
-                    if (r < rows) {
-                        const float inv = pow2(-e);
-                        const uint2 x = codes8_of(v, inv, infinite), y = codes8_of(v + 8, inv, infinite);
-                        reinterpret_cast<uint4*>(a.z)[(row0 + r) * 2 + (lane & 1)] = make_uint4(x.x, x.y, y.x, y.y);
-                        if ((lane & 1) == 0) a.z_scale[row0 + r] = (uint8_t)(e + 127);
-                    }
-                }
+            if (kPlain) {
+                narrow_copy_as<float>(st, static_cast<float*>(a.y0) + row0 * w0, rows * w0, nullptr, a.vec_y, lane);
+                if (a.split)
+                    narrow_copy_as<float>(st + 16 * kM * w0, static_cast<float*>(a.y1) + row0 * w1, rows * w1, nullptr,
+                                          a.vec_y, lane);
             } else if (pass == 0) {
-                narrow_run(st, a.z, a.out_dtype, row0, rows, 0, a.n, nullptr, lane);
-            } else if (a.split) {
-                narrow_run(st, a.y0, a.out_dtype, row0, rows, 0, a.split, nullptr, lane);
-                narrow_run(st, a.y1, a.out_dtype, row0, rows, a.split, a.n - a.split, nullptr, lane);
+                narrow_copy(st, a.z, a.out_dtype, row0 * a.n, rows * a.n, nullptr, a.vec_y, lane);
             } else {
-                narrow_run(st, a.y0, a.out_dtype, row0, rows, 0, a.n, a.residual, lane);
+                narrow_copy(st, a.y0, a.out_dtype, row0 * w0, rows * w0, a.residual, a.vec_y, lane);
+                if (a.split) narrow_copy(st + 16 * kM * w0, a.y1, a.out_dtype, row0 * w1, rows * w1, nullptr, a.vec_y, lane);
             }
         }
     }
@@ -392,43 +600,19 @@ __device__ __forceinline__ void to_parts(float a, float b, bool half, uint32_t (
     }
 }
 
-// Element e of the 16 rows' gradients, g0's run first, then g1's: its place
-// (row, column) and value.
-struct GradRun {
-    const void *g0, *g1;
-    int dtype, w0, w1, rows;
-    unsigned inv0, inv1;
-    int64_t row0;
-    __device__ __forceinline__ GradRun(const SmallGradArgs& a, int64_t row0_)
-        : g0(a.g0), g1(a.g1), dtype(a.s.out_dtype), w0(a.s.split ? a.s.split : a.s.n), w1(a.s.split ? a.s.n - a.s.split : 1),
-          rows((int)min((int64_t)16, a.s.rows - row0_)), row0(row0_) {
-        inv0 = 65536u / (unsigned)w0 + 1;   // t / w for t < 1024, w <= 32
-        inv1 = 65536u / (unsigned)w1 + 1;
-        if (!a.s.split) w1 = 0;
-    }
-    __device__ __forceinline__ float value(int e) const {
-        if (e < rows * w0) return load_param(g0, dtype, row0 * w0 + e);
-        e -= rows * w0;
-        return e < rows * w1 ? load_param(g1, dtype, row0 * w1 + e) : 0.f;
-    }
-    // offset in the staged rows, -1 behind the end
-    __device__ __forceinline__ int place(int e) const {
-        if (e < rows * w0) {
-            const int r = (int)((e * inv0) >> 16);
-            return r * kNarrowPitch + e - r * w0;
-        }
-        e -= rows * w0;
-        if (e >= rows * w1) return -1;
-        const int r = (int)((e * inv1) >> 16);
-        return r * kNarrowPitch + w0 + e - r * w1;
-    }
-};
+template <int kXT, bool kG32> struct GradType { typedef __nv_bfloat16 type; };
+template <int kXT> struct GradType<kXT, true> { typedef float type; };
+template <> struct GradType<kXHalf, false> { typedef __half type; };
 
 // kXT: the type of x (and, for 16-bit ones, of everything); kParts: 3 with
 // float32 weights; kNF: output channels / 8.
-template <int kXT, int kParts, int kNF>
-__global__ void __launch_bounds__(32 * kGradWarps, kParts == 3 ? 2 : 3) k_narrow_grad(const SmallGradArgs a) {
+__host__ __device__ constexpr int narrow_grad_ctas(int parts, int nf) { return parts == 3 ? 2 : nf > 2 ? 3 : 4; }
+
+// kG32: float32 gradients beside 16-bit operands.
+template <int kXT, int kParts, int kNF, bool kG32>
+__global__ void __launch_bounds__(32 * kGradWarps, narrow_grad_ctas(kParts, kNF)) k_narrow_grad(const SmallGradArgs a) {
     typedef NarrowGradShape<kXT, kParts> Shape;
+    typedef typename GradType<kXT, kG32>::type TG;
     constexpr int kPX = Shape::kPX, kKS = kNF > 2 ? 2 : 1;   // steps of 16 output channels in grad_x's sum
     constexpr bool kHalf = kXT == kXHalf;
     extern __shared__ __align__(16) char smem_raw[];
@@ -473,57 +657,56 @@ __global__ void __launch_bounds__(32 * kGradWarps, kParts == 3 ? 2 : 3) k_narrow
     const int64_t blocks = (a.s.rows + 15) / 16, stride = (int64_t)gridDim.x * kGradWarps;
     int64_t block = (int64_t)blockIdx.x * kGradWarps + warp;
     constexpr int kRun = kNF * 4;   // 16 rows x 8 kNF columns / 32 lanes
-    float gn[kRun];                 // the next rows' gradients, x and z, loaded ahead
-    uint4 xn[2][NarrowShape<kXT>::kRaw];
-    uint8_t xs[2];
+    // Element e = 32 i + lane of the rows' gradients: the run of g0's 16 rows,
+    // then g1's; where it goes in the staged rows, the same for every 16 rows.
+    const int w0 = a.s.split ? a.s.split : n, w1 = n - w0, run0 = 16 * w0;
+    uint16_t place[kRun];
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+        const int e = i * 32 + lane;
+        place[i] = 0xffff;
+        if (e < run0) place[i] = (uint16_t)(e / w0 * kNarrowPitch + e % w0);
+        else if (e < 16 * n) place[i] = (uint16_t)((e - run0) / w1 * kNarrowPitch + w0 + (e - run0) % w1);
+    }
+    TG gn[kRun];                    // the next rows' gradients, x and z, loaded ahead
+    NarrowRaw<kXT> xn;
     uint4 zn = make_uint4(0, 0, 0, 0);
     uint8_t zs = 127;
     auto load_rows = [&](int64_t b) {
-        const GradRun run(a, b * 16);
+        const TG* p0 = static_cast<const TG*>(a.g0) + b * 16 * w0 + lane;
+        const TG* p1 = static_cast<const TG*>(a.g1) + b * 16 * w1 + lane - run0;
+        const int limit = (int)min((int64_t)16, a.s.rows - b * 16) * kNarrowPitch;
 #pragma unroll
-        for (int i = 0; i < kRun; ++i) gn[i] = run.value(i * 32 + lane);
+        for (int i = 0; i < kRun; ++i)
+            gn[i] = *(place[i] < limit ? (i * 32 + lane < run0 ? p0 : p1) + i * 32 : p0 - lane);
         if (a.s.z_scale) {   // a lane per half row
-            const int64_t row = b * 16 + (lane >> 1);
-            const bool live = row < a.s.rows;
-            zn = live ? reinterpret_cast<const uint4*>(a.s.z)[row * 2 + (lane & 1)] : make_uint4(0, 0, 0, 0);
-            zs = live ? a.s.z_scale[row] : 127;
+            const int64_t row = min(b * 16 + (lane >> 1), a.s.rows - 1);   // behind the last: its own, times 0
+            zn = reinterpret_cast<const uint4*>(a.s.z)[row * 2 + (lane & 1)];
+            zs = a.s.z_scale[row];
         }
         if (!a.need_w) return;
-        NarrowRaw<kXT> r;
-        narrow_load<kXT, 1>(r, a.s, b * 16, blockIdx.y, lane);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-            for (int i = 0; i < NarrowShape<kXT>::kRaw; ++i) xn[h][i] = r.v[0][h][i];
-            if (kXT == kX8) xs[h] = r.scale[0][h];
-        }
+        narrow_load<kXT, 1>(xn, a.s, b * 16, blockIdx.y, lane);
     };
     if (block < blocks) load_rows(block);
     for (; block < blocks; block += stride) {
         const int64_t row0 = block * 16;
         const int rows = (int)min((int64_t)16, a.s.rows - row0);
         __syncwarp();
-        {
-            const GradRun run(a, row0);
 #pragma unroll
-            for (int i = 0; i < kRun; ++i) {
-                const int at = run.place(i * 32 + lane);
-                if (at >= 0) st[at] = gn[i];
-            }
-        }
-        if (rows < 16)
-            for (int i = rows * kNarrowPitch + lane; i < 16 * kNarrowPitch; i += 32) st[i] = 0.f;
+        for (int i = 0; i < kRun; ++i)   // 0 behind the last row
+            if (place[i] != 0xffff) st[place[i]] = place[i] < rows * kNarrowPitch ? to_f32(gn[i]) : 0.f;
         if (a.need_w) {   // x, widened, into the tile
+            narrow_mask<kXT, 1>(xn, k, blockIdx.y, lane);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 uint16_t* row = tile + (g + 8 * h) * kTilePitch + t * 16;
                 if (kXT == kX8) {
                     float v[16];
-                    const float sc = scale_of(xs[h]);
-                    values4(v, xn[h][0].x, sc);
-                    values4(v + 4, xn[h][0].y, sc);
-                    values4(v + 8, xn[h][0].z, sc);
-                    values4(v + 12, xn[h][0].w, sc);
+                    const float sc = scale_of(xn.scale[0][h]);
+                    values4(v, xn.v[0][h][0].x, sc);
+                    values4(v + 4, xn.v[0][h][0].y, sc);
+                    values4(v + 8, xn.v[0][h][0].z, sc);
+                    values4(v + 12, xn.v[0][h][0].w, sc);
                     union { uint4 u[2]; __nv_bfloat162 b[8]; } o;   // exact
 #pragma unroll
                     for (int i = 0; i < 8; ++i) o.b[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
@@ -532,7 +715,7 @@ __global__ void __launch_bounds__(32 * kGradWarps, kParts == 3 ? 2 : 3) k_narrow
                 } else if (kXT == kXFloat) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const uint4& q = xn[h][i % NarrowShape<kXT>::kRaw];
+                        const uint4& q = xn.v[0][h][i % NarrowShape<kXT>::kRaw];
                         uint32_t lo[3], hi[3];
                         split3_pair(__uint_as_float(q.x), __uint_as_float(q.y), lo);
                         split3_pair(__uint_as_float(q.z), __uint_as_float(q.w), hi);
@@ -541,8 +724,8 @@ __global__ void __launch_bounds__(32 * kGradWarps, kParts == 3 ? 2 : 3) k_narrow
                             *reinterpret_cast<uint2*>(row + (p % kPX) * 16 * kTilePitch + i * 4) = make_uint2(lo[p], hi[p]);
                     }
                 } else {
-                    reinterpret_cast<uint4*>(row)[0] = xn[h][0];
-                    reinterpret_cast<uint4*>(row)[1] = xn[h][1 % NarrowShape<kXT>::kRaw];
+                    reinterpret_cast<uint4*>(row)[0] = xn.v[0][h][0];
+                    reinterpret_cast<uint4*>(row)[1] = xn.v[0][h][1 % NarrowShape<kXT>::kRaw];
                 }
             }
         }
