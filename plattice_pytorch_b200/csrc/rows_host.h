@@ -4,9 +4,58 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <cuda.h>
+
 #include "../../include/plattice.h"
 
 namespace plr {
+
+// ------------------------------------------------- products on the tensor cores
+// (rows_mma.cuh has the kernel and what the kinds and their operands are)
+
+enum Kind { kForward = 0, kGradX = 1, kGradW = 2 };
+
+constexpr int kBM = 128, kBK = 64;   // rows of a tile, depth of a slice of the sum
+
+// A 16-bit operand [parts][rows][pitch] of `width` columns.
+struct Operand {
+    const void* p = nullptr;
+    int64_t rows = 0, width = 0, pitch = 0;
+    int parts = 1;
+};
+
+struct MmaArgs {
+    // result
+    void* y0;
+    void* y1;             // split: columns split.. of D
+    const void* bias;     // null: none
+    const void* residual;
+    void* z;              // kept pre-activation (null: none)
+    uint8_t* z_scale;
+    int64_t ni, nj;       // D is ni x nj
+    int bias_dtype, out_dtype, act, split;
+    // sum
+    int steps;            // 64-deep slices of r
+    int part_steps;       // of a part (kGradW); parts are numbered tile-slowest
+    int parts;
+    unsigned pairs_a, pairs_b;   // parts of A and B of each product, 2 bits each
+    int pairs;
+    bool half;            // operands are float16 (else bfloat16)
+    unsigned* fault;      // host-mapped word that reports a wait that gave up (may be null)
+};
+
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+inline int64_t mma_tiles(int64_t ni, int64_t nj, int bn) { return ceil_div(ni, kBM) * ceil_div(nj, bn); }
+
+// TMA map of an operand: boxes of 64 columns x box_rows rows, zeros outside.
+cudaError_t make_map(CUtensorMap* m, const Operand& o, int box_rows);
+
+// Products with tiles of bn columns (256, 128, 64; the forward also 32).
+// aligned: rows of the result (the forward: of y0, residual and z) allow
+// 16-byte accesses.
+cudaError_t mma_forward(int bn, bool aligned, const Operand& x, const Operand& w, const MmaArgs& p, cudaStream_t s);
+cudaError_t mma_grad_x(int bn, bool aligned, const Operand& gz, const Operand& w, const MmaArgs& p, cudaStream_t s);
+cudaError_t mma_grad_w(int bn, const Operand& x, const Operand& gz, const MmaArgs& p, cudaStream_t s);
 
 // Status code of a CUDA result; an error is noted for
 // plattice_last_error_detail under the call's name.
@@ -18,6 +67,8 @@ int rows_poll(const char* call);
 
 // SMs of the current device (148 when it cannot be asked).
 int sm_count();
+
+constexpr int kMaxSmem = 232448;   // shared memory a CTA can have
 
 inline bool dtype_ok(int d) { return d == PLATTICE_F32 || d == PLATTICE_BF16 || d == PLATTICE_F16; }
 inline size_t dtype_size(int d) { return d == PLATTICE_F32 ? 4 : 2; }

@@ -6,8 +6,8 @@
 #include "plattice_runtime.h"
 #include "rows_common.cuh"
 #include "rows_host.h"
-#include "rows_mma.cuh"
-#include "rows_narrow.cuh"
+#include "rows_narrow.h"
+#include "rows_split.cuh"
 
 namespace plr {
 
@@ -209,7 +209,6 @@ __global__ void __launch_bounds__(256) k_add_parts(T* __restrict__ out, const fl
 
 static int64_t up256(int64_t n) { return (n + 255) & ~255ll; }
 static int64_t up8(int64_t n) { return (n + 7) & ~7ll; }
-static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Buffers of a call, one after the other in its workspace.
 struct Carve {
@@ -233,6 +232,9 @@ static bool linear_shape_ok(const plattice_linear_args* a) {
     return fits(a->rows, width8(a->k)) && fits(a->rows, width8(a->n)) && fits(a->k, a->n);
 }
 
+// Parts summed: few results over the warps of a CTA (a thread each would add
+// hundreds of parts one after the other: 7.8 against 3.5 us for 64 x 64 and
+// 296 parts), many by a thread each.
 template <typename T>
 static cudaError_t add_parts(void* out, const float* partial, int parts, int64_t n, cudaStream_t s) {
     k_add_parts<T><<<(unsigned)ceil_div(n, 256), 256, 0, s>>>(static_cast<T*>(out), partial, parts, n);
@@ -240,19 +242,16 @@ static cudaError_t add_parts(void* out, const float* partial, int parts, int64_t
 }
 
 static cudaError_t add_parts_to(void* out, int dtype, const float* partial, int parts, int64_t n, cudaStream_t s) {
+    if (parts > 8 && n <= 8192) {
+        k_sum_lines<<<(unsigned)ceil_div(n, 32), 1024, 0, s>>>(out, dtype, n, nullptr, dtype, 0, partial, parts);
+        return cudaGetLastError();
+    }
     if (dtype == PLATTICE_F32) return add_parts<float>(out, partial, parts, n, s);
     if (dtype == PLATTICE_BF16) return add_parts<__nv_bfloat16>(out, partial, parts, n, s);
     return add_parts<__half>(out, partial, parts, n, s);
 }
 
 // ---- products on the tensor cores
-
-// A 16-bit operand [parts][rows][pitch] of `width` columns.
-struct Operand {
-    const void* p = nullptr;
-    int64_t rows = 0, width = 0, pitch = 0;
-    int parts = 1;
-};
 
 // Whether TMA can read the rows where they are.
 static bool tma_ready(const void* p, int dtype, int64_t width) {
@@ -303,8 +302,7 @@ static EncodeTiled encode_tiled() {
     return f;
 }
 
-// Boxes of 64 columns x `box_rows` rows, zeros outside the operand.
-static cudaError_t make_map(CUtensorMap* m, const Operand& o, int box_rows) {
+cudaError_t make_map(CUtensorMap* m, const Operand& o, int box_rows) {
     const EncodeTiled enc = encode_tiled();
     if (!enc) return cudaErrorNotSupported;
     const cuuint64_t dims[3] = {(cuuint64_t)o.width, (cuuint64_t)o.rows, (cuuint64_t)o.parts};
@@ -319,8 +317,6 @@ static cudaError_t make_map(CUtensorMap* m, const Operand& o, int box_rows) {
 // Cycles of a 64-deep slice of a 128 x bn tile: the MMA itself (512 at 256
 // columns), or below that what staging the operands' slices takes.
 static double slice_cost(int bn) { return bn == 256 ? 512 : bn == 128 ? 300 : bn == 64 ? 220 : 200; }
-
-static int64_t mma_tiles(int64_t ni, int64_t nj, int bn) { return ceil_div(ni, kBM) * ceil_div(nj, bn); }
 
 // Columns of a tile: the cheapest number of rounds over the device's SMs
 // (wide tiles do more per byte staged, narrow ones fill the device when D is
@@ -352,38 +348,6 @@ static int choose_parts(int64_t ni, int64_t nj, int bn, int64_t steps) {
     return best;
 }
 
-template <int kKind, bool kX8, int kBN>
-static cudaError_t launch_mma(const Operand& a, const Operand& b, const MmaArgs& p, cudaStream_t s) {
-    int unused = 0;
-    cudaError_t e = pl::kernel_once(
-        reinterpret_cast<const void*>(k_mma<kKind, kX8, kBN>),
-        [](int*) {
-            return cudaFuncSetAttribute(k_mma<kKind, kX8, kBN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        smem_bytes(kKind, kX8, kBN));
-        },
-        &unused);
-    if (e != cudaSuccess) return e;
-    CUtensorMap ma, mb;
-    if (kX8) memset(&ma, 0, sizeof(ma));
-    else if ((e = make_map(&ma, a, a_mn(kKind) ? kBK : kBM)) != cudaSuccess) return e;
-    if ((e = make_map(&mb, b, b_mn(kKind) ? kBK : kBN)) != cudaSuccess) return e;
-    const int64_t tiles = mma_tiles(p.ni, p.nj, kBN) * p.parts;
-    if (tiles > INT_MAX) return cudaErrorInvalidValue;
-    const int ctas = (int)(tiles < sm_count() ? tiles : sm_count());
-    k_mma<kKind, kX8, kBN><<<ctas, role_threads(kKind, kX8) + (kX8 ? 32 * kConvertWarps : 0), smem_bytes(kKind, kX8, kBN), s>>>(
-        ma, mb, p, (unsigned)tiles);
-    return cudaGetLastError();
-}
-
-template <int kKind, bool kX8>
-static cudaError_t run_mma(int bn, const Operand& a, const Operand& b, const MmaArgs& p, cudaStream_t s) {
-    if (bn == 256) return launch_mma<kKind, kX8, 256>(a, b, p, s);
-    if (bn == 128) return launch_mma<kKind, kX8, 128>(a, b, p, s);
-    if (bn == 64) return launch_mma<kKind, kX8, 64>(a, b, p, s);
-    if constexpr (kKind != kGradX) return launch_mma<kKind, kX8, 32>(a, b, p, s);
-    return cudaErrorInvalidValue;
-}
-
 // The sum's side of the arguments: slices of r and the products of parts.
 static void sum_args(MmaArgs* p, int64_t nr, int parts, int parts_a, int parts_b) {
     p->steps = (int)ceil_div(nr, kBK);
@@ -406,20 +370,6 @@ static cudaError_t unpacked(Operand* o, const plattice_linear_args* a, void* ws,
     return unpack_rows(ws, PLATTICE_BF16, o->pitch, static_cast<const uint8_t*>(a->x), a->x_scale, a->rows, a->k, s);
 }
 
-static void x8_args(MmaArgs* p, const plattice_linear_args* a) {
-    p->q = static_cast<const uint8_t*>(a->x);
-    p->q_scale = a->x_scale;
-    p->q_rows = a->rows;
-    p->q_width = width8(a->k);
-}
-
-// Whether an 8-bit x is unpacked to bfloat16 before the product rather than on
-// its way through it: when several tiles along j would each widen the same
-// slice (the widening and the MMA share the shared memory's bandwidth, so a
-// 256-wide tile then runs at a third of its rate), one pass over x, 5 bytes a
-// value, costs less.
-static bool unpack_first(int n, int bn) { return n > bn; }
-
 // How a forward runs: few rows a warp per output channel, few output channels
 // a warp per rows with the weights in shared memory, else the tiled product.
 // Measured at their borders: see k_few and k_narrow.
@@ -435,7 +385,6 @@ static Way forward_way(const plattice_linear_args* a) {
 
 struct ForwardPlan {
     Way way;
-    bool unpack;
     int bn;
     int64_t x, w, bytes;
 };
@@ -446,9 +395,8 @@ static ForwardPlan forward_plan(const plattice_linear_args* a) {
     p.way = forward_way(a);
     if (p.way == kWayTiles) {
         p.bn = choose_bn(a->rows, a->n, 32);
-        p.unpack = a->x_scale && unpack_first(a->n, p.bn);
-        if (p.unpack) p.x = c.take(a->rows * up8(a->k) * 2);
-        else if (!a->x_scale && !tma_ready(a->x, a->dtype, a->k)) p.x = c.take(repack_bytes(a->dtype, a->rows, a->k));
+        if (a->x_scale) p.x = c.take(a->rows * up8(a->k) * 2);
+        else if (!tma_ready(a->x, a->dtype, a->k)) p.x = c.take(repack_bytes(a->dtype, a->rows, a->k));
         p.w = tma_ready(a->w, a->dtype, a->k) ? 0 : c.take(repack_bytes(a->dtype, a->n, a->k));
     }
     p.bytes = c.at;
@@ -459,7 +407,7 @@ struct BackwardPlan {
     bool narrow;
     int lines;       // narrow: CTAs along the rows
     int64_t line_bytes;
-    bool gz_needed, unpack;
+    bool gz_needed;
     int shift, strips;
     int bn_x, bn_w, parts_b, parts_w;
     int64_t gz, x, w, partial_b, partial_w, pitch, bytes;
@@ -490,11 +438,10 @@ static BackwardPlan backward_plan(const plattice_linear_args* a) {
     p.pitch = up8(a->n);
     if (p.gz_needed) p.gz = c.take(repack_bytes(a->dtype, a->rows, a->n));
     p.bn_x = choose_bn(a->rows, a->k, 64);
-    p.bn_w = a->n > 128 ? 256 : a->n > 64 ? 128 : a->n > 32 ? 64 : 32;
+    p.bn_w = a->n > 128 ? 256 : a->n > 64 ? 128 : 64;
     p.parts_w = choose_parts(a->k, a->n, p.bn_w, ceil_div(a->rows, kBK));
     if (a->grad_x && !tma_ready(a->w, a->dtype, a->k)) p.w = c.take(repack_bytes(a->dtype, a->n, a->k));
-    p.unpack = a->x_scale && unpack_first(a->n, p.bn_w);
-    if (a->grad_w && p.unpack) p.x = c.take(a->rows * up8(a->k) * 2);
+    if (a->grad_w && a->x_scale) p.x = c.take(a->rows * up8(a->k) * 2);
     if (a->grad_w && !a->x_scale && !tma_ready(a->x, a->dtype, a->k))
         p.x = c.take(repack_bytes(a->dtype, a->rows, a->k));
     if (a->grad_w && p.parts_w > 1) p.partial_w = c.take((int64_t)p.parts_w * a->n * a->k * 4);
@@ -509,57 +456,6 @@ static cudaError_t launch_grad_z(const GradArgs& g, const BackwardPlan& p, cudaS
     return cudaGetLastError();
 }
 
-template <int kXT, int kNF, bool kW3, bool kSplit, bool kPlain>
-static cudaError_t launch_narrow(const SmallArgs& a, int64_t blocks, cudaStream_t s) {
-    const int64_t smem = narrow_fragments(a.k, kNF, kW3 ? 3 : 1) + narrow_staging(NarrowShape<kXT>::kM);
-    int unused = 0;
-    const cudaError_t e = pl::kernel_once(
-        reinterpret_cast<const void*>(k_narrow<kXT, kNF, kW3, kSplit, kPlain>),
-        [](int*) {
-            return cudaFuncSetAttribute(k_narrow<kXT, kNF, kW3, kSplit, kPlain>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        (int)(kNarrowMost + narrow_staging(2)));
-        },
-        &unused);
-    if (e != cudaSuccess) return e;
-    // one round of CTAs: as many as are resident at a time
-    const int64_t need = kSplit ? blocks : ceil_div(blocks, kNarrowWarps);
-    const int64_t fit = kMaxSmem / (smem + 1024), ctas = narrow_ctas(kXT, kNF);
-    const int64_t most = (fit < ctas ? fit : ctas) * sm_count();
-    k_narrow<kXT, kNF, kW3, kSplit, kPlain><<<(unsigned)(need < most ? need : most), 32 * kNarrowWarps, smem, s>>>(a);
-    return cudaGetLastError();
-}
-
-template <int kXT, bool kW3, int kNF>
-static cudaError_t run_narrow_as(const SmallArgs& a, cudaStream_t s) {
-    const int64_t blocks = ceil_div(a.rows, 16 * NarrowShape<kXT>::kM);
-    // fewer blocks of rows than a warp on each SM would take: the warps of a
-    // CTA share a block instead (at least two chunks of channels to share)
-    if (blocks <= 2 * (int64_t)sm_count() && a.k > 64) return launch_narrow<kXT, kNF, kW3, true, false>(a, blocks, s);
-    if (a.out_dtype == PLATTICE_F32 && a.act == PLATTICE_ACT_NONE && !a.residual && !a.z)
-        return launch_narrow<kXT, kNF, kW3, false, true>(a, blocks, s);
-    return launch_narrow<kXT, kNF, kW3, false, false>(a, blocks, s);
-}
-
-template <int kXT, bool kW3>
-static cudaError_t run_narrow(const SmallArgs& a, cudaStream_t s) {
-    switch ((a.n + 7) / 8) {
-        case 1: return run_narrow_as<kXT, kW3, 1>(a, s);
-        case 2: return run_narrow_as<kXT, kW3, 2>(a, s);
-        case 3: return run_narrow_as<kXT, kW3, 3>(a, s);
-        default: return run_narrow_as<kXT, kW3, 4>(a, s);
-    }
-}
-
-template <typename TW>
-static cudaError_t run_few(const SmallArgs& a, cudaStream_t s) {
-    const unsigned ctas = (unsigned)ceil_div(a.n, 32);
-    if (a.rows == 1) k_few<TW, 1><<<ctas, 32 * kFewWarps, 0, s>>>(a);
-    else if (a.rows == 2) k_few<TW, 2><<<ctas, 32 * kFewWarps, 0, s>>>(a);
-    else if (a.rows <= 4) k_few<TW, 4><<<ctas, 32 * kFewWarps, 0, s>>>(a);
-    else k_few<TW, 8><<<ctas, 32 * kFewWarps, 0, s>>>(a);
-    return cudaGetLastError();
-}
-
 static cudaError_t forward_small(const plattice_linear_args* a, Way way, cudaStream_t s) {
     const int e = a->dtype == PLATTICE_F32 ? 4 : 8;   // elements of 16 bytes
     const SmallArgs p{a->x, a->x_scale, a->w, a->bias, a->residual, a->y0, a->y1, a->z, a->z_scale, a->rows,
@@ -567,22 +463,15 @@ static cudaError_t forward_small(const plattice_linear_args* a, Way way, cudaStr
                       a->k % e == 0 && aligned16(a->x), a->k % 8 == 0 && aligned16(a->w),
                       aligned16(a->y0) && (!a->y1 || aligned16(a->y1)) && (!a->residual || aligned16(a->residual)) &&
                           (!a->z || aligned16(a->z))};
-    if (way == kWayFew)
-        return a->dtype == PLATTICE_F32    ? run_few<float>(p, s)
-               : a->dtype == PLATTICE_BF16 ? run_few<__nv_bfloat16>(p, s)
-                                           : run_few<__half>(p, s);
-    if (a->x_scale) return a->dtype == PLATTICE_F32 ? run_narrow<kX8, true>(p, s) : run_narrow<kX8, false>(p, s);
-    return a->dtype == PLATTICE_F32    ? run_narrow<kXFloat, true>(p, s)
-           : a->dtype == PLATTICE_BF16 ? run_narrow<kXBf16, false>(p, s)
-                                       : run_narrow<kXHalf, false>(p, s);
+    return way == kWayFew ? run_few_rows(p, a->dtype, s) : run_narrow(p, a->dtype, s);
 }
 
 static cudaError_t forward_mma(const plattice_linear_args* a, const ForwardPlan& p, cudaStream_t s) {
     char* ws = static_cast<char*>(a->workspace);
     Operand x, w;
     cudaError_t e = cudaSuccess;
-    if (p.unpack) e = unpacked(&x, a, ws + p.x, s);
-    else if (!a->x_scale) e = operand(&x, a->x, a->dtype, a->rows, a->k, ws + p.x, s);
+    if (a->x_scale) e = unpacked(&x, a, ws + p.x, s);
+    else e = operand(&x, a->x, a->dtype, a->rows, a->k, ws + p.x, s);
     if (e == cudaSuccess) e = operand(&w, a->w, a->dtype, a->n, a->k, ws + p.w, s);
     if (e != cudaSuccess) return e;
     MmaArgs m{};
@@ -598,49 +487,12 @@ static cudaError_t forward_mma(const plattice_linear_args* a, const ForwardPlan&
     m.out_dtype = a->out_dtype;
     m.act = a->act;
     m.split = a->split;
-    m.vec = a->n % 8 == 0 && aligned16(a->y0) && (!a->residual || aligned16(a->residual)) &&
-            (!a->z || a->z_scale || aligned16(a->z));
+    const bool aligned = a->n % 8 == 0 && aligned16(a->y0) && (!a->residual || aligned16(a->residual)) &&
+                         (!a->z || a->z_scale || aligned16(a->z));
     m.half = a->dtype == PLATTICE_F16;
     m.fault = pl::fault_word();
     sum_args(&m, a->k, 1, x.parts, w.parts);
-    if (!a->x_scale || p.unpack) return run_mma<kForward, false>(p.bn, x, w, m, s);
-    x8_args(&m, a);
-    return run_mma<kForward, true>(p.bn, x, w, m, s);
-}
-
-template <int kXT, int kParts, int kNF, bool kG32>
-static cudaError_t launch_narrow_grad(const SmallGradArgs& a, int lines, cudaStream_t s) {
-    int unused = 0;
-    const cudaError_t e = pl::kernel_once(
-        reinterpret_cast<const void*>(k_narrow_grad<kXT, kParts, kNF, kG32>),
-        [](int*) {
-            return cudaFuncSetAttribute(k_narrow_grad<kXT, kParts, kNF, kG32>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        NarrowGradShape<kXT, kParts>::kBytes);
-        },
-        &unused);
-    if (e != cudaSuccess) return e;
-    const int64_t slices = ceil_div(a.s.k, 64);
-    if (slices > 65535) return cudaErrorInvalidValue;
-    k_narrow_grad<kXT, kParts, kNF, kG32><<<dim3(lines, (unsigned)slices), 32 * kGradWarps,
-                                            NarrowGradShape<kXT, kParts>::kBytes, s>>>(a);
-    return cudaGetLastError();
-}
-
-template <int kXT, int kParts, bool kG32>
-static cudaError_t run_narrow_grad_as(const SmallGradArgs& a, int lines, cudaStream_t s) {
-    switch ((a.s.n + 7) / 8) {
-        case 1: return launch_narrow_grad<kXT, kParts, 1, kG32>(a, lines, s);
-        case 2: return launch_narrow_grad<kXT, kParts, 2, kG32>(a, lines, s);
-        case 3: return launch_narrow_grad<kXT, kParts, 3, kG32>(a, lines, s);
-        default: return launch_narrow_grad<kXT, kParts, 4, kG32>(a, lines, s);
-    }
-}
-
-template <int kXT, int kParts>
-static cudaError_t run_narrow_grad(const SmallGradArgs& a, int lines, cudaStream_t s) {
-    if constexpr (kParts == 1)
-        if (a.s.out_dtype != PLATTICE_F32) return run_narrow_grad_as<kXT, kParts, false>(a, lines, s);
-    return run_narrow_grad_as<kXT, kParts, true>(a, lines, s);
+    return mma_forward(p.bn, aligned, x, w, m, s);
 }
 
 static cudaError_t backward_narrow(const plattice_linear_args* a, const BackwardPlan& p, cudaStream_t s) {
@@ -669,15 +521,7 @@ static cudaError_t backward_narrow(const plattice_linear_args* a, const Backward
     g.need_w = a->grad_w != nullptr;
     g.need_b = a->grad_bias != nullptr;
     g.vec_gx = a->k % 8 == 0 && aligned16(a->grad_x);
-    cudaError_t e;
-    if (a->x_scale || !a->x)   // without x (no weight gradient) its type does not matter
-        e = a->dtype == PLATTICE_F32    ? run_narrow_grad<kX8, 3>(g, p.lines, s)
-            : a->dtype == PLATTICE_BF16 ? run_narrow_grad<kX8, 1>(g, p.lines, s)
-                                        : run_narrow_grad<kXHalf, 1>(g, p.lines, s);
-    else
-        e = a->dtype == PLATTICE_F32    ? run_narrow_grad<kXFloat, 3>(g, p.lines, s)
-            : a->dtype == PLATTICE_BF16 ? run_narrow_grad<kXBf16, 1>(g, p.lines, s)
-                                        : run_narrow_grad<kXHalf, 1>(g, p.lines, s);
+    const cudaError_t e = run_narrow_grad(g, a->dtype, p.lines, s);
     if (e != cudaSuccess || !(a->grad_w || a->grad_bias)) return e;
     const int64_t nw = (int64_t)a->n * a->k, columns = nw + a->n;
     k_sum_lines<<<(unsigned)ceil_div(columns, 32), 1024, 0, s>>>(a->grad_w, a->dtype, nw, a->grad_bias, a->bias_dtype, a->n,
@@ -722,15 +566,14 @@ static cudaError_t backward_mma(const plattice_linear_args* a, const BackwardPla
         m.ni = a->rows;
         m.nj = a->k;
         m.out_dtype = a->dtype;
-        m.vec = a->k % 8 == 0 && aligned16(a->grad_x);
         sum_args(&m, a->n, 1, gz.parts, w.parts);
-        e = run_mma<kGradX, false>(p.bn_x, gz, w, m, s);
+        e = mma_grad_x(p.bn_x, a->k % 8 == 0 && aligned16(a->grad_x), gz, w, m, s);
         if (e != cudaSuccess) return e;
     }
     if (a->grad_w) {
         Operand x;
-        if (p.unpack) e = unpacked(&x, a, ws + p.x, s);
-        else if (!a->x_scale) e = operand(&x, a->x, a->dtype, a->rows, a->k, ws + p.x, s);
+        if (a->x_scale) e = unpacked(&x, a, ws + p.x, s);
+        else e = operand(&x, a->x, a->dtype, a->rows, a->k, ws + p.x, s);
         if (e != cudaSuccess) return e;
         m.ni = a->k;
         m.nj = a->n;
@@ -738,12 +581,7 @@ static cudaError_t backward_mma(const plattice_linear_args* a, const BackwardPla
         const bool direct = p.parts_w == 1;
         m.y0 = direct ? a->grad_w : ws + p.partial_w;
         m.out_dtype = direct ? a->dtype : PLATTICE_F32;
-        if (!a->x_scale || p.unpack) {
-            e = run_mma<kGradW, false>(p.bn_w, x, gz, m, s);
-        } else {
-            x8_args(&m, a);
-            e = run_mma<kGradW, true>(p.bn_w, x, gz, m, s);
-        }
+        e = mma_grad_w(p.bn_w, x, gz, m, s);
         if (e == cudaSuccess && !direct)
             e = add_parts_to(a->grad_w, a->dtype, reinterpret_cast<const float*>(ws + p.partial_w), m.parts,
                              (int64_t)a->n * a->k, s);

@@ -12,35 +12,39 @@
 //
 // Operands are 16-bit.  float32 operands come as three bfloat16 parts whose
 // sum is the value (8 + 8 + 8 significant bits); the six products of parts
-// down to 2^-16 of the largest are added, the small ones first.  An 8-bit x
-// is widened to bfloat16 (exact) on its way to shared memory by warps of its
-// own, so HBM carries one byte a value.
+// down to 2^-16 of the largest are added, the small ones first.  8-bit rows
+// come unpacked to bfloat16 (exact).
 //
 // One CTA per SM walks over 128 x kBN tiles of D (times parts of the sum for
 // kGradW): one thread issues TMA copies of 64-deep slices into a ring of
-// stages, one issues the MMAs, eight warps empty the other of two
+// stages, one issues the MMAs, the epilogue's warps empty the other of two
 // accumulators (activation, residual, stores) meanwhile.  Every wait is
 // bounded: a wait that gives up ends all roles, copies and MMAs in flight are
 // waited for, tensor memory is freed and the call's failure is reported.
 #pragma once
 #include <cuda.h>
+#include <limits.h>
 
+#include "plattice_runtime.h"
 #include "rows_common.cuh"
+#include "rows_host.h"
 
 namespace plr {
 
-enum Kind { kForward = 0, kGradX = 1, kGradW = 2 };
+constexpr int kStageA = kBM * kBK * 2;
 
-constexpr int kBM = 128, kBK = 64;
-constexpr int kConvertWarps = 8;
+// What an epilogue is compiled for: rows of any alignment, everything looked
+// up at run time; rows on 16-byte boundaries; those without activation,
+// residual, split and kept pre-activation.  (Control flow that asks for each of
+// these at every 16 columns cost a third of a plain forward's time.)
+enum Mode { kAny = 0, kAligned = 1, kPlain = 2 };
+
 // Warps that empty accumulators.  The forward's work per output (activation,
 // residual, 8-bit codes) waits more than it issues: 16 warps hide what 8 do
-// not (422 -> 2xx us at 32768 x 1024 -> 4096, gelu, residual, kept z).
-// Beside converting warps, and for the plain stores of the gradients, 8 do.
-__host__ __device__ constexpr int epilogue_warps(int kind, bool x8) { return kind == 0 && !x8 ? 16 : 8; }
-__host__ __device__ constexpr int role_threads(int kind, bool x8) { return 128 + 32 * epilogue_warps(kind, x8); }
-constexpr int kStageA = kBM * kBK * 2;
-constexpr int kMaxSmem = 232448;   // shared memory a CTA can have
+// not (422 against 353 us at 32768 x 1024 -> 4096, gelu, residual, kept z).
+// For the plain stores of the gradients 8 do.
+__host__ __device__ constexpr int epilogue_warps(int kind) { return kind == 0 ? 16 : 8; }
+__host__ __device__ constexpr int role_threads(int kind) { return 128 + 32 * epilogue_warps(kind); }
 
 __host__ __device__ constexpr bool a_mn(int kind) { return kind == kGradW; }
 __host__ __device__ constexpr bool b_mn(int kind) { return kind != kForward; }
@@ -48,42 +52,14 @@ __host__ __device__ constexpr bool b_mn(int kind) { return kind != kForward; }
 __host__ __device__ constexpr int b_columns(int kind, int bn) { return b_mn(kind) && bn < 64 ? 64 : bn; }
 __host__ __device__ constexpr int stage_bytes(int kind, int bn) { return kStageA + b_columns(kind, bn) * kBK * 2; }
 constexpr int kWarpStaging = 32 * 16 * 4 + 32 * 4;   // a 32 x 16 float tile and 32 biases
-__host__ __device__ constexpr int fixed_smem(int kind, bool x8) {
-    return 1024 + epilogue_warps(kind, x8) * kWarpStaging + 256;
-}
-__host__ __device__ constexpr int stages(int kind, bool x8, int bn) {
-    const int n = (kMaxSmem - 16 - fixed_smem(kind, x8)) / stage_bytes(kind, bn);
+__host__ __device__ constexpr int fixed_smem(int kind) { return 1024 + epilogue_warps(kind) * kWarpStaging + 256; }
+__host__ __device__ constexpr int stages(int kind, int bn) {
+    const int n = (kMaxSmem - 16 - fixed_smem(kind)) / stage_bytes(kind, bn);
     return n > 8 ? 8 : n;
 }
-__host__ __device__ constexpr int smem_bytes(int kind, bool x8, int bn) {
-    return fixed_smem(kind, x8) + stages(kind, x8, bn) * stage_bytes(kind, bn);
+__host__ __device__ constexpr int smem_bytes(int kind, int bn) {
+    return fixed_smem(kind) + stages(kind, bn) * stage_bytes(kind, bn);
 }
-
-struct MmaArgs {
-    // result
-    void* y0;
-    void* y1;             // split: columns split.. of D
-    const void* bias;     // null: none
-    const void* residual;
-    void* z;              // kept pre-activation (null: none)
-    uint8_t* z_scale;
-    int64_t ni, nj;       // D is ni x nj
-    int bias_dtype, out_dtype, act, split;
-    bool vec;             // rows of y0, residual and z allow 16-byte accesses
-    // sum
-    int steps;            // 64-deep slices of r
-    int part_steps;       // of a part (kGradW); parts are numbered tile-slowest
-    int parts;
-    unsigned pairs_a, pairs_b;   // parts of A and B of each product, 2 bits each
-    int pairs;
-    bool half;            // operands are float16 (else bfloat16)
-    // 8-bit A
-    const uint8_t* q;
-    const uint8_t* q_scale;
-    int64_t q_rows;
-    int64_t q_width;
-    unsigned* fault;      // host-mapped word that reports a wait that gave up (may be null)
-};
 
 // ------------------------------------------------------------- PTX wrappers
 
@@ -193,16 +169,9 @@ __device__ __forceinline__ Tile tile_at(const MmaArgs& p, unsigned t) {
 
 // ---------------------------------------------------------------- epilogue
 
-__device__ __forceinline__ void store8_as(void* p, int dtype, int64_t at, const float (&v)[8], bool vec, int n) {
-    if (dtype == PLATTICE_F32) store8(static_cast<float*>(p) + at, v, vec, n);
-    else if (dtype == PLATTICE_BF16) store8(static_cast<__nv_bfloat16*>(p) + at, v, vec, n);
-    else store8(static_cast<__half*>(p) + at, v, vec, n);
-}
-__device__ __forceinline__ void load8_as(float (&v)[8], const void* p, int dtype, int64_t at, bool vec, int n) {
-    if (dtype == PLATTICE_F32) load8(v, static_cast<const float*>(p) + at, vec, n);
-    else if (dtype == PLATTICE_BF16) load8(v, static_cast<const __nv_bfloat16*>(p) + at, vec, n);
-    else load8(v, static_cast<const __half*>(p) + at, vec, n);
-}
+template <int kOut> struct OutType { typedef float type; };
+template <> struct OutType<PLATTICE_BF16> { typedef __nv_bfloat16 type; };
+template <> struct OutType<PLATTICE_F16> { typedef __half type; };
 
 // Half a warp's 32 x 32 tile in shared memory, 16 columns: float4 c of row r at
 // slot c ^ ((r >> 1) & 3), free of bank conflicts both a row per lane and two
@@ -214,89 +183,104 @@ __device__ __forceinline__ float staged_at(const float* s, int row, int c) {
     return s[row * 16 + (((c >> 2) ^ ((row >> 1) & 3)) << 2) + (c & 3)];
 }
 
-__device__ __forceinline__ void stage_rows(float* s, const float* v, int lane) {
+__device__ __forceinline__ void stage_rows(float* s, const float (&v)[16], int lane) {
     __syncwarp();
 #pragma unroll
     for (int c = 0; c < 4; ++c) *staged(s, lane, c) = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
     __syncwarp();
 }
 
-// 32 x 16 of the residual as store_half's lanes take them, loaded a half piece
-// ahead: a load waited for at each store would cost a trip to HBM twice a half
-// (652 us against 422 at 32768 x 1024 -> 4096, gelu, residual, kept z).
+// 32 x 16 of the residual as store_aligned's lanes take them, loaded a half
+// piece ahead: a load waited for at each store would cost a trip to HBM twice a
+// half (652 us against 422 at 32768 x 1024 -> 4096, gelu, residual, kept z).
 struct Ahead {
     uint4 r[2];   // twice 8 columns of a 16-bit type (float32 is loaded at the store)
     bool have;
 };
 
+template <int kOut>
 __device__ __forceinline__ void load_ahead(Ahead& a, const MmaArgs& p, int64_t row0, int64_t col0, int lane) {
-    a.have = p.residual && p.out_dtype != PLATTICE_F32 && p.vec && col0 + 16 <= p.nj && row0 + 32 <= p.ni;
+    a.have = kOut != PLATTICE_F32 && p.residual && col0 + 16 <= p.nj && row0 + 32 <= p.ni;
     if (!a.have) return;
 #pragma unroll
     for (int it = 0; it < 2; ++it)
-        a.r[it] = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.residual) +
+        a.r[it] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.residual) +
                                                   (row0 + it * 16 + (lane >> 1)) * p.nj + col0 + (lane & 1) * 8);
-}
-
-template <typename T> __device__ __forceinline__ void add_pairs(float (&v)[8], const uint4& r) {
-    union { uint4 u; typename Pair<T>::type h[4]; } x;
-    x.u = r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = pair_f32(x.h[i]);
-        add2(v[2 * i], v[2 * i + 1], f.x, f.y);
-    }
-}
-
-__device__ __forceinline__ void add_ahead(float (&v)[8], const Ahead& a, int it, int dtype) {
-    if (dtype == PLATTICE_BF16) {
-        add_pairs<__nv_bfloat16>(v, a.r[it]);
-    } else {
-        add_pairs<__half>(v, a.r[it]);
-    }
 }
 
 // 16 columns of 32 rows (a row per lane) to (row0, col0) of an [ni][nj] tensor,
 // `add` (the residual, same layout) added: through the staging to two lanes a
-// row, 8 columns each.
-__device__ __forceinline__ void store_half(float* s, const float (&v)[16], void* dst, const MmaArgs& p, int64_t row0,
-                                           int64_t col0, const void* add, const Ahead& ahead, int lane) {
-    stage_rows(s, v, lane);
-    const int rows = (int)min((int64_t)32, p.ni - row0);
-    if (!p.vec) {   // rows on no 16-byte boundaries: a lane per column, two rows at a time
-        const int64_t col = col0 + (lane & 15);
-        if (col >= p.nj) return;
-        float x[16];
+// row, 8 columns each.  nj is a multiple of 8: a lane's columns all exist or
+// none does.
+template <int kOut>
+__device__ __forceinline__ void store_aligned(float* s, const float (&v)[16], void* dst, const MmaArgs& p, int64_t row0,
+                                              int64_t col0, const void* add, const Ahead& ahead, int lane) {
+    typedef typename OutType<kOut>::type T;
+    const int rows = (int)min((int64_t)32, p.ni - row0), c = (lane & 1) * 8;
+    const bool have = col0 + c < p.nj;
+    T* out = static_cast<T*>(dst) + (row0 + (lane >> 1)) * p.nj + col0 + c;
+    if constexpr (sizeof(T) == 2) {
+        if (!add) {   // rounded before the staging: half its traffic.  Row r's two
+                      // 16-byte slots change places with r >> 2: no bank conflicts
+            uint4* q = reinterpret_cast<uint4*>(s);
+            union { uint4 u[2]; typename Pair<T>::type h[8]; } o;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {   // all of the residual's loads before the first store
-            const int r = (lane >> 4) + 2 * i;
-            x[i] = add && r < rows ? load_param(add, p.out_dtype, (row0 + r) * p.nj + col) : 0.f;
-        }
+            for (int i = 0; i < 8; ++i) pair_from(o.h[i], v[2 * i], v[2 * i + 1]);
+            __syncwarp();
+            q[lane * 2 + ((lane >> 2) & 1)] = o.u[0];
+            q[lane * 2 + (((lane >> 2) & 1) ^ 1)] = o.u[1];
+            __syncwarp();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int r = (lane >> 4) + 2 * i;
-            if (r < rows) store_param(dst, p.out_dtype, (row0 + r) * p.nj + col, x[i] + staged_at(s, r, lane & 15));
+            for (int it = 0; it < 2; ++it) {
+                const int r = it * 16 + (lane >> 1);
+                if (r < rows && have)
+                    *reinterpret_cast<uint4*>(out + (int64_t)it * 16 * p.nj) = q[r * 2 + ((lane & 1) ^ ((r >> 2) & 1))];
+            }
+            return;
         }
-        return;
     }
-    const int c = (lane & 1) * 8, n = (int)min((int64_t)16, p.nj - col0) - c;
-    const bool vec = n >= 8;
+    stage_rows(s, v, lane);
 #pragma unroll
     for (int it = 0; it < 2; ++it) {
         const int r = it * 16 + (lane >> 1);
-        if (r >= rows || n <= 0) continue;
-        const int64_t at = (row0 + r) * p.nj + col0 + c;
+        if (r >= rows || !have) continue;
         const float4 a = *staged(s, r, c >> 2), b = *staged(s, r, (c >> 2) + 1);
         float o[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-        if (add && ahead.have) {
-            add_ahead(o, ahead, it, p.out_dtype);
-        } else if (add) {
-            float q[8];
-            load8_as(q, add, p.out_dtype, at, vec, n);
+        if (add) {
+            Raw8<T> q;
+            float t[8];
+            if constexpr (sizeof(T) == 2) {
+                if (ahead.have) q.u = ahead.r[it];
+                else q.load(static_cast<const T*>(add) + (out - static_cast<T*>(dst)) + (int64_t)it * 16 * p.nj, true, 8);
+            } else {
+                q.load(static_cast<const T*>(add) + (out - static_cast<T*>(dst)) + (int64_t)it * 16 * p.nj, true, 8);
+            }
+            q.widen(t);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) o[i] += q[i];
+            for (int i = 0; i < 8; i += 2) add2(o[i], o[i + 1], t[i], t[i + 1]);
         }
-        store8_as(dst, p.out_dtype, at, o, vec, n);
+        store8(out + (int64_t)it * 16 * p.nj, o, true, 8);
+    }
+}
+
+// The same where rows lie on no 16-byte boundaries: a lane per column, two
+// rows at a time, all of the residual's loads before the first store.
+__device__ __forceinline__ void store_any(float* s, const float (&v)[16], void* dst, const MmaArgs& p, int64_t row0,
+                                          int64_t col0, const void* add, int lane) {
+    stage_rows(s, v, lane);
+    const int rows = (int)min((int64_t)32, p.ni - row0);
+    const int64_t col = col0 + (lane & 15);
+    if (col >= p.nj) return;
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int r = (lane >> 4) + 2 * i;
+        x[i] = add && r < rows ? load_param(add, p.out_dtype, (row0 + r) * p.nj + col) : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int r = (lane >> 4) + 2 * i;
+        if (r < rows) store_param(dst, p.out_dtype, (row0 + r) * p.nj + col, x[i] + staged_at(s, r, lane & 15));
     }
 }
 
@@ -331,27 +315,28 @@ struct Block8 {
 };
 
 // Half a 32-column piece (16 columns from col0), a row per lane.
-template <int kKind>
+template <int kKind, int kOut, int kMode>
 __device__ __forceinline__ void finish16(float (&v)[16], const MmaArgs& p, const Tile& t, int64_t row0, int64_t col0,
                                          float* s, Ahead& ahead, Block8& block, int half, int lane) {
+    typedef typename OutType<kOut>::type T;
     if (kKind == kGradW) {
         // D is [input channel][output channel], its result [output channel]
         // [input channel]: a lane per input channel stores whole lines
         const int64_t i = row0 + lane;
         if (i >= p.ni) return;
         const int left = (int)min((int64_t)16, p.nj - col0);
-        const int64_t at = ((int64_t)t.part * p.nj + col0) * p.ni + i;
+        T* out = static_cast<T*>(p.y0) + ((int64_t)t.part * p.nj + col0) * p.ni + i;
 #pragma unroll
-        for (int c = 0; c < 16; ++c)
-            if (c < left) store_param(p.y0, p.out_dtype, at + (int64_t)c * p.ni, v[c]);
+        for (int c = 0; c < 16; ++c, out += p.ni)
+            if (c < left) *out = from_f32<T>(v[c]);
         return;
     }
-    if (kKind == kGradX) {
-        store_half(s, v, p.y0, p, row0, col0, nullptr, ahead, lane);
+    if (kKind == kForward && p.bias) add_bias(v, s + 32 * 16 + half * 16);
+    if (kMode == kPlain) {
+        store_aligned<kOut>(s, v, p.y0, p, row0, col0, nullptr, ahead, lane);
         return;
     }
-    if (p.bias) add_bias(v, s + 32 * 16 + half * 16);
-    if (p.z_scale) {
+    if (kKind == kForward && p.z_scale) {
         const float inv = pow2(-block.exponent);
         const uint2 x = codes8_of(v, inv, block.infinite), y = codes8_of(v + 8, inv, block.infinite);
         if (half == 0) {
@@ -364,82 +349,27 @@ __device__ __forceinline__ void finish16(float (&v)[16], const MmaArgs& p, const
                          : "memory");
             p.z_scale[at] = (uint8_t)(block.exponent + 127);
         }
-    } else if (p.z) {
-        if (col0 < p.nj) store_half(s, v, p.z, p, row0, col0, nullptr, ahead, lane);
+    } else if (kKind == kForward && p.z && col0 < p.nj) {
+        if (kMode == kAligned) store_aligned<kOut>(s, v, p.z, p, row0, col0, nullptr, ahead, lane);
+        else store_any(s, v, p.z, p, row0, col0, nullptr, lane);
     }
     if (col0 >= p.nj) return;
-    activate(v, p.act);
-    if (p.split) store_split(s, v, p, row0, col0, lane);
-    else store_half(s, v, p.y0, p, row0, col0, p.residual, ahead, lane);
-}
-
-// ------------------------------------------------- widening an 8-bit operand
-
-constexpr int kAhead = 4;   // slices whose codes are in flight per thread
-
-struct Codes {
-    uint4 c[2];
-    uint8_t scale;
-};
-
-// 32 codes of one scale per thread and slice.  K-major: 128 rows x 64
-// channels, two threads a row; MN-major: 64 rows x 128 channels, neighbouring
-// lanes on neighbouring rows, so that the 8 lanes of a shared-memory phase
-// write 8 different 16-byte columns of the swizzle.
-template <bool kMN>
-__device__ __forceinline__ void convert_place(int t, int& row, int& channel) {
-    row = kMN ? t & 63 : t >> 1;
-    channel = kMN ? (t >> 6) * 32 : (t & 1) * 32;
-}
-
-template <bool kMN>
-__device__ __forceinline__ Codes load_codes(const MmaArgs& p, const Tile& t, int step, int thread) {
-    int row, ch;
-    convert_place<kMN>(thread, row, ch);
-    const int64_t m = (kMN ? (int64_t)step * kBK : t.i0) + row;
-    const int64_t c = (kMN ? t.i0 : (int64_t)step * kBK) + ch;
-    Codes r;
-    r.c[0] = r.c[1] = make_uint4(0, 0, 0, 0);
-    r.scale = 127;
-    if (m < p.q_rows && c < p.q_width) {
-        const int64_t at = m * p.q_width + c;
-        const uint4* src = reinterpret_cast<const uint4*>(p.q + at);
-        r.c[0] = src[0];
-        r.c[1] = src[1];
-        r.scale = p.q_scale[at >> 5];
-    }
-    return r;
-}
-
-template <bool kMN>
-__device__ __forceinline__ void store_codes(uint32_t slice, const Codes& k, int thread) {
-    int row, ch;
-    convert_place<kMN>(thread, row, ch);
-    const uint32_t base = slice + (kMN ? (ch >> 6) * 8192 : 0) + row * 128;
-    const int chunk = (ch & 63) >> 3;
-    const float scale = scale_of(k.scale);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint4& q = k.c[i >> 1];
-        const uint2 w = i & 1 ? make_uint2(q.z, q.w) : make_uint2(q.x, q.y);
-        float f[8];
-        values8(f, w, scale);
-        union { uint4 u; __nv_bfloat162 h[4]; } o;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o.h[j] = __floats2bfloat162_rn(f[2 * j], f[2 * j + 1]);   // exact
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(base + (((chunk + i) ^ (row & 7)) << 4)),
-                     "r"(o.u.x), "r"(o.u.y), "r"(o.u.z), "r"(o.u.w)
-                     : "memory");
-    }
+    const void* add = kKind == kForward ? p.residual : nullptr;
+    if (kKind == kForward) activate(v, p.act);
+    if (kMode == kAligned) store_aligned<kOut>(s, v, p.y0, p, row0, col0, add, ahead, lane);
+    else if (kKind == kForward && p.split) store_split(s, v, p, row0, col0, lane);
+    else store_any(s, v, p.y0, p, row0, col0, add, lane);
 }
 
 // -------------------------------------------------------------- the kernel
 
-template <int kKind, bool kX8, int kBN>
-__global__ void __launch_bounds__(role_threads(kKind, kX8) + (kX8 ? 32 * kConvertWarps : 0), 1)
+// kOut: the type of y0 (kAny: looked up).
+template <int kKind, int kBN, int kOut, int kMode>
+__global__ void __launch_bounds__(role_threads(kKind), 1)
     k_mma(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const MmaArgs p,
           unsigned tiles) {
-    constexpr int kStages = stages(kKind, kX8, kBN), kEpilogueWarps = epilogue_warps(kKind, kX8);
+    constexpr int kStages = stages(kKind, kBN), kEpilogueWarps = epilogue_warps(kKind);
+    constexpr bool kKeeps = kKind == kForward && kMode != kPlain;   // a kept pre-activation, a residual
     constexpr int kGroups = kEpilogueWarps / 4;   // warps that share 32 accumulator rows
     constexpr int kStage = stage_bytes(kKind, kBN);
     constexpr int kColumns = 2 * kBN;   // tensor memory: two accumulators
@@ -462,7 +392,7 @@ __global__ void __launch_bounds__(role_threads(kKind, kX8) + (kX8 ? 32 * kConver
     if (threadIdx.x == 0) {
         dead_flag = 0;
         for (int s = 0; s < kStages; ++s) {
-            bar_init(full(s), 1 + (kX8 ? kConvertWarps : 0));
+            bar_init(full(s), 1);
             bar_init(empty(s), 1);
         }
         for (int b = 0; b < 2; ++b) {
@@ -494,14 +424,12 @@ __global__ void __launch_bounds__(role_threads(kKind, kX8) + (kX8 ? 32 * kConver
                     for (int k = tile.begin; k < tile.end; ++k) {
                         if (!bar_wait(empty(s), phase ^ 1, dead)) goto copies_done;
                         const uint32_t a = ring + s * kStage, b = a + kStageA;
-                        bar_expect(full(s), (kX8 ? 0 : kStageA) + b_columns(kKind, kBN) * kBK * 2);
-                        if (!kX8) {
-                            if (a_mn(kKind)) {
-                                for (int g = 0; g < kBM / 64; ++g)
-                                    tma_load(a + g * 8192, &map_a, full(s), (int)tile.i0 + g * 64, k * kBK, za);
-                            } else {
-                                tma_load(a, &map_a, full(s), k * kBK, (int)tile.i0, za);
-                            }
+                        bar_expect(full(s), kStageA + b_columns(kKind, kBN) * kBK * 2);
+                        if (a_mn(kKind)) {
+                            for (int g = 0; g < kBM / 64; ++g)
+                                tma_load(a + g * 8192, &map_a, full(s), (int)tile.i0 + g * 64, k * kBK, za);
+                        } else {
+                            tma_load(a, &map_a, full(s), k * kBK, (int)tile.i0, za);
                         }
                         if (b_mn(kKind)) {
                             for (int g = 0; g < b_columns(kKind, kBN) / 64; ++g)
@@ -579,7 +507,7 @@ __global__ void __launch_bounds__(role_threads(kKind, kX8) + (kX8 ? 32 * kConver
             };
             ahead.have = false;
             bias_ahead(group);
-            if (kKind == kForward && group < kPieces) load_ahead(ahead, p, row0, tile.j0 + group * 32, lane);
+            if (kKeeps && kMode == kAligned && group < kPieces) load_ahead<kOut>(ahead, p, row0, tile.j0 + group * 32, lane);
             if (!warp_wait(acc_full(buf), (n >> 1) & 1, dead)) break;
             fence_after();
             const uint32_t base = tmem + buf * kBN + ((uint32_t)(quarter * 32) << 16);
@@ -595,7 +523,7 @@ __global__ void __launch_bounds__(role_threads(kKind, kX8) + (kX8 ? 32 * kConver
                     __syncwarp();
                 }
                 bias_ahead(c + kGroups);
-                if (kKind == kForward && live && p.z_scale) {
+                if (kKeeps && live && p.z_scale) {
                     float amax = 0.f;   // of both halves, which are read again below
 #pragma unroll 1
                     for (int h = 0; h < 2; ++h) {
@@ -616,61 +544,12 @@ __global__ void __launch_bounds__(role_threads(kKind, kX8) + (kX8 ? 32 * kConver
                         __syncwarp();
                         if (lane == 0) bar_arrive(acc_empty(buf));
                     }
-                    if (live) finish16<kKind>(v, p, tile, row0, col0 + h * 16, s, ahead, block, h, lane);
+                    if (live) finish16<kKind, kOut, kMode>(v, p, tile, row0, col0 + h * 16, s, ahead, block, h, lane);
                     const int64_t next = h == 0 ? col0 + 16 : col0 + kGroups * 32;
-                    if (kKind == kForward && (h == 0 || c + kGroups < kPieces)) load_ahead(ahead, p, row0, next, lane);
+                    if (kKeeps && kMode == kAligned && (h == 0 || c + kGroups < kPieces)) load_ahead<kOut>(ahead, p, row0, next, lane);
                 }
             }
             if (group >= kPieces && lane == 0) bar_arrive(acc_empty(buf));
-        }
-    } else if (kX8 && warp >= 4 + kEpilogueWarps) {
-        // ---- widening 8-bit rows
-        const int thread = threadIdx.x - role_threads(kKind, kX8);
-        constexpr bool kMN = a_mn(kKind);
-        Codes ahead[kAhead];
-        // cursor of the next slice to load
-        unsigned lt = blockIdx.x;
-        Tile ltile = lt < tiles ? tile_at<kBN>(p, lt) : Tile{};
-        int lpair = 0, lk = ltile.begin;
-        auto load_next = [&](Codes& c) {
-            if (lt >= tiles) return false;
-            c = load_codes<kMN>(p, ltile, lk, thread);
-            if (++lk == ltile.end) {
-                lk = ltile.begin;
-                if (++lpair == p.pairs) {
-                    lpair = 0;
-                    lt += gridDim.x;
-                    if (lt < tiles) {
-                        ltile = tile_at<kBN>(p, lt);
-                        lk = ltile.begin;
-                    }
-                }
-            }
-            return true;
-        };
-        bool have[kAhead];
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u) have[u] = load_next(ahead[u]);
-        int s = 0, phase = 0;
-        bool more = true;
-        while (more) {
-#pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                if (!more || !have[u]) {
-                    more = false;
-                    continue;
-                }
-                if (!warp_wait(empty(s), phase ^ 1, dead)) {
-                    more = false;
-                    continue;
-                }
-                store_codes<kMN>(ring + s * kStage, ahead[u], thread);
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the MMA reads what was written
-                __syncwarp();
-                if (lane == 0) bar_arrive(full(s));
-                if (++s == kStages) s = 0, phase ^= 1;
-                have[u] = load_next(ahead[u]);
-            }
         }
     }
     __syncwarp();
@@ -680,6 +559,45 @@ __global__ void __launch_bounds__(role_threads(kKind, kX8) + (kX8 ? 32 * kConver
     if (warp == 2)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kColumns) : "memory");
     if (threadIdx.x == 0 && dead_flag && p.fault) *reinterpret_cast<volatile unsigned*>(p.fault) = 1;
+}
+
+// ------------------------------------------------------------------ launch
+
+template <int kKind, int kBN, int kOut, int kMode>
+cudaError_t launch_mma(const Operand& a, const Operand& b, const MmaArgs& p, cudaStream_t s) {
+    int unused = 0;
+    cudaError_t e = pl::kernel_once(
+        reinterpret_cast<const void*>(k_mma<kKind, kBN, kOut, kMode>),
+        [](int*) {
+            return cudaFuncSetAttribute(k_mma<kKind, kBN, kOut, kMode>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        smem_bytes(kKind, kBN));
+        },
+        &unused);
+    if (e != cudaSuccess) return e;
+    CUtensorMap ma, mb;
+    if ((e = make_map(&ma, a, a_mn(kKind) ? kBK : kBM)) != cudaSuccess) return e;
+    if ((e = make_map(&mb, b, b_mn(kKind) ? kBK : kBN)) != cudaSuccess) return e;
+    const int64_t tiles = mma_tiles(p.ni, p.nj, kBN) * p.parts;
+    if (tiles > INT_MAX) return cudaErrorInvalidValue;
+    const int ctas = (int)(tiles < sm_count() ? tiles : sm_count());
+    k_mma<kKind, kBN, kOut, kMode><<<ctas, role_threads(kKind), smem_bytes(kKind, kBN), s>>>(ma, mb, p, (unsigned)tiles);
+    return cudaGetLastError();
+}
+
+template <int kKind, int kOut, int kMode>
+cudaError_t launch_bn(int bn, const Operand& a, const Operand& b, const MmaArgs& p, cudaStream_t s) {
+    if (bn == 256) return launch_mma<kKind, 256, kOut, kMode>(a, b, p, s);
+    if (bn == 128) return launch_mma<kKind, 128, kOut, kMode>(a, b, p, s);
+    if (bn == 64) return launch_mma<kKind, 64, kOut, kMode>(a, b, p, s);
+    if constexpr (kKind == kForward) return launch_mma<kKind, 32, kOut, kMode>(a, b, p, s);
+    return cudaErrorInvalidValue;
+}
+
+template <int kKind, int kMode>
+cudaError_t launch_out(int bn, const Operand& a, const Operand& b, const MmaArgs& p, cudaStream_t s) {
+    if (p.out_dtype == PLATTICE_F32) return launch_bn<kKind, PLATTICE_F32, kMode>(bn, a, b, p, s);
+    if (p.out_dtype == PLATTICE_BF16) return launch_bn<kKind, PLATTICE_BF16, kMode>(bn, a, b, p, s);
+    return launch_bn<kKind, PLATTICE_F16, kMode>(bn, a, b, p, s);
 }
 
 }  // namespace plr

@@ -1,0 +1,15 @@
+// rows_mma_grad.cu -- the tiled products of the linear map's gradients.
+#include "rows_mma.cuh"
+
+namespace plr {
+
+cudaError_t mma_grad_x(int bn, bool aligned, const Operand& gz, const Operand& w, const MmaArgs& p, cudaStream_t s) {
+    if (!aligned) return launch_bn<kGradX, PLATTICE_F32, kAny>(bn, gz, w, p, s);
+    return launch_out<kGradX, kPlain>(bn, gz, w, p, s);
+}
+
+cudaError_t mma_grad_w(int bn, const Operand& x, const Operand& gz, const MmaArgs& p, cudaStream_t s) {
+    return launch_out<kGradW, kAny>(bn, x, gz, p, s);
+}
+
+}  // namespace plr

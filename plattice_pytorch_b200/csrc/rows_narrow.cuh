@@ -4,56 +4,15 @@
 // 128-row tensor-memory tile would be mostly padding, and staging it costs
 // more than the product.
 #pragma once
+#include "plattice_runtime.h"
 #include "rows_common.cuh"
+#include "rows_host.h"
+#include "rows_narrow.h"
+#include "rows_split.cuh"
 
 namespace plr {
 
 enum XType { kX8 = 0, kXBf16 = 1, kXHalf = 2, kXFloat = 3 };
-
-struct SmallArgs {
-    const void* x;
-    const uint8_t* x_scale;
-    const void* w;
-    const void* bias;
-    const void* residual;
-    void* y0;
-    void* y1;
-    void* z;
-    uint8_t* z_scale;
-    int64_t rows;
-    int k, n, split, act;
-    int w_dtype, out_dtype, bias_dtype;
-    bool vec_x;    // 16-byte accesses to x's rows
-    bool vec_w;    // the same for w's
-    bool vec_y;    // the outputs and the residual begin on 16-byte boundaries
-};
-
-// A float32 value as three bfloat16 whose sum it is: each takes the leading 8
-// significant bits of what is left (cut, not rounded, so that none overflows
-// and the remainders are exact).  What is not finite stays in the first part.
-__device__ __forceinline__ void split3(float v, __nv_bfloat16 (&o)[3]) {
-    const bool fine = fabsf(v) <= 3.402823466e38f;
-#pragma unroll
-    for (int i = 0; i < 3; ++i) {
-        // cutting a NaN's low bits could leave an infinity: round those
-        const __nv_bfloat16 h = fine ? __ushort_as_bfloat16((unsigned short)(__float_as_uint(v) >> 16))
-                                     : __float2bfloat16_rn(i == 0 ? v : 0.f);
-        o[i] = h;
-        v = fine ? v - __bfloat162float(h) : v;
-    }
-}
-
-// The same of two finite values into packed parts; a value that is not finite
-// makes all its products NaN (infinity minus infinity in the second part).
-__device__ __forceinline__ void split3_pair(float a, float b, uint32_t (&o)[3]) {
-#pragma unroll
-    for (int i = 0; i < 3; ++i) {
-        const uint32_t ua = __float_as_uint(a) & 0xffff0000u, ub = __float_as_uint(b) & 0xffff0000u;
-        o[i] = (ua >> 16) | ub;
-        a -= __uint_as_float(ua);
-        b -= __uint_as_float(ub);
-    }
-}
 
 // ------------------------------------------------------- at most 32 channels
 //
@@ -81,12 +40,9 @@ template <int kXT> struct NarrowShape {
     static constexpr int kRaw = kXT == kX8 ? 1 : kXT == kXFloat ? 4 : 2;        // 16-byte loads per row and 64 channels
 };
 
-__host__ __device__ inline int narrow_steps(int k) { return (k + 63) / 64 * 4; }   // of 16 channels
-__host__ inline int64_t narrow_fragments(int k, int nf, int parts) { return (int64_t)parts * narrow_steps(k) * nf * 256; }
 constexpr int kNarrowWarps = 8;
 constexpr int kNarrowPitch = 33;
 __host__ inline int64_t narrow_staging(int m) { return (int64_t)kNarrowWarps * 16 * m * kNarrowPitch * 4; }
-constexpr int64_t kNarrowMost = 64 * 1024;   // bytes of weights: two CTAs then share an SM
 
 // CTAs that the registers let share an SM (more would spill).
 __host__ __device__ constexpr int narrow_ctas(int xt, int nf) { return xt == kXFloat || (xt == kX8 && nf > 1) ? 2 : 3; }
@@ -562,17 +518,6 @@ __global__ void __launch_bounds__(32 * kNarrowWarps, narrow_ctas(kXT, kNF)) k_na
 // goes to `partial`, one line of n k + n sums per CTA of a slice's column;
 // k_sum_lines adds those in order.  Read once: grad_y and z per slice, x;
 // written once: grad_x.
-struct SmallGradArgs {
-    SmallArgs s;          // x, x_scale, w, z, z_scale, rows, k, n, split, act, types, alignments
-    const void* g0;
-    const void* g1;
-    void* grad_x;
-    float* partial;       // [gridDim.x][n k + n]: grad_w [n][k], then grad_bias [n]
-    bool need_x, need_w, need_b;
-    bool vec_gx;          // 16-byte accesses to grad_x's rows
-};
-
-constexpr int kGradWarps = 4;
 constexpr int kTilePitch = 72;   // 16-bit elements: rows 144 bytes apart, no bank conflicts for ldmatrix
 
 template <int kXT, int kParts> struct NarrowGradShape {
@@ -606,7 +551,6 @@ template <> struct GradType<kXHalf, false> { typedef __half type; };
 
 // kXT: the type of x (and, for 16-bit ones, of everything); kParts: 3 with
 // float32 weights; kNF: output channels / 8.
-__host__ __device__ constexpr int narrow_grad_ctas(int parts, int nf) { return parts == 3 ? 2 : nf > 2 ? 3 : 4; }
 
 // kG32: float32 gradients beside 16-bit operands.
 template <int kXT, int kParts, int kNF, bool kG32>
