@@ -257,7 +257,9 @@ __device__ __forceinline__ void values4(float* v, unsigned codes, float scale) {
     const __half2 a(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(codes & 0xffff), __NV_E4M3));
     const __half2 b(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(codes >> 16), __NV_E4M3));
     const float2 fa = __half22float2(a), fb = __half22float2(b);
-    v[0] = fa.x * scale; v[1] = fa.y * scale; v[2] = fb.x * scale; v[3] = fb.y * scale;
+    const uint64_t s = both(scale);
+    pair_to(mul2(pair_of(fa.x, fa.y), s), v[0], v[1]);
+    pair_to(mul2(pair_of(fb.x, fb.y), s), v[2], v[3]);
 }
 
 __device__ __forceinline__ float value1(uint8_t code, float scale) {

@@ -265,23 +265,37 @@ __device__ __forceinline__ void store_aligned(float* s, const float (&v)[16], vo
 
 // The same where rows lie on no 16-byte boundaries: a lane per column, two
 // rows at a time, all of the residual's loads before the first store.
+template <typename T>
+__device__ __forceinline__ void store_any_as(const float* s, T* dst, const MmaArgs& p, int64_t row0, int64_t col0,
+                                             const T* add, int lane) {
+    const int rows = (int)min((int64_t)32, p.ni - row0) - (lane >> 4);   // of this lane, every second
+    const int64_t col = col0 + (lane & 15), at = (row0 + (lane >> 4)) * p.nj + col;
+    if (col >= p.nj) return;
+    T* out = dst + at;
+    const int64_t step = 2 * p.nj;
+    float x[16];
+    if (add) {
+        const T* in = add + at;
+#pragma unroll
+        for (int i = 0; i < 16; ++i, in += step) x[i] = 2 * i < rows ? to_f32(*in) : 0.f;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i, out += step)
+        if (2 * i < rows) *out = from_f32<T>(x[i] + staged_at(s, (lane >> 4) + 2 * i, lane & 15));
+}
+
 __device__ __forceinline__ void store_any(float* s, const float (&v)[16], void* dst, const MmaArgs& p, int64_t row0,
                                           int64_t col0, const void* add, int lane) {
     stage_rows(s, v, lane);
-    const int rows = (int)min((int64_t)32, p.ni - row0);
-    const int64_t col = col0 + (lane & 15);
-    if (col >= p.nj) return;
-    float x[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const int r = (lane >> 4) + 2 * i;
-        x[i] = add && r < rows ? load_param(add, p.out_dtype, (row0 + r) * p.nj + col) : 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const int r = (lane >> 4) + 2 * i;
-        if (r < rows) store_param(dst, p.out_dtype, (row0 + r) * p.nj + col, x[i] + staged_at(s, r, lane & 15));
-    }
+    if (p.out_dtype == PLATTICE_F32)
+        store_any_as(s, static_cast<float*>(dst), p, row0, col0, static_cast<const float*>(add), lane);
+    else if (p.out_dtype == PLATTICE_BF16)
+        store_any_as(s, static_cast<__nv_bfloat16*>(dst), p, row0, col0, static_cast<const __nv_bfloat16*>(add), lane);
+    else
+        store_any_as(s, static_cast<__half*>(dst), p, row0, col0, static_cast<const __half*>(add), lane);
 }
 
 // Two tensors of a split: columns below `split` and the others.

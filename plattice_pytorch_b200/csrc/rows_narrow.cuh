@@ -512,7 +512,7 @@ __global__ void __launch_bounds__(32 * kNarrowWarps, narrow_ctas(kXT, kNF)) k_na
 // ------------------------------------ backward, at most 32 output channels
 //
 // One pass: a warp takes 16 rows and a slice of 64 input channels, makes gz
-// (grad_y act'(z), rounded to the operands' type) once in shared memory, and
+// (grad_y act'(z)) once in shared memory, and
 // from it the rows' grad_x (gz w) and its share of grad_w (x^T gz, kept in
 // registers over all of the warp's rows) and grad_bias.  What a CTA gathered
 // goes to `partial`, one line of n k + n sums per CTA of a slice's column;
@@ -520,28 +520,41 @@ __global__ void __launch_bounds__(32 * kNarrowWarps, narrow_ctas(kXT, kNF)) k_na
 // written once: grad_x.
 constexpr int kTilePitch = 72;   // 16-bit elements: rows 144 bytes apart, no bank conflicts for ldmatrix
 
+// kParts: of the weights, 3 with float32 ones.  gz has 3 parts then, else 2:
+// it is made here in float32, and a second 16-bit part (28 more matrix
+// instructions a block of rows, 8 % of the pass) keeps what rounding it to
+// one would add to both gradients' errors.
 template <int kXT, int kParts> struct NarrowGradShape {
     static constexpr int kPX = kXT == kXFloat ? 3 : 1;
+    static constexpr int kPZ = kParts == 3 ? 3 : 2;
     static constexpr int kFragBytes = kParts * 2 * 8 * 32 * 8;                        // weights of the slice
     static constexpr int kWarpBytes = 16 * kNarrowPitch * 4 + kPX * 16 * kTilePitch * 2;
     static constexpr int kBytes = kFragBytes + kGradWarps * kWarpBytes + 64 * 33 * 4;
 };
 
-template <int kP>
-__device__ __forceinline__ void to_parts(float a, float b, bool half, uint32_t (&o)[kP]) {
-    if (kP == 3) {
-        uint32_t t[3];
-        split3_pair(a, b, t);
-#pragma unroll
-        for (int i = 0; i < kP; ++i) o[i] = t[i];
-    } else if (half) {
-        union { __half2 h; uint32_t u; } x;
-        x.h = __floats2half2_rn(a, b);
-        o[0] = x.u;
+// a and b as kP packed parts: one rounded, two (rounded, and what that left),
+// or split3's three.
+template <int kP, bool kHalf>
+__device__ __forceinline__ void to_parts(float a, float b, uint32_t (&o)[kP]) {
+    if constexpr (kP == 3) {
+        split3_pair(a, b, o);
     } else {
-        union { __nv_bfloat162 h; uint32_t u; } x;
-        x.h = __floats2bfloat162_rn(a, b);
-        o[0] = x.u;
+#pragma unroll
+        for (int i = 0; i < kP; ++i) {
+            if (kHalf) {
+                union { __half2 h; uint32_t u; } x;
+                x.h = __floats2half2_rn(a, b);
+                o[i] = x.u;
+                a -= __low2float(x.h);
+                b -= __high2float(x.h);
+            } else {
+                union { __nv_bfloat162 h; uint32_t u; } x;
+                x.h = __floats2bfloat162_rn(a, b);
+                o[i] = x.u;
+                a -= __low2float(x.h);
+                b -= __high2float(x.h);
+            }
+        }
     }
 }
 
@@ -557,7 +570,7 @@ template <int kXT, int kParts, int kNF, bool kG32>
 __global__ void __launch_bounds__(32 * kGradWarps, narrow_grad_ctas(kParts, kNF)) k_narrow_grad(const SmallGradArgs a) {
     typedef NarrowGradShape<kXT, kParts> Shape;
     typedef typename GradType<kXT, kG32>::type TG;
-    constexpr int kPX = Shape::kPX, kKS = kNF > 2 ? 2 : 1;   // steps of 16 output channels in grad_x's sum
+    constexpr int kPX = Shape::kPX, kPZ = Shape::kPZ, kKS = kNF > 2 ? 2 : 1;   // steps of 16 output channels in grad_x's sum
     constexpr bool kHalf = kXT == kXHalf;
     extern __shared__ __align__(16) char smem_raw[];
     uint2* frag = reinterpret_cast<uint2*>(smem_raw);   // [kParts][kKS][8][32]
@@ -580,8 +593,8 @@ __global__ void __launch_bounds__(32 * kGradWarps, narrow_grad_ctas(kParts, kNF)
             for (int j = 0; j < 4; ++j)
                 v[j] = o + j < n && ch < k ? load_param(a.s.w, a.s.w_dtype, (int64_t)(o + j) * k + ch) : 0.f;
             uint32_t lo[kParts], hi[kParts];
-            to_parts<kParts>(v[0], v[1], kHalf, lo);
-            to_parts<kParts>(v[2], v[3], kHalf, hi);
+            to_parts<kParts, kHalf>(v[0], v[1], lo);
+            to_parts<kParts, kHalf>(v[2], v[3], hi);
 #pragma unroll
             for (int p = 0; p < kParts; ++p) frag[p * kKS * 256 + i] = make_uint2(lo[p], hi[p]);
         }
@@ -704,17 +717,17 @@ __global__ void __launch_bounds__(32 * kGradWarps, narrow_grad_ctas(kParts, kNF)
             for (int r = 0; r < 16; ++r) db += st[r * kNarrowPitch + lane];
         }
         if (a.need_x) {
-            uint32_t o[kKS][kParts][4];
+            uint32_t o[kKS][kPZ][4];
 #pragma unroll
             for (int s = 0; s < kKS; ++s)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const float* p = st + (g + 8 * h) * kNarrowPitch + t * cols_per_lane + s * 4;
-                    uint32_t lo[kParts], hi[kParts];
-                    to_parts<kParts>(p[0], p[1], kHalf, lo);
-                    to_parts<kParts>(p[2], p[3], kHalf, hi);
+                    uint32_t lo[kPZ], hi[kPZ];
+                    to_parts<kPZ, kHalf>(p[0], p[1], lo);
+                    to_parts<kPZ, kHalf>(p[2], p[3], hi);
 #pragma unroll
-                    for (int q = 0; q < kParts; ++q) {
+                    for (int q = 0; q < kPZ; ++q) {
                         o[s][q][h] = lo[q];
                         o[s][q][2 + h] = hi[q];
                     }
@@ -725,9 +738,9 @@ __global__ void __launch_bounds__(32 * kGradWarps, narrow_grad_ctas(kParts, kNF)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) dx[f][i] = 0.f;
 #pragma unroll
-                for (int sum = 2; sum >= 0; --sum)   // small products first
+                for (int sum = kPZ - 1; sum >= 0; --sum)   // small products first
 #pragma unroll
-                    for (int pa = 0; pa < kParts; ++pa) {
+                    for (int pa = 0; pa < kPZ; ++pa) {
                         const int pb = sum - pa;
                         if (pb < 0 || pb >= kParts) continue;
 #pragma unroll
@@ -755,16 +768,16 @@ __global__ void __launch_bounds__(32 * kGradWarps, narrow_grad_ctas(kParts, kNF)
             }
         }
         if (a.need_w) {
-            uint32_t b[kParts][kNF][2];
+            uint32_t b[kPZ][kNF][2];
 #pragma unroll
             for (int f = 0; f < kNF; ++f)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const float* p = st + (2 * t + 8 * h) * kNarrowPitch + f * 8 + g;
-                    uint32_t o[kParts];
-                    to_parts<kParts>(p[0], p[kNarrowPitch], kHalf, o);
+                    uint32_t o[kPZ];
+                    to_parts<kPZ, kHalf>(p[0], p[kNarrowPitch], o);
 #pragma unroll
-                    for (int q = 0; q < kParts; ++q) b[q][f][h] = o[q];
+                    for (int q = 0; q < kPZ; ++q) b[q][f][h] = o[q];
                 }
 #pragma unroll
             for (int m = 0; m < 4; ++m) {
@@ -779,11 +792,11 @@ __global__ void __launch_bounds__(32 * kGradWarps, narrow_grad_ctas(kParts, kNF)
                                  : "memory");
                 }
 #pragma unroll
-                for (int sum = 2; sum >= 0; --sum)
+                for (int sum = kPZ - 1; sum >= 0; --sum)
 #pragma unroll
                     for (int px = 0; px < kPX; ++px) {
                         const int pb = sum - px;
-                        if (pb < 0 || pb >= kParts) continue;
+                        if (pb < 0 || pb >= kPZ) continue;
 #pragma unroll
                         for (int f = 0; f < kNF; ++f)
                             mma16816<kHalf>(dw[m][f], x[px][0], x[px][1], x[px][2], x[px][3],
