@@ -240,10 +240,15 @@ int status_poll(const char** name, unsigned* seq) {
     return st;
 }
 
-unsigned* fault_word() {
+unsigned* fault_word(cudaStream_t stream) {
     Ring& r = ring();
     std::lock_guard<std::mutex> lk(r.mu);
     if (!r.fault_host && !r.fault_unavailable) {
+        cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+        if (cudaStreamIsCapturing(stream, &capture) != cudaSuccess || capture != cudaStreamCaptureStatusNone) {
+            cudaGetLastError();
+            return nullptr;
+        }
         void *p = nullptr, *d = nullptr;
         if (cudaHostAlloc(&p, sizeof(unsigned), cudaHostAllocPortable | cudaHostAllocMapped) != cudaSuccess ||
             cudaHostGetDevicePointer(&d, p, 0) != cudaSuccess || !d) {

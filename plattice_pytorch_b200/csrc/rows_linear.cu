@@ -80,7 +80,7 @@ constexpr int kTogether = 2;
 // and the sums of the unrounded gz over a CTA's rows.  2^shift threads of 8
 // columns share a row; gridDim.x strips of columns, gridDim.y parts of rows.
 template <typename TG, typename T, bool kFast>
-__global__ void __launch_bounds__(256, 3) k_grad_z(const GradArgs a) {
+__global__ void __launch_bounds__(256, 4) k_grad_z(const GradArgs a) {
     __shared__ float sums[8 * 256];
     const int lane = threadIdx.x & ((1 << a.shift) - 1), rows = 256 >> a.shift;
     const int col = ((int)blockIdx.x << (a.shift + 3)) + lane * 8;
@@ -413,10 +413,21 @@ struct BackwardPlan {
     int64_t gz, x, w, partial_b, partial_w, pitch, bytes;
 };
 
+// Whether the backward runs in one pass over slices of 64 input channels
+// (k_narrow_grad), each of which makes gz anew, or as tiled products.  Measured
+// (us, one pass / tiles), 16-bit types: n 16, k 512, 65536 rows 48 / 55; k 1896,
+// 34559 rows 119 / 93, from 8 bits 115 / 125; from 8 bits n 32: k 128, 262144
+// rows 76 / 76, k 256 135 / 125; float32 n 8, k 2048, 8192 rows 72 / 115.
+static bool backward_is_narrow(const plattice_linear_args* a) {
+    if (a->n > 32) return false;
+    if (a->dtype == PLATTICE_F32 || a->k <= 128) return true;
+    return a->n <= 24 && (a->x_scale || a->k <= 768);
+}
+
 static BackwardPlan backward_plan(const plattice_linear_args* a) {
     BackwardPlan p{};
     Carve c;
-    p.narrow = a->n <= 32;
+    p.narrow = backward_is_narrow(a);
     if (p.narrow) {
         // one round of CTAs over the slices of 64 channels
         const int64_t slices = ceil_div(a->k, 64), need = ceil_div(ceil_div(a->rows, 16), kGradWarps);
@@ -490,7 +501,7 @@ static cudaError_t forward_mma(const plattice_linear_args* a, const ForwardPlan&
     const bool aligned = a->n % 8 == 0 && aligned16(a->y0) && (!a->residual || aligned16(a->residual)) &&
                          (!a->z || a->z_scale || aligned16(a->z));
     m.half = a->dtype == PLATTICE_F16;
-    m.fault = pl::fault_word();
+    m.fault = pl::fault_word(s);
     sum_args(&m, a->k, 1, x.parts, w.parts);
     return mma_forward(p.bn, aligned, x, w, m, s);
 }
@@ -557,7 +568,7 @@ static cudaError_t backward_mma(const plattice_linear_args* a, const BackwardPla
     cudaError_t e = cudaSuccess;
     MmaArgs m{};
     m.half = a->dtype == PLATTICE_F16;
-    m.fault = pl::fault_word();
+    m.fault = pl::fault_word(s);
     if (a->grad_x) {
         Operand w;
         e = operand(&w, a->w, a->dtype, a->n, a->k, ws + p.w, s);
@@ -632,6 +643,7 @@ int plattice_linear_backward(const plattice_linear_args* a, void* stream) {
             e = cudaMemsetAsync(a->grad_bias, 0, (size_t)a->n * dtype_size(a->bias_dtype), s);
         return rows_status(e, "plattice_linear_backward");
     }
+    if (!a->grad_x && !a->grad_w && !a->grad_bias) return PLATTICE_OK;
     if (!a->grad0 || (a->split && !a->grad1) || (a->grad_x && !a->w) || (a->grad_w && !a->x) ||
         (a->act != PLATTICE_ACT_NONE && !a->z))
         return PLATTICE_ERR_INVALID;

@@ -153,15 +153,30 @@ struct Tile {
     int part, begin, end;   // slices [begin, end) of the sum
 };
 
-// Tiles are numbered along j first, then i, then the parts of the sum.
+// Tiles of a part are numbered in bands of kBand columns of tiles, along j
+// first: the tiles that run at a time then form a block about as high as it is
+// wide (148 SMs: 12 x 12 of 128 x 256), which shares most of the slices it
+// reads.  Parts of the sum come one after the other.
+constexpr unsigned kBand = 12;
+
 template <int kBN>
 __device__ __forceinline__ Tile tile_at(const MmaArgs& p, unsigned t) {
     const unsigned nj = (unsigned)((p.nj + kBN - 1) / kBN), ni = (unsigned)((p.ni + kBM - 1) / kBM);
     Tile r;
-    const unsigned u = t / nj;
-    r.j0 = (int64_t)(t - u * nj) * kBN;
-    r.part = (int)(u / ni);
-    r.i0 = (int64_t)(u - r.part * ni) * kBM;
+    r.part = 0;
+    if (p.parts > 1) {
+        r.part = (int)(t / (ni * nj));
+        t -= r.part * (ni * nj);
+    }
+    unsigned first = 0, width = nj;
+    if (nj > kBand + kBand / 2) {   // up to there one band
+        first = t / (ni * kBand) * kBand;
+        t -= first * ni;
+        width = min(kBand, nj - first);
+    }
+    const unsigned i = t / width;
+    r.i0 = (int64_t)i * kBM;
+    r.j0 = (int64_t)(first + t - i * width) * kBN;
     r.begin = r.part * p.part_steps;
     r.end = min(p.steps, r.begin + p.part_steps);
     return r;

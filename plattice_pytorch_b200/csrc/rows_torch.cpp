@@ -86,7 +86,7 @@ py::object rows_pack8(const py::object& x_) {
     const at::Tensor* x = floating(x_);
     if (!rows_tensor(x)) return py::none();
     const int64_t c = x->size(-1), rows = x->numel() / c;
-    if (c > INT_MAX) return py::none();
+    if (c > (1 << 30)) return py::none();
     const c10::cuda::CUDAGuard guard(x->device());
     const Rows8 r = empty8(rows, c, x->options());
     const int rc = g_rows.pack8(r.q.data_ptr<uint8_t>(), r.scale.data_ptr<uint8_t>(), x->data_ptr(),
@@ -185,7 +185,7 @@ Input input_of(const py::object& x_, const py::object& scale_, const py::object&
 }
 
 bool weight_ok(const at::Tensor* w) {
-    return w && w->dim() == 2 && w->size(0) >= 1 && w->size(1) >= 1 && w->size(0) <= INT_MAX && w->size(1) <= INT_MAX;
+    return w && w->dim() == 2 && w->size(0) >= 1 && w->size(1) >= 1 && w->size(0) <= (1 << 30) && w->size(1) <= (1 << 30);
 }
 
 // keep: 0 nothing, 1 as 8-bit rows, 2 in the output's type.  Gives

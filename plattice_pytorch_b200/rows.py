@@ -35,6 +35,7 @@ _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
 _KEEP = {None: 0, "8bit": 1, "full": 2}
 _MAX_NORM = 16384
+_MAX_CHANNELS = 1 << 30
 
 
 def _width8(c):
@@ -54,7 +55,8 @@ class Rows8:
         _check_input(q, "q")
         _check_input(scale, "scale")
         _require(q.dtype == torch.uint8 and scale.dtype == torch.uint8, "q and scale must be uint8")
-        _require(len(shape) >= 1 and min(shape) >= 0 and shape[-1] >= 1, "shape must be [..., c] with c >= 1")
+        _require(len(shape) >= 1 and min(shape) >= 0 and 1 <= shape[-1] <= _MAX_CHANNELS,
+                 "shape must be [..., c] with 1 <= c <= 2^30")
         rows, width = _rows_of(shape), _width8(shape[-1])
         _require(tuple(q.shape) == (rows, width), f"q must be [{rows}, {width}] for shape {shape}")
         _require(tuple(scale.shape) == (rows, width // 32), f"scale must be [{rows}, {width // 32}] for shape {shape}")
@@ -83,7 +85,7 @@ def _empty8(shape, device):
 def _check_rows(t, name, channels=None):
     _check_input(t, name)
     _require(t.dtype in _DTYPES, f"{name} must be float32, bfloat16 or float16")
-    _require(t.dim() >= 1 and t.shape[-1] >= 1, f"{name} must be [..., channels]")
+    _require(t.dim() >= 1 and 1 <= t.shape[-1] <= _MAX_CHANNELS, f"{name} must be [..., channels], at most 2^30")
     _require(channels is None or int(t.shape[-1]) == channels, f"{name} must have {channels} channels")
 
 
@@ -247,7 +249,8 @@ def _linear_common(x, weight, act, out_dtype, lead=None):
     linear call; ``lead`` is that shape where ``x`` is None."""
     _check_input(weight, "weight")
     _require(weight.dtype in _DTYPES, "weight must be float32, bfloat16 or float16")
-    _require(weight.dim() == 2 and weight.shape[0] >= 1 and weight.shape[1] >= 1, "weight must be [n, k]")
+    _require(weight.dim() == 2 and 1 <= weight.shape[0] <= _MAX_CHANNELS and 1 <= weight.shape[1] <= _MAX_CHANNELS,
+             "weight must be [n, k], each at most 2^30")
     n, k = (int(s) for s in weight.shape)
     if isinstance(x, Rows8):
         _require(weight.dtype != torch.float16, "weight must be float32 or bfloat16 for 8-bit rows")

@@ -472,3 +472,75 @@ def test_refusals_on_the_device(dev, R):
             call()
     got = R.linear_backward(torch.ones(4, 3, device=dev), None, w, need=(True, False, True))
     assert got[0].shape == (4, 8) and got[1] is None and got[2].tolist() == [4.0, 4.0, 4.0]
+
+
+# Several tiles along each side, more tiles than SMs, bands of columns (n over
+# 18 tiles of 256), parts of the sum, depths that end inside a slice.
+BIG_SHAPES = [(300, 200, 5200), (20000, 72, 264), (5000, 1100, 96), (130, 2100, 1000)]
+
+
+@pytest.mark.parametrize("dtype,x8", KINDS)
+@pytest.mark.parametrize("rows,k,n", BIG_SHAPES)
+def test_linear_many_tiles(dev, R, rows, k, n, dtype, x8):
+    t = DTYPES[dtype]
+    x, xe, w = _linear_input(rows, k, n, t, x8, R, dev)
+    b, res = 0.3 * _randn((n,), 22), _randn((rows, n), 23, t)
+    y, z = R.linear(x, w.to(dev), b.to(dev), act="silu", residual=res.to(dev), keep="8bit")
+    ye, ze = ref.linear(xe, f64(w), f64(b), "silu", f64(res))
+    tol = _forward_tolerance(xe, f64(w), f64(b), ze, ye, k, t)
+    assert worst(f64(y), ye, tol + 2 * U * np.abs(f64(res))) <= 1
+    plain, _ = R.linear(x, w.to(dev), out_dtype=torch.float32)
+    pe, _ = ref.linear(xe, f64(w))
+    assert worst(f64(plain), pe, _forward_tolerance(xe, f64(w), None, pe * 0, pe, k, torch.float32)) <= 1
+    gy = _randn((rows, n), 26, t)
+    got = R.linear_backward(gy.to(dev), x, w.to(dev), z, act="silu", bias_dtype=torch.float32)
+    _check_gradients(got, f64(gy), xe, f64(w), f64(R.unpack8(z)), "silu", t, t)
+
+
+@pytest.mark.parametrize("n,k", [(8, 200), (24, 130), (32, 64), (17, 1000)])
+@pytest.mark.parametrize("dtype,x8", KINDS)
+def test_linear_narrow_many_rows(dev, R, n, k, dtype, x8):
+    """More blocks of rows than warps, several slices of channels."""
+    t, rows = DTYPES[dtype], 30011
+    x, xe, w = _linear_input(rows, k, n, t, x8, R, dev)
+    y, z = R.linear(x, w.to(dev), act="gelu", keep="8bit")
+    ye, ze = ref.linear(xe, f64(w), None, "gelu")
+    assert worst(f64(y), ye, _forward_tolerance(xe, f64(w), None, ze, ye, k, t)) <= 1
+    gy = _randn((rows, n), 26, t)
+    got = R.linear_backward(gy.to(dev), x, w.to(dev), z, act="gelu", bias_dtype=torch.float32)
+    _check_gradients(got, f64(gy), xe, f64(w), f64(R.unpack8(z)), "gelu", t, t)
+
+
+def test_offsets_beyond_32_bits(dev, R):
+    """A tensor of more than 2^31 values: the last rows come out as they do alone."""
+    if torch.cuda.mem_get_info(dev)[0] < 24 << 30:
+        pytest.skip("needs 24 GB of free device memory")
+    rows, c = 1 << 20, 2112
+    assert rows * c > 1 << 31
+    tail = _randn((40, c), 80, torch.bfloat16).to(dev)
+    x = torch.zeros(rows, c, dtype=torch.bfloat16, device=dev)
+    x[-40:] = tail
+    r = R.pack8(x)
+    alone = R.pack8(tail)
+    assert torch.equal(r.q[-40:], alone.q) and torch.equal(r.scale[-40:], alone.scale) and not r.q[:-40].any()
+    assert torch.equal(R.unpack8(r, torch.bfloat16)[-40:], R.unpack8(alone, torch.bfloat16))
+    gain = _randn((c,), 81).to(dev)
+    y, _, rstd = R.rms_norm(x, gain)
+    ya, _, ra = R.rms_norm(tail, gain)
+    assert torch.equal(y[-40:], ya) and torch.equal(rstd[-40:], ra)
+    del y, rstd
+    w, gy = _randn((8, c), 82, torch.bfloat16, c ** -0.5).to(dev), torch.zeros(rows, 8, dtype=torch.bfloat16, device=dev)
+    gy[-40:] = _randn((40, 8), 83, torch.bfloat16).to(dev)
+    out, _ = R.linear(r, w, out_dtype=torch.float32)
+    xe = f64(R.unpack8(alone))
+    oe = xe @ f64(w).T
+    assert worst(f64(out[-40:]), oe, _forward_tolerance(xe, f64(w), None, oe * 0, oe, c, torch.float32)) <= 1
+    for src, se in ((r, xe), (x, f64(tail))):
+        got = R.linear_backward(gy, src, w, bias_dtype=torch.float32)
+        assert not got[0][:-40].any()
+        _check_gradients((got[0][-40:], got[1], got[2]), f64(gy[-40:]), se, f64(w), None, "none", torch.bfloat16,
+                         torch.bfloat16)
+    w = _randn((40, c), 84, torch.bfloat16, c ** -0.5).to(dev)
+    out, _ = R.linear(x, w)
+    oe = f64(tail) @ f64(w).T
+    assert worst(f64(out[-40:]), oe, _forward_tolerance(f64(tail), f64(w), None, oe * 0, oe, c, torch.bfloat16)) <= 1
