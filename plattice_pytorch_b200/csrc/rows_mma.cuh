@@ -44,7 +44,7 @@ enum Mode { kAny = 0, kAligned = 1, kPlain = 2 };
 // not (422 against 353 us at 32768 x 1024 -> 4096, gelu, residual, kept z).
 // For the plain stores of the gradients 8 do.
 __host__ __device__ constexpr int epilogue_warps(int kind) { return kind == 0 ? 16 : 8; }
-__host__ __device__ constexpr int role_threads(int kind) { return 128 + 32 * epilogue_warps(kind); }
+__host__ __device__ constexpr int role_threads(int kind) { return 64 + 32 * epilogue_warps(kind); }
 
 __host__ __device__ constexpr bool a_mn(int kind) { return kind == kGradW; }
 __host__ __device__ constexpr bool b_mn(int kind) { return kind != kForward; }
@@ -138,6 +138,23 @@ __device__ __forceinline__ void tmem_load16(float (&v)[16], uint32_t addr) {
     for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+__device__ __forceinline__ void tmem_load32(float (&v)[32], uint32_t addr) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr)
+        : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
 // Shared-memory operand descriptor of a slice in the 128-byte swizzle: 8-row
 // groups of 128 bytes lie 1024 bytes apart (along i for K-major, along r for
 // MN-major slices); MN-major groups of 64 columns lie 64 rows = 8192 bytes apart.
@@ -198,37 +215,36 @@ __device__ __forceinline__ float staged_at(const float* s, int row, int c) {
     return s[row * 16 + (((c >> 2) ^ ((row >> 1) & 3)) << 2) + (c & 3)];
 }
 
-__device__ __forceinline__ void stage_rows(float* s, const float (&v)[16], int lane) {
+__device__ __forceinline__ void stage_rows(float* s, const float* v, int lane) {
     __syncwarp();
 #pragma unroll
     for (int c = 0; c < 4; ++c) *staged(s, lane, c) = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
     __syncwarp();
 }
 
-// 32 x 16 of the residual as store_aligned's lanes take them, loaded a half
-// piece ahead: a load waited for at each store would cost a trip to HBM twice a
-// half (652 us against 422 at 32768 x 1024 -> 4096, gelu, residual, kept z).
+// 32 x 32 of the residual as store_aligned's lanes take them, loaded a piece
+// ahead: a load waited for at each store would cost a trip to HBM four times a
+// piece (652 us against 422 at 32768 x 1024 -> 4096, gelu, residual, kept z).
 struct Ahead {
-    uint4 r[2];   // twice 8 columns of a 16-bit type (float32 is loaded at the store)
+    uint4 r[4];   // twice 8 columns of each half, of a 16-bit type (float32 is loaded at the store)
     bool have;
 };
 
 template <int kOut>
 __device__ __forceinline__ void load_ahead(Ahead& a, const MmaArgs& p, int64_t row0, int64_t col0, int lane) {
-    a.have = kOut != PLATTICE_F32 && p.residual && col0 + 16 <= p.nj && row0 + 32 <= p.ni;
+    a.have = kOut != PLATTICE_F32 && p.residual && col0 + 32 <= p.nj && row0 + 32 <= p.ni;
     if (!a.have) return;
+    const uint16_t* src = static_cast<const uint16_t*>(p.residual) + (row0 + (lane >> 1)) * p.nj + col0 + (lane & 1) * 8;
 #pragma unroll
-    for (int it = 0; it < 2; ++it)
-        a.r[it] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.residual) +
-                                                  (row0 + it * 16 + (lane >> 1)) * p.nj + col0 + (lane & 1) * 8);
+    for (int i = 0; i < 4; ++i) a.r[i] = *reinterpret_cast<const uint4*>(src + (i & 1) * 16 * p.nj + (i >> 1) * 16);
 }
 
 // 16 columns of 32 rows (a row per lane) to (row0, col0) of an [ni][nj] tensor,
 // `add` (the residual, same layout) added: through the staging to two lanes a
 // row, 8 columns each.  nj is a multiple of 8: a lane's columns all exist or
 // none does.
-template <int kOut>
-__device__ __forceinline__ void store_aligned(float* s, const float (&v)[16], void* dst, const MmaArgs& p, int64_t row0,
+template <int kOut, int kHalf = 0>
+__device__ __forceinline__ void store_aligned(float* s, const float* v, void* dst, const MmaArgs& p, int64_t row0,
                                               int64_t col0, const void* add, const Ahead& ahead, int lane) {
     typedef typename OutType<kOut>::type T;
     const int rows = (int)min((int64_t)32, p.ni - row0), c = (lane & 1) * 8;
@@ -265,7 +281,7 @@ __device__ __forceinline__ void store_aligned(float* s, const float (&v)[16], vo
             Raw8<T> q;
             float t[8];
             if constexpr (sizeof(T) == 2) {
-                if (ahead.have) q.u = ahead.r[it];
+                if (ahead.have) q.u = ahead.r[kHalf * 2 + it];
                 else q.load(static_cast<const T*>(add) + (out - static_cast<T*>(dst)) + (int64_t)it * 16 * p.nj, true, 8);
             } else {
                 q.load(static_cast<const T*>(add) + (out - static_cast<T*>(dst)) + (int64_t)it * 16 * p.nj, true, 8);
@@ -302,7 +318,7 @@ __device__ __forceinline__ void store_any_as(const float* s, T* dst, const MmaAr
         if (2 * i < rows) *out = from_f32<T>(x[i] + staged_at(s, (lane >> 4) + 2 * i, lane & 15));
 }
 
-__device__ __forceinline__ void store_any(float* s, const float (&v)[16], void* dst, const MmaArgs& p, int64_t row0,
+__device__ __forceinline__ void store_any(float* s, const float* v, void* dst, const MmaArgs& p, int64_t row0,
                                           int64_t col0, const void* add, int lane) {
     stage_rows(s, v, lane);
     if (p.out_dtype == PLATTICE_F32)
@@ -314,7 +330,7 @@ __device__ __forceinline__ void store_any(float* s, const float (&v)[16], void* 
 }
 
 // Two tensors of a split: columns below `split` and the others.
-__device__ __forceinline__ void store_split(float* s, const float (&v)[16], const MmaArgs& p, int64_t row0,
+__device__ __forceinline__ void store_split(float* s, const float* v, const MmaArgs& p, int64_t row0,
                                             int64_t col0, int lane) {
     stage_rows(s, v, lane);
     const int rows = (int)min((int64_t)32, p.ni - row0), c = lane & 15;
@@ -327,7 +343,7 @@ __device__ __forceinline__ void store_split(float* s, const float (&v)[16], cons
     }
 }
 
-__device__ __forceinline__ void add_bias(float (&v)[16], const float* sb) {
+__device__ __forceinline__ void add_bias(float* v, const float* sb) {
 #pragma unroll
     for (int c = 0; c < 16; c += 4) {
         const float4 b = *reinterpret_cast<const float4*>(sb + c);
@@ -336,17 +352,58 @@ __device__ __forceinline__ void add_bias(float (&v)[16], const float* sb) {
     }
 }
 
-// Scale of the kept 8-bit rows: 32 columns are one block.
-struct Block8 {
-    int exponent;
+// A row's 32 columns, one block of the kept 8-bit rows: its codes and scale, a
+// lane's 32 bytes in one store (whole sectors).
+__device__ __forceinline__ void keep_codes(const float (&v)[32], const MmaArgs& p, int64_t row, int64_t col0) {
     bool infinite;
-    uint4 first;   // codes of the first half, stored together with the second's
-};
+    const int e = block_exponent(finite_amax_of(v, infinite));
+    if (row >= p.ni) return;
+    const float inv = pow2(-e);
+    uint2 q[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q[i] = codes8_of(v + 8 * i, inv, infinite);
+    const int64_t at = row * ((p.nj + 31) / 32) + (col0 >> 5);
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(static_cast<uint8_t*>(p.z) + at * 32),
+                 "r"(q[0].x), "r"(q[0].y), "r"(q[1].x), "r"(q[1].y), "r"(q[2].x), "r"(q[2].y), "r"(q[3].x), "r"(q[3].y)
+                 : "memory");
+    p.z_scale[at] = (uint8_t)(e + 127);
+}
 
-// Half a 32-column piece (16 columns from col0), a row per lane.
+// A 32-column piece of the forward, a row per lane, with whatever is asked for.
+template <int kOut, int kMode>
+__device__ __forceinline__ void finish32(float (&v)[32], const MmaArgs& p, int64_t row0, int64_t col0, float* s,
+                                         const Ahead& ahead, int lane) {
+    if (p.bias) {
+        add_bias(v, s + 32 * 16);
+        add_bias(v + 16, s + 32 * 16 + 16);
+    }
+    const bool second = col0 + 16 < p.nj;
+    if (p.z_scale) {
+        keep_codes(v, p, row0 + lane, col0);
+    } else if (p.z) {
+        if (kMode == kAligned) store_aligned<kOut>(s, v, p.z, p, row0, col0, nullptr, ahead, lane);
+        else store_any(s, v, p.z, p, row0, col0, nullptr, lane);
+        if (kMode == kAligned && second) store_aligned<kOut>(s, v + 16, p.z, p, row0, col0 + 16, nullptr, ahead, lane);
+        else if (second) store_any(s, v + 16, p.z, p, row0, col0 + 16, nullptr, lane);
+    }
+    activate(v, p.act);
+    if (kMode == kAligned) {
+        store_aligned<kOut, 0>(s, v, p.y0, p, row0, col0, p.residual, ahead, lane);
+        if (second) store_aligned<kOut, 1>(s, v + 16, p.y0, p, row0, col0 + 16, p.residual, ahead, lane);
+    } else if (p.split) {
+        store_split(s, v, p, row0, col0, lane);
+        if (second) store_split(s, v + 16, p, row0, col0 + 16, lane);
+    } else {
+        store_any(s, v, p.y0, p, row0, col0, p.residual, lane);
+        if (second) store_any(s, v + 16, p.y0, p, row0, col0 + 16, p.residual, lane);
+    }
+}
+
+// Half a 32-column piece (16 columns from col0) of a plain forward or a
+// gradient, a row per lane.
 template <int kKind, int kOut, int kMode>
 __device__ __forceinline__ void finish16(float (&v)[16], const MmaArgs& p, const Tile& t, int64_t row0, int64_t col0,
-                                         float* s, Ahead& ahead, Block8& block, int half, int lane) {
+                                         float* s, int half, int lane) {
     typedef typename OutType<kOut>::type T;
     if (kKind == kGradW) {
         // D is [input channel][output channel], its result [output channel]
@@ -361,33 +418,8 @@ __device__ __forceinline__ void finish16(float (&v)[16], const MmaArgs& p, const
         return;
     }
     if (kKind == kForward && p.bias) add_bias(v, s + 32 * 16 + half * 16);
-    if (kMode == kPlain) {
-        store_aligned<kOut>(s, v, p.y0, p, row0, col0, nullptr, ahead, lane);
-        return;
-    }
-    if (kKind == kForward && p.z_scale) {
-        const float inv = pow2(-block.exponent);
-        const uint2 x = codes8_of(v, inv, block.infinite), y = codes8_of(v + 8, inv, block.infinite);
-        if (half == 0) {
-            block.first = make_uint4(x.x, x.y, y.x, y.y);
-        } else if (row0 + lane < p.ni) {   // a lane's 32 bytes in one store: whole sectors
-            const int64_t at = (row0 + lane) * ((p.nj + 31) / 32) + (col0 >> 5);
-            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(static_cast<uint8_t*>(p.z) + at * 32),
-                         "r"(block.first.x), "r"(block.first.y), "r"(block.first.z), "r"(block.first.w), "r"(x.x),
-                         "r"(x.y), "r"(y.x), "r"(y.y)
-                         : "memory");
-            p.z_scale[at] = (uint8_t)(block.exponent + 127);
-        }
-    } else if (kKind == kForward && p.z && col0 < p.nj) {
-        if (kMode == kAligned) store_aligned<kOut>(s, v, p.z, p, row0, col0, nullptr, ahead, lane);
-        else store_any(s, v, p.z, p, row0, col0, nullptr, lane);
-    }
-    if (col0 >= p.nj) return;
-    const void* add = kKind == kForward ? p.residual : nullptr;
-    if (kKind == kForward) activate(v, p.act);
-    if (kMode == kAligned) store_aligned<kOut>(s, v, p.y0, p, row0, col0, add, ahead, lane);
-    else if (kKind == kForward && p.split) store_split(s, v, p, row0, col0, lane);
-    else store_any(s, v, p.y0, p, row0, col0, add, lane);
+    if (kMode == kPlain) store_aligned<kOut>(s, v, p.y0, p, row0, col0, nullptr, Ahead{}, lane);
+    else store_any(s, v, p.y0, p, row0, col0, nullptr, lane);
 }
 
 // -------------------------------------------------------------- the kernel
@@ -431,7 +463,7 @@ __global__ void __launch_bounds__(role_threads(kKind), 1)
         bar_init(drained, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 2) {
+    if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_slot)),
                      "r"(kColumns)
                      : "memory");
@@ -517,11 +549,11 @@ __global__ void __launch_bounds__(role_threads(kKind), 1)
                 while (!bar_try(drained, 0) && clock64() - begin < 200000000ll) {}
             }
         }
-    } else if (warp >= 4 && warp < 4 + kEpilogueWarps) {
+    } else {
         // ---- epilogue: warp w reads the 32 accumulator rows 32 (w % 4)..,
         // the warps of a quarter take turns over its 32-column pieces
-        const int quarter = warp & 3, group = (warp - 4) >> 2;
-        float* s = staging + (warp - 4) * (kWarpStaging / 4);
+        const int quarter = warp & 3, group = (warp - 2) >> 2;
+        float* s = staging + (warp - 2) * (kWarpStaging / 4);
         int n = 0;
         for (unsigned t = blockIdx.x; t < tiles; t += gridDim.x, ++n) {
             const Tile tile = tile_at<kBN>(p, t);
@@ -534,6 +566,11 @@ __global__ void __launch_bounds__(role_threads(kKind), 1)
                 const int64_t col = tile.j0 + c * 32 + lane;
                 bias = kKind == kForward && p.bias && c < kPieces && col < p.nj ? load_param(p.bias, p.bias_dtype, col) : 0.f;
             };
+            auto release = [&] {
+                fence_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(acc_empty(buf));
+            };
             ahead.have = false;
             bias_ahead(group);
             if (kKeeps && kMode == kAligned && group < kPieces) load_ahead<kOut>(ahead, p, row0, tile.j0 + group * 32, lane);
@@ -544,38 +581,29 @@ __global__ void __launch_bounds__(role_threads(kKind), 1)
             for (int c = group; c < kPieces; c += kGroups) {
                 const int64_t col0 = tile.j0 + c * 32;
                 const bool live = col0 < p.nj && row0 < p.ni;
-                float v[16];
-                Block8 block{0, false, {}};
+                const bool last = c + kGroups >= kPieces;
                 __syncwarp();
                 if (kKind == kForward && live && p.bias) {
                     s[32 * 16 + lane] = bias;
                     __syncwarp();
                 }
                 bias_ahead(c + kGroups);
-                if (kKeeps && live && p.z_scale) {
-                    float amax = 0.f;   // of both halves, which are read again below
+                if constexpr (kKeeps) {
+                    float v[32];
+                    tmem_load32(v, base + c * 32);
+                    if (last) release();   // the accumulator is free before any of the work on its values
+                    if (live) finish32<kOut, kMode>(v, p, row0, col0, s, ahead, lane);
+                    if (kMode == kAligned && !last) load_ahead<kOut>(ahead, p, row0, col0 + kGroups * 32, lane);
+                } else {
+                    float v[16];
 #pragma unroll 1
                     for (int h = 0; h < 2; ++h) {
-                        tmem_load16(v, base + c * 32 + h * 16);
-                        if (p.bias) add_bias(v, s + 32 * 16 + h * 16);
-                        bool infinite;
-                        amax = fmaxf(amax, finite_amax_of(v, infinite));
-                        block.infinite |= infinite;
-                    }
-                    block.exponent = block_exponent(amax);
-                }
-#pragma unroll 1
-                for (int h = 0; h < 2; ++h) {
-                    __syncwarp();
-                    tmem_load16(v, base + c * 32 + h * 16);
-                    if (h == 1 && c + kGroups >= kPieces) {
-                        fence_before();
                         __syncwarp();
-                        if (lane == 0) bar_arrive(acc_empty(buf));
+                        tmem_load16(v, base + c * 32 + h * 16);
+                        if (h == 1 && last) release();
+                        if (live && col0 + h * 16 < p.nj)
+                            finish16<kKind, kOut, kMode>(v, p, tile, row0, col0 + h * 16, s, h, lane);
                     }
-                    if (live) finish16<kKind, kOut, kMode>(v, p, tile, row0, col0 + h * 16, s, ahead, block, h, lane);
-                    const int64_t next = h == 0 ? col0 + 16 : col0 + kGroups * 32;
-                    if (kKeeps && kMode == kAligned && (h == 0 || c + kGroups < kPieces)) load_ahead<kOut>(ahead, p, row0, next, lane);
                 }
             }
             if (group >= kPieces && lane == 0) bar_arrive(acc_empty(buf));
@@ -585,7 +613,7 @@ __global__ void __launch_bounds__(role_threads(kKind), 1)
     fence_before();
     __syncthreads();
     fence_after();
-    if (warp == 2)
+    if (warp == 1)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kColumns) : "memory");
     if (threadIdx.x == 0 && dead_flag && p.fault) *reinterpret_cast<volatile unsigned*>(p.fault) = 1;
 }
