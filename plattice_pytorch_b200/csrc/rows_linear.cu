@@ -618,6 +618,7 @@ static cudaError_t backward_narrow(const plattice_linear_args* a, const Backward
     g.need_w = a->grad_w != nullptr;
     g.need_b = a->grad_bias != nullptr;
     g.vec_gx = a->k % 8 == 0 && aligned16(a->grad_x);
+    g.vec_g = aligned16(a->grad0) && (!a->split || aligned16(a->grad1));
     const cudaError_t e = run_narrow_grad(g, a->dtype, p.lines, s);
     if (e != cudaSuccess || !(a->grad_w || a->grad_bias)) return e;
     const int64_t nw = (int64_t)a->n * a->k, columns = nw + a->n;

@@ -528,7 +528,8 @@ template <int kXT, int kParts> struct NarrowGradShape {
     static constexpr int kPX = kXT == kXFloat ? 3 : 1;
     static constexpr int kPZ = kParts == 3 ? 3 : 2;
     static constexpr int kFragBytes = kParts * 2 * 8 * 32 * 8;                        // weights of the slice
-    static constexpr int kWarpBytes = 16 * kNarrowPitch * 4 + kPX * 16 * kTilePitch * 2;
+    static constexpr int kStaged = 16 * kNarrowPitch + 4;   // gz of 16 rows, and a place for what is behind them
+    static constexpr int kWarpBytes = kStaged * 4 + kPX * 16 * kTilePitch * 2;
     static constexpr int kBytes = kFragBytes + kGradWarps * kWarpBytes + 64 * 33 * 4;
 };
 
@@ -577,7 +578,7 @@ __global__ void __launch_bounds__(32 * kGradWarps, narrow_grad_ctas(kParts, kNF)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     char* mine = smem_raw + Shape::kFragBytes + warp * Shape::kWarpBytes;
     float* st = reinterpret_cast<float*>(mine);                                       // gz, 16 x 33
-    uint16_t* tile = reinterpret_cast<uint16_t*>(mine + 16 * kNarrowPitch * 4);       // x, [kPX][16][72]
+    uint16_t* tile = reinterpret_cast<uint16_t*>(mine + Shape::kStaged * 4);          // x, [kPX][16][72]
     float* gather = reinterpret_cast<float*>(smem_raw + Shape::kFragBytes + kGradWarps * Shape::kWarpBytes);
     const int ch0 = blockIdx.y * 64, n = a.s.n, k = a.s.k;
     const int cols_per_lane = kKS * 4;   // output channels of lane t in grad_x's sum: t cols_per_lane..
@@ -613,29 +614,41 @@ __global__ void __launch_bounds__(32 * kGradWarps, narrow_grad_ctas(kParts, kNF)
 
     const int64_t blocks = (a.s.rows + 15) / 16, stride = (int64_t)gridDim.x * kGradWarps;
     int64_t block = (int64_t)blockIdx.x * kGradWarps + warp;
-    constexpr int kRun = kNF * 4;   // 16 rows x 8 kNF columns / 32 lanes
-    // Element e = 32 i + lane of the rows' gradients: the run of g0's 16 rows,
-    // then g1's; where it goes in the staged rows, the same for every 16 rows.
+    // The rows' gradients are the run of g0's 16 rows, then g1's.  A lane takes
+    // kPer elements (16 bytes) from (32 i + lane) kPer on; where each goes in
+    // the staged rows is the same for every 16 rows.
+    constexpr int kPer = 16 / (int)sizeof(TG), kVecs = (16 * 8 * kNF / kPer + 31) / 32, kRun = kVecs * kPer;
     const int w0 = a.s.split ? a.s.split : n, w1 = n - w0, run0 = 16 * w0;
     uint16_t place[kRun];
 #pragma unroll
     for (int i = 0; i < kRun; ++i) {
-        const int e = i * 32 + lane;
-        place[i] = 0xffff;
+        const int e = (i / kPer * 32 + lane) * kPer + i % kPer;
+        place[i] = 16 * kNarrowPitch;
         if (e < run0) place[i] = (uint16_t)(e / w0 * kNarrowPitch + e % w0);
         else if (e < 16 * n) place[i] = (uint16_t)((e - run0) / w1 * kNarrowPitch + w0 + (e - run0) % w1);
     }
-    TG gn[kRun];                    // the next rows' gradients, x and z, loaded ahead
+    union { uint4 v[kVecs]; TG e[kRun]; } gn;   // the next rows' gradients, x and z, loaded ahead
     NarrowRaw<kXT> xn;
     uint4 zn = make_uint4(0, 0, 0, 0);
     uint8_t zs = 127;
     auto load_rows = [&](int64_t b) {
-        const TG* p0 = static_cast<const TG*>(a.g0) + b * 16 * w0 + lane;
-        const TG* p1 = static_cast<const TG*>(a.g1) + b * 16 * w1 + lane - run0;
-        const int limit = (int)min((int64_t)16, a.s.rows - b * 16) * kNarrowPitch;
+        const TG* p0 = static_cast<const TG*>(a.g0) + b * 16 * w0;
+        const TG* p1 = static_cast<const TG*>(a.g1) + b * 16 * w1 - run0;
+        const int rows = (int)min((int64_t)16, a.s.rows - b * 16);
+        if (a.vec_g && rows == 16) {
 #pragma unroll
-        for (int i = 0; i < kRun; ++i)
-            gn[i] = *(place[i] < limit ? (i * 32 + lane < run0 ? p0 : p1) + i * 32 : p0 - lane);
+            for (int i = 0; i < kVecs; ++i) {
+                const int e = (i * 32 + lane) * kPer;
+                gn.v[i] = *reinterpret_cast<const uint4*>(e < run0 ? p0 + e : e < 16 * n ? p1 + e : p0);
+            }
+        } else {   // rows on other boundaries, and the last ones
+            const int limit = rows * kNarrowPitch;
+#pragma unroll
+            for (int i = 0; i < kRun; ++i) {
+                const int e = (i / kPer * 32 + lane) * kPer + i % kPer;
+                gn.e[i] = *(place[i] < limit ? e < run0 ? p0 + e : p1 + e : p0);
+            }
+        }
         if (a.s.z_scale) {   // a lane per half row
             const int64_t row = min(b * 16 + (lane >> 1), a.s.rows - 1);   // behind the last: its own, times 0
             zn = reinterpret_cast<const uint4*>(a.s.z)[row * 2 + (lane & 1)];
@@ -649,9 +662,13 @@ __global__ void __launch_bounds__(32 * kGradWarps, narrow_grad_ctas(kParts, kNF)
         const int64_t row0 = block * 16;
         const int rows = (int)min((int64_t)16, a.s.rows - row0);
         __syncwarp();
+        if (rows == 16) {
 #pragma unroll
-        for (int i = 0; i < kRun; ++i)   // 0 behind the last row
-            if (place[i] != 0xffff) st[place[i]] = place[i] < rows * kNarrowPitch ? to_f32(gn[i]) : 0.f;
+            for (int i = 0; i < kRun; ++i) st[place[i]] = to_f32(gn.e[i]);
+        } else {   // 0 behind the last row
+#pragma unroll
+            for (int i = 0; i < kRun; ++i) st[place[i]] = place[i] < rows * kNarrowPitch ? to_f32(gn.e[i]) : 0.f;
+        }
         if (a.need_w) {   // x, widened, into the tile
             narrow_mask<kXT, 1>(xn, k, blockIdx.y, lane);
 #pragma unroll

@@ -31,6 +31,7 @@ struct SmallGradArgs {
     float* partial;       // [gridDim.x][n k + n]: grad_w [n][k], then grad_bias [n]
     bool need_x, need_w, need_b;
     bool vec_gx;          // 16-byte accesses to grad_x's rows
+    bool vec_g;           // g0 and g1 begin on 16-byte boundaries
 };
 
 __host__ __device__ inline int narrow_steps(int k) { return (k + 63) / 64 * 4; }   // of 16 channels
