@@ -41,11 +41,17 @@ struct MmaArgs {
     unsigned pairs_a, pairs_b;   // parts of A and B of each product, 2 bits each
     int pairs;
     bool half;            // operands are float16 (else bfloat16)
+    bool precise;         // the result ends in float32 (not in 16 bits after a float32 sum of parts)
     unsigned* fault;      // host-mapped word that reports a wait that gave up (may be null)
 };
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline int64_t mma_tiles(int64_t ni, int64_t nj, int bn) { return ceil_div(ni, kBM) * ceil_div(nj, bn); }
+
+// Whether a sum of `steps` slices goes in chunks (rows_mma.cuh, kChunk).
+inline bool chunked(int steps, int out_dtype, bool precise) {
+    return precise && out_dtype == PLATTICE_F32 && steps > 8;
+}
 
 // TMA map of an operand: boxes of 64 columns x box_rows rows, zeros outside.
 cudaError_t make_map(CUtensorMap* m, const Operand& o, int box_rows);

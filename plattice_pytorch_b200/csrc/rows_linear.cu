@@ -400,10 +400,10 @@ static double slice_cost(int bn) { return bn == 256 ? 512 : bn == 128 ? 300 : bn
 // Columns of a tile: the cheapest number of rounds over the device's SMs
 // (wide tiles do more per byte staged, narrow ones fill the device when D is
 // small and waste less when it is narrow).
-static int choose_bn(int64_t ni, int64_t nj, int least) {
+static int choose_bn(int64_t ni, int64_t nj, int least, bool deep) {
     int best = least;
     double cost = 1e300;
-    for (int bn = 256; bn >= least; bn /= 2) {
+    for (int bn = deep ? 128 : 256; bn >= least; bn /= 2) {
         const double c = (double)ceil_div(mma_tiles(ni, nj, bn), sm_count()) * slice_cost(bn);
         if (c < cost) cost = c, best = bn;
     }
@@ -473,7 +473,7 @@ static ForwardPlan forward_plan(const plattice_linear_args* a) {
     Carve c;
     p.way = forward_way(a);
     if (p.way == kWayTiles) {
-        p.bn = choose_bn(a->rows, a->n, 32);
+        p.bn = choose_bn(a->rows, a->n, 32, chunked((int)ceil_div(a->k, kBK), a->out_dtype, true));
         if (a->x_scale) p.x = c.take(a->rows * up8(a->k) * 2);
         else if (!tma_ready(a->x, a->dtype, a->k)) p.x = c.take(repack_bytes(a->dtype, a->rows, a->k));
         p.w = tma_ready(a->w, a->dtype, a->k) ? 0 : c.take(repack_bytes(a->dtype, a->n, a->k));
@@ -527,8 +527,9 @@ static BackwardPlan backward_plan(const plattice_linear_args* a) {
                     tma_ready(a->grad0, a->dtype, a->n));
     p.pitch = up8(a->n);
     if (p.gz_needed) p.gz = c.take(repack_bytes(a->dtype, a->rows, a->n));
-    p.bn_x = choose_bn(a->rows, a->k, 64);
-    p.bn_w = a->n > 128 ? 256 : a->n > 64 ? 128 : 64;
+    p.bn_x = choose_bn(a->rows, a->k, 64, chunked((int)ceil_div(a->n, kBK), a->dtype, true));
+    const bool deep_w = a->dtype == PLATTICE_F32 && a->rows > 8 * kBK;   // chunks, or parts no deeper than one
+    p.bn_w = a->n > 128 && !deep_w ? 256 : a->n > 64 ? 128 : 64;
     p.parts_w = choose_parts(a->k, a->n, p.bn_w, ceil_div(a->rows, kBK));
     if (a->grad_x && !tma_ready(a->w, a->dtype, a->k)) p.w = c.take(repack_bytes(a->dtype, a->n, a->k));
     if (a->grad_w && a->x_scale) p.x = c.take(a->rows * up8(a->k) * 2);
@@ -588,6 +589,7 @@ static cudaError_t forward_mma(const plattice_linear_args* a, const ForwardPlan&
                          (!a->z || a->z_scale || aligned16(a->z));
     m.half = a->dtype == PLATTICE_F16;
     m.fault = pl::fault_word(s);
+    m.precise = true;
     sum_args(&m, a->k, 1, x.parts, w.parts);
     return mma_forward(p.bn, aligned, x, w, m, s);
 }
@@ -664,6 +666,7 @@ static cudaError_t backward_mma(const plattice_linear_args* a, const BackwardPla
         m.ni = a->rows;
         m.nj = a->k;
         m.out_dtype = a->dtype;
+        m.precise = true;
         sum_args(&m, a->n, 1, gz.parts, w.parts);
         e = mma_grad_x(p.bn_x, a->k % 8 == 0 && aligned16(a->grad_x), gz, w, m, s);
         if (e != cudaSuccess) return e;
@@ -679,6 +682,7 @@ static cudaError_t backward_mma(const plattice_linear_args* a, const BackwardPla
         const bool direct = p.parts_w == 1;
         m.y0 = direct ? a->grad_w : ws + p.partial_w;
         m.out_dtype = direct ? a->dtype : PLATTICE_F32;
+        m.precise = a->dtype == PLATTICE_F32;
         e = mma_grad_w(p.bn_w, x, gz, m, s);
         if (e == cudaSuccess && !direct)
             e = add_parts_to(a->grad_w, a->dtype, reinterpret_cast<const float*>(ws + p.partial_w), m.parts,

@@ -43,8 +43,16 @@ enum Mode { kAny = 0, kAligned = 1, kPlain = 2 };
 // residual, 8-bit codes) waits more than it issues: 16 warps hide what 8 do
 // not (422 against 353 us at 32768 x 1024 -> 4096, gelu, residual, kept z).
 // For the plain stores of the gradients 8 do.
-__host__ __device__ constexpr int epilogue_warps(int kind) { return kind == 0 ? 16 : 8; }
-__host__ __device__ constexpr int role_threads(int kind) { return 64 + 32 * epilogue_warps(kind); }
+__host__ __device__ constexpr int epilogue_warps(int kind, bool chunked) { return kind == 0 || chunked ? 16 : 8; }
+__host__ __device__ constexpr int role_threads(int kind, bool chunked) { return 64 + 32 * epilogue_warps(kind, chunked); }
+
+// A float32 result of a deep sum (kChunked): the MMA cuts where an addition
+// rounds, so that an accumulator drifts by about 2^-26 of itself with each of
+// them (1.1e-6 of the result at a depth of 1024, 4.5e-6 at 4096).  The sum then
+// goes in chunks of kChunk slices through the two accumulators, and the
+// epilogue adds those in registers, rounding; a warp holds one 32-column
+// piece, so tiles are at most 128 wide.
+constexpr int kChunk = 8;
 
 __host__ __device__ constexpr bool a_mn(int kind) { return kind == kGradW; }
 __host__ __device__ constexpr bool b_mn(int kind) { return kind != kForward; }
@@ -52,13 +60,15 @@ __host__ __device__ constexpr bool b_mn(int kind) { return kind != kForward; }
 __host__ __device__ constexpr int b_columns(int kind, int bn) { return b_mn(kind) && bn < 64 ? 64 : bn; }
 __host__ __device__ constexpr int stage_bytes(int kind, int bn) { return kStageA + b_columns(kind, bn) * kBK * 2; }
 constexpr int kWarpStaging = 32 * 16 * 4 + 32 * 4;   // a 32 x 16 float tile and 32 biases
-__host__ __device__ constexpr int fixed_smem(int kind) { return 1024 + epilogue_warps(kind) * kWarpStaging + 256; }
-__host__ __device__ constexpr int stages(int kind, int bn) {
-    const int n = (kMaxSmem - 16 - fixed_smem(kind)) / stage_bytes(kind, bn);
+__host__ __device__ constexpr int fixed_smem(int kind, bool chunked) {
+    return 1024 + epilogue_warps(kind, chunked) * kWarpStaging + 256;
+}
+__host__ __device__ constexpr int stages(int kind, int bn, bool chunked) {
+    const int n = (kMaxSmem - 16 - fixed_smem(kind, chunked)) / stage_bytes(kind, bn);
     return n > 8 ? 8 : n;
 }
-__host__ __device__ constexpr int smem_bytes(int kind, int bn) {
-    return fixed_smem(kind) + stages(kind, bn) * stage_bytes(kind, bn);
+__host__ __device__ constexpr int smem_bytes(int kind, int bn, bool chunked) {
+    return fixed_smem(kind, chunked) + stages(kind, bn, chunked) * stage_bytes(kind, bn);
 }
 
 // ------------------------------------------------------------- PTX wrappers
@@ -425,11 +435,11 @@ __device__ __forceinline__ void finish16(float (&v)[16], const MmaArgs& p, const
 // -------------------------------------------------------------- the kernel
 
 // kOut: the type of y0 (kAny: looked up).
-template <int kKind, int kBN, int kOut, int kMode>
-__global__ void __launch_bounds__(role_threads(kKind), 1)
+template <int kKind, int kBN, int kOut, int kMode, bool kChunked>
+__global__ void __launch_bounds__(role_threads(kKind, kChunked), 1)
     k_mma(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const MmaArgs p,
           unsigned tiles) {
-    constexpr int kStages = stages(kKind, kBN), kEpilogueWarps = epilogue_warps(kKind);
+    constexpr int kStages = stages(kKind, kBN, kChunked), kEpilogueWarps = epilogue_warps(kKind, kChunked);
     constexpr bool kKeeps = kKind == kForward && kMode != kPlain;   // a kept pre-activation, a residual
     constexpr int kGroups = kEpilogueWarps / 4;   // warps that share 32 accumulator rows
     constexpr int kStage = stage_bytes(kKind, kBN);
@@ -480,9 +490,11 @@ __global__ void __launch_bounds__(role_threads(kKind), 1)
             int s = 0, phase = 0, issued = 0;
             for (unsigned t = blockIdx.x; t < tiles && !*dead; t += gridDim.x) {
                 const Tile tile = tile_at<kBN>(p, t);
+                for (int from = tile.begin; from < tile.end; from += kChunked ? kChunk : tile.end - tile.begin) {
+                const int to = kChunked ? min(tile.end, from + kChunk) : tile.end;
                 for (int pair = 0; pair < p.pairs; ++pair) {
                     const int za = (p.pairs_a >> (2 * pair)) & 3, zb = (p.pairs_b >> (2 * pair)) & 3;
-                    for (int k = tile.begin; k < tile.end; ++k) {
+                    for (int k = from; k < to; ++k) {
                         if (!bar_wait(empty(s), phase ^ 1, dead)) goto copies_done;
                         const uint32_t a = ring + s * kStage, b = a + kStageA;
                         bar_expect(full(s), kStageA + b_columns(kKind, kBN) * kBK * 2);
@@ -501,6 +513,7 @@ __global__ void __launch_bounds__(role_threads(kKind), 1)
                         ++issued;
                         if (++s == kStages) s = 0, phase ^= 1;
                     }
+                }
                 }
             }
         copies_done:
@@ -521,27 +534,35 @@ __global__ void __launch_bounds__(role_threads(kKind), 1)
                                    ((uint32_t)(kBM >> 4) << 24);
             constexpr int kStepA = (a_mn(kKind) ? 2048 : 32) >> 4, kStepB = (b_mn(kKind) ? 2048 : 32) >> 4;
             int s = 0, phase = 0, n = 0;
-            for (unsigned t = blockIdx.x; t < tiles; t += gridDim.x, ++n) {
+            bool going = true;
+            for (unsigned t = blockIdx.x; t < tiles && going; t += gridDim.x) {
                 const Tile tile = tile_at<kBN>(p, t);
-                const int buf = n & 1;
-                if (!bar_wait(acc_empty(buf), ((n >> 1) & 1) ^ 1, dead)) break;
-                fence_after();
-                const uint32_t d = tmem + buf * kBN;
-                const int count = p.pairs * (tile.end - tile.begin);
-                int k = 0;
-                for (; k < count; ++k) {
-                    if (!bar_wait(full(s), phase, dead)) break;
+                for (int from = tile.begin; from < tile.end && going; ++n) {
+                    const int to = kChunked ? min(tile.end, from + kChunk) : tile.end, buf = n & 1;
+                    if (!bar_wait(acc_empty(buf), ((n >> 1) & 1) ^ 1, dead)) {
+                        going = false;
+                        break;
+                    }
                     fence_after();
-                    const uint64_t a = operand_desc(ring + s * kStage, a_mn(kKind));
-                    const uint64_t b = operand_desc(ring + s * kStage + kStageA, b_mn(kKind));
+                    const uint32_t d = tmem + buf * kBN;
+                    const int count = p.pairs * (to - from);
+                    from = to;
+                    for (int k = 0; k < count; ++k) {
+                        if (!bar_wait(full(s), phase, dead)) {
+                            going = false;
+                            break;
+                        }
+                        fence_after();
+                        const uint64_t a = operand_desc(ring + s * kStage, a_mn(kKind));
+                        const uint64_t b = operand_desc(ring + s * kStage + kStageA, b_mn(kKind));
 #pragma unroll
-                    for (int u = 0; u < kBK / 16; ++u)
-                        mma_f16(d, a + u * kStepA, b + u * kStepB, idesc, k > 0 || u > 0);
-                    mma_commit(empty(s));
-                    if (++s == kStages) s = 0, phase ^= 1;
+                        for (int u = 0; u < kBK / 16; ++u)
+                            mma_f16(d, a + u * kStepA, b + u * kStepB, idesc, k > 0 || u > 0);
+                        mma_commit(empty(s));
+                        if (++s == kStages) s = 0, phase ^= 1;
+                    }
+                    if (going) mma_commit(acc_full(buf));
                 }
-                if (k < count) break;
-                mma_commit(acc_full(buf));
             }
             if (*dead) {   // MMAs in flight end before the shared memory they read goes
                 mma_commit(drained);
@@ -555,6 +576,59 @@ __global__ void __launch_bounds__(role_threads(kKind), 1)
         const int quarter = warp & 3, group = (warp - 2) >> 2;
         float* s = staging + (warp - 2) * (kWarpStaging / 4);
         int n = 0;
+        if constexpr (kChunked) {
+            static_assert(kBN / 32 <= kGroups, "a piece a warp");
+            for (unsigned t = blockIdx.x; t < tiles; t += gridDim.x) {
+                const Tile tile = tile_at<kBN>(p, t);
+                const bool mine = group < kBN / 32;
+                const int64_t row0 = tile.i0 + quarter * 32, col0 = tile.j0 + group * 32;
+                const bool live = mine && col0 < p.nj && row0 < p.ni;
+                float sum[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) sum[i] = 0.f;
+                bool given_up = false;
+                for (int from = tile.begin; from < tile.end; from += kChunk, ++n) {
+                    const int buf = n & 1;
+                    if (!warp_wait(acc_full(buf), (n >> 1) & 1, dead)) {
+                        given_up = true;
+                        break;
+                    }
+                    fence_after();
+                    if (mine) {
+                        float v[16];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            tmem_load16(v, tmem + buf * kBN + ((uint32_t)(quarter * 32) << 16) + group * 32 + h * 16);
+#pragma unroll
+                            for (int i = 0; i < 16; i += 2) add2(sum[h * 16 + i], sum[h * 16 + i + 1], v[i], v[i + 1]);
+                        }
+                    }
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(acc_empty(buf));
+                }
+                if (given_up) break;
+                if (!live) continue;
+                if (kKind == kForward && p.bias) {
+                    __syncwarp();
+                    s[32 * 16 + lane] = col0 + lane < p.nj ? load_param(p.bias, p.bias_dtype, col0 + lane) : 0.f;
+                    __syncwarp();
+                }
+                if constexpr (kKeeps) {
+                    Ahead ahead;
+                    ahead.have = false;
+                    finish32<kOut, kMode>(sum, p, row0, col0, s, ahead, lane);
+                } else {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float v[16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) v[i] = sum[h * 16 + i];
+                        if (col0 + h * 16 < p.nj) finish16<kKind, kOut, kMode>(v, p, tile, row0, col0 + h * 16, s, h, lane);
+                    }
+                }
+            }
+        } else
         for (unsigned t = blockIdx.x; t < tiles; t += gridDim.x, ++n) {
             const Tile tile = tile_at<kBN>(p, t);
             constexpr int kPieces = kBN / 32;
@@ -620,14 +694,14 @@ __global__ void __launch_bounds__(role_threads(kKind), 1)
 
 // ------------------------------------------------------------------ launch
 
-template <int kKind, int kBN, int kOut, int kMode>
+template <int kKind, int kBN, int kOut, int kMode, bool kChunked>
 cudaError_t launch_mma(const Operand& a, const Operand& b, const MmaArgs& p, cudaStream_t s) {
     int unused = 0;
     cudaError_t e = pl::kernel_once(
-        reinterpret_cast<const void*>(k_mma<kKind, kBN, kOut, kMode>),
+        reinterpret_cast<const void*>(k_mma<kKind, kBN, kOut, kMode, kChunked>),
         [](int*) {
-            return cudaFuncSetAttribute(k_mma<kKind, kBN, kOut, kMode>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        smem_bytes(kKind, kBN));
+            return cudaFuncSetAttribute(k_mma<kKind, kBN, kOut, kMode, kChunked>,
+                                        cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(kKind, kBN, kChunked));
         },
         &unused);
     if (e != cudaSuccess) return e;
@@ -637,24 +711,34 @@ cudaError_t launch_mma(const Operand& a, const Operand& b, const MmaArgs& p, cud
     const int64_t tiles = mma_tiles(p.ni, p.nj, kBN) * p.parts;
     if (tiles > INT_MAX) return cudaErrorInvalidValue;
     const int ctas = (int)(tiles < sm_count() ? tiles : sm_count());
-    k_mma<kKind, kBN, kOut, kMode><<<ctas, role_threads(kKind), smem_bytes(kKind, kBN), s>>>(ma, mb, p, (unsigned)tiles);
+    k_mma<kKind, kBN, kOut, kMode, kChunked>
+        <<<ctas, role_threads(kKind, kChunked), smem_bytes(kKind, kBN, kChunked), s>>>(ma, mb, p, (unsigned)tiles);
     return cudaGetLastError();
 }
 
-template <int kKind, int kOut, int kMode>
+// kDeep: float32 results, whose deep sums go in chunks.
+template <int kKind, int kOut, int kMode, bool kDeep>
 cudaError_t launch_bn(int bn, const Operand& a, const Operand& b, const MmaArgs& p, cudaStream_t s) {
-    if (bn == 256) return launch_mma<kKind, 256, kOut, kMode>(a, b, p, s);
-    if (bn == 128) return launch_mma<kKind, 128, kOut, kMode>(a, b, p, s);
-    if (bn == 64) return launch_mma<kKind, 64, kOut, kMode>(a, b, p, s);
-    if constexpr (kKind == kForward) return launch_mma<kKind, 32, kOut, kMode>(a, b, p, s);
+    if constexpr (kDeep) {
+        if (chunked(p.part_steps, p.out_dtype, p.precise)) {
+            if (bn > 64) return launch_mma<kKind, 128, kOut, kMode, true>(a, b, p, s);
+            if constexpr (kKind == kForward)
+                if (bn == 32) return launch_mma<kKind, 32, kOut, kMode, true>(a, b, p, s);
+            return launch_mma<kKind, 64, kOut, kMode, true>(a, b, p, s);
+        }
+    }
+    if (bn == 256) return launch_mma<kKind, 256, kOut, kMode, false>(a, b, p, s);
+    if (bn == 128) return launch_mma<kKind, 128, kOut, kMode, false>(a, b, p, s);
+    if (bn == 64) return launch_mma<kKind, 64, kOut, kMode, false>(a, b, p, s);
+    if constexpr (kKind == kForward) return launch_mma<kKind, 32, kOut, kMode, false>(a, b, p, s);
     return cudaErrorInvalidValue;
 }
 
 template <int kKind, int kMode>
 cudaError_t launch_out(int bn, const Operand& a, const Operand& b, const MmaArgs& p, cudaStream_t s) {
-    if (p.out_dtype == PLATTICE_F32) return launch_bn<kKind, PLATTICE_F32, kMode>(bn, a, b, p, s);
-    if (p.out_dtype == PLATTICE_BF16) return launch_bn<kKind, PLATTICE_BF16, kMode>(bn, a, b, p, s);
-    return launch_bn<kKind, PLATTICE_F16, kMode>(bn, a, b, p, s);
+    if (p.out_dtype == PLATTICE_F32) return launch_bn<kKind, PLATTICE_F32, kMode, true>(bn, a, b, p, s);
+    if (p.out_dtype == PLATTICE_BF16) return launch_bn<kKind, PLATTICE_BF16, kMode, false>(bn, a, b, p, s);
+    return launch_bn<kKind, PLATTICE_F16, kMode, false>(bn, a, b, p, s);
 }
 
 }  // namespace plr

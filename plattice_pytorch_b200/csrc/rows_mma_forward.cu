@@ -4,7 +4,7 @@
 namespace plr {
 
 cudaError_t mma_forward(int bn, bool aligned, const Operand& x, const Operand& w, const MmaArgs& p, cudaStream_t s) {
-    if (!aligned || p.split) return launch_bn<kForward, PLATTICE_F32, kAny>(bn, x, w, p, s);
+    if (!aligned || p.split) return launch_bn<kForward, PLATTICE_F32, kAny, true>(bn, x, w, p, s);
     if (p.act == PLATTICE_ACT_NONE && !p.residual && !p.z) return launch_out<kForward, kPlain>(bn, x, w, p, s);
     return launch_out<kForward, kAligned>(bn, x, w, p, s);
 }

@@ -4,7 +4,7 @@
 namespace plr {
 
 cudaError_t mma_grad_x(int bn, bool aligned, const Operand& gz, const Operand& w, const MmaArgs& p, cudaStream_t s) {
-    if (!aligned) return launch_bn<kGradX, PLATTICE_F32, kAny>(bn, gz, w, p, s);
+    if (!aligned) return launch_bn<kGradX, PLATTICE_F32, kAny, true>(bn, gz, w, p, s);
     return launch_out<kGradX, kPlain>(bn, gz, w, p, s);
 }
 

@@ -397,6 +397,15 @@ __global__ void __launch_bounds__(32 * kNarrowWarps, narrow_ctas(kXT, kNF)) k_na
                 continue;
             } else {
             narrow_mask<kXT>(raw, a.k, c, lane);
+            // the sum of these 64 channels by itself: the matrix instruction cuts
+            // where an addition rounds, by which a long chain of them drifts
+            float sum[kM][kNF][4];
+#pragma unroll
+            for (int m = 0; m < kM; ++m)
+#pragma unroll
+                for (int f = 0; f < kNF; ++f)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sum[m][f][i] = 0.f;
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
                 uint2 b[kPB][kNF];
@@ -409,17 +418,24 @@ __global__ void __launch_bounds__(32 * kNarrowWarps, narrow_ctas(kXT, kNF)) k_na
                     uint32_t o[kPA][4];
                     narrow_operand<kXT, kPA>(raw, m, s, o);
 #pragma unroll
-                    for (int sum = 2; sum >= 0; --sum)   // small products first
+                    for (int size = 2; size >= 0; --size)   // small products first
 #pragma unroll
                         for (int pa = 0; pa < kPA; ++pa) {
-                            const int pb = sum - pa;
+                            const int pb = size - pa;
                             if (pb < 0 || pb >= kPB) continue;
 #pragma unroll
                             for (int f = 0; f < kNF; ++f)
-                                mma16816<kXT == kXHalf>(acc[m][f], o[pa][0], o[pa][1], o[pa][2], o[pa][3], b[pb][f]);
+                                mma16816<kXT == kXHalf>(sum[m][f], o[pa][0], o[pa][1], o[pa][2], o[pa][3], b[pb][f]);
                         }
                 }
             }
+#pragma unroll
+            for (int m = 0; m < kM; ++m)
+#pragma unroll
+                for (int f = 0; f < kNF; ++f) {
+                    add2(acc[m][f][0], acc[m][f][1], sum[m][f][0], sum[m][f][1]);
+                    add2(acc[m][f][2], acc[m][f][3], sum[m][f][2], sum[m][f][3]);
+                }
             }
         }
         const int rows = (int)min((int64_t)(16 * kM), a.rows - row0);
@@ -731,7 +747,12 @@ __global__ void __launch_bounds__(32 * kGradWarps, narrow_grad_ctas(kParts, kNF)
         }
         if (a.need_b) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) db += st[r * kNarrowPitch + lane];
+            for (int r = 0; r < 16; r += 8) {   // short chains: many rows drift less
+                float t[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) t[i] = st[(r + i) * kNarrowPitch + lane];
+                db += ((t[0] + t[1]) + (t[2] + t[3])) + ((t[4] + t[5]) + (t[6] + t[7]));
+            }
         }
         if (a.need_x) {
             uint32_t o[kKS][kPZ][4];
@@ -808,6 +829,14 @@ __global__ void __launch_bounds__(32 * kGradWarps, narrow_grad_ctas(kParts, kNF)
                                  : "r"((uint32_t)__cvta_generic_to_shared(src))
                                  : "memory");
                 }
+                // float32: the sum of these rows by itself (see k_narrow)
+                float rows16[kNF][4];
+                if (kParts == 3) {
+#pragma unroll
+                    for (int f = 0; f < kNF; ++f)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) rows16[f][i] = 0.f;
+                }
 #pragma unroll
                 for (int sum = kPZ - 1; sum >= 0; --sum)
 #pragma unroll
@@ -816,9 +845,16 @@ __global__ void __launch_bounds__(32 * kGradWarps, narrow_grad_ctas(kParts, kNF)
                         if (pb < 0 || pb >= kPZ) continue;
 #pragma unroll
                         for (int f = 0; f < kNF; ++f)
-                            mma16816<kHalf>(dw[m][f], x[px][0], x[px][1], x[px][2], x[px][3],
+                            mma16816<kHalf>(kParts == 3 ? rows16[f] : dw[m][f], x[px][0], x[px][1], x[px][2], x[px][3],
                                             make_uint2(b[pb][f][0], b[pb][f][1]));
                     }
+                if (kParts == 3) {
+#pragma unroll
+                    for (int f = 0; f < kNF; ++f) {
+                        add2(dw[m][f][0], dw[m][f][1], rows16[f][0], rows16[f][1]);
+                        add2(dw[m][f][2], dw[m][f][3], rows16[f][2], rows16[f][3]);
+                    }
+                }
             }
         }
     }
