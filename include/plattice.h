@@ -288,7 +288,8 @@ const char* plattice_profile_stage_name(int stage);
  * device.  No call synchronises.
  *
  * Element types.  Parameters (gain, bias) and their gradients may be of any of
- * the three types; all other tensors of a call share one. */
+ * the three types; the other tensors of a call are of `dtype`, but for a linear
+ * map's `out_dtype`. */
 #define PLATTICE_F32 0
 #define PLATTICE_BF16 1
 #define PLATTICE_F16 2
@@ -356,7 +357,8 @@ typedef struct plattice_linear_args {
     void* grad_x;
     void* grad_w;
     void* grad_bias;
-    void* workspace;            /* 256-byte aligned */
+    void* workspace;            /* 256-byte aligned; its size depends on the other pointers' alignment:
+                                   ask for it with the arguments of the call */
     size_t workspace_bytes;
     long long rows;
     int k, n, split;

@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(256, 4) k_grad_z(const GradArgs a) {
 // 16 exponents (largest values of 0.1 to 3584; other blocks are computed).  The
 // lookups conflict over the banks about three ways, and still take a third of
 // the exponentials and reciprocals they replace: 32768 x 4096, gelu, bfloat16:
-// 165 -> 1xx us, of which moving 675 MB is 103.
+// 165 -> 120 us, of which moving 675 MB is 103.
 constexpr int kTableLow = 127 - 12, kTableScales = 16;
 
 template <typename TG, typename T, int kAct>

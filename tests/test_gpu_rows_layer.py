@@ -181,3 +181,53 @@ def test_checkpoint_precision_setting(P):
     with pytest.raises(RuntimeError, match="checkpoint precision"):
         P.PLOO.set_checkpoint_precision("int8")
     assert P.PLOO.get_checkpoint_precision() == "fp32"
+
+
+def test_layer_step_captured_and_replayed(dev, P):
+    """Forward and gradients of the layer in a CUDA graph, replayed on new inputs."""
+    torch.manual_seed(2)
+    m = P.PermutoLatticeLayer(64, 5, 3, act="gelu", dtype=torch.bfloat16, device=dev)
+    x = _randn((24, 20, 64), 20, torch.bfloat16).to(dev).requires_grad_(True)
+    gy = _randn((24, 20, 64), 21, torch.bfloat16).to(dev)
+    leaves = [x, *m.parameters()]
+
+    def step():
+        y = m(x)
+        return [y, *torch.autograd.grad(y, leaves, gy)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for seed in (22, 23):
+        with torch.no_grad():
+            x.copy_(_randn((24, 20, 64), seed, torch.bfloat16).to(dev))
+        graph.replay()
+        got_now = [g.detach().float().clone() for g in got]
+        for g, e in zip(got_now, step()):
+            # the splat's atomics add in another order, and bfloat16 then rounds the other way now and then:
+            # at most a step (2^-7) of a value near the largest
+            e = e.detach().float()
+            assert float((g - e).abs().max()) <= 2.0 ** -7 * float(e.abs().max())
+
+
+def test_layer_on_another_stream_and_twice_at_once(dev, P):
+    torch.manual_seed(3)
+    m = P.PermutoLatticeLayer(40, 3, 4, act="silu", device=dev)
+    xs = [_randn((17, 23, 40), 30 + i).to(dev) for i in range(2)]
+    with torch.no_grad():
+        want = [m(x) for x in xs]
+        streams = [torch.cuda.Stream() for _ in xs]
+        torch.cuda.synchronize()
+        got = []
+        for s, x in zip(streams, xs):
+            with torch.cuda.stream(s):
+                got.append(m(x))
+        torch.cuda.synchronize()
+    for g, e in zip(got, want):
+        # lattice sums differ by their order: 1e-5 relative + 5e-6 each, through a product of 4 weights below 1
+        assert float((g - e).abs().max()) <= 1e-4
