@@ -74,6 +74,19 @@ struct Rows8 {
     at::Tensor q, scale;
 };
 
+// Whether q and scale are the 8-bit rows of a tensor of `rows` x c (a Rows8's
+// fields can be changed after it was checked).
+bool holds(const at::Tensor& q, const at::Tensor& scale, int64_t rows, int64_t c) {
+    return c >= 1 && c <= (1 << 30) && q.size(0) == rows && q.size(1) == width8(c) && scale.size(0) == rows &&
+           scale.size(1) == width8(c) / 32 && q.device() == scale.device() && (uintptr_t)q.data_ptr() % 16 == 0;
+}
+
+int64_t rows_of(const std::vector<int64_t>& shape) {
+    int64_t n = 1;
+    for (size_t i = 0; i + 1 < shape.size(); ++i) n *= shape[i];
+    return n;
+}
+
 Rows8 empty8(int64_t rows, int64_t c, const at::TensorOptions& like) {
     const auto o = like.dtype(at::kByte);
     return {at::empty({rows, width8(c)}, o), at::empty({rows, width8(c) / 32}, o)};
@@ -95,10 +108,10 @@ py::object rows_pack8(const py::object& x_) {
     return pair(r);
 }
 
-// q, scale and shape are a Rows8's, checked when it was made
 py::object rows_unpack8(const py::object& q_, const py::object& scale_, const std::vector<int64_t>& shape, int dtype) {
     const at::Tensor *q = bytes(q_), *scale = bytes(scale_);
-    if (!q || !scale || shape.empty() || dtype < 0 || dtype > 2) return py::none();
+    if (!q || !scale || shape.empty() || dtype < 0 || dtype > 2 || !holds(*q, *scale, rows_of(shape), shape.back()))
+        return py::none();
     const c10::cuda::CUDAGuard guard(q->device());
     const at::Tensor y = at::empty(
         shape, q->options().dtype(dtype == PLATTICE_F32 ? at::kFloat : dtype == PLATTICE_BF16 ? at::kBFloat16 : at::kHalf));
@@ -176,6 +189,7 @@ Input input_of(const py::object& x_, const py::object& scale_, const py::object&
         in.scale = bytes(scale_);
         if (!in.x || !in.scale || w.scalar_type() == at::kHalf) return in;
         in.lead = shape_.cast<std::vector<int64_t>>();
+        if (in.lead.empty() || !holds(*in.x, *in.scale, rows_of(in.lead), in.lead.back())) return in;
     }
     in.k = in.lead.back();
     in.lead.pop_back();
@@ -289,7 +303,9 @@ py::object rows_linear_backward(const py::object& g0_, const py::object& g1_, co
             a.z = z->data_ptr();
         } else {
             const at::Tensor *z = bytes(z_), *zs = bytes(z_scale_);
-            if (!z || !zs || z_shape_.cast<std::vector<int64_t>>() != shape || z->device() != w->device()) return py::none();
+            if (!z || !zs || z_shape_.cast<std::vector<int64_t>>() != shape || z->device() != w->device() ||
+                !holds(*z, *zs, in.rows, n))
+                return py::none();
             a.z = z->data_ptr();
             a.z_scale = zs->data_ptr<uint8_t>();
         }

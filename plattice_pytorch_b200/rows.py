@@ -165,6 +165,7 @@ def unpack8(r, dtype=torch.float32):
         if type(got) is int:
             _raise("plattice_rows_unpack8", got, f"shape={r.shape}")
         return got
+    r = Rows8(r.q, r.scale, r.shape)   # its fields may have been changed since it was made
     y = torch.empty(r.shape, dtype=dtype, device=r.device)
     rc = _call(r.device.index, _lib_h().plattice_rows_unpack8, y.data_ptr(), _DTYPES[dtype], r.q.data_ptr(),
                r.scale.data_ptr(), r.q.shape[0], r.shape[-1], _raw_stream(r.device.index))
@@ -254,6 +255,7 @@ def _linear_common(x, weight, act, out_dtype, lead=None):
     n, k = (int(s) for s in weight.shape)
     if isinstance(x, Rows8):
         _require(weight.dtype != torch.float16, "weight must be float32 or bfloat16 for 8-bit rows")
+        x = Rows8(x.q, x.scale, x.shape)
         _require(x.shape[-1] == k, f"x must have {k} channels")
     elif x is not None:
         _check_rows(x, "x", k)
@@ -382,6 +384,7 @@ def linear_backward(grad_y, x, weight, z=None, act="none", bias_dtype=None, need
     if act != "none":
         _require(z is not None, "z is needed for the backward of an activation")
         if isinstance(z, Rows8):
+            z = Rows8(z.q, z.scale, z.shape)
             _require(z.shape == lead + (n,), f"z must be {lead + (n,)}")
             _require(z.device == dev, "z must be on the rows' device")
             a.z, a.z_scale = z.q.data_ptr(), z.scale.data_ptr()

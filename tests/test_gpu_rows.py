@@ -544,3 +544,52 @@ def test_offsets_beyond_32_bits(dev, R):
     out, _ = R.linear(x, w)
     oe = f64(tail) @ f64(w).T
     assert worst(f64(out[-40:]), oe, _forward_tolerance(f64(tail), f64(w), None, oe * 0, oe, c, torch.bfloat16)) <= 1
+
+
+@pytest.mark.parametrize("rows,k,n", [(300, 5000, 24), (140, 9000, 8), (3, 5000, 24), (1, 264, 520), (2, 100, 40), (9, 72, 40),
+                                      (600, 640, 700)])
+@pytest.mark.parametrize("dtype,x8", KINDS)
+def test_linear_deep_sums_and_few_rows(dev, R, rows, k, n, dtype, x8):
+    """Few output channels over more input channels than shared memory holds
+    weights of, few rows, sums deeper than a chunk on both sides."""
+    t = DTYPES[dtype]
+    x, xe, w = _linear_input(rows, k, n, t, x8, R, dev)
+    b = 0.3 * _randn((n,), 22)
+    for out, act, keep in ((torch.float32, "none", None), (t, "relu", "8bit"), (torch.float32, "silu", "full")):
+        y, z = R.linear(x, w.to(dev), b.to(dev), act=act, out_dtype=out, keep=keep)
+        ye, ze = ref.linear(xe, f64(w), f64(b), act)
+        assert worst(f64(y), ye, _forward_tolerance(xe, f64(w), f64(b), ze, ye, k, out)) <= 1
+        gy = _randn((rows, n), 26, out)
+        got = R.linear_backward(gy.to(dev), x, w.to(dev), z, act=act, bias_dtype=torch.float32)
+        zk = None if z is None else f64(R.unpack8(z)) if keep == "8bit" else f64(z)
+        _check_gradients(got, f64(gy), xe, f64(w), zk, act, t, out)
+
+
+@pytest.mark.parametrize("k,n", [(1024, 40), (4096, 72), (2048, 24)])
+def test_float32_sums_stay_float32(dev, R, k, n):
+    """A deep sum of float32 products is as near as float32 additions in
+    blocks are: u sqrt(m) of the sum of squares' root for random signs, m the
+    longest chain of additions (here at most k / 16), where a chain that cuts
+    instead of rounding would be off by u m."""
+    rows = 512
+    x, w = _randn((rows, k), 90), _randn((n, k), 91, scale=k ** -0.5)
+    y, _ = R.linear(x.to(dev), w.to(dev))
+    ye = f64(x) @ f64(w).T
+    rel = np.linalg.norm(f64(y) - ye) / np.linalg.norm(ye)
+    assert rel <= 2 * U * np.sqrt(k / 16) + 4 * U
+    gy = _randn((8192, n), 92)
+    xl = _randn((8192, 64), 93)
+    got = R.linear_backward(gy.to(dev), xl.to(dev), _randn((n, 64), 94).to(dev))
+    we = f64(gy).T @ f64(xl)
+    assert np.linalg.norm(f64(got[1]) - we) / np.linalg.norm(we) <= 2 * U * np.sqrt(8192 / 16) + 4 * U
+
+
+def test_changed_fields_of_rows8_are_refused(dev, R):
+    w = torch.zeros(5, 64, device=dev)
+    for shape in ((7, 64), (3, 64), (4, 32), (4, 65)):
+        r = R.pack8(torch.zeros(4, 64, device=dev))
+        r.shape = shape
+        for call in (lambda: R.unpack8(r), lambda: R.linear(r, w),
+                     lambda: R.linear_backward(torch.zeros(4, 5, device=dev), r, w)):
+            with pytest.raises(RuntimeError):
+                call()
