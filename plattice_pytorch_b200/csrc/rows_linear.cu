@@ -498,7 +498,7 @@ struct BackwardPlan {
 // 34559 rows 119 / 93, from 8 bits 115 / 125; from 8 bits n 32: k 128, 262144
 // rows 76 / 76, k 256 135 / 125; float32 n 8, k 2048, 8192 rows 72 / 115.
 static bool backward_is_narrow(const plattice_linear_args* a) {
-    if (a->n > 32) return false;
+    if (a->n > 32 || a->k > kNarrowGradMost) return false;
     if (a->dtype == PLATTICE_F32 || a->k <= 128) return true;
     return a->n <= 24 && (a->x_scale || a->k <= 768);
 }

@@ -38,6 +38,7 @@ __host__ __device__ inline int narrow_steps(int k) { return (k + 63) / 64 * 4; }
 __host__ inline int64_t narrow_fragments(int k, int nf, int parts) { return (int64_t)parts * narrow_steps(k) * nf * 256; }
 constexpr int64_t kNarrowMost = 64 * 1024;   // bytes of weights: two CTAs then share an SM
 constexpr int kGradWarps = 4;
+constexpr int kNarrowGradMost = 65535 * 64;      // input channels of the narrow backward: slices are gridDim.y
 // CTAs of the narrow backward that share an SM
 __host__ __device__ constexpr int narrow_grad_ctas(int parts, int nf) { return parts == 3 ? 2 : nf > 2 ? 3 : 4; }
 

@@ -15,9 +15,7 @@ static cudaError_t launch_narrow_grad(const SmallGradArgs& a, int lines, cudaStr
         },
         &unused);
     if (e != cudaSuccess) return e;
-    const int64_t slices = ceil_div(a.s.k, 64);
-    if (slices > 65535) return cudaErrorInvalidValue;
-    k_narrow_grad<kXT, kParts, kNF, kG32><<<dim3(lines, (unsigned)slices), 32 * kGradWarps,
+    k_narrow_grad<kXT, kParts, kNF, kG32><<<dim3(lines, (unsigned)ceil_div(a.s.k, 64)), 32 * kGradWarps,
                                             NarrowGradShape<kXT, kParts>::kBytes, s>>>(a);
     return cudaGetLastError();
 }

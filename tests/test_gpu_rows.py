@@ -584,6 +584,49 @@ def test_float32_sums_stay_float32(dev, R, k, n):
     assert np.linalg.norm(f64(got[1]) - we) / np.linalg.norm(we) <= 2 * U * np.sqrt(8192 / 16) + 4 * U
 
 
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+@pytest.mark.parametrize("dtype,out32", [("fp32", True), ("bf16", False), ("bf16", True)])
+def test_linear_backward_many_kept_values(dev, R, dtype, out32, act):
+    """Millions of kept 8-bit values, their blocks' scales from 2^-24 to 2^8:
+    the slopes of some come from a table, of the others from the function."""
+    t = DTYPES[dtype]
+    out = torch.float32 if out32 else t
+    rows, k, n = 20000, 40, 256
+    x, xe, w = _linear_input(rows, k, n, t, True, R, dev)
+    z = _randn((rows, n), 98) * 2.0 ** torch.randint(-22, 10, (rows, n // 32), generator=torch.Generator().manual_seed(99)
+                                                     ).repeat_interleave(32, 1)
+    z8 = R.pack8(z.clamp(-100, 100).to(dev))
+    gy = _randn((rows, n), 100, out)
+    got = R.linear_backward(gy.to(dev), x, w.to(dev), z8, act=act, bias_dtype=torch.float32)
+    _check_gradients(got, f64(gy), xe, f64(w), f64(R.unpack8(z8)), act, t, out)
+
+
+@pytest.mark.parametrize("dtype,x8", [("fp32", False), ("bf16", True)])
+def test_linear_backward_of_millions_of_channels(dev, R, dtype, x8):
+    """More input channels than a grid has room for slices of 64 of."""
+    t, rows, k, n = DTYPES[dtype], 3, 65535 * 64 + 40, 2
+    x, xe, w = _linear_input(rows, k, n, t, x8, R, dev)
+    gy = _randn((rows, n), 97, t)
+    got = R.linear_backward(gy.to(dev), x, w.to(dev), bias_dtype=torch.float32)
+    _check_gradients(got, f64(gy), xe, f64(w), None, "none", t, t)
+
+
+@pytest.mark.parametrize("c", [256, 250, 33, 1030])
+def test_norm_sum_in_place(dev, R, c):
+    """The C call with h stored over x, or over the residual."""
+    from plattice_pytorch_b200 import _lib
+    rows = 3001
+    x, r, gain = (_randn(s, i).to(dev) for i, s in ((101, (rows, c)), (102, (rows, c)), (103, (c,))))
+    y, h, rstd = R.rms_norm(x, gain, r)
+    for over in range(2):
+        a, b, y2, rstd2 = x.clone(), r.clone(), torch.empty_like(y), torch.empty_like(rstd)
+        rc = _lib.lib().plattice_rms_norm(y2.data_ptr(), None, (a, b)[over].data_ptr(), rstd2.data_ptr(), a.data_ptr(),
+                                          b.data_ptr(), gain.data_ptr(), 0, 0, 1e-6, rows, c,
+                                          torch.cuda.current_stream().cuda_stream)
+        assert rc == 0
+        assert torch.equal((a, b)[over], h) and torch.equal(y2, y) and torch.equal(rstd2, rstd)
+
+
 def test_changed_fields_of_rows8_are_refused(dev, R):
     w = torch.zeros(5, 64, device=dev)
     for shape in ((7, 64), (3, 64), (4, 32), (4, 65)):
