@@ -336,12 +336,14 @@ int plattice_rms_norm_backward(void* grad_x, void* grad_gain, const void* grad_y
  * to y0 [rows][split] and the others to y1 [rows][n - split] (0 < split < n; no
  * residual, no activation): the features and values of a filter call.
  * z non-NULL (forward): the pre-activation is kept there, as 8-bit rows when
- * z_scale is non-NULL (z then on a 32-byte boundary), else in out_dtype.
+ * z_scale is non-NULL (z then on a 32-byte boundary; 16 do for the backward),
+ * else in out_dtype.
  *
  * Backward, with gz = grad_y act'(z) (z as kept, or NULL without activation):
  *   grad_x = gz w, grad_w = gz^T x (both in dtype), grad_bias = sum_r gz
  * (bias_dtype); each output may be NULL.  gz is rounded to dtype before the
- * two products (n > 32; with fewer output channels it is not).  Sums are held in float32 and added in a fixed order. */
+ * two products (n > 32; with fewer output channels it is not).  Sums are held in
+ * float32 and added in a fixed order. */
 typedef struct plattice_linear_args {
     const void* x;
     const uint8_t* x_scale;

@@ -311,6 +311,10 @@ static bool linear_shape_ok(const plattice_linear_args* a) {
     return fits(a->rows, width8(a->k)) && fits(a->rows, width8(a->n)) && fits(a->k, a->n);
 }
 
+static bool workspace_ok(const plattice_linear_args* a, int64_t bytes) {
+    return a->workspace && ((uintptr_t)a->workspace & 255) == 0 && a->workspace_bytes >= (size_t)bytes;
+}
+
 // Parts summed: few results over the warps of a CTA (a thread each would add
 // hundreds of parts one after the other: 7.8 against 3.5 us for 64 x 64 and
 // 296 parts), many by a thread each.
@@ -711,7 +715,7 @@ int plattice_linear(const plattice_linear_args* a, void* stream) {
     if (a->z_scale && ((uintptr_t)a->z & 31)) return PLATTICE_ERR_INVALID;   // codes leave 32 bytes at a time
     if (a->x_scale && !aligned16(a->x)) return PLATTICE_ERR_INVALID;
     const ForwardPlan p = forward_plan(a);
-    if (p.bytes && (!a->workspace || a->workspace_bytes < (size_t)p.bytes)) return PLATTICE_ERR_WORKSPACE;
+    if (p.bytes && !workspace_ok(a, p.bytes)) return PLATTICE_ERR_WORKSPACE;
     const int rc = rows_poll("plattice_linear");
     if (rc != PLATTICE_OK) return rc;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -739,8 +743,9 @@ int plattice_linear_backward(const plattice_linear_args* a, void* stream) {
         (a->act != PLATTICE_ACT_NONE && !a->z))
         return PLATTICE_ERR_INVALID;
     if (a->x_scale && !aligned16(a->x)) return PLATTICE_ERR_INVALID;
+    if (a->act != PLATTICE_ACT_NONE && a->z_scale && !aligned16(a->z)) return PLATTICE_ERR_INVALID;
     const BackwardPlan p = backward_plan(a);
-    if (!a->workspace || a->workspace_bytes < (size_t)p.bytes) return PLATTICE_ERR_WORKSPACE;
+    if (!workspace_ok(a, p.bytes)) return PLATTICE_ERR_WORKSPACE;
     const int rc = rows_poll("plattice_linear_backward");
     if (rc != PLATTICE_OK) return rc;
     if (p.narrow) return rows_status(backward_narrow(a, p, s), "plattice_linear_backward");

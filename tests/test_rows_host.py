@@ -83,6 +83,15 @@ def test_linear_arguments(lib):
     assert lib.plattice_linear(ctypes.byref(_args(rows=0)), None) == _lib.OK
 
 
+def test_linear_alignments(lib):
+    """Codes and workspaces on the boundaries that the kernels' wide accesses need."""
+    from plattice_pytorch_b200 import _lib
+    for n in (24, 72):
+        assert lib.plattice_linear_backward(ctypes.byref(_args(n=n, act=2, z=264, z_scale=256)), None) == _lib.ERR_INVALID
+        assert lib.plattice_linear_backward(ctypes.byref(_args(n=n, workspace=272)), None) == _lib.ERR_WORKSPACE
+    assert lib.plattice_linear(ctypes.byref(_args(n=72, workspace=264)), None) == _lib.ERR_WORKSPACE
+
+
 @pytest.fixture
 def rows(monkeypatch):
     """The module with CPU tensors let through its first check and the library out of reach."""
