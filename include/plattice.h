@@ -341,8 +341,8 @@ int plattice_rms_norm_backward(void* grad_x, void* grad_gain, const void* grad_y
  *
  * Backward, with gz = grad_y act'(z) (z as kept, or NULL without activation):
  *   grad_x = gz w, grad_w = gz^T x (both in dtype), grad_bias = sum_r gz
- * (bias_dtype); each output may be NULL.  gz is rounded to dtype before the
- * two products (n > 32; with fewer output channels it is not).  Sums are held in
+ * (bias_dtype); each output may be NULL.  gz may be rounded to dtype before the
+ * two products (with few output channels it keeps more).  Sums are held in
  * float32 and added in a fixed order. */
 typedef struct plattice_linear_args {
     const void* x;

@@ -140,6 +140,14 @@ class PermutoLatticeBatchFunction(Function):
         return None, grad_values
 
 
+def _long_rows(shape):
+    """The shape as which an image [H, W, vd] is kept in 8 bits: one long row,
+    with blocks of 32 values across pixels (a pixel's own 1 to 8 values would
+    fill a block of their own), or one per line of an image that no row holds."""
+    n = math.prod(shape)
+    return (n,) if n <= rows._MAX_CHANNELS else (shape[0], n // shape[0])
+
+
 class PermutoLatticeFeatureFunction(Function):
     """``PermutoLatticeFeatureFunction.apply(features, values) -> out`` with
     gradients for both inputs.  The feature gradient needs ``values`` and
@@ -152,9 +160,7 @@ class PermutoLatticeFeatureFunction(Function):
         ctx.shape = out.shape
         ctx.eight = PLOO._CHECKPOINT8 and out.numel() > 0
         if ctx.eight:
-            # one long row: blocks of 32 values across pixels, since a pixel's
-            # own 1 to 8 values would fill a block of their own
-            kept = [rows.pack8(t.view(-1)) for t in (values, out)] if ctx.needs_input_grad[0] else []
+            kept = [rows.pack8(t.view(_long_rows(t.shape))) for t in (values, out)] if ctx.needs_input_grad[0] else []
             ctx.save_for_backward(weight, feature, *(t for r in kept for t in (r.q, r.scale)))
         else:
             ctx.save_for_backward(weight, feature, values, out)
@@ -168,8 +174,8 @@ class PermutoLatticeFeatureFunction(Function):
         grad_features = None
         if ctx.needs_input_grad[0]:
             if ctx.eight:
-                flat = (math.prod(ctx.shape),)
-                values, out = (rows.unpack8(rows.Rows8(kept[i], kept[i + 1], flat)).view(ctx.shape) for i in (0, 2))
+                values, out = (rows.unpack8(rows.Rows8(kept[i], kept[i + 1], _long_rows(ctx.shape))).view(ctx.shape)
+                               for i in (0, 2))
             else:
                 values, out = kept
             grad_features = PLOO.feature_grad(ctx.lattice, feature, values, g, weight, out)

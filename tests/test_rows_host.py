@@ -169,6 +169,16 @@ def test_python_refusals(rows):
         R.pack8(x)
 
 
+def test_rows_of_kept_images(rows):
+    from plattice_pytorch_b200 import plattice
+    for shape, want in (((5, 7, 3), (105,)), ((1 << 14, 1 << 13, 8), (1 << 30,)),
+                        ((1 << 14, (1 << 13) + 1, 8), (1 << 14, (1 << 16) + 8))):
+        t = torch.empty(shape, device="meta")
+        kept = t.view(plattice._long_rows(shape))
+        assert tuple(kept.shape) == want
+        rows._check_rows(kept, "x")   # what pack8 takes
+
+
 def test_reference_codes_match_torch():
     """The tests' own e4m3 encoder against torch's conversion, every tie included."""
     v = ref.E4M3[:127]
