@@ -453,17 +453,31 @@ static cudaError_t unpacked(Operand* o, const plattice_linear_args* a, void* ws,
     return unpack_rows(ws, PLATTICE_BF16, o->pitch, static_cast<const uint8_t*>(a->x), a->x_scale, a->rows, a->k, s);
 }
 
-// How a forward runs: few rows a warp per output channel, few output channels
-// a warp per rows with the weights in shared memory, else the tiled product.
-// Measured at their borders: see k_few and k_narrow.
+// How a forward runs.  k_few where its CTAs of 16 rows x 32 channels fit on the
+// device at a time (with float32 weights, whose parts the tiles need written
+// first, up to three times that); k_narrow with at most 32 output channels;
+// else tiles.  16-bit rows that TMA can read go to the tiles too once n k is
+// above 1536.  Measured (us; bfloat16 unless noted):
+//   k_few / tiles   1024 -> 4096, 16 rows 4.6 / 9.4, 32 rows (1.7 rounds) 8.5 / 9.0;
+//     256 -> 256, 256 rows 3.3 / 4.6, 512 rows 5.6 / 4.6; float32, 512 -> 512, 128
+//     rows 6.2 / 20.3, 512 rows (3.5 rounds) 21.1 / 20.7
+//   k_few / k_narrow   64 -> 24, 2300 rows 3.1 / 3.2, 4700 rows 5.3 / 3.3; float32,
+//     256 -> 24, 2300 rows 4.3 / 6.2, 9400 rows 14.1 / 9.6
+//   k_narrow / tiles   262144 rows, n 8: k 64 9.6 / 13.8, k 256 26.6 / 27.3, k 1024
+//     103 / 88; n 24: k 64 15.4 / 15.6, k 128 21.5 / 17.2; k 100 (no 16-byte rows)
+//     34.6 / 52.4; 65536 rows, n 24, from 8 bits: k 64 7.0 / 10.4, k 1024 38 / 65;
+//     float32: k 64 9.6 / 19.6, k 1024 107 / 225
 enum Way { kWayFew, kWayNarrow, kWayTiles };
 
-constexpr int kFewRows = 8;
-
 static Way forward_way(const plattice_linear_args* a) {
+    const int64_t few = ceil_div(a->rows, 16) * ceil_div(a->n, 32);
+    if (few <= sm_count()) return kWayFew;
     const int parts = a->dtype == PLATTICE_F32 ? 3 : 1;
-    if (a->n <= 32 && narrow_fragments(a->k, (int)ceil_div(a->n, 8), parts) <= kNarrowMost) return kWayNarrow;
-    return a->rows <= kFewRows ? kWayFew : kWayTiles;
+    const bool tiles_read = !a->x_scale && tma_ready(a->x, a->dtype, a->k);
+    if (a->n <= 32 && (!tiles_read || (int64_t)a->n * a->k <= 1536) &&
+        narrow_fragments(a->k, (int)ceil_div(a->n, 8), parts) <= kNarrowMost)
+        return kWayNarrow;
+    return parts == 3 && few <= 3 * (int64_t)sm_count() ? kWayFew : kWayTiles;
 }
 
 struct ForwardPlan {
@@ -522,7 +536,7 @@ static BackwardPlan backward_plan(const plattice_linear_args* a) {
     }
     while (p.shift < 5 && (8 << p.shift) < a->n) ++p.shift;   // a row's columns / 8, at most a warp
     p.strips = (int)ceil_div(a->n, 8 << p.shift);
-    const int64_t need = ceil_div(a->rows, 256 >> p.shift), most = ceil_div(8 * (int64_t)sm_count(), p.strips);
+    const int64_t need = ceil_div(a->rows, 256 >> p.shift), most = ceil_div(4 * (int64_t)sm_count(), p.strips);   // one round
     p.parts_b = (int)(need < most ? need : most);
     if (p.parts_b < 1) p.parts_b = 1;
     p.partial_b = c.take((int64_t)p.parts_b * a->n * 4);
@@ -547,8 +561,10 @@ static BackwardPlan backward_plan(const plattice_linear_args* a) {
 template <typename TG, typename T>
 static cudaError_t launch_grad_z(const GradArgs& g, const BackwardPlan& p, cudaStream_t s) {
     const bool fast = g.vec && !g.split && g.pitch % 8 == 0;
-    // from 4 M values on (below, filling the tables takes what they save)
-    const bool table = fast && g.z_scale && g.rows * g.n >= (1 << 22);
+    // below 8 M values filling the tables takes what they save (us, 256 columns,
+    // bfloat16, gelu, table / computed: 4096 rows 6.2 / 3.9, 16384 8.1 / 7.5, 32768
+    // 12.1 / 13.6, 131072 32.3 / 44.6)
+    const bool table = fast && g.z_scale && g.rows * g.n >= (1 << 23);
     if (table && g.act == PLATTICE_ACT_GELU)
         k_grad_z_table<TG, T, PLATTICE_ACT_GELU><<<dim3(p.strips, p.parts_b), 256, 0, s>>>(g);
     else if (table && g.act == PLATTICE_ACT_SILU)

@@ -27,9 +27,10 @@ static cudaError_t launch_narrow(const SmallArgs& a, int64_t blocks, cudaStream_
 template <int kXT, bool kW3, int kNF>
 static cudaError_t run_narrow_as(const SmallArgs& a, cudaStream_t s) {
     const int64_t blocks = ceil_div(a.rows, 16 * NarrowShape<kXT>::kM);
-    // fewer blocks of rows than a warp on each SM would take: the warps of a
-    // CTA share a block instead (at least two chunks of channels to share)
-    if (blocks <= 2 * (int64_t)sm_count() && a.k > 64) return launch_narrow<kXT, kNF, kW3, true, false>(a, blocks, s);
+    // few blocks of rows and many channels: the warps of a CTA share a block
+    // (us, n 24, shared / apart: float32, 4700 rows, k 128 6.8 / 6.2, k 768 15.4 /
+    // 21.6; from 8 bits, 9400 rows, k 256 8.7 / 8.0, k 1024 18.7 / 22.4)
+    if (blocks * 256 <= (int64_t)sm_count() * a.k) return launch_narrow<kXT, kNF, kW3, true, false>(a, blocks, s);
     if (a.out_dtype == PLATTICE_F32 && a.act == PLATTICE_ACT_NONE && !a.residual && !a.z)
         return launch_narrow<kXT, kNF, kW3, false, true>(a, blocks, s);
     return launch_narrow<kXT, kNF, kW3, false, false>(a, blocks, s);
@@ -52,20 +53,19 @@ cudaError_t run_narrow(const SmallArgs& a, int dtype, cudaStream_t s) {
                                     : run_narrow_nf<kXHalf, false>(a, s);
 }
 
-template <typename TW>
+template <int kWT, bool kX8In>
 static cudaError_t run_few(const SmallArgs& a, cudaStream_t s) {
-    const unsigned ctas = (unsigned)ceil_div(a.n, 32);
-    if (a.rows == 1) k_few<TW, 1><<<ctas, 32 * kFewWarps, 0, s>>>(a);
-    else if (a.rows == 2) k_few<TW, 2><<<ctas, 32 * kFewWarps, 0, s>>>(a);
-    else if (a.rows <= 4) k_few<TW, 4><<<ctas, 32 * kFewWarps, 0, s>>>(a);
-    else k_few<TW, 8><<<ctas, 32 * kFewWarps, 0, s>>>(a);
+    const dim3 ctas((unsigned)ceil_div(a.n, 32), (unsigned)ceil_div(a.rows, 16));
+    if (a.rows <= 8) k_few<kWT, kX8In, 1><<<ctas, 64 * few_splits(kWT), 0, s>>>(a);
+    else k_few<kWT, kX8In, 2><<<ctas, 64 * few_splits(kWT), 0, s>>>(a);
     return cudaGetLastError();
 }
 
 cudaError_t run_few_rows(const SmallArgs& a, int dtype, cudaStream_t s) {
-    return dtype == PLATTICE_F32    ? run_few<float>(a, s)
-           : dtype == PLATTICE_BF16 ? run_few<__nv_bfloat16>(a, s)
-                                    : run_few<__half>(a, s);
+    if (a.x_scale) return dtype == PLATTICE_F32 ? run_few<kXFloat, true>(a, s) : run_few<kXBf16, true>(a, s);
+    return dtype == PLATTICE_F32    ? run_few<kXFloat, false>(a, s)
+           : dtype == PLATTICE_BF16 ? run_few<kXBf16, false>(a, s)
+                                    : run_few<kXHalf, false>(a, s);
 }
 
 }  // namespace plr

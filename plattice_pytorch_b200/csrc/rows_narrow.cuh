@@ -1,6 +1,6 @@
 // rows_narrow.cuh -- the linear map where one side is small: at most 32 output
-// channels (the projections to the filter's features and values), or at most
-// 8 rows.  Both read what they need once and are bound by that read; a
+// channels (the projections to the filter's features and values), or few rows.
+// Both read what they need once and are bound by that read; a
 // 128-row tensor-memory tile would be mostly padding, and staging it costs
 // more than the product.
 #pragma once
@@ -253,6 +253,11 @@ __device__ __forceinline__ void narrow_fetch(NarrowCodes& r, const SmallArgs& a,
 }
 __device__ __forceinline__ float lane_finite(float v) { return is_infinite(fabsf(v)) ? 0.f : fmaxf(fabsf(v), 0.f); }
 
+// The type of the weights.
+template <int kXT, bool kFloat> struct WeightType { typedef __nv_bfloat16 type; };
+template <int kXT> struct WeightType<kXT, true> { typedef float type; };
+template <> struct WeightType<kXHalf, false> { typedef __half type; };
+
 // kSplit: few rows and many channels: the CTA's warps take turns over the
 // channels of the same rows and their sums are added in shared memory, in order.
 // kPlain: float32 results without activation, residual and kept z, as the
@@ -264,6 +269,7 @@ __global__ void __launch_bounds__(32 * kNarrowWarps, narrow_ctas(kXT, kNF)) k_na
     __shared__ float sbias[32];
     __shared__ float column[32];   // 8-bit rows: the power of two that undoes a channel's
     typedef typename NarrowLoad<kXT>::type Raw;
+    const typename WeightType<kXT, kW3>::type* weights = static_cast<const typename WeightType<kXT, kW3>::type*>(a.w);
     const int steps = narrow_steps(a.k), chunks = steps / 4;
     uint2* frag = reinterpret_cast<uint2*>(smem_raw);   // [kPB][steps][kNF][32]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -275,7 +281,7 @@ __global__ void __launch_bounds__(32 * kNarrowWarps, narrow_ctas(kXT, kNF)) k_na
         for (int c = warp; c < 32; c += kNarrowWarps) {
             float most = 0.f;
             if (c < a.n)
-                for (int ch = lane; ch < a.k; ch += 32) most = fmaxf(most, lane_finite(load_param(a.w, a.w_dtype, (int64_t)c * a.k + ch)));
+                for (int ch = lane; ch < a.k; ch += 32) most = fmaxf(most, lane_finite(to_f32(weights[(int64_t)c * a.k + ch])));
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
             const int e = min(max((__float_as_int(most) >> 23) - 127 - 14, -120), 120);
@@ -290,7 +296,7 @@ __global__ void __launch_bounds__(32 * kNarrowWarps, narrow_ctas(kXT, kNF)) k_na
         float v[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            v[j] = col < a.n && ch + j < a.k ? load_param(a.w, a.w_dtype, (int64_t)col * a.k + ch + j) : 0.f;
+            v[j] = col < a.n && ch + j < a.k ? to_f32(weights[(int64_t)col * a.k + ch + j]) : 0.f;
         uint32_t lo[3], hi[3];
         if (kXT == kX8) {
             const float up = 1.f / column[col];   // a power of two
@@ -609,13 +615,15 @@ __global__ void __launch_bounds__(32 * kGradWarps, narrow_grad_ctas(kParts, kNF)
     // fragment f, column c of the weights is channel (c >> 1) 16 + 2 f + (c & 1)
     // of the slice, so that a lane ends up with 16 neighbouring channels
     if (a.need_x) {
+        typedef typename WeightType<kXT, kParts == 3>::type TW;
+        const TW* weights = static_cast<const TW*>(a.s.w);
         for (int i = threadIdx.x; i < kKS * 8 * 32; i += blockDim.x) {
             const int l = i & 31, f = (i >> 5) & 7, s = i >> 8;
             const int ch = ch0 + (l >> 3) * 16 + 2 * f + ((l >> 2) & 1), o = (l & 3) * cols_per_lane + s * 4;
             float v[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                v[j] = o + j < n && ch < k ? load_param(a.s.w, a.s.w_dtype, (int64_t)(o + j) * k + ch) : 0.f;
+                v[j] = o + j < n && ch < k ? to_f32(weights[(int64_t)(o + j) * k + ch]) : 0.f;
             uint32_t lo[kParts], hi[kParts];
             to_parts<kParts, kHalf>(v[0], v[1], lo);
             to_parts<kParts, kHalf>(v[2], v[3], hi);
@@ -902,95 +910,119 @@ __global__ void __launch_bounds__(32 * kGradWarps, narrow_grad_ctas(kParts, kNF)
 
 // -------------------------------------------------------------- few rows
 //
-// One warp per output channel reads its weights once, 16 bytes a lane, against
-// the rows in shared memory (float32, in pieces of 1024 channels); a CTA takes
-// 32 channels, the block of a kept 8-bit pre-activation.  Bound by the read of
-// w: 1024 -> 4096 in bfloat16 (8.4 MB, 1.3 us at the copy rate) takes 4.0 us, of
-// which launching and the last reduction are the larger part (the tiled product:
-// 11 us, since its 128-row slices are staged whatever they hold).
+// The same products with the sides changed over: 16 output channels are the
+// rows of the matrix instruction and 8 or 16 input rows its columns.  Both
+// operands' registers are loaded from memory as they lie there (neither has a
+// second reader in a warp), 32 bytes of a 16-bit type per row and load; a CTA
+// takes 32 channels, the block of a kept 8-bit pre-activation, and its warps
+// take turns over the input channels, 64 at a time, whose sums are added in
+// shared memory in order.  Bound by the read of w and its latency: 1024 -> 4096 in bfloat16 (8.4
+// MB, 1.3 us at the copy rate) takes 3.5 us with 1 row, 4.6 with 16, of which
+// launching is 2.2; 4096 -> 4096 (33.5 MB, 5.1 us) 6.0 and 9.6.
+constexpr int few_splits(int wt) { return wt == kXFloat ? 8 : 16; }   // warps that share the input channels
 
-constexpr int kFewWarps = 32, kFewPiece = 1024;
-
-template <typename TW, int kRows>
-__global__ void __launch_bounds__(32 * kFewWarps) k_few(const SmallArgs a) {
-    __shared__ __align__(16) float sx[kRows][kFewPiece];
-    __shared__ float sz[kRows][32];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int col = blockIdx.x * 32 + warp;
-    const TW* w = static_cast<const TW*>(a.w) + (int64_t)min(col, a.n - 1) * a.k;
-    const int width = (a.k + 31) / 32 * 32;
-    float acc[kRows];
+template <int kWT, bool kX8In, int kN>
+__global__ void __launch_bounds__(64 * few_splits(kWT)) k_few(const SmallArgs a) {
+    constexpr int kSplits = few_splits(kWT), kPW = kWT == kXFloat ? 3 : 1, kXT = kX8In ? (int)kX8 : kWT;
+    constexpr int kPX = kXT == kXFloat ? 3 : 1;
+    __shared__ float part[kSplits][8 * kN][33];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int half = warp & 1, split = warp >> 1, chunks = narrow_steps(a.k) / 4;
+    SmallArgs w = a;   // the weights as the rows of a load
+    w.x = a.w;
+    w.rows = a.n;
+    w.vec_x = a.vec_w;
+    const int64_t col0 = (int64_t)blockIdx.x * 32 + half * 16, row0 = (int64_t)blockIdx.y * (8 * kN);
+    float acc[kN][4];
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) acc[r] = 0.f;
-    for (int base = 0; base < a.k; base += kFewPiece) {
-        Raw8<TW> raw[kFewPiece / 256];   // in flight while the rows are staged
+    for (int j = 0; j < kN; ++j)
 #pragma unroll
-        for (int j = 0; j < kFewPiece / 256; ++j) {
-            const int c = base + j * 256 + lane * 8, left = a.k - c;
-            raw[j].load(w + (left > 0 ? c : 0), a.vec_w && left >= 8, left);
-        }
-        __syncthreads();
-        for (int i = threadIdx.x; i < kRows * kFewPiece; i += 32 * kFewWarps) {
-            const int r = i / kFewPiece, c = i % kFewPiece;
-            float v = 0.f;
-            if (r < a.rows && base + c < a.k) {
-                if (a.x_scale) {
-                    const int64_t at = (int64_t)r * width + base + c;
-                    float q[4];
-                    values4(q, static_cast<const uint8_t*>(a.x)[at], scale_of(a.x_scale[at >> 5]));
-                    v = q[0];
+        for (int i = 0; i < 4; ++i) acc[j][i] = 0.f;
+    if (col0 < a.n) {
+        for (int c = split; c < chunks; c += kSplits) {
+            NarrowRaw<kWT> wr;
+            NarrowRaw<kXT> xr;
+            narrow_load<kWT, 1>(wr, w, col0, c, lane);
+            narrow_load<kXT, 1>(xr, a, row0, c, lane);
+            narrow_mask<kWT, 1>(wr, a.k, c, lane);
+            narrow_mask<kXT, 1>(xr, a.k, c, lane);
+            float sum[kN][4];
+#pragma unroll
+            for (int j = 0; j < kN; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[j][i] = 0.f;
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                uint32_t o[kPW][4], b[kPX][4];
+                narrow_operand<kWT, kPW>(wr, 0, s, o);
+                if constexpr (kX8In) {
+#pragma unroll
+                    for (int h = 0; h < kN; ++h) {
+                        const uint4& q = xr.v[0][h][0];
+                        float v[4];   // exact in bfloat16
+                        values4(v, s == 0 ? q.x : s == 1 ? q.y : s == 2 ? q.z : q.w, scale_of(xr.scale[0][h]));
+                        union { __nv_bfloat162 p; uint32_t u; } x, y;
+                        x.p = __floats2bfloat162_rn(v[0], v[1]);
+                        y.p = __floats2bfloat162_rn(v[2], v[3]);
+                        b[0][h] = x.u;
+                        b[0][2 + h] = y.u;
+                    }
                 } else {
-                    v = to_f32(static_cast<const TW*>(a.x)[(int64_t)r * a.k + base + c]);
+                    narrow_operand<kXT, kPX>(xr, 0, s, b);
                 }
-            }
-            // a lane's 8 channels as two float4 of separate halves: no bank conflicts
-            sx[r][(c & ~255) + ((c >> 2) & 1) * 128 + ((c & 255) >> 3) * 4 + (c & 3)] = v;
-        }
-        __syncthreads();
 #pragma unroll
-        for (int j = 0; j < kFewPiece / 256; ++j) {
-            if (base + j * 256 >= a.k) break;
-            float v[8];
-            raw[j].widen(v);
+                for (int size = 2; size >= 0; --size)   // small products first
 #pragma unroll
-            for (int r = 0; r < kRows; ++r) {
-                const float4 p = *reinterpret_cast<const float4*>(&sx[r][j * 256 + lane * 4]);
-                const float4 q = *reinterpret_cast<const float4*>(&sx[r][j * 256 + 128 + lane * 4]);
-                acc[r] = fmaf(v[0], p.x, fmaf(v[1], p.y, fmaf(v[2], p.z, fmaf(v[3], p.w, acc[r]))));
-                acc[r] = fmaf(v[4], q.x, fmaf(v[5], q.y, fmaf(v[6], q.z, fmaf(v[7], q.w, acc[r]))));
+                    for (int pw = 0; pw < kPW; ++pw) {
+                        const int px = size - pw;
+                        if (px < 0 || px >= kPX) continue;
+#pragma unroll
+                        for (int j = 0; j < kN; ++j)
+                            mma16816<kWT == kXHalf>(sum[j], o[pw][0], o[pw][1], o[pw][2], o[pw][3],
+                                                    make_uint2(b[px][j], b[px][2 + j]));
+                    }
             }
+#pragma unroll
+            for (int j = 0; j < kN; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[j][i] += sum[j][i];
         }
     }
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) {
+    for (int j = 0; j < kN; ++j)
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) acc[r] += __shfl_xor_sync(0xffffffffu, acc[r], o);
-        if (lane == 0) sz[r][warp] = col < a.n ? acc[r] + (a.bias ? load_param(a.bias, a.bias_dtype, col) : 0.f) : 0.f;
-    }
+        for (int i = 0; i < 4; ++i) part[split][j * 8 + t * 2 + (i & 1)][half * 16 + (i >> 1) * 8 + g] = acc[j][i];
     __syncthreads();
-    if (warp >= kRows || warp >= a.rows) return;
+    const int64_t row = row0 + warp;
+    if (warp >= 8 * kN || row >= a.rows) return;
     // a warp per row, a lane per channel
     const int c = blockIdx.x * 32 + lane;
-    float z = sz[warp][lane];
+    const bool have = c < a.n;
+    float z = 0.f;
+    if (have && a.bias) z = load_param(a.bias, a.bias_dtype, c);
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < kSplits; ++i) sum += part[i][warp][lane];
+    z = have ? z + sum : 0.f;
     if (a.z_scale) {
-        float amax = is_infinite(fabsf(z)) ? 0.f : fabsf(z);
+        float amax = lane_finite(z);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
         const int e = block_exponent(amax);
         const float v[8] = {z, 0, 0, 0, 0, 0, 0, 0};
-        const int64_t at = (int64_t)warp * ((a.n + 31) / 32) + blockIdx.x;
+        const int64_t at = row * ((a.n + 31) / 32) + blockIdx.x;
         static_cast<uint8_t*>(a.z)[at * 32 + lane] = (uint8_t)codes8_of(v, pow2(-e), is_infinite(fabsf(z))).x;
         if (lane == 0) a.z_scale[at] = (uint8_t)(e + 127);
-    } else if (a.z && c < a.n) {
-        store_param(a.z, a.out_dtype, (int64_t)warp * a.n + c, z);
+    } else if (a.z && have) {
+        store_param(a.z, a.out_dtype, row * a.n + c, z);
     }
-    if (c >= a.n) return;
+    if (!have) return;
     float y[2] = {z, 0.f};
     activate(y, a.act);
-    if (a.residual) y[0] += load_param(a.residual, a.out_dtype, (int64_t)warp * a.n + c);
-    if (c < a.split) store_param(a.y0, a.out_dtype, (int64_t)warp * a.split + c, y[0]);
-    else if (a.split) store_param(a.y1, a.out_dtype, (int64_t)warp * (a.n - a.split) + c - a.split, y[0]);
-    else store_param(a.y0, a.out_dtype, (int64_t)warp * a.n + c, y[0]);
+    if (a.residual) y[0] += load_param(a.residual, a.out_dtype, row * a.n + c);
+    if (c < a.split) store_param(a.y0, a.out_dtype, row * a.split + c, y[0]);
+    else if (a.split) store_param(a.y1, a.out_dtype, row * (a.n - a.split) + c - a.split, y[0]);
+    else store_param(a.y0, a.out_dtype, row * a.n + c, y[0]);
 }
 
 }  // namespace plr

@@ -36,7 +36,10 @@ struct SmallGradArgs {
 
 __host__ __device__ inline int narrow_steps(int k) { return (k + 63) / 64 * 4; }   // of 16 channels
 __host__ inline int64_t narrow_fragments(int k, int nf, int parts) { return (int64_t)parts * narrow_steps(k) * nf * 256; }
-constexpr int64_t kNarrowMost = 64 * 1024;   // bytes of weights: two CTAs then share an SM
+// Bytes of weights that k_narrow takes: what fits beside its staging (even one
+// CTA an SM beats the tiles, which write float32's parts first: 65536 rows,
+// 1024 -> 24, float32: 107 against 225 us).
+constexpr int64_t kNarrowMost = 190 * 1024;
 constexpr int kGradWarps = 4;
 constexpr int kNarrowGradMost = 65535 * 64;      // input channels of the narrow backward: slices are gridDim.y
 // CTAs of the narrow backward that share an SM

@@ -636,3 +636,48 @@ def test_changed_fields_of_rows8_are_refused(dev, R):
                      lambda: R.linear_backward(torch.zeros(4, 5, device=dev), r, w)):
             with pytest.raises(RuntimeError):
                 call()
+
+
+# Rows enough for the forms that many rows take, at sizes where each can go wrong.
+LARGER_SHAPES = [(2500, 50, 24), (2401, 7, 2), (2400, 264, 1), (4000, 64, 8), (2500, 1000, 32), (2385, 1, 16),
+                 (9500, 200, 17), (2100, 130, 200), (2500, 96, 33), (2401, 512, 72), (3700, 33, 257), (8000, 29, 41),
+                 (2500, 9000, 8), (150, 72, 5000), (17, 40, 4800), (2370, 640, 32)]
+
+
+@pytest.mark.parametrize("dtype,x8", KINDS)
+@pytest.mark.parametrize("rows,k,n", LARGER_SHAPES)
+@pytest.mark.parametrize("act,residual,keep,out32", [("none", False, None, True), ("gelu", True, "8bit", False),
+                                                     ("silu", False, "full", False), ("relu", True, None, True)])
+def test_linear_larger(dev, R, rows, k, n, dtype, x8, act, residual, keep, out32):
+    test_linear(dev, R, rows, k, n, dtype, x8, act, residual, keep, out32)
+
+
+@pytest.mark.parametrize("dtype,x8", KINDS)
+@pytest.mark.parametrize("rows,k,n,split", [(2500, 64, 24, 16), (2399, 50, 8, 5), (2500, 700, 13, 1), (3000, 96, 150, 70)])
+def test_linear_split_larger(dev, R, rows, k, n, split, dtype, x8):
+    test_linear_split(dev, R, rows, k, n, split, dtype, x8)
+
+
+def test_repeat_stream_and_graph_larger(dev, R):
+    test_repeat_stream_and_graph_give_the_same_bits(dev, R, 7001)
+
+
+@pytest.mark.parametrize("k,n", [(64, 24), (200, 24), (64, 40), (72, 520)])
+def test_not_finite_and_unaligned_larger(dev, R, k, n):
+    """Rows of values that are not finite stay in their rows, and storage that
+    starts one element later gives the same products within their bounds."""
+    rows = 5000
+    for dtype in DTYPES.values():
+        x, w = _randn((rows, k), 63, dtype), _randn((n, k), 64, dtype, k ** -0.5)
+        clean, _ = R.linear(x.to(dev), w.to(dev))
+        moved = torch.empty(rows * k + 1, dtype=dtype, device=dev)[1:].view(rows, k).copy_(x)
+        y, _ = R.linear(moved, w.to(dev))
+        ye = f64(x) @ f64(w).T
+        for got in (clean, y):
+            assert worst(f64(got), ye, _forward_tolerance(f64(x), f64(w), None, 0 * ye, ye, k, dtype)) <= 1
+        x[5, 3], x[4130, 60] = float("nan"), float("inf")
+        y, _ = R.linear(x.to(dev), w.to(dev))
+        good = torch.ones(rows, dtype=torch.bool)
+        good[5] = good[4130] = False
+        assert torch.equal(y.cpu()[good], clean.cpu()[good])
+        assert not torch.isfinite(y[5]).any() and not torch.isfinite(y[4130]).any()

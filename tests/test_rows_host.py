@@ -72,7 +72,7 @@ def test_linear_arguments(lib):
                    {"split": 5, "act": 1}, {"rows": 1 << 40}):
             assert size(ctypes.byref(_args(**kw)), ctypes.byref(b)) == _lib.ERR_INVALID, kw
             assert f(ctypes.byref(_args(**kw)), None) == _lib.ERR_INVALID, kw
-        assert f(ctypes.byref(_args(workspace=None, n=72)), None) == _lib.ERR_WORKSPACE   # float32: parts of x and w
+        assert f(ctypes.byref(_args(workspace=None, rows=100000, n=72)), None) == _lib.ERR_WORKSPACE   # float32: parts of x and w
         assert f(ctypes.byref(_args(workspace_bytes=0, rows=100000, n=72)), None) == _lib.ERR_WORKSPACE
         assert f(ctypes.byref(_args(dtype=1, out_dtype=1, x=264, x_scale=256)), None) == _lib.ERR_INVALID   # codes not aligned
     for kw in ({"x": None}, {"w": None}, {"y0": None}, {"split": 5, "y1": None}, {"z": None, "z_scale": 256},
@@ -89,7 +89,7 @@ def test_linear_alignments(lib):
     for n in (24, 72):
         assert lib.plattice_linear_backward(ctypes.byref(_args(n=n, act=2, z=264, z_scale=256)), None) == _lib.ERR_INVALID
         assert lib.plattice_linear_backward(ctypes.byref(_args(n=n, workspace=272)), None) == _lib.ERR_WORKSPACE
-    assert lib.plattice_linear(ctypes.byref(_args(n=72, workspace=264)), None) == _lib.ERR_WORKSPACE
+    assert lib.plattice_linear(ctypes.byref(_args(rows=100000, n=72, workspace=264)), None) == _lib.ERR_WORKSPACE
 
 
 @pytest.fixture
