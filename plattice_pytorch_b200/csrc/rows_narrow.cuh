@@ -407,15 +407,16 @@ __global__ void __launch_bounds__(32 * kNarrowWarps, narrow_ctas(kXT, kNF)) k_na
                 continue;
             } else {
             narrow_mask<kXT>(raw, a.k, c, lane);
-            // the sum of these 64 channels by itself: the matrix instruction cuts
-            // where an addition rounds, by which a long chain of them drifts
-            float sum[kM][kNF][4];
+            // the sum of these 64 channels by itself, and float32's products of small
+            // parts apart from it: the matrix instruction cuts where an addition
+            // rounds, by which a long chain of them drifts
+            float sum[kM][kNF][4], low[kM][kNF][4];
 #pragma unroll
             for (int m = 0; m < kM; ++m)
 #pragma unroll
                 for (int f = 0; f < kNF; ++f)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) sum[m][f][i] = 0.f;
+                    for (int i = 0; i < 4; ++i) sum[m][f][i] = low[m][f][i] = 0.f;
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
                 uint2 b[kPB][kNF];
@@ -435,7 +436,7 @@ __global__ void __launch_bounds__(32 * kNarrowWarps, narrow_ctas(kXT, kNF)) k_na
                             if (pb < 0 || pb >= kPB) continue;
 #pragma unroll
                             for (int f = 0; f < kNF; ++f)
-                                mma16816<kXT == kXHalf>(sum[m][f], o[pa][0], o[pa][1], o[pa][2], o[pa][3], b[pb][f]);
+                                mma16816<kXT == kXHalf>(size ? low[m][f] : sum[m][f], o[pa][0], o[pa][1], o[pa][2], o[pa][3], b[pb][f]);
                         }
                 }
             }
@@ -443,6 +444,10 @@ __global__ void __launch_bounds__(32 * kNarrowWarps, narrow_ctas(kXT, kNF)) k_na
             for (int m = 0; m < kM; ++m)
 #pragma unroll
                 for (int f = 0; f < kNF; ++f) {
+                    if (kPA == 3) {
+                        add2(sum[m][f][0], sum[m][f][1], low[m][f][0], low[m][f][1]);
+                        add2(sum[m][f][2], sum[m][f][3], low[m][f][2], low[m][f][3]);
+                    }
                     add2(acc[m][f][0], acc[m][f][1], sum[m][f][0], sum[m][f][1]);
                     add2(acc[m][f][2], acc[m][f][3], sum[m][f][2], sum[m][f][3]);
                 }
@@ -946,11 +951,11 @@ __global__ void __launch_bounds__(64 * few_splits(kWT)) k_few(const SmallArgs a)
             narrow_load<kXT, 1>(xr, a, row0, c, lane);
             narrow_mask<kWT, 1>(wr, a.k, c, lane);
             narrow_mask<kXT, 1>(xr, a.k, c, lane);
-            float sum[kN][4];
+            float sum[kN][4], low[kN][4];   // low: float32's products of small parts (see k_narrow)
 #pragma unroll
             for (int j = 0; j < kN; ++j)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) sum[j][i] = 0.f;
+                for (int i = 0; i < 4; ++i) sum[j][i] = low[j][i] = 0.f;
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
                 uint32_t o[kPW][4], b[kPX][4];
@@ -978,14 +983,14 @@ __global__ void __launch_bounds__(64 * few_splits(kWT)) k_few(const SmallArgs a)
                         if (px < 0 || px >= kPX) continue;
 #pragma unroll
                         for (int j = 0; j < kN; ++j)
-                            mma16816<kWT == kXHalf>(sum[j], o[pw][0], o[pw][1], o[pw][2], o[pw][3],
+                            mma16816<kWT == kXHalf>(size ? low[j] : sum[j], o[pw][0], o[pw][1], o[pw][2], o[pw][3],
                                                     make_uint2(b[px][j], b[px][2 + j]));
                     }
             }
 #pragma unroll
             for (int j = 0; j < kN; ++j)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[j][i] += sum[j][i];
+                for (int i = 0; i < 4; ++i) acc[j][i] += kPW == 3 ? sum[j][i] + low[j][i] : sum[j][i];
         }
     }
 #pragma unroll
