@@ -6,6 +6,7 @@
 // one by one and raises the message, or makes the call itself.  A failed
 // library call gives its status as an int.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/extension.h>
@@ -87,9 +88,19 @@ int64_t rows_of(const std::vector<int64_t>& shape) {
     return n;
 }
 
-Rows8 empty8(int64_t rows, int64_t c, const at::TensorOptions& like) {
-    const auto o = like.dtype(at::kByte);
-    return {at::empty({rows, width8(c)}, o), at::empty({rows, width8(c) / 32}, o)};
+// at::empty without the dispatcher's way there (0.3 us of a call's host time
+// per tensor; a call makes up to five).
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType t, const at::Device& d) {
+    return at::detail::empty_cuda(sizes, t, d, std::nullopt);
+}
+at::Tensor fresh_like(const at::Tensor& t) { return fresh(t.sizes(), t.scalar_type(), t.device()); }
+
+at::ScalarType type_of(int dtype) {
+    return dtype == PLATTICE_F32 ? at::kFloat : dtype == PLATTICE_BF16 ? at::kBFloat16 : at::kHalf;
+}
+
+Rows8 empty8(int64_t rows, int64_t c, const at::Device& d) {
+    return {fresh({rows, width8(c)}, at::kByte, d), fresh({rows, width8(c) / 32}, at::kByte, d)};
 }
 
 py::object wrap(const at::Tensor& t) { return py::reinterpret_steal<py::object>(THPVariable_Wrap(t)); }
@@ -101,7 +112,7 @@ py::object rows_pack8(const py::object& x_) {
     const int64_t c = x->size(-1), rows = x->numel() / c;
     if (c > (1 << 30)) return py::none();
     const c10::cuda::CUDAGuard guard(x->device());
-    const Rows8 r = empty8(rows, c, x->options());
+    const Rows8 r = empty8(rows, c, x->device());
     const int rc = g_rows.pack8(r.q.data_ptr<uint8_t>(), r.scale.data_ptr<uint8_t>(), x->data_ptr(),
                                 dtype_code(x->scalar_type()), rows, (int)c, stream_of(x->device()));
     if (rc) return py::int_(rc);
@@ -113,8 +124,7 @@ py::object rows_unpack8(const py::object& q_, const py::object& scale_, const st
     if (!q || !scale || shape.empty() || dtype < 0 || dtype > 2 || !holds(*q, *scale, rows_of(shape), shape.back()))
         return py::none();
     const c10::cuda::CUDAGuard guard(q->device());
-    const at::Tensor y = at::empty(
-        shape, q->options().dtype(dtype == PLATTICE_F32 ? at::kFloat : dtype == PLATTICE_BF16 ? at::kBFloat16 : at::kHalf));
+    const at::Tensor y = fresh(shape, type_of(dtype), q->device());
     const int rc = g_rows.unpack8(y.data_ptr(), dtype, q->data_ptr<uint8_t>(), scale->data_ptr<uint8_t>(), q->size(0),
                                   (int)shape.back(), stream_of(q->device()));
     if (rc) return py::int_(rc);
@@ -131,12 +141,12 @@ py::object rows_rms_norm(const py::object& x_, const py::object& gain_, const py
         (!residual_.is_none() && (!residual || !like(*residual, *x))))
         return py::none();
     const c10::cuda::CUDAGuard guard(x->device());
-    const at::Tensor rstd = at::empty(x->sizes().slice(0, x->dim() - 1), x->options().dtype(at::kFloat));
-    const at::Tensor h = residual ? at::empty(x->sizes(), x->options()) : at::Tensor();
+    const at::Tensor rstd = fresh(x->sizes().slice(0, x->dim() - 1), at::kFloat, x->device());
+    const at::Tensor h = residual ? fresh_like(*x) : at::Tensor();
     Rows8 y8;
     at::Tensor y;
-    if (pack) y8 = empty8(rows, c, x->options());
-    else y = at::empty(x->sizes(), x->options());
+    if (pack) y8 = empty8(rows, c, x->device());
+    else y = fresh_like(*x);
     const int rc = g_rows.norm(pack ? y8.q.data_ptr() : y.data_ptr(), pack ? y8.scale.data_ptr<uint8_t>() : nullptr,
                                residual ? h.data_ptr() : nullptr, rstd.data_ptr<float>(), x->data_ptr(),
                                residual ? residual->data_ptr() : nullptr, gain->data_ptr(), dtype_code(x->scalar_type()),
@@ -159,8 +169,8 @@ py::object rows_rms_norm_backward(const py::object& gy_, const py::object& h_, c
     size_t need = 0;
     int rc = g_rows.norm_ws(rows, (int)c, &need);
     if (rc) return py::int_(rc);
-    const at::Tensor gx = at::empty(h->sizes(), h->options()), gg = at::empty(gain->sizes(), gain->options());
-    const at::Tensor ws = at::empty({(int64_t)need}, h->options().dtype(at::kByte));
+    const at::Tensor gx = fresh_like(*h), gg = fresh_like(*gain);
+    const at::Tensor ws = fresh({(int64_t)need}, at::kByte, h->device());
     rc = g_rows.norm_backward(gx.data_ptr(), gg.data_ptr(), gy->data_ptr(), h->data_ptr(), rstd->data_ptr<float>(),
                               gain->data_ptr(), gh ? gh->data_ptr() : nullptr, ws.data_ptr(), need,
                               dtype_code(h->scalar_type()), dtype_code(gain->scalar_type()), rows, (int)c,
@@ -214,34 +224,34 @@ py::object rows_linear(const py::object& x_, const py::object& scale_, const py:
     const int64_t n = w->size(0);
     const at::Tensor* bias = bias_.is_none() ? nullptr : floating(bias_);
     const at::Tensor* residual = residual_.is_none() ? nullptr : floating(residual_);
-    const auto out = w->options().dtype(out32 ? at::kFloat : w->scalar_type());
+    const at::ScalarType out = out32 ? at::kFloat : w->scalar_type();
     if ((!bias_.is_none() && !param(bias, n, w->device())) || split < 0 || split >= n || (split && (act || residual)))
         return py::none();
     std::vector<int64_t> shape(in.lead);
     shape.push_back(n);
     if (!residual_.is_none() && (!residual || residual->sizes() != at::IntArrayRef(shape) ||
-                                 residual->scalar_type() != out.dtype().toScalarType() || residual->device() != w->device()))
+                                 residual->scalar_type() != out || residual->device() != w->device()))
         return py::none();
     const c10::cuda::CUDAGuard guard(w->device());
     plattice_linear_args a = {};
     at::Tensor y0, y1, z, z_scale;
     if (split) {
         shape.back() = split;
-        y0 = at::empty(shape, out);
+        y0 = fresh(shape, out, w->device());
         shape.back() = n - split;
-        y1 = at::empty(shape, out);
+        y1 = fresh(shape, out, w->device());
         a.y1 = y1.data_ptr();
     } else {
-        y0 = at::empty(shape, out);
+        y0 = fresh(shape, out, w->device());
     }
     if (keep == 1) {
-        const Rows8 r = empty8(in.rows, n, out);
+        const Rows8 r = empty8(in.rows, n, w->device());
         z = r.q;
         z_scale = r.scale;
         a.z_scale = z_scale.data_ptr<uint8_t>();
     } else if (keep == 2) {
         shape.back() = n;
-        z = at::empty(shape, out);
+        z = fresh(shape, out, w->device());
     }
     a.x = in.x->data_ptr();
     a.x_scale = in.scale ? in.scale->data_ptr<uint8_t>() : nullptr;
@@ -262,7 +272,7 @@ py::object rows_linear(const py::object& x_, const py::object& scale_, const py:
     if (rc) return py::int_(rc);
     at::Tensor ws;
     if (a.workspace_bytes) {
-        ws = at::empty({(int64_t)a.workspace_bytes}, w->options().dtype(at::kByte));
+        ws = fresh({(int64_t)a.workspace_bytes}, at::kByte, w->device());
         a.workspace = ws.data_ptr();
     }
     rc = g_rows.linear(&a, stream_of(w->device()));
@@ -311,19 +321,18 @@ py::object rows_linear_backward(const py::object& g0_, const py::object& g1_, co
         }
     }
     const c10::cuda::CUDAGuard guard(w->device());
-    const auto opts = w->options();
     at::Tensor gx, gw, gb;
     if (need_x) {
         shape.back() = in.k;
-        gx = at::empty(shape, opts);
+        gx = fresh(shape, w->scalar_type(), w->device());
         a.grad_x = gx.data_ptr();
     }
     if (need_w) {
-        gw = at::empty(w->sizes(), opts);
+        gw = fresh_like(*w);
         a.grad_w = gw.data_ptr();
     }
     if (need_b) {
-        gb = at::empty({n}, opts.dtype(bias_dtype == PLATTICE_F32 ? at::kFloat : bias_dtype == PLATTICE_BF16 ? at::kBFloat16 : at::kHalf));
+        gb = fresh({n}, type_of(bias_dtype), w->device());
         a.grad_bias = gb.data_ptr();
     }
     a.x = in.x->data_ptr();
@@ -340,7 +349,7 @@ py::object rows_linear_backward(const py::object& g0_, const py::object& g1_, co
     a.act = act;
     int rc = g_rows.linear_backward_ws(&a, &a.workspace_bytes);
     if (rc) return py::int_(rc);
-    const at::Tensor ws = at::empty({(int64_t)a.workspace_bytes}, opts.dtype(at::kByte));
+    const at::Tensor ws = fresh({(int64_t)a.workspace_bytes}, at::kByte, w->device());
     a.workspace = ws.data_ptr();
     rc = g_rows.linear_backward(&a, stream_of(w->device()));
     if (rc) return py::int_(rc);

@@ -681,3 +681,24 @@ def test_not_finite_and_unaligned_larger(dev, R, k, n):
         good[5] = good[4130] = False
         assert torch.equal(y.cpu()[good], clean.cpu()[good])
         assert not torch.isfinite(y[5]).any() and not torch.isfinite(y[4130]).any()
+
+
+def test_inference_mode_and_inputs_with_gradients(dev, R):
+    """The calls are not autograd Functions: they give the same under every
+    grad mode, and nothing they return has a history."""
+    x = _randn((70, 64), 110).to(dev)
+    w, g = _randn((40, 64), 111).to(dev), _randn((64,), 112).to(dev)
+
+    def run(x, w, g):
+        y8, h, rstd = R.rms_norm(x, g, x, pack=True)
+        y, z = R.linear(y8, w, act="gelu", keep="8bit")
+        gx, gw, gb = R.linear_backward(y, y8, w, z, act="gelu")
+        return [R.unpack8(y8), h, rstd, y, R.unpack8(z), gx, gw, gb, *R.rms_norm_backward(gx, h, rstd, g)]
+    want = run(x, w, g)
+    with torch.inference_mode():
+        got = run(x.clone(), w.clone(), g.clone())
+        assert all(t.is_inference() for t in got)
+    got2 = run(*(t.clone().requires_grad_() for t in (x, w, g)))
+    assert not any(t.requires_grad for t in got2)
+    for a, b, c in zip(want, got, got2):
+        assert torch.equal(a, b) and torch.equal(a, c)
