@@ -470,18 +470,20 @@ static cudaError_t unpacked(Operand* o, const plattice_linear_args* a, void* ws,
 
 // How a forward runs.  k_few where its CTAs of 16 rows x 32 channels fit on the
 // device at a time (with float32 weights, whose parts the tiles need written
-// first, up to three times that); k_narrow with at most 32 output channels;
-// else tiles.  16-bit rows that TMA can read go to the tiles too once n k is
-// above 1536.  Measured (us; bfloat16 unless noted):
-//   k_few / tiles   1024 -> 4096, 16 rows 4.6 / 9.4, 32 rows (1.7 rounds) 8.5 / 9.0;
-//     256 -> 256, 256 rows 3.3 / 4.6, 512 rows 5.6 / 4.6; float32, 512 -> 512, 128
-//     rows 6.2 / 20.3, 512 rows (3.5 rounds) 21.1 / 20.7
+// first, up to twice that); k_narrow with at most 32 output channels; else
+// tiles.  Of 16-bit types the tiles take, too, rows that TMA can read once n k is
+// above 1536, and deep sums of a few thousand rows (narrow_shares).  Measured (us;
+// bfloat16 unless noted):
+//   k_few / tiles   1024 -> 4096, 16 rows 4.7 / 9.3, 32 rows (1.7 rounds) 8.5 / 8.7;
+//     256 -> 256, 256 rows 3.3 / 4.2, 512 rows 5.7 / 4.3; float32, 512 -> 512, 128
+//     rows 6.3 / 16.6, 256 rows 11.5 / 16.8, 512 rows (3.5 rounds) 21.6 / 17.1
 //   k_few / k_narrow   64 -> 24, 2300 rows 3.1 / 3.2, 4700 rows 5.3 / 3.3; float32,
 //     256 -> 24, 2300 rows 4.3 / 6.2, 9400 rows 14.1 / 9.6
-//   k_narrow / tiles   262144 rows, n 8: k 64 9.6 / 13.8, k 256 26.6 / 27.3, k 1024
-//     103 / 88; n 24: k 64 15.4 / 15.6, k 128 21.5 / 17.2; k 100 (no 16-byte rows)
-//     34.6 / 52.4; 65536 rows, n 24, from 8 bits: k 64 7.0 / 10.4, k 1024 38 / 65;
-//     float32: k 64 9.6 / 19.6, k 1024 107 / 225
+//   k_narrow / tiles   262144 rows, n 8: k 64 9.6 / 13.7, k 192 21.5 / 22.0, k 1024
+//     106 / 88; n 24: k 64 14.0 / 15.5, k 128 19.9 / 17.1; k 100 (no 16-byte rows)
+//     33.4 / 52.3; 65536 rows, n 24, from 8 bits: k 64 7.0 / 10.3, k 1024 38 / 62;
+//     float32: k 64 9.4 / 18.2, k 1024 94 / 206; 9400 rows, n 24: from 8 bits, k 1024
+//     18.2 / 12.2, float32, k 768 23.0 / 29.9
 enum Way { kWayFew, kWayNarrow, kWayTiles };
 
 static Way forward_way(const plattice_linear_args* a) {
@@ -490,9 +492,10 @@ static Way forward_way(const plattice_linear_args* a) {
     const int parts = a->dtype == PLATTICE_F32 ? 3 : 1;
     const bool tiles_read = !a->x_scale && tma_ready(a->x, a->dtype, a->k);
     if (a->n <= 32 && (!tiles_read || (int64_t)a->n * a->k <= 1536) &&
+        !(parts == 1 && narrow_shares(ceil_div(a->rows, a->x_scale ? 32 : 16), a->k)) &&
         narrow_fragments(a->k, (int)ceil_div(a->n, 8), parts) <= kNarrowMost)
         return kWayNarrow;
-    return parts == 3 && few <= 3 * (int64_t)sm_count() ? kWayFew : kWayTiles;
+    return parts == 3 && few <= 2 * (int64_t)sm_count() ? kWayFew : kWayTiles;
 }
 
 struct ForwardPlan {
@@ -527,13 +530,14 @@ struct BackwardPlan {
 
 // Whether the backward runs in one pass over slices of 64 input channels
 // (k_narrow_grad), each of which makes gz anew, or as tiled products.  Measured
-// (us, one pass / tiles), 16-bit types: n 16, k 512, 65536 rows 48 / 55; k 1896,
-// 34559 rows 119 / 93, from 8 bits 115 / 125; from 8 bits n 32: k 128, 262144
-// rows 76 / 76, k 256 135 / 125; float32 n 8, k 2048, 8192 rows 72 / 115.
+// (us, one pass / tiles), bfloat16, 65536 rows: n 16, k 512 43 / 53, k 768 80 / 70;
+// n 24, k 256 35.5 / 36.6, k 512 85 / 55; 100 rows, n 16, k 512 8.7 / 14.0; from 8
+// bits: 34559 rows, n 16, k 1896 102 / 126, 262144 rows, n 32, k 256 103 / 118;
+// float32, 8192 rows, n 8, k 2048 69 / 112.
 static bool backward_is_narrow(const plattice_linear_args* a) {
     if (a->n > 32 || a->k > kNarrowGradMost) return false;
-    if (a->dtype == PLATTICE_F32 || a->k <= 128) return true;
-    return a->n <= 24 && (a->x_scale || a->k <= 768);
+    if (a->dtype == PLATTICE_F32 || (int64_t)a->n * a->k <= 8192) return true;
+    return a->x_scale && a->n <= 24;
 }
 
 static BackwardPlan backward_plan(const plattice_linear_args* a) {

@@ -27,10 +27,8 @@ static cudaError_t launch_narrow(const SmallArgs& a, int64_t blocks, cudaStream_
 template <int kXT, bool kW3, int kNF>
 static cudaError_t run_narrow_as(const SmallArgs& a, cudaStream_t s) {
     const int64_t blocks = ceil_div(a.rows, 16 * NarrowShape<kXT>::kM);
-    // few blocks of rows and many channels: the warps of a CTA share a block
-    // (us, n 24, shared / apart: float32, 4700 rows, k 128 6.8 / 6.2, k 768 15.4 /
-    // 21.6; from 8 bits, 9400 rows, k 256 8.7 / 8.0, k 1024 18.7 / 22.4)
-    if (blocks * 256 <= (int64_t)sm_count() * a.k) return launch_narrow<kXT, kNF, kW3, true, false>(a, blocks, s);
+    if constexpr (kW3)
+        if (narrow_shares(blocks, a.k)) return launch_narrow<kXT, kNF, kW3, true, false>(a, blocks, s);
     if (a.out_dtype == PLATTICE_F32 && a.act == PLATTICE_ACT_NONE && !a.residual && !a.z)
         return launch_narrow<kXT, kNF, kW3, false, true>(a, blocks, s);
     return launch_narrow<kXT, kNF, kW3, false, false>(a, blocks, s);
