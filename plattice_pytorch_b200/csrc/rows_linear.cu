@@ -533,10 +533,14 @@ struct BackwardPlan {
 // (us, one pass / tiles), bfloat16, 65536 rows: n 16, k 512 43 / 53, k 768 80 / 70;
 // n 24, k 256 35.5 / 36.6, k 512 85 / 55; 100 rows, n 16, k 512 8.7 / 14.0; from 8
 // bits: 34559 rows, n 16, k 1896 102 / 126, 262144 rows, n 32, k 256 103 / 118;
-// float32, 8192 rows, n 8, k 2048 69 / 112.
+// float32, 8192 rows, n 8, k 2048 69 / 112.  Rows on no 16-byte boundaries, whose
+// channels the pass loads and stores one by one: bfloat16, k 50, n 24, 262144 rows
+// 71 / 83; k 95, n 8, 20000 rows 26 / 29; k 95, n 4, 848040 rows 587 / 267.
 static bool backward_is_narrow(const plattice_linear_args* a) {
     if (a->n > 32 || a->k > kNarrowGradMost) return false;
-    if (a->dtype == PLATTICE_F32 || (int64_t)a->n * a->k <= 8192) return true;
+    if (a->dtype == PLATTICE_F32) return true;
+    if (a->k % 8 && a->k > 64 && a->rows > 24000) return false;
+    if ((int64_t)a->n * a->k <= 8192) return true;
     return a->x_scale && a->n <= 24;
 }
 
@@ -595,7 +599,7 @@ static cudaError_t launch_grad_z(const GradArgs& g, const BackwardPlan& p, cudaS
 static cudaError_t forward_small(const plattice_linear_args* a, Way way, cudaStream_t s) {
     const int e = a->dtype == PLATTICE_F32 ? 4 : 8;   // elements of 16 bytes
     const SmallArgs p{a->x, a->x_scale, a->w, a->bias, a->residual, a->y0, a->y1, a->z, a->z_scale, a->rows,
-                      a->k, a->n, a->split, a->act, a->dtype, a->out_dtype, a->bias_dtype,
+                      a->k, a->n, a->split, a->act, a->out_dtype, a->bias_dtype,
                       a->k % e == 0 && aligned16(a->x), a->k % 8 == 0 && aligned16(a->w),
                       aligned16(a->y0) && (!a->y1 || aligned16(a->y1)) && (!a->residual || aligned16(a->residual)) &&
                           (!a->z || aligned16(a->z))};
@@ -647,7 +651,6 @@ static cudaError_t backward_narrow(const plattice_linear_args* a, const Backward
     g.s.n = a->n;
     g.s.split = a->split;
     g.s.act = a->act;
-    g.s.w_dtype = a->dtype;
     g.s.out_dtype = a->out_dtype;
     g.s.vec_x = a->k % per == 0 && aligned16(a->x);
     g.g0 = a->grad0;

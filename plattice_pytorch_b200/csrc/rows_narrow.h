@@ -17,7 +17,7 @@ struct SmallArgs {
     uint8_t* z_scale;
     int64_t rows;
     int k, n, split, act;
-    int w_dtype, out_dtype, bias_dtype;
+    int out_dtype, bias_dtype;
     bool vec_x;    // 16-byte accesses to x's rows
     bool vec_w;    // the same for w's
     bool vec_y;    // the outputs and the residual begin on 16-byte boundaries
