@@ -138,7 +138,7 @@ __device__ __forceinline__ void narrow_load(NarrowRaw<kXT>& r, const SmallArgs& 
 #pragma unroll
                 for (int i = 0; i < NarrowShape<kXT>::kRaw; ++i) {
                     const int c = ch + i * kPer;
-                    r.v[m][h][i] = *reinterpret_cast<const uint4*>(p + (c < a.k ? c : 0) * kSize);
+                    r.v[m][h][i] = *reinterpret_cast<const uint4*>(p + (int64_t)(c < a.k ? c : 0) * kSize);
                 }
             } else {
 #pragma unroll
