@@ -14,14 +14,14 @@ namespace plr {
 // ----------------------------------------------------- operands for the MMAs
 
 __device__ __forceinline__ void store_parts(__nv_bfloat16* p, int64_t stride, const float (&v)[8], bool vec, int n) {
-    union { uint4 u; __nv_bfloat16 h[8]; } o[3];
+    union { uint4 u; uint32_t w[4]; __nv_bfloat16 h[8]; } o[3];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        __nv_bfloat16 t[3];
-        split3(v[i], t);
-        o[0].h[i] = t[0];
-        o[1].h[i] = t[1];
-        o[2].h[i] = t[2];
+    for (int i = 0; i < 4; ++i) {
+        uint32_t t[3];
+        split_pair(v[2 * i], v[2 * i + 1], t);
+        o[0].w[i] = t[0];
+        o[1].w[i] = t[1];
+        o[2].w[i] = t[2];
     }
 #pragma unroll
     for (int j = 0; j < 3; ++j) {

@@ -23,7 +23,7 @@ enum XType { kX8 = 0, kXBf16 = 1, kXHalf = 2, kXFloat = 3 };
 // instruction's pairs: 16 bytes of codes (32 of a 16-bit type, 64 of float32)
 // per row and load, straight into the operand's registers.
 //
-// float32 runs as three bfloat16 parts (split3), six products, small first.
+// float32 runs as three bfloat16 parts (split_pair), six products, small first.
 //
 // 8-bit rows go in as float16, one conversion a pair of codes and exact, with
 // their scales left out: a step then stays within a block of 32 channels (lane
@@ -189,8 +189,8 @@ __device__ __forceinline__ void narrow_operand(const NarrowRaw<kXT>& r, int m, i
         if (kXT == kXFloat) {
             const uint4& q = r.v[m][h][s];
             uint32_t lo[3], hi[3];
-            split3_pair(__uint_as_float(q.x), __uint_as_float(q.y), lo);
-            split3_pair(__uint_as_float(q.z), __uint_as_float(q.w), hi);
+            split_pair(__uint_as_float(q.x), __uint_as_float(q.y), lo);
+            split_pair(__uint_as_float(q.z), __uint_as_float(q.w), hi);
 #pragma unroll
             for (int p = 0; p < kPA; ++p) {
                 o[p][h] = lo[p];
@@ -305,8 +305,8 @@ __global__ void __launch_bounds__(32 * kNarrowWarps, narrow_ctas(kXT, kNF)) k_na
             half_parts(v[0], v[1], lo);
             half_parts(v[2], v[3], hi);
         } else if (kW3) {
-            split3_pair(v[0], v[1], lo);
-            split3_pair(v[2], v[3], hi);
+            split_pair(v[0], v[1], lo);
+            split_pair(v[2], v[3], hi);
         } else if (kXT == kXHalf) {
             union { __half2 h; uint32_t u; } x, y;
             x.h = __floats2half2_rn(v[0], v[1]);
@@ -568,11 +568,11 @@ template <int kXT, int kParts> struct NarrowGradShape {
 };
 
 // a and b as kP packed parts: one rounded, two (rounded, and what that left),
-// or split3's three.
+// or split_pair's three.
 template <int kP, bool kHalf>
 __device__ __forceinline__ void to_parts(float a, float b, uint32_t (&o)[kP]) {
     if constexpr (kP == 3) {
-        split3_pair(a, b, o);
+        split_pair(a, b, o);
     } else {
 #pragma unroll
         for (int i = 0; i < kP; ++i) {
@@ -727,8 +727,8 @@ __global__ void __launch_bounds__(32 * kGradWarps, narrow_grad_ctas(kParts, kNF)
                     for (int i = 0; i < 4; ++i) {
                         const uint4& q = xn.v[0][h][i % NarrowShape<kXT>::kRaw];
                         uint32_t lo[3], hi[3];
-                        split3_pair(__uint_as_float(q.x), __uint_as_float(q.y), lo);
-                        split3_pair(__uint_as_float(q.z), __uint_as_float(q.w), hi);
+                        split_pair(__uint_as_float(q.x), __uint_as_float(q.y), lo);
+                        split_pair(__uint_as_float(q.z), __uint_as_float(q.w), hi);
 #pragma unroll
                         for (int p = 0; p < 3; ++p)
                             *reinterpret_cast<uint2*>(row + (p % kPX) * 16 * kTilePitch + i * 4) = make_uint2(lo[p], hi[p]);
