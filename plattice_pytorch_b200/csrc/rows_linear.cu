@@ -18,7 +18,7 @@ __device__ __forceinline__ void store_parts(__nv_bfloat16* p, int64_t stride, co
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         uint32_t t[3];
-        split_pair(v[2 * i], v[2 * i + 1], t);
+        split_any(v[2 * i], v[2 * i + 1], t);
         o[0].w[i] = t[0];
         o[1].w[i] = t[1];
         o[2].w[i] = t[2];

@@ -104,16 +104,26 @@ __device__ __forceinline__ void codes_to_half(uint32_t codes, uint32_t& lo, uint
         : "r"(codes));
 }
 
-// Three float16 parts of a pair, rounded: 11 + 11 + 2 and more bits.
+// Float16 parts of a pair, rounded: 11 + 11 + 2 and more bits.  Of several, what
+// is not finite is the last and the first a 1 (see split_any).
+template <int kParts>
 __device__ __forceinline__ void half_parts(float a, float b, uint32_t (&o)[3]) {
+    union { __half2 h; uint32_t u; } x, last;
+    last.u = 0;
+    if (kParts > 1 && !(fabsf(a) + fabsf(b) < INFINITY)) {
+        const bool fa = fabsf(a) < INFINITY, fb = fabsf(b) < INFINITY;
+        last.h = __floats2half2_rn(fa ? 0.f : a, fb ? 0.f : b);
+        a = fa ? a : copysignf(1.f, a);
+        b = fb ? b : copysignf(1.f, b);
+    }
 #pragma unroll
-    for (int i = 0; i < 3; ++i) {
-        union { __half2 h; uint32_t u; } x;
+    for (int i = 0; i < kParts; ++i) {
         x.h = __floats2half2_rn(a, b);
         o[i] = x.u;
         a -= __low2float(x.h);
         b -= __high2float(x.h);
     }
+    o[kParts - 1] |= last.u;
 }
 
 template <int kXT, int kFragments = NarrowShape<kXT>::kM>
@@ -181,16 +191,22 @@ __device__ __forceinline__ void narrow_mask(NarrowRaw<kXT>& r, int k, int chunk,
             }
 }
 
-// The operand registers of step s (4 of the lane's 16 channels), part p of kPA.
-template <int kXT, int kPA>
+// The operand registers of step s (4 of the lane's 16 channels), part p of kPA;
+// kAny: float32 values may not be finite.
+template <int kXT, int kPA, bool kAny>
 __device__ __forceinline__ void narrow_operand(const NarrowRaw<kXT>& r, int m, int s, uint32_t (&o)[kPA][4]) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         if (kXT == kXFloat) {
             const uint4& q = r.v[m][h][s];
             uint32_t lo[3], hi[3];
-            split_pair(__uint_as_float(q.x), __uint_as_float(q.y), lo);
-            split_pair(__uint_as_float(q.z), __uint_as_float(q.w), hi);
+            if constexpr (kAny) {
+                split_any(__uint_as_float(q.x), __uint_as_float(q.y), lo);
+                split_any(__uint_as_float(q.z), __uint_as_float(q.w), hi);
+            } else {
+                split_pair(__uint_as_float(q.x), __uint_as_float(q.y), lo);
+                split_pair(__uint_as_float(q.z), __uint_as_float(q.w), hi);
+            }
 #pragma unroll
             for (int p = 0; p < kPA; ++p) {
                 o[p][h] = lo[p];
@@ -202,6 +218,37 @@ __device__ __forceinline__ void narrow_operand(const NarrowRaw<kXT>& r, int m, i
             o[0][2 + h] = s & 1 ? q.w : q.y;
         }
     }
+}
+
+// float32's products are made as if all values were finite.  Where one is not, or
+// one of their products is past float32's range, the products of small parts say
+// so: they are made again from split_any's parts.
+template <bool kValue> struct Fixed { static constexpr bool value = kValue; };
+
+template <int kM, int kN>
+__device__ __forceinline__ bool small_not_finite(const float (&low)[kM][kN][4]) {
+    uint64_t w = 0;
+#pragma unroll
+    for (int m = 0; m < kM; ++m)
+#pragma unroll
+        for (int f = 0; f < kN; ++f) {
+            watch(w, low[m][f][0], low[m][f][1]);
+            watch(w, low[m][f][2], low[m][f][3]);
+        }
+    return not_finite(w);
+}
+
+// A sum that is infinite without its small parts stays so (those of a product
+// far past the range may be infinite the other way).
+template <int kM, int kN>
+__device__ __forceinline__ void drop_beside_infinity(float (&low)[kM][kN][4], const float (&sum)[kM][kN][4]) {
+#pragma unroll
+    for (int m = 0; m < kM; ++m)
+#pragma unroll
+        for (int f = 0; f < kN; ++f)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (is_infinite(fabsf(sum[m][f][i]))) low[m][f][i] = 0.f;
 }
 
 // Copies a run of `count` staged values to elements at.. of a tensor, `add`'s
@@ -302,11 +349,11 @@ __global__ void __launch_bounds__(32 * kNarrowWarps, narrow_ctas(kXT, kNF)) k_na
             const float up = 1.f / column[col];   // a power of two
 #pragma unroll
             for (int j = 0; j < 4; ++j) v[j] *= up;
-            half_parts(v[0], v[1], lo);
-            half_parts(v[2], v[3], hi);
+            half_parts<kPB>(v[0], v[1], lo);
+            half_parts<kPB>(v[2], v[3], hi);
         } else if (kW3) {
-            split_pair(v[0], v[1], lo);
-            split_pair(v[2], v[3], hi);
+            split_any(v[0], v[1], lo);
+            split_any(v[2], v[3], hi);
         } else if (kXT == kXHalf) {
             union { __half2 h; uint32_t u; } x, y;
             x.h = __floats2half2_rn(v[0], v[1]);
@@ -411,33 +458,60 @@ __global__ void __launch_bounds__(32 * kNarrowWarps, narrow_ctas(kXT, kNF)) k_na
             // parts apart from it: the matrix instruction cuts where an addition
             // rounds, by which a long chain of them drifts
             float sum[kM][kNF][4], low[kM][kNF][4];
+            auto clear = [&] {
 #pragma unroll
-            for (int m = 0; m < kM; ++m)
+                for (int m = 0; m < kM; ++m)
 #pragma unroll
-                for (int f = 0; f < kNF; ++f)
+                    for (int f = 0; f < kNF; ++f)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) sum[m][f][i] = low[m][f][i] = 0.f;
+                        for (int i = 0; i < 4; ++i) sum[m][f][i] = low[m][f][i] = 0.f;
+            };
+            auto step = [&](int m, int s, const uint32_t (&o)[kPA][4]) {
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                uint2 b[kPB][kNF];
+                for (int size = 2; size >= 0; --size)   // small products first
 #pragma unroll
-                for (int p = 0; p < kPB; ++p)
+                    for (int pa = 0; pa < kPA; ++pa) {
+                        const int pb = size - pa;
+                        if (pb < 0 || pb >= kPB) continue;
 #pragma unroll
-                    for (int f = 0; f < kNF; ++f) b[p][f] = frag[((p * steps + c * 4 + s) * kNF + f) * 32 + lane];
+                        for (int f = 0; f < kNF; ++f)
+                            mma16816<kXT == kXHalf>(size ? low[m][f] : sum[m][f], o[pa][0], o[pa][1], o[pa][2], o[pa][3],
+                                                    frag[((pb * steps + c * 4 + s) * kNF + f) * 32 + lane]);
+                    }
+            };
+            clear();
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
 #pragma unroll
                 for (int m = 0; m < kM; ++m) {
                     uint32_t o[kPA][4];
-                    narrow_operand<kXT, kPA>(raw, m, s, o);
+                    narrow_operand<kXT, kPA, false>(raw, m, s, o);
+                    step(m, s, o);
+                }
+            if constexpr (kPA == 3) {
+                if (__any_sync(0xffffffffu, small_not_finite(low))) {   // rare: from memory again, 4 channels at a time
+                    clear();
+#pragma unroll 1
+                    for (int s = 0; s < 4; ++s) {
+                        uint32_t o[kPA][4];
 #pragma unroll
-                    for (int size = 2; size >= 0; --size)   // small products first
+                        for (int h = 0; h < 2; ++h) {
+                            const int64_t row = min(row0 + h * 8 + g, a.rows - 1);
+                            const int ch = c * 64 + t * 16 + s * 4;
+                            float v[8];
+                            load8(v, static_cast<const float*>(a.x) + row * a.k + ch, false, min(a.k - ch, 4));
+                            uint32_t lo[3], hi[3];
+                            split_any(v[0], v[1], lo);
+                            split_any(v[2], v[3], hi);
 #pragma unroll
-                        for (int pa = 0; pa < kPA; ++pa) {
-                            const int pb = size - pa;
-                            if (pb < 0 || pb >= kPB) continue;
-#pragma unroll
-                            for (int f = 0; f < kNF; ++f)
-                                mma16816<kXT == kXHalf>(size ? low[m][f] : sum[m][f], o[pa][0], o[pa][1], o[pa][2], o[pa][3], b[pb][f]);
+                            for (int p = 0; p < kPA; ++p) {
+                                o[p][h] = lo[p];
+                                o[p][2 + h] = hi[p];
+                            }
                         }
+                        step(0, s, o);
+                    }
+                    drop_beside_infinity(low, sum);
                 }
             }
 #pragma unroll
@@ -567,28 +641,24 @@ template <int kXT, int kParts> struct NarrowGradShape {
     static constexpr int kBytes = kFragBytes + kGradWarps * kWarpBytes + 64 * 33 * 4;
 };
 
-// a and b as kP packed parts: one rounded, two (rounded, and what that left),
-// or split_pair's three.
-template <int kP, bool kHalf>
+// a and b as kP packed parts: bfloat16, or float16, rounded.  kAny: they may not
+// be finite (two parts then meet an operand of one).
+template <int kP, bool kHalf, bool kAny>
 __device__ __forceinline__ void to_parts(float a, float b, uint32_t (&o)[kP]) {
-    if constexpr (kP == 3) {
+    if constexpr (!kHalf && kAny && kP == 2) {
+        split_one_sign(a, b, o);
+    } else if constexpr (!kHalf && kAny) {
+        split_any(a, b, o);
+    } else if constexpr (!kHalf) {
         split_pair(a, b, o);
     } else {
 #pragma unroll
         for (int i = 0; i < kP; ++i) {
-            if (kHalf) {
-                union { __half2 h; uint32_t u; } x;
-                x.h = __floats2half2_rn(a, b);
-                o[i] = x.u;
-                a -= __low2float(x.h);
-                b -= __high2float(x.h);
-            } else {
-                union { __nv_bfloat162 h; uint32_t u; } x;
-                x.h = __floats2bfloat162_rn(a, b);
-                o[i] = x.u;
-                a -= __low2float(x.h);
-                b -= __high2float(x.h);
-            }
+            union { __half2 h; uint32_t u; } x;
+            x.h = __floats2half2_rn(a, b);
+            o[i] = x.u;
+            a -= __low2float(x.h);
+            b -= __high2float(x.h);
         }
     }
 }
@@ -630,8 +700,8 @@ __global__ void __launch_bounds__(32 * kGradWarps, narrow_grad_ctas(kParts, kNF)
             for (int j = 0; j < 4; ++j)
                 v[j] = o + j < n && ch < k ? to_f32(weights[(int64_t)(o + j) * k + ch]) : 0.f;
             uint32_t lo[kParts], hi[kParts];
-            to_parts<kParts, kHalf>(v[0], v[1], lo);
-            to_parts<kParts, kHalf>(v[2], v[3], hi);
+            to_parts<kParts, kHalf, true>(v[0], v[1], lo);
+            to_parts<kParts, kHalf, true>(v[2], v[3], hi);
 #pragma unroll
             for (int p = 0; p < kParts; ++p) frag[p * kKS * 256 + i] = make_uint2(lo[p], hi[p]);
         }
@@ -723,16 +793,27 @@ __global__ void __launch_bounds__(32 * kGradWarps, narrow_grad_ctas(kParts, kNF)
                     reinterpret_cast<uint4*>(row)[0] = o.u[0];
                     reinterpret_cast<uint4*>(row)[1] = o.u[1];
                 } else if (kXT == kXFloat) {
+                    auto put = [&](auto any) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const uint4& q = xn.v[0][h][i % NarrowShape<kXT>::kRaw];
+                            uint32_t lo[3], hi[3];
+                            to_parts<3, false, decltype(any)::value>(__uint_as_float(q.x), __uint_as_float(q.y), lo);
+                            to_parts<3, false, decltype(any)::value>(__uint_as_float(q.z), __uint_as_float(q.w), hi);
+#pragma unroll
+                            for (int p = 0; p < 3; ++p)
+                                *reinterpret_cast<uint2*>(row + (p % kPX) * 16 * kTilePitch + i * 4) = make_uint2(lo[p], hi[p]);
+                        }
+                    };
+                    uint64_t w = 0;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const uint4& q = xn.v[0][h][i % NarrowShape<kXT>::kRaw];
-                        uint32_t lo[3], hi[3];
-                        split_pair(__uint_as_float(q.x), __uint_as_float(q.y), lo);
-                        split_pair(__uint_as_float(q.z), __uint_as_float(q.w), hi);
-#pragma unroll
-                        for (int p = 0; p < 3; ++p)
-                            *reinterpret_cast<uint2*>(row + (p % kPX) * 16 * kTilePitch + i * 4) = make_uint2(lo[p], hi[p]);
+                        watch(w, __uint_as_float(q.x), __uint_as_float(q.y));
+                        watch(w, __uint_as_float(q.z), __uint_as_float(q.w));
                     }
+                    if (!not_finite(w)) put(Fixed<false>());
+                    else put(Fixed<true>());
                 } else {
                     reinterpret_cast<uint4*>(row)[0] = xn.v[0][h][0];
                     reinterpret_cast<uint4*>(row)[1] = xn.v[0][h][1 % NarrowShape<kXT>::kRaw];
@@ -765,118 +846,124 @@ __global__ void __launch_bounds__(32 * kGradWarps, narrow_grad_ctas(kParts, kNF)
             }
             __syncwarp();
         }
-        if (a.need_b) {
+        // sums of the columns, for the bias's gradient and to see whether all is finite
+        float column = 0.f;
 #pragma unroll
-            for (int r = 0; r < 16; r += 8) {   // short chains: many rows drift less
-                float t[8];
+        for (int r = 0; r < 16; r += 8) {   // short chains: many rows drift less
+            float t[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) t[i] = st[(r + i) * kNarrowPitch + lane];
-                db += ((t[0] + t[1]) + (t[2] + t[3])) + ((t[4] + t[5]) + (t[6] + t[7]));
-            }
+            for (int i = 0; i < 8; ++i) t[i] = st[(r + i) * kNarrowPitch + lane];
+            const float part = ((t[0] + t[1]) + (t[2] + t[3])) + ((t[4] + t[5]) + (t[6] + t[7]));
+            column += part;
+            db += part;
         }
-        if (a.need_x) {
-            uint32_t o[kKS][kPZ][4];
+        auto products = [&](auto any) {
+            if (a.need_x) {
+                uint32_t o[kKS][kPZ][4];
 #pragma unroll
-            for (int s = 0; s < kKS; ++s)
+                for (int s = 0; s < kKS; ++s)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float* p = st + (g + 8 * h) * kNarrowPitch + t * cols_per_lane + s * 4;
-                    uint32_t lo[kPZ], hi[kPZ];
-                    to_parts<kPZ, kHalf>(p[0], p[1], lo);
-                    to_parts<kPZ, kHalf>(p[2], p[3], hi);
+                    for (int h = 0; h < 2; ++h) {
+                        const float* p = st + (g + 8 * h) * kNarrowPitch + t * cols_per_lane + s * 4;
+                        uint32_t lo[kPZ], hi[kPZ];
+                        to_parts<kPZ, kHalf, decltype(any)::value>(p[0], p[1], lo);
+                        to_parts<kPZ, kHalf, decltype(any)::value>(p[2], p[3], hi);
 #pragma unroll
-                    for (int q = 0; q < kPZ; ++q) {
-                        o[s][q][h] = lo[q];
-                        o[s][q][2 + h] = hi[q];
+                        for (int q = 0; q < kPZ; ++q) {
+                            o[s][q][h] = lo[q];
+                            o[s][q][2 + h] = hi[q];
+                        }
+                    }
+                float dx[8][4];
+#pragma unroll
+                for (int f = 0; f < 8; ++f) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) dx[f][i] = 0.f;
+#pragma unroll
+                    for (int sum = kPZ - 1; sum >= 0; --sum)   // small products first
+#pragma unroll
+                        for (int pa = 0; pa < kPZ; ++pa) {
+                            const int pb = sum - pa;
+                            if (pb < 0 || pb >= kParts) continue;
+#pragma unroll
+                            for (int s = 0; s < kKS; ++s)
+                                mma16816<kHalf>(dx[f], o[s][pa][0], o[s][pa][1], o[s][pa][2], o[s][pa][3],
+                                                frag[((pb * kKS + s) * 8 + f) * 32 + lane]);
+                        }
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {   // 16 neighbouring channels of rows g and g + 8
+                    if (g + 8 * h >= rows) continue;
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        const int ch = ch0 + t * 16 + q * 8, left = k - ch;
+                        if (left <= 0) continue;
+                        float v[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) v[i] = dx[q * 4 + (i >> 1)][h * 2 + (i & 1)];
+                        const int64_t at = (row0 + g + 8 * h) * k + ch;
+                        const bool vec = a.vec_gx && left >= 8;
+                        if (kXT == kXHalf) store8(static_cast<__half*>(a.grad_x) + at, v, vec, left);
+                        else if (kParts == 3) store8(static_cast<float*>(a.grad_x) + at, v, vec, left);
+                        else store8(static_cast<__nv_bfloat16*>(a.grad_x) + at, v, vec, left);
                     }
                 }
-            float dx[8][4];
+            }
+            if (a.need_w) {
+                uint32_t b[kPZ][kNF][2];
 #pragma unroll
-            for (int f = 0; f < 8; ++f) {
+                for (int f = 0; f < kNF; ++f)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) dx[f][i] = 0.f;
+                    for (int h = 0; h < 2; ++h) {
+                        const float* p = st + (2 * t + 8 * h) * kNarrowPitch + f * 8 + g;
+                        uint32_t o[kPZ];
+                        to_parts<kPZ, kHalf, decltype(any)::value>(p[0], p[kNarrowPitch], o);
 #pragma unroll
-                for (int sum = kPZ - 1; sum >= 0; --sum)   // small products first
-#pragma unroll
-                    for (int pa = 0; pa < kPZ; ++pa) {
-                        const int pb = sum - pa;
-                        if (pb < 0 || pb >= kParts) continue;
-#pragma unroll
-                        for (int s = 0; s < kKS; ++s)
-                            mma16816<kHalf>(dx[f], o[s][pa][0], o[s][pa][1], o[s][pa][2], o[s][pa][3],
-                                            frag[((pb * kKS + s) * 8 + f) * 32 + lane]);
+                        for (int q = 0; q < kPZ; ++q) b[q][f][h] = o[q];
                     }
-            }
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {   // 16 neighbouring channels of rows g and g + 8
-                if (g + 8 * h >= rows) continue;
+                for (int m = 0; m < 4; ++m) {
+                    uint32_t x[kPX][4];
 #pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    const int ch = ch0 + t * 16 + q * 8, left = k - ch;
-                    if (left <= 0) continue;
-                    float v[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] = dx[q * 4 + (i >> 1)][h * 2 + (i & 1)];
-                    const int64_t at = (row0 + g + 8 * h) * k + ch;
-                    const bool vec = a.vec_gx && left >= 8;
-                    if (kXT == kXHalf) store8(static_cast<__half*>(a.grad_x) + at, v, vec, left);
-                    else if (kParts == 3) store8(static_cast<float*>(a.grad_x) + at, v, vec, left);
-                    else store8(static_cast<__nv_bfloat16*>(a.grad_x) + at, v, vec, left);
-                }
-            }
-        }
-        if (a.need_w) {
-            uint32_t b[kPZ][kNF][2];
-#pragma unroll
-            for (int f = 0; f < kNF; ++f)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float* p = st + (2 * t + 8 * h) * kNarrowPitch + f * 8 + g;
-                    uint32_t o[kPZ];
-                    to_parts<kPZ, kHalf>(p[0], p[kNarrowPitch], o);
-#pragma unroll
-                    for (int q = 0; q < kPZ; ++q) b[q][f][h] = o[q];
-                }
-#pragma unroll
-            for (int m = 0; m < 4; ++m) {
-                uint32_t x[kPX][4];
-#pragma unroll
-                for (int q = 0; q < kPX; ++q) {
-                    const uint16_t* src = tile + q * 16 * kTilePitch + ((lane >> 4) * 8 + (lane & 7)) * kTilePitch +
-                                          m * 16 + ((lane >> 3) & 1) * 8;
-                    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-                                 : "=r"(x[q][0]), "=r"(x[q][1]), "=r"(x[q][2]), "=r"(x[q][3])
-                                 : "r"((uint32_t)__cvta_generic_to_shared(src))
-                                 : "memory");
-                }
-                // float32: the sum of these rows by itself (see k_narrow)
-                float rows16[kNF][4];
-                if (kParts == 3) {
-#pragma unroll
-                    for (int f = 0; f < kNF; ++f)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) rows16[f][i] = 0.f;
-                }
-#pragma unroll
-                for (int sum = kPZ - 1; sum >= 0; --sum)
-#pragma unroll
-                    for (int px = 0; px < kPX; ++px) {
-                        const int pb = sum - px;
-                        if (pb < 0 || pb >= kPZ) continue;
+                    for (int q = 0; q < kPX; ++q) {
+                        const uint16_t* src = tile + q * 16 * kTilePitch + ((lane >> 4) * 8 + (lane & 7)) * kTilePitch +
+                                              m * 16 + ((lane >> 3) & 1) * 8;
+                        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                                     : "=r"(x[q][0]), "=r"(x[q][1]), "=r"(x[q][2]), "=r"(x[q][3])
+                                     : "r"((uint32_t)__cvta_generic_to_shared(src))
+                                     : "memory");
+                    }
+                    // float32: the sum of these rows by itself (see k_narrow)
+                    float rows16[kNF][4];
+                    if (kParts == 3) {
 #pragma unroll
                         for (int f = 0; f < kNF; ++f)
-                            mma16816<kHalf>(kParts == 3 ? rows16[f] : dw[m][f], x[px][0], x[px][1], x[px][2], x[px][3],
-                                            make_uint2(b[pb][f][0], b[pb][f][1]));
-                    }
-                if (kParts == 3) {
 #pragma unroll
-                    for (int f = 0; f < kNF; ++f) {
-                        add2(dw[m][f][0], dw[m][f][1], rows16[f][0], rows16[f][1]);
-                        add2(dw[m][f][2], dw[m][f][3], rows16[f][2], rows16[f][3]);
+                            for (int i = 0; i < 4; ++i) rows16[f][i] = 0.f;
+                    }
+#pragma unroll
+                    for (int sum = kPZ - 1; sum >= 0; --sum)
+#pragma unroll
+                        for (int px = 0; px < kPX; ++px) {
+                            const int pb = sum - px;
+                            if (pb < 0 || pb >= kPZ) continue;
+#pragma unroll
+                            for (int f = 0; f < kNF; ++f)
+                                mma16816<kHalf>(kParts == 3 ? rows16[f] : dw[m][f], x[px][0], x[px][1], x[px][2], x[px][3],
+                                                make_uint2(b[pb][f][0], b[pb][f][1]));
+                        }
+                    if (kParts == 3) {
+#pragma unroll
+                        for (int f = 0; f < kNF; ++f) {
+                            add2(dw[m][f][0], dw[m][f][1], rows16[f][0], rows16[f][1]);
+                            add2(dw[m][f][2], dw[m][f][3], rows16[f][2], rows16[f][3]);
+                        }
                     }
                 }
             }
-        }
+        };
+        if (!__any_sync(0xffffffffu, !(fabsf(column) < INFINITY))) products(Fixed<false>());
+        else products(Fixed<true>());
     }
 
     // the CTA's sums, warp after warp
@@ -951,46 +1038,60 @@ __global__ void __launch_bounds__(64 * few_splits(kWT)) k_few(const SmallArgs a)
             narrow_load<kXT, 1>(xr, a, row0, c, lane);
             narrow_mask<kWT, 1>(wr, a.k, c, lane);
             narrow_mask<kXT, 1>(xr, a.k, c, lane);
-            float sum[kN][4], low[kN][4];   // low: float32's products of small parts (see k_narrow)
+            float sum[1][kN][4], low[1][kN][4];   // low: float32's products of small parts (see k_narrow)
+            auto products = [&](const NarrowRaw<kWT>& wr, const NarrowRaw<kXT>& xr, auto any) {
 #pragma unroll
-            for (int j = 0; j < kN; ++j)
+                for (int j = 0; j < kN; ++j)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) sum[j][i] = low[j][i] = 0.f;
+                    for (int i = 0; i < 4; ++i) sum[0][j][i] = low[0][j][i] = 0.f;
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                uint32_t o[kPW][4], b[kPX][4];
-                narrow_operand<kWT, kPW>(wr, 0, s, o);
-                if constexpr (kX8In) {
+                for (int s = 0; s < 4; ++s) {
+                    uint32_t o[kPW][4], b[kPX][4];
+                    narrow_operand<kWT, kPW, decltype(any)::value>(wr, 0, s, o);
+                    if constexpr (kX8In) {
 #pragma unroll
-                    for (int h = 0; h < kN; ++h) {
-                        const uint4& q = xr.v[0][h][0];
-                        float v[4];   // exact in bfloat16
-                        values4(v, s == 0 ? q.x : s == 1 ? q.y : s == 2 ? q.z : q.w, scale_of(xr.scale[0][h]));
-                        union { __nv_bfloat162 p; uint32_t u; } x, y;
-                        x.p = __floats2bfloat162_rn(v[0], v[1]);
-                        y.p = __floats2bfloat162_rn(v[2], v[3]);
-                        b[0][h] = x.u;
-                        b[0][2 + h] = y.u;
+                        for (int h = 0; h < kN; ++h) {
+                            const uint4& q = xr.v[0][h][0];
+                            float v[4];   // exact in bfloat16
+                            values4(v, s == 0 ? q.x : s == 1 ? q.y : s == 2 ? q.z : q.w, scale_of(xr.scale[0][h]));
+                            union { __nv_bfloat162 p; uint32_t u; } x, y;
+                            x.p = __floats2bfloat162_rn(v[0], v[1]);
+                            y.p = __floats2bfloat162_rn(v[2], v[3]);
+                            b[0][h] = x.u;
+                            b[0][2 + h] = y.u;
+                        }
+                    } else {
+                        narrow_operand<kXT, kPX, decltype(any)::value>(xr, 0, s, b);
                     }
-                } else {
-                    narrow_operand<kXT, kPX>(xr, 0, s, b);
+#pragma unroll
+                    for (int size = 2; size >= 0; --size)   // small products first
+#pragma unroll
+                        for (int pw = 0; pw < kPW; ++pw) {
+                            const int px = size - pw;
+                            if (px < 0 || px >= kPX) continue;
+#pragma unroll
+                            for (int j = 0; j < kN; ++j)
+                                mma16816<kWT == kXHalf>(size ? low[0][j] : sum[0][j], o[pw][0], o[pw][1], o[pw][2], o[pw][3],
+                                                        make_uint2(b[px][j], b[px][2 + j]));
+                        }
+                }
+            };
+            products(wr, xr, Fixed<false>());
+            if constexpr (kPW == 3)
+                if (__any_sync(0xffffffffu, small_not_finite(low))) {   // rare
+                    NarrowRaw<kWT> w2;
+                    NarrowRaw<kXT> x2;
+                    narrow_load<kWT, 1>(w2, w, col0, c, lane);
+                    narrow_load<kXT, 1>(x2, a, row0, c, lane);
+                    narrow_mask<kWT, 1>(w2, a.k, c, lane);
+                    narrow_mask<kXT, 1>(x2, a.k, c, lane);
+                    products(w2, x2, Fixed<true>());
+                    drop_beside_infinity(low, sum);
                 }
 #pragma unroll
-                for (int size = 2; size >= 0; --size)   // small products first
-#pragma unroll
-                    for (int pw = 0; pw < kPW; ++pw) {
-                        const int px = size - pw;
-                        if (px < 0 || px >= kPX) continue;
-#pragma unroll
-                        for (int j = 0; j < kN; ++j)
-                            mma16816<kWT == kXHalf>(size ? low[j] : sum[j], o[pw][0], o[pw][1], o[pw][2], o[pw][3],
-                                                    make_uint2(b[px][j], b[px][2 + j]));
-                    }
-            }
-#pragma unroll
             for (int j = 0; j < kN; ++j)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[j][i] += kPW == 3 ? sum[j][i] + low[j][i] : sum[j][i];
+                for (int i = 0; i < 4; ++i) acc[j][i] += kPW == 3 ? sum[0][j][i] + low[0][j][i] : sum[0][j][i];
         }
     }
 #pragma unroll

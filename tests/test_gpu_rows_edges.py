@@ -2,11 +2,13 @@
 that are not finite or nearly infinite, float32's last bits, mixed types,
 largest sizes.  Definitions in float64 as in rows_reference.py; u = 2^-24 is
 half a float32 step."""
+import math
+
 import numpy as np
 import pytest
 import torch
 
-from rows_reference import U, f64
+from rows_reference import U, f64, half_step
 
 pytestmark = pytest.mark.gpu
 
@@ -54,6 +56,75 @@ def test_float32_products_are_float32(dev, R, rows, n):
         gy[0, n - 1] = float(a)
         gx, gw, _ = R.linear_backward(gy, x, w)
         assert abs(f64(gx)[0, 0] / e - 1) <= 4 * U and abs(f64(gw)[n - 1, 0] / float(a) ** 2 - 1) <= 4 * U
+
+
+# ---------------------------------------------------------------- not finite
+
+def _same(got, want, tol):
+    """The same infinities and NaN; finite values within tol."""
+    got = f64(got)
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    inf = np.isinf(want)
+    assert np.array_equal(np.isinf(got), inf) and np.array_equal(got[inf], want[inf])
+    fine = np.isfinite(want)
+    assert (np.abs(got - want)[fine] <= tol[fine]).all()
+
+
+def _weighted(x, w):
+    with np.errstate(invalid="ignore"):
+        return (x[:, None, :] * w[None, :, :]).sum(-1)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,n", FORMS)
+@pytest.mark.parametrize("k", [50, 64, 700])
+def test_infinite_inputs_give_infinite_sums(dev, R, rows, n, k, dtype):
+    t = DTYPES[dtype]
+    x, w = _randn((rows, k), 16, t), _randn((n, k), 17, t)
+    x[0, 3], x[rows - 1, k - 1] = math.inf, -math.inf
+    x[rows // 2, 7], x[rows // 2, 8] = math.inf, math.nan
+    w[1, 5], w[n - 1, 3] = -math.inf, math.inf
+    x[1, 5] = 0.0   # times the infinite weight: NaN
+    y, _ = R.linear(x.to(dev), w.to(dev))
+    some = [0, 1, 2, rows // 2, rows - 1]
+    e = _weighted(f64(x[some]), f64(w))
+    tol = (2 * U * (k + 8) + half_step(t)) * _weighted(np.abs(np.where(np.isfinite(f64(x[some])), f64(x[some]), 0)),
+                                                       np.abs(np.where(np.isfinite(f64(w)), f64(w), 0))) + 1e-6
+    _same(y[some], e, tol)
+
+
+@pytest.mark.parametrize("rows,n", FORMS)
+def test_infinite_weights_of_8_bit_rows(dev, R, rows, n):
+    k = 96
+    for t in (torch.float32, torch.bfloat16):
+        x, w = R.pack8(_randn((rows, k), 18).abs().add(0.5).to(dev)), _randn((n, k), 19, t)
+        w[0, 5], w[n - 1, 95] = math.inf, -math.inf
+        y, _ = R.linear(x, w.to(dev), out_dtype=torch.float32)
+        xe = f64(R.unpack8(x))[:3]
+        e = _weighted(xe, f64(w))
+        _same(y[:3], e, 2 * U * (k + 8) * _weighted(np.abs(xe), np.abs(np.where(np.isfinite(f64(w)), f64(w), 0))) + 1e-6)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("out32", [False, True])
+@pytest.mark.parametrize("rows,k,n", [(37, 64, 24), (375, 50, 8), (500, 72, 40), (503, 33, 91)])
+def test_infinite_gradients_and_inputs(dev, R, rows, k, n, dtype, out32):
+    """An infinite gradient and an infinite input, in the sums they belong to and
+    in no other."""
+    t = DTYPES[dtype]
+    out = torch.float32 if out32 else t
+    x, w, gy = _randn((rows, k), 20, t), _randn((n, k), 21, t), _randn((rows, n), 22, out)
+    x[5, 2] = math.inf
+    gy[3, 1] = -math.inf
+    got = R.linear_backward(gy.to(dev), x.to(dev), w.to(dev), bias_dtype=torch.float32)
+    ge, xe, we = f64(gy), f64(x), f64(w)
+    fin = lambda a: np.abs(np.where(np.isfinite(a), a, 0))  # noqa: E731
+    with np.errstate(invalid="ignore"):
+        gx = np.stack([(ge * we[:, j][None]).sum(1) for j in range(k)], 1)
+        gw = np.stack([(ge * xe[:, j][:, None]).sum(0) for j in range(k)], 1)
+    _same(got[0], gx, (2 * U * (n + 8) + 2.0 ** -16 + half_step(t)) * (fin(ge) @ fin(we)) + 1e-6)
+    _same(got[1], gw, (2 * U * (rows + 8) + 2.0 ** -16 + half_step(t)) * (fin(ge).T @ fin(xe)) + 1e-6)
+    _same(got[2], ge.sum(0), 2 * U * (rows + 8) * fin(ge).sum(0))
 
 
 # ------------------------------------------------------- arguments and sizes
