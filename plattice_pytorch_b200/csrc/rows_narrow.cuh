@@ -148,7 +148,8 @@ __device__ __forceinline__ void narrow_load(NarrowRaw<kXT>& r, const SmallArgs& 
 #pragma unroll
                 for (int i = 0; i < NarrowShape<kXT>::kRaw; ++i) {
                     const int c = ch + i * kPer;
-                    r.v[m][h][i] = *reinterpret_cast<const uint4*>(p + (int64_t)(c < a.k ? c : 0) * kSize);
+                    // below 2^32: at most 2^30 channels
+                    r.v[m][h][i] = *reinterpret_cast<const uint4*>(p + (uint32_t)(c < a.k ? c : 0) * (uint32_t)kSize);
                 }
             } else {
 #pragma unroll
