@@ -642,12 +642,12 @@ template <int kXT, int kParts> struct NarrowGradShape {
     static constexpr int kBytes = kFragBytes + kGradWarps * kWarpBytes + 64 * 33 * 4;
 };
 
-// a and b as kP packed parts: bfloat16, or float16, rounded.  kAny: they may not
-// be finite (two parts then meet an operand of one).
+// a and b as kP packed parts: bfloat16 (two beside operands of one), or float16,
+// rounded.  kAny: they may not be finite.
 template <int kP, bool kHalf, bool kAny>
 __device__ __forceinline__ void to_parts(float a, float b, uint32_t (&o)[kP]) {
-    if constexpr (!kHalf && kAny && kP == 2) {
-        split_one_sign(a, b, o);
+    if constexpr (!kHalf && kP == 2) {
+        split_one_sign<kAny>(a, b, o);
     } else if constexpr (!kHalf && kAny) {
         split_any(a, b, o);
     } else if constexpr (!kHalf) {
@@ -780,6 +780,9 @@ __global__ void __launch_bounds__(32 * kGradWarps, narrow_grad_ctas(kParts, kNF)
             narrow_mask<kXT, 1>(xn, k, blockIdx.y, lane);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
+                if (rows < 16 && g + 8 * h >= rows)   // what was read is the last row again: times 0, were it finite
+#pragma unroll
+                    for (int i = 0; i < NarrowShape<kXT>::kRaw; ++i) xn.v[0][h][i] = make_uint4(0, 0, 0, 0);
                 uint16_t* row = tile + (g + 8 * h) * kTilePitch + t * 16;
                 if (kXT == kX8) {
                     float v[16];

@@ -54,15 +54,16 @@ __device__ __forceinline__ void split_any(float a, float b, uint32_t (&o)[kParts
     o[kParts - 1] |= last;   // 0 so far
 }
 
-// Two parts of any values for products with an operand of a single part, which
-// may itself be infinite: both parts have the value's sign and neither is 0
-// where the value is not (2^-30 of it is added), so that infinity times them is
-// not NaN.  The first is cut, the second rounded: off by at most 2^-16.
+// Two parts for products with an operand of a single part, which may itself be
+// infinite: both parts have the value's sign and neither is 0 where the value is
+// not (2^-20 of it goes to the second), so that infinity times them is not NaN.
+// The first is cut, the second rounded: off by at most 2^-16 + 2^-20.
+template <bool kAny>
 __device__ __forceinline__ void split_one_sign(float a, float b, uint32_t (&o)[2]) {
-    const uint32_t last = take_not_finite(a, b);
+    const uint32_t first = kAny ? take_not_finite(a, b) : 0;
     const uint32_t ua = __float_as_uint(a) & 0xffff0000u, ub = __float_as_uint(b) & 0xffff0000u;
-    o[0] = ua >> 16 | ub | last;   // a 1's bits are among an infinity's
-    const float ra = fmaf(a, 9.3132257e-10f, a - __uint_as_float(ua)), rb = fmaf(b, 9.3132257e-10f, b - __uint_as_float(ub));
+    o[0] = ua >> 16 | ub | first;   // a 1's bits are among an infinity's
+    const float ra = fmaf(a, 1.f + 9.5367432e-7f, -__uint_as_float(ua)), rb = fmaf(b, 1.f + 9.5367432e-7f, -__uint_as_float(ub));
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(o[1]) : "f"(rb), "f"(ra));
 }
 

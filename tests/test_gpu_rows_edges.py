@@ -106,6 +106,18 @@ def test_infinite_weights_of_8_bit_rows(dev, R, rows, n):
 
 
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("rows,k,n", [(37, 64, 24), (1, 40, 3), (375, 50, 8), (503, 33, 91)])
+def test_infinite_input_in_the_last_row(dev, R, rows, k, n, dtype):
+    """Where the last block of rows is not whole, the last row counts once."""
+    t = DTYPES[dtype]
+    x, w, gy = _randn((rows, k), 20, t), _randn((n, k), 21, t), _randn((rows, n), 22, t)
+    x[rows - 1, 2] = math.inf
+    _, gw, _ = R.linear_backward(gy.to(dev), x.to(dev), w.to(dev))
+    e = f64(gy).T @ f64(x)
+    _same(gw, e, (2 * U * (rows + 8) + half_step(t)) * (np.abs(f64(gy)).T @ np.abs(np.where(np.isfinite(f64(x)), f64(x), 0))) + 1e-6)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 @pytest.mark.parametrize("out32", [False, True])
 @pytest.mark.parametrize("rows,k,n", [(37, 64, 24), (375, 50, 8), (500, 72, 40), (503, 33, 91)])
 def test_infinite_gradients_and_inputs(dev, R, rows, k, n, dtype, out32):
