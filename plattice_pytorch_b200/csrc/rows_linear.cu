@@ -3,6 +3,8 @@
 #include <limits.h>
 #include <string.h>
 
+#include <type_traits>
+
 #include "plattice_runtime.h"
 #include "rows_common.cuh"
 #include "rows_host.h"
@@ -13,18 +15,21 @@ namespace plr {
 
 // ----------------------------------------------------- operands for the MMAs
 
+// How a value is stored: N bfloat16 parts, one tensor of them after the other.
+template <int N> struct Parts { static constexpr int kParts = N; };
+
+template <int N>
 __device__ __forceinline__ void store_parts(__nv_bfloat16* p, int64_t stride, const float (&v)[8], bool vec, int n) {
-    union { uint4 u; uint32_t w[4]; __nv_bfloat16 h[8]; } o[3];
+    union { uint4 u; uint32_t w[4]; __nv_bfloat16 h[8]; } o[N];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        uint32_t t[3];
+        uint32_t t[N];
         split_any(v[2 * i], v[2 * i + 1], t);
-        o[0].w[i] = t[0];
-        o[1].w[i] = t[1];
-        o[2].w[i] = t[2];
+#pragma unroll
+        for (int j = 0; j < N; ++j) o[j].w[i] = t[j];
     }
 #pragma unroll
-    for (int j = 0; j < 3; ++j) {
+    for (int j = 0; j < N; ++j) {
         if (vec) *reinterpret_cast<uint4*>(p + j * stride) = o[j].u;
         else
 #pragma unroll
@@ -33,10 +38,17 @@ __device__ __forceinline__ void store_parts(__nv_bfloat16* p, int64_t stride, co
     }
 }
 
-// Rows of c elements copied to rows of `pitch` (a multiple of 8): what TMA
-// needs when the rows do not lie on 16-byte boundaries; float32 becomes its
-// three parts.  Costs one read and one (float32: 1.5) write of the operand.
+// 8 values as a T (a type, or Parts) from element `at` of a tensor of `size`.
 template <typename T>
+__device__ __forceinline__ void store8_as(void* p, int64_t at, int64_t size, const float (&v)[8], bool vec, int n) {
+    if constexpr (std::is_empty_v<T>) store_parts<T::kParts>(static_cast<__nv_bfloat16*>(p) + at, size, v, vec, n);
+    else store8(static_cast<T*>(p) + at, v, vec, n);
+}
+
+// Rows of c elements copied to rows of `pitch` (a multiple of 8) as TO: what TMA
+// needs when the rows do not lie on 16-byte boundaries, and values as parts.
+// Costs one read and one (float32: 1.5, float16 as parts: 2) write of the operand.
+template <typename T, typename TO>
 __global__ void __launch_bounds__(256) k_repack(void* __restrict__ out, const T* __restrict__ x, int64_t rows, int c,
                                                 unsigned groups, bool vec) {
     const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -45,8 +57,7 @@ __global__ void __launch_bounds__(256) k_repack(void* __restrict__ out, const T*
     const int col = (int)(t - row * groups) * 8, left = c - col;
     float v[8];
     load8(v, x + row * c + col, vec && left >= 8, left);
-    if (sizeof(T) == 4) store_parts(static_cast<__nv_bfloat16*>(out) + t * 8, rows * groups * 8, v, true, 8);
-    else store8(static_cast<T*>(out) + t * 8, v, true, 8);
+    store8_as<TO>(out, t * 8, rows * groups * 8, v, true, 8);
 }
 
 // ------------------------------------------------- backward: gz and its sums
@@ -56,12 +67,13 @@ struct GradArgs {
     const void* g1;
     const void* z;
     const uint8_t* z_scale;
-    void* gz;           // [rows][pitch] in the operands' type, float32 as three bfloat16 parts; null: not stored
+    void* gz;           // [rows][pitch] in the operands' type or as bfloat16 parts; null: not stored
     int64_t pitch;
     float* partial;     // [gridDim.y][n]; null: no bias gradient
     int64_t rows;
     int n, split, act;
     int shift;          // log2 of the threads that share a row
+    bool halved;        // gz is stored times 1/2 (float16)
     bool vec;           // rows of grad_y and z allow 16-byte accesses
 };
 
@@ -73,12 +85,22 @@ __device__ __forceinline__ void times_slope(float (&g)[8], float (&z)[8]) {
     for (int i = 0; i < 8; i += 2) mul2(g[i], g[i + 1], z[i], z[i + 1]);
 }
 
+template <typename T> __device__ __forceinline__ void halve(float (&g)[8], bool halved) {
+    if constexpr (std::is_same_v<T, __half>) {
+        const float f = halved ? 0.5f : 1.f;
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) mul2(g[i], g[i + 1], f, f);
+    }
+}
+
 constexpr int kTogether = 2;
 
-// gz = grad_y act'(z), rounded to the operands' type for the two products (a
-// tensor core takes no wider operand; one rounding, as a stored gradient has),
-// and the sums of the unrounded gz over a CTA's rows.  2^shift threads of 8
-// columns share a row; gridDim.x strips of columns, gridDim.y parts of rows.
+// gz = grad_y act'(z) as the two products take it, and the sums of the unrounded
+// gz over a CTA's rows.  bfloat16 operands take it rounded to one part (a tensor
+// core takes no wider operand; one rounding, as a stored gradient has), float32
+// ones as three parts; float16 ones as two bfloat16 parts (gz_parts) or rounded, too
+// (gz_halved).  2^shift threads of 8 columns share a row; gridDim.x strips of
+// columns, gridDim.y parts of rows.
 template <typename TG, typename T, bool kFast>
 __global__ void __launch_bounds__(256, 4) k_grad_z(const GradArgs a) {
     __shared__ float sums[8 * 256];
@@ -94,11 +116,9 @@ __global__ void __launch_bounds__(256, 4) k_grad_z(const GradArgs a) {
 #pragma unroll
         for (int i = 0; i < 8; i += 2) add2(acc[i], acc[i + 1], g[i], g[i + 1]);
         if (!a.gz) return;
+        halve<T>(g, a.halved);
         const int64_t at = row * a.pitch + col;   // zeros up to the pitch
-        if constexpr (sizeof(T) == 4)
-            store_parts(static_cast<__nv_bfloat16*>(a.gz) + at, a.rows * a.pitch, g, kFast || wide == 8, wide);
-        else
-            store8(static_cast<T*>(a.gz) + at, g, kFast || (a.pitch % 8 == 0 && wide == 8), wide);
+        store8_as<T>(a.gz, at, a.rows * a.pitch, g, kFast || (a.pitch % 8 == 0 && wide == 8), wide);
     };
     const int64_t stride = (int64_t)gridDim.y * rows;
     int64_t row = (int64_t)blockIdx.y * rows + (threadIdx.x >> a.shift);
@@ -231,9 +251,9 @@ __global__ void __launch_bounds__(256, 4) k_grad_z_table(const GradArgs a) {
                     add2(acc[i], acc[i + 1], v[i], v[i + 1]);
                 }
                 if (!a.gz) continue;
+                halve<T>(v, a.halved);
                 const int64_t at = (row + u * stride) * a.pitch + col;
-                if constexpr (sizeof(T) == 4) store_parts(static_cast<__nv_bfloat16*>(a.gz) + at, a.rows * a.pitch, v, true, 8);
-                else store8(static_cast<T*>(a.gz) + at, v, true, 8);
+                store8_as<T>(a.gz, at, a.rows * a.pitch, v, true, 8);
             }
         }
     }
@@ -341,29 +361,50 @@ static bool tma_ready(const void* p, int dtype, int64_t width) {
     return dtype != PLATTICE_F32 && width % 8 == 0 && aligned16(p);
 }
 
-static int64_t repack_bytes(int dtype, int64_t rows, int64_t width) {
-    return rows * up8(width) * 2 * (dtype == PLATTICE_F32 ? 3 : 1);
+// Parts that the tiled backward's gz is made of: float32's three; of float16
+// operands beside float32 gradients, which can be far smaller and far larger than
+// float16 holds, two bfloat16 (the operands have two then, too); else one.
+static int gz_parts(const plattice_linear_args* a) {
+    if (a->dtype == PLATTICE_F32) return 3;
+    return a->dtype == PLATTICE_F16 && a->out_dtype == PLATTICE_F32 ? 2 : 1;
+}
+
+// A float16 gradient times a slope (of up to 1.13) can be past float16's largest:
+// the tiled backward's gz is stored halved, and its products are doubled.
+static bool gz_halved(const plattice_linear_args* a) {
+    return a->dtype == PLATTICE_F16 && a->act != PLATTICE_ACT_NONE && gz_parts(a) == 1;
+}
+
+// Parts of w, and of an x that is not in 8 bits: in the forward, in the tiled
+// backward, and in the one of a single pass (NarrowGradShape).
+static int forward_parts(const plattice_linear_args* a) { return a->dtype == PLATTICE_F32 ? 3 : 1; }
+static int tiled_parts(const plattice_linear_args* a) { return a->dtype == PLATTICE_BF16 ? 1 : gz_parts(a); }
+static int pass_parts(const plattice_linear_args* a) {
+    return a->dtype == PLATTICE_F16 && a->act != PLATTICE_ACT_NONE ? 2 : tiled_parts(a);
+}
+
+static int64_t repack_bytes(int parts, int64_t rows, int64_t width) { return rows * up8(width) * 2 * parts; }
+
+template <typename T, typename TO>
+static void repack(void* ws, const void* p, int64_t rows, int64_t width, cudaStream_t s) {
+    const unsigned groups = (unsigned)(up8(width) / 8);
+    k_repack<T, TO><<<(unsigned)ceil_div(rows * groups, 256), 256, 0, s>>>(ws, static_cast<const T*>(p), rows, (int)width,
+                                                                         groups, width % 8 == 0 && aligned16(p));
 }
 
 // The operand where it is, or repacked into `ws`.
-static cudaError_t operand(Operand* o, const void* p, int dtype, int64_t rows, int64_t width, void* ws,
+static cudaError_t operand(Operand* o, const void* p, int dtype, int parts, int64_t rows, int64_t width, void* ws,
                            cudaStream_t s) {
     *o = Operand{p, rows, width, width, 1};
-    if (tma_ready(p, dtype, width)) return cudaSuccess;
+    if (parts == 1 && tma_ready(p, dtype, width)) return cudaSuccess;
     o->p = ws;
     o->pitch = up8(width);
-    o->parts = dtype == PLATTICE_F32 ? 3 : 1;
-    const unsigned groups = (unsigned)(o->pitch / 8);
-    const int64_t ctas = ceil_div(rows * groups, 256);
-    if (ctas > INT_MAX) return cudaErrorInvalidValue;
-    const bool vec = width % 8 == 0 && aligned16(p);
-    if (dtype == PLATTICE_F32)
-        k_repack<float><<<(unsigned)ctas, 256, 0, s>>>(ws, static_cast<const float*>(p), rows, (int)width, groups, vec);
-    else if (dtype == PLATTICE_BF16)
-        k_repack<__nv_bfloat16><<<(unsigned)ctas, 256, 0, s>>>(ws, static_cast<const __nv_bfloat16*>(p), rows, (int)width,
-                                                              groups, vec);
-    else
-        k_repack<__half><<<(unsigned)ctas, 256, 0, s>>>(ws, static_cast<const __half*>(p), rows, (int)width, groups, vec);
+    o->parts = parts;
+    if (ceil_div(rows * (o->pitch / 8), 256) > INT_MAX) return cudaErrorInvalidValue;
+    if (dtype == PLATTICE_F32) repack<float, Parts<3>>(ws, p, rows, width, s);
+    else if (dtype == PLATTICE_BF16) repack<__nv_bfloat16, __nv_bfloat16>(ws, p, rows, width, s);
+    else if (parts == 2) repack<__half, Parts<2>>(ws, p, rows, width, s);
+    else repack<__half, __half>(ws, p, rows, width, s);
     return cudaGetLastError();
 }
 
@@ -431,16 +472,29 @@ static int choose_parts(int64_t ni, int64_t nj, int bn, int64_t steps) {
     return best;
 }
 
+// The products of parts that make up one of values, small ones first: those down
+// to 2^-16 of the largest of float32's three parts, to 2^-9 of float16's two (the
+// other is within 2^-18, and the result has 11 bits).
+template <typename F> static void for_products(int parts_a, int parts_b, F f) {
+    static const unsigned char all[6][2] = {{0, 2}, {1, 1}, {2, 0}, {0, 1}, {1, 0}, {0, 0}};
+    for (const auto& c : all)
+        if (c[0] < parts_a && c[1] < parts_b && !(parts_a == 2 && parts_b == 2 && c[0] + c[1] == 2)) f(c[0], c[1]);
+}
+static int product_count(int parts_a, int parts_b) {
+    int n = 0;
+    for_products(parts_a, parts_b, [&](int, int) { ++n; });
+    return n;
+}
+
 // Columns of a tile of kGradW: as wide as the result and the mode allow, but
 // where the sum is short (at most 16 slices, products of parts counted) the
 // narrowest whose tiles run in one round, since emptying an accumulator is then
 // most of the time (bfloat16, 64 / 256 wide: 100 rows, 1024 x 1024 4.4 / 6.4 us;
 // 1000 rows, 256 x 256 4.9 / 6.4; 5000 rows, 512 x 512 9.5 / 8.8).
 static int choose_bn_w(const plattice_linear_args* a) {
-    const bool f32 = a->dtype == PLATTICE_F32;
-    const bool deep = f32 && a->rows > 8 * kBK;   // chunks, or parts no deeper than one
+    const bool deep = a->dtype == PLATTICE_F32 && a->rows > 8 * kBK;   // chunks, or parts no deeper than one
     const int widest = a->n > 128 && !deep ? 256 : a->n > 64 ? 128 : 64;
-    if (ceil_div(a->rows, kBK) * (!f32 ? 1 : a->x_scale ? 3 : 6) > 16) return widest;
+    if (ceil_div(a->rows, kBK) * product_count(a->x_scale ? 1 : tiled_parts(a), gz_parts(a)) > 16) return widest;
     int bn = 64;
     while (bn < widest && mma_tiles(a->k, a->n, bn) > sm_count()) bn *= 2;
     return bn;
@@ -451,15 +505,13 @@ static void sum_args(MmaArgs* p, int64_t nr, int parts, int parts_a, int parts_b
     p->steps = (int)ceil_div(nr, kBK);
     p->part_steps = (int)ceil_div(p->steps, parts);
     p->parts = (int)ceil_div(p->steps, p->part_steps);   // none is empty
-    static const unsigned char pairs33[6][2] = {{0, 2}, {1, 1}, {2, 0}, {0, 1}, {1, 0}, {0, 0}};
     p->pairs = 0;
     p->pairs_a = p->pairs_b = 0;
-    for (const auto& c : pairs33) {
-        if (c[0] >= parts_a || c[1] >= parts_b) continue;
-        p->pairs_a |= (unsigned)c[0] << (2 * p->pairs);
-        p->pairs_b |= (unsigned)c[1] << (2 * p->pairs);
+    for_products(parts_a, parts_b, [&](int i, int j) {
+        p->pairs_a |= (unsigned)i << (2 * p->pairs);
+        p->pairs_b |= (unsigned)j << (2 * p->pairs);
         ++p->pairs;
-    }
+    });
 }
 
 // The 8-bit x as a bfloat16 operand in `ws`.
@@ -511,8 +563,8 @@ static ForwardPlan forward_plan(const plattice_linear_args* a) {
     if (p.way == kWayTiles) {
         p.bn = choose_bn(a->rows, a->n, 32, chunked((int)ceil_div(a->k, kBK), a->out_dtype, true));
         if (a->x_scale) p.x = c.take(a->rows * up8(a->k) * 2);
-        else if (!tma_ready(a->x, a->dtype, a->k)) p.x = c.take(repack_bytes(a->dtype, a->rows, a->k));
-        p.w = tma_ready(a->w, a->dtype, a->k) ? 0 : c.take(repack_bytes(a->dtype, a->n, a->k));
+        else if (!tma_ready(a->x, a->dtype, a->k)) p.x = c.take(repack_bytes(forward_parts(a), a->rows, a->k));
+        p.w = tma_ready(a->w, a->dtype, a->k) ? 0 : c.take(repack_bytes(forward_parts(a), a->n, a->k));
     }
     p.bytes = c.at;
     return p;
@@ -551,7 +603,7 @@ static BackwardPlan backward_plan(const plattice_linear_args* a) {
     if (p.narrow) {
         // one round of CTAs over the slices of 64 channels
         const int64_t slices = ceil_div(a->k, 64), need = ceil_div(ceil_div(a->rows, 16), kGradWarps);
-        const int64_t most = ceil_div(narrow_grad_ctas(a->dtype == PLATTICE_F32 ? 3 : 1, (a->n + 7) / 8) * (int64_t)sm_count(), slices);
+        const int64_t most = ceil_div(narrow_grad_ctas(pass_parts(a), (a->n + 7) / 8) * (int64_t)sm_count(), slices);
         p.lines = (int)(need < most ? (need < 1 ? 1 : need) : most);
         p.partial_w = c.take((int64_t)p.lines * ((int64_t)a->n * a->k + a->n) * 4);
         p.bytes = c.at;
@@ -567,14 +619,15 @@ static BackwardPlan backward_plan(const plattice_linear_args* a) {
     p.gz_needed = !(a->act == PLATTICE_ACT_NONE && !a->split && a->out_dtype == a->dtype &&
                     tma_ready(a->grad0, a->dtype, a->n));
     p.pitch = up8(a->n);
-    if (p.gz_needed) p.gz = c.take(repack_bytes(a->dtype, a->rows, a->n));
+    if (p.gz_needed) p.gz = c.take(repack_bytes(gz_parts(a), a->rows, a->n));
     p.bn_x = choose_bn(a->rows, a->k, 64, chunked((int)ceil_div(a->n, kBK), a->dtype, true));
     p.bn_w = choose_bn_w(a);
     p.parts_w = choose_parts(a->k, a->n, p.bn_w, ceil_div(a->rows, kBK));
-    if (a->grad_x && !tma_ready(a->w, a->dtype, a->k)) p.w = c.take(repack_bytes(a->dtype, a->n, a->k));
+    const int parts = tiled_parts(a);
+    if (a->grad_x && (parts > 1 || !tma_ready(a->w, a->dtype, a->k))) p.w = c.take(repack_bytes(parts, a->n, a->k));
     if (a->grad_w && a->x_scale) p.x = c.take(a->rows * up8(a->k) * 2);
-    if (a->grad_w && !a->x_scale && !tma_ready(a->x, a->dtype, a->k))
-        p.x = c.take(repack_bytes(a->dtype, a->rows, a->k));
+    if (a->grad_w && !a->x_scale && (parts > 1 || !tma_ready(a->x, a->dtype, a->k)))
+        p.x = c.take(repack_bytes(parts, a->rows, a->k));
     if (a->grad_w && p.parts_w > 1) p.partial_w = c.take((int64_t)p.parts_w * a->n * a->k * 4);
     p.bytes = c.at;
     return p;
@@ -582,17 +635,16 @@ static BackwardPlan backward_plan(const plattice_linear_args* a) {
 
 template <typename TG, typename T>
 static cudaError_t launch_grad_z(const GradArgs& g, const BackwardPlan& p, cudaStream_t s) {
+    const dim3 ctas(p.strips, p.parts_b);
     const bool fast = g.vec && !g.split && g.pitch % 8 == 0;
     // below 8 M values filling the tables takes what they save (us, 256 columns,
     // bfloat16, gelu, table / computed: 4096 rows 6.2 / 3.9, 16384 8.1 / 7.5, 32768
     // 12.1 / 13.6, 131072 32.3 / 44.6)
     const bool table = fast && g.z_scale && g.rows * g.n >= (1 << 23);
-    if (table && g.act == PLATTICE_ACT_GELU)
-        k_grad_z_table<TG, T, PLATTICE_ACT_GELU><<<dim3(p.strips, p.parts_b), 256, 0, s>>>(g);
-    else if (table && g.act == PLATTICE_ACT_SILU)
-        k_grad_z_table<TG, T, PLATTICE_ACT_SILU><<<dim3(p.strips, p.parts_b), 256, 0, s>>>(g);
-    else if (fast) k_grad_z<TG, T, true><<<dim3(p.strips, p.parts_b), 256, 0, s>>>(g);
-    else k_grad_z<TG, T, false><<<dim3(p.strips, p.parts_b), 256, 0, s>>>(g);
+    if (table && g.act == PLATTICE_ACT_GELU) k_grad_z_table<TG, T, PLATTICE_ACT_GELU><<<ctas, 256, 0, s>>>(g);
+    else if (table && g.act == PLATTICE_ACT_SILU) k_grad_z_table<TG, T, PLATTICE_ACT_SILU><<<ctas, 256, 0, s>>>(g);
+    else if (fast) k_grad_z<TG, T, true><<<ctas, 256, 0, s>>>(g);
+    else k_grad_z<TG, T, false><<<ctas, 256, 0, s>>>(g);
     return cudaGetLastError();
 }
 
@@ -611,8 +663,8 @@ static cudaError_t forward_mma(const plattice_linear_args* a, const ForwardPlan&
     Operand x, w;
     cudaError_t e = cudaSuccess;
     if (a->x_scale) e = unpacked(&x, a, ws + p.x, s);
-    else e = operand(&x, a->x, a->dtype, a->rows, a->k, ws + p.x, s);
-    if (e == cudaSuccess) e = operand(&w, a->w, a->dtype, a->n, a->k, ws + p.w, s);
+    else e = operand(&x, a->x, a->dtype, forward_parts(a), a->rows, a->k, ws + p.x, s);
+    if (e == cudaSuccess) e = operand(&w, a->w, a->dtype, forward_parts(a), a->n, a->k, ws + p.w, s);
     if (e != cudaSuccess) return e;
     MmaArgs m{};
     m.y0 = a->y0;
@@ -632,6 +684,7 @@ static cudaError_t forward_mma(const plattice_linear_args* a, const ForwardPlan&
     m.half = a->dtype == PLATTICE_F16;
     m.fault = pl::fault_word(s);
     m.precise = true;
+    m.scale = 1.f;
     sum_args(&m, a->k, 1, x.parts, w.parts);
     return mma_forward(p.bn, aligned, x, w, m, s);
 }
@@ -662,7 +715,7 @@ static cudaError_t backward_narrow(const plattice_linear_args* a, const Backward
     g.need_b = a->grad_bias != nullptr;
     g.vec_gx = a->k % 8 == 0 && aligned16(a->grad_x);
     g.vec_g = aligned16(a->grad0) && (!a->split || aligned16(a->grad1));
-    const cudaError_t e = run_narrow_grad(g, a->dtype, p.lines, s);
+    const cudaError_t e = run_narrow_grad(g, a->dtype, pass_parts(a), p.lines, s);
     if (e != cudaSuccess || !(a->grad_w || a->grad_bias)) return e;
     const int64_t nw = (int64_t)a->n * a->k, columns = nw + a->n;
     k_sum_lines<<<(unsigned)ceil_div(columns, 32), 1024, 0, s>>>(a->grad_w, a->dtype, nw, a->grad_bias, a->bias_dtype, a->n,
@@ -677,13 +730,13 @@ static cudaError_t grad_z(const plattice_linear_args* a, const BackwardPlan& p, 
     if (!store && !a->grad_bias) return cudaSuccess;
     const GradArgs g{a->grad0, a->grad1, slope ? a->z : nullptr, slope ? a->z_scale : nullptr, store ? ws + p.gz : nullptr, p.pitch,
                      a->grad_bias ? reinterpret_cast<float*>(ws + p.partial_b) : nullptr, a->rows, a->n, a->split,
-                     a->act, p.shift,
+                     a->act, p.shift, gz_halved(a),
                      a->n % 8 == 0 && aligned16(a->grad0) && (!slope || a->z_scale || aligned16(a->z))};
     cudaError_t e;
     if (a->out_dtype == PLATTICE_F32)
-        e = a->dtype == PLATTICE_F32    ? launch_grad_z<float, float>(g, p, s)
+        e = a->dtype == PLATTICE_F32    ? launch_grad_z<float, Parts<3>>(g, p, s)
             : a->dtype == PLATTICE_BF16 ? launch_grad_z<float, __nv_bfloat16>(g, p, s)
-                                        : launch_grad_z<float, __half>(g, p, s);
+                                        : launch_grad_z<float, Parts<2>>(g, p, s);
     else
         e = a->dtype == PLATTICE_BF16 ? launch_grad_z<__nv_bfloat16, __nv_bfloat16>(g, p, s)
                                       : launch_grad_z<__half, __half>(g, p, s);
@@ -693,15 +746,16 @@ static cudaError_t grad_z(const plattice_linear_args* a, const BackwardPlan& p, 
 
 static cudaError_t backward_mma(const plattice_linear_args* a, const BackwardPlan& p, cudaStream_t s) {
     char* ws = static_cast<char*>(a->workspace);
-    Operand gz{p.gz_needed ? ws + p.gz : a->grad0, a->rows, a->n, p.gz_needed ? p.pitch : a->n,
-               a->dtype == PLATTICE_F32 ? 3 : 1};
+    const Operand gz{p.gz_needed ? ws + p.gz : a->grad0, a->rows, a->n, p.gz_needed ? p.pitch : a->n, gz_parts(a)};
+    const int parts = tiled_parts(a);
     cudaError_t e = cudaSuccess;
     MmaArgs m{};
-    m.half = a->dtype == PLATTICE_F16;
+    m.half = a->dtype == PLATTICE_F16 && parts == 1;
+    m.scale = gz_halved(a) ? 2.f : 1.f;
     m.fault = pl::fault_word(s);
     if (a->grad_x) {
         Operand w;
-        e = operand(&w, a->w, a->dtype, a->n, a->k, ws + p.w, s);
+        e = operand(&w, a->w, a->dtype, parts, a->n, a->k, ws + p.w, s);
         if (e != cudaSuccess) return e;
         m.y0 = a->grad_x;
         m.ni = a->rows;
@@ -715,7 +769,7 @@ static cudaError_t backward_mma(const plattice_linear_args* a, const BackwardPla
     if (a->grad_w) {
         Operand x;
         if (a->x_scale) e = unpacked(&x, a, ws + p.x, s);
-        else e = operand(&x, a->x, a->dtype, a->rows, a->k, ws + p.x, s);
+        else e = operand(&x, a->x, a->dtype, parts, a->rows, a->k, ws + p.x, s);
         if (e != cudaSuccess) return e;
         m.ni = a->k;
         m.nj = a->n;

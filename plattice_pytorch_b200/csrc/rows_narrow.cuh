@@ -629,38 +629,40 @@ __global__ void __launch_bounds__(32 * kNarrowWarps, narrow_ctas(kXT, kNF)) k_na
 // where the gradient's pass and two tiled products took 72.
 constexpr int kTilePitch = 72;   // 16-bit elements: rows 144 bytes apart, no bank conflicts for ldmatrix
 
-// kParts: of the weights, 3 with float32 ones.  gz has 3 parts then, else 2:
-// it is made here in float32, and a second 16-bit part (28 more matrix
-// instructions a block of rows, 8 % of the pass) keeps what rounding it to
-// one would add to both gradients' errors.
+// kParts: of the weights: 3 with float32 ones, 1 or 2 with 16-bit ones.
+//
+// gz = grad_y act'(z) is made here in float32.  float16 holds only a small part of
+// what that can be (gradients of 1e-8 or 1e6, float16's largest times a slope above
+// 1), so float16 operands run as two bfloat16 parts each (exact; gz's two hold 16
+// bits), three products, unless the gradients are float16 themselves and there is
+// no activation: then gz is one float16 part, as it came.  Beside bfloat16 operands
+// gz has two parts, too: 28 more matrix instructions a block of rows, 8 % of the
+// pass, keep what rounding it to one would add to both gradients' errors.
 template <int kXT, int kParts> struct NarrowGradShape {
-    static constexpr int kPX = kXT == kXFloat ? 3 : 1;
-    static constexpr int kPZ = kParts == 3 ? 3 : 2;
+    static constexpr bool kHalf = kXT == kXHalf && kParts == 1;                       // float16 matrix instructions
+    static constexpr int kPX = kXT == kXFloat ? 3 : kParts == 2 ? 2 : 1;
+    static constexpr int kPZ = kHalf ? 1 : kParts == 3 ? 3 : 2;
     static constexpr int kFragBytes = kParts * 2 * 8 * 32 * 8;                        // weights of the slice
     static constexpr int kStaged = 16 * kNarrowPitch + 4;   // gz of 16 rows, and a place for what is behind them
     static constexpr int kWarpBytes = kStaged * 4 + kPX * 16 * kTilePitch * 2;
     static constexpr int kBytes = kFragBytes + kGradWarps * kWarpBytes + 64 * 33 * 4;
 };
 
-// a and b as kP packed parts: bfloat16 (two beside operands of one), or float16,
-// rounded.  kAny: they may not be finite.
-template <int kP, bool kHalf, bool kAny>
+// a and b as kP packed parts, bfloat16 or a float16.  kAny: they may not be finite;
+// kLone: they meet operands of a single part.
+template <int kP, bool kHalf, bool kAny, bool kLone = false>
 __device__ __forceinline__ void to_parts(float a, float b, uint32_t (&o)[kP]) {
-    if constexpr (!kHalf && kP == 2) {
+    if constexpr (kHalf) {
+        static_assert(kP == 1, "float16 operands of one part");
+        union { __half2 h; uint32_t u; } x;
+        x.h = __floats2half2_rn(a, b);
+        o[0] = x.u;
+    } else if constexpr (kLone && kP == 2) {
         split_one_sign<kAny>(a, b, o);
-    } else if constexpr (!kHalf && kAny) {
+    } else if constexpr (kAny) {
         split_any(a, b, o);
-    } else if constexpr (!kHalf) {
-        split_pair(a, b, o);
     } else {
-#pragma unroll
-        for (int i = 0; i < kP; ++i) {
-            union { __half2 h; uint32_t u; } x;
-            x.h = __floats2half2_rn(a, b);
-            o[i] = x.u;
-            a -= __low2float(x.h);
-            b -= __high2float(x.h);
-        }
+        split_pair(a, b, o);
     }
 }
 
@@ -668,16 +670,14 @@ template <int kXT, bool kG32> struct GradType { typedef __nv_bfloat16 type; };
 template <int kXT> struct GradType<kXT, true> { typedef float type; };
 template <> struct GradType<kXHalf, false> { typedef __half type; };
 
-// kXT: the type of x (and, for 16-bit ones, of everything); kParts: 3 with
-// float32 weights; kNF: output channels / 8.
-
-// kG32: float32 gradients beside 16-bit operands.
+// kXT: the type of x (and, for 16-bit ones, of everything); kNF: output channels / 8;
+// kG32: float32 gradients.
 template <int kXT, int kParts, int kNF, bool kG32>
 __global__ void __launch_bounds__(32 * kGradWarps, narrow_grad_ctas(kParts, kNF)) k_narrow_grad(const SmallGradArgs a) {
     typedef NarrowGradShape<kXT, kParts> Shape;
     typedef typename GradType<kXT, kG32>::type TG;
     constexpr int kPX = Shape::kPX, kPZ = Shape::kPZ, kKS = kNF > 2 ? 2 : 1;   // steps of 16 output channels in grad_x's sum
-    constexpr bool kHalf = kXT == kXHalf;
+    constexpr bool kHalf = Shape::kHalf;
     extern __shared__ __align__(16) char smem_raw[];
     uint2* frag = reinterpret_cast<uint2*>(smem_raw);   // [kParts][kKS][8][32]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -818,6 +818,22 @@ __global__ void __launch_bounds__(32 * kGradWarps, narrow_grad_ctas(kParts, kNF)
                     }
                     if (!not_finite(w)) put(Fixed<false>());
                     else put(Fixed<true>());
+                } else if (kPX == 2) {   // float16 as two bfloat16
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        union { uint4 u; __half2 h[4]; } q;
+                        q.u = xn.v[0][h][i % NarrowShape<kXT>::kRaw];
+                        uint32_t o[4][2];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const float2 f = __half22float2(q.h[j]);
+                            split_any(f.x, f.y, o[j]);
+                        }
+#pragma unroll
+                        for (int p = 0; p < 2; ++p)
+                            reinterpret_cast<uint4*>(row + (p % kPX) * 16 * kTilePitch)[i] =
+                                make_uint4(o[0][p], o[1][p], o[2][p], o[3][p]);
+                    }
                 } else {
                     reinterpret_cast<uint4*>(row)[0] = xn.v[0][h][0];
                     reinterpret_cast<uint4*>(row)[1] = xn.v[0][h][1 % NarrowShape<kXT>::kRaw];
@@ -870,8 +886,8 @@ __global__ void __launch_bounds__(32 * kGradWarps, narrow_grad_ctas(kParts, kNF)
                     for (int h = 0; h < 2; ++h) {
                         const float* p = st + (g + 8 * h) * kNarrowPitch + t * cols_per_lane + s * 4;
                         uint32_t lo[kPZ], hi[kPZ];
-                        to_parts<kPZ, kHalf, decltype(any)::value>(p[0], p[1], lo);
-                        to_parts<kPZ, kHalf, decltype(any)::value>(p[2], p[3], hi);
+                        to_parts<kPZ, kHalf, decltype(any)::value, kPX == 1 && kParts == 1>(p[0], p[1], lo);
+                        to_parts<kPZ, kHalf, decltype(any)::value, kPX == 1 && kParts == 1>(p[2], p[3], hi);
 #pragma unroll
                         for (int q = 0; q < kPZ; ++q) {
                             o[s][q][h] = lo[q];
@@ -921,7 +937,7 @@ __global__ void __launch_bounds__(32 * kGradWarps, narrow_grad_ctas(kParts, kNF)
                     for (int h = 0; h < 2; ++h) {
                         const float* p = st + (2 * t + 8 * h) * kNarrowPitch + f * 8 + g;
                         uint32_t o[kPZ];
-                        to_parts<kPZ, kHalf, decltype(any)::value>(p[0], p[kNarrowPitch], o);
+                        to_parts<kPZ, kHalf, decltype(any)::value, kPX == 1 && kParts == 1>(p[0], p[kNarrowPitch], o);
 #pragma unroll
                         for (int q = 0; q < kPZ; ++q) b[q][f][h] = o[q];
                     }

@@ -53,6 +53,7 @@ inline bool narrow_shares(int64_t blocks, int k) { return blocks * 256 <= (int64
 
 cudaError_t run_narrow(const SmallArgs& a, int dtype, cudaStream_t s);
 cudaError_t run_few_rows(const SmallArgs& a, int dtype, cudaStream_t s);
-cudaError_t run_narrow_grad(const SmallGradArgs& a, int dtype, int lines, cudaStream_t s);
+// parts: of the weights (NarrowGradShape).
+cudaError_t run_narrow_grad(const SmallGradArgs& a, int dtype, int parts, int lines, cudaStream_t s);
 
 }  // namespace plr

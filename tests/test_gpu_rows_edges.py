@@ -8,7 +8,8 @@ import numpy as np
 import pytest
 import torch
 
-from rows_reference import U, f64, half_step
+import rows_reference as ref
+from rows_reference import U, f64, half_step, worst
 
 pytestmark = pytest.mark.gpu
 
@@ -31,6 +32,79 @@ def R():
 def _randn(shape, seed, dtype=torch.float32, scale=1.0):
     g = torch.Generator().manual_seed(seed)
     return (torch.randn(*shape, generator=g) * scale).to(dtype)
+
+
+# ------------------------------------------------- float16 with any gradient
+
+# One row, few output channels in one pass, tiled products; the last with rows
+# that lie on no 16-byte boundaries.
+GRAD_SHAPES = [(1, 64, 24), (377, 50, 8), (3000, 200, 17), (500, 72, 40), (3000, 600, 24), (700, 33, 91)]
+
+
+def _check_grads(got, gy, xe, we, ze, act, t, out, gz_error):
+    """Gradients against their definitions: gz off by gz_error of itself (and
+    the slope's functions, 2^-18 of gy), sums 2 u a term, one rounding to t."""
+    xr, wr, br, gz = ref.linear_backward(gy, xe, we, ze, act)
+    rows, n = gz.shape
+    az = np.abs(gz) * (gz_error + 2 * U) + 2.0 ** -18 * np.abs(gy) * (act != "none")
+    tiny = (t is torch.float16) * 2.0 ** -25 + 1e-37
+    for g, e, off, m, size in ((got[0], xr, az @ np.abs(we), n, np.abs(gz) @ np.abs(we)),
+                               (got[1], wr, az.T @ np.abs(xe), rows, np.abs(gz).T @ np.abs(xe))):
+        g = f64(g)
+        assert np.isfinite(g).all()
+        assert worst(g, e, off + 2 * U * (m + 8) * size + half_step(t) * np.abs(e) + tiny) <= 1
+    assert worst(f64(got[2]), br, az.sum(0) + (rows + 8) * U * np.abs(gz).sum(0) + U * np.abs(br) + 1e-37) <= 1
+
+
+@pytest.mark.parametrize("act", ["none", "gelu", "relu"])
+@pytest.mark.parametrize("scale", [1e-9, 1e-6, 1e6])
+@pytest.mark.parametrize("rows,k,n", GRAD_SHAPES)
+def test_float16_with_float32_gradients_of_any_size(dev, R, rows, k, n, scale, act):
+    """Gradients that float16 does not hold, with weights and inputs that bring
+    the results back into its range.  gz keeps 16 bits or more (2^-17), and
+    what its parts' products leave out is 2^-17 of them."""
+    t = torch.float16
+    back = min(max(1 / scale, 1e-4), 1e4) / 8   # float16 holds x and w
+    x, w = _randn((rows, k), 1, t, back / math.sqrt(rows)), _randn((n, k), 2, t, back / math.sqrt(n))
+    gy = _randn((rows, n), 3, scale=scale)
+    z = None if act == "none" else _randn((rows, n), 4).to(dev)
+    got = R.linear_backward(gy.to(dev), x.to(dev), w.to(dev), z, act=act, bias_dtype=torch.float32)
+    _check_grads(got, f64(gy), f64(x), f64(w), None if z is None else f64(z), act, t, torch.float32, 2.0 ** -16)
+
+
+def test_float16_weight_gradient_of_a_million_tiny_gradients(dev, R):
+    rows = 1 << 20
+    for n, k in ((5, 16), (40, 16)):
+        x, w = torch.ones(rows, k, dtype=torch.float16, device=dev), torch.ones(n, k, dtype=torch.float16, device=dev)
+        gx, gw, gb = R.linear_backward(torch.full((rows, n), 1e-8, device=dev), x, w, bias_dtype=torch.float32)
+        # one rounding to float16 after float32 sums of like terms
+        assert worst(f64(gw), np.full((n, k), rows * 1e-8), (2.0 ** -11 + 2.0 ** -16 + rows / 16 * 2.0 ** -25 / 8) * rows * 1e-8) <= 1
+        assert worst(f64(gb), np.full(n, rows * 1e-8), 2.0 ** -12 * rows * 1e-8) <= 1
+        assert worst(f64(gx), np.full((rows, k), n * 1e-8), 2.0 ** -25 + 2.0 ** -11 * n * 1e-8) <= 1
+
+
+@pytest.mark.parametrize("rows,k,n", GRAD_SHAPES)
+@pytest.mark.parametrize("keep", ["8bit", "full"])
+def test_float16_gradients_behind_an_activation(dev, R, rows, k, n, keep):
+    """float16 gradients at the type's end: times gelu's slope they are past it.
+    gz is off by half a step of float16, and by one of its smallest (2^-24)."""
+    t = torch.float16
+    gy = torch.where(_randn((rows, n), 5) > 0, 6.5e4, 3e-3).to(t)
+    z = _randn((rows, n), 6, t).abs().to(dev) + 1   # slopes of 1.08 to 1.13
+    z8 = R.pack8(z) if keep == "8bit" else z
+    x, w = _randn((rows, k), 7, t, 1e-3), _randn((n, k), 8, t, 1e-3)
+    got = R.linear_backward(gy.to(dev), x.to(dev), w.to(dev), z8, act="gelu", bias_dtype=torch.float32)
+    ze = f64(R.unpack8(z8)) if keep == "8bit" else f64(z)
+    _check_grads(got, f64(gy), f64(x), f64(w), ze, "gelu", t, t, 2.0 ** -11)
+
+
+def test_float16_split_gradients(dev, R):
+    t, rows, k = torch.float16, 900, 64
+    for n, cut in ((24, 16), (90, 50)):
+        x, w, gy = _randn((rows, k), 9, t, 1e-4), _randn((n, k), 10, t, 1e-4), _randn((rows, n), 11, scale=1e6)
+        pair = (gy[:, :cut].contiguous().to(dev), gy[:, cut:].contiguous().to(dev))
+        got = R.linear_backward(pair, x.to(dev), w.to(dev), bias_dtype=torch.float32)
+        _check_grads(got, f64(gy), f64(x), f64(w), None, "none", t, torch.float32, 2.0 ** -16)
 
 
 # ---------------------------------------------------------------- float32
@@ -105,7 +179,7 @@ def test_infinite_weights_of_8_bit_rows(dev, R, rows, n):
         _same(y[:3], e, 2 * U * (k + 8) * _weighted(np.abs(xe), np.abs(np.where(np.isfinite(f64(w)), f64(w), 0))) + 1e-6)
 
 
-@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,k,n", [(37, 64, 24), (1, 40, 3), (375, 50, 8), (503, 33, 91)])
 def test_infinite_input_in_the_last_row(dev, R, rows, k, n, dtype):
     """Where the last block of rows is not whole, the last row counts once."""
@@ -117,7 +191,7 @@ def test_infinite_input_in_the_last_row(dev, R, rows, k, n, dtype):
     _same(gw, e, (2 * U * (rows + 8) + half_step(t)) * (np.abs(f64(gy)).T @ np.abs(np.where(np.isfinite(f64(x)), f64(x), 0))) + 1e-6)
 
 
-@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("out32", [False, True])
 @pytest.mark.parametrize("rows,k,n", [(37, 64, 24), (375, 50, 8), (500, 72, 40), (503, 33, 91)])
 def test_infinite_gradients_and_inputs(dev, R, rows, k, n, dtype, out32):
