@@ -341,10 +341,10 @@ int plattice_rms_norm_backward(void* grad_x, void* grad_gain, const void* grad_y
  *
  * Backward, with gz = grad_y act'(z) (z as kept, or NULL without activation):
  *   grad_x = gz w, grad_w = gz^T x (both in dtype), grad_bias = sum_r gz
- * (bias_dtype); each output may be NULL.  gz may be rounded to dtype before the
- * two products (with few output channels it keeps more), but within float32's
- * range: beside float32 gradients float16 operands take it as 16 bits of any
- * size.  Sums are held in float32 and added in a fixed order. */
+ * (bias_dtype); each output may be NULL.  16-bit gradients: gz may be rounded to
+ * their type before the two products (with few output channels it keeps more);
+ * float32 ones: it keeps at least 16 bits, of any size.  Sums are held in float32
+ * and added in a fixed order. */
 typedef struct plattice_linear_args {
     const void* x;
     const uint8_t* x_scale;

@@ -15,16 +15,21 @@ namespace plr {
 
 // ----------------------------------------------------- operands for the MMAs
 
-// How a value is stored: N bfloat16 parts, one tensor of them after the other.
-template <int N> struct Parts { static constexpr int kParts = N; };
+// How a value is stored: N bfloat16 parts, one tensor of them after the other;
+// kLone: for products with operands of a single part.
+template <int N, bool kLone = false> struct Parts {
+    static constexpr int kParts = N;
+    static constexpr bool lone = kLone;
+};
 
-template <int N>
+template <int N, bool kLone>
 __device__ __forceinline__ void store_parts(__nv_bfloat16* p, int64_t stride, const float (&v)[8], bool vec, int n) {
     union { uint4 u; uint32_t w[4]; __nv_bfloat16 h[8]; } o[N];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         uint32_t t[N];
-        split_any(v[2 * i], v[2 * i + 1], t);
+        if constexpr (kLone) split_one_sign<true>(v[2 * i], v[2 * i + 1], t);
+        else split_any(v[2 * i], v[2 * i + 1], t);
 #pragma unroll
         for (int j = 0; j < N; ++j) o[j].w[i] = t[j];
     }
@@ -41,7 +46,7 @@ __device__ __forceinline__ void store_parts(__nv_bfloat16* p, int64_t stride, co
 // 8 values as a T (a type, or Parts) from element `at` of a tensor of `size`.
 template <typename T>
 __device__ __forceinline__ void store8_as(void* p, int64_t at, int64_t size, const float (&v)[8], bool vec, int n) {
-    if constexpr (std::is_empty_v<T>) store_parts<T::kParts>(static_cast<__nv_bfloat16*>(p) + at, size, v, vec, n);
+    if constexpr (std::is_empty_v<T>) store_parts<T::kParts, T::lone>(static_cast<__nv_bfloat16*>(p) + at, size, v, vec, n);
     else store8(static_cast<T*>(p) + at, v, vec, n);
 }
 
@@ -96,11 +101,11 @@ template <typename T> __device__ __forceinline__ void halve(float (&g)[8], bool 
 constexpr int kTogether = 2;
 
 // gz = grad_y act'(z) as the two products take it, and the sums of the unrounded
-// gz over a CTA's rows.  bfloat16 operands take it rounded to one part (a tensor
-// core takes no wider operand; one rounding, as a stored gradient has), float32
-// ones as three parts; float16 ones as two bfloat16 parts (gz_parts) or rounded, too
-// (gz_halved).  2^shift threads of 8 columns share a row; gridDim.x strips of
-// columns, gridDim.y parts of rows.
+// gz over a CTA's rows.  Behind 16-bit gradients gz is rounded to their type (a
+// tensor core takes no wider operand; one rounding, as a stored gradient has;
+// gz_halved); behind float32 ones it is two bfloat16 parts beside 16-bit operands,
+// three beside float32 ones (gz_parts).  2^shift threads of 8 columns share a row;
+// gridDim.x strips of columns, gridDim.y parts of rows.
 template <typename TG, typename T, bool kFast>
 __global__ void __launch_bounds__(256, 4) k_grad_z(const GradArgs a) {
     __shared__ float sums[8 * 256];
@@ -361,12 +366,12 @@ static bool tma_ready(const void* p, int dtype, int64_t width) {
     return dtype != PLATTICE_F32 && width % 8 == 0 && aligned16(p);
 }
 
-// Parts that the tiled backward's gz is made of: float32's three; of float16
-// operands beside float32 gradients, which can be far smaller and far larger than
-// float16 holds, two bfloat16 (the operands have two then, too); else one.
+// Parts that the tiled backward's gz is made of: three beside float32 operands;
+// behind float32 gradients, whose 16 leading bits stay and which can be far smaller
+// and far larger than float16 holds, two bfloat16 (float16 operands have two then,
+// too); else one.
 static int gz_parts(const plattice_linear_args* a) {
-    if (a->dtype == PLATTICE_F32) return 3;
-    return a->dtype == PLATTICE_F16 && a->out_dtype == PLATTICE_F32 ? 2 : 1;
+    return a->dtype == PLATTICE_F32 ? 3 : a->out_dtype == PLATTICE_F32 ? 2 : 1;
 }
 
 // A float16 gradient times a slope (of up to 1.13) can be past float16's largest:
@@ -735,7 +740,7 @@ static cudaError_t grad_z(const plattice_linear_args* a, const BackwardPlan& p, 
     cudaError_t e;
     if (a->out_dtype == PLATTICE_F32)
         e = a->dtype == PLATTICE_F32    ? launch_grad_z<float, Parts<3>>(g, p, s)
-            : a->dtype == PLATTICE_BF16 ? launch_grad_z<float, __nv_bfloat16>(g, p, s)
+            : a->dtype == PLATTICE_BF16 ? launch_grad_z<float, Parts<2, true>>(g, p, s)
                                         : launch_grad_z<float, Parts<2>>(g, p, s);
     else
         e = a->dtype == PLATTICE_BF16 ? launch_grad_z<__nv_bfloat16, __nv_bfloat16>(g, p, s)

@@ -107,6 +107,25 @@ def test_float16_split_gradients(dev, R):
         _check_grads(got, f64(gy), f64(x), f64(w), None, "none", t, torch.float32, 2.0 ** -16)
 
 
+# ---------------------------------- float32 gradients beside 16-bit operands
+
+@pytest.mark.parametrize("x8", [False, True])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("rows,k,n", GRAD_SHAPES)
+def test_float32_gradients_keep_16_bits(dev, R, rows, k, n, dtype, x8):
+    """Sums whose large parts cancel: what rounding gz to 8 or 11 bits would
+    lose is all that is left of them."""
+    t = DTYPES[dtype]
+    if x8 and t is torch.float16:
+        pytest.skip("8-bit rows take no float16 weights")
+    sign = lambda s, i: torch.where(_randn(s, i) > 0, 1.0, -1.0)  # noqa: E731
+    x, w = sign((rows, k), 12), sign((n, k), 13).to(t)
+    gy = 1 + 2.0 ** -10 * torch.rand(rows, n, generator=torch.Generator().manual_seed(14))
+    xin = R.pack8(x.to(dev)) if x8 else x.to(t).to(dev)
+    got = R.linear_backward(gy.to(dev), xin, w.to(dev), bias_dtype=torch.float32)
+    _check_grads(got, f64(gy), f64(x), f64(w), None, "none", t, torch.float32, 2.0 ** -16)
+
+
 # ---------------------------------------------------------------- float32
 
 FORMS = [(3, 24), (5000, 24), (700, 40), (5000, 72)]   # rows, n: few rows, few channels, tiles
