@@ -306,7 +306,8 @@ const char* plattice_profile_stage_name(int stage);
  * with which the block's largest finite magnitude is at most 448 (the exponent
  * is held in -110..120); a value that is not finite comes back as NaN and its
  * neighbours are kept.  q is 16-byte aligned.  Rounding: at most 2^-4 of a
- * value, or 2^-10 of the scale for small ones. */
+ * value, or 2^-10 of the scale for small ones (finite values stay finite: next
+ * to float32's largest they are held at 240 * 2^120). */
 int plattice_rows_pack8(uint8_t* q, uint8_t* scale, const void* x, int dtype, long long rows, int c, void* stream);
 int plattice_rows_unpack8(void* y, int dtype, const uint8_t* q, const uint8_t* scale, long long rows, int c,
                           void* stream);

@@ -5,7 +5,8 @@
 // to 32 (codes behind the last channel are 0), and one byte per 32 channels,
 // 127 + s: the codes stand for code * 2^s.  2^s is the smallest power of two
 // with amax <= 448 * 2^s (448: the largest e4m3 value), so nothing saturates
-// and a block's largest value keeps at least 3 mantissa bits.  A power of two
+// (but for values next to float32's largest, held8) and a block's largest value
+// keeps at least 3 mantissa bits.  A power of two
 // makes code * 2^s exact in bfloat16 and float32 (4 significant bits), so a
 // product of bfloat16 operands reads the checkpoint without a further
 // rounding.  s is clamped to [-110, 120]: the smallest non-zero value is then
@@ -183,6 +184,18 @@ template <> struct Raw8<float> {
 
 // --------------------------------------------------------------- 8-bit rows
 
+// NaN stays NaN in both
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float y;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+
 // s of a block whose largest finite magnitude is amax: amax = 1.f * 2^e needs
 // 2^(e-8) when 1.f <= 1.75 (448 = 1.75 * 2^8), twice that otherwise.
 __device__ __forceinline__ int block_exponent(float amax) {
@@ -229,10 +242,25 @@ __device__ __forceinline__ float finite_amax_of(const float (&v)[N], bool& infin
     return amax;
 }
 
+// At the largest scale codes of 256 stand for infinity: values that would round to
+// them (from 248 2^120 on) are held at the code below, within 2^-4 of them.
+__device__ __forceinline__ bool largest_scale(float inv) { return inv == pow2(-kScaleMax); }
+__device__ __forceinline__ float held8(float v) {
+    const float most = 240.f * pow2(kScaleMax);
+    return max_nan(min_nan(v, most), -most);
+}
+
 // Codes of 8 values, finite or NaN, times 2^-s (multiplying by a power of two
 // is exact, so the one rounding is the conversion's).
-__device__ __forceinline__ uint2 codes8(const float* v, float inv) {
+__device__ __forceinline__ uint2 codes8(const float* values, float inv) {
     unsigned w[2];
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = values[i];
+    if (largest_scale(inv)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = held8(v[i]);
+    }
     const uint64_t m = both(inv);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -292,18 +320,6 @@ __device__ __forceinline__ float reciprocal_fast(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// NaN stays NaN in both
-__device__ __forceinline__ float min_nan(float a, float b) {
-    float y;
-    asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
-    return y;
-}
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float y;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
-    return y;
-}
-
 // Phi(-|z|) and exp(-z^2 / 2), by the rational approximation of the error
 // function 7.1.26 of Abramowitz and Stegun, Handbook of Mathematical
 // Functions (off by at most 1.5e-7 of erf, about a float32 step of 1): a

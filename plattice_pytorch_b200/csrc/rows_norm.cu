@@ -70,6 +70,7 @@ __global__ void __launch_bounds__(256) k_pack8(uint8_t* __restrict__ q, uint8_t*
 constexpr int kBlocks = 8;
 
 __device__ __forceinline__ uint8_t code1(float v, float inv) {
+    if (largest_scale(inv) && !is_infinite(fabsf(v))) v = held8(v);
     return (uint8_t)__nv_cvt_float_to_fp8(is_infinite(fabsf(v)) ? __int_as_float(0x7fffffff) : v * inv, __NV_SATFINITE,
                                           __NV_E4M3);
 }
@@ -261,6 +262,10 @@ __device__ __forceinline__ void store_group8(uint8_t* q, uint8_t* scale, float (
         for (int o = kLanes / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
         const int s = block_exponent(amax);
         const float inv = pow2(-s);
+        if (kWide < 8 && largest_scale(inv)) {
+#pragma unroll
+            for (int i = first; i < first + kTimes * kWide; ++i) y[i] = held8(y[i]);
+        }
 #pragma unroll
         for (int i = first; i < first + kTimes * kWide; i += kWide) {
             const int col = channel_of<L, kWide>(lane, k, i);

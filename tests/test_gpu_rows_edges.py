@@ -232,6 +232,41 @@ def test_infinite_gradients_and_inputs(dev, R, rows, k, n, dtype, out32):
     _same(got[2], ge.sum(0), 2 * U * (rows + 8) * fin(ge).sum(0))
 
 
+# ------------------------------------------------- the largest finite values
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("c", [1, 3, 32, 50, 64])
+def test_pack8_of_the_largest_values(dev, R, c, dtype):
+    """A block whose largest value is above 240 2^120 stays finite and within
+    2^-4 of itself."""
+    t = DTYPES[dtype]
+    top = torch.finfo(t).max
+    for v in (top, -top, 3.32e38, 3.25e38, 3.2e38):
+        x = torch.zeros(5, c)
+        x[1, c // 2], x[3, 0] = v, v / 2
+        x = x.to(t)
+        y = f64(R.unpack8(R.pack8(x.to(dev))))
+        assert np.isfinite(y).all() and worst(y, f64(x), 2.0 ** -4 * np.abs(f64(x)) + 1e-37) <= 1
+
+
+@pytest.mark.parametrize("c", [1, 2, 31, 34, 64, 520])
+def test_norm_in_8_bits_of_the_largest_values(dev, R, c):
+    x = torch.ones(7, c, device=dev)
+    gain = torch.full((c,), 3.35e38, device=dev)
+    y8, _, _ = R.rms_norm(x, gain, pack=True)
+    y = f64(R.unpack8(y8))
+    assert np.isfinite(y).all() and worst(y, np.full((7, c), 3.35e38), 2.0 ** -4 * 3.36e38) <= 1
+
+
+@pytest.mark.parametrize("rows,n", FORMS)
+def test_kept_z_of_the_largest_values(dev, R, rows, n):
+    for t in (torch.float32, torch.bfloat16):
+        b = torch.full((n,), 3.38e38, dtype=t, device=dev)
+        _, z = R.linear(torch.zeros(rows, 8, dtype=t, device=dev), torch.zeros(n, 8, dtype=t, device=dev), b, act="relu", keep="8bit")
+        y = f64(R.unpack8(z))
+        assert np.isfinite(y).all() and worst(y, np.broadcast_to(f64(b), y.shape), 2.0 ** -4 * 3.4e38) <= 1
+
+
 # ------------------------------------------------------- arguments and sizes
 
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
