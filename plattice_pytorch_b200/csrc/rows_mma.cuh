@@ -400,6 +400,11 @@ __device__ __forceinline__ void finish32(float (&v)[32], const MmaArgs& p, int64
     }
     const bool second = col0 + 16 < p.nj;
     if (p.z_scale) {
+        if (col0 + 32 > p.nj) {   // zeros behind the last column (a row that is not finite makes NaN there)
+            const int left = (int)(p.nj - col0);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = i < left ? v[i] : 0.f;
+        }
         keep_codes(v, p, row0 + lane, col0);
     } else if (p.z) {
         if (kMode == kAligned) store_aligned<kOut>(s, v, p.z, p, row0, col0, nullptr, ahead, lane);

@@ -574,7 +574,7 @@ __global__ void __launch_bounds__(32 * kNarrowWarps, narrow_ctas(kXT, kNF)) k_na
                 const int r = m * 16 + (lane >> 1), c0 = (lane & 1) * 16;
                 float v[16];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) v[i] = c0 + i < kNF * 8 ? st[r * kNarrowPitch + c0 + i] : 0.f;
+                for (int i = 0; i < 16; ++i) v[i] = c0 + i < a.n ? st[r * kNarrowPitch + c0 + i] : 0.f;
                 bool infinite;
                 float amax = finite_amax_of(v, infinite);
                 amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));

@@ -361,6 +361,11 @@ __global__ void __launch_bounds__(L > 256 ? L : 256) k_rms_norm(const NormArgs a
             float y[8];   // the gain is 0 behind the last channel
 #pragma unroll
             for (int i = 0; i < 8; ++i) y[i] = v[k][i] * rstd * gain[k][i];
+            if (a.yscale && !(rstd < INFINITY)) {   // rare: zeros there all the same
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (channel_of<L, kWide>(lane, k, i) >= a.c) y[i] = 0.f;
+            }
             if (a.yscale)
                 store_group8<L, kWide>(static_cast<uint8_t*>(a.y) + row * width, a.yscale + row * (width / 32), y, lane, k,
                                       width, live);

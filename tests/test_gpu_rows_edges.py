@@ -232,6 +232,25 @@ def test_infinite_gradients_and_inputs(dev, R, rows, k, n, dtype, out32):
     _same(got[2], ge.sum(0), 2 * U * (rows + 8) * fin(ge).sum(0))
 
 
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_padding_of_rows_that_are_not_finite(dev, R, dtype, bad):
+    """Zeros behind the last channel, whatever the row holds."""
+    t = DTYPES[dtype]
+    for c in (1, 3, 8, 33, 50, 72, 1030):
+        x = _randn((40, c), 23, t)
+        x[3], x[7, 0] = bad, bad
+        y8, _, _ = R.rms_norm(x.to(dev), torch.ones(c, device=dev), pack=True)
+        assert not y8.q[:, c:].any()
+        assert not R.pack8(x.to(dev)).q[:, c:].any()
+    for rows, n in FORMS + [(5000, 9), (5000, 41)]:
+        x = _randn((rows, 64), 24, t)
+        x[1], x[2, 5] = bad, bad
+        for xin in (x.to(dev),) + ((R.pack8(x.to(dev)),) if t is not torch.float16 else ()):
+            _, z = R.linear(xin, _randn((n, 64), 25, t).to(dev), act="relu", keep="8bit")
+            assert not z.q[:, n:].any()
+
+
 # ------------------------------------------------- the largest finite values
 
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
