@@ -320,23 +320,26 @@ __device__ __forceinline__ float reciprocal_fast(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// Phi(-|z|) and exp(-z^2 / 2), by the rational approximation of the error
-// function 7.1.26 of Abramowitz and Stegun, Handbook of Mathematical
-// Functions (off by at most 1.5e-7 of erf, about a float32 step of 1): a
-// reciprocal, an exponential and six multiply-adds.  The product's epilogue
-// computes it for every output on the way out, where a full-precision erf
-// would take longer than the matrix instructions it runs beside.
+// Phi(-|z|) and exp(-z^2 / 2).  Phi(-x) = exp(-x^2 / 2) R(x) with R smooth and
+// falling like 1 / x: R(x) is t times a polynomial of degree 7 in t = 1 / (1 + 0.3
+// x), whose coefficients are the minimax fit of the relative error over 0 <= x <=
+// 16, computed as a linear program (1.9e-7; evaluated in float32 5.2e-7, and the
+// exponential's argument adds u z^2, u = 2^-24).  So the tail is good relative to
+// itself as far as float32 holds it.  The product's epilogue computes this for
+// every output on the way out, beside the matrix instructions.
 __device__ __forceinline__ uint64_t tail2(float z0, float z1, uint64_t& e) {
-    constexpr float kP = 0.3275911f * 0.70710678118654752f;
-    const uint64_t t = pair_of(reciprocal_fast(fmaf(kP, fabsf(z0), 1.f)), reciprocal_fast(fmaf(kP, fabsf(z1), 1.f)));
+    const uint64_t t = pair_of(reciprocal_fast(fmaf(0.3f, fabsf(z0), 1.f)), reciprocal_fast(fmaf(0.3f, fabsf(z1), 1.f)));
     const uint64_t z = pair_of(z0, z1);
     float x0, x1;
     pair_to(mul2(mul2(z, both(-0.72134752044448170f)), z), x0, x1);   // log2(e) / 2
     e = pair_of(exp2_fast(x0), exp2_fast(x1));
-    uint64_t q = fma2(both(0.5f * 1.061405429f), t, both(0.5f * -1.453152027f));
-    q = fma2(q, t, both(0.5f * 1.421413741f));
-    q = fma2(q, t, both(0.5f * -0.284496736f));
-    q = fma2(q, t, both(0.5f * 0.254829592f));
+    uint64_t q = fma2(both(0.03468257764877231f), t, both(-0.15303787828018373f));
+    q = fma2(q, t, both(0.1991376515281999f));
+    q = fma2(q, t, both(-0.04702725808130784f));
+    q = fma2(q, t, both(0.12504815173945477f));
+    q = fma2(q, t, both(0.10096930636298611f));
+    q = fma2(q, t, both(0.12058744223124965f));
+    q = fma2(q, t, both(0.11963991150309353f));
     return mul2(mul2(q, t), e);
 }
 
@@ -370,9 +373,10 @@ template <int kAct> __device__ __forceinline__ void slope2(float& a, float& b) {
         const float x = max_nan(min_nan(a, 16.f), -16.f), y = max_nan(min_nan(b, 16.f), -16.f);
         uint64_t e;
         const uint64_t q = tail2(x, y, e);
-        float u, v;
-        pair_to(fma2(q, both(-1.f), both(0.5f)), u, v);   // 1/2 - Phi(-|z|), with the sign of z: Phi(z) - 1/2
-        const uint64_t p = add2(pair_of(copysignf(u, x), copysignf(v, y)), both(0.5f));
+        float q0, q1, p0, p1;
+        pair_to(q, q0, q1);
+        pair_to(fma2(q, both(-1.f), both(1.f)), p0, p1);
+        const uint64_t p = pair_of(x < 0.f ? q0 : p0, y < 0.f ? q1 : p1);   // Phi(z)
         pair_to(fma2(mul2(pair_of(x, y), both(0.39894228040143268f)), e, p), a, b);
     } else if (kAct == PLATTICE_ACT_SILU) {
         float x, y;

@@ -151,6 +151,30 @@ def test_float32_products_are_float32(dev, R, rows, n):
         assert abs(f64(gx)[0, 0] / e - 1) <= 4 * U and abs(f64(gw)[n - 1, 0] / float(a) ** 2 - 1) <= 4 * U
 
 
+@pytest.mark.parametrize("rows,n", FORMS)
+def test_gelu_in_float32(dev, R, rows, n):
+    """Relative to the value, into the tail: 15 u of the fit, the reciprocal and
+    the exponential, and u z^2 of the exponent's rounding."""
+    z = torch.linspace(-12.5, 12.5, rows * n).view(rows, n)
+    z[0, :4] = torch.tensor([0.0, -1e-6, 1e-6, -0.5])
+    w = torch.eye(n)
+    y, kept = R.linear(z.to(dev), w.to(dev), act="gelu", keep="full")
+    assert torch.equal(kept.cpu(), z)
+    ze = f64(z)
+    phi = np.vectorize(lambda t: 0.5 * math.erfc(-t / math.sqrt(2)))(ze)
+    tol = 2.0 ** -20 * (1 + ze * ze / 16) + 2 * U
+    assert worst(f64(y), ze * phi, tol * np.abs(ze * phi) + 1e-37) <= 1
+    for kept8 in (False, True):
+        zk = R.pack8(z.to(dev)) if kept8 else z.to(dev)
+        ze = f64(R.unpack8(zk)) if kept8 else f64(z)
+        phi = np.vectorize(lambda t: 0.5 * math.erfc(-t / math.sqrt(2)))(ze)
+        dens = ze * np.exp(-ze * ze / 2) / math.sqrt(2 * math.pi)
+        gx, _, _ = R.linear_backward(torch.ones(rows, n, device=dev), z.to(dev), w.to(dev), zk, act="gelu",
+                                     need=(True, False, False))
+        tol = 2.0 ** -20 * (1 + ze * ze / 16) + 2 * U
+        assert worst(f64(gx), phi + dens, tol * (phi + np.abs(dens)) + 1e-37) <= 1
+
+
 # ---------------------------------------------------------------- not finite
 
 def _same(got, want, tol):
