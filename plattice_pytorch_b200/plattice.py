@@ -207,10 +207,11 @@ class RowLinearFunction(Function):
     act(x weight^T + bias) + residual`` over ``x [..., k]``, gradients for the
     first four.  ``checkpoint8``: what the backward needs of the activations is
     kept in 8 bits (``x`` only where that is smaller: 33 bytes per 32 channels,
-    so not for a few channels of a 16-bit type, nor for float16 weights)."""
+    so not for a few channels of a 16-bit type, nor for float16 weights), else as
+    it is."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias, residual, act="none", checkpoint8=True):
+    def forward(ctx, x, weight, bias, residual, act="none", checkpoint8=False):
         y, z = rows.linear(x, weight, bias, act=act, residual=residual,
                            keep=None if act == "none" else "8bit" if checkpoint8 else "full")
         ctx.act, ctx.bias_dtype = act, None if bias is None else bias.dtype
@@ -240,9 +241,10 @@ class RowNormLinearFunction(Function):
     :func:`rows.linear`; gradients for the first five.  Returns ``y`` (with
     ``split`` its two tensors), followed by ``h`` when there is a residual.
 
-    ``checkpoint8``: the norm's result exists only in 8 bits, which the forward
-    and the backward both read, and the pre-activation is kept in 8 bits
-    (float16 rows keep both as they are)."""
+    ``checkpoint8`` (on by default: False for results without 8-bit roundings):
+    the norm's result exists only in 8 bits, which the forward and the backward
+    both read, and the pre-activation is kept in 8 bits (float16 rows keep both
+    as they are)."""
 
     @staticmethod
     def forward(ctx, x, residual, gain, weight, bias, eps=1e-6, act="none", split=0, out_dtype=None,
@@ -282,10 +284,11 @@ class PermutoLatticeLayer(Module):
 
     for ``x [H, W, channels]`` in the parameters' type (float32, bfloat16 or
     float16; the filter itself runs in float32).  ``pd`` features and ``vd``
-    values per pixel.  ``checkpoint8``: the norm's result and what the backward
-    needs of the projections are kept in 8 bits."""
+    values per pixel.  ``checkpoint8``: the norm's result, also as the forward
+    reads it, and what the backward needs of the projections are kept in 8 bits
+    (each off by at most 2^-4 of itself), else in the parameters' type."""
 
-    def __init__(self, channels, pd, vd, act="none", eps=1e-6, checkpoint8=True, dtype=torch.float32, device=None):
+    def __init__(self, channels, pd, vd, act="none", eps=1e-6, checkpoint8=False, dtype=torch.float32, device=None):
         super().__init__()
         PLOO._check_dims(pd, vd)
         PLOO._require(act in rows.ACTIVATIONS, f"act must be one of {', '.join(rows.ACTIVATIONS)}")

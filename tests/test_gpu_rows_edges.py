@@ -326,3 +326,46 @@ def test_channels_whose_byte_offsets_pass_32_bits(dev, R, dtype):
     y, _ = R.linear(x, w, out_dtype=torch.float32)
     e = f64(x[0, at]) * f64(w[0, at])
     assert abs(f64(y)[0, 0] - e.sum()) <= 2.0 ** -20 * abs(e).sum()   # six terms in float32
+
+
+# ---------------------------------------------------------------- under autograd
+
+@pytest.fixture
+def P():
+    import plattice_pytorch_b200 as P
+    return P
+
+
+def test_layer_is_float32_unless_asked(dev, P):
+    """What a layer computes is not rounded to 8 bits without a word of the caller."""
+    torch.manual_seed(5)
+    m = P.PermutoLatticeLayer(64, 5, 3, act="gelu", device=dev)
+    x = _randn((13, 29, 64), 32).to(dev)
+    with torch.no_grad():
+        n, _, _ = P.rows.rms_norm(x, m.gain)
+        (f, v), _ = P.rows.linear(n, m.w_in, m.b_in, split=5, out_dtype=torch.float32)
+        o = P.PermutoLatticeFeatureFunction.apply(f, v)
+        want = P.RowLinearFunction.apply(o, m.w_out, m.b_out, x, "gelu", False)
+        scale = float((want - x).abs().max())
+        assert float((m(x) - want).abs().max()) <= 1e-4 * scale   # atomics of the filter's splat
+    w = _randn((40, 64), 33).to(dev).requires_grad_(True)
+    gy = _randn((13, 29, 40), 34).to(dev)
+    P.RowLinearFunction.apply(x, w, None, None).backward(gy)
+    assert torch.equal(w.grad, P.rows.linear_backward(gy, x, w.detach())[1])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_layer_in_8_bits_when_asked(dev, P, dtype):
+    """checkpoint8=True is the chain of the Functions with it."""
+    t = DTYPES[dtype]
+    torch.manual_seed(6)
+    m = P.PermutoLatticeLayer(64, 5, 3, act="silu", checkpoint8=True, dtype=t, device=dev)
+    x = _randn((16, 24, 64), 35, t).to(dev).requires_grad_(True)
+    y = m(x)
+    f, v = P.RowNormLinearFunction.apply(x, None, m.gain, m.w_in, m.b_in, 1e-6, "none", 5, torch.float32, True)
+    o = P.PermutoLatticeFeatureFunction.apply(f, v)
+    want = P.RowLinearFunction.apply(o.to(t), m.w_out, m.b_out, x, "silu", True)
+    # the splat's atomics add in another order (1e-4 here), then a step of the type (at most 2^-7 of a value)
+    assert float((y - want).detach().float().abs().max()) <= 1e-4 + 2.0 ** -7 * float(want.detach().float().abs().max())
+    for g, p in zip(torch.autograd.grad(y.float().square().mean(), [x, *m.parameters()]), [x, *m.parameters()]):
+        assert g.shape == p.shape and g.dtype == p.dtype and bool(torch.isfinite(g).all()) and bool(g.any())
