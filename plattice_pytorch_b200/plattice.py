@@ -244,7 +244,8 @@ class RowNormLinearFunction(Function):
     ``checkpoint8`` (on by default: False for results without 8-bit roundings):
     the norm's result exists only in 8 bits, which the forward and the backward
     both read, and the pre-activation is kept in 8 bits (float16 rows keep both
-    as they are)."""
+    as they are).  ``x`` and ``weight`` then may be float32 and bfloat16 or the
+    other way; without, they have the same type."""
 
     @staticmethod
     def forward(ctx, x, residual, gain, weight, bias, eps=1e-6, act="none", split=0, out_dtype=None,
@@ -270,8 +271,8 @@ class RowNormLinearFunction(Function):
                                           bias_dtype=ctx.bias_dtype,
                                           need=(need[0] or need[1] or need[2], need[3], need[4]))
         gx = gg = None
-        if gn is not None:
-            gx, gg = rows.rms_norm_backward(gn, h, rstd, gain, gh)
+        if gn is not None:   # in the weight's type, which 8-bit rows leave open
+            gx, gg = rows.rms_norm_backward(gn.to(h.dtype), h, rstd, gain, gh)
         return (gx if need[0] else None, gx if need[1] else None, gg if need[2] else None, gw, gb,
                 None, None, None, None, None)
 

@@ -369,3 +369,26 @@ def test_layer_in_8_bits_when_asked(dev, P, dtype):
     assert float((y - want).detach().float().abs().max()) <= 1e-4 + 2.0 ** -7 * float(want.detach().float().abs().max())
     for g, p in zip(torch.autograd.grad(y.float().square().mean(), [x, *m.parameters()]), [x, *m.parameters()]):
         assert g.shape == p.shape and g.dtype == p.dtype and bool(torch.isfinite(g).all()) and bool(g.any())
+
+
+@pytest.mark.parametrize("xt,wt", [("fp32", "bf16"), ("bf16", "fp32")])
+@pytest.mark.parametrize("residual", [False, True])
+def test_norm_linear_of_mixed_types(dev, P, xt, wt, residual):
+    leaf = lambda s, i, t: _randn(s, i, DTYPES[t]).to(dev).requires_grad_(True)  # noqa: E731
+    x, gain, w, b = leaf((50, 64), 26, xt), leaf((64,), 27, xt), leaf((8, 64), 28, wt), leaf((8,), 29, wt)
+    r = leaf((50, 64), 30, xt) if residual else None
+    out = P.RowNormLinearFunction.apply(x, r, gain, w, b)
+    out = out if residual else (out,)
+    gs = [_randn(tuple(o.shape), 31 + i, o.dtype).to(dev) for i, o in enumerate(out)]
+    torch.autograd.backward(out, gs)
+    with torch.no_grad():
+        n, h, rstd = P.rows.rms_norm(x, gain, r, pack=True)
+        y, _ = P.rows.linear(n, w, b)
+        gn, gw, gb = P.rows.linear_backward(gs[0], n, w)
+        gx, gg = P.rows.rms_norm_backward(gn.to(x.dtype), h, rstd, gain, gs[1] if residual else None)
+    assert torch.equal(out[0], y)
+    for got, want in ((x.grad, gx), (gain.grad, gg), (w.grad, gw), (b.grad, gb)):
+        assert got.dtype == want.dtype and torch.equal(got, want)
+    assert r is None or torch.equal(r.grad, gx)
+    with pytest.raises(RuntimeError, match="same type"):
+        P.RowNormLinearFunction.apply(x, r, gain, w, b, 1e-6, "none", 0, None, False)
