@@ -353,8 +353,10 @@ def linear_backward(grad_y, x, weight, z=None, act="none", bias_dtype=None, need
     activation; ``x`` may be None when ``grad_weight`` is not wanted).  The
     gradient of the residual is ``grad_y`` itself."""
     pair = isinstance(grad_y, (tuple, list))
+    _require(not pair or (len(grad_y) == 2 and all(isinstance(g, torch.Tensor) for g in grad_y)),
+             "grad_y must be a tensor or a pair of tensors")
     cpp = _cpp()
-    if cpp is not None and act in ACTIVATIONS and x is not None and (not pair or len(grad_y) == 2):
+    if cpp is not None and act in ACTIVATIONS and x is not None:
         eight, z8 = type(x) is Rows8, type(z) is Rows8
         got = cpp.rows_linear_backward(
             *(grad_y if pair else (grad_y, None)), x.q if eight else x, x.scale if eight else None,
@@ -365,7 +367,6 @@ def linear_backward(grad_y, x, weight, z=None, act="none", bias_dtype=None, need
             if type(got) is int:
                 _raise("plattice_linear_backward", got, f"x={tuple(x.shape)} weight={tuple(weight.shape)}")
             return got
-    _require(not pair or len(grad_y) == 2, "grad_y must be a tensor or a pair of tensors")
     first = grad_y[0] if pair else grad_y
     _check_rows(first, "grad_y")
     _require(x is not None or not need[1], "x is needed for grad_weight")

@@ -328,6 +328,13 @@ def test_channels_whose_byte_offsets_pass_32_bits(dev, R, dtype):
     assert abs(f64(y)[0, 0] - e.sum()) <= 2.0 ** -20 * abs(e).sum()   # six terms in float32
 
 
+def test_half_a_pair_of_gradients_is_refused(dev, R):
+    x, w, g = torch.zeros(4, 8, device=dev), torch.zeros(3, 8, device=dev), torch.zeros(4, 3, device=dev)
+    for pair in ((g, None), [g, None], (None, g)):
+        with pytest.raises(RuntimeError, match="grad_y"):
+            R.linear_backward(pair, x, w)
+
+
 # ---------------------------------------------------------------- under autograd
 
 @pytest.fixture
