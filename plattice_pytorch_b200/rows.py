@@ -117,7 +117,7 @@ _CALLS = ("plattice_rows_pack8", "plattice_rows_unpack8", "plattice_rms_norm",
 def _cpp():
     """The torch extension's forms of the calls below (the same tests,
     allocations and library calls in one step), pointed at the loaded library;
-    None when the extension is not built.  They answer None to arguments that
+    None when the extension is not built, or from older sources.  They answer None to arguments that
     fail a test: the Python form then finds which and raises its message."""
     global _EXT
     if _EXT is _UNSET:
@@ -125,7 +125,7 @@ def _cpp():
             from . import _plattice_torch as m
             m.set_rows_entry_points([ctypes.cast(getattr(_lib.lib(), n), ctypes.c_void_p).value for n in _CALLS])
             _EXT = m
-        except ImportError:
+        except (ImportError, AttributeError):   # AttributeError: built before these calls
             _EXT = None
     return _EXT
 
