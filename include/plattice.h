@@ -285,7 +285,9 @@ const char* plattice_profile_stage_name(int stage);
 /* Row operators (no reference counterpart): what a network needs on either
  * side of the filter, where its features and values are learned.  A row is a
  * pixel's channels; tensors are [rows][channels], contiguous, on the current
- * device.  No call synchronises.
+ * device.  No call synchronises.  A bounded wait of a product that gives up is
+ * reported as any other call's failure (top of this file), captured calls'
+ * included.
  *
  * Element types.  Parameters (gain, bias) and their gradients may be of any of
  * the three types; the other tensors of a call are of `dtype`, but for a linear

@@ -240,15 +240,14 @@ int status_poll(const char** name, unsigned* seq) {
     return st;
 }
 
-unsigned* fault_word(cudaStream_t stream) {
+unsigned* fault_word() {
     Ring& r = ring();
     std::lock_guard<std::mutex> lk(r.mu);
     if (!r.fault_host && !r.fault_unavailable) {
-        cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
-        if (cudaStreamIsCapturing(stream, &capture) != cudaSuccess || capture != cudaStreamCaptureStatusNone) {
-            cudaGetLastError();
-            return nullptr;
-        }
+        // once per process, also when the first call is being captured: an
+        // allocation is not part of a capture and allowed in the relaxed mode
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        const bool relaxed = cudaThreadExchangeStreamCaptureMode(&mode) == cudaSuccess;
         void *p = nullptr, *d = nullptr;
         if (cudaHostAlloc(&p, sizeof(unsigned), cudaHostAllocPortable | cudaHostAllocMapped) != cudaSuccess ||
             cudaHostGetDevicePointer(&d, p, 0) != cudaSuccess || !d) {
@@ -260,6 +259,7 @@ unsigned* fault_word(cudaStream_t stream) {
             r.fault_host = static_cast<unsigned*>(p);
             r.fault_dev = static_cast<unsigned*>(d);
         }
+        if (relaxed) cudaThreadExchangeStreamCaptureMode(&mode);
     }
     return r.fault_dev;
 }

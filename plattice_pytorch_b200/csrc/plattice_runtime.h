@@ -46,9 +46,8 @@ StatusTicket status_ticket(const char* call);
 int status_poll(const char** name, unsigned* seq);
 
 // Device address of a pinned, mapped word that a kernel of a call without a
-// ticket sets to non-zero when a bounded wait of its own gives up (nullptr:
-// not available, or not yet and `stream` is being captured, where nothing may
-// be allocated); status_poll reports and clears it.
-unsigned* fault_word(cudaStream_t stream);
+// ticket sets to non-zero when a bounded wait of its own gives up (nullptr: not
+// available); status_poll reports and clears it.
+unsigned* fault_word();
 
 }  // namespace pl

@@ -687,7 +687,7 @@ static cudaError_t forward_mma(const plattice_linear_args* a, const ForwardPlan&
     const bool aligned = a->n % 8 == 0 && aligned16(a->y0) && (!a->residual || aligned16(a->residual)) &&
                          (!a->z || a->z_scale || aligned16(a->z));
     m.half = a->dtype == PLATTICE_F16;
-    m.fault = pl::fault_word(s);
+    m.fault = pl::fault_word();
     m.precise = true;
     m.scale = 1.f;
     sum_args(&m, a->k, 1, x.parts, w.parts);
@@ -757,7 +757,7 @@ static cudaError_t backward_mma(const plattice_linear_args* a, const BackwardPla
     MmaArgs m{};
     m.half = a->dtype == PLATTICE_F16 && parts == 1;
     m.scale = gz_halved(a) ? 2.f : 1.f;
-    m.fault = pl::fault_word(s);
+    m.fault = pl::fault_word();
     if (a->grad_x) {
         Operand w;
         e = operand(&w, a->w, a->dtype, parts, a->n, a->k, ws + p.w, s);

@@ -3,6 +3,8 @@ that are not finite or nearly infinite, float32's last bits, mixed types,
 largest sizes.  Definitions in float64 as in rows_reference.py; u = 2^-24 is
 half a float32 step."""
 import math
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -333,6 +335,32 @@ def test_half_a_pair_of_gradients_is_refused(dev, R):
     for pair in ((g, None), [g, None], (None, g)):
         with pytest.raises(RuntimeError, match="grad_y"):
             R.linear_backward(pair, x, w)
+
+
+_CAPTURED = """
+import ctypes, sys, torch
+from plattice_pytorch_b200 import _lib, rows
+word = ctypes.CDLL(_lib.LIB_PATH)._ZN2pl10fault_wordEv
+word.restype = ctypes.c_void_p
+x, w = torch.randn(512, 64, device="cuda"), torch.randn(72, 64, device="cuda")
+rows.pack8(x)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y, _ = rows.linear(x, w)
+    there = word()
+graph.replay()
+torch.cuda.synchronize()
+assert float((y - x.double() @ w.double().t()).abs().max()) < 1e-3
+assert there, "no word"
+"""
+
+
+def test_first_product_in_a_capture_can_report_a_fault(dev):
+    """A captured product whose waits give up has a place to say so, also when
+    no product ran before the capture."""
+    got = subprocess.run([sys.executable, "-c", _CAPTURED], capture_output=True, text=True, timeout=300)
+    assert got.returncode == 0, got.stderr[-2000:]
 
 
 # ---------------------------------------------------------------- under autograd
