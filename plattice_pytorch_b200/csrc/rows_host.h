@@ -43,6 +43,7 @@ struct MmaArgs {
     bool half;            // operands are float16 (else bfloat16)
     float scale;          // of a gradient's results, a power of two
     bool precise;         // the result ends in float32 (not in 16 bits after a float32 sum of parts)
+    long long patience;   // cycles that a wait may take
     unsigned* fault;      // host-mapped word that reports a wait that gave up (may be null)
 };
 

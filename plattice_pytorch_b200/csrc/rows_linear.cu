@@ -517,6 +517,8 @@ static void sum_args(MmaArgs* p, int64_t nr, int parts, int parts_a, int parts_b
         p->pairs_b |= (unsigned)j << (2 * p->pairs);
         ++p->pairs;
     });
+    // a slice takes 200 to 500 cycles, bound by memory up to some 2000
+    p->patience = 4000000000ll + 4096ll * p->part_steps * p->pairs;
 }
 
 // The 8-bit x as a bfloat16 operand in `ws`.

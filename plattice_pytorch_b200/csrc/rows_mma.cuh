@@ -100,22 +100,24 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, int parity) {
     return done != 0;
 }
 
-// Waits for the phase; false when another role has given up or the wait
-// itself does, after about two seconds of clock cycles.
-__device__ __forceinline__ bool bar_wait(uint32_t bar, int parity, volatile int* dead) {
+// Waits for the phase; false when another role has given up or the wait itself
+// does, after `patience` clock cycles: about two seconds, and more than a sum takes
+// as a whole (an accumulator is full when all of its slices are in: 2^24 of them
+// take three seconds).
+__device__ __forceinline__ bool bar_wait(uint32_t bar, int parity, long long patience, volatile int* dead) {
     if (bar_try(bar, parity)) return true;
     const long long begin = clock64();
-    for (int i = 0; i < (1 << 26); ++i) {
+    for (long long i = 0; i < patience; ++i) {   // a try takes a cycle at least
         if (bar_try(bar, parity)) return true;
-        if ((i & 15) == 15 && (*dead || clock64() - begin > 4000000000ll)) break;
+        if ((i & 15) == 15 && (*dead || clock64() - begin > patience)) break;
     }
     *dead = 1;
     return false;
 }
 
 // The same for all lanes of a warp, with one answer.
-__device__ __forceinline__ bool warp_wait(uint32_t bar, int parity, volatile int* dead) {
-    return __all_sync(0xffffffffu, bar_wait(bar, parity, dead));
+__device__ __forceinline__ bool warp_wait(uint32_t bar, int parity, long long patience, volatile int* dead) {
+    return __all_sync(0xffffffffu, bar_wait(bar, parity, patience, dead));
 }
 
 // One lane of a converged warp.
@@ -515,7 +517,7 @@ __global__ void __launch_bounds__(role_threads(kKind, kChunked), 1)
                 for (int pair = 0; pair < p.pairs; ++pair) {
                     const int za = (p.pairs_a >> (2 * pair)) & 3, zb = (p.pairs_b >> (2 * pair)) & 3;
                     for (int k = from; k < to; ++k) {
-                        if (!bar_wait(empty(s), phase ^ 1, dead)) goto copies_done;
+                        if (!bar_wait(empty(s), phase ^ 1, p.patience, dead)) goto copies_done;
                         const uint32_t a = ring + s * kStage, b = a + kStageA;
                         bar_expect(full(s), kStageA + b_columns(kKind, kBN) * kBK * 2);
                         if (a_mn(kKind)) {
@@ -562,7 +564,7 @@ __global__ void __launch_bounds__(role_threads(kKind, kChunked), 1)
             const Tile tile = tile_at<kBN>(p, t);
             for (int from = tile.begin; from < tile.end && going; ++n) {
                 const int to = kChunked ? min(tile.end, from + kChunk) : tile.end, buf = n & 1;
-                if (!warp_wait(acc_empty(buf), ((n >> 1) & 1) ^ 1, dead)) {
+                if (!warp_wait(acc_empty(buf), ((n >> 1) & 1) ^ 1, p.patience, dead)) {
                     going = false;
                     break;
                 }
@@ -571,7 +573,7 @@ __global__ void __launch_bounds__(role_threads(kKind, kChunked), 1)
                 const int count = p.pairs * (to - from);
                 from = to;
                 for (int k = 0; k < count; ++k) {
-                    if (!warp_wait(full(s), phase, dead)) {
+                    if (!warp_wait(full(s), phase, p.patience, dead)) {
                         going = false;
                         break;
                     }
@@ -615,7 +617,7 @@ __global__ void __launch_bounds__(role_threads(kKind, kChunked), 1)
                 bool given_up = false;
                 for (int from = tile.begin; from < tile.end; from += kChunk, ++n) {
                     const int buf = n & 1;
-                    if (!warp_wait(acc_full(buf), (n >> 1) & 1, dead)) {
+                    if (!warp_wait(acc_full(buf), (n >> 1) & 1, p.patience, dead)) {
                         given_up = true;
                         break;
                     }
@@ -674,7 +676,7 @@ __global__ void __launch_bounds__(role_threads(kKind, kChunked), 1)
             ahead.have = false;
             bias_ahead(group);
             if (kKeeps && kMode == kAligned && group < kPieces) load_ahead<kOut>(ahead, p, row0, tile.j0 + group * 32, lane);
-            if (!warp_wait(acc_full(buf), (n >> 1) & 1, dead)) break;
+            if (!warp_wait(acc_full(buf), (n >> 1) & 1, p.patience, dead)) break;
             fence_after();
             const uint32_t base = tmem + buf * kBN + ((uint32_t)(quarter * 32) << 16);
 #pragma unroll 1

@@ -330,6 +330,24 @@ def test_channels_whose_byte_offsets_pass_32_bits(dev, R, dtype):
     assert abs(f64(y)[0, 0] - e.sum()) <= 2.0 ** -20 * abs(e).sum()   # six terms in float32
 
 
+def test_sum_that_takes_seconds(dev, R):
+    """An input gradient over 2^30 output channels: one tile of 2^24 slices,
+    longer than a wait that does not know its sum would have patience for."""
+    n, k = 1 << 30, 8
+    if torch.cuda.mem_get_info(dev)[0] < 32 << 30:
+        pytest.skip("needs 32 GB of free device memory")
+    w, gy = torch.zeros(n, k, dtype=torch.bfloat16, device=dev), torch.zeros(1, n, dtype=torch.bfloat16, device=dev)
+    at = [0, 12345, n // 2 + 7, n - 65, n - 1]
+    w[at] = _randn((5, k), 52, torch.bfloat16).to(dev)
+    gy[0, at] = _randn((5,), 53, torch.bfloat16).to(dev)
+    x = torch.zeros(1, k, dtype=torch.bfloat16, device=dev)
+    gx, _, _ = R.linear_backward(gy, x, w, need=(True, False, False))
+    e = f64(gy[0, at]) @ f64(w[at])
+    assert worst(f64(gx)[0], e, (2.0 ** -8 + 2.0 ** -20) * (np.abs(f64(gy[0, at])) @ np.abs(f64(w[at])))) <= 1
+    torch.cuda.synchronize()
+    R.linear_backward(gy[:, :64].contiguous(), x, w[:64], need=(True, False, False))   # would report it
+
+
 def test_half_a_pair_of_gradients_is_refused(dev, R):
     x, w, g = torch.zeros(4, 8, device=dev), torch.zeros(3, 8, device=dev), torch.zeros(4, 3, device=dev)
     for pair in ((g, None), [g, None], (None, g)):
