@@ -227,7 +227,7 @@ __device__ __forceinline__ float finite_amax(float (&v)[N]) {
 }
 
 // The same of values that must stay: infinities are passed over in amax and
-// codes8_of gives them the NaN code.
+// codes_of gives them the NaN code.
 template <int N>
 __device__ __forceinline__ float finite_amax_of(const float (&v)[N], bool& infinite) {
     float amax = 0.f;
@@ -252,15 +252,8 @@ __device__ __forceinline__ float held8(float v) {
 
 // Codes of 8 values, finite or NaN, times 2^-s (multiplying by a power of two
 // is exact, so the one rounding is the conversion's).
-__device__ __forceinline__ uint2 codes8(const float* values, float inv) {
+__device__ __forceinline__ uint2 codes8_below(const float* v, float inv) {   // below the largest scale
     unsigned w[2];
-    float v[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = values[i];
-    if (largest_scale(inv)) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = held8(v[i]);
-    }
     const uint64_t m = both(inv);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -273,12 +266,29 @@ __device__ __forceinline__ uint2 codes8(const float* values, float inv) {
     return make_uint2(w[0], w[1]);
 }
 
-__device__ __forceinline__ uint2 codes8_of(const float* v, float inv, bool infinite) {
-    if (!infinite) return codes8(v, inv);
+__device__ __forceinline__ uint2 codes8(const float* v, float inv) {
+    if (!largest_scale(inv)) return codes8_below(v, inv);
     float t[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) t[i] = is_infinite(fabsf(v[i])) ? __int_as_float(0x7fffffff) : v[i];
-    return codes8(t, inv);
+    for (int i = 0; i < 8; ++i) t[i] = held8(v[i]);
+    return codes8_below(t, inv);
+}
+
+// Codes of 8 N values that must stay.
+template <int N>
+__device__ __forceinline__ void codes_of(uint2 (&q)[N], const float* v, float inv, bool infinite) {
+    if (!infinite && !largest_scale(inv)) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) q[i] = codes8_below(v + 8 * i, inv);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        float t[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) t[j] = is_infinite(fabsf(v[8 * i + j])) ? __int_as_float(0x7fffffff) : v[8 * i + j];
+        q[i] = codes8(t, inv);
+    }
 }
 
 __device__ __forceinline__ void values4(float* v, unsigned codes, float scale) {

@@ -383,8 +383,7 @@ __device__ __forceinline__ void keep_codes(const float (&v)[32], const MmaArgs& 
     if (row >= p.ni) return;
     const float inv = pow2(-e);
     uint2 q[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) q[i] = codes8_of(v + 8 * i, inv, infinite);
+    codes_of(q, v, inv, infinite);
     const int64_t at = row * ((p.nj + 31) / 32) + (col0 >> 5);
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(static_cast<uint8_t*>(p.z) + at * 32),
                  "r"(q[0].x), "r"(q[0].y), "r"(q[1].x), "r"(q[1].y), "r"(q[2].x), "r"(q[2].y), "r"(q[3].x), "r"(q[3].y)

@@ -581,8 +581,9 @@ __global__ void __launch_bounds__(32 * kNarrowWarps, narrow_ctas(kXT, kNF)) k_na
                 const int e = block_exponent(amax);
                 if (r < rows) {
                     const float inv = pow2(-e);
-                    const uint2 x = codes8_of(v, inv, infinite), y = codes8_of(v + 8, inv, infinite);
-                    reinterpret_cast<uint4*>(a.z)[(row0 + r) * 2 + (lane & 1)] = make_uint4(x.x, x.y, y.x, y.y);
+                    uint2 q[2];
+                    codes_of(q, v, inv, infinite);
+                    reinterpret_cast<uint4*>(a.z)[(row0 + r) * 2 + (lane & 1)] = make_uint4(q[0].x, q[0].y, q[1].x, q[1].y);
                     if ((lane & 1) == 0) a.z_scale[row0 + r] = (uint8_t)(e + 127);
                 }
             }
@@ -1137,7 +1138,9 @@ __global__ void __launch_bounds__(64 * few_splits(kWT)) k_few(const SmallArgs a)
         const int e = block_exponent(amax);
         const float v[8] = {z, 0, 0, 0, 0, 0, 0, 0};
         const int64_t at = row * ((a.n + 31) / 32) + blockIdx.x;
-        static_cast<uint8_t*>(a.z)[at * 32 + lane] = (uint8_t)codes8_of(v, pow2(-e), is_infinite(fabsf(z))).x;
+        uint2 q[1];
+        codes_of(q, v, pow2(-e), is_infinite(fabsf(z)));
+        static_cast<uint8_t*>(a.z)[at * 32 + lane] = (uint8_t)q[0].x;
         if (lane == 0) a.z_scale[at] = (uint8_t)(e + 127);
     } else if (a.z && have) {
         store_param(a.z, a.out_dtype, row * a.n + c, z);
