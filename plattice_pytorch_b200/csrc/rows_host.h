@@ -50,9 +50,16 @@ struct MmaArgs {
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline int64_t mma_tiles(int64_t ni, int64_t nj, int bn) { return ceil_div(ni, kBM) * ceil_div(nj, bn); }
 
+// The deepest sum that an accumulator takes for a 16-bit result.  The MMA cuts
+// where an addition rounds: sums of like terms drift by up to 2^-23 with each 16
+// (float16, whose products have 22 bits, 1.0e-4 at a depth of 16384 and 8.7e-4 at a
+// million; bfloat16's of 16 bits drift from some thousand on).  Held to a quarter of
+// half a step of the type.
+inline int64_t deepest_sum(int dtype) { return dtype == PLATTICE_F16 ? 16384 : 131072; }
+
 // Whether a sum of `steps` slices goes in chunks (rows_mma.cuh, kChunk).
 inline bool chunked(int steps, int out_dtype, bool precise) {
-    return precise && out_dtype == PLATTICE_F32 && steps > 8;
+    return precise && (out_dtype == PLATTICE_F32 ? steps > 8 : (int64_t)steps * kBK > deepest_sum(out_dtype));
 }
 
 // TMA map of an operand: boxes of 64 columns x box_rows rows, zeros outside.

@@ -463,12 +463,13 @@ static int choose_bn(int64_t ni, int64_t nj, int least, bool deep) {
 // Parts of kGradW's sum: the cheapest of rounds over the SMs, where a part
 // costs its slices and some 6 more for filling and emptying the accumulator,
 // plus writing and adding the partial results (8 bytes an element, about
-// 3 bytes a cycle and SM).
-static int choose_parts(int64_t ni, int64_t nj, int bn, int64_t steps) {
+// 3 bytes a cycle and SM).  `deepest`: rows that a part may have.
+static int choose_parts(int64_t ni, int64_t nj, int bn, int64_t steps, int64_t deepest) {
     const int64_t tiles = mma_tiles(ni, nj, bn);
-    int best = 1;
+    const int least = (int)ceil_div(steps * kBK, deepest), most = least > 256 ? least : 256;
+    int best = least;
     double cost = 1e300;
-    for (int p = 1; p <= 256 && p <= steps; ++p) {
+    for (int p = least; p <= most && p <= steps; ++p) {
         const double rounds = (double)ceil_div(tiles * p, sm_count());
         double c = rounds * (double)(ceil_div(steps, p) + 6) * slice_cost(bn);
         if (p > 1) c += (double)p * ni * nj * 8 / (3.0 * 8 * sm_count());
@@ -629,7 +630,8 @@ static BackwardPlan backward_plan(const plattice_linear_args* a) {
     if (p.gz_needed) p.gz = c.take(repack_bytes(gz_parts(a), a->rows, a->n));
     p.bn_x = choose_bn(a->rows, a->k, 64, chunked((int)ceil_div(a->n, kBK), a->dtype, true));
     p.bn_w = choose_bn_w(a);
-    p.parts_w = choose_parts(a->k, a->n, p.bn_w, ceil_div(a->rows, kBK));
+    p.parts_w = choose_parts(a->k, a->n, p.bn_w, ceil_div(a->rows, kBK),
+                             a->dtype == PLATTICE_F32 ? INT_MAX : deepest_sum(a->dtype));   // float32: in chunks
     const int parts = tiled_parts(a);
     if (a->grad_x && (parts > 1 || !tma_ready(a->w, a->dtype, a->k))) p.w = c.take(repack_bytes(parts, a->n, a->k));
     if (a->grad_w && a->x_scale) p.x = c.take(a->rows * up8(a->k) * 2);

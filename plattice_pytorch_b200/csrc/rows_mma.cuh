@@ -50,9 +50,10 @@ enum Mode { kAny = 0, kAligned = 1, kPlain = 2 };
 __host__ __device__ constexpr int epilogue_warps(int kind, bool chunked) { return kind == 0 || chunked ? 16 : 8; }
 __host__ __device__ constexpr int role_threads(int kind, bool chunked) { return 64 + 32 * epilogue_warps(kind, chunked); }
 
-// A float32 result of a deep sum (kChunked): the MMA cuts where an addition
+// A float32 result of a deep sum (kChunked; a 16-bit one of a far deeper): the MMA cuts where an addition
 // rounds, so that an accumulator drifts by about 2^-26 of itself with each of
-// them (1.1e-6 of the result at a depth of 1024, 4.5e-6 at 4096).  The sum then
+// them, terms of both signs (1.1e-6 of the result at a depth of 1024, 4.5e-6 at
+// 4096; float16 terms of one sign: 2^-23).  The sum then
 // goes in chunks of kChunk slices through the two accumulators, and the
 // epilogue adds those in registers, rounding; a warp holds one 32-column
 // piece, so tiles are at most 128 wide.
@@ -743,7 +744,7 @@ cudaError_t launch_mma(const Operand& a, const Operand& b, const MmaArgs& p, cud
     return cudaGetLastError();
 }
 
-// kDeep: float32 results, whose deep sums go in chunks.
+// kDeep: results whose deep sums go in chunks.
 template <int kKind, int kOut, int kMode, bool kDeep>
 cudaError_t launch_bn(int bn, const Operand& a, const Operand& b, const MmaArgs& p, cudaStream_t s) {
     if constexpr (kDeep) {

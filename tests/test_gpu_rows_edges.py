@@ -348,6 +348,40 @@ def test_sum_that_takes_seconds(dev, R):
     R.linear_backward(gy[:, :64].contiguous(), x, w[:64], need=(True, False, False))   # would report it
 
 
+def test_weight_gradient_of_a_million_like_rows(dev, R):
+    """Sums of like terms in float16: one rounding, and a step of float32 cut for
+    each 16 of the at most 16384 rows that the matrix instructions add up."""
+    rows, k, n, t = 1 << 20, 4096, 1024, torch.float16
+    if torch.cuda.mem_get_info(dev)[0] < 32 << 30:
+        pytest.skip("needs 32 GB of free device memory")
+    g = torch.Generator().manual_seed(54)
+    part = lambda m, bits: (1 + torch.randint(0, 1 << bits, (m,), generator=g) * 2.0 ** -bits).to(t).to(dev)  # noqa: E731
+    a, b, h, c = part(rows, 4), part(k, 4), part(rows, 4), part(n, 4) / 256   # 5 bits each; sums below 65504
+    _, gw, _ = R.linear_backward(h[:, None] * c, a[:, None] * b, torch.zeros(n, k, dtype=t, device=dev), need=(False, True, False))
+    e = (a.double() * h.double()).sum() * c.double()[:, None] * b.double()   # products of 10 bits: exact in float16
+    assert float((gw.double() / e - 1).abs().max()) <= 2.0 ** -11 + 16384 / 16 * 2.0 ** -23 + 70 * U
+
+
+@pytest.mark.parametrize("dtype,deep", [("fp16", 1 << 17), ("bf16", 1 << 20)])
+def test_deep_sums_of_like_terms(dev, R, dtype, deep):
+    """The same over input and output channels: one rounding, and at most a step of
+    float32 cut for each 16 of a chunk of 512, which then are added in float32."""
+    t = DTYPES[dtype]
+    g = torch.Generator().manual_seed(55)
+    part = lambda m: (1 + torch.randint(0, 8, (m,), generator=g) / 8).to(t).to(dev)  # noqa: E731  4 bits
+    bound = half_step(t) + 32 * 2.0 ** -23 + deep / 512 * U
+    b, d = part(deep) / 16, part(deep) / 16
+    total = (b.double() * d.double()).sum()
+    for rows, n in ((400, 200), (5000, 40)):
+        a, c = part(rows), part(n)
+        y, _ = R.linear(a[:, None] * b, c[:, None] * d)
+        assert float((y.double() / (a.double()[:, None] * c.double() * total) - 1).abs().max()) <= bound
+    a, c = part(200), part(64)
+    gx, _, _ = R.linear_backward(a[:, None] * b, torch.zeros(200, 64, dtype=t, device=dev), d[:, None] * c,
+                                 need=(True, False, False))
+    assert float((gx.double() / (a.double()[:, None] * c.double() * total) - 1).abs().max()) <= bound
+
+
 def test_half_a_pair_of_gradients_is_refused(dev, R):
     x, w, g = torch.zeros(4, 8, device=dev), torch.zeros(3, 8, device=dev), torch.zeros(4, 3, device=dev)
     for pair in ((g, None), [g, None], (None, g)):
