@@ -380,13 +380,9 @@ static bool gz_halved(const plattice_linear_args* a) {
     return a->dtype == PLATTICE_F16 && a->act != PLATTICE_ACT_NONE && gz_parts(a) == 1;
 }
 
-// Parts of w, and of an x that is not in 8 bits: in the forward, in the tiled
-// backward, and in the one of a single pass (NarrowGradShape).
+// Parts of w, and of an x that is not in 8 bits.
 static int forward_parts(const plattice_linear_args* a) { return a->dtype == PLATTICE_F32 ? 3 : 1; }
-static int tiled_parts(const plattice_linear_args* a) { return a->dtype == PLATTICE_BF16 ? 1 : gz_parts(a); }
-static int pass_parts(const plattice_linear_args* a) {
-    return a->dtype == PLATTICE_F16 && a->act != PLATTICE_ACT_NONE ? 2 : tiled_parts(a);
-}
+static int backward_parts(const plattice_linear_args* a) { return a->dtype == PLATTICE_BF16 ? 1 : gz_parts(a); }
 
 static int64_t repack_bytes(int parts, int64_t rows, int64_t width) { return rows * up8(width) * 2 * parts; }
 
@@ -500,7 +496,7 @@ static int product_count(int parts_a, int parts_b) {
 static int choose_bn_w(const plattice_linear_args* a) {
     const bool deep = a->dtype == PLATTICE_F32 && a->rows > 8 * kBK;   // chunks, or parts no deeper than one
     const int widest = a->n > 128 && !deep ? 256 : a->n > 64 ? 128 : 64;
-    if (ceil_div(a->rows, kBK) * product_count(a->x_scale ? 1 : tiled_parts(a), gz_parts(a)) > 16) return widest;
+    if (ceil_div(a->rows, kBK) * product_count(a->x_scale ? 1 : backward_parts(a), gz_parts(a)) > 16) return widest;
     int bn = 64;
     while (bn < widest && mma_tiles(a->k, a->n, bn) > sm_count()) bn *= 2;
     return bn;
@@ -611,7 +607,7 @@ static BackwardPlan backward_plan(const plattice_linear_args* a) {
     if (p.narrow) {
         // one round of CTAs over the slices of 64 channels
         const int64_t slices = ceil_div(a->k, 64), need = ceil_div(ceil_div(a->rows, 16), kGradWarps);
-        const int64_t most = ceil_div(narrow_grad_ctas(pass_parts(a), (a->n + 7) / 8) * (int64_t)sm_count(), slices);
+        const int64_t most = ceil_div(narrow_grad_ctas(backward_parts(a), (a->n + 7) / 8) * (int64_t)sm_count(), slices);
         p.lines = (int)(need < most ? (need < 1 ? 1 : need) : most);
         p.partial_w = c.take((int64_t)p.lines * ((int64_t)a->n * a->k + a->n) * 4);
         p.bytes = c.at;
@@ -632,7 +628,7 @@ static BackwardPlan backward_plan(const plattice_linear_args* a) {
     p.bn_w = choose_bn_w(a);
     p.parts_w = choose_parts(a->k, a->n, p.bn_w, ceil_div(a->rows, kBK),
                              a->dtype == PLATTICE_F32 ? INT_MAX : deepest_sum(a->dtype));   // float32: in chunks
-    const int parts = tiled_parts(a);
+    const int parts = backward_parts(a);
     if (a->grad_x && (parts > 1 || !tma_ready(a->w, a->dtype, a->k))) p.w = c.take(repack_bytes(parts, a->n, a->k));
     if (a->grad_w && a->x_scale) p.x = c.take(a->rows * up8(a->k) * 2);
     if (a->grad_w && !a->x_scale && (parts > 1 || !tma_ready(a->x, a->dtype, a->k)))
@@ -724,7 +720,7 @@ static cudaError_t backward_narrow(const plattice_linear_args* a, const Backward
     g.need_b = a->grad_bias != nullptr;
     g.vec_gx = a->k % 8 == 0 && aligned16(a->grad_x);
     g.vec_g = aligned16(a->grad0) && (!a->split || aligned16(a->grad1));
-    const cudaError_t e = run_narrow_grad(g, a->dtype, pass_parts(a), p.lines, s);
+    const cudaError_t e = run_narrow_grad(g, a->dtype, backward_parts(a), p.lines, s);
     if (e != cudaSuccess || !(a->grad_w || a->grad_bias)) return e;
     const int64_t nw = (int64_t)a->n * a->k, columns = nw + a->n;
     k_sum_lines<<<(unsigned)ceil_div(columns, 32), 1024, 0, s>>>(a->grad_w, a->dtype, nw, a->grad_bias, a->bias_dtype, a->n,
@@ -756,7 +752,7 @@ static cudaError_t grad_z(const plattice_linear_args* a, const BackwardPlan& p, 
 static cudaError_t backward_mma(const plattice_linear_args* a, const BackwardPlan& p, cudaStream_t s) {
     char* ws = static_cast<char*>(a->workspace);
     const Operand gz{p.gz_needed ? ws + p.gz : a->grad0, a->rows, a->n, p.gz_needed ? p.pitch : a->n, gz_parts(a)};
-    const int parts = tiled_parts(a);
+    const int parts = backward_parts(a);
     cudaError_t e = cudaSuccess;
     MmaArgs m{};
     m.half = a->dtype == PLATTICE_F16 && parts == 1;

@@ -632,32 +632,38 @@ constexpr int kTilePitch = 72;   // 16-bit elements: rows 144 bytes apart, no ba
 
 // kParts: of the weights: 3 with float32 ones, 1 or 2 with 16-bit ones.
 //
-// gz = grad_y act'(z) is made here in float32.  float16 holds only a small part of
-// what that can be (gradients of 1e-8 or 1e6, float16's largest times a slope above
-// 1), so float16 operands run as two bfloat16 parts each (exact; gz's two hold 16
-// bits), three products, unless the gradients are float16 themselves and there is
-// no activation: then gz is one float16 part, as it came.  Beside bfloat16 operands
-// gz has two parts, too: 28 more matrix instructions a block of rows, 8 % of the
-// pass, keep what rounding it to one would add to both gradients' errors.
+// gz = grad_y act'(z) is made here in float32 and has two parts beside 16-bit
+// operands: 28 more matrix instructions a block of rows, 8 % of the pass, keep what
+// rounding it to one would add to both gradients' errors.  float16 holds only a
+// small part of what gz can be:
+// * behind float32 gradients (of 1e-8 or 1e6) float16 operands run as two bfloat16
+//   parts each (kParts 2, exact; gz's two hold 16 bits), three products;
+// * a float16 gradient is one float16 part as it came, or behind an activation two
+//   of half of gz (a slope of up to 1.13 can take it past the type), the results
+//   doubled.
 template <int kXT, int kParts> struct NarrowGradShape {
     static constexpr bool kHalf = kXT == kXHalf && kParts == 1;                       // float16 matrix instructions
     static constexpr int kPX = kXT == kXFloat ? 3 : kParts == 2 ? 2 : 1;
-    static constexpr int kPZ = kHalf ? 1 : kParts == 3 ? 3 : 2;
+    static constexpr int kPZ = kParts == 3 ? 3 : 2;
     static constexpr int kFragBytes = kParts * 2 * 8 * 32 * 8;                        // weights of the slice
     static constexpr int kStaged = 16 * kNarrowPitch + 4;   // gz of 16 rows, and a place for what is behind them
     static constexpr int kWarpBytes = kStaged * 4 + kPX * 16 * kTilePitch * 2;
     static constexpr int kBytes = kFragBytes + kGradWarps * kWarpBytes + 64 * 33 * 4;
 };
 
-// a and b as kP packed parts, bfloat16 or a float16.  kAny: they may not be finite;
-// kLone: they meet operands of a single part.
+// a and b as kP packed parts, bfloat16 or float16 (rounded).  kAny: they may not be
+// finite (float16: one part then); kLone: they meet operands of a single part.
 template <int kP, bool kHalf, bool kAny, bool kLone = false>
 __device__ __forceinline__ void to_parts(float a, float b, uint32_t (&o)[kP]) {
     if constexpr (kHalf) {
-        static_assert(kP == 1, "float16 operands of one part");
-        union { __half2 h; uint32_t u; } x;
-        x.h = __floats2half2_rn(a, b);
-        o[0] = x.u;
+#pragma unroll
+        for (int i = 0; i < kP; ++i) {
+            union { __half2 h; uint32_t u; } x;
+            x.h = __floats2half2_rn(a, b);
+            o[i] = x.u;
+            a -= __low2float(x.h);
+            b -= __high2float(x.h);
+        }
     } else if constexpr (kLone && kP == 2) {
         split_one_sign<kAny>(a, b, o);
     } else if constexpr (kAny) {
@@ -691,6 +697,7 @@ __global__ void __launch_bounds__(32 * kGradWarps, narrow_grad_ctas(kParts, kNF)
 
     // fragment f, column c of the weights is channel (c >> 1) 16 + 2 f + (c & 1)
     // of the slice, so that a lane ends up with 16 neighbouring channels
+    bool odd = false;   // float16: weights that are not finite
     if (a.need_x) {
         typedef typename WeightType<kXT, kParts == 3>::type TW;
         const TW* weights = static_cast<const TW*>(a.s.w);
@@ -702,6 +709,9 @@ __global__ void __launch_bounds__(32 * kGradWarps, narrow_grad_ctas(kParts, kNF)
             for (int j = 0; j < 4; ++j)
                 v[j] = o + j < n && ch < k ? to_f32(weights[(int64_t)(o + j) * k + ch]) : 0.f;
             uint32_t lo[kParts], hi[kParts];
+            if (kHalf)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) odd |= !(fabsf(v[j]) < INFINITY);
             to_parts<kParts, kHalf, true>(v[0], v[1], lo);
             to_parts<kParts, kHalf, true>(v[2], v[3], hi);
 #pragma unroll
@@ -709,7 +719,11 @@ __global__ void __launch_bounds__(32 * kGradWarps, narrow_grad_ctas(kParts, kNF)
         }
     }
     for (int i = lane; i < 16 * kNarrowPitch; i += 32) st[i] = 0.f;   // columns behind n stay 0
-    __syncthreads();
+    // float16: one part of gz where it is a gradient as it came, or meets what is
+    // not finite (a second part of 0 would make NaN of it)
+    const bool single = kHalf && (__syncthreads_or(odd) || !a.s.z);
+    if (!kHalf) __syncthreads();
+    const float down = kHalf && a.s.z ? 0.5f : 1.f, up = kHalf && a.s.z ? 2.f : 1.f;
 
     float dw[4][kNF][4];
 #pragma unroll
@@ -777,6 +791,7 @@ __global__ void __launch_bounds__(32 * kGradWarps, narrow_grad_ctas(kParts, kNF)
 #pragma unroll
             for (int i = 0; i < kRun; ++i) st[place[i]] = place[i] < rows * kNarrowPitch ? to_f32(gn.e[i]) : 0.f;
         }
+        odd = false;
         if (a.need_w) {   // x, widened, into the tile
             narrow_mask<kXT, 1>(xn, k, blockIdx.y, lane);
 #pragma unroll
@@ -838,6 +853,13 @@ __global__ void __launch_bounds__(32 * kGradWarps, narrow_grad_ctas(kParts, kNF)
                 } else {
                     reinterpret_cast<uint4*>(row)[0] = xn.v[0][h][0];
                     reinterpret_cast<uint4*>(row)[1] = xn.v[0][h][1 % NarrowShape<kXT>::kRaw];
+                    if (kHalf && !single) {
+                        const __half2* q = reinterpret_cast<const __half2*>(row);   // its own 16 again
+                        __half2 w = __float2half2_rn(0.f);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) w = __hfma2(q[i], __float2half2_rn(0.f), w);
+                        odd |= !(__low2float(w) + __high2float(w) == 0.f);
+                    }
                 }
             }
         }
@@ -879,18 +901,20 @@ __global__ void __launch_bounds__(32 * kGradWarps, narrow_grad_ctas(kParts, kNF)
             db += part;
         }
         auto products = [&](auto any) {
+            constexpr bool kAny = decltype(any)::value;
+            constexpr int kZ = kHalf && kAny ? 1 : kPZ;
             if (a.need_x) {
-                uint32_t o[kKS][kPZ][4];
+                uint32_t o[kKS][kZ][4];
 #pragma unroll
                 for (int s = 0; s < kKS; ++s)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const float* p = st + (g + 8 * h) * kNarrowPitch + t * cols_per_lane + s * 4;
-                        uint32_t lo[kPZ], hi[kPZ];
-                        to_parts<kPZ, kHalf, decltype(any)::value, kPX == 1 && kParts == 1>(p[0], p[1], lo);
-                        to_parts<kPZ, kHalf, decltype(any)::value, kPX == 1 && kParts == 1>(p[2], p[3], hi);
+                        uint32_t lo[kZ], hi[kZ];
+                        to_parts<kZ, kHalf, kAny, kPX == 1 && kParts == 1>(p[0] * down, p[1] * down, lo);
+                        to_parts<kZ, kHalf, kAny, kPX == 1 && kParts == 1>(p[2] * down, p[3] * down, hi);
 #pragma unroll
-                        for (int q = 0; q < kPZ; ++q) {
+                        for (int q = 0; q < kZ; ++q) {
                             o[s][q][h] = lo[q];
                             o[s][q][2 + h] = hi[q];
                         }
@@ -901,9 +925,9 @@ __global__ void __launch_bounds__(32 * kGradWarps, narrow_grad_ctas(kParts, kNF)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) dx[f][i] = 0.f;
 #pragma unroll
-                    for (int sum = kPZ - 1; sum >= 0; --sum)   // small products first
+                    for (int sum = kZ - 1; sum >= 0; --sum)   // small products first
 #pragma unroll
-                        for (int pa = 0; pa < kPZ; ++pa) {
+                        for (int pa = 0; pa < kZ; ++pa) {
                             const int pb = sum - pa;
                             if (pb < 0 || pb >= kParts) continue;
 #pragma unroll
@@ -921,7 +945,7 @@ __global__ void __launch_bounds__(32 * kGradWarps, narrow_grad_ctas(kParts, kNF)
                         if (left <= 0) continue;
                         float v[8];
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) v[i] = dx[q * 4 + (i >> 1)][h * 2 + (i & 1)];
+                        for (int i = 0; i < 8; ++i) v[i] = dx[q * 4 + (i >> 1)][h * 2 + (i & 1)] * up;
                         const int64_t at = (row0 + g + 8 * h) * k + ch;
                         const bool vec = a.vec_gx && left >= 8;
                         if (kXT == kXHalf) store8(static_cast<__half*>(a.grad_x) + at, v, vec, left);
@@ -931,16 +955,16 @@ __global__ void __launch_bounds__(32 * kGradWarps, narrow_grad_ctas(kParts, kNF)
                 }
             }
             if (a.need_w) {
-                uint32_t b[kPZ][kNF][2];
+                uint32_t b[kZ][kNF][2];
 #pragma unroll
                 for (int f = 0; f < kNF; ++f)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const float* p = st + (2 * t + 8 * h) * kNarrowPitch + f * 8 + g;
-                        uint32_t o[kPZ];
-                        to_parts<kPZ, kHalf, decltype(any)::value, kPX == 1 && kParts == 1>(p[0], p[kNarrowPitch], o);
+                        uint32_t o[kZ];
+                        to_parts<kZ, kHalf, kAny, kPX == 1 && kParts == 1>(p[0] * down, p[kNarrowPitch] * down, o);
 #pragma unroll
-                        for (int q = 0; q < kPZ; ++q) b[q][f][h] = o[q];
+                        for (int q = 0; q < kZ; ++q) b[q][f][h] = o[q];
                     }
 #pragma unroll
                 for (int m = 0; m < 4; ++m) {
@@ -963,11 +987,11 @@ __global__ void __launch_bounds__(32 * kGradWarps, narrow_grad_ctas(kParts, kNF)
                             for (int i = 0; i < 4; ++i) rows16[f][i] = 0.f;
                     }
 #pragma unroll
-                    for (int sum = kPZ - 1; sum >= 0; --sum)
+                    for (int sum = kZ - 1; sum >= 0; --sum)
 #pragma unroll
                         for (int px = 0; px < kPX; ++px) {
                             const int pb = sum - px;
-                            if (pb < 0 || pb >= kPZ) continue;
+                            if (pb < 0 || pb > kZ - 1) continue;
 #pragma unroll
                             for (int f = 0; f < kNF; ++f)
                                 mma16816<kHalf>(kParts == 3 ? rows16[f] : dw[m][f], x[px][0], x[px][1], x[px][2], x[px][3],
@@ -983,7 +1007,7 @@ __global__ void __launch_bounds__(32 * kGradWarps, narrow_grad_ctas(kParts, kNF)
                 }
             }
         };
-        if (!__any_sync(0xffffffffu, !(fabsf(column) < INFINITY))) products(Fixed<false>());
+        if (!single && !__any_sync(0xffffffffu, odd || !(fabsf(column) < INFINITY))) products(Fixed<false>());
         else products(Fixed<true>());
     }
 
@@ -1000,7 +1024,7 @@ __global__ void __launch_bounds__(32 * kGradWarps, narrow_grad_ctas(kParts, kNF)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         float* p = gather + (m * 16 + (i >> 1) * 8 + g) * 33 + f * 8 + t * 2 + (i & 1);
-                        *p = w ? *p + dw[m][f][i] : dw[m][f][i];
+                        *p = (w ? *p : 0.f) + dw[m][f][i] * up;
                     }
         }
         __syncthreads();

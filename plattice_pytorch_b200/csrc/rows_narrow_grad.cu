@@ -32,14 +32,14 @@ static cudaError_t run_narrow_grad_as(const SmallGradArgs& a, int lines, cudaStr
 
 template <int kXT, int kParts>
 static cudaError_t run_narrow_grad_nf(const SmallGradArgs& a, int lines, cudaStream_t s) {
-    if constexpr (kParts < 3)
+    if constexpr (kParts == 1)
         if (a.s.out_dtype != PLATTICE_F32) return run_narrow_grad_as<kXT, kParts, false>(a, lines, s);
     return run_narrow_grad_as<kXT, kParts, true>(a, lines, s);
 }
 
 cudaError_t run_narrow_grad(const SmallGradArgs& a, int dtype, int parts, int lines, cudaStream_t s) {
     if (dtype == PLATTICE_F16)
-        return parts == 2 ? run_narrow_grad_nf<kXHalf, 2>(a, lines, s) : run_narrow_grad_as<kXHalf, 1, false>(a, lines, s);
+        return parts == 2 ? run_narrow_grad_as<kXHalf, 2, true>(a, lines, s) : run_narrow_grad_as<kXHalf, 1, false>(a, lines, s);
     if (a.s.x_scale || !a.s.x)   // without x (no weight gradient) its type does not matter
         return dtype == PLATTICE_F32 ? run_narrow_grad_nf<kX8, 3>(a, lines, s) : run_narrow_grad_nf<kX8, 1>(a, lines, s);
     return dtype == PLATTICE_F32 ? run_narrow_grad_nf<kXFloat, 3>(a, lines, s) : run_narrow_grad_nf<kXBf16, 1>(a, lines, s);
