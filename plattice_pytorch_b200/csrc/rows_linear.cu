@@ -591,12 +591,16 @@ struct BackwardPlan {
 // bits: 34559 rows, n 16, k 1896 102 / 126, 262144 rows, n 32, k 256 103 / 118;
 // float32, 8192 rows, n 8, k 2048 69 / 112.  Rows on no 16-byte boundaries, whose
 // channels the pass loads and stores one by one: bfloat16, k 50, n 24, 262144 rows
-// 71 / 83; k 95, n 8, 20000 rows 26 / 29; k 95, n 4, 848040 rows 587 / 267.
+// 71 / 83; k 95, n 8, 20000 rows 26 / 29; k 95, n 4, 848040 rows 587 / 267.  Float32
+// gradients beside 16-bit operands, whose parts cost the tiles more: bfloat16, 65536
+// rows: n 16, k 768 84 / 92, k 1024 78 / 111; n 24, k 512 84 / 71; float16: n 16, k
+// 1024 100 / 196; n 24, k 512 113 / 126; n 32, k 512 130 / 113.
 static bool backward_is_narrow(const plattice_linear_args* a) {
     if (a->n > 32 || a->k > kNarrowGradMost) return false;
     if (a->dtype == PLATTICE_F32) return true;
     if (a->k % 8 && a->k > 64 && a->rows > 24000) return false;
-    if ((int64_t)a->n * a->k <= 8192) return true;
+    const bool two = a->out_dtype == PLATTICE_F32 && a->n <= (a->dtype == PLATTICE_F16 ? 24 : 16);
+    if ((int64_t)a->n * a->k <= (two ? 16384 : 8192)) return true;
     return a->x_scale && a->n <= 24;
 }
 
