@@ -41,7 +41,6 @@ struct MmaArgs {
     unsigned pairs_a, pairs_b;   // parts of A and B of each product, 2 bits each
     int pairs;
     bool half;            // operands are float16 (else bfloat16)
-    float scale;          // of a gradient's results, a power of two
     bool precise;         // the result ends in float32 (not in 16 bits after a float32 sum of parts)
     long long patience;   // cycles that a wait may take
     unsigned* fault;      // host-mapped word that reports a wait that gave up (may be null)

@@ -78,7 +78,6 @@ struct GradArgs {
     int64_t rows;
     int n, split, act;
     int shift;          // log2 of the threads that share a row
-    bool halved;        // gz is stored times 1/2 (float16)
     bool vec;           // rows of grad_y and z allow 16-byte accesses
 };
 
@@ -90,20 +89,12 @@ __device__ __forceinline__ void times_slope(float (&g)[8], float (&z)[8]) {
     for (int i = 0; i < 8; i += 2) mul2(g[i], g[i + 1], z[i], z[i + 1]);
 }
 
-template <typename T> __device__ __forceinline__ void halve(float (&g)[8], bool halved) {
-    if constexpr (std::is_same_v<T, __half>) {
-        const float f = halved ? 0.5f : 1.f;
-#pragma unroll
-        for (int i = 0; i < 8; i += 2) mul2(g[i], g[i + 1], f, f);
-    }
-}
-
 constexpr int kTogether = 2;
 
 // gz = grad_y act'(z) as the two products take it, and the sums of the unrounded
 // gz over a CTA's rows.  Behind 16-bit gradients gz is rounded to their type (a
-// tensor core takes no wider operand; one rounding, as a stored gradient has;
-// gz_halved); behind float32 ones it is two bfloat16 parts beside 16-bit operands,
+// tensor core takes no wider operand; one rounding, as a stored gradient has, also
+// past float16's largest); behind float32 ones it is two bfloat16 parts beside 16-bit operands,
 // three beside float32 ones (gz_parts).  2^shift threads of 8 columns share a row;
 // gridDim.x strips of columns, gridDim.y parts of rows.
 template <typename TG, typename T, bool kFast>
@@ -121,7 +112,6 @@ __global__ void __launch_bounds__(256, 4) k_grad_z(const GradArgs a) {
 #pragma unroll
         for (int i = 0; i < 8; i += 2) add2(acc[i], acc[i + 1], g[i], g[i + 1]);
         if (!a.gz) return;
-        halve<T>(g, a.halved);
         const int64_t at = row * a.pitch + col;   // zeros up to the pitch
         store8_as<T>(a.gz, at, a.rows * a.pitch, g, kFast || (a.pitch % 8 == 0 && wide == 8), wide);
     };
@@ -256,7 +246,6 @@ __global__ void __launch_bounds__(256, 4) k_grad_z_table(const GradArgs a) {
                     add2(acc[i], acc[i + 1], v[i], v[i + 1]);
                 }
                 if (!a.gz) continue;
-                halve<T>(v, a.halved);
                 const int64_t at = (row + u * stride) * a.pitch + col;
                 store8_as<T>(a.gz, at, a.rows * a.pitch, v, true, 8);
             }
@@ -372,12 +361,6 @@ static bool tma_ready(const void* p, int dtype, int64_t width) {
 // too); else one.
 static int gz_parts(const plattice_linear_args* a) {
     return a->dtype == PLATTICE_F32 ? 3 : a->out_dtype == PLATTICE_F32 ? 2 : 1;
-}
-
-// A float16 gradient times a slope (of up to 1.13) can be past float16's largest:
-// the tiled backward's gz is stored halved, and its products are doubled.
-static bool gz_halved(const plattice_linear_args* a) {
-    return a->dtype == PLATTICE_F16 && a->act != PLATTICE_ACT_NONE && gz_parts(a) == 1;
 }
 
 // Parts of w, and of an x that is not in 8 bits.
@@ -693,7 +676,6 @@ static cudaError_t forward_mma(const plattice_linear_args* a, const ForwardPlan&
     m.half = a->dtype == PLATTICE_F16;
     m.fault = pl::fault_word();
     m.precise = true;
-    m.scale = 1.f;
     sum_args(&m, a->k, 1, x.parts, w.parts);
     return mma_forward(p.bn, aligned, x, w, m, s);
 }
@@ -739,7 +721,7 @@ static cudaError_t grad_z(const plattice_linear_args* a, const BackwardPlan& p, 
     if (!store && !a->grad_bias) return cudaSuccess;
     const GradArgs g{a->grad0, a->grad1, slope ? a->z : nullptr, slope ? a->z_scale : nullptr, store ? ws + p.gz : nullptr, p.pitch,
                      a->grad_bias ? reinterpret_cast<float*>(ws + p.partial_b) : nullptr, a->rows, a->n, a->split,
-                     a->act, p.shift, gz_halved(a),
+                     a->act, p.shift,
                      a->n % 8 == 0 && aligned16(a->grad0) && (!slope || a->z_scale || aligned16(a->z))};
     cudaError_t e;
     if (a->out_dtype == PLATTICE_F32)
@@ -760,7 +742,6 @@ static cudaError_t backward_mma(const plattice_linear_args* a, const BackwardPla
     cudaError_t e = cudaSuccess;
     MmaArgs m{};
     m.half = a->dtype == PLATTICE_F16 && parts == 1;
-    m.scale = gz_halved(a) ? 2.f : 1.f;
     m.fault = pl::fault_word();
     if (a->grad_x) {
         Operand w;

@@ -433,10 +433,6 @@ template <int kKind, int kOut, int kMode>
 __device__ __forceinline__ void finish16(float (&v)[16], const MmaArgs& p, const Tile& t, int64_t row0, int64_t col0,
                                          float* s, int half, int lane) {
     typedef typename OutType<kOut>::type T;
-    if (kKind != kForward) {
-#pragma unroll
-        for (int i = 0; i < 16; i += 2) mul2(v[i], v[i + 1], p.scale, p.scale);
-    }
     if (kKind == kGradW) {
         // D is [input channel][output channel], its result [output channel]
         // [input channel]: a lane per input channel stores whole lines

@@ -638,9 +638,9 @@ constexpr int kTilePitch = 72;   // 16-bit elements: rows 144 bytes apart, no ba
 // small part of what gz can be:
 // * behind float32 gradients (of 1e-8 or 1e6) float16 operands run as two bfloat16
 //   parts each (kParts 2, exact; gz's two hold 16 bits), three products;
-// * a float16 gradient is one float16 part as it came, or behind an activation two
-//   of half of gz (a slope of up to 1.13 can take it past the type), the results
-//   doubled.
+// * a float16 gradient is one float16 part as it came, or behind an activation two,
+//   the first held at the type's largest number (a slope of up to 1.13 can take gz
+//   past it).
 template <int kXT, int kParts> struct NarrowGradShape {
     static constexpr bool kHalf = kXT == kXHalf && kParts == 1;                       // float16 matrix instructions
     static constexpr int kPX = kXT == kXFloat ? 3 : kParts == 2 ? 2 : 1;
@@ -659,7 +659,8 @@ __device__ __forceinline__ void to_parts(float a, float b, uint32_t (&o)[kP]) {
 #pragma unroll
         for (int i = 0; i < kP; ++i) {
             union { __half2 h; uint32_t u; } x;
-            x.h = __floats2half2_rn(a, b);
+            if (i < kP - 1) asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(x.u) : "f"(b), "f"(a));
+            else x.h = __floats2half2_rn(a, b);
             o[i] = x.u;
             a -= __low2float(x.h);
             b -= __high2float(x.h);
@@ -723,7 +724,6 @@ __global__ void __launch_bounds__(32 * kGradWarps, narrow_grad_ctas(kParts, kNF)
     // not finite (a second part of 0 would make NaN of it)
     const bool single = kHalf && (__syncthreads_or(odd) || !a.s.z);
     if (!kHalf) __syncthreads();
-    const float down = kHalf && a.s.z ? 0.5f : 1.f, up = kHalf && a.s.z ? 2.f : 1.f;
 
     float dw[4][kNF][4];
 #pragma unroll
@@ -911,8 +911,8 @@ __global__ void __launch_bounds__(32 * kGradWarps, narrow_grad_ctas(kParts, kNF)
                     for (int h = 0; h < 2; ++h) {
                         const float* p = st + (g + 8 * h) * kNarrowPitch + t * cols_per_lane + s * 4;
                         uint32_t lo[kZ], hi[kZ];
-                        to_parts<kZ, kHalf, kAny, kPX == 1 && kParts == 1>(p[0] * down, p[1] * down, lo);
-                        to_parts<kZ, kHalf, kAny, kPX == 1 && kParts == 1>(p[2] * down, p[3] * down, hi);
+                        to_parts<kZ, kHalf, kAny, kPX == 1 && kParts == 1>(p[0], p[1], lo);
+                        to_parts<kZ, kHalf, kAny, kPX == 1 && kParts == 1>(p[2], p[3], hi);
 #pragma unroll
                         for (int q = 0; q < kZ; ++q) {
                             o[s][q][h] = lo[q];
@@ -945,7 +945,7 @@ __global__ void __launch_bounds__(32 * kGradWarps, narrow_grad_ctas(kParts, kNF)
                         if (left <= 0) continue;
                         float v[8];
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) v[i] = dx[q * 4 + (i >> 1)][h * 2 + (i & 1)] * up;
+                        for (int i = 0; i < 8; ++i) v[i] = dx[q * 4 + (i >> 1)][h * 2 + (i & 1)];
                         const int64_t at = (row0 + g + 8 * h) * k + ch;
                         const bool vec = a.vec_gx && left >= 8;
                         if (kXT == kXHalf) store8(static_cast<__half*>(a.grad_x) + at, v, vec, left);
@@ -962,7 +962,7 @@ __global__ void __launch_bounds__(32 * kGradWarps, narrow_grad_ctas(kParts, kNF)
                     for (int h = 0; h < 2; ++h) {
                         const float* p = st + (2 * t + 8 * h) * kNarrowPitch + f * 8 + g;
                         uint32_t o[kZ];
-                        to_parts<kZ, kHalf, kAny, kPX == 1 && kParts == 1>(p[0] * down, p[kNarrowPitch] * down, o);
+                        to_parts<kZ, kHalf, kAny, kPX == 1 && kParts == 1>(p[0], p[kNarrowPitch], o);
 #pragma unroll
                         for (int q = 0; q < kZ; ++q) b[q][f][h] = o[q];
                     }
@@ -1024,7 +1024,7 @@ __global__ void __launch_bounds__(32 * kGradWarps, narrow_grad_ctas(kParts, kNF)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         float* p = gather + (m * 16 + (i >> 1) * 8 + g) * 33 + f * 8 + t * 2 + (i & 1);
-                        *p = (w ? *p : 0.f) + dw[m][f][i] * up;
+                        *p = w ? *p + dw[m][f][i] : dw[m][f][i];
                     }
         }
         __syncthreads();

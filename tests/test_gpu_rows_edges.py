@@ -85,11 +85,11 @@ def test_float16_weight_gradient_of_a_million_tiny_gradients(dev, R):
         assert worst(f64(gx), np.full((rows, k), n * 1e-8), 2.0 ** -25 + 2.0 ** -11 * n * 1e-8) <= 1
 
 
-@pytest.mark.parametrize("rows,k,n", GRAD_SHAPES)
+@pytest.mark.parametrize("rows,k,n", GRAD_SHAPES[:3])
 @pytest.mark.parametrize("keep", ["8bit", "full"])
 def test_float16_gradients_behind_an_activation(dev, R, rows, k, n, keep):
-    """float16 gradients at the type's end: times gelu's slope they are past it.
-    gz is off by half a step of float16, and by one of its smallest (2^-24)."""
+    """float16 gradients at the type's end, in one pass: times gelu's slope they
+    are past it, and gz has a second part for that."""
     t = torch.float16
     gy = torch.where(_randn((rows, n), 5) > 0, 6.5e4, 3e-3).to(t)
     z = _randn((rows, n), 6, t).abs().to(dev) + 1   # slopes of 1.08 to 1.13
@@ -97,7 +97,22 @@ def test_float16_gradients_behind_an_activation(dev, R, rows, k, n, keep):
     x, w = _randn((rows, k), 7, t, 1e-3), _randn((n, k), 8, t, 1e-3)
     got = R.linear_backward(gy.to(dev), x.to(dev), w.to(dev), z8, act="gelu", bias_dtype=torch.float32)
     ze = f64(R.unpack8(z8)) if keep == "8bit" else f64(z)
-    _check_grads(got, f64(gy), f64(x), f64(w), ze, "gelu", t, t, 2.0 ** -11)
+    _check_grads(got, f64(gy), f64(x), f64(w), ze, "gelu", t, t, 2.0 ** -16)
+
+
+@pytest.mark.parametrize("rows,k,n", GRAD_SHAPES)
+@pytest.mark.parametrize("act", ["none", "relu", "silu"])
+def test_smallest_float16_gradients(dev, R, rows, k, n, act):
+    """Gradients of float16's smallest number: a relu leaves them as they are,
+    a slope rounds each to a step or none at most."""
+    t = torch.float16
+    gy = torch.full((rows, n), 2.0 ** -24).to(t)
+    z = _randn((rows, n), 57, t).abs() + 1   # slopes of 0.9 to 1.1
+    x, w = torch.full((rows, k), 1024.0).to(t), torch.full((n, k), 1024.0).to(t)
+    gx, gw, gb = R.linear_backward(gy.to(dev), x.to(dev), w.to(dev), None if act == "none" else z.to(dev), act=act)
+    off = 0.1 + 2.0 ** -11 if act == "silu" else 2.0 ** -11   # |slope - 1| <= 0.1
+    assert worst(f64(gx), np.full((rows, k), n * 2.0 ** -14), off * n * 2.0 ** -14 + 2.0 ** -25) <= 1
+    assert worst(f64(gw), np.full((n, k), rows * 2.0 ** -14), off * rows * 2.0 ** -14 + 2.0 ** -25) <= 1
 
 
 def test_float16_split_gradients(dev, R):
