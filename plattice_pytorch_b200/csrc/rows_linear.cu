@@ -560,7 +560,6 @@ static ForwardPlan forward_plan(const plattice_linear_args* a) {
 struct BackwardPlan {
     bool narrow;
     int lines;       // narrow: CTAs along the rows
-    int64_t line_bytes;
     bool gz_needed;
     int shift, strips;
     int bn_x, bn_w, parts_b, parts_w;

@@ -20,8 +20,8 @@
 // stages, one issues the MMAs, the epilogue's warps empty the other of two
 // accumulators (activation, residual, stores) meanwhile.  Bound by the tensor
 // cores where the sum is deep (8192 x 8192 x 8192 in bfloat16: 832 us, 1321
-// TFLOP/s; the input gradient of 32768 x 1024 -> 4096: 176 us, 1560), by the
-// epilogue where it is not (its forward with gelu, residual and kept z: 300 us,
+// TFLOP/s; the input gradient of 32768 x 1024 -> 4096: 177 us, 1553), by the
+// epilogue where it is not (its forward with gelu, residual and kept z: 302 us,
 // plain 215), by HBM where K and n are small (262144 x 64 -> 64: 17 us, 67 MB).  Every wait is
 // bounded: a wait that gives up ends all roles, copies and MMAs in flight are
 // waited for, tensor memory is freed and the call's failure is reported.
@@ -50,12 +50,12 @@ enum Mode { kAny = 0, kAligned = 1, kPlain = 2 };
 __host__ __device__ constexpr int epilogue_warps(int kind, bool chunked) { return kind == 0 || chunked ? 16 : 8; }
 __host__ __device__ constexpr int role_threads(int kind, bool chunked) { return 64 + 32 * epilogue_warps(kind, chunked); }
 
-// A float32 result of a deep sum (kChunked; a 16-bit one of a far deeper): the MMA cuts where an addition
-// rounds, so that an accumulator drifts by about 2^-26 of itself with each of
-// them, terms of both signs (1.1e-6 of the result at a depth of 1024, 4.5e-6 at
-// 4096; float16 terms of one sign: 2^-23).  The sum then
-// goes in chunks of kChunk slices through the two accumulators, and the
-// epilogue adds those in registers, rounding; a warp holds one 32-column
+// A float32 result of a deep sum, and a 16-bit one of a far deeper (deepest_sum):
+// kChunked.  The MMA cuts where an addition rounds, so that an accumulator drifts
+// by about 2^-26 of itself with each of them, terms of both signs (1.1e-6 of the
+// result at a depth of 1024, 4.5e-6 at 4096; float16 terms of one sign: 2^-23).
+// The sum then goes in chunks of kChunk slices through the two accumulators, and
+// the epilogue adds those in registers, rounding; a warp holds one 32-column
 // piece, so tiles are at most 128 wide.
 constexpr int kChunk = 8;
 

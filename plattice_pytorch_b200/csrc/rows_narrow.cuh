@@ -35,9 +35,10 @@ enum XType { kX8 = 0, kXBf16 = 1, kXHalf = 2, kXFloat = 3 };
 // included, took five instructions a pair: 35 against 25 us for 1048576 rows,
 // 64 -> 8.)
 //
-// Bound by instruction issue (500 a block of 32 rows, 2.3 an SM and cycle), at
-// 25 us for those 1048576 rows (103 MB, 15.7 us at the copy rate), where tiles
-// of 128 rows took 109.
+// 25 us for those 1048576 rows (103 MB, 15.7 us at the copy rate), where tiles of
+// 128 rows took 109.  500 instructions a block of 32 rows, issued in 65 % of the
+// cycles: bound by that and by what 24 warps an SM, all that the registers leave,
+// cannot hide.
 
 template <int kXT> struct NarrowShape {
     static constexpr int kM = kXT == kX8 ? 2 : 1;                               // 16-row fragments

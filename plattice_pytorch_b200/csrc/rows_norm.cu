@@ -13,7 +13,7 @@ namespace plr {
 //
 // A thread takes 8 channels, 4 neighbouring lanes a block of 32.  Both kernels
 // move each byte once and are bound by HBM: 262144 x 256 in bfloat16 (203 MB,
-// 31.1 us at the copy rate) takes 34.7 us to pack and 33.5 to unpack.  A CTA
+// 31.1 us at the copy rate) takes 35.5 us to pack and 33.4 to unpack.  A CTA
 // takes kUnits x 256 such groups of 8, so that each thread has kUnits
 // independent loads in flight.
 
@@ -165,8 +165,8 @@ __global__ void __launch_bounds__(256) k_unpack8_any(T* __restrict__ y, int64_t 
 // per row); a thread holds kChunks groups of 8 channels in registers, so a row
 // is read once whatever its statistics need.  Bound by HBM: 262144 x 256 in
 // bfloat16 with residual and 8-bit result (472 MB, 72 us at the copy rate) takes
-// 79 us, 65536 x 1024 85, 1048576 x 64 85 (each 82 at the copy rate), 262144 x
-// 250 111.  The mean of squares is summed in float32.  h is rounded to the rows' type where it is stored; y is computed
+// 80 us, 65536 x 1024 86, 1048576 x 64 85 (each 82 at the copy rate), 262144 x
+// 250 112.  The mean of squares is summed in float32.  h is rounded to the rows' type where it is stored; y is computed
 // from the unrounded sum, one rounding from its definition.
 
 // Sum over the threads of a row.  `turn` alternates from call to call: sums of
