@@ -397,6 +397,25 @@ def test_deep_sums_of_like_terms(dev, R, dtype, deep):
     assert float((gx.double() / (a.double()[:, None] * c.double() * total) - 1).abs().max()) <= bound
 
 
+@pytest.mark.parametrize("dtype,x8", [("fp32", False), ("bf16", False), ("fp16", False), ("fp32", True), ("bf16", True)])
+@pytest.mark.parametrize("rows,n,cut", [(3, 24, 16), (5000, 24, 16), (5000, 7, 3), (700, 40, 33), (5000, 72, 1)])
+def test_split_result_beside_a_kept_z(dev, R, rows, n, cut, dtype, x8):
+    """Without activation the kept z is the result before the split, rounded once
+    from the same sum."""
+    t, k = DTYPES[dtype], 40
+    x, w, b = _randn((rows, k), 58, t).to(dev), _randn((n, k), 59, t).to(dev), _randn((n,), 60).to(dev)
+    xin = R.pack8(x) if x8 else x
+    for keep in ("full", "8bit"):
+        (f, v), z = R.linear(xin, w, b, split=cut, keep=keep)
+        y = torch.cat([f, v], 1)
+        if keep == "full":
+            assert torch.equal(z, y)
+        else:
+            unit = np.repeat(2.0 ** (z.scale.cpu().numpy().astype(np.float64) - 127), 32, 1)[:, :n]
+            off = (2.0 ** -4 + 2 * half_step(t)) * np.abs(f64(y)) + 2.0 ** -10 * unit
+            assert worst(f64(R.unpack8(z)), f64(y), off) <= 1
+
+
 def test_half_a_pair_of_gradients_is_refused(dev, R):
     x, w, g = torch.zeros(4, 8, device=dev), torch.zeros(3, 8, device=dev), torch.zeros(4, 3, device=dev)
     for pair in ((g, None), [g, None], (None, g)):
