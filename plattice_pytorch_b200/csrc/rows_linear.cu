@@ -530,7 +530,9 @@ static Way forward_way(const plattice_linear_args* a) {
     if (few <= sm_count()) return kWayFew;
     const int parts = a->dtype == PLATTICE_F32 ? 3 : 1;
     const bool tiles_read = !a->x_scale && tma_ready(a->x, a->dtype, a->k);
-    if (a->n <= 32 && (!tiles_read || (int64_t)a->n * a->k <= 1536) &&
+    // k_narrow stages its results in the split's order: a z kept whole beside them goes through tiles
+    const bool order = a->split && a->z && !a->z_scale;
+    if (a->n <= 32 && !order && (!tiles_read || (int64_t)a->n * a->k <= 1536) &&
         !(parts == 1 && narrow_shares(ceil_div(a->rows, a->x_scale ? 32 : 16), a->k)) &&
         narrow_fragments(a->k, (int)ceil_div(a->n, 8), parts) <= kNarrowMost)
         return kWayNarrow;

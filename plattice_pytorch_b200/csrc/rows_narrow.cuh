@@ -589,7 +589,7 @@ __global__ void __launch_bounds__(32 * kNarrowWarps, narrow_ctas(kXT, kNF)) k_na
                 }
             }
         }
-        const bool full_z = !kPlain && a.z && !a.z_scale;
+        const bool full_z = !kPlain && a.z && !a.z_scale;   // without a split (forward_way)
         for (int pass = full_z ? 0 : 1; pass < 2; ++pass) {   // a kept z, then y
             __syncwarp();
 #pragma unroll
@@ -598,12 +598,8 @@ __global__ void __launch_bounds__(32 * kNarrowWarps, narrow_ctas(kXT, kNF)) k_na
                 for (int f = 0; f < kNF; ++f) {
                     if (!kPlain && pass == 1) activate(acc[m][f], a.act);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int r = m * 16 + (i >> 1) * 8 + g, c = f * 8 + t * 2 + (i & 1);
-                        if (put[f][i & 1] < 0) continue;
-                        if (!kPlain && pass == 0) st[r * a.n + c] = acc[m][f][i];   // a kept z is one tensor
-                        else st[r * width[f][i & 1] + put[f][i & 1]] = acc[m][f][i];
-                    }
+                    for (int i = 0; i < 4; ++i)
+                        if (put[f][i & 1] >= 0) st[(m * 16 + (i >> 1) * 8 + g) * width[f][i & 1] + put[f][i & 1]] = acc[m][f][i];
                 }
             __syncwarp();
             if (kPlain) {
