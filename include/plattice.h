@@ -45,7 +45,7 @@
 extern "C" {
 #endif
 
-#define PLATTICE_ABI_VERSION 6
+#define PLATTICE_ABI_VERSION 7
 
 /* status codes */
 #define PLATTICE_OK 0
@@ -374,6 +374,116 @@ int plattice_linear_workspace_size(const plattice_linear_args* args, size_t* byt
 int plattice_linear(const plattice_linear_args* args, void* stream);
 int plattice_linear_backward_workspace_size(const plattice_linear_args* args, size_t* bytes);
 int plattice_linear_backward(const plattice_linear_args* args, void* stream);
+
+/* Rows from labels: y[i] = scale * table[ids[i]] with table [n][c], both in
+ * `dtype`; ids are int64 (ids_wide != 0) or int32.  An id outside 0..n-1 (the
+ * "ignored" of label maps) gives a row of zeros.  n < 2^31, c <= 2^21. */
+int plattice_embed(void* y, const void* ids, int ids_wide, const void* table, int dtype, float scale,
+                   long long count, long long n, int c, void* stream);
+
+/* Its gradient: grad_table[v] = scale * sum of grad_y[i] over the i with ids[i]
+ * = v (0 where there is none), in table_dtype.  The rows of a label are added in
+ * float32, in an order that the sizes fix.  count < 2^31; workspace 256-byte
+ * aligned. */
+int plattice_embed_backward_workspace_size(long long count, long long n, int c, size_t* bytes);
+int plattice_embed_backward(void* grad_table, int table_dtype, const void* grad_y, int dtype, const void* ids,
+                            int ids_wide, float scale, void* workspace, size_t workspace_bytes, long long count,
+                            long long n, int c, void* stream);
+
+/* Gated linear recurrence along lines of rows: x, gate, h [lines][steps][c] in
+ * `dtype`, for every line and channel
+ *   h[t] = gate[t] h[t-1] + u[t],  u = x, or (1 - gate) x with blend,
+ * from h[-1] = state [lines][c] (float32; NULL: zeros), the steps taken from the
+ * last to the first with reverse.  last [lines][c]: h after the last step taken
+ * (NULL: not wanted).  states (NULL: not kept) [lines][ceil(steps / 16)][c]
+ * float32: h before every 16th step taken, what the backward starts from.  The
+ * recurrence is held in float32; h is its rounding.
+ *
+ * Backward, with G[t] = grad_h[t] + gate[t+1] G[t+1] (grad_last, if any, in the
+ * place of gate[t+1] G[t+1] after the last step):
+ *   grad_x = G, or (1 - gate) G with blend;  grad_gate[t] = G[t] h[t-1], or
+ *   G[t] (h[t-1] - x[t]);  grad_state = gate[0] G[0] (NULL: not wanted).
+ * h is computed again from states, in float32. */
+#define PLATTICE_SCAN_KEEP 16
+typedef struct plattice_scan_args {
+    const void* x;
+    const void* gate;
+    const float* state;     /* forward */
+    void* h;                /* forward */
+    float* last;            /* forward */
+    float* states;          /* forward: output; backward: input */
+    const void* grad_h;     /* backward */
+    const float* grad_last; /* backward: NULL for zeros */
+    void* grad_x;
+    void* grad_gate;
+    float* grad_state;
+    void* workspace;        /* 256-byte aligned */
+    size_t workspace_bytes;
+    long long lines, steps;
+    int c, dtype, blend, reverse;
+} plattice_scan_args;
+int plattice_scan_workspace_size(const plattice_scan_args* args, size_t* bytes);
+int plattice_scan(const plattice_scan_args* args, void* stream);
+int plattice_scan_backward_workspace_size(const plattice_scan_args* args, size_t* bytes);
+int plattice_scan_backward(const plattice_scan_args* args, void* stream);
+
+/* Log probabilities of rows of scores, logits [rows][n] in `dtype`:
+ *   stats[r] = (m, s): the largest score and log(sum_j exp(x_j - m))  (float32),
+ *   logp[r] = x_label - m - s;  entropy[r] = -sum_j p_j log p_j,
+ *   top_logp, top_ids [rows][top]: the `top` largest log probabilities, falling,
+ *   and their classes (equal scores: the lowest class first; NaN last).
+ * A label outside 0..n-1 has logp 0.  A score of -inf is a class that the row
+ * may not have; a row of nothing else has stats (-inf, 0), log probabilities
+ * -inf and entropy 0.  NaN or +inf in a row make all its numbers NaN.  logp
+ * with labels, entropy, lse and the top pair may be NULL.  top <= PLATTICE_MAX_TOP.
+ *
+ * Backward, from the same logits and labels and the forward's stats:
+ *   grad_j = grad_logp ([j = label] - p_j) - grad_entropy p_j (log p_j + entropy)
+ *            + grad_lse p_j      (lse = m + s),
+ * each incoming gradient float32 [rows] or NULL (grad_logp needs labels,
+ * grad_entropy the forward's entropy); 0 for a row of -inf only. */
+#define PLATTICE_MAX_TOP 32
+typedef struct plattice_log_probs_args {
+    const void* logits;
+    const void* labels;
+    float* logp;
+    float* entropy;            /* forward: output; backward: input */
+    float* stats;              /* forward: output; backward: input */
+    float* lse;                /* forward: m + s, NULL: not wanted */
+    float* top_logp;
+    long long* top_ids;
+    const float* grad_logp;    /* backward */
+    const float* grad_entropy;
+    const float* grad_lse;
+    void* grad_logits;
+    long long rows;
+    int n, top, dtype, labels_wide;
+} plattice_log_probs_args;
+int plattice_log_probs(const plattice_log_probs_args* args, void* stream);
+int plattice_log_probs_backward(const plattice_log_probs_args* args, void* stream);
+
+/* The norm of many gradients together, and the gradients scaled down to a
+ * largest norm:
+ *   norm = sqrt(sum over all tensors and values of g^2)
+ *   out = g * min(1, max_norm / (norm + eps)), rounded to out_dtype
+ * with out_dtype the tensor's type or PLATTICE_F32, out the tensor itself (in its
+ * own type) or memory of its own; memory that any out shares with another tensor
+ * is refused (PLATTICE_ERR_INVALID).  Squares are added in float32 by eights (in
+ * float64 where those would not hold them) and then in float64, in an order that
+ * the sizes fix.  norm_in (device, float32) non-NULL: the norm to use, such as
+ * one over several processes; the gradients are then read only to be scaled.
+ * norm_out (device, float32; may be norm_in): the norm.  max_norm >= 0, infinite
+ * for a copy; without out pointers (all NULL) only the norm is computed.  The
+ * arrays are read before the call returns. */
+typedef struct plattice_grad {
+    const void* g;
+    void* out;
+    long long size;
+    int dtype, out_dtype;
+} plattice_grad;
+int plattice_clip_grads_workspace_size(const plattice_grad* grads, int count, size_t* bytes);
+int plattice_clip_grads(const plattice_grad* grads, int count, float max_norm, float eps, const float* norm_in,
+                        float* norm_out, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -5,11 +5,12 @@ module (forward / backward) and ``plattice_pytorch_b200.plattice`` its
 plattice.py (PermutoLatticeFunction, PermutoLattice).  The work is done by
 libplattice_b200.so through the C ABI of include/plattice.h.
 """
-from . import PLOO, rows
+from . import PLOO, grads, rows
 from .plattice import (LatticeFilterFunction, PermutoLattice, PermutoLatticeBatchFunction,
                        PermutoLatticeFeatureFunction, PermutoLatticeFunction, PermutoLatticeLayer,
-                       RowLinearFunction, RowNormLinearFunction)
+                       RowEmbedFunction, RowLinearFunction, RowLogProbFunction, RowNormLinearFunction,
+                       RowScanFunction)
 
-__all__ = ["PLOO", "rows", "PermutoLattice", "PermutoLatticeFunction", "PermutoLatticeBatchFunction",
+__all__ = ["PLOO", "rows", "grads", "PermutoLattice", "PermutoLatticeFunction", "PermutoLatticeBatchFunction",
            "PermutoLatticeFeatureFunction", "LatticeFilterFunction", "PermutoLatticeLayer", "RowLinearFunction",
-           "RowNormLinearFunction"]
+           "RowNormLinearFunction", "RowEmbedFunction", "RowScanFunction", "RowLogProbFunction"]

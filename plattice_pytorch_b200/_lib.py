@@ -13,7 +13,7 @@ LIB_PATH = os.path.join(HERE, "libplattice_b200.so")
 
 OK, ERR_INVALID, ERR_WORKSPACE, ERR_CUDA, ERR_DEVICE = 0, 1, 2, 3, 4
 DEV_TABLE_FULL, DEV_WAIT_LIMIT, DEV_ROUND_LIMIT = 2, 4, 8
-ABI_VERSION = 6
+ABI_VERSION = 7
 
 class LinearArgs(ctypes.Structure):
     """plattice_linear_args of include/plattice.h."""
@@ -21,6 +21,27 @@ class LinearArgs(ctypes.Structure):
                                                "grad0", "grad1", "grad_x", "grad_w", "grad_bias", "workspace")]
                 + [("workspace_bytes", ctypes.c_size_t), ("rows", ctypes.c_longlong)]
                 + [(n, ctypes.c_int) for n in ("k", "n", "split", "dtype", "out_dtype", "bias_dtype", "act")])
+
+
+class ScanArgs(ctypes.Structure):
+    """plattice_scan_args of include/plattice.h."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "gate", "state", "h", "last", "states", "grad_h", "grad_last",
+                                               "grad_x", "grad_gate", "grad_state", "workspace")]
+                + [("workspace_bytes", ctypes.c_size_t), ("lines", ctypes.c_longlong), ("steps", ctypes.c_longlong)]
+                + [(n, ctypes.c_int) for n in ("c", "dtype", "blend", "reverse")])
+
+
+class LogProbsArgs(ctypes.Structure):
+    """plattice_log_probs_args of include/plattice.h."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("logits", "labels", "logp", "entropy", "stats", "lse", "top_logp", "top_ids",
+                                               "grad_logp", "grad_entropy", "grad_lse", "grad_logits")]
+                + [("rows", ctypes.c_longlong)] + [(n, ctypes.c_int) for n in ("n", "top", "dtype", "labels_wide")])
+
+
+class Grad(ctypes.Structure):
+    """plattice_grad of include/plattice.h."""
+    _fields_ = [("g", ctypes.c_void_p), ("out", ctypes.c_void_p), ("size", ctypes.c_longlong),
+                ("dtype", ctypes.c_int), ("out_dtype", ctypes.c_int)]
 
 
 _lock = threading.Lock()
@@ -140,6 +161,26 @@ def lib():
             getattr(L, name).argtypes = [A, P]
             getattr(L, name + "_workspace_size").restype = I
             getattr(L, name + "_workspace_size").argtypes = [A, ctypes.POINTER(S)]
+        F = ctypes.c_float
+        L.plattice_embed.restype = I
+        L.plattice_embed.argtypes = [P, P, I, P, I, F, LL, LL, I, P]
+        L.plattice_embed_backward_workspace_size.restype = I
+        L.plattice_embed_backward_workspace_size.argtypes = [LL, LL, I, ctypes.POINTER(S)]
+        L.plattice_embed_backward.restype = I
+        L.plattice_embed_backward.argtypes = [P, I, P, I, P, I, F, P, S, LL, LL, I, P]
+        A = ctypes.POINTER(ScanArgs)
+        for name in ("plattice_scan", "plattice_scan_backward"):
+            getattr(L, name).restype = I
+            getattr(L, name).argtypes = [A, P]
+            getattr(L, name + "_workspace_size").restype = I
+            getattr(L, name + "_workspace_size").argtypes = [A, ctypes.POINTER(S)]
+        for name in ("plattice_log_probs", "plattice_log_probs_backward"):
+            getattr(L, name).restype = I
+            getattr(L, name).argtypes = [ctypes.POINTER(LogProbsArgs), P]
+        L.plattice_clip_grads_workspace_size.restype = I
+        L.plattice_clip_grads_workspace_size.argtypes = [ctypes.POINTER(Grad), I, ctypes.POINTER(S)]
+        L.plattice_clip_grads.restype = I
+        L.plattice_clip_grads.argtypes = [ctypes.POINTER(Grad), I, F, F, P, P, P, S, P]
         v = L.plattice_abi_version()
         if v != ABI_VERSION:
             raise ImportError(f"{LIB_PATH} has ABI version {v}, expected {ABI_VERSION}: rebuild it")

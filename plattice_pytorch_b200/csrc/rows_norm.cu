@@ -19,27 +19,6 @@ namespace plr {
 
 constexpr int kUnits = 4;
 
-// Splits the flat group index of (CTA base + offset) into row and group: one
-// 64-bit division per CTA, a multiplication and its correction per thread.
-struct GroupAt {
-    int64_t row0;
-    unsigned rem, groups;
-    float inv;
-    __device__ __forceinline__ GroupAt(int64_t base, unsigned groups_) : groups(groups_) {
-        row0 = base / groups;
-        rem = (unsigned)(base - row0 * groups);
-        inv = 1.f / (float)groups;
-    }
-    __device__ __forceinline__ void at(unsigned offset, int64_t& row, unsigned& g) const {
-        const unsigned t = rem + offset;
-        unsigned r = (unsigned)((float)t * inv);   // at most offset / groups + 1: off by one at most
-        if (r * groups > t) --r;
-        if (t - r * groups >= groups) ++r;
-        row = row0 + r;
-        g = t - r * groups;
-    }
-};
-
 // Rows without padding and aligned (c a multiple of 32): group g is elements
 // 8 g.. whatever its row.
 template <typename T>

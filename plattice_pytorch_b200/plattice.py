@@ -27,6 +27,8 @@ do; its backward is the value gradient on the same lattice.
 reference) are the row operators of ``rows.py`` under autograd, and
 ``PermutoLatticeLayer`` chains them around the filter: norm, projection to
 learned features and values, filter, projection back, residual.
+``RowEmbedFunction``, ``RowScanFunction`` and ``RowLogProbFunction`` are the
+others: rows from labels, the recurrence along lines, and the loss over labels.
 """
 import ctypes
 import math
@@ -62,7 +64,8 @@ def _cpp_function():
     return _EXT
 
 __all__ = ["PermutoLatticeFunction", "PermutoLattice", "LatticeFilterFunction", "PermutoLatticeBatchFunction",
-           "PermutoLatticeFeatureFunction", "RowLinearFunction", "RowNormLinearFunction", "PermutoLatticeLayer"]
+           "PermutoLatticeFeatureFunction", "RowLinearFunction", "RowNormLinearFunction", "PermutoLatticeLayer",
+           "RowEmbedFunction", "RowScanFunction", "RowLogProbFunction"]
 
 
 class PermutoLatticeFunction(Function):
@@ -275,6 +278,72 @@ class RowNormLinearFunction(Function):
             gx, gg = rows.rms_norm_backward(gn.to(h.dtype), h, rstd, gain, gh)
         return (gx if need[0] else None, gx if need[1] else None, gg if need[2] else None, gw, gb,
                 None, None, None, None, None)
+
+
+class RowEmbedFunction(Function):
+    """``RowEmbedFunction.apply(ids, table, scale) -> scale * table[ids]``
+    (:func:`rows.embed`), gradient for the table."""
+
+    @staticmethod
+    def forward(ctx, ids, table, scale=1.0):
+        y = rows.embed(ids, table, scale)
+        ctx.save_for_backward(ids)
+        ctx.n, ctx.scale = int(table.shape[0]), scale
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_y):
+        (ids,) = ctx.saved_tensors
+        return None, rows.embed_backward(grad_y.contiguous(), ids, ctx.n, ctx.scale), None
+
+
+class RowScanFunction(Function):
+    """``RowScanFunction.apply(x, gate, state, blend, reverse) -> (h, last)``
+    (:func:`rows.scan`), gradients for the first three (``state`` may be None)."""
+
+    @staticmethod
+    def forward(ctx, x, gate, state=None, blend=False, reverse=False):
+        h, last, states = rows.scan(x, gate, state, blend, reverse, keep=any(ctx.needs_input_grad))
+        ctx.set_materialize_grads(False)
+        if states is not None:
+            ctx.save_for_backward(x, gate, states)
+        ctx.how = blend, reverse
+        return h, last
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_h, grad_last):
+        if grad_h is None and grad_last is None:
+            return None, None, None, None, None
+        x, gate, states = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        g = torch.zeros_like(x) if grad_h is None else grad_h.contiguous()
+        last = None if grad_last is None else grad_last.contiguous()
+        gx, ga, gs = rows.scan_backward(g, x, gate, states, last, *ctx.how)
+        return (*(g if n else None for g, n in zip((gx, ga, gs), need)), None, None)
+
+
+class RowLogProbFunction(Function):
+    """``RowLogProbFunction.apply(logits, labels) -> (logp, entropy, lse)``
+    (:func:`rows.log_probs`), gradient for the logits.  The mean of ``-logp`` over
+    the labels that count is the cross entropy."""
+
+    @staticmethod
+    def forward(ctx, logits, labels):
+        r = rows.log_probs(logits, labels)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(logits, labels, r.entropy, r.stats)
+        return r.logp, r.entropy, r.lse
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *grads):
+        if all(g is None for g in grads):
+            return None, None
+        logits, labels, entropy, stats = ctx.saved_tensors
+        r = rows.LogProbs(None, entropy, None, stats, None, None)
+        return rows.log_probs_backward(logits, r, labels, *(None if g is None else g.contiguous() for g in grads)), None
 
 
 class PermutoLatticeLayer(Module):

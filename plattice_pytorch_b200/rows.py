@@ -17,25 +17,38 @@ Functions and the module that chains them):
   ``x`` a tensor or Rows8; the backward reads the same Rows8 that the forward
   read, and the pre-activation from Rows8 too.
 
+* :func:`embed` / :func:`embed_backward` -- rows from a label map, and the
+  gradient of the table they come from.
+* :func:`scan` / :func:`scan_backward` -- a gated linear recurrence along the
+  lines of rows (an image's lines: edge-aware smoothing with learned gates).
+* :func:`log_probs` / :func:`log_probs_backward` -- from rows of scores the log
+  probabilities of given labels, the entropies and the best alternatives.
+
 Tensors are contiguous CUDA tensors ``[..., channels]`` of float32, bfloat16
 or float16; as for the filter, a failed check raises RuntimeError, kernels run
 on PyTorch's current stream of the tensors' device, and no call synchronises.
 No reference counterpart.
 """
+import collections
 import ctypes
+import math
 
 import torch
 
 from . import _lib
 from .PLOO import _call, _check_input, _lib_h, _raise, _raw_stream, _require
 
-__all__ = ["Rows8", "pack8", "unpack8", "rms_norm", "rms_norm_backward", "linear", "linear_backward", "ACTIVATIONS"]
+__all__ = ["Rows8", "pack8", "unpack8", "rms_norm", "rms_norm_backward", "linear", "linear_backward", "ACTIVATIONS",
+           "embed", "embed_backward", "scan", "scan_backward", "LogProbs", "log_probs", "log_probs_backward"]
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
 _KEEP = {None: 0, "8bit": 1, "full": 2}
 _MAX_NORM = 16384
 _MAX_CHANNELS = 1 << 30
+_MAX_EMBED = 1 << 21
+_MAX_TOP = 32
+_SCAN_KEEP = 16   # steps between the states that a scan keeps
 
 
 def _width8(c):
@@ -401,3 +414,205 @@ def linear_backward(grad_y, x, weight, z=None, act="none", bias_dtype=None, need
     a.grad_x, a.grad_w, a.grad_bias = _ptr(grad_x), _ptr(grad_w), _ptr(grad_b)
     _linear_call("plattice_linear_backward", a, dev)
     return grad_x, grad_w, grad_b
+
+
+# ---------------------------------------------------------------- rows from labels
+
+def _check_labels(t, name, shape, device):
+    _check_input(t, name)
+    _require(t.dtype in (torch.int64, torch.int32), f"{name} must be int64 or int32")
+    _require(shape is None or tuple(t.shape) == tuple(shape), f"{name} must be {None if shape is None else tuple(shape)}")
+    _require(t.device == device, f"{name} must be on the rows' device")
+
+
+def _check_scale(scale):
+    _require(isinstance(scale, (int, float)) and math.isfinite(scale), "scale must be a finite number")
+
+
+def embed(ids, table, scale=1.0):
+    """Rows from labels: ``y [..., c] = scale * table[ids]`` in the type of
+    ``table [n, c]`` (at most 2^21 channels), ``ids [...]`` int64 or int32.  A
+    label outside ``0..n-1`` (the "ignored" of label maps) gives a row of zeros."""
+    _check_input(table, "table")
+    _require(table.dtype in _DTYPES, "table must be float32, bfloat16 or float16")
+    _require(table.dim() == 2 and 1 <= table.shape[0] < 1 << 31 and 1 <= table.shape[1] <= _MAX_EMBED,
+             "table must be [n, c], c at most 2^21")
+    _check_labels(ids, "ids", None, table.device)
+    _check_scale(scale)
+    n, c = (int(s) for s in table.shape)
+    y = torch.empty((*ids.shape, c), dtype=table.dtype, device=table.device)
+    rc = _call(y.device.index, _lib_h().plattice_embed, y.data_ptr(), ids.data_ptr(), int(ids.dtype == torch.int64),
+               table.data_ptr(), _DTYPES[table.dtype], scale, ids.numel(), n, c, _raw_stream(y.device.index))
+    if rc:
+        _raise("plattice_embed", rc, f"ids={tuple(ids.shape)} table={tuple(table.shape)}")
+    return y
+
+
+def embed_backward(grad_y, ids, n, scale=1.0, dtype=None):
+    """Gradient of :func:`embed`'s table: ``[n, c]`` in ``dtype`` (default
+    ``grad_y``'s), row v the sum of ``scale * grad_y`` over the places where
+    ``ids`` is v.  Fewer than 2^31 ids."""
+    _check_rows(grad_y, "grad_y")
+    c, dev = int(grad_y.shape[-1]), grad_y.device
+    _require(c <= _MAX_EMBED, "grad_y must have at most 2^21 channels")
+    _check_labels(ids, "ids", grad_y.shape[:-1], dev)
+    _require(ids.numel() < 1 << 31, "ids must be fewer than 2^31")
+    _require(isinstance(n, int) and 1 <= n < 1 << 31, "n must be in [1, 2^31)")
+    _check_scale(scale)
+    dtype = grad_y.dtype if dtype is None else dtype
+    _require(dtype in _DTYPES, "dtype must be float32, bfloat16 or float16")
+    b = ctypes.c_size_t(0)
+    rc = _lib_h().plattice_embed_backward_workspace_size(ids.numel(), n, c, ctypes.byref(b))
+    if rc:
+        _raise("plattice_embed_backward_workspace_size", rc, f"ids={tuple(ids.shape)} n={n} c={c}")
+    grad = torch.empty((n, c), dtype=dtype, device=dev)
+    ws = torch.empty(b.value, dtype=torch.uint8, device=dev)
+    rc = _call(dev.index, _lib_h().plattice_embed_backward, grad.data_ptr(), _DTYPES[dtype], grad_y.data_ptr(),
+               _DTYPES[grad_y.dtype], ids.data_ptr(), int(ids.dtype == torch.int64), scale, ws.data_ptr(), b.value,
+               ids.numel(), n, c, _raw_stream(dev.index))
+    if rc:
+        _raise("plattice_embed_backward", rc, f"ids={tuple(ids.shape)} n={n} c={c}")
+    return grad
+
+
+# ---------------------------------------------------------------- recurrence along lines
+
+def _scan_common(x, gate, blend, reverse):
+    """Checked (args struct, shape of a state, shape of the kept states, device) of a scan."""
+    _check_rows(x, "x")
+    _require(x.dim() >= 2, "x must be [..., steps, channels]")
+    _check_like(gate, "gate", x.shape, x.dtype, x.device)
+    a = _lib.ScanArgs()
+    a.x, a.gate = x.data_ptr(), gate.data_ptr()
+    a.steps, a.c = int(x.shape[-2]), int(x.shape[-1])
+    a.lines = _rows_of(x.shape[:-1])
+    a.dtype, a.blend, a.reverse = _DTYPES[x.dtype], bool(blend), bool(reverse)
+    lead = tuple(x.shape[:-2])
+    return a, lead + (a.c,), lead + (-(-a.steps // _SCAN_KEEP), a.c), x.device
+
+
+def _scan_call(name, a, dev):
+    b = ctypes.c_size_t(0)
+    rc = _call(dev.index, getattr(_lib_h(), name + "_workspace_size"), ctypes.byref(a), ctypes.byref(b))
+    if rc:
+        _raise(name + "_workspace_size", rc, f"lines={a.lines} steps={a.steps} c={a.c}")
+    ws = torch.empty(b.value, dtype=torch.uint8, device=dev)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), b.value
+    rc = _call(dev.index, getattr(_lib_h(), name), ctypes.byref(a), _raw_stream(dev.index))
+    if rc:
+        _raise(name, rc, f"lines={a.lines} steps={a.steps} c={a.c}")
+
+
+def scan(x, gate, state=None, blend=False, reverse=False, keep=False):
+    """Gated linear recurrence along the lines of ``x [..., steps, c]``:
+    ``h[t] = gate[t] h[t-1] + x[t]``, with ``blend`` ``gate[t] h[t-1] + (1 -
+    gate[t]) x[t]``, for every line and channel by itself: ``(h, last, states)``.
+
+    ``gate`` as ``x`` (any values; 0 starts afresh, so that lines of several
+    lengths can lie behind one another).  ``state [..., c]`` float32: h before the
+    first step (None: zeros).  ``last [..., c]`` float32: h after the last, to go
+    on from (a single step at a time is ``steps`` 1).  ``reverse``: the steps are
+    taken from the last to the first.  The recurrence is held in float32, ``h`` is
+    its rounding to the type of ``x``.  ``states``: with ``keep`` what
+    :func:`scan_backward` needs, h before every 16th step in float32."""
+    a, one, many, dev = _scan_common(x, gate, blend, reverse)
+    if state is not None:
+        _check_like(state, "state", one, torch.float32, dev)
+        a.state = state.data_ptr()
+    h = torch.empty_like(x)
+    last = torch.empty(one, dtype=torch.float32, device=dev)
+    states = torch.empty(many, dtype=torch.float32, device=dev) if keep else None
+    a.h, a.last, a.states = h.data_ptr(), last.data_ptr(), _ptr(states)
+    _scan_call("plattice_scan", a, dev)
+    return h, last, states
+
+
+def scan_backward(grad_h, x, gate, states, grad_last=None, blend=False, reverse=False):
+    """Gradients of :func:`scan` from its inputs and the ``states`` it kept:
+    ``(grad_x, grad_gate, grad_state)``, the first two in the type of ``x``, the
+    last ``[..., c]`` in float32.  ``grad_last`` (float32) is the gradient of
+    ``last``, None for zeros."""
+    a, one, many, dev = _scan_common(x, gate, blend, reverse)
+    _check_like(grad_h, "grad_h", x.shape, x.dtype, dev)
+    _check_like(states, "states", many, torch.float32, dev)
+    if grad_last is not None:
+        _check_like(grad_last, "grad_last", one, torch.float32, dev)
+        a.grad_last = grad_last.data_ptr()
+    grad_x, grad_gate = torch.empty_like(x), torch.empty_like(x)
+    grad_state = torch.empty(one, dtype=torch.float32, device=dev)
+    a.grad_h, a.states = grad_h.data_ptr(), states.data_ptr()
+    a.grad_x, a.grad_gate, a.grad_state = grad_x.data_ptr(), grad_gate.data_ptr(), grad_state.data_ptr()
+    _scan_call("plattice_scan_backward", a, dev)
+    return grad_x, grad_gate, grad_state
+
+
+# ---------------------------------------------------------------- log probabilities
+
+class LogProbs(collections.namedtuple("LogProbs", "logp entropy lse stats top_logp top_ids")):
+    """What :func:`log_probs` gives: ``logp [...]`` of the labels (None without
+    labels), ``entropy [...]``, ``lse [...]`` the logarithm of the sum of the
+    scores' exponentials, ``stats [..., 2]`` its two parts (the largest score, the
+    logarithm of the sum relative to it) for the backward, ``top_logp [..., top]``
+    and ``top_ids [..., top]`` the best alternatives (None without); all float32
+    but the int64 ids."""
+
+    __slots__ = ()
+
+
+def _log_probs_common(logits, labels):
+    _check_rows(logits, "logits")
+    a = _lib.LogProbsArgs()
+    a.logits, a.dtype = logits.data_ptr(), _DTYPES[logits.dtype]
+    a.rows, a.n = _rows_of(logits.shape), int(logits.shape[-1])
+    if labels is not None:
+        _check_labels(labels, "labels", logits.shape[:-1], logits.device)
+        a.labels, a.labels_wide = labels.data_ptr(), labels.dtype == torch.int64
+    return a, tuple(logits.shape[:-1]), logits.device
+
+
+def log_probs(logits, labels=None, top=0):
+    """Log probabilities under the softmax of the rows ``logits [..., n]``:
+    those of ``labels [...]`` (int64 or int32; outside ``0..n-1``, the "ignored"
+    of label maps, 0), the rows' entropies and the ``top`` (at most 32) best
+    alternatives, falling, of equal scores the lowest class first.  Gives
+    :class:`LogProbs`.
+
+    A score of -inf is a class that the row may not have; a row of nothing else
+    has log probabilities of -inf and entropy 0.  NaN or +inf in a row make its
+    numbers NaN (of the alternatives' classes NaN is the last choice)."""
+    a, lead, dev = _log_probs_common(logits, labels)
+    _require(isinstance(top, int) and 0 <= top <= min(_MAX_TOP, a.n), f"top must be in [0, min(n, {_MAX_TOP})]")
+    new = lambda *s, dtype=torch.float32: torch.empty(lead + s, dtype=dtype, device=dev)  # noqa: E731
+    r = LogProbs(None if labels is None else new(), new(), new(), new(2), new(top) if top else None,
+                 new(top, dtype=torch.int64) if top else None)
+    a.logp, a.entropy, a.lse, a.stats = _ptr(r.logp), r.entropy.data_ptr(), r.lse.data_ptr(), r.stats.data_ptr()
+    a.top, a.top_logp, a.top_ids = top, _ptr(r.top_logp), _ptr(r.top_ids)
+    rc = _call(dev.index, _lib_h().plattice_log_probs, ctypes.byref(a), _raw_stream(dev.index))
+    if rc:
+        _raise("plattice_log_probs", rc, f"logits={tuple(logits.shape)} top={top}")
+    return r
+
+
+def log_probs_backward(logits, result, labels=None, grad_logp=None, grad_entropy=None, grad_lse=None):
+    """Gradient of the ``logits`` of :func:`log_probs` in their type, from its
+    ``result``, the same ``labels`` and the gradients (float32 ``[...]``, None for
+    zeros) of ``logp``, ``entropy`` and ``lse``.  The alternatives have none.  A row
+    of -inf only has gradient 0."""
+    a, lead, dev = _log_probs_common(logits, labels)
+    _require(isinstance(result, LogProbs), "result must be LogProbs")
+    _check_like(result.stats, "result.stats", lead + (2,), torch.float32, dev)
+    _require(grad_logp is None or labels is not None, "labels are needed for grad_logp")
+    a.stats = result.stats.data_ptr()
+    if grad_entropy is not None:
+        _check_like(result.entropy, "result.entropy", lead, torch.float32, dev)
+        a.entropy = result.entropy.data_ptr()
+    for name, g in (("grad_logp", grad_logp), ("grad_entropy", grad_entropy), ("grad_lse", grad_lse)):
+        if g is not None:
+            _check_like(g, name, lead, torch.float32, dev)
+            setattr(a, name, g.data_ptr())
+    grad = torch.empty_like(logits)
+    a.grad_logits = grad.data_ptr()
+    rc = _call(dev.index, _lib_h().plattice_log_probs_backward, ctypes.byref(a), _raw_stream(dev.index))
+    if rc:
+        _raise("plattice_log_probs_backward", rc, f"logits={tuple(logits.shape)}")
+    return grad
