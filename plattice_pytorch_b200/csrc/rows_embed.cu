@@ -38,8 +38,10 @@ __global__ void __launch_bounds__(256) k_embed(T* __restrict__ y, Labels ids, co
 #pragma unroll
     for (int u = 0; u < kEmbedUnits; ++u) {
         const unsigned o = u * 256 + threadIdx.x;
+        float f[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[u].set(i, v[u].at(i) * scale);
+        for (int i = 0; i < V; ++i) f[i] = v[u].at(i) * scale;
+        v[u].from(f);
         if (base + o < all) v[u].store(y + (base + o) * V);
     }
 }

@@ -16,6 +16,7 @@
 namespace plr {
 
 constexpr int kSteps = PLATTICE_SCAN_KEEP;
+constexpr int kThreads = 128;
 
 struct ScanArgs {
     const void *x, *a;
@@ -26,149 +27,357 @@ struct ScanArgs {
     const float* grad_last;
     void *gx, *ga;
     float* gs;
-    int64_t lines, steps;
+    float2* sums;            // cut lines: [line][piece][c] (product of the gates, result from 0)
+    float2* tile_sums;       // [line][tile][c], of a CTA's pieces together
+    int64_t lines, steps, blocks;   // blocks of kSteps in a line
+    int64_t tiles;           // CTAs a line's steps are cut over
     int c, reverse;
+    int lanes, pieces;       // of a CTA: lanes x pieces = kThreads
+    int piece_blocks;        // blocks of a piece
 };
 
-// Where a thread's channels lie: element of step s of its line, and of a state.
-struct At {
-    int64_t first, stride;   // of the step taken first, to the next
-    int64_t state;           // in [lines][c]
-    __device__ __forceinline__ At(const ScanArgs& p, int64_t index, int units, int v) {
-        const int64_t line = index / units, col = (index - line * units) * v;
-        first = (line * p.steps + (p.reverse ? p.steps - 1 : 0)) * p.c + col;
-        stride = p.reverse ? -(int64_t)p.c : p.c;
-        state = line * p.c + col;
+// What a thread works on: V channels of a line, blocks first..end-1 of it.  Whole
+// lines: neighbouring threads take neighbouring channels, of several lines where
+// a line has few.  Cut lines: a CTA has `pieces` pieces of its lanes' channels.
+template <int V, bool kCut> struct Work {
+    int64_t line, col, piece, first, end, tile;
+    int lane, own;           // of the CTA's lanes, pieces
+    bool here;
+    __device__ __forceinline__ Work(const ScanArgs& p, int64_t tile_) : tile(tile_) {
+        const int units = p.c / V;
+        if (!kCut) {
+            const int64_t index = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+            lane = own = 0;
+            line = index / units;
+            col = (index - line * units) * V;
+            here = line < p.lines;
+            piece = first = 0;
+            end = p.blocks;
+            return;
+        }
+        lane = threadIdx.x % p.lanes;
+        own = threadIdx.x / p.lanes;
+        const int wide = (units + p.lanes - 1) / p.lanes;
+        line = blockIdx.x / wide;
+        col = ((int64_t)(blockIdx.x - line * wide) * p.lanes + lane) * V;
+        here = col < p.c;
+        piece = tile * p.pieces + own;
+        first = piece * p.piece_blocks;
+        end = first + p.piece_blocks < p.blocks ? first + p.piece_blocks : p.blocks;
     }
 };
 
-template <typename T, int V, bool kBlend>
-__global__ void __launch_bounds__(128) k_scan(ScanArgs p) {
-    const int units = p.c / V;
-    const int64_t index = (int64_t)blockIdx.x * 128 + threadIdx.x;
-    if (index >= p.lines * units) return;
-    const At at(p, index, units, V);
-    const int64_t blocks = (p.steps + kSteps - 1) / kSteps, line = index / units;
+// Element of the first step of block b of a line, and from a step to the next.
+__device__ __forceinline__ int64_t stride_of(const ScanArgs& p) { return p.reverse ? -(int64_t)p.c : p.c; }
+__device__ __forceinline__ int64_t start_of(const ScanArgs& p, int64_t line, int64_t col, int64_t b) {
+    const int64_t t = b * kSteps;
+    int64_t o = (line * p.steps + (p.reverse ? p.steps - 1 - t : t)) * p.c + col;
+    asm volatile("" : "+l"(o));   // one offset a block: otherwise 16 addresses a tensor are carried along in registers
+    return o;
+}
+__device__ __forceinline__ int steps_of(const ScanArgs& p, int64_t b) {
+    const int64_t left = p.steps - b * kSteps;
+    return left < kSteps ? (int)left : kSteps;
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void load_block(Vec<T, V> (&v)[kSteps], const void* base, int64_t o, int64_t stride, int n) {
+    const T* p = static_cast<const T*>(base) + o;
+    if (n == kSteps) {
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i, p += stride) v[i].load(p);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i, p += stride) {
+            if (i < n) v[i].load(p);
+            else v[i].zero();
+        }
+    }
+}
+
+template <bool kBlend> __device__ __forceinline__ float input(float a, float x) { return kBlend ? (1.f - a) * x : x; }
+
+// ---------------------------------------------------------------- cut lines
+//
+// Lines that do not fill the device by themselves are cut: a thread takes a
+// piece, a CTA `pieces` neighbouring ones of its lanes.  The first kernel gives
+// for each piece and for the CTA's pieces together what it does to a state: s ->
+// f s + r.  The second one's CTAs each go through the CTAs before them, then
+// through their own pieces, and know every piece's first state.
+
+__device__ __forceinline__ float2 then(float2 first, float2 second) {   // the map of both
+    return make_float2(first.x * second.x, fmaf(second.x, first.y, second.y));
+}
+
+// Pieces of a backward pass are gone through from the last on.
+template <typename T, int V, bool kBlend, bool kGrad>
+__global__ void __launch_bounds__(kThreads) k_scan_sums(const __grid_constant__ ScanArgs p) {
+    __shared__ float2 shared[kThreads * V];
+    const Work<V, true> w(p, blockIdx.y);
+    float f[V], r[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        f[j] = 1.f;
+        r[j] = 0.f;
+    }
+    if (w.here) {
+        const int64_t stride = stride_of(p);
+        for (int64_t k = w.first; k < w.end; ++k) {
+            const int64_t b = kGrad ? w.first + w.end - 1 - k : k, o = start_of(p, w.line, w.col, b);
+            const int n = steps_of(p, b);
+            Vec<T, V> x[kSteps], a[kSteps];
+            load_block<T, V>(x, kGrad ? p.g : p.x, o, stride, n);
+            load_block<T, V>(a, p.a, o, stride, n);
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                const int t = kGrad ? kSteps - 1 - i : i;
+                if (t < n) {
+#pragma unroll
+                    for (int j = 0; j < V; ++j) {
+                        const float gate = a[t].at(j), v = x[t].at(j);
+                        r[j] = kGrad ? gate * (v + r[j]) : fmaf(gate, r[j], input<kBlend>(gate, v));
+                        f[j] *= gate;
+                    }
+                }
+            }
+        }
+        if (w.first < p.blocks)
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                p.sums[(w.line * p.tiles * p.pieces + w.piece) * p.c + w.col + j] = make_float2(f[j], r[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) shared[threadIdx.x * V + j] = make_float2(f[j], r[j]);
+    __syncthreads();
+    if (w.own == 0 && w.here)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            float2 all = make_float2(1.f, 0.f);
+            for (int k = 0; k < p.pieces; ++k)
+                all = then(all, shared[((kGrad ? p.pieces - 1 - k : k) * p.lanes + w.lane) * V + j]);
+            p.tile_sums[(w.line * p.tiles + w.tile) * p.c + w.col + j] = all;
+        }
+}
+
+// The state that the thread's piece starts from: s goes through the maps of the
+// CTAs before, in as many parts as the CTA has pieces, then of its pieces before.
+template <int V, bool kGrad>
+__device__ __forceinline__ void first_state(float (&s)[V], const ScanArgs& p, const Work<V, true>& w) {
+    __shared__ float2 shared[kThreads * V];
+    const int64_t before = kGrad ? p.tiles - 1 - w.tile : w.tile, part = (before + p.pieces - 1) / p.pieces;
+    float2 all[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) all[j] = make_float2(1.f, 0.f);
+    if (w.here) {
+        const int64_t to = (w.own + 1) * part < before ? (w.own + 1) * part : before;
+        const float2* sums = p.tile_sums + w.line * p.tiles * p.c + w.col;
+        for (int64_t k = w.own * part; k < to; k += 8) {
+            float2 m[8][V];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    m[i][j] = k + i < to ? sums[(kGrad ? p.tiles - 1 - k - i : k + i) * p.c + j] : make_float2(1.f, 0.f);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int j = 0; j < V; ++j) all[j] = then(all[j], m[i][j]);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) shared[threadIdx.x * V + j] = all[j];
+    __syncthreads();
+    if (w.here) {
+        for (int k = 0; k < p.pieces; ++k)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float2 m = shared[(k * p.lanes + w.lane) * V + j];
+                s[j] = fmaf(m.x, s[j], m.y);
+            }
+        const float2* sums = p.sums + (w.line * p.tiles + w.tile) * p.pieces * p.c + w.col;
+        for (int k = 0; k < (kGrad ? p.pieces - 1 - w.own : w.own); ++k) {
+            const int other = kGrad ? p.pieces - 1 - k : k;
+            if ((w.tile * p.pieces + other) * p.piece_blocks < p.blocks)
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const float2 m = sums[(int64_t)other * p.c + j];
+                    s[j] = fmaf(m.x, s[j], m.y);
+                }
+        }
+    }
+}
+
+// ---------------------------------------------------------------- the passes
+
+template <typename T, int V, bool kBlend, bool kCut>
+__global__ void __launch_bounds__(kThreads) k_scan(const __grid_constant__ ScanArgs p) {
+    const Work<V, kCut> w(p, kCut ? (int64_t)gridDim.y - 1 - blockIdx.y : 0);   // what was read last may still be in the L2
     float h[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) h[j] = p.state ? p.state[at.state + j] : 0.f;
-    for (int64_t b = 0; b < blocks; ++b) {
-        const int64_t t0 = b * kSteps;
-        const int n = p.steps - t0 < kSteps ? (int)(p.steps - t0) : kSteps;
-        const int64_t o = at.first + t0 * at.stride;
+    for (int j = 0; j < V; ++j) h[j] = w.here && p.state ? p.state[w.line * p.c + w.col + j] : 0.f;
+    if constexpr (kCut) first_state<V, false>(h, p, w);
+    if (!w.here || w.first >= p.blocks) return;
+    const int64_t stride = stride_of(p);
+    for (int64_t b = w.first; b < w.end; ++b) {
+        const int n = steps_of(p, b);
+        const int64_t o = start_of(p, w.line, w.col, b);
         Vec<T, V> x[kSteps], a[kSteps];
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i)
-            if (i < n) {
-                x[i].load(static_cast<const T*>(p.x) + o + i * at.stride);
-                a[i].load(static_cast<const T*>(p.a) + o + i * at.stride);
-            }
+        load_block<T, V>(x, p.x, o, stride, n);
+        load_block<T, V>(a, p.a, o, stride, n);
         if (p.states) {
-            float* s = p.states + (line * blocks + b) * p.c + (at.state - line * p.c);
+            float* s = p.states + (w.line * p.blocks + b) * p.c + w.col;
 #pragma unroll
             for (int j = 0; j < V; ++j) s[j] = h[j];
         }
+        T* y = static_cast<T*>(p.h) + o;
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i)
+        for (int i = 0; i < kSteps; ++i, y += stride) {
             if (i < n) {
-                Vec<T, V> y;
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    const float g = a[i].at(j), u = kBlend ? (1.f - g) * x[i].at(j) : x[i].at(j);
-                    h[j] = fmaf(g, h[j], u);
-                    y.set(j, h[j]);
+                    const float gate = a[i].at(j);
+                    h[j] = fmaf(gate, h[j], input<kBlend>(gate, x[i].at(j)));
                 }
-                y.store(static_cast<T*>(p.h) + o + i * at.stride);
+                Vec<T, V> v;
+                v.from(h);
+                v.store(y);
             }
+        }
     }
-    if (p.last)
+    if (p.last && w.end == p.blocks)
 #pragma unroll
-        for (int j = 0; j < V; ++j) p.last[at.state + j] = h[j];
+        for (int j = 0; j < V; ++j) p.last[w.line * p.c + w.col + j] = h[j];
 }
 
-template <typename T, int V, bool kBlend>
-__global__ void __launch_bounds__(128) k_scan_grad(ScanArgs p) {
-    const int units = p.c / V;
-    const int64_t index = (int64_t)blockIdx.x * 128 + threadIdx.x;
-    if (index >= p.lines * units) return;
-    const At at(p, index, units, V);
-    const int64_t blocks = (p.steps + kSteps - 1) / kSteps, line = index / units;
+template <typename T, int V, bool kBlend, bool kCut>
+__global__ void __launch_bounds__(kThreads, 4) k_scan_grad(const __grid_constant__ ScanArgs p) {
+    const Work<V, kCut> w(p, kCut ? blockIdx.y : 0);
     float r[V];   // what reaches h from later steps
 #pragma unroll
-    for (int j = 0; j < V; ++j) r[j] = p.grad_last ? p.grad_last[at.state + j] : 0.f;
-    for (int64_t b = blocks - 1; b >= 0; --b) {
-        const int64_t t0 = b * kSteps;
-        const int n = p.steps - t0 < kSteps ? (int)(p.steps - t0) : kSteps;
-        const int64_t o = at.first + t0 * at.stride;
+    for (int j = 0; j < V; ++j) r[j] = w.here && p.grad_last ? p.grad_last[w.line * p.c + w.col + j] : 0.f;
+    if constexpr (kCut) first_state<V, true>(r, p, w);
+    if (!w.here || w.first >= p.blocks) return;
+    const int64_t stride = stride_of(p);
+    for (int64_t b = w.end - 1; b >= w.first; --b) {
+        const int n = steps_of(p, b);
+        const int64_t o = start_of(p, w.line, w.col, b);
         Vec<T, V> x[kSteps], a[kSteps], g[kSteps];
         float h[V], d[kSteps][V];   // d: h[t-1], or h[t-1] - x[t]
-        const float* s = p.states + (line * blocks + b) * p.c + (at.state - line * p.c);
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i)
-            if (i < n) {
-                x[i].load(static_cast<const T*>(p.x) + o + i * at.stride);
-                a[i].load(static_cast<const T*>(p.a) + o + i * at.stride);
-                g[i].load(static_cast<const T*>(p.g) + o + i * at.stride);
-            }
+        const float* s = p.states + (w.line * p.blocks + b) * p.c + w.col;
 #pragma unroll
         for (int j = 0; j < V; ++j) h[j] = s[j];
+        load_block<T, V>(x, p.x, o, stride, n);
+        load_block<T, V>(a, p.a, o, stride, n);
+        load_block<T, V>(g, p.g, o, stride, n);
 #pragma unroll
         for (int i = 0; i < kSteps; ++i)
-            if (i < n) {
 #pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const float ga = a[i].at(j), xv = x[i].at(j);
-                    d[i][j] = kBlend ? h[j] - xv : h[j];
-                    h[j] = fmaf(ga, h[j], kBlend ? (1.f - ga) * xv : xv);
-                }
+            for (int j = 0; j < V; ++j) {
+                const float gate = a[i].at(j), v = x[i].at(j);
+                d[i][j] = kBlend ? h[j] - v : h[j];
+                h[j] = fmaf(gate, h[j], input<kBlend>(gate, v));
             }
+        T* gx = static_cast<T*>(p.gx) + o + (kSteps - 1) * stride;
+        T* ga = static_cast<T*>(p.ga) + o + (kSteps - 1) * stride;
 #pragma unroll
-        for (int i = kSteps - 1; i >= 0; --i)
+        for (int i = kSteps - 1; i >= 0; --i, gx -= stride, ga -= stride)
             if (i < n) {
-                Vec<T, V> gx, ga;
+                float fx[V], fa[V];
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
                     const float gate = a[i].at(j), whole = g[i].at(j) + r[j];
-                    gx.set(j, kBlend ? (1.f - gate) * whole : whole);
-                    ga.set(j, whole * d[i][j]);
+                    fx[j] = kBlend ? (1.f - gate) * whole : whole;
+                    fa[j] = whole * d[i][j];
                     r[j] = gate * whole;
                 }
-                gx.store(static_cast<T*>(p.gx) + o + i * at.stride);
-                ga.store(static_cast<T*>(p.ga) + o + i * at.stride);
+                Vec<T, V> vx, va;
+                vx.from(fx);
+                va.from(fa);
+                vx.store(gx);
+                va.store(ga);
             }
     }
-    if (p.gs)
+    if (p.gs && w.first == 0)
 #pragma unroll
-        for (int j = 0; j < V; ++j) p.gs[at.state + j] = r[j];
+        for (int j = 0; j < V; ++j) p.gs[w.line * p.c + w.col + j] = r[j];
 }
 
 // ------------------------------------------------------------------ host side
 
+// Threads that fill the device (each has 16 steps of two or three tensors in
+// flight), and those below which lines are cut: a cut line is read twice.
+constexpr int64_t kEnough = 148 * 512, kFew = 148 * 192;
+
+struct ScanPlan {
+    int v, lanes, pieces, piece_blocks;
+    int64_t wide, tiles, tile_sums, bytes;   // wide: CTAs beside one another
+    bool cut;
+};
+
+static ScanPlan scan_plan(const plattice_scan_args* q, bool grad) {
+    ScanPlan p = {};
+    uintptr_t bits = (uintptr_t)q->x | (uintptr_t)q->gate;
+    bits |= grad ? (uintptr_t)q->grad_h | (uintptr_t)q->grad_x | (uintptr_t)q->grad_gate : (uintptr_t)q->h;
+    const int v = widest(q->c, dtype_size(q->dtype), bits);
+    p.v = q->dtype != PLATTICE_F32 && v >= 2 ? 2 : 1;
+    const int64_t units = q->c / p.v, blocks = ceil_div(q->steps, kSteps), threads = q->lines * units;
+    p.cut = threads < kFew && blocks >= 8;
+    p.tiles = 1;
+    if (!p.cut) {
+        p.wide = ceil_div(threads, kThreads);
+        return p;
+    }
+    p.lanes = 1;
+    while (p.lanes < 32 && p.lanes < units) p.lanes <<= 1;
+    const int64_t length = blocks / ceil_div(kEnough, threads);
+    p.piece_blocks = length < 1 ? 1 : length > (1 << 20) ? 1 << 20 : (int)length;
+    p.pieces = kThreads / p.lanes;
+    p.wide = q->lines * ceil_div(units, p.lanes);
+    p.tiles = ceil_div(blocks, (int64_t)p.piece_blocks * p.pieces);
+    const int64_t one = q->lines * p.tiles * q->c * (int64_t)sizeof(float2);
+    p.tile_sums = one * p.pieces;
+    p.bytes = one * (p.pieces + 1);
+    return p;
+}
+
 template <typename T, int V, bool kBlend>
-static cudaError_t launch(const ScanArgs& p, bool grad, cudaStream_t s) {
-    const int64_t ctas = ceil_div(p.lines * (p.c / V), 128);
-    if (ctas > 0x7fffffff) return cudaErrorInvalidValue;
-    if (grad) k_scan_grad<T, V, kBlend><<<(unsigned)ctas, 128, 0, s>>>(p);
-    else k_scan<T, V, kBlend><<<(unsigned)ctas, 128, 0, s>>>(p);
+static cudaError_t launch(const ScanArgs& a, const ScanPlan& p, bool grad, cudaStream_t s) {
+    if (p.wide > 0x7fffffff || p.tiles > 65535) return cudaErrorInvalidValue;
+    const dim3 grid((unsigned)p.wide, (unsigned)p.tiles);
+    if (grad) {
+        if (p.cut) {
+            k_scan_sums<T, V, kBlend, true><<<grid, kThreads, 0, s>>>(a);
+            k_scan_grad<T, V, kBlend, true><<<grid, kThreads, 0, s>>>(a);
+        } else {
+            k_scan_grad<T, V, kBlend, false><<<grid, kThreads, 0, s>>>(a);
+        }
+    } else if (p.cut) {
+        k_scan_sums<T, V, kBlend, false><<<grid, kThreads, 0, s>>>(a);
+        k_scan<T, V, kBlend, true><<<grid, kThreads, 0, s>>>(a);
+    } else {
+        k_scan<T, V, kBlend, false><<<grid, kThreads, 0, s>>>(a);
+    }
     return cudaGetLastError();
 }
 
 template <typename T>
-static cudaError_t launch(const ScanArgs& p, bool blend, bool grad, int v, cudaStream_t s) {
+static cudaError_t launch(const ScanArgs& a, const ScanPlan& p, bool blend, bool grad, cudaStream_t s) {
     constexpr int kPair = sizeof(T) == 2 ? 2 : 1;
-    if (v >= kPair) return blend ? launch<T, kPair, true>(p, grad, s) : launch<T, kPair, false>(p, grad, s);
-    return blend ? launch<T, 1, true>(p, grad, s) : launch<T, 1, false>(p, grad, s);
+    if (p.v == kPair) return blend ? launch<T, kPair, true>(a, p, grad, s) : launch<T, kPair, false>(a, p, grad, s);
+    return blend ? launch<T, 1, true>(a, p, grad, s) : launch<T, 1, false>(a, p, grad, s);
 }
 
 static int run(const plattice_scan_args* q, bool grad, cudaStream_t s, const char* call) {
-    const ScanArgs p{q->x, q->gate, q->state, q->h, q->last, q->states, q->grad_h, q->grad_last, q->grad_x, q->grad_gate,
-                     q->grad_state, q->lines, q->steps, q->c, q->reverse};
-    uintptr_t bits = (uintptr_t)p.x | (uintptr_t)p.a;
-    bits |= grad ? (uintptr_t)p.g | (uintptr_t)p.gx | (uintptr_t)p.ga : (uintptr_t)p.h;
-    const int v = widest(p.c, dtype_size(q->dtype), bits);
-    const cudaError_t e = q->dtype == PLATTICE_F32    ? launch<float>(p, q->blend, grad, v, s)
-                          : q->dtype == PLATTICE_BF16 ? launch<__nv_bfloat16>(p, q->blend, grad, v, s)
-                                                      : launch<__half>(p, q->blend, grad, v, s);
+    const ScanPlan p = scan_plan(q, grad);
+    if (p.bytes && (!q->workspace || ((uintptr_t)q->workspace & 255) || q->workspace_bytes < (size_t)p.bytes))
+        return PLATTICE_ERR_WORKSPACE;
+    float2* ws = static_cast<float2*>(q->workspace);
+    const ScanArgs a{q->x, q->gate, q->state, q->h, q->last, q->states, q->grad_h, q->grad_last, q->grad_x, q->grad_gate,
+                     q->grad_state, ws, ws + p.tile_sums / (int64_t)sizeof(float2), q->lines, q->steps,
+                     ceil_div(q->steps, kSteps), p.tiles, q->c, q->reverse, p.lanes, p.pieces, p.piece_blocks};
+    const cudaError_t e = q->dtype == PLATTICE_F32    ? launch<float>(a, p, q->blend, grad, s)
+                          : q->dtype == PLATTICE_BF16 ? launch<__nv_bfloat16>(a, p, q->blend, grad, s)
+                                                      : launch<__half>(a, p, q->blend, grad, s);
     return rows_status(e, call);
 }
 
@@ -185,7 +394,7 @@ extern "C" {
 
 int plattice_scan_workspace_size(const plattice_scan_args* q, size_t* bytes) {
     if (!bytes || !shape_ok(q)) return PLATTICE_ERR_INVALID;
-    *bytes = 0;
+    *bytes = q->lines && q->steps ? (size_t)scan_plan(q, false).bytes : 0;
     return PLATTICE_OK;
 }
 
@@ -205,7 +414,9 @@ int plattice_scan(const plattice_scan_args* q, void* stream) {
 }
 
 int plattice_scan_backward_workspace_size(const plattice_scan_args* q, size_t* bytes) {
-    return plattice_scan_workspace_size(q, bytes);
+    if (!bytes || !shape_ok(q)) return PLATTICE_ERR_INVALID;
+    *bytes = q->lines && q->steps ? (size_t)scan_plan(q, true).bytes : 0;
+    return PLATTICE_OK;
 }
 
 int plattice_scan_backward(const plattice_scan_args* q, void* stream) {
