@@ -11,7 +11,7 @@
 // confident answer keep their precision.
 //
 // A row is read once and held: few classes by a thread out of shared memory,
-// up to kWarpVectors accesses a lane by a warp in registers, more by a CTA or a
+// up to five accesses a lane by a warp in registers, more by a CTA or a
 // cluster of them in registers, and only rows that no cluster holds are read
 // again.  So the largest score is known before the first exponential, which
 // costs a subtraction, a product, a bound, the exponential and two sums (five
@@ -40,6 +40,8 @@ struct LogpArgs {
     void* gx;
     int64_t rows;
     int n, top;
+    template <typename T> __device__ __forceinline__ const T* lo() const { return static_cast<const T*>(x); }
+    template <typename T> __device__ __forceinline__ const T* hi() const { return static_cast<const T*>(x) + rows * n; }
 };
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -58,20 +60,33 @@ template <typename T> struct Piece {
         if (std::is_same<T, float>::value) return 0xff800000u;
         return std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
     }
-    __device__ __forceinline__ void load(const T* x, int64_t first, int n) {
+    // Elements first.. of the row x[0..n), which lies in a tensor lo..hi.
+    __device__ __forceinline__ void load(const T* x, int64_t first, int64_t n, const T* lo, const T* hi) {
+        const T* at = x + first;
         if (first >= 0 && first + kN <= n) {
-            q = *reinterpret_cast<const uint4*>(x + first);
-        } else {
-            q = make_uint4(closed(), closed(), closed(), closed());
-            if (first > -kN && first < n) {
-                union { uint4 u; T e[kN]; } r;
-                r.u = q;
-#pragma unroll
-                for (int i = 0; i < kN; ++i)
-                    if (first + i >= 0 && first + i < n) r.e[i] = x[first + i];
-                q = r.u;
-            }
+            q = *reinterpret_cast<const uint4*>(at);
+            return;
         }
+        if (first <= -kN || first >= n) {
+            q = make_uint4(closed(), closed(), closed(), closed());
+            return;
+        }
+        union { uint4 u; T e[kN]; uint16_t h[8]; uint32_t w[4]; } r;
+        r.u = make_uint4(closed(), closed(), closed(), closed());
+        if (at >= lo && at + kN <= hi) {   // the neighbouring rows' elements come along
+            r.u = *reinterpret_cast<const uint4*>(at);
+#pragma unroll
+            for (int i = 0; i < kN; ++i)
+                if (first + i < 0 || first + i >= n) {
+                    if constexpr (sizeof(T) == 4) r.w[i] = closed();
+                    else r.h[i] = (uint16_t)closed();
+                }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kN; ++i)
+                if (first + i >= 0 && first + i < n) r.e[i] = x[first + i];
+        }
+        q = r.u;
     }
     __device__ __forceinline__ uint32_t word(int i) const { return i == 0 ? q.x : i == 1 ? q.y : i == 2 ? q.z : q.w; }
     __device__ __forceinline__ float2 pair(int i) const {   // elements 2 i, 2 i + 1
@@ -83,6 +98,30 @@ template <typename T> struct Piece {
             const uint32_t w = word(i);
             return __half22float2(*reinterpret_cast<const __half2*>(&w));
         }
+    }
+    // Puts -inf in the place of elements equal to m; gives their number.
+    __device__ __forceinline__ int take(float m) {
+        int count = 0;
+        if constexpr (std::is_same<T, float>::value) {
+            uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (__uint_as_float(w[i]) == m) w[i] = closed(), ++count;
+            q = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+            typedef typename Pair<T>::type P;
+            P both_m;
+            pair_from(both_m, m, m);
+            uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t same = __heq2_mask(*reinterpret_cast<const P*>(&w[i]), both_m);
+                w[i] = (w[i] & ~same) | (same & closed());
+                count += __popc(same) >> 4;
+            }
+            q = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        return count;
     }
     __device__ __forceinline__ float most() const {   // NaN where there is one
         if constexpr (std::is_same<T, float>::value) {
@@ -125,45 +164,38 @@ struct Sums {
     int equal;
 };
 
+// `own`: the largest of these scores.  The few threads that hold the largest of
+// the row first take it out.
 template <typename T, int K>
-__device__ __forceinline__ void add_up(Sums& s, const Piece<T> (&q)[K], float m, float own) {
+__device__ __forceinline__ void add_up(Sums& s, const Piece<T> (&all)[K], float m, float own) {
     constexpr int kPairs = Piece<T>::kN / 2;
-    const uint64_t minus = both(-m), scale = both(kLog2e);
-    if (own < m) {   // no score of this thread's is the largest
-        uint64_t sum = 0ull, weighted = 0ull;
+    Piece<T> q[K];
 #pragma unroll
-        for (int k = 0; k < K; ++k)
+    for (int k = 0; k < K; ++k) q[k] = all[k];
+    if (own == m) {
 #pragma unroll
-            for (int i = 0; i < kPairs; ++i) {
-                const float2 v = q[k].pair(i);
-                float a, b;
-                pair_to(mul2(add2(pair_of(v.x, v.y), minus), scale), a, b);
-                a = fmaxf(a, kLowest);
-                b = fmaxf(b, kLowest);
-                const uint64_t e = pair_of(exp2_fast(a), exp2_fast(b));
-                sum = add2(sum, e);
-                weighted = fma2(e, pair_of(a, b), weighted);
-            }
-        float a, b;
-        pair_to(sum, a, b);
-        s.below += a + b;
-        pair_to(weighted, a, b);
-        s.weighted += a + b;
-    } else {
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-#pragma unroll
-            for (int i = 0; i < 2 * kPairs; ++i) {
-                const float2 v = q[k].pair(i / 2);
-                const float d = (i % 2 ? v.y : v.x) - m, t = fmaxf(d * kLog2e, kLowest), e = exp2_fast(t);
-                if (d == 0.f) {
-                    ++s.equal;
-                } else {
-                    s.below += e;
-                    s.weighted = fmaf(e, t, s.weighted);
-                }
-            }
+        for (int k = 0; k < K; ++k) s.equal += q[k].take(m);
     }
+    const uint64_t minus = both(-m), scale = both(kLog2e);
+    uint64_t sum = 0ull, weighted = 0ull;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) {
+            const float2 v = q[k].pair(i);
+            float a, b;
+            pair_to(mul2(add2(pair_of(v.x, v.y), minus), scale), a, b);
+            a = fmaxf(a, kLowest);
+            b = fmaxf(b, kLowest);
+            const uint64_t e = pair_of(exp2_fast(a), exp2_fast(b));
+            sum = add2(sum, e);
+            weighted = fma2(e, pair_of(a, b), weighted);
+        }
+    float a, b;
+    pair_to(sum, a, b);
+    s.below += a + b;
+    pair_to(weighted, a, b);
+    s.weighted += a + b;
 }
 
 // A row's numbers from its sums, written by one thread.
@@ -208,250 +240,392 @@ __device__ __forceinline__ uint64_t warp_best(uint64_t v) {
     return (uint64_t)hi << 32 | lo;
 }
 
-constexpr int kCandidates = 96;   // of a warp
+// The `top` best of `count` distinct keys, out[i] the i-th; by a warp.
+__device__ __forceinline__ void in_order(uint64_t* out, const uint64_t* keys, int count, int top) {
+    for (int i = threadIdx.x & 31; i < count; i += 32) {
+        const uint64_t mine = keys[i];
+        int greater = 0;
+        for (int j = 0; j < count; ++j) greater += keys[j] > mine;
+        if (greater < top) out[greater] = mine;
+    }
+}
 
-// The `top` best of `count` keys in shared memory: lane i gets the i-th (0 where
-// there are fewer).
-__device__ __forceinline__ uint64_t best_of(const uint64_t* keys, int count, int top) {
-    const int lane = threadIdx.x & 31;
-    uint64_t mine = 0, before = ~0ull;
-    for (int k = 0; k < top; ++k) {
-        uint64_t b = 0;
-        for (int i = lane; i < count; i += 32) {
-            const uint64_t v = keys[i];
+// The scores that are at least `bound`, anywhere in a thread's pieces (element i of
+// piece k is class first + k step + i), go to `room` in any order: the keys differ.
+template <typename T, int K>
+__device__ __forceinline__ void gather(const Piece<T> (&q)[K], int64_t first, int64_t step, float bound, uint64_t* room, int* count,
+                                       int most) {
+    constexpr int kN = Piece<T>::kN;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        if (!(q[k].most() >= bound)) continue;
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            const float2 f = q[k].pair(i / 2);
+            const float x = i % 2 ? f.y : f.x;
+            if (x >= bound) {
+                const int at = atomicAdd(count, 1);
+                if (at < most) room[at] = ranked(x, first + k * step + i);
+            }
+        }
+    }
+}
+
+// The best key below `before` of the pieces first, first + step, .. < end of a row,
+// read again: for rows whose scores are so alike (or so many -inf) that no bound
+// keeps the candidates few.
+template <typename T>
+__device__ __forceinline__ uint64_t best_below(const LogpArgs& p, const T* x, int64_t first, int64_t step, int64_t end, uint64_t before) {
+    constexpr int kN = Piece<T>::kN;
+    uint64_t b = 0;
+#pragma unroll 1
+    for (; first < end; first += step) {
+        Piece<T> q;
+        q.load(x, first, end, p.lo<T>(), p.hi<T>());
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            const int64_t j = first + i;
+            const float2 f = q.pair(i / 2);
+            const uint64_t v = j >= 0 && j < end ? ranked(i % 2 ? f.y : f.x, j) : 0;
             if (v < before && v > b) b = v;
         }
-        before = warp_best(b);
-        if (lane == k) mine = before;
     }
-    return mine;
+    return b;
 }
 
-// The `top` best of a warp's pieces (element i of piece k is class first + k step
-// + i) and of a list from before, held as the result.  The scores that are at
-// least the top-th largest of the lanes' own largest ones hold them all; mostly
-// they are few more, and only they are put in order.
-template <typename T, int K>
-__device__ __forceinline__ uint64_t best_of_pieces(const Piece<T> (&q)[K], int64_t first, int64_t step, int n, float own, bool plain,
-                                                   int top, uint64_t list, uint64_t* room, int* count) {
-    constexpr int kN = Piece<T>::kN;
-    const int lane = threadIdx.x & 31;
-    if (plain) {
-        float bound = 0.f, v = own;
-        for (int k = 0; k < top; ++k) {
-            bound = warp_max(v);
-            const unsigned at = __ballot_sync(0xffffffffu, v == bound);
-            if (lane == __ffs(at) - 1) v = -INFINITY;
-        }
-        if (lane == 0) *count = 0;
-        __syncwarp();
-        if (bound > -INFINITY) {
-            if (own >= bound) {
-#pragma unroll
-                for (int k = 0; k < K; ++k) {
-                    if (!(q[k].most() >= bound)) continue;
-#pragma unroll
-                    for (int i = 0; i < kN; ++i) {
-                        const float2 f = q[k].pair(i / 2);
-                        const float x = i % 2 ? f.y : f.x;
-                        if (x >= bound) {   // never outside the row
-                            const int at = atomicAdd(count, 1);   // in any order: all keys differ
-                            if (at < kCandidates) room[at] = ranked(x, first + k * step + i);
-                        }
-                    }
-                }
-            }
-            __syncwarp();
-            const int c = *count;
-            if (c + 32 <= kCandidates) {
-                room[c + lane] = list;
-                __syncwarp();
-                const uint64_t got = best_of(room, c + 32, top);
-                __syncwarp();
-                return got;
-            }
-        }
-        __syncwarp();
-    }
-    uint64_t mine = 0, before = ~0ull;
-    for (int t = 0; t < top; ++t) {
-        uint64_t b = list < before ? list : 0;
-#pragma unroll 1
-        for (int k = 0; k < K; ++k) {
-            Piece<T> piece = q[0];
-#pragma unroll
-            for (int o = 1; o < K; ++o)
-                if (o == k) piece = q[o];
-#pragma unroll
-            for (int i = 0; i < kN; ++i) {
-                const int64_t j = first + k * step + i;
-                const float2 f = piece.pair(i / 2);
-                const uint64_t v = j >= 0 && j < n ? ranked(i % 2 ? f.y : f.x, j) : 0;
-                if (v < before && v > b) b = v;
-            }
-        }
-        before = warp_best(b);
-        if (lane == t) mine = before;
-    }
-    return mine;
-}
-
-__device__ __forceinline__ void write_top(const LogpArgs& p, int64_t row, const Row& r, uint64_t mine) {
-    const int lane = threadIdx.x & 31;
-    if (lane < p.top) {
-        p.top_ids[row * p.top + lane] = class_of(mine);
-        p.top_logp[row * p.top + lane] = r.logp(score_of(mine));
-    }
+__device__ __forceinline__ void write_top(const LogpArgs& p, int64_t row, int place, uint64_t key, float m, float s) {
+    p.top_ids[row * p.top + place] = class_of(key);
+    p.top_logp[row * p.top + place] = m == -INFINITY ? -INFINITY : (score_of(key) - m) - s;
 }
 
 // ------------------------------------------------------------- a row by a warp
+//
+// Up to 16 neighbouring rows one after the other, the next one's loads under way;
+// lane r keeps row r's sums, and the logarithms, quotients and stores of all of
+// them are made together at the end (one by one they cost more than the
+// exponentials of 256 classes).
 
-constexpr int kWarpVectors = 5;
+constexpr int kWarpRows = 16, kWarpRoom = 64;
 
-template <typename T, int K, int kRows>
-__global__ void __launch_bounds__(256) k_logp_warp(const __grid_constant__ LogpArgs p) {
-    __shared__ uint64_t room[8][kCandidates];
-    __shared__ int count[8];
+template <typename T, int K, bool kTop>
+__global__ void __launch_bounds__(128) k_logp_warp(const __grid_constant__ LogpArgs p, int rows_each) {
+    __shared__ uint64_t room[4][kWarpRoom];
+    __shared__ int count[4];
+    extern __shared__ uint64_t staged[];   // [4][rows_each][top]
     constexpr int kN = Piece<T>::kN;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int64_t base = ((int64_t)blockIdx.x * 8 + warp) * kRows; base < p.rows; base += (int64_t)gridDim.x * 8 * kRows) {
-        Piece<T> q[kRows][K];
-        int64_t first[kRows];
-#pragma unroll
-        for (int r = 0; r < kRows; ++r) {
+    uint64_t* best = staged + (size_t)warp * rows_each * p.top;
+    const int64_t all = (p.rows + rows_each - 1) / rows_each;
+    for (int64_t group = (int64_t)blockIdx.x * 4 + warp; group < all; group += (int64_t)gridDim.x * 4) {
+        const int64_t base = group * rows_each;
+        const int rows = p.rows - base < rows_each ? (int)(p.rows - base) : rows_each;
+        Piece<T> q[K], next[K];
+        int64_t first = 0, first_next;
+        const auto load = [&](int r) {
             const T* x = static_cast<const T*>(p.x) + (base + r) * p.n;
-            first[r] = (int64_t)lane * kN - Piece<T>::shift_of(x);
-            const int n = base + r < p.rows ? p.n : 0;
+            first_next = (int64_t)lane * kN - Piece<T>::shift_of(x);
 #pragma unroll
-            for (int k = 0; k < K; ++k) q[r][k].load(x, first[r] + k * 32 * kN, n);
-        }
+            for (int k = 0; k < K; ++k) next[k].load(x, first_next + k * 32 * kN, r < rows ? p.n : -kN, p.lo<T>(), p.hi<T>());
+        };
+        load(0);
+        float most = 0.f;
+        Sums sums = {0.f, 0.f, 0};
+        for (int r = 0; r < rows; ++r) {
 #pragma unroll
-        for (int r = 0; r < kRows; ++r) {
-            const int64_t row = base + r;
-            if (row >= p.rows) break;
-            float own = q[r][0].most();
+            for (int k = 0; k < K; ++k) q[k] = next[k];
+            first = first_next;
+            load(r + 1);
+            float own = q[0].most();
 #pragma unroll
-            for (int k = 1; k < K; ++k) own = max_nan(own, q[r][k].most());
+            for (int k = 1; k < K; ++k) own = max_nan(own, q[k].most());
             const float m = warp_max(own);
             const bool plain = m < INFINITY && m > -INFINITY;
+            if (kTop) {
+                // The scores that are at least the top-th largest of the lanes' largest ones
+                // hold the best; mostly they are few more.
+                bool done = false;
+                uint64_t* out = best + r * p.top;
+                if (plain) {
+                    float bound = 0.f, v = own;
+                    for (int k = 0; k < p.top; ++k) {
+                        bound = warp_max(v);
+                        const unsigned at = __ballot_sync(0xffffffffu, v == bound);
+                        if (lane == __ffs(at) - 1) v = -INFINITY;
+                    }
+                    if (lane == 0) count[warp] = 0;
+                    __syncwarp();
+                    if (bound > -INFINITY) {
+                        if (own >= bound) gather(q, first, 32 * kN, bound, room[warp], &count[warp], kWarpRoom);
+                        __syncwarp();
+                        const int c = count[warp];
+                        done = c <= kWarpRoom;
+                        if (done) in_order(out, room[warp], c, p.top);
+                    }
+                    __syncwarp();
+                }
+                if (!done) {
+                    uint64_t before = ~0ull;
+                    for (int k = 0; k < p.top; ++k) {
+                        before = warp_best(best_below(p, static_cast<const T*>(p.x) + (base + r) * p.n, first, 32 * kN, p.n, before));
+                        if (lane == 0) out[k] = before;
+                    }
+                }
+            }
             Sums t = {0.f, 0.f, 0};
             if (plain) {
-                add_up(t, q[r], m, own);
+                add_up(t, q, m, own);
                 warp_sums(t.below, t.weighted);
                 t.equal = (int)__reduce_add_sync(0xffffffffu, (unsigned)t.equal);
             }
-            const Row done(m, t.below, t.equal);
-            if (lane == 0) done.write(p, row, static_cast<const T*>(p.x) + row * p.n, t);
-            if (p.top)
-                write_top(p, row, done, best_of_pieces(q[r], first[r], 32 * kN, p.n, own, plain, p.top, 0, room[warp], &count[warp]));
+            if (lane == r) {
+                most = m;
+                sums = t;
+            }
+        }
+        const Row mine(most, sums.below, sums.equal);
+        if (lane < rows) mine.write(p, base + lane, static_cast<const T*>(p.x) + (base + lane) * p.n, sums);
+        if (kTop) {
+            __syncwarp();
+            for (int i = 0; i < rows * p.top; i += 32) {
+                const int e = i + lane, r = e / p.top;
+                const float m = __shfl_sync(0xffffffffu, mine.m, r & 31), s = __shfl_sync(0xffffffffu, mine.s, r & 31);
+                if (e < rows * p.top) write_top(p, base + r, e - r * p.top, best[e], m, s);
+            }
+            __syncwarp();
         }
     }
 }
 
-// ------------------------------------------------------------- a row by a cluster
+// ------------------------------------------------------------- a row by CTAs
+//
+// A CTA of kThreads, or a cluster of per_row of them, goes through rows, kPieces
+// accesses a thread and row.  kLoop false: the accesses of the next two rows are
+// under way as asynchronous copies, to places in shared memory that only the
+// thread itself reads, so that they need no barrier.  kLoop true: rows that no
+// cluster holds; each CTA takes its share in `rounds`, twice.  What is left to do
+// for a row when its sums are known is made for 32 rows at a time.
 
-// CTAs of kThreads threads, gridDim a multiple of the cluster.  Each holds K
-// pieces a thread at a time, `rounds` times; a row of one round is read once.
-template <typename T, int K, int kThreads>
-__global__ void __launch_bounds__(kThreads) k_logp_cluster(const __grid_constant__ LogpArgs p, int rounds, int per_row) {
-    constexpr int kWarps = kThreads / 32, kN = Piece<T>::kN;
-    __shared__ uint64_t room[kWarps][kCandidates], lists[(kWarps > 8 ? kWarps : 8) * 32], best[32];   // lists: of the warps, then of the CTAs
-    __shared__ int count[kWarps];
-    __shared__ float part_m[kWarps], cta_m;
-    __shared__ Sums part[kWarps], cta;
+constexpr int kRoom = 256, kBatch = 32;
+
+__device__ __forceinline__ void copy16(uint4* to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+
+struct Batch {
+    float m[kBatch];
+    Sums sums[kBatch];
+};
+
+template <typename T, int kThreads, int kPieces, int kAhead, bool kTop>
+__global__ void __launch_bounds__(kThreads, kThreads == 512 ? 2 : kThreads == 256 ? 3 : 6) k_logp_ctas(const __grid_constant__ LogpArgs p, int64_t share, int rounds, int per_row) {
+    constexpr bool kLoop = kAhead == 0;
+    constexpr int kWarps = kThreads / 32, kN = Piece<T>::kN, kSegment = kThreads / 32;   // 32 segments of threads
+    extern __shared__ uint4 ring[];   // [kAhead][kPieces][kThreads], then [kBatch][top] keys
+    __shared__ uint64_t room[2][kRoom], merged[8 * 32];
+    __shared__ int count[2];
+    __shared__ float segment[32], part_m[2][kWarps], cta_m[2], bound_at;
+    __shared__ Sums part[2][kWarps], cta[2];
+    __shared__ Batch batch;
+    uint64_t* best = reinterpret_cast<uint64_t*>(ring + (kLoop ? 0 : kAhead * kPieces * kThreads));
     const cg::cluster_group cluster = cg::this_cluster();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rank = per_row > 1 ? (int)cluster.block_rank() : 0;
-    const auto sync = [&] {
-        if (per_row > 1) cluster.sync();
-        else __syncthreads();
+    const int64_t rows_at = gridDim.x / per_row, row0 = blockIdx.x / per_row;
+    const int64_t step = (int64_t)kThreads * kN;
+    const auto row_of = [&](int64_t row) { return static_cast<const T*>(p.x) + row * p.n; };
+    const auto start_of = [&](const T* x) {
+        return (rank * share + threadIdx.x) * kN - Piece<T>::shift_of(x);
     };
-    for (int64_t row = blockIdx.x / per_row; row < p.rows; row += gridDim.x / per_row) {
-        const T* x = static_cast<const T*>(p.x) + row * p.n;
-        const int64_t step = (int64_t)kThreads * kN, start = ((int64_t)rank * rounds * K * kThreads + threadIdx.x) * kN - Piece<T>::shift_of(x);
-        Piece<T> q[K];
+    const auto end_of = [&](const T* x) {   // of this CTA's share of a row
+        const int64_t e = (rank + 1) * share * kN - Piece<T>::shift_of(x);
+        return e < p.n ? e : (int64_t)p.n;
+    };
+    const auto ahead = [&](int64_t row, int stage) {
+        if (row < p.rows) {
+            const T* x = row_of(row);
+            const int64_t first = start_of(x), end = end_of(x);
+#pragma unroll
+            for (int k = 0; k < kPieces; ++k) {
+                uint4* to = ring + (stage * kPieces + k) * kThreads + threadIdx.x;
+                const int64_t at = first + k * step;
+                if (at >= 0 && at + kN <= end) {
+                    copy16(to, x + at);
+                } else {
+                    Piece<T> q;
+                    q.load(x, at, end, p.lo<T>(), p.hi<T>());
+                    *to = q.q;
+                }
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    // The rows of a batch: row0 + (i0 + i) rows_at.
+    const auto finish = [&](int64_t i0, int n) {
+        __syncthreads();
+        if (rank == 0 && warp == 0) {
+            const bool here = lane < n;
+            const Sums t = here ? batch.sums[lane] : Sums{0.f, 0.f, 1};
+            const Row mine(here ? batch.m[lane] : 0.f, t.below, t.equal);
+            const int64_t row = row0 + (i0 + lane) * rows_at;
+            if (here) mine.write(p, row, row_of(row), t);
+            for (int i = 0; i < n * p.top; i += 32) {
+                const int e = i + lane, r = p.top ? e / p.top : 0;
+                const float m = __shfl_sync(0xffffffffu, mine.m, r & 31), s = __shfl_sync(0xffffffffu, mine.s, r & 31);
+                if (e < n * p.top) write_top(p, row0 + (i0 + r) * rows_at, e - r * p.top, best[e], m, s);
+            }
+        }
+        __syncthreads();
+    };
+    if (threadIdx.x < 2) count[threadIdx.x] = 0;
+    __syncthreads();
+    if (!kLoop) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) ahead(row0 + i * rows_at, i);
+    }
+    int64_t it = 0;
+    int held = 0;
+    for (int64_t row = row0; row < p.rows; row += rows_at, ++it) {
+        const T* x = row_of(row);
+        const int64_t start = start_of(x), end = end_of(x);
+        const int buf = (int)(it & 1);
+        Piece<T> q[kPieces];
         const auto load = [&](int round) {
 #pragma unroll
-            for (int k = 0; k < K; ++k) q[k].load(x, start + ((int64_t)round * K + k) * step, p.n);
+            for (int k = 0; k < kPieces; ++k) q[k].load(x, start + ((int64_t)round * kPieces + k) * step, end, p.lo<T>(), p.hi<T>());
         };
         const auto most = [&] {
             float v = q[0].most();
 #pragma unroll
-            for (int k = 1; k < K; ++k) v = max_nan(v, q[k].most());
+            for (int k = 1; k < kPieces; ++k) v = max_nan(v, q[k].most());
             return v;
         };
-        float own = -INFINITY, m;
-        for (int round = 0; round < rounds; ++round) {
-            load(round);
-            own = max_nan(own, most());
-        }
-        m = warp_max(own);
-        if (lane == 0) part_m[warp] = m;
-        __syncthreads();
-        m = part_m[0];
+        float own = -INFINITY;
+        if (kLoop) {
+            for (int round = 0; round < rounds; ++round) {
+                load(round);
+                own = max_nan(own, most());
+            }
+        } else {
+            constexpr int kSlots = kAhead > 0 ? kAhead : 1;
+            const int slot = (int)(it % kSlots);
+            asm volatile("cp.async.wait_group %0;" ::"n"(kSlots - 1) : "memory");
+            const uint4* from = ring + slot * kPieces * kThreads + threadIdx.x;
 #pragma unroll
-        for (int w = 1; w < kWarps; ++w) m = max_nan(m, part_m[w]);
+            for (int k = 0; k < kPieces; ++k) q[k].q = from[k * kThreads];
+            own = most();   // the places have been read
+            ahead(row + kSlots * rows_at, slot);
+        }
+        float m = warp_max(own);
+        if (lane == 0) part_m[buf][warp] = m;
+        if (kTop) {   // the largest of each of 32 neighbouring groups of threads (no NaN there: fmaxf)
+            float v = own;
+#pragma unroll
+            for (int d = 1; d < (kSegment < 32 ? kSegment : 32); d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
+            if (threadIdx.x % kSegment == 0) segment[threadIdx.x / kSegment] = v;
+        }
+        __syncthreads();
+        m = warp_max(part_m[buf][lane % kWarps]);
         if (per_row > 1) {
-            if (threadIdx.x == 0) cta_m = m;
+            if (threadIdx.x == 0) cta_m[buf] = m;
             cluster.sync();
-            for (int c = 0; c < per_row; ++c) m = max_nan(m, *cluster.map_shared_rank(&cta_m, c));
+            m = warp_max(*cluster.map_shared_rank(&cta_m[buf], lane % per_row));
         }
         const bool plain = m < INFINITY && m > -INFINITY;
+        bool bounded = false;
+        if (kTop && plain) {   // the same for all threads
+            if (warp == 0) {
+                const float mine = segment[lane];
+                int before = 0;   // segments in front of this one
+                for (int i = 0; i < 32; ++i) before += segment[i] > mine || (segment[i] == mine && i < lane);
+                if (before == p.top - 1) bound_at = fmaxf(mine, -3.4028234e38f);   // at least the scores above -inf
+            }
+            __syncthreads();
+            bounded = true;
+        }
         Sums t = {0.f, 0.f, 0};
-        uint64_t list = 0;
-        for (int round = 0; round < rounds; ++round) {
-            if (rounds > 1) {
+        for (int round = 0; round < (kLoop ? rounds : 1); ++round) {
+            if (kLoop) {
                 load(round);
                 own = most();
             }
+            if (bounded && own >= bound_at)
+                gather(q, start + (int64_t)round * kPieces * step, step, bound_at, room[buf], &count[buf], kRoom);
             if (plain) add_up(t, q, m, own);
-            if (p.top) list = best_of_pieces(q, start + (int64_t)round * K * step, step, p.n, own, plain, p.top, list, room[warp], &count[warp]);
         }
         warp_sums(t.below, t.weighted);
         t.equal = (int)__reduce_add_sync(0xffffffffu, (unsigned)t.equal);
-        if (lane == 0) part[warp] = t;
-        if (lane < p.top) lists[warp * p.top + lane] = list;
+        if (lane == 0) part[buf][warp] = t;
         __syncthreads();
-        if (warp == 0) {
-            Sums all = part[0];
-#pragma unroll
-            for (int w = 1; w < kWarps; ++w) {
-                all.below += part[w].below;
-                all.weighted += part[w].weighted;
-                all.equal += part[w].equal;
+        uint64_t* out = best + held * p.top;   // of this CTA, where a cluster has several
+        if (kTop) {
+            const int c = count[buf];
+            if (bounded && c <= kRoom && c >= (per_row > 1 && end <= start - threadIdx.x * kN ? 0 : p.top)) {
+                if (warp == 0) {
+                    if (lane < p.top) out[lane] = 0;   // a share may have fewer
+                    __syncwarp();
+                    in_order(out, room[buf], c, p.top);
+                }
+            } else {
+                uint64_t before = ~0ull;
+                for (int k = 0; k < p.top; ++k) {
+                    uint64_t b = best_below(p, x, start, step, end, before);
+                    b = warp_best(b);
+                    __syncthreads();
+                    if (lane == 0) merged[warp] = b;
+                    __syncthreads();
+                    before = warp_best(merged[lane % kWarps]);
+                    if (threadIdx.x == 0) out[k] = before;
+                }
             }
-            uint64_t mine = p.top ? best_of(lists, kWarps * p.top, p.top) : 0;
-            if (per_row > 1) {
-                if (lane == 0) cta = all;
-                best[lane] = mine;
-            }
-            if (per_row == 1) {
-                const Row done(m, all.below, all.equal);
-                if (lane == 0) done.write(p, row, x, all);
-                if (p.top) write_top(p, row, done, mine);
+            __syncthreads();
+            if (threadIdx.x == 0) count[buf] = 0;
+        }
+        if (warp == kWarps - 1) {
+            Sums all = lane < kWarps ? part[buf][lane] : Sums{0.f, 0.f, 0};
+            warp_sums(all.below, all.weighted);
+            all.equal = (int)__reduce_add_sync(0xffffffffu, (unsigned)all.equal);
+            if (lane == 0) {
+                if (per_row > 1) {
+                    cta[buf] = all;
+                } else {
+                    batch.m[held] = m;
+                    batch.sums[held] = all;
+                }
             }
         }
         if (per_row > 1) {
             cluster.sync();
             if (rank == 0 && warp == 0) {
-                Sums all = cta;
-                for (int c = 1; c < per_row; ++c) {
-                    const Sums o = *cluster.map_shared_rank(&cta, c);
-                    all.below += o.below;
-                    all.weighted += o.weighted;
-                    all.equal += o.equal;
+                Sums all = lane < per_row ? *cluster.map_shared_rank(&cta[buf], lane % per_row) : Sums{0.f, 0.f, 0};
+                warp_sums(all.below, all.weighted);
+                all.equal = (int)__reduce_add_sync(0xffffffffu, (unsigned)all.equal);
+                if (lane == 0) {
+                    batch.m[held] = m;
+                    batch.sums[held] = all;
                 }
-                const Row done(m, all.below, all.equal);
-                if (lane == 0) done.write(p, row, x, all);
-                if (p.top) {
+                if (kTop) {
                     for (int c = 0; c < per_row; ++c)
-                        if (lane < p.top) lists[c * p.top + lane] = cluster.map_shared_rank(best, c)[lane];
+                        if (lane < p.top) merged[c * p.top + lane] = *cluster.map_shared_rank(out + lane, c);
                     __syncwarp();
-                    write_top(p, row, done, best_of(lists, per_row * p.top, p.top));
+                    int n = 0;   // keys that are there, close together
+                    for (int i = lane; i < (per_row * p.top + 31) / 32 * 32; i += 32) {
+                        const uint64_t v = i < per_row * p.top ? merged[i] : 0;
+                        const unsigned there = __ballot_sync(0xffffffffu, v != 0);
+                        if (v) merged[n + __popc(there & ((1u << lane) - 1))] = v;
+                        n += __popc(there);
+                        __syncwarp();
+                    }
+                    in_order(out, merged, n, p.top);
                 }
             }
+            if (kTop) cluster.sync();   // the others' lists have been read
         }
-        sync();   // what was shared may be written again, and outlives its readers
+        if (++held == kBatch) {
+            finish(it - held + 1, held);
+            held = 0;
+        }
     }
+    if (held) finish(it - held, held);
+    if (per_row > 1) cluster.sync();   // what is shared outlives its readers
 }
 
 // ------------------------------------------------------------- few classes
@@ -613,7 +787,7 @@ __global__ void __launch_bounds__(256) k_logp_grad(const __grid_constant__ LogpA
             if (first - (int64_t)(threadIdx.x % kLanes) * kN >= p.n) break;
             Piece<T> q[kUnroll];
 #pragma unroll
-            for (int k = 0; k < kUnroll; ++k) q[k].load(x, first + k * kLanes * kN, piece + k < pieces ? p.n : 0);
+            for (int k = 0; k < kUnroll; ++k) q[k].load(x, first + k * kLanes * kN, piece + k < pieces ? p.n : -kN, p.lo<T>(), p.hi<T>());
 #pragma unroll
             for (int k = 0; k < kUnroll; ++k) {
                 const int64_t at = first + k * kLanes * kN;
@@ -660,26 +834,54 @@ static int64_t vectors_of(const LogpArgs& a, int kn) {   // of a row, wherever i
 
 static unsigned grid_of(int64_t ctas) { return (unsigned)(ctas < (1 << 30) ? ctas : 1 << 30); }
 
-template <typename T, int K, int kThreads>
-static cudaError_t launch_cluster(const LogpArgs& a, int rounds, int per_row, cudaStream_t s) {
+// As many CTAs as are resident at a time (in clusters of per_row).
+template <typename T, int kThreads, int kPieces, int kAhead, bool kTop>
+static cudaError_t launch_ctas(const LogpArgs& a, int64_t nv, int per_row, cudaStream_t s) {
+    const auto kernel = k_logp_ctas<T, kThreads, kPieces, kAhead, kTop>;
+    constexpr int kRing = kAhead * kPieces * kThreads * 16;
+    const int64_t share = ceil_div(nv, per_row);
+    int resident = 0;
+    const cudaError_t e = pl::kernel_once(
+        reinterpret_cast<const void*>(kernel),
+        [](int* n) {
+            const auto k = k_logp_ctas<T, kThreads, kPieces, kAhead, kTop>;
+            const int most = kRing + (kTop ? kBatch * PLATTICE_MAX_TOP * 8 : 0);
+            const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+            return e != cudaSuccess ? e : cudaOccupancyMaxActiveBlocksPerMultiprocessor(n, k, kThreads, most);
+        },
+        &resident);
+    if (e != cudaSuccess) return e;
+    int64_t rows = (int64_t)(resident > 0 ? resident : 1) * sm_count() / per_row;
+    if (rows < 1) rows = 1;
+    if (rows > a.rows) rows = a.rows;
     cudaLaunchConfig_t c = {};
-    const int64_t rows = a.rows < (1 << 24) ? a.rows : 1 << 24;
     c.gridDim = dim3((unsigned)(rows * per_row));
     c.blockDim = dim3(kThreads);
+    c.dynamicSmemBytes = kRing + (size_t)kBatch * a.top * 8;
     c.stream = s;
     cudaLaunchAttribute attr = {};
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = (unsigned)per_row;
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     c.attrs = &attr;
-    c.numAttrs = 1;
-    return cudaLaunchKernelEx(&c, k_logp_cluster<T, K, kThreads>, a, rounds, per_row);
+    c.numAttrs = per_row > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&c, kernel, a, share, (int)ceil_div(share, kPieces * kThreads), per_row);
+}
+
+template <typename T, int kThreads, int kPieces, int kAhead>
+static cudaError_t launch_ctas(const LogpArgs& a, int64_t nv, int per_row, cudaStream_t s) {
+    return a.top ? launch_ctas<T, kThreads, kPieces, kAhead, true>(a, nv, per_row, s)
+                 : launch_ctas<T, kThreads, kPieces, kAhead, false>(a, nv, per_row, s);
 }
 
 template <typename T, int K>
 static cudaError_t launch_warp(const LogpArgs& a, cudaStream_t s) {
-    constexpr int kRows = K == 1 ? 2 : 1;
-    k_logp_warp<T, K, kRows><<<grid_of(ceil_div(a.rows, 8 * kRows)), 256, 0, s>>>(a);
+    // rows a warp takes one after the other: few where there are few, so that all SMs work
+    const int64_t want = a.rows / (sm_count() * 32);
+    const int each = want < 1 ? 1 : want > kWarpRows ? kWarpRows : (int)want;
+    const unsigned ctas = grid_of(ceil_div(a.rows, 4 * each));
+    if (a.top) k_logp_warp<T, K, true><<<ctas, 128, (size_t)4 * each * a.top * 8, s>>>(a, each);
+    else k_logp_warp<T, K, false><<<ctas, 128, 0, s>>>(a, each);
     return cudaGetLastError();
 }
 
@@ -687,23 +889,26 @@ template <typename T>
 static cudaError_t forward(const LogpArgs& a, cudaStream_t s) {
     constexpr int kN = Piece<T>::kN;
     if (a.n <= kFewClasses) {
-        k_logp_few<T><<<grid_of(ceil_div(a.rows, kTileRows)), kTileRows, kTileRows * pitch_of<T>(a.n) * sizeof(T), s>>>(a, aligned16(a.x));
+        k_logp_few<T><<<grid_of(ceil_div(a.rows, kTileRows)), kTileRows, kTileRows * pitch_of<T>(a.n) * sizeof(T), s>>>(
+            a, aligned16(a.x));
         return cudaGetLastError();
     }
     const int64_t nv = vectors_of(a, kN);
     if (nv <= 32) return launch_warp<T, 1>(a, s);
     if (nv <= 64) return launch_warp<T, 2>(a, s);
     if (nv <= 96) return launch_warp<T, 3>(a, s);
-    if (nv <= 32 * kWarpVectors) return launch_warp<T, kWarpVectors>(a, s);
+    if (nv <= 128) return launch_warp<T, 4>(a, s);
+    if (nv <= 160) return launch_warp<T, 5>(a, s);
     // The smallest cluster that holds the row; a larger one where the rows leave SMs without work.
     int per_row = 1;
     while (per_row < 8 && (nv > 4096 * (int64_t)per_row || (a.rows * per_row * 2 <= sm_count() && nv >= 1024 * (int64_t)per_row)))
         per_row *= 2;
-    const int64_t each = ceil_div(nv, per_row);
-    if (each <= 512) return launch_cluster<T, 4, 128>(a, 1, per_row, s);
-    if (each <= 1024) return launch_cluster<T, 4, 256>(a, 1, per_row, s);
-    if (each <= 2048) return launch_cluster<T, 4, 512>(a, 1, per_row, s);
-    return launch_cluster<T, 8, 512>(a, (int)ceil_div(each, 4096), per_row, s);
+    const int64_t share = ceil_div(nv, per_row);
+    if (share <= 512) return launch_ctas<T, 128, 4, 3>(a, nv, per_row, s);
+    if (share <= 1024) return launch_ctas<T, 128, 8, 2>(a, nv, per_row, s);
+    if (share <= 2048) return launch_ctas<T, 256, 8, 2>(a, nv, per_row, s);
+    if (share <= 4096) return launch_ctas<T, 512, 8, 1>(a, nv, per_row, s);
+    return launch_ctas<T, 512, 8, 0>(a, nv, per_row, s);
 }
 
 template <typename T>
