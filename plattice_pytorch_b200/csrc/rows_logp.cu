@@ -61,7 +61,7 @@ template <typename T> struct Piece {
         return std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
     }
     // Elements first.. of the row x[0..n), which lies in a tensor lo..hi.
-    __device__ __forceinline__ void load(const T* x, int64_t first, int64_t n, const T* lo, const T* hi) {
+    template <typename Int> __device__ __forceinline__ void load(const T* x, Int first, Int n, const T* lo, const T* hi) {
         const T* at = x + first;
         if (first >= 0 && first + kN <= n) {
             q = *reinterpret_cast<const uint4*>(at);
@@ -87,6 +87,11 @@ template <typename T> struct Piece {
                 if (first + i >= 0 && first + i < n) r.e[i] = x[first + i];
         }
         q = r.u;
+    }
+    // The same where all rows begin on 16-byte boundaries: there are no parts.
+    template <typename Int> __device__ __forceinline__ void load_whole(const T* x, Int first, Int n) {
+        if (first < n) q = *reinterpret_cast<const uint4*>(x + first);
+        else q = make_uint4(closed(), closed(), closed(), closed());
     }
     __device__ __forceinline__ uint32_t word(int i) const { return i == 0 ? q.x : i == 1 ? q.y : i == 2 ? q.z : q.w; }
     __device__ __forceinline__ float2 pair(int i) const {   // elements 2 i, 2 i + 1
@@ -157,6 +162,53 @@ __device__ __forceinline__ void warp_sums(float& a, float& b) {
     b = __shfl_sync(0xffffffffu, keep, 16);
 }
 
+// t = (x - m) log2(e) + delta in one multiply-add: delta, what the rounding of m
+// log2(e) leaves, is the same for all of a row and taken out of its sums.  Scores
+// so far below m that their exponential is 0 anyway (-inf among them, which would
+// give 0 times infinity) are held at `bound`, 16-bit ones before they are widened:
+// 140 or |m| / 64 below, which their own rounding leaves at least 100.
+template <typename T> struct Exponents {
+    float c, delta;
+    uint32_t bound;
+    bool fast;    // m is far enough from the type's ends (the same for a row)
+    __device__ __forceinline__ explicit Exponents(float m) {
+        c = -(m * kLog2e);
+        delta = fmaf(m, kLog2e, c);
+        fast = fabsf(m) < 1e38f;
+        if constexpr (sizeof(T) == 2) {
+            typename Pair<T>::type b;
+            const float low = m - fmaxf(140.f, fabsf(m) * (1.f / 64.f));
+            pair_from(b, low, low);
+            bound = *reinterpret_cast<const uint32_t*>(&b);
+            if (std::is_same<T, __half>::value) fast = m > -60000.f && m < INFINITY;
+        }
+    }
+    __device__ __forceinline__ uint64_t at(const Piece<T>& q, int i) const {   // of elements 2 i, 2 i + 1
+        if constexpr (sizeof(T) == 2) {
+            typedef typename Pair<T>::type P;
+            const uint32_t w = q.word(i);
+            const P held = __hmax2(*reinterpret_cast<const P*>(&w), *reinterpret_cast<const P*>(&bound));
+            const float2 v = pair_f32(held);
+            return fma2(pair_of(v.x, v.y), both(kLog2e), both(c));
+        } else {
+            const float2 v = q.pair(i);
+            float a, b;
+            pair_to(fma2(pair_of(v.x, v.y), both(kLog2e), both(c)), a, b);
+            return pair_of(fmaxf(a, kLowest), fmaxf(b, kLowest));
+        }
+    }
+};
+__device__ __forceinline__ uint64_t exp2_pair(uint64_t t) {
+    float a, b;
+    pair_to(t, a, b);
+    return pair_of(exp2_fast(a), exp2_fast(b));
+}
+__device__ __forceinline__ float both_added(uint64_t v) {
+    float a, b;
+    pair_to(v, a, b);
+    return a + b;
+}
+
 // What a set of scores adds up to beside a largest score m: the exponentials of
 // the scores below m, those times their exponents of 2, and the scores equal to m.
 struct Sums {
@@ -167,35 +219,36 @@ struct Sums {
 // `own`: the largest of these scores.  The few threads that hold the largest of
 // the row first take it out.
 template <typename T, int K>
-__device__ __forceinline__ void add_up(Sums& s, const Piece<T> (&all)[K], float m, float own) {
+__device__ __forceinline__ void add_up(Sums& s, Piece<T> (&q)[K], float m, float own) {
     constexpr int kPairs = Piece<T>::kN / 2;
-    Piece<T> q[K];
-#pragma unroll
-    for (int k = 0; k < K; ++k) q[k] = all[k];
     if (own == m) {
 #pragma unroll
         for (int k = 0; k < K; ++k) s.equal += q[k].take(m);
     }
-    const uint64_t minus = both(-m), scale = both(kLog2e);
-    uint64_t sum = 0ull, weighted = 0ull;
+    const Exponents<T> x(m);
+    if (x.fast) {
+        uint64_t sum = 0ull, weighted = 0ull;
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+        for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int i = 0; i < kPairs; ++i) {
-            const float2 v = q[k].pair(i);
-            float a, b;
-            pair_to(mul2(add2(pair_of(v.x, v.y), minus), scale), a, b);
-            a = fmaxf(a, kLowest);
-            b = fmaxf(b, kLowest);
-            const uint64_t e = pair_of(exp2_fast(a), exp2_fast(b));
-            sum = add2(sum, e);
-            weighted = fma2(e, pair_of(a, b), weighted);
-        }
-    float a, b;
-    pair_to(sum, a, b);
-    s.below += a + b;
-    pair_to(weighted, a, b);
-    s.weighted += a + b;
+            for (int i = 0; i < kPairs; ++i) {
+                const uint64_t t = x.at(q[k], i), e = exp2_pair(t);
+                sum = add2(sum, e);
+                weighted = fma2(e, t, weighted);
+            }
+        const float f = exp2_fast(-x.delta), b = both_added(sum) * f;
+        s.below += b;
+        s.weighted += fmaf(both_added(weighted), f, -x.delta * b);
+    } else {
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int i = 0; i < 2 * kPairs; ++i) {
+                const float2 v = q[k].pair(i / 2);
+                const float t = fmaxf(((i % 2 ? v.y : v.x) - m) * kLog2e, kLowest), e = exp2_fast(t);
+                s.below += e;
+                s.weighted = fmaf(e, t, s.weighted);
+            }
+    }
 }
 
 // A row's numbers from its sums, written by one thread.
@@ -307,25 +360,93 @@ __device__ __forceinline__ void write_top(const LogpArgs& p, int64_t row, int pl
 
 constexpr int kWarpRows = 16, kWarpRoom = 64;
 
-template <typename T, int K, bool kTop>
+// The best of 16-bit scores: class and score make a key of 32 bits, whose largest
+// of the warp is one instruction; a lane's next largest is that of key - taken
+// (mod 2^32, where those that were taken are smallest).
+template <typename T, int K>
+__device__ __forceinline__ void best_of_16(uint64_t* out, const Piece<T> (&q)[K], int first, int n, int top) {
+    typedef typename Pair<T>::type P;
+    uint32_t key[8 * K];
+    const P zero = {};
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t raw = q[k].word(i);
+            const P v = __hadd2(*reinterpret_cast<const P*>(&raw), zero);   // -0 as 0
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(&v);
+            const uint32_t u = w ^ (((w >> 15) & 0x00010001u) * 0xffffu | 0x80008000u);
+            const int j = first + k * 256 + 2 * i;
+            key[8 * k + 2 * i] = (unsigned)j < (unsigned)n ? u << 16 | (0xffff - j) : 0u;
+            key[8 * k + 2 * i + 1] = (unsigned)(j + 1) < (unsigned)n ? (u & 0xffff0000u) | (0xfffe - j) : 0u;
+        }
+    uint32_t best = 0, mine = 0;
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int i = 0; i < 8 * K; ++i) best = max(best, key[i]);
+    for (int t = 0; t < top; ++t) {
+        const uint32_t taken = __reduce_max_sync(0xffffffffu, best);
+        if (lane == t) mine = taken;
+        uint32_t left = 0;
+#pragma unroll
+        for (int i = 0; i < 8 * K; ++i) left = __viaddmax_u32(key[i], 0u - taken, left);
+        left += taken;
+        if (best == taken) best = left < taken ? left : 0u;   // another lane's best stays
+    }
+    if (lane < top) {
+        const uint16_t u = (uint16_t)(mine >> 16), h = u & 0x8000 ? u ^ 0x8000 : ~u;
+        out[lane] = ranked(to_f32(*reinterpret_cast<const T*>(&h)), 0xffff - (int)(mine & 0xffff));
+    }
+}
+
+// The best by a bound: the scores that are at least the top-th largest of the
+// lanes' largest ones hold them; mostly they are few more.  False where not.
+template <typename T, int K>
+__device__ __forceinline__ bool best_by_bound(uint64_t* out, const Piece<T> (&q)[K], int first, float own, int top, uint64_t* room,
+                                              int* count) {
+    const int lane = threadIdx.x & 31;
+    float bound = 0.f, v = own;
+    for (int k = 0; k < top; ++k) {
+        bound = warp_max(v);
+        const unsigned at = __ballot_sync(0xffffffffu, v == bound);
+        if (lane == __ffs(at) - 1) v = -INFINITY;
+    }
+    bound = fmaxf(bound, -3.4028234e38f);   // at least the scores above -inf
+    if (lane == 0) *count = 0;
+    __syncwarp();
+    if (own >= bound) gather(q, first, 32 * Piece<T>::kN, bound, room, count, kWarpRoom);
+    __syncwarp();
+    const int c = *count;
+    const bool done = c >= top && c <= kWarpRoom;
+    if (done) in_order(out, room, c, top);
+    __syncwarp();
+    return done;
+}
+
+template <typename T, int K, bool kTop, bool kWhole>
 __global__ void __launch_bounds__(128) k_logp_warp(const __grid_constant__ LogpArgs p, int rows_each) {
     __shared__ uint64_t room[4][kWarpRoom];
     __shared__ int count[4];
     extern __shared__ uint64_t staged[];   // [4][rows_each][top]
     constexpr int kN = Piece<T>::kN;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = p.n;
     uint64_t* best = staged + (size_t)warp * rows_each * p.top;
     const int64_t all = (p.rows + rows_each - 1) / rows_each;
     for (int64_t group = (int64_t)blockIdx.x * 4 + warp; group < all; group += (int64_t)gridDim.x * 4) {
         const int64_t base = group * rows_each;
         const int rows = p.rows - base < rows_each ? (int)(p.rows - base) : rows_each;
+        const T* x = static_cast<const T*>(p.x) + base * n;
         Piece<T> q[K], next[K];
-        int64_t first = 0, first_next;
+        int first = 0, first_next;
         const auto load = [&](int r) {
-            const T* x = static_cast<const T*>(p.x) + (base + r) * p.n;
-            first_next = (int64_t)lane * kN - Piece<T>::shift_of(x);
+            const T* y = x + r * n;
+            first_next = lane * kN - (kWhole ? 0 : Piece<T>::shift_of(y));
 #pragma unroll
-            for (int k = 0; k < K; ++k) next[k].load(x, first_next + k * 32 * kN, r < rows ? p.n : -kN, p.lo<T>(), p.hi<T>());
+            for (int k = 0; k < K; ++k) {
+                const int at = first_next + k * 32 * kN, end = r < rows ? n : -kN;
+                if (kWhole) next[k].load_whole(y, at, end);
+                else next[k].load(y, at, end, p.lo<T>(), p.hi<T>());
+            }
         };
         load(0);
         float most = 0.f;
@@ -341,32 +462,16 @@ __global__ void __launch_bounds__(128) k_logp_warp(const __grid_constant__ LogpA
             const float m = warp_max(own);
             const bool plain = m < INFINITY && m > -INFINITY;
             if (kTop) {
-                // The scores that are at least the top-th largest of the lanes' largest ones
-                // hold the best; mostly they are few more.
-                bool done = false;
                 uint64_t* out = best + r * p.top;
+                bool done = false;
                 if (plain) {
-                    float bound = 0.f, v = own;
-                    for (int k = 0; k < p.top; ++k) {
-                        bound = warp_max(v);
-                        const unsigned at = __ballot_sync(0xffffffffu, v == bound);
-                        if (lane == __ffs(at) - 1) v = -INFINITY;
-                    }
-                    if (lane == 0) count[warp] = 0;
-                    __syncwarp();
-                    if (bound > -INFINITY) {
-                        if (own >= bound) gather(q, first, 32 * kN, bound, room[warp], &count[warp], kWarpRoom);
-                        __syncwarp();
-                        const int c = count[warp];
-                        done = c <= kWarpRoom;
-                        if (done) in_order(out, room[warp], c, p.top);
-                    }
-                    __syncwarp();
+                    if constexpr (sizeof(T) == 2 && K <= 2) best_of_16(out, q, first, n, p.top), done = true;
+                    else done = best_by_bound(out, q, first, own, p.top, room[warp], &count[warp]);
                 }
                 if (!done) {
                     uint64_t before = ~0ull;
                     for (int k = 0; k < p.top; ++k) {
-                        before = warp_best(best_below(p, static_cast<const T*>(p.x) + (base + r) * p.n, first, 32 * kN, p.n, before));
+                        before = warp_best(best_below(p, x + r * n, first, 32 * kN, n, before));
                         if (lane == 0) out[k] = before;
                     }
                 }
@@ -383,7 +488,7 @@ __global__ void __launch_bounds__(128) k_logp_warp(const __grid_constant__ LogpA
             }
         }
         const Row mine(most, sums.below, sums.equal);
-        if (lane < rows) mine.write(p, base + lane, static_cast<const T*>(p.x) + (base + lane) * p.n, sums);
+        if (lane < rows) mine.write(p, base + lane, x + lane * n, sums);
         if (kTop) {
             __syncwarp();
             for (int i = 0; i < rows * p.top; i += 32) {
@@ -659,7 +764,7 @@ __device__ __forceinline__ void tile_copy(T* tile, T* x, int count, int n, bool 
     const int whole = vec ? count / kN : 0;
     for (int i = threadIdx.x; i < whole; i += kTileRows) {
         if (pitch == n) {
-            if (kIn) reinterpret_cast<uint4*>(tile)[i] = reinterpret_cast<const uint4*>(x)[i];
+            if (kIn) copy16(reinterpret_cast<uint4*>(tile) + i, reinterpret_cast<const uint4*>(x) + i);
             else reinterpret_cast<uint4*>(x)[i] = reinterpret_cast<const uint4*>(tile)[i];
             continue;
         }
@@ -678,6 +783,7 @@ __device__ __forceinline__ void tile_copy(T* tile, T* x, int count, int n, bool 
         if (kIn) tile[at.row * pitch + at.j] = x[i];
         else x[i] = tile[at.row * pitch + at.j];
     }
+    if (kIn) asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 template <typename T>
@@ -721,17 +827,16 @@ __global__ void __launch_bounds__(kTileRows) k_logp_few(const __grid_constant__ 
 
 // ------------------------------------------------------------- the gradient
 
-// What the elements of a row have in common.
+// What the elements of a row have in common: p (all - ge log p), and gl more at
+// the label.
 struct RowGrad {
-    float m, s, all, ge, gl;   // p (all - ge log p), and gl more at the label
-    float rest;                // of all without gl: at the label
+    float m, s, all, ge, gl;
+    float rest;   // of all without gl: at the label
     int label;
-    bool empty;
     __device__ __forceinline__ RowGrad(const LogpArgs& p, int64_t row) {
         const float2 st = p.stats[row];
         m = st.x;
         s = st.y;
-        empty = m == -INFINITY;
         label = p.gl ? p.labels.at(row, p.n) : -1;
         gl = label >= 0 ? p.gl[row] : 0.f;
         ge = p.ge ? p.ge[row] : 0.f;
@@ -741,13 +846,69 @@ struct RowGrad {
     // The label's own 1 - p would lose what a confident answer leaves.
     __device__ __forceinline__ float at_label(float x) const {
         const float lp = (x - m) - s, t = max_nan(lp * kLog2e, kLowest);
-        return empty ? 0.f : fmaf(exp2_fast(t), fmaf(-ge * kLn2, t, rest), -gl * expm1f(lp));
+        return m == -INFINITY ? 0.f : fmaf(exp2_fast(t), fmaf(-ge * kLn2, t, rest), -gl * expm1f(lp));
     }
     __device__ __forceinline__ float at(float x) const {
         const float t = max_nan(((x - m) - s) * kLog2e, kLowest);   // NaN of a row that has one stays
-        return empty ? 0.f : exp2_fast(t) * fmaf(-ge * kLn2, t, all);
+        return m == -INFINITY ? 0.f : exp2_fast(t) * fmaf(-ge * kLn2, t, all);
     }
 };
+
+// The gradients of a piece at class `at` of its row.  log2 p = t - kappa with t of
+// Exponents and kappa = delta + s log2(e), so that p (all - ge log p) = 2^t (a + b t).
+template <typename T> struct PieceGrad {
+    static constexpr int kN = Piece<T>::kN;
+    RowGrad g;
+    Exponents<T> x;
+    float a, b;
+    __device__ __forceinline__ explicit PieceGrad(const RowGrad& g_) : g(g_), x(g_.m) {
+        const float kappa = fmaf(g.s, kLog2e, x.delta), f = exp2_fast(-kappa), e = g.ge * kLn2;
+        a = f * fmaf(e, kappa, g.all);
+        b = -f * e;
+    }
+    __device__ __forceinline__ void of(float (&v)[kN], const Piece<T>& q, int64_t at) const {
+        if (x.fast) {
+#pragma unroll
+            for (int i = 0; i < kN / 2; ++i) {
+                const uint64_t t = x.at(q, i);
+                pair_to(mul2(exp2_pair(t), fma2(t, both(b), both(a))), v[2 * i], v[2 * i + 1]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kN; ++i) {
+                const float2 f = q.pair(i / 2);
+                v[i] = g.at(i % 2 ? f.y : f.x);
+            }
+        }
+        const int64_t l = g.label - at;
+        if (l >= 0 && l < kN && g.label >= 0) {
+            float own = 0.f;
+#pragma unroll
+            for (int i = 0; i < kN; ++i) {
+                const float2 f = q.pair(i / 2);
+                own = i == l ? (i % 2 ? f.y : f.x) : own;
+            }
+            own = g.at_label(own);
+#pragma unroll
+            for (int i = 0; i < kN; ++i) v[i] = i == l ? own : v[i];
+        }
+    }
+};
+
+// `whole`: all of the piece is in the row and the gradient's row lies as the scores' does.
+template <typename T>
+__device__ __forceinline__ void store_piece(T* gx, const float (&v)[Piece<T>::kN], int64_t at, int64_t n, bool whole) {
+    constexpr int kN = Piece<T>::kN;
+    if (whole) {
+        Vec<T, kN> o;
+        o.from(v);
+        o.store(gx + at);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kN; ++i)
+            if (at + i >= 0 && at + i < n) gx[at + i] = from_f32<T>(v[i]);
+    }
+}
 
 template <typename T>
 __global__ void __launch_bounds__(kTileRows) k_logp_few_grad(const __grid_constant__ LogpArgs p, bool vec, bool vec_out) {
@@ -770,66 +931,84 @@ __global__ void __launch_bounds__(kTileRows) k_logp_few_grad(const __grid_consta
     }
 }
 
-// kLanes neighbouring threads a row (32, or the CTA); each takes pieces kLanes apart,
-// blockIdx.y gives the first of its `pieces` ones.
-template <typename T, int kLanes>
-__global__ void __launch_bounds__(256) k_logp_grad(const __grid_constant__ LogpArgs p, int pieces, bool same) {
-    constexpr int kN = Piece<T>::kN, kUnroll = 4;
-    const int64_t rows_at = gridDim.x * (int64_t)(256 / kLanes);
-    for (int64_t row = (int64_t)blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes; row < p.rows; row += rows_at) {
-        const T* x = static_cast<const T*>(p.x) + row * p.n;
-        T* gx = static_cast<T*>(p.gx) + row * p.n;
-        const RowGrad g(p, row);
-        const int shift = Piece<T>::shift_of(x);
-        const uint64_t minus = both(-g.m), less = both(-g.s), scale = both(kLog2e), ge = both(-g.ge * kLn2), all = both(g.all);
-        for (int piece = 0; piece < pieces; piece += kUnroll) {
-            const int64_t first = (((int64_t)blockIdx.y * pieces + piece) * kLanes + threadIdx.x % kLanes) * kN - shift;
-            if (first - (int64_t)(threadIdx.x % kLanes) * kN >= p.n) break;
-            Piece<T> q[kUnroll];
+// A warp a row, up to 32 neighbouring ones after another; lane r reads what row r's
+// elements have in common.  kAtOnce accesses are under way together.
+constexpr int kAtOnce = 4;
+
+template <typename T, bool kWhole>
+__global__ void __launch_bounds__(128) k_logp_grad_warp(const __grid_constant__ LogpArgs p, int rows_each, int pieces, bool same) {
+    constexpr int kN = Piece<T>::kN;
+    const int lane = threadIdx.x & 31, n = p.n;
+    const int64_t all = (p.rows + rows_each - 1) / rows_each;
+    for (int64_t group = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5); group < all; group += (int64_t)gridDim.x * 4) {
+        const int64_t base = group * rows_each;
+        const int rows = p.rows - base < rows_each ? (int)(p.rows - base) : rows_each;
+        const T* x = static_cast<const T*>(p.x) + base * n;
+        T* gx = static_cast<T*>(p.gx) + base * n;
+        const RowGrad own(p, base + (lane < rows ? lane : rows - 1));
+        const int count = rows * pieces;   // piece i: of row i / pieces
+        for (int i0 = 0, r0 = 0, k0 = 0; i0 < count; i0 += kAtOnce) {
+            Piece<T> q[kAtOnce];
+            int row[kAtOnce], at[kAtOnce];
 #pragma unroll
-            for (int k = 0; k < kUnroll; ++k) q[k].load(x, first + k * kLanes * kN, piece + k < pieces ? p.n : -kN, p.lo<T>(), p.hi<T>());
-#pragma unroll
-            for (int k = 0; k < kUnroll; ++k) {
-                const int64_t at = first + k * kLanes * kN;
-                if (piece + k >= pieces || at >= p.n) continue;
-                float v[kN];
-#pragma unroll
-                for (int i = 0; i < kN / 2; ++i) {
-                    const float2 f = q[k].pair(i);
-                    float a, b;
-                    pair_to(mul2(add2(add2(pair_of(f.x, f.y), minus), less), scale), a, b);
-                    a = max_nan(a, kLowest);
-                    b = max_nan(b, kLowest);
-                    pair_to(mul2(pair_of(exp2_fast(a), exp2_fast(b)), fma2(pair_of(a, b), ge, all)), v[2 * i], v[2 * i + 1]);
-                }
-                const int64_t l = g.label - at;
-                if (g.label >= 0 && l >= 0 && l < kN) {
-                    const float own = g.at_label(to_f32(x[g.label]));
-#pragma unroll
-                    for (int i = 0; i < kN; ++i) v[i] = i == l ? own : v[i];
-                }
-                if (g.empty)
-#pragma unroll
-                    for (int i = 0; i < kN; ++i) v[i] = 0.f;
-                if (same && at >= 0 && at + kN <= p.n) {
-                    Vec<T, kN> o;
-                    o.from(v);
-                    o.store(gx + at);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < kN; ++i)
-                        if (at + i >= 0 && at + i < p.n) gx[at + i] = from_f32<T>(v[i]);
-                }
+            for (int u = 0; u < kAtOnce; ++u) {
+                const T* y = x + r0 * n;
+                row[u] = r0;
+                at[u] = (k0 * 32 + lane) * kN - (kWhole ? 0 : Piece<T>::shift_of(y));
+                const int end = r0 < rows ? n : -kN;
+                if (kWhole) q[u].load_whole(y, at[u], end);
+                else q[u].load(y, at[u], end, p.lo<T>(), p.hi<T>());
+                if (++k0 == pieces) k0 = 0, ++r0;
             }
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) {
+                if (row[u] >= rows) break;
+                RowGrad g = own;
+                g.m = __shfl_sync(0xffffffffu, own.m, row[u]);
+                g.s = __shfl_sync(0xffffffffu, own.s, row[u]);
+                g.all = __shfl_sync(0xffffffffu, own.all, row[u]);
+                g.ge = __shfl_sync(0xffffffffu, own.ge, row[u]);
+                g.gl = __shfl_sync(0xffffffffu, own.gl, row[u]);
+                g.rest = __shfl_sync(0xffffffffu, own.rest, row[u]);
+                g.label = __shfl_sync(0xffffffffu, own.label, row[u]);
+                float v[kN];
+                PieceGrad<T>(g).of(v, q[u], at[u]);
+                if (at[u] < n)
+                    store_piece<T>(gx + row[u] * n, v, at[u], n, same && (kWhole || (at[u] >= 0 && at[u] + kN <= n)));
+            }
+        }
+    }
+}
+
+// A CTA a share of a row: kAtOnce accesses a thread.
+template <typename T>
+__global__ void __launch_bounds__(256) k_logp_grad(const __grid_constant__ LogpArgs p, int64_t shares, bool same) {
+    constexpr int kN = Piece<T>::kN;
+    const int64_t all = p.rows * shares;
+    for (int64_t share = blockIdx.x; share < all; share += gridDim.x) {
+        const int64_t row = share / shares;
+        const T* x = static_cast<const T*>(p.x) + row * p.n;
+        const int64_t first = ((share - row * shares) * (256 * kAtOnce) + threadIdx.x) * kN - Piece<T>::shift_of(x), n = p.n;
+        Piece<T> q[kAtOnce];
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) q[k].load(x, first + k * 256 * kN, n, p.lo<T>(), p.hi<T>());
+        const PieceGrad<T> g(RowGrad(p, row));
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {
+            const int64_t at = first + k * 256 * kN;
+            if (at >= n) break;
+            float v[kN];
+            g.of(v, q[k], at);
+            store_piece<T>(static_cast<T*>(p.gx) + row * n, v, at, n, same && at >= 0 && at + kN <= n);
         }
     }
 }
 
 // ------------------------------------------------------------------ host side
 
-static int64_t vectors_of(const LogpArgs& a, int kn) {   // of a row, wherever it begins
-    const bool aligned = a.n % kn == 0 && aligned16(a.x);
-    return ceil_div((int64_t)a.n + (aligned ? 0 : kn - 1), kn);
+template <typename T> static bool whole_rows(const LogpArgs& a) { return a.n % Piece<T>::kN == 0 && aligned16(a.x); }
+template <typename T> static int64_t vectors_of(const LogpArgs& a) {   // of a row, wherever it begins
+    return ceil_div((int64_t)a.n + (whole_rows<T>(a) ? 0 : Piece<T>::kN - 1), Piece<T>::kN);
 }
 
 static unsigned grid_of(int64_t ctas) { return (unsigned)(ctas < (1 << 30) ? ctas : 1 << 30); }
@@ -874,26 +1053,34 @@ static cudaError_t launch_ctas(const LogpArgs& a, int64_t nv, int per_row, cudaS
                  : launch_ctas<T, kThreads, kPieces, kAhead, false>(a, nv, per_row, s);
 }
 
+// Rows a warp takes one after the other: few where there are few, so that all SMs work.
+static int rows_each(int64_t rows, int most) {
+    const int64_t want = rows / (sm_count() * 32);
+    return want < 1 ? 1 : want > most ? most : (int)want;
+}
+
+template <typename T, int K, bool kTop>
+static cudaError_t launch_warp(const LogpArgs& a, cudaStream_t s) {
+    const int each = rows_each(a.rows, kWarpRows);
+    const unsigned ctas = grid_of(ceil_div(a.rows, 4 * each));
+    const size_t smem = (size_t)4 * each * a.top * 8;
+    if (whole_rows<T>(a)) k_logp_warp<T, K, kTop, true><<<ctas, 128, smem, s>>>(a, each);
+    else k_logp_warp<T, K, kTop, false><<<ctas, 128, smem, s>>>(a, each);
+    return cudaGetLastError();
+}
 template <typename T, int K>
 static cudaError_t launch_warp(const LogpArgs& a, cudaStream_t s) {
-    // rows a warp takes one after the other: few where there are few, so that all SMs work
-    const int64_t want = a.rows / (sm_count() * 32);
-    const int each = want < 1 ? 1 : want > kWarpRows ? kWarpRows : (int)want;
-    const unsigned ctas = grid_of(ceil_div(a.rows, 4 * each));
-    if (a.top) k_logp_warp<T, K, true><<<ctas, 128, (size_t)4 * each * a.top * 8, s>>>(a, each);
-    else k_logp_warp<T, K, false><<<ctas, 128, 0, s>>>(a, each);
-    return cudaGetLastError();
+    return a.top ? launch_warp<T, K, true>(a, s) : launch_warp<T, K, false>(a, s);
 }
 
 template <typename T>
 static cudaError_t forward(const LogpArgs& a, cudaStream_t s) {
-    constexpr int kN = Piece<T>::kN;
     if (a.n <= kFewClasses) {
         k_logp_few<T><<<grid_of(ceil_div(a.rows, kTileRows)), kTileRows, kTileRows * pitch_of<T>(a.n) * sizeof(T), s>>>(
             a, aligned16(a.x));
         return cudaGetLastError();
     }
-    const int64_t nv = vectors_of(a, kN);
+    const int64_t nv = vectors_of<T>(a);
     if (nv <= 32) return launch_warp<T, 1>(a, s);
     if (nv <= 64) return launch_warp<T, 2>(a, s);
     if (nv <= 96) return launch_warp<T, 3>(a, s);
@@ -913,20 +1100,21 @@ static cudaError_t forward(const LogpArgs& a, cudaStream_t s) {
 
 template <typename T>
 static cudaError_t backward(const LogpArgs& a, cudaStream_t s) {
-    constexpr int kN = Piece<T>::kN;
     if (a.n <= kFewClasses) {
         k_logp_few_grad<T><<<grid_of(ceil_div(a.rows, kTileRows)), kTileRows, kTileRows * pitch_of<T>(a.n) * sizeof(T), s>>>(
             a, aligned16(a.x), aligned16(a.gx));
         return cudaGetLastError();
     }
-    const int64_t nv = vectors_of(a, kN);
+    const int64_t nv = vectors_of<T>(a);
     const bool same = (((uintptr_t)a.x ^ (uintptr_t)a.gx) & 15) == 0;
-    if (nv <= 32 * 8) {
-        k_logp_grad<T, 32><<<grid_of(ceil_div(a.rows, 8)), 256, 0, s>>>(a, (int)ceil_div(nv, 32), same);
+    if (nv <= 160) {
+        const int each = rows_each(a.rows, 32), pieces = (int)ceil_div(nv, 32);
+        const unsigned ctas = grid_of(ceil_div(a.rows, 4 * each));
+        if (whole_rows<T>(a)) k_logp_grad_warp<T, true><<<ctas, 128, 0, s>>>(a, each, pieces, same);
+        else k_logp_grad_warp<T, false><<<ctas, 128, 0, s>>>(a, each, pieces, same);
     } else {
-        int64_t pieces = 4, y = ceil_div(nv, 256 * pieces);
-        if (y > 65535) y = 65535, pieces = ceil_div(ceil_div(nv, 256), y);
-        k_logp_grad<T, 256><<<dim3(grid_of(a.rows), (unsigned)y), 256, 0, s>>>(a, (int)pieces, same);
+        const int64_t shares = ceil_div(nv, 256 * kAtOnce);
+        k_logp_grad<T><<<grid_of(a.rows * shares), 256, 0, s>>>(a, shares, same);
     }
     return cudaGetLastError();
 }
