@@ -66,7 +66,7 @@ def build(jobs=None, verbose_ptxas=False, force=False):
                                                            os.path.join(CSRC, "plattice_pd.cu"), "-o", obj]))
     for name in ("plattice_capi", "plattice_runtime", "plattice_noalloc", "rows_norm", "rows_linear",
                  "rows_mma_forward", "rows_mma_grad", "rows_narrow", "rows_narrow_grad", "rows_embed", "rows_scan", "rows_logp",
-                 "rows_clip"):
+                 "rows_logp_f32", "rows_logp_bf16", "rows_logp_f16", "rows_clip"):
         obj = os.path.join(BUILD, f"{name}.o")
         units.append((obj, [nvcc()] + NVCC_FLAGS + extra + ["-c", os.path.join(CSRC, f"{name}.cu"), "-o", obj]))
     todo = [(o, c) for o, c in units if force or _stale(o, deps[os.path.basename(o).split("_")[0]])]

@@ -1,1125 +1,7 @@
-// rows_logp.cu -- log probabilities of given labels, entropy and the best
-// alternatives of rows of scores, and the scores' gradient.
-//
-//   m = max x, s = log sum exp(x - m);  log p_j = (x_j - m) - s
-//   entropy = -sum p log p = s - sum exp(x - m) (x - m) / sum exp(x - m)
-//   grad_j = g_l ([j = label] - p_j) - g_e p_j (log p_j + entropy) + g_z p_j
-//
-// m and s are kept apart: their sum would lose s beside a large m (rows whose
-// scores are all the type's lowest value, say).  The sum leaves one 1 of the
-// largest score out, so that s = log1p(rest) and the log probability of a
-// confident answer keep their precision.
-//
-// A row is read once and held: few classes by a thread out of shared memory,
-// up to five accesses a lane by a warp in registers, more by a CTA or a
-// cluster of them in registers, and only rows that no cluster holds are read
-// again.  So the largest score is known before the first exponential, which
-// costs a subtraction, a product, a bound, the exponential and two sums (five
-// instructions an element in pairs; the special function unit takes one element
-// in 16 a clock and SM, 60 us for the 268 M of 8192 x 32768, which take 83 us to
-// read).
-#include <cooperative_groups.h>
-
-#include "plattice_runtime.h"
+// rows_logp.cu -- C entry points of the log probabilities; the kernels are
+// rows_logp.cuh, made for a type each by rows_logp_f32.cu and its siblings.
 #include "rows_host.h"
-#include "rows_vec.cuh"
-
-namespace plr {
-
-namespace cg = cooperative_groups;
-
-struct LogpArgs {
-    const void* x;
-    Labels labels;         // p null: none
-    float *logp, *entropy;
-    float2* stats;
-    float* lse;
-    float* top_logp;
-    long long* top_ids;
-    const float *gl, *ge, *gz;
-    void* gx;
-    int64_t rows;
-    int n, top;
-    template <typename T> __device__ __forceinline__ const T* lo() const { return static_cast<const T*>(x); }
-    template <typename T> __device__ __forceinline__ const T* hi() const { return static_cast<const T*>(x) + rows * n; }
-};
-
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr float kLowest = -200.f;   // of an exponent of 2: beyond it the exponential is 0
-
-// ------------------------------------------------------------- rows in registers
-
-// 16 bytes of a row: kN elements.  Accesses lie on 16-byte boundaries of memory,
-// the first of a row perhaps before its start: `shift` elements.  Elements
-// outside the row are -inf.
-template <typename T> struct Piece {
-    static constexpr int kN = 16 / (int)sizeof(T);
-    uint4 q;
-    static __device__ __forceinline__ int shift_of(const T* x) { return (int)((uintptr_t)x & 15) / (int)sizeof(T); }
-    static __device__ __forceinline__ uint32_t closed() {
-        if (std::is_same<T, float>::value) return 0xff800000u;
-        return std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
-    }
-    // Elements first.. of the row x[0..n), which lies in a tensor lo..hi.
-    template <typename Int> __device__ __forceinline__ void load(const T* x, Int first, Int n, const T* lo, const T* hi) {
-        const T* at = x + first;
-        if (first >= 0 && first + kN <= n) {
-            q = *reinterpret_cast<const uint4*>(at);
-            return;
-        }
-        if (first <= -kN || first >= n) {
-            q = make_uint4(closed(), closed(), closed(), closed());
-            return;
-        }
-        union { uint4 u; T e[kN]; uint16_t h[8]; uint32_t w[4]; } r;
-        r.u = make_uint4(closed(), closed(), closed(), closed());
-        if (at >= lo && at + kN <= hi) {   // the neighbouring rows' elements come along
-            r.u = *reinterpret_cast<const uint4*>(at);
-#pragma unroll
-            for (int i = 0; i < kN; ++i)
-                if (first + i < 0 || first + i >= n) {
-                    if constexpr (sizeof(T) == 4) r.w[i] = closed();
-                    else r.h[i] = (uint16_t)closed();
-                }
-        } else {
-#pragma unroll
-            for (int i = 0; i < kN; ++i)
-                if (first + i >= 0 && first + i < n) r.e[i] = x[first + i];
-        }
-        q = r.u;
-    }
-    // The same where all rows begin on 16-byte boundaries: there are no parts.
-    template <typename Int> __device__ __forceinline__ void load_whole(const T* x, Int first, Int n) {
-        if (first < n) q = *reinterpret_cast<const uint4*>(x + first);
-        else q = make_uint4(closed(), closed(), closed(), closed());
-    }
-    __device__ __forceinline__ uint32_t word(int i) const { return i == 0 ? q.x : i == 1 ? q.y : i == 2 ? q.z : q.w; }
-    __device__ __forceinline__ float2 pair(int i) const {   // elements 2 i, 2 i + 1
-        if constexpr (std::is_same<T, float>::value) {
-            return make_float2(__uint_as_float(word(2 * i)), __uint_as_float(word(2 * i + 1)));
-        } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-            return make_float2(__uint_as_float(word(i) << 16), __uint_as_float(word(i) & 0xffff0000u));
-        } else {
-            const uint32_t w = word(i);
-            return __half22float2(*reinterpret_cast<const __half2*>(&w));
-        }
-    }
-    // Puts -inf in the place of elements equal to m; gives their number.
-    __device__ __forceinline__ int take(float m) {
-        int count = 0;
-        if constexpr (std::is_same<T, float>::value) {
-            uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (__uint_as_float(w[i]) == m) w[i] = closed(), ++count;
-            q = make_uint4(w[0], w[1], w[2], w[3]);
-        } else {
-            typedef typename Pair<T>::type P;
-            P both_m;
-            pair_from(both_m, m, m);
-            uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t same = __heq2_mask(*reinterpret_cast<const P*>(&w[i]), both_m);
-                w[i] = (w[i] & ~same) | (same & closed());
-                count += __popc(same) >> 4;
-            }
-            q = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-        return count;
-    }
-    __device__ __forceinline__ float most() const {   // NaN where there is one
-        if constexpr (std::is_same<T, float>::value) {
-            return max_nan(max_nan(__uint_as_float(q.x), __uint_as_float(q.y)), max_nan(__uint_as_float(q.z), __uint_as_float(q.w)));
-        } else {
-            typedef typename Pair<T>::type P;
-            const P* p = reinterpret_cast<const P*>(&q);
-            const P a = __hmax2_nan(__hmax2_nan(p[0], p[1]), __hmax2_nan(p[2], p[3]));
-            const float2 f = pair_f32(a);
-            return max_nan(f.x, f.y);
-        }
-    }
-};
-
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-    for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-    return v;
-}
-__device__ __forceinline__ float warp_max(float v) {   // NaN where there is one
-    float r;
-    asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
-    return r;
-}
-// Sums of two values over the warp: in the lanes of one half a's, of the other b's.
-__device__ __forceinline__ void warp_sums(float& a, float& b) {
-    const int lane = threadIdx.x & 31;
-    float keep = lane < 16 ? a : b;
-    keep += __shfl_xor_sync(0xffffffffu, lane < 16 ? b : a, 16);
-#pragma unroll
-    for (int d = 8; d; d >>= 1) keep += __shfl_xor_sync(0xffffffffu, keep, d);
-    a = __shfl_sync(0xffffffffu, keep, 0);
-    b = __shfl_sync(0xffffffffu, keep, 16);
-}
-
-// t = (x - m) log2(e) + delta in one multiply-add: delta, what the rounding of m
-// log2(e) leaves, is the same for all of a row and taken out of its sums.  Scores
-// so far below m that their exponential is 0 anyway (-inf among them, which would
-// give 0 times infinity) are held at `bound`, 16-bit ones before they are widened:
-// 140 or |m| / 64 below, which their own rounding leaves at least 100.
-template <typename T> struct Exponents {
-    float c, delta;
-    uint32_t bound;
-    bool fast;    // m is far enough from the type's ends (the same for a row)
-    __device__ __forceinline__ explicit Exponents(float m) {
-        c = -(m * kLog2e);
-        delta = fmaf(m, kLog2e, c);
-        fast = fabsf(m) < 1e38f;
-        if constexpr (sizeof(T) == 2) {
-            typename Pair<T>::type b;
-            const float low = m - fmaxf(140.f, fabsf(m) * (1.f / 64.f));
-            pair_from(b, low, low);
-            bound = *reinterpret_cast<const uint32_t*>(&b);
-            if (std::is_same<T, __half>::value) fast = m > -60000.f && m < INFINITY;
-        }
-    }
-    __device__ __forceinline__ uint64_t at(const Piece<T>& q, int i) const {   // of elements 2 i, 2 i + 1
-        if constexpr (sizeof(T) == 2) {
-            typedef typename Pair<T>::type P;
-            const uint32_t w = q.word(i);
-            const P held = __hmax2(*reinterpret_cast<const P*>(&w), *reinterpret_cast<const P*>(&bound));
-            const float2 v = pair_f32(held);
-            return fma2(pair_of(v.x, v.y), both(kLog2e), both(c));
-        } else {
-            const float2 v = q.pair(i);
-            float a, b;
-            pair_to(fma2(pair_of(v.x, v.y), both(kLog2e), both(c)), a, b);
-            return pair_of(fmaxf(a, kLowest), fmaxf(b, kLowest));
-        }
-    }
-};
-__device__ __forceinline__ uint64_t exp2_pair(uint64_t t) {
-    float a, b;
-    pair_to(t, a, b);
-    return pair_of(exp2_fast(a), exp2_fast(b));
-}
-__device__ __forceinline__ float both_added(uint64_t v) {
-    float a, b;
-    pair_to(v, a, b);
-    return a + b;
-}
-
-// What a set of scores adds up to beside a largest score m: the exponentials of
-// the scores below m, those times their exponents of 2, and the scores equal to m.
-struct Sums {
-    float below, weighted;
-    int equal;
-};
-
-// `own`: the largest of these scores.  The few threads that hold the largest of
-// the row first take it out.
-template <typename T, int K>
-__device__ __forceinline__ void add_up(Sums& s, Piece<T> (&q)[K], float m, float own) {
-    constexpr int kPairs = Piece<T>::kN / 2;
-    if (own == m) {
-#pragma unroll
-        for (int k = 0; k < K; ++k) s.equal += q[k].take(m);
-    }
-    const Exponents<T> x(m);
-    if (x.fast) {
-        uint64_t sum = 0ull, weighted = 0ull;
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-#pragma unroll
-            for (int i = 0; i < kPairs; ++i) {
-                const uint64_t t = x.at(q[k], i), e = exp2_pair(t);
-                sum = add2(sum, e);
-                weighted = fma2(e, t, weighted);
-            }
-        const float f = exp2_fast(-x.delta), b = both_added(sum) * f;
-        s.below += b;
-        s.weighted += fmaf(both_added(weighted), f, -x.delta * b);
-    } else {
-        for (int k = 0; k < K; ++k)
-#pragma unroll
-            for (int i = 0; i < 2 * kPairs; ++i) {
-                const float2 v = q[k].pair(i / 2);
-                const float t = fmaxf(((i % 2 ? v.y : v.x) - m) * kLog2e, kLowest), e = exp2_fast(t);
-                s.below += e;
-                s.weighted = fmaf(e, t, s.weighted);
-            }
-    }
-}
-
-// A row's numbers from its sums, written by one thread.
-struct Row {
-    float m, s;
-    bool empty, lost;   // -inf only; with a NaN or +inf
-    __device__ __forceinline__ Row(float most, float below, int equal) : m(most) {
-        empty = m == -INFINITY;
-        lost = !(m < INFINITY);
-        s = lost ? __int_as_float(0x7fffffff) : empty ? 0.f : log1pf(below + (float)(equal - 1));
-    }
-    __device__ __forceinline__ float logp(float x) const { return empty ? -INFINITY : (x - m) - s; }
-    template <typename T>
-    __device__ __forceinline__ void write(const LogpArgs& p, int64_t row, const T* x, const Sums& t) const {
-        p.stats[row] = make_float2(m, s);
-        if (p.lse) p.lse[row] = m + s;
-        if (p.entropy) p.entropy[row] = empty ? 0.f : s - t.weighted * kLn2 / (t.below + (float)t.equal);
-        if (p.logp) {
-            const int l = p.labels.at(row, p.n);
-            p.logp[row] = l < 0 ? 0.f : logp(to_f32(x[l]));
-        }
-    }
-};
-
-// ------------------------------------------------------------- the best alternatives
-
-// Scores in order as unsigned numbers (-0 as 0, NaN below all), the class behind
-// them so that of equal scores the lowest class is the greatest.  0: none.
-__device__ __forceinline__ uint64_t ranked(float v, int64_t j) {
-    const unsigned b = __float_as_uint(v + 0.f);
-    const unsigned u = v != v ? 0u : (b & 0x80000000u) ? ~b : b | 0x80000000u;
-    return (uint64_t)u << 32 | (unsigned)~(unsigned)j;
-}
-__device__ __forceinline__ int class_of(uint64_t key) { return (int)~(unsigned)key; }
-__device__ __forceinline__ float score_of(uint64_t key) {
-    const unsigned u = (unsigned)(key >> 32);
-    return u == 0 ? __int_as_float(0x7fffffff) : __uint_as_float((u & 0x80000000u) ? u & 0x7fffffffu : ~u);
-}
-__device__ __forceinline__ uint64_t warp_best(uint64_t v) {
-    const unsigned hi = __reduce_max_sync(0xffffffffu, (unsigned)(v >> 32));
-    const unsigned lo = __reduce_max_sync(0xffffffffu, (unsigned)(v >> 32) == hi ? (unsigned)v : 0u);
-    return (uint64_t)hi << 32 | lo;
-}
-
-// The `top` best of `count` distinct keys, out[i] the i-th; by a warp.
-__device__ __forceinline__ void in_order(uint64_t* out, const uint64_t* keys, int count, int top) {
-    for (int i = threadIdx.x & 31; i < count; i += 32) {
-        const uint64_t mine = keys[i];
-        int greater = 0;
-        for (int j = 0; j < count; ++j) greater += keys[j] > mine;
-        if (greater < top) out[greater] = mine;
-    }
-}
-
-// The scores that are at least `bound`, anywhere in a thread's pieces (element i of
-// piece k is class first + k step + i), go to `room` in any order: the keys differ.
-template <typename T, int K>
-__device__ __forceinline__ void gather(const Piece<T> (&q)[K], int64_t first, int64_t step, float bound, uint64_t* room, int* count,
-                                       int most) {
-    constexpr int kN = Piece<T>::kN;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-        if (!(q[k].most() >= bound)) continue;
-#pragma unroll
-        for (int i = 0; i < kN; ++i) {
-            const float2 f = q[k].pair(i / 2);
-            const float x = i % 2 ? f.y : f.x;
-            if (x >= bound) {
-                const int at = atomicAdd(count, 1);
-                if (at < most) room[at] = ranked(x, first + k * step + i);
-            }
-        }
-    }
-}
-
-// The best key below `before` of the pieces first, first + step, .. < end of a row,
-// read again: for rows whose scores are so alike (or so many -inf) that no bound
-// keeps the candidates few.
-template <typename T>
-__device__ __forceinline__ uint64_t best_below(const LogpArgs& p, const T* x, int64_t first, int64_t step, int64_t end, uint64_t before) {
-    constexpr int kN = Piece<T>::kN;
-    uint64_t b = 0;
-#pragma unroll 1
-    for (; first < end; first += step) {
-        Piece<T> q;
-        q.load(x, first, end, p.lo<T>(), p.hi<T>());
-#pragma unroll
-        for (int i = 0; i < kN; ++i) {
-            const int64_t j = first + i;
-            const float2 f = q.pair(i / 2);
-            const uint64_t v = j >= 0 && j < end ? ranked(i % 2 ? f.y : f.x, j) : 0;
-            if (v < before && v > b) b = v;
-        }
-    }
-    return b;
-}
-
-__device__ __forceinline__ void write_top(const LogpArgs& p, int64_t row, int place, uint64_t key, float m, float s) {
-    p.top_ids[row * p.top + place] = class_of(key);
-    p.top_logp[row * p.top + place] = m == -INFINITY ? -INFINITY : (score_of(key) - m) - s;
-}
-
-// ------------------------------------------------------------- a row by a warp
-//
-// Up to 16 neighbouring rows one after the other, the next one's loads under way;
-// lane r keeps row r's sums, and the logarithms, quotients and stores of all of
-// them are made together at the end (one by one they cost more than the
-// exponentials of 256 classes).
-
-constexpr int kWarpRows = 16, kWarpRoom = 64;
-
-// The best of 16-bit scores: class and score make a key of 32 bits, whose largest
-// of the warp is one instruction; a lane's next largest is that of key - taken
-// (mod 2^32, where those that were taken are smallest).
-template <typename T, int K>
-__device__ __forceinline__ void best_of_16(uint64_t* out, const Piece<T> (&q)[K], int first, int n, int top) {
-    typedef typename Pair<T>::type P;
-    uint32_t key[8 * K];
-    const P zero = {};
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t raw = q[k].word(i);
-            const P v = __hadd2(*reinterpret_cast<const P*>(&raw), zero);   // -0 as 0
-            const uint32_t w = *reinterpret_cast<const uint32_t*>(&v);
-            const uint32_t u = w ^ (((w >> 15) & 0x00010001u) * 0xffffu | 0x80008000u);
-            const int j = first + k * 256 + 2 * i;
-            key[8 * k + 2 * i] = (unsigned)j < (unsigned)n ? u << 16 | (0xffff - j) : 0u;
-            key[8 * k + 2 * i + 1] = (unsigned)(j + 1) < (unsigned)n ? (u & 0xffff0000u) | (0xfffe - j) : 0u;
-        }
-    uint32_t best = 0, mine = 0;
-    const int lane = threadIdx.x & 31;
-#pragma unroll
-    for (int i = 0; i < 8 * K; ++i) best = max(best, key[i]);
-    for (int t = 0; t < top; ++t) {
-        const uint32_t taken = __reduce_max_sync(0xffffffffu, best);
-        if (lane == t) mine = taken;
-        uint32_t left = 0;
-#pragma unroll
-        for (int i = 0; i < 8 * K; ++i) left = __viaddmax_u32(key[i], 0u - taken, left);
-        left += taken;
-        if (best == taken) best = left < taken ? left : 0u;   // another lane's best stays
-    }
-    if (lane < top) {
-        const uint16_t u = (uint16_t)(mine >> 16), h = u & 0x8000 ? u ^ 0x8000 : ~u;
-        out[lane] = ranked(to_f32(*reinterpret_cast<const T*>(&h)), 0xffff - (int)(mine & 0xffff));
-    }
-}
-
-// The best by a bound: the scores that are at least the top-th largest of the
-// lanes' largest ones hold them; mostly they are few more.  False where not.
-template <typename T, int K>
-__device__ __forceinline__ bool best_by_bound(uint64_t* out, const Piece<T> (&q)[K], int first, float own, int top, uint64_t* room,
-                                              int* count) {
-    const int lane = threadIdx.x & 31;
-    float bound = 0.f, v = own;
-    for (int k = 0; k < top; ++k) {
-        bound = warp_max(v);
-        const unsigned at = __ballot_sync(0xffffffffu, v == bound);
-        if (lane == __ffs(at) - 1) v = -INFINITY;
-    }
-    bound = fmaxf(bound, -3.4028234e38f);   // at least the scores above -inf
-    if (lane == 0) *count = 0;
-    __syncwarp();
-    if (own >= bound) gather(q, first, 32 * Piece<T>::kN, bound, room, count, kWarpRoom);
-    __syncwarp();
-    const int c = *count;
-    const bool done = c >= top && c <= kWarpRoom;
-    if (done) in_order(out, room, c, top);
-    __syncwarp();
-    return done;
-}
-
-template <typename T, int K, bool kTop, bool kWhole>
-__global__ void __launch_bounds__(128) k_logp_warp(const __grid_constant__ LogpArgs p, int rows_each) {
-    __shared__ uint64_t room[4][kWarpRoom];
-    __shared__ int count[4];
-    extern __shared__ uint64_t staged[];   // [4][rows_each][top]
-    constexpr int kN = Piece<T>::kN;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = p.n;
-    uint64_t* best = staged + (size_t)warp * rows_each * p.top;
-    const int64_t all = (p.rows + rows_each - 1) / rows_each;
-    for (int64_t group = (int64_t)blockIdx.x * 4 + warp; group < all; group += (int64_t)gridDim.x * 4) {
-        const int64_t base = group * rows_each;
-        const int rows = p.rows - base < rows_each ? (int)(p.rows - base) : rows_each;
-        const T* x = static_cast<const T*>(p.x) + base * n;
-        Piece<T> q[K], next[K];
-        int first = 0, first_next;
-        const auto load = [&](int r) {
-            const T* y = x + r * n;
-            first_next = lane * kN - (kWhole ? 0 : Piece<T>::shift_of(y));
-#pragma unroll
-            for (int k = 0; k < K; ++k) {
-                const int at = first_next + k * 32 * kN, end = r < rows ? n : -kN;
-                if (kWhole) next[k].load_whole(y, at, end);
-                else next[k].load(y, at, end, p.lo<T>(), p.hi<T>());
-            }
-        };
-        load(0);
-        float most = 0.f;
-        Sums sums = {0.f, 0.f, 0};
-        for (int r = 0; r < rows; ++r) {
-#pragma unroll
-            for (int k = 0; k < K; ++k) q[k] = next[k];
-            first = first_next;
-            load(r + 1);
-            float own = q[0].most();
-#pragma unroll
-            for (int k = 1; k < K; ++k) own = max_nan(own, q[k].most());
-            const float m = warp_max(own);
-            const bool plain = m < INFINITY && m > -INFINITY;
-            if (kTop) {
-                uint64_t* out = best + r * p.top;
-                bool done = false;
-                if (plain) {
-                    if constexpr (sizeof(T) == 2 && K <= 2) best_of_16(out, q, first, n, p.top), done = true;
-                    else done = best_by_bound(out, q, first, own, p.top, room[warp], &count[warp]);
-                }
-                if (!done) {
-                    uint64_t before = ~0ull;
-                    for (int k = 0; k < p.top; ++k) {
-                        before = warp_best(best_below(p, x + r * n, first, 32 * kN, n, before));
-                        if (lane == 0) out[k] = before;
-                    }
-                }
-            }
-            Sums t = {0.f, 0.f, 0};
-            if (plain) {
-                add_up(t, q, m, own);
-                warp_sums(t.below, t.weighted);
-                t.equal = (int)__reduce_add_sync(0xffffffffu, (unsigned)t.equal);
-            }
-            if (lane == r) {
-                most = m;
-                sums = t;
-            }
-        }
-        const Row mine(most, sums.below, sums.equal);
-        if (lane < rows) mine.write(p, base + lane, x + lane * n, sums);
-        if (kTop) {
-            __syncwarp();
-            for (int i = 0; i < rows * p.top; i += 32) {
-                const int e = i + lane, r = e / p.top;
-                const float m = __shfl_sync(0xffffffffu, mine.m, r & 31), s = __shfl_sync(0xffffffffu, mine.s, r & 31);
-                if (e < rows * p.top) write_top(p, base + r, e - r * p.top, best[e], m, s);
-            }
-            __syncwarp();
-        }
-    }
-}
-
-// ------------------------------------------------------------- a row by CTAs
-//
-// A CTA of kThreads, or a cluster of per_row of them, goes through rows, kPieces
-// accesses a thread and row.  kLoop false: the accesses of the next two rows are
-// under way as asynchronous copies, to places in shared memory that only the
-// thread itself reads, so that they need no barrier.  kLoop true: rows that no
-// cluster holds; each CTA takes its share in `rounds`, twice.  What is left to do
-// for a row when its sums are known is made for 32 rows at a time.
-
-constexpr int kRoom = 256, kBatch = 32;
-
-__device__ __forceinline__ void copy16(uint4* to, const void* from) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
-}
-
-struct Batch {
-    float m[kBatch];
-    Sums sums[kBatch];
-};
-
-template <typename T, int kThreads, int kPieces, int kAhead, bool kTop>
-__global__ void __launch_bounds__(kThreads, kThreads == 512 ? 2 : kThreads == 256 ? 3 : 6) k_logp_ctas(const __grid_constant__ LogpArgs p, int64_t share, int rounds, int per_row) {
-    constexpr bool kLoop = kAhead == 0;
-    constexpr int kWarps = kThreads / 32, kN = Piece<T>::kN, kSegment = kThreads / 32;   // 32 segments of threads
-    extern __shared__ uint4 ring[];   // [kAhead][kPieces][kThreads], then [kBatch][top] keys
-    __shared__ uint64_t room[2][kRoom], merged[8 * 32];
-    __shared__ int count[2];
-    __shared__ float segment[32], part_m[2][kWarps], cta_m[2], bound_at;
-    __shared__ Sums part[2][kWarps], cta[2];
-    __shared__ Batch batch;
-    uint64_t* best = reinterpret_cast<uint64_t*>(ring + (kLoop ? 0 : kAhead * kPieces * kThreads));
-    const cg::cluster_group cluster = cg::this_cluster();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rank = per_row > 1 ? (int)cluster.block_rank() : 0;
-    const int64_t rows_at = gridDim.x / per_row, row0 = blockIdx.x / per_row;
-    const int64_t step = (int64_t)kThreads * kN;
-    const auto row_of = [&](int64_t row) { return static_cast<const T*>(p.x) + row * p.n; };
-    const auto start_of = [&](const T* x) {
-        return (rank * share + threadIdx.x) * kN - Piece<T>::shift_of(x);
-    };
-    const auto end_of = [&](const T* x) {   // of this CTA's share of a row
-        const int64_t e = (rank + 1) * share * kN - Piece<T>::shift_of(x);
-        return e < p.n ? e : (int64_t)p.n;
-    };
-    const auto ahead = [&](int64_t row, int stage) {
-        if (row < p.rows) {
-            const T* x = row_of(row);
-            const int64_t first = start_of(x), end = end_of(x);
-#pragma unroll
-            for (int k = 0; k < kPieces; ++k) {
-                uint4* to = ring + (stage * kPieces + k) * kThreads + threadIdx.x;
-                const int64_t at = first + k * step;
-                if (at >= 0 && at + kN <= end) {
-                    copy16(to, x + at);
-                } else {
-                    Piece<T> q;
-                    q.load(x, at, end, p.lo<T>(), p.hi<T>());
-                    *to = q.q;
-                }
-            }
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-    // The rows of a batch: row0 + (i0 + i) rows_at.
-    const auto finish = [&](int64_t i0, int n) {
-        __syncthreads();
-        if (rank == 0 && warp == 0) {
-            const bool here = lane < n;
-            const Sums t = here ? batch.sums[lane] : Sums{0.f, 0.f, 1};
-            const Row mine(here ? batch.m[lane] : 0.f, t.below, t.equal);
-            const int64_t row = row0 + (i0 + lane) * rows_at;
-            if (here) mine.write(p, row, row_of(row), t);
-            for (int i = 0; i < n * p.top; i += 32) {
-                const int e = i + lane, r = p.top ? e / p.top : 0;
-                const float m = __shfl_sync(0xffffffffu, mine.m, r & 31), s = __shfl_sync(0xffffffffu, mine.s, r & 31);
-                if (e < n * p.top) write_top(p, row0 + (i0 + r) * rows_at, e - r * p.top, best[e], m, s);
-            }
-        }
-        __syncthreads();
-    };
-    if (threadIdx.x < 2) count[threadIdx.x] = 0;
-    __syncthreads();
-    if (!kLoop) {
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) ahead(row0 + i * rows_at, i);
-    }
-    int64_t it = 0;
-    int held = 0;
-    for (int64_t row = row0; row < p.rows; row += rows_at, ++it) {
-        const T* x = row_of(row);
-        const int64_t start = start_of(x), end = end_of(x);
-        const int buf = (int)(it & 1);
-        Piece<T> q[kPieces];
-        const auto load = [&](int round) {
-#pragma unroll
-            for (int k = 0; k < kPieces; ++k) q[k].load(x, start + ((int64_t)round * kPieces + k) * step, end, p.lo<T>(), p.hi<T>());
-        };
-        const auto most = [&] {
-            float v = q[0].most();
-#pragma unroll
-            for (int k = 1; k < kPieces; ++k) v = max_nan(v, q[k].most());
-            return v;
-        };
-        float own = -INFINITY;
-        if (kLoop) {
-            for (int round = 0; round < rounds; ++round) {
-                load(round);
-                own = max_nan(own, most());
-            }
-        } else {
-            constexpr int kSlots = kAhead > 0 ? kAhead : 1;
-            const int slot = (int)(it % kSlots);
-            asm volatile("cp.async.wait_group %0;" ::"n"(kSlots - 1) : "memory");
-            const uint4* from = ring + slot * kPieces * kThreads + threadIdx.x;
-#pragma unroll
-            for (int k = 0; k < kPieces; ++k) q[k].q = from[k * kThreads];
-            own = most();   // the places have been read
-            ahead(row + kSlots * rows_at, slot);
-        }
-        float m = warp_max(own);
-        if (lane == 0) part_m[buf][warp] = m;
-        if (kTop) {   // the largest of each of 32 neighbouring groups of threads (no NaN there: fmaxf)
-            float v = own;
-#pragma unroll
-            for (int d = 1; d < (kSegment < 32 ? kSegment : 32); d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
-            if (threadIdx.x % kSegment == 0) segment[threadIdx.x / kSegment] = v;
-        }
-        __syncthreads();
-        m = warp_max(part_m[buf][lane % kWarps]);
-        if (per_row > 1) {
-            if (threadIdx.x == 0) cta_m[buf] = m;
-            cluster.sync();
-            m = warp_max(*cluster.map_shared_rank(&cta_m[buf], lane % per_row));
-        }
-        const bool plain = m < INFINITY && m > -INFINITY;
-        bool bounded = false;
-        if (kTop && plain) {   // the same for all threads
-            if (warp == 0) {
-                const float mine = segment[lane];
-                int before = 0;   // segments in front of this one
-                for (int i = 0; i < 32; ++i) before += segment[i] > mine || (segment[i] == mine && i < lane);
-                if (before == p.top - 1) bound_at = fmaxf(mine, -3.4028234e38f);   // at least the scores above -inf
-            }
-            __syncthreads();
-            bounded = true;
-        }
-        Sums t = {0.f, 0.f, 0};
-        for (int round = 0; round < (kLoop ? rounds : 1); ++round) {
-            if (kLoop) {
-                load(round);
-                own = most();
-            }
-            if (bounded && own >= bound_at)
-                gather(q, start + (int64_t)round * kPieces * step, step, bound_at, room[buf], &count[buf], kRoom);
-            if (plain) add_up(t, q, m, own);
-        }
-        warp_sums(t.below, t.weighted);
-        t.equal = (int)__reduce_add_sync(0xffffffffu, (unsigned)t.equal);
-        if (lane == 0) part[buf][warp] = t;
-        __syncthreads();
-        uint64_t* out = best + held * p.top;   // of this CTA, where a cluster has several
-        if (kTop) {
-            const int c = count[buf];
-            if (bounded && c <= kRoom && c >= (per_row > 1 && end <= start - threadIdx.x * kN ? 0 : p.top)) {
-                if (warp == 0) {
-                    if (lane < p.top) out[lane] = 0;   // a share may have fewer
-                    __syncwarp();
-                    in_order(out, room[buf], c, p.top);
-                }
-            } else {
-                uint64_t before = ~0ull;
-                for (int k = 0; k < p.top; ++k) {
-                    uint64_t b = best_below(p, x, start, step, end, before);
-                    b = warp_best(b);
-                    __syncthreads();
-                    if (lane == 0) merged[warp] = b;
-                    __syncthreads();
-                    before = warp_best(merged[lane % kWarps]);
-                    if (threadIdx.x == 0) out[k] = before;
-                }
-            }
-            __syncthreads();
-            if (threadIdx.x == 0) count[buf] = 0;
-        }
-        if (warp == kWarps - 1) {
-            Sums all = lane < kWarps ? part[buf][lane] : Sums{0.f, 0.f, 0};
-            warp_sums(all.below, all.weighted);
-            all.equal = (int)__reduce_add_sync(0xffffffffu, (unsigned)all.equal);
-            if (lane == 0) {
-                if (per_row > 1) {
-                    cta[buf] = all;
-                } else {
-                    batch.m[held] = m;
-                    batch.sums[held] = all;
-                }
-            }
-        }
-        if (per_row > 1) {
-            cluster.sync();
-            if (rank == 0 && warp == 0) {
-                Sums all = lane < per_row ? *cluster.map_shared_rank(&cta[buf], lane % per_row) : Sums{0.f, 0.f, 0};
-                warp_sums(all.below, all.weighted);
-                all.equal = (int)__reduce_add_sync(0xffffffffu, (unsigned)all.equal);
-                if (lane == 0) {
-                    batch.m[held] = m;
-                    batch.sums[held] = all;
-                }
-                if (kTop) {
-                    for (int c = 0; c < per_row; ++c)
-                        if (lane < p.top) merged[c * p.top + lane] = *cluster.map_shared_rank(out + lane, c);
-                    __syncwarp();
-                    int n = 0;   // keys that are there, close together
-                    for (int i = lane; i < (per_row * p.top + 31) / 32 * 32; i += 32) {
-                        const uint64_t v = i < per_row * p.top ? merged[i] : 0;
-                        const unsigned there = __ballot_sync(0xffffffffu, v != 0);
-                        if (v) merged[n + __popc(there & ((1u << lane) - 1))] = v;
-                        n += __popc(there);
-                        __syncwarp();
-                    }
-                    in_order(out, merged, n, p.top);
-                }
-            }
-            if (kTop) cluster.sync();   // the others' lists have been read
-        }
-        if (++held == kBatch) {
-            finish(it - held + 1, held);
-            held = 0;
-        }
-    }
-    if (held) finish(it - held, held);
-    if (per_row > 1) cluster.sync();   // what is shared outlives its readers
-}
-
-// ------------------------------------------------------------- few classes
-
-constexpr int kFewClasses = 64, kTileRows = 128;
-
-// A tile of rows lies in memory as one stretch: 16 bytes at a time (its start
-// allows that when the tensor's does) to shared memory, where rows are `pitch`
-// apart, so that a thread a row meets few others in its banks: an odd number of
-// words, or a word and a half more or less.
-template <typename T> __host__ __device__ inline int pitch_of(int n) {
-    return sizeof(T) == 4 ? n | 1 : n % 4 == 0 ? n + 2 : n;
-}
-
-struct Place {   // of an element of a tile: at most 128 x 64 of them, so the quotient is exact
-    int row, j;
-    __device__ __forceinline__ Place(int i, int n) {
-        row = (int)(((unsigned)i * ((1u << 20) / (unsigned)n + 1u)) >> 20);
-        j = i - row * n;
-    }
-    __device__ __forceinline__ void next(int n) {
-        if (++j == n) j = 0, ++row;
-    }
-};
-
-// kIn: memory to tile, else back.
-template <typename T, bool kIn>
-__device__ __forceinline__ void tile_copy(T* tile, T* x, int count, int n, bool vec) {
-    constexpr int kN = 16 / (int)sizeof(T);
-    const int pitch = pitch_of<T>(n);
-    const int whole = vec ? count / kN : 0;
-    for (int i = threadIdx.x; i < whole; i += kTileRows) {
-        if (pitch == n) {
-            if (kIn) copy16(reinterpret_cast<uint4*>(tile) + i, reinterpret_cast<const uint4*>(x) + i);
-            else reinterpret_cast<uint4*>(x)[i] = reinterpret_cast<const uint4*>(tile)[i];
-            continue;
-        }
-        union { uint4 u; T e[kN]; } r;
-        Place at(i * kN, n);
-        if (kIn) r.u = reinterpret_cast<const uint4*>(x)[i];
-#pragma unroll
-        for (int k = 0; k < kN; ++k, at.next(n)) {
-            if (kIn) tile[at.row * pitch + at.j] = r.e[k];
-            else r.e[k] = tile[at.row * pitch + at.j];
-        }
-        if (!kIn) reinterpret_cast<uint4*>(x)[i] = r.u;
-    }
-    for (int i = whole * kN + threadIdx.x; i < count; i += kTileRows) {
-        const Place at(i, n);
-        if (kIn) tile[at.row * pitch + at.j] = x[i];
-        else x[i] = tile[at.row * pitch + at.j];
-    }
-    if (kIn) asm volatile("cp.async.wait_all;" ::: "memory");
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kTileRows) k_logp_few(const __grid_constant__ LogpArgs p, bool vec) {
-    extern __shared__ uint4 memory[];
-    T* tile = reinterpret_cast<T*>(memory);
-    for (int64_t base = (int64_t)blockIdx.x * kTileRows; base < p.rows; base += (int64_t)gridDim.x * kTileRows) {
-        const int rows = p.rows - base < kTileRows ? (int)(p.rows - base) : kTileRows, n = p.n;
-        tile_copy<T, true>(tile, const_cast<T*>(static_cast<const T*>(p.x)) + base * n, rows * n, n, vec);
-        __syncthreads();
-        if ((int)threadIdx.x < rows) {
-            const int64_t row = base + threadIdx.x;
-            const T* x = tile + threadIdx.x * pitch_of<T>(n);
-            float m = -INFINITY;
-            for (int j = 0; j < n; ++j) m = max_nan(m, to_f32(x[j]));
-            Sums t = {0.f, 0.f, 0};
-            if (m < INFINITY && m > -INFINITY)
-                for (int j = 0; j < n; ++j) {
-                    const float d = to_f32(x[j]) - m, e2 = fmaxf(d * kLog2e, kLowest), e = exp2_fast(e2);
-                    t.equal += d == 0.f;
-                    t.below += d == 0.f ? 0.f : e;
-                    t.weighted = fmaf(e, e2, t.weighted);
-                }
-            const Row done(m, t.below, t.equal);
-            done.write(p, row, x, t);
-            uint64_t before = ~0ull;
-            for (int k = 0; k < p.top; ++k) {
-                uint64_t b = 0;
-                for (int j = 0; j < n; ++j) {
-                    const uint64_t v = ranked(to_f32(x[j]), j);
-                    if (v < before && v > b) b = v;
-                }
-                before = b;
-                p.top_ids[row * p.top + k] = class_of(b);
-                p.top_logp[row * p.top + k] = done.logp(score_of(b));
-            }
-        }
-        __syncthreads();
-    }
-}
-
-// ------------------------------------------------------------- the gradient
-
-// What the elements of a row have in common: p (all - ge log p), and gl more at
-// the label.
-struct RowGrad {
-    float m, s, all, ge, gl;
-    float rest;   // of all without gl: at the label
-    int label;
-    __device__ __forceinline__ RowGrad(const LogpArgs& p, int64_t row) {
-        const float2 st = p.stats[row];
-        m = st.x;
-        s = st.y;
-        label = p.gl ? p.labels.at(row, p.n) : -1;
-        gl = label >= 0 ? p.gl[row] : 0.f;
-        ge = p.ge ? p.ge[row] : 0.f;
-        rest = (p.gz ? p.gz[row] : 0.f) - (p.ge ? ge * p.entropy[row] : 0.f);
-        all = rest - gl;
-    }
-    // The label's own 1 - p would lose what a confident answer leaves.
-    __device__ __forceinline__ float at_label(float x) const {
-        const float lp = (x - m) - s, t = max_nan(lp * kLog2e, kLowest);
-        return m == -INFINITY ? 0.f : fmaf(exp2_fast(t), fmaf(-ge * kLn2, t, rest), -gl * expm1f(lp));
-    }
-    __device__ __forceinline__ float at(float x) const {
-        const float t = max_nan(((x - m) - s) * kLog2e, kLowest);   // NaN of a row that has one stays
-        return m == -INFINITY ? 0.f : exp2_fast(t) * fmaf(-ge * kLn2, t, all);
-    }
-};
-
-// The gradients of a piece at class `at` of its row.  log2 p = t - kappa with t of
-// Exponents and kappa = delta + s log2(e), so that p (all - ge log p) = 2^t (a + b t).
-template <typename T> struct PieceGrad {
-    static constexpr int kN = Piece<T>::kN;
-    RowGrad g;
-    Exponents<T> x;
-    float a, b;
-    __device__ __forceinline__ explicit PieceGrad(const RowGrad& g_) : g(g_), x(g_.m) {
-        const float kappa = fmaf(g.s, kLog2e, x.delta), f = exp2_fast(-kappa), e = g.ge * kLn2;
-        a = f * fmaf(e, kappa, g.all);
-        b = -f * e;
-    }
-    __device__ __forceinline__ void of(float (&v)[kN], const Piece<T>& q, int64_t at) const {
-        if (x.fast) {
-#pragma unroll
-            for (int i = 0; i < kN / 2; ++i) {
-                const uint64_t t = x.at(q, i);
-                pair_to(mul2(exp2_pair(t), fma2(t, both(b), both(a))), v[2 * i], v[2 * i + 1]);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < kN; ++i) {
-                const float2 f = q.pair(i / 2);
-                v[i] = g.at(i % 2 ? f.y : f.x);
-            }
-        }
-        const int64_t l = g.label - at;
-        if (l >= 0 && l < kN && g.label >= 0) {
-            float own = 0.f;
-#pragma unroll
-            for (int i = 0; i < kN; ++i) {
-                const float2 f = q.pair(i / 2);
-                own = i == l ? (i % 2 ? f.y : f.x) : own;
-            }
-            own = g.at_label(own);
-#pragma unroll
-            for (int i = 0; i < kN; ++i) v[i] = i == l ? own : v[i];
-        }
-    }
-};
-
-// `whole`: all of the piece is in the row and the gradient's row lies as the scores' does.
-template <typename T>
-__device__ __forceinline__ void store_piece(T* gx, const float (&v)[Piece<T>::kN], int64_t at, int64_t n, bool whole) {
-    constexpr int kN = Piece<T>::kN;
-    if (whole) {
-        Vec<T, kN> o;
-        o.from(v);
-        o.store(gx + at);
-    } else {
-#pragma unroll
-        for (int i = 0; i < kN; ++i)
-            if (at + i >= 0 && at + i < n) gx[at + i] = from_f32<T>(v[i]);
-    }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kTileRows) k_logp_few_grad(const __grid_constant__ LogpArgs p, bool vec, bool vec_out) {
-    extern __shared__ uint4 memory[];
-    T* tile = reinterpret_cast<T*>(memory);
-    for (int64_t base = (int64_t)blockIdx.x * kTileRows; base < p.rows; base += (int64_t)gridDim.x * kTileRows) {
-        const int rows = p.rows - base < kTileRows ? (int)(p.rows - base) : kTileRows, n = p.n;
-        tile_copy<T, true>(tile, const_cast<T*>(static_cast<const T*>(p.x)) + base * n, rows * n, n, vec);
-        __syncthreads();
-        if ((int)threadIdx.x < rows) {
-            const RowGrad g(p, base + threadIdx.x);
-            T* x = tile + threadIdx.x * pitch_of<T>(n);
-            const float label = g.label >= 0 ? to_f32(x[g.label]) : 0.f;
-            for (int j = 0; j < n; ++j) x[j] = from_f32<T>(g.at(to_f32(x[j])));
-            if (g.label >= 0) x[g.label] = from_f32<T>(g.at_label(label));
-        }
-        __syncthreads();
-        tile_copy<T, false>(tile, static_cast<T*>(p.gx) + base * n, rows * n, n, vec_out);
-        __syncthreads();
-    }
-}
-
-// A warp a row, up to 32 neighbouring ones after another; lane r reads what row r's
-// elements have in common.  kAtOnce accesses are under way together.
-constexpr int kAtOnce = 4;
-
-template <typename T, bool kWhole>
-__global__ void __launch_bounds__(128) k_logp_grad_warp(const __grid_constant__ LogpArgs p, int rows_each, int pieces, bool same) {
-    constexpr int kN = Piece<T>::kN;
-    const int lane = threadIdx.x & 31, n = p.n;
-    const int64_t all = (p.rows + rows_each - 1) / rows_each;
-    for (int64_t group = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5); group < all; group += (int64_t)gridDim.x * 4) {
-        const int64_t base = group * rows_each;
-        const int rows = p.rows - base < rows_each ? (int)(p.rows - base) : rows_each;
-        const T* x = static_cast<const T*>(p.x) + base * n;
-        T* gx = static_cast<T*>(p.gx) + base * n;
-        const RowGrad own(p, base + (lane < rows ? lane : rows - 1));
-        const int count = rows * pieces;   // piece i: of row i / pieces
-        for (int i0 = 0, r0 = 0, k0 = 0; i0 < count; i0 += kAtOnce) {
-            Piece<T> q[kAtOnce];
-            int row[kAtOnce], at[kAtOnce];
-#pragma unroll
-            for (int u = 0; u < kAtOnce; ++u) {
-                const T* y = x + r0 * n;
-                row[u] = r0;
-                at[u] = (k0 * 32 + lane) * kN - (kWhole ? 0 : Piece<T>::shift_of(y));
-                const int end = r0 < rows ? n : -kN;
-                if (kWhole) q[u].load_whole(y, at[u], end);
-                else q[u].load(y, at[u], end, p.lo<T>(), p.hi<T>());
-                if (++k0 == pieces) k0 = 0, ++r0;
-            }
-#pragma unroll
-            for (int u = 0; u < kAtOnce; ++u) {
-                if (row[u] >= rows) break;
-                RowGrad g = own;
-                g.m = __shfl_sync(0xffffffffu, own.m, row[u]);
-                g.s = __shfl_sync(0xffffffffu, own.s, row[u]);
-                g.all = __shfl_sync(0xffffffffu, own.all, row[u]);
-                g.ge = __shfl_sync(0xffffffffu, own.ge, row[u]);
-                g.gl = __shfl_sync(0xffffffffu, own.gl, row[u]);
-                g.rest = __shfl_sync(0xffffffffu, own.rest, row[u]);
-                g.label = __shfl_sync(0xffffffffu, own.label, row[u]);
-                float v[kN];
-                PieceGrad<T>(g).of(v, q[u], at[u]);
-                if (at[u] < n)
-                    store_piece<T>(gx + row[u] * n, v, at[u], n, same && (kWhole || (at[u] >= 0 && at[u] + kN <= n)));
-            }
-        }
-    }
-}
-
-// A CTA a share of a row: kAtOnce accesses a thread.
-template <typename T>
-__global__ void __launch_bounds__(256) k_logp_grad(const __grid_constant__ LogpArgs p, int64_t shares, bool same) {
-    constexpr int kN = Piece<T>::kN;
-    const int64_t all = p.rows * shares;
-    for (int64_t share = blockIdx.x; share < all; share += gridDim.x) {
-        const int64_t row = share / shares;
-        const T* x = static_cast<const T*>(p.x) + row * p.n;
-        const int64_t first = ((share - row * shares) * (256 * kAtOnce) + threadIdx.x) * kN - Piece<T>::shift_of(x), n = p.n;
-        Piece<T> q[kAtOnce];
-#pragma unroll
-        for (int k = 0; k < kAtOnce; ++k) q[k].load(x, first + k * 256 * kN, n, p.lo<T>(), p.hi<T>());
-        const PieceGrad<T> g(RowGrad(p, row));
-#pragma unroll
-        for (int k = 0; k < kAtOnce; ++k) {
-            const int64_t at = first + k * 256 * kN;
-            if (at >= n) break;
-            float v[kN];
-            g.of(v, q[k], at);
-            store_piece<T>(static_cast<T*>(p.gx) + row * n, v, at, n, same && at >= 0 && at + kN <= n);
-        }
-    }
-}
-
-// ------------------------------------------------------------------ host side
-
-template <typename T> static bool whole_rows(const LogpArgs& a) { return a.n % Piece<T>::kN == 0 && aligned16(a.x); }
-template <typename T> static int64_t vectors_of(const LogpArgs& a) {   // of a row, wherever it begins
-    return ceil_div((int64_t)a.n + (whole_rows<T>(a) ? 0 : Piece<T>::kN - 1), Piece<T>::kN);
-}
-
-static unsigned grid_of(int64_t ctas) { return (unsigned)(ctas < (1 << 30) ? ctas : 1 << 30); }
-
-// As many CTAs as are resident at a time (in clusters of per_row).
-template <typename T, int kThreads, int kPieces, int kAhead, bool kTop>
-static cudaError_t launch_ctas(const LogpArgs& a, int64_t nv, int per_row, cudaStream_t s) {
-    const auto kernel = k_logp_ctas<T, kThreads, kPieces, kAhead, kTop>;
-    constexpr int kRing = kAhead * kPieces * kThreads * 16;
-    const int64_t share = ceil_div(nv, per_row);
-    int resident = 0;
-    const cudaError_t e = pl::kernel_once(
-        reinterpret_cast<const void*>(kernel),
-        [](int* n) {
-            const auto k = k_logp_ctas<T, kThreads, kPieces, kAhead, kTop>;
-            const int most = kRing + (kTop ? kBatch * PLATTICE_MAX_TOP * 8 : 0);
-            const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
-            return e != cudaSuccess ? e : cudaOccupancyMaxActiveBlocksPerMultiprocessor(n, k, kThreads, most);
-        },
-        &resident);
-    if (e != cudaSuccess) return e;
-    int64_t rows = (int64_t)(resident > 0 ? resident : 1) * sm_count() / per_row;
-    if (rows < 1) rows = 1;
-    if (rows > a.rows) rows = a.rows;
-    cudaLaunchConfig_t c = {};
-    c.gridDim = dim3((unsigned)(rows * per_row));
-    c.blockDim = dim3(kThreads);
-    c.dynamicSmemBytes = kRing + (size_t)kBatch * a.top * 8;
-    c.stream = s;
-    cudaLaunchAttribute attr = {};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = (unsigned)per_row;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    c.attrs = &attr;
-    c.numAttrs = per_row > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&c, kernel, a, share, (int)ceil_div(share, kPieces * kThreads), per_row);
-}
-
-template <typename T, int kThreads, int kPieces, int kAhead>
-static cudaError_t launch_ctas(const LogpArgs& a, int64_t nv, int per_row, cudaStream_t s) {
-    return a.top ? launch_ctas<T, kThreads, kPieces, kAhead, true>(a, nv, per_row, s)
-                 : launch_ctas<T, kThreads, kPieces, kAhead, false>(a, nv, per_row, s);
-}
-
-// Rows a warp takes one after the other: few where there are few, so that all SMs work.
-static int rows_each(int64_t rows, int most) {
-    const int64_t want = rows / (sm_count() * 32);
-    return want < 1 ? 1 : want > most ? most : (int)want;
-}
-
-template <typename T, int K, bool kTop>
-static cudaError_t launch_warp(const LogpArgs& a, cudaStream_t s) {
-    const int each = rows_each(a.rows, kWarpRows);
-    const unsigned ctas = grid_of(ceil_div(a.rows, 4 * each));
-    const size_t smem = (size_t)4 * each * a.top * 8;
-    if (whole_rows<T>(a)) k_logp_warp<T, K, kTop, true><<<ctas, 128, smem, s>>>(a, each);
-    else k_logp_warp<T, K, kTop, false><<<ctas, 128, smem, s>>>(a, each);
-    return cudaGetLastError();
-}
-template <typename T, int K>
-static cudaError_t launch_warp(const LogpArgs& a, cudaStream_t s) {
-    return a.top ? launch_warp<T, K, true>(a, s) : launch_warp<T, K, false>(a, s);
-}
-
-template <typename T>
-static cudaError_t forward(const LogpArgs& a, cudaStream_t s) {
-    if (a.n <= kFewClasses) {
-        k_logp_few<T><<<grid_of(ceil_div(a.rows, kTileRows)), kTileRows, kTileRows * pitch_of<T>(a.n) * sizeof(T), s>>>(
-            a, aligned16(a.x));
-        return cudaGetLastError();
-    }
-    const int64_t nv = vectors_of<T>(a);
-    if (nv <= 32) return launch_warp<T, 1>(a, s);
-    if (nv <= 64) return launch_warp<T, 2>(a, s);
-    if (nv <= 96) return launch_warp<T, 3>(a, s);
-    if (nv <= 128) return launch_warp<T, 4>(a, s);
-    if (nv <= 160) return launch_warp<T, 5>(a, s);
-    // The smallest cluster that holds the row; a larger one where the rows leave SMs without work.
-    int per_row = 1;
-    while (per_row < 8 && (nv > 4096 * (int64_t)per_row || (a.rows * per_row * 2 <= sm_count() && nv >= 1024 * (int64_t)per_row)))
-        per_row *= 2;
-    const int64_t share = ceil_div(nv, per_row);
-    if (share <= 512) return launch_ctas<T, 128, 4, 3>(a, nv, per_row, s);
-    if (share <= 1024) return launch_ctas<T, 128, 8, 2>(a, nv, per_row, s);
-    if (share <= 2048) return launch_ctas<T, 256, 8, 2>(a, nv, per_row, s);
-    if (share <= 4096) return launch_ctas<T, 512, 8, 1>(a, nv, per_row, s);
-    return launch_ctas<T, 512, 8, 0>(a, nv, per_row, s);
-}
-
-template <typename T>
-static cudaError_t backward(const LogpArgs& a, cudaStream_t s) {
-    if (a.n <= kFewClasses) {
-        k_logp_few_grad<T><<<grid_of(ceil_div(a.rows, kTileRows)), kTileRows, kTileRows * pitch_of<T>(a.n) * sizeof(T), s>>>(
-            a, aligned16(a.x), aligned16(a.gx));
-        return cudaGetLastError();
-    }
-    const int64_t nv = vectors_of<T>(a);
-    const bool same = (((uintptr_t)a.x ^ (uintptr_t)a.gx) & 15) == 0;
-    if (nv <= 160) {
-        const int each = rows_each(a.rows, 32), pieces = (int)ceil_div(nv, 32);
-        const unsigned ctas = grid_of(ceil_div(a.rows, 4 * each));
-        if (whole_rows<T>(a)) k_logp_grad_warp<T, true><<<ctas, 128, 0, s>>>(a, each, pieces, same);
-        else k_logp_grad_warp<T, false><<<ctas, 128, 0, s>>>(a, each, pieces, same);
-    } else {
-        const int64_t shares = ceil_div(nv, 256 * kAtOnce);
-        k_logp_grad<T><<<grid_of(a.rows * shares), 256, 0, s>>>(a, shares, same);
-    }
-    return cudaGetLastError();
-}
-
-}  // namespace plr
+#include "rows_logp.h"
 
 using namespace plr;
 
@@ -1132,7 +14,7 @@ static bool logp_ok(const plattice_log_probs_args* q) {
 }
 
 static LogpArgs logp_args(const plattice_log_probs_args* q) {
-    return {q->logits, {q->labels, q->labels_wide}, q->logp, q->entropy, reinterpret_cast<float2*>(q->stats), q->lse, q->top_logp,
+    return {q->logits, q->labels, q->labels_wide, q->logp, q->entropy, reinterpret_cast<float2*>(q->stats), q->lse, q->top_logp,
             q->top_ids, q->grad_logp, q->grad_entropy, q->grad_lse, q->grad_logits, q->rows, q->n, q->top};
 }
 
@@ -1144,9 +26,9 @@ int plattice_log_probs(const plattice_log_probs_args* q, void* stream) {
         return PLATTICE_ERR_INVALID;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const LogpArgs a = logp_args(q);
-    const cudaError_t e = q->dtype == PLATTICE_F32    ? forward<float>(a, s)
-                          : q->dtype == PLATTICE_BF16 ? forward<__nv_bfloat16>(a, s)
-                                                      : forward<__half>(a, s);
+    const cudaError_t e = q->dtype == PLATTICE_F32    ? logp_forward<float>(a, s)
+                          : q->dtype == PLATTICE_BF16 ? logp_forward<__nv_bfloat16>(a, s)
+                                                      : logp_forward<__half>(a, s);
     return rows_status(e, "plattice_log_probs");
 }
 
@@ -1158,9 +40,9 @@ int plattice_log_probs_backward(const plattice_log_probs_args* q, void* stream) 
         return PLATTICE_ERR_INVALID;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const LogpArgs a = logp_args(q);
-    const cudaError_t e = q->dtype == PLATTICE_F32    ? backward<float>(a, s)
-                          : q->dtype == PLATTICE_BF16 ? backward<__nv_bfloat16>(a, s)
-                                                      : backward<__half>(a, s);
+    const cudaError_t e = q->dtype == PLATTICE_F32    ? logp_backward<float>(a, s)
+                          : q->dtype == PLATTICE_BF16 ? logp_backward<__nv_bfloat16>(a, s)
+                                                      : logp_backward<__half>(a, s);
     return rows_status(e, "plattice_log_probs_backward");
 }
 
