@@ -11,6 +11,8 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/extension.h>
 
+#include <cmath>
+
 #include "plattice.h"
 
 namespace {
@@ -357,6 +359,289 @@ py::object rows_linear_backward(const py::object& g0_, const py::object& g1_, co
     return py::make_tuple(need_x ? wrap(gx) : none, need_w ? wrap(gw) : none, need_b ? wrap(gb) : none);
 }
 
+// ------------------------------------------------ labels, lines, log probabilities, clipping
+
+struct MoreEntry {
+    decltype(&plattice_embed) embed = nullptr;
+    decltype(&plattice_embed_backward_workspace_size) embed_backward_ws = nullptr;
+    decltype(&plattice_embed_backward) embed_backward = nullptr;
+    decltype(&plattice_scan_workspace_size) scan_ws = nullptr;
+    decltype(&plattice_scan) scan = nullptr;
+    decltype(&plattice_scan_backward_workspace_size) scan_backward_ws = nullptr;
+    decltype(&plattice_scan_backward) scan_backward = nullptr;
+    decltype(&plattice_log_probs) log_probs = nullptr;
+    decltype(&plattice_log_probs_backward) log_probs_backward = nullptr;
+    decltype(&plattice_clip_grads_workspace_size) clip_ws = nullptr;
+    decltype(&plattice_clip_grads) clip = nullptr;
+} g_more;
+
+void set_more_entry_points(const std::vector<int64_t>& a) {
+    TORCH_CHECK(a.size() == 11, "eleven entry points");
+    set_one(g_more.embed, a[0]);
+    set_one(g_more.embed_backward_ws, a[1]);
+    set_one(g_more.embed_backward, a[2]);
+    set_one(g_more.scan_ws, a[3]);
+    set_one(g_more.scan, a[4]);
+    set_one(g_more.scan_backward_ws, a[5]);
+    set_one(g_more.scan_backward, a[6]);
+    set_one(g_more.log_probs, a[7]);
+    set_one(g_more.log_probs_backward, a[8]);
+    set_one(g_more.clip_ws, a[9]);
+    set_one(g_more.clip, a[10]);
+}
+
+// A contiguous CUDA tensor of int64 or int32.
+const at::Tensor* labels_of(const py::handle& o) {
+    if (!THPVariable_Check(o.ptr())) return nullptr;
+    const at::Tensor& t = THPVariable_Unpack(o.ptr());
+    return t.is_cuda() && t.layout() == at::kStrided && t.is_contiguous() &&
+                   (t.scalar_type() == at::kLong || t.scalar_type() == at::kInt)
+               ? &t
+               : nullptr;
+}
+bool wide(const at::Tensor& labels) { return labels.scalar_type() == at::kLong; }
+bool is_f32(const at::Tensor* t, at::IntArrayRef sizes, const at::Device& d) {
+    return t && t->scalar_type() == at::kFloat && t->sizes() == sizes && t->device() == d;
+}
+
+py::object rows_embed(const py::object& ids_, const py::object& table_, double scale) {
+    const at::Tensor *ids = labels_of(ids_), *table = floating(table_);
+    if (!ids || !table || table->dim() != 2 || table->size(0) < 1 || table->size(0) > 0x7fffffff || table->size(1) < 1 ||
+        table->size(1) > (1 << 21) || ids->device() != table->device() || !std::isfinite(scale))
+        return py::none();
+    const c10::cuda::CUDAGuard guard(table->device());
+    c10::SmallVector<int64_t, 8> shape(ids->sizes().begin(), ids->sizes().end());
+    shape.push_back(table->size(1));
+    const at::Tensor y = fresh(shape, table->scalar_type(), table->device());
+    const int rc = g_more.embed(y.data_ptr(), ids->data_ptr(), wide(*ids), table->data_ptr(), dtype_code(table->scalar_type()),
+                                (float)scale, ids->numel(), table->size(0), (int)table->size(1), stream_of(table->device()));
+    if (rc) return py::int_(rc);
+    return wrap(y);
+}
+
+py::object rows_embed_backward(const py::object& gy_, const py::object& ids_, int64_t n, double scale, int dtype) {
+    const at::Tensor *gy = floating(gy_), *ids = labels_of(ids_);
+    if (!rows_tensor(gy) || !ids || gy->size(-1) > (1 << 21) || ids->sizes() != gy->sizes().slice(0, gy->dim() - 1) ||
+        ids->device() != gy->device() || ids->numel() > 0x7fffffff || n < 1 || n > 0x7fffffff || !std::isfinite(scale))
+        return py::none();
+    const c10::cuda::CUDAGuard guard(gy->device());
+    const int64_t c = gy->size(-1), count = ids->numel();
+    if (dtype < 0) dtype = dtype_code(gy->scalar_type());
+    size_t need = 0;
+    int rc = g_more.embed_backward_ws(count, n, (int)c, &need);
+    if (rc) return py::int_(rc);
+    const at::Tensor grad = fresh({n, c}, type_of(dtype), gy->device()), ws = fresh({(int64_t)need}, at::kByte, gy->device());
+    rc = g_more.embed_backward(grad.data_ptr(), dtype, gy->data_ptr(), dtype_code(gy->scalar_type()), ids->data_ptr(), wide(*ids),
+                               (float)scale, ws.data_ptr(), need, count, n, (int)c, stream_of(gy->device()));
+    if (rc) return py::int_(rc);
+    return wrap(grad);
+}
+
+// Checked arguments that the scan and its backward have in common; false where not.
+struct ScanCall {
+    plattice_scan_args a = {};
+    c10::SmallVector<int64_t, 8> one, many;   // shapes of a state, of the kept ones
+    at::Tensor ws;
+    bool set(const at::Tensor* x, const at::Tensor* gate, bool blend, bool reverse) {
+        if (!rows_tensor(x) || x->dim() < 2 || !gate || !like(*gate, *x) || x->size(-1) > (1 << 30)) return false;
+        a.x = x->data_ptr();
+        a.gate = gate->data_ptr();
+        a.steps = x->size(-2);
+        a.c = (int)x->size(-1);
+        a.lines = 1;
+        for (int64_t i = 0; i < x->dim() - 2; ++i) {
+            one.push_back(x->size(i));
+            a.lines *= x->size(i);
+        }
+        many = one;
+        one.push_back(a.c);
+        many.push_back((a.steps + PLATTICE_SCAN_KEEP - 1) / PLATTICE_SCAN_KEEP);
+        many.push_back(a.c);
+        a.dtype = dtype_code(x->scalar_type());
+        a.blend = blend;
+        a.reverse = reverse;
+        return true;
+    }
+    template <typename Size, typename Call> int run(Size size, Call call, const at::Device& d) {
+        const int rc = size(&a, &a.workspace_bytes);
+        if (rc) return rc;
+        if (a.workspace_bytes) {
+            ws = fresh({(int64_t)a.workspace_bytes}, at::kByte, d);
+            a.workspace = ws.data_ptr();
+        }
+        return call(&a, stream_of(d));
+    }
+};
+
+py::object rows_scan(const py::object& x_, const py::object& gate_, const py::object& state_, bool blend, bool reverse, bool keep) {
+    const at::Tensor *x = floating(x_), *gate = floating(gate_), *state = state_.is_none() ? nullptr : floating(state_);
+    ScanCall c;
+    if (!c.set(x, gate, blend, reverse) || (!state_.is_none() && !is_f32(state, c.one, x->device()))) return py::none();
+    const c10::cuda::CUDAGuard guard(x->device());
+    const at::Tensor h = fresh_like(*x), last = fresh(c.one, at::kFloat, x->device());
+    at::Tensor states;
+    if (keep) {
+        states = fresh(c.many, at::kFloat, x->device());
+        c.a.states = states.data_ptr<float>();
+    }
+    c.a.state = state ? state->data_ptr<float>() : nullptr;
+    c.a.h = h.data_ptr();
+    c.a.last = last.data_ptr<float>();
+    const int rc = c.run(g_more.scan_ws, g_more.scan, x->device());
+    if (rc) return py::int_(rc);
+    return py::make_tuple(wrap(h), wrap(last), keep ? wrap(states) : py::object(py::none()));
+}
+
+py::object rows_scan_backward(const py::object& gh_, const py::object& x_, const py::object& gate_, const py::object& states_,
+                              const py::object& glast_, bool blend, bool reverse) {
+    const at::Tensor *gh = floating(gh_), *x = floating(x_), *gate = floating(gate_), *states = floating(states_),
+                     *glast = glast_.is_none() ? nullptr : floating(glast_);
+    ScanCall c;
+    if (!c.set(x, gate, blend, reverse) || !gh || !like(*gh, *x) || !is_f32(states, c.many, x->device()) ||
+        (!glast_.is_none() && !is_f32(glast, c.one, x->device())))
+        return py::none();
+    const c10::cuda::CUDAGuard guard(x->device());
+    const at::Tensor gx = fresh_like(*x), ga = fresh_like(*x), gs = fresh(c.one, at::kFloat, x->device());
+    c.a.grad_h = gh->data_ptr();
+    c.a.states = states->data_ptr<float>();
+    c.a.grad_last = glast ? glast->data_ptr<float>() : nullptr;
+    c.a.grad_x = gx.data_ptr();
+    c.a.grad_gate = ga.data_ptr();
+    c.a.grad_state = gs.data_ptr<float>();
+    const int rc = c.run(g_more.scan_backward_ws, g_more.scan_backward, x->device());
+    if (rc) return py::int_(rc);
+    return py::make_tuple(wrap(gx), wrap(ga), wrap(gs));
+}
+
+bool set_scores(plattice_log_probs_args& a, const at::Tensor* x, const py::object& labels_) {
+    if (!rows_tensor(x) || x->size(-1) > (1 << 30)) return false;
+    a.logits = x->data_ptr();
+    a.dtype = dtype_code(x->scalar_type());
+    a.n = (int)x->size(-1);
+    a.rows = x->numel() / a.n;
+    if (labels_.is_none()) return true;
+    const at::Tensor* l = labels_of(labels_);
+    if (!l || l->sizes() != x->sizes().slice(0, x->dim() - 1) || l->device() != x->device()) return false;
+    a.labels = l->data_ptr();
+    a.labels_wide = wide(*l);
+    return true;
+}
+
+py::object rows_log_probs(const py::object& x_, const py::object& labels_, int64_t top) {
+    const at::Tensor* x = floating(x_);
+    plattice_log_probs_args a = {};
+    if (!set_scores(a, x, labels_) || top < 0 || top > a.n || top > PLATTICE_MAX_TOP) return py::none();
+    const c10::cuda::CUDAGuard guard(x->device());
+    const at::Device d = x->device();
+    c10::SmallVector<int64_t, 8> lead(x->sizes().begin(), x->sizes().end() - 1), more(lead);
+    at::Tensor logp, top_logp, top_ids;
+    const at::Tensor entropy = fresh(lead, at::kFloat, d), lse = fresh(lead, at::kFloat, d);
+    if (a.labels || !labels_.is_none()) {
+        logp = fresh(lead, at::kFloat, d);
+        a.logp = logp.data_ptr<float>();
+    }
+    more.push_back(2);
+    const at::Tensor stats = fresh(more, at::kFloat, d);
+    if (top) {
+        more.back() = top;
+        top_logp = fresh(more, at::kFloat, d);
+        top_ids = fresh(more, at::kLong, d);
+        a.top_logp = top_logp.data_ptr<float>();
+        a.top_ids = reinterpret_cast<long long*>(top_ids.data_ptr<int64_t>());
+    }
+    a.entropy = entropy.data_ptr<float>();
+    a.lse = lse.data_ptr<float>();
+    a.stats = stats.data_ptr<float>();
+    a.top = (int)top;
+    const int rc = g_more.log_probs(&a, stream_of(d));
+    if (rc) return py::int_(rc);
+    const py::object none = py::none();
+    return py::make_tuple(logp.defined() ? wrap(logp) : none, wrap(entropy), wrap(lse), wrap(stats), top ? wrap(top_logp) : none,
+                          top ? wrap(top_ids) : none);
+}
+
+py::object rows_log_probs_backward(const py::object& x_, const py::object& stats_, const py::object& entropy_,
+                                   const py::object& labels_, const py::object& gl_, const py::object& ge_, const py::object& gz_) {
+    const at::Tensor *x = floating(x_), *stats = floating(stats_);
+    plattice_log_probs_args a = {};
+    if (!set_scores(a, x, labels_)) return py::none();
+    const at::Device d = x->device();
+    c10::SmallVector<int64_t, 8> lead(x->sizes().begin(), x->sizes().end() - 1), two(lead);
+    two.push_back(2);
+    if (!is_f32(stats, two, d) || (!gl_.is_none() && labels_.is_none())) return py::none();
+    a.stats = stats->data_ptr<float>();
+    const auto part = [&](const py::object& o, const float*& to) {
+        if (o.is_none()) return true;
+        const at::Tensor* t = floating(o);
+        if (!is_f32(t, lead, d)) return false;
+        to = t->data_ptr<float>();
+        return true;
+    };
+    const float* entropy = nullptr;
+    if (!part(gl_, a.grad_logp) || !part(ge_, a.grad_entropy) || !part(gz_, a.grad_lse)) return py::none();
+    if (a.grad_entropy && (entropy_.is_none() || !part(entropy_, entropy))) return py::none();
+    a.entropy = const_cast<float*>(entropy);
+    const c10::cuda::CUDAGuard guard(d);
+    const at::Tensor grad = fresh_like(*x);
+    a.grad_logits = grad.data_ptr();
+    const int rc = g_more.log_probs_backward(&a, stream_of(d));
+    if (rc) return py::int_(rc);
+    return wrap(grad);
+}
+
+// out None: the norm alone.  norm None: the tensors' own.  `out` written in place
+// of what it held counts as changed for autograd.
+py::object clip_grads(const std::vector<py::object>& tensors, const py::object& out_, double max_norm, double eps,
+                      const py::object& norm_) {
+    if (tensors.empty() || tensors.size() > 0x7fffffff) return py::none();
+    c10::SmallVector<plattice_grad, 64> table(tensors.size());
+    std::vector<py::object> outs;
+    const at::Tensor* first = nullptr;
+    if (!out_.is_none()) {
+        if (!py::isinstance<py::list>(out_) || py::len(out_) != tensors.size()) return py::none();
+        outs = out_.cast<std::vector<py::object>>();
+    }
+    const bool grad_mode = at::GradMode::is_enabled();
+    for (size_t i = 0; i < tensors.size(); ++i) {
+        const at::Tensor* t = floating(tensors[i]);
+        if (!t) return py::none();
+        if (!first) first = t;
+        if (t->device() != first->device()) return py::none();
+        plattice_grad& g = table[i];
+        g = {t->data_ptr(), nullptr, t->numel(), dtype_code(t->scalar_type()), dtype_code(t->scalar_type())};
+        if (outs.empty()) continue;
+        const at::Tensor* o = floating(outs[i]);
+        if (!o || o->sizes() != t->sizes() || o->device() != t->device() ||
+            (o->scalar_type() != t->scalar_type() && o->scalar_type() != at::kFloat) || (grad_mode && o->requires_grad()))
+            return py::none();
+        g.out = o->data_ptr();
+        g.out_dtype = dtype_code(o->scalar_type());
+    }
+    const at::Device d = first->device();
+    const c10::cuda::CUDAGuard guard(d);
+    at::Tensor norm, ws;
+    size_t need = 0;
+    if (norm_.is_none()) {
+        norm = fresh({}, at::kFloat, d);
+        const int rc = g_more.clip_ws(table.data(), (int)table.size(), &need);
+        if (rc) return py::int_(rc);
+        ws = fresh({(int64_t)need}, at::kByte, d);
+    } else {
+        const at::Tensor* t = floating(norm_);
+        if (!is_f32(t, {}, d)) return py::none();
+        norm = *t;
+    }
+    const bool own = norm_.is_none();
+    const int rc = g_more.clip(table.data(), (int)table.size(), (float)max_norm, (float)eps, own ? nullptr : norm.data_ptr<float>(),
+                               own ? norm.data_ptr<float>() : nullptr, own ? ws.data_ptr() : nullptr, need, stream_of(d));
+    if (rc) return py::int_(rc);
+    for (const py::object& o : outs) {
+        const at::Tensor& t = THPVariable_Unpack(o.ptr());
+        if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    }
+    return own ? wrap(norm) : norm_;
+}
+
 }  // namespace
 
 void register_rows(py::module_& m) {
@@ -367,4 +652,12 @@ void register_rows(py::module_& m) {
     m.def("rows_rms_norm_backward", &rows_rms_norm_backward);
     m.def("rows_linear", &rows_linear);
     m.def("rows_linear_backward", &rows_linear_backward);
+    m.def("set_more_entry_points", &set_more_entry_points, "addresses of the operators below");
+    m.def("rows_embed", &rows_embed);
+    m.def("rows_embed_backward", &rows_embed_backward);
+    m.def("rows_scan", &rows_scan);
+    m.def("rows_scan_backward", &rows_scan_backward);
+    m.def("rows_log_probs", &rows_log_probs);
+    m.def("rows_log_probs_backward", &rows_log_probs_backward);
+    m.def("clip_grads", &clip_grads);
 }

@@ -16,9 +16,11 @@ import torch
 
 from . import _lib
 from .PLOO import _call, _check_input, _lib_h, _raise, _raw_stream, _require
-from .rows import _DTYPES, _check_like
+from .rows import _DTYPES, _check_like, _cpp
 
 __all__ = ["grad_norm", "clip_grads"]
+
+_SHARED = "(none may share memory with what is written)"
 
 
 def _listed(tensors, name):
@@ -50,7 +52,7 @@ def _run(tensors, out, max_norm, eps, norm_in):
                None if norm_in is None else norm_in.data_ptr(), None if norm_in is not None else norm.data_ptr(),
                None if ws is None else ws.data_ptr(), b.value, _raw_stream(dev.index))
     if rc:
-        _raise("plattice_clip_grads", rc, f"{len(tensors)} tensors (none may share memory with what is written)")
+        _raise("plattice_clip_grads", rc, f"{len(tensors)} tensors {_SHARED}")
     return norm
 
 
@@ -58,6 +60,13 @@ def grad_norm(tensors):
     """Norm of all values of ``tensors`` together: ``sqrt(sum g^2)``, a float32
     tensor without dimensions.  Squares that float32 does not hold are added in
     float64, sums of more than eight always."""
+    if not isinstance(tensors, (list, torch.Tensor)):
+        tensors = list(tensors)
+    cpp = _cpp()
+    if cpp is not None and type(tensors) is list and (got := cpp.clip_grads(tensors, None, 0.0, 0.0, None)) is not None:
+        if type(got) is int:
+            _raise("plattice_clip_grads", got, f"{len(tensors)} tensors")
+        return got
     return _run(_listed(tensors, "tensors"), None, 0.0, 0.0, None)
 
 
@@ -73,6 +82,17 @@ def clip_grads(tensors, max_norm, out=None, norm=None, eps=1e-6):
     (``out`` is then a copy).  A norm that is not finite scales by 0 or NaN, as
     the formula says.  What is written may share no memory with another tensor of
     either list, nor may a tensor that is scaled in place be listed twice."""
+    if not isinstance(tensors, (list, torch.Tensor)):
+        tensors = list(tensors)
+    if not isinstance(out, (list, torch.Tensor, type(None))):
+        out = list(out)
+    cpp = _cpp()
+    if (cpp is not None and type(tensors) is list and type(max_norm) in (float, int) and max_norm >= 0
+            and type(eps) in (float, int) and 0 <= eps < float("inf")
+            and (got := cpp.clip_grads(tensors, tensors if out is None else out, max_norm, eps, norm)) is not None):
+        if type(got) is int:
+            _raise("plattice_clip_grads", got, f"{len(tensors)} tensors {_SHARED}")
+        return got
     tensors = _listed(tensors, "tensors")
     _require(isinstance(max_norm, (int, float)) and max_norm >= 0, "max_norm must be a number, at least 0")
     _require(isinstance(eps, (int, float)) and 0 <= eps < float("inf"), "eps must be a finite number, at least 0")

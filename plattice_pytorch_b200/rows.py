@@ -125,6 +125,10 @@ _EXT = _UNSET
 _CALLS = ("plattice_rows_pack8", "plattice_rows_unpack8", "plattice_rms_norm",
           "plattice_rms_norm_backward_workspace_size", "plattice_rms_norm_backward", "plattice_linear_workspace_size",
           "plattice_linear", "plattice_linear_backward_workspace_size", "plattice_linear_backward")
+_MORE_CALLS = ("plattice_embed", "plattice_embed_backward_workspace_size", "plattice_embed_backward",
+               "plattice_scan_workspace_size", "plattice_scan", "plattice_scan_backward_workspace_size",
+               "plattice_scan_backward", "plattice_log_probs", "plattice_log_probs_backward",
+               "plattice_clip_grads_workspace_size", "plattice_clip_grads")
 
 
 def _cpp():
@@ -136,7 +140,9 @@ def _cpp():
     if _EXT is _UNSET:
         try:
             from . import _plattice_torch as m
-            m.set_rows_entry_points([ctypes.cast(getattr(_lib.lib(), n), ctypes.c_void_p).value for n in _CALLS])
+            at = lambda names: [ctypes.cast(getattr(_lib.lib(), n), ctypes.c_void_p).value for n in names]  # noqa: E731
+            m.set_rows_entry_points(at(_CALLS))
+            m.set_more_entry_points(at(_MORE_CALLS))
             _EXT = m
         except (ImportError, AttributeError):   # AttributeError: built before these calls
             _EXT = None
@@ -433,6 +439,11 @@ def embed(ids, table, scale=1.0):
     """Rows from labels: ``y [..., c] = scale * table[ids]`` in the type of
     ``table [n, c]`` (at most 2^21 channels), ``ids [...]`` int64 or int32.  A
     label outside ``0..n-1`` (the "ignored" of label maps) gives a row of zeros."""
+    cpp = _cpp()
+    if cpp is not None and type(scale) in (float, int) and (got := cpp.rows_embed(ids, table, scale)) is not None:
+        if type(got) is int:
+            _raise("plattice_embed", got, f"ids={tuple(ids.shape)} table={tuple(table.shape)}")
+        return got
     _check_input(table, "table")
     _require(table.dtype in _DTYPES, "table must be float32, bfloat16 or float16")
     _require(table.dim() == 2 and 1 <= table.shape[0] < 1 << 31 and 1 <= table.shape[1] <= _MAX_EMBED,
@@ -452,6 +463,12 @@ def embed_backward(grad_y, ids, n, scale=1.0, dtype=None):
     """Gradient of :func:`embed`'s table: ``[n, c]`` in ``dtype`` (default
     ``grad_y``'s), row v the sum of ``scale * grad_y`` over the places where
     ``ids`` is v.  Fewer than 2^31 ids."""
+    cpp = _cpp()
+    if (cpp is not None and type(scale) in (float, int) and type(n) is int and (dtype is None or dtype in _DTYPES) and 0 < n < 1 << 31
+            and (got := cpp.rows_embed_backward(grad_y, ids, n, scale, -1 if dtype is None else _DTYPES[dtype])) is not None):
+        if type(got) is int:
+            _raise("plattice_embed_backward", got, f"ids={tuple(ids.shape)} n={n} c={grad_y.shape[-1]}")
+        return got
     _check_rows(grad_y, "grad_y")
     c, dev = int(grad_y.shape[-1]), grad_y.device
     _require(c <= _MAX_EMBED, "grad_y must have at most 2^21 channels")
@@ -515,6 +532,11 @@ def scan(x, gate, state=None, blend=False, reverse=False, keep=False):
     taken from the last to the first.  The recurrence is held in float32, ``h`` is
     its rounding to the type of ``x``.  ``states``: with ``keep`` what
     :func:`scan_backward` needs, h before every 16th step in float32."""
+    cpp = _cpp()
+    if cpp is not None and (got := cpp.rows_scan(x, gate, state, bool(blend), bool(reverse), bool(keep))) is not None:
+        if type(got) is int:
+            _raise("plattice_scan", got, f"x={tuple(x.shape)}")
+        return got
     a, one, many, dev = _scan_common(x, gate, blend, reverse)
     if state is not None:
         _check_like(state, "state", one, torch.float32, dev)
@@ -532,6 +554,12 @@ def scan_backward(grad_h, x, gate, states, grad_last=None, blend=False, reverse=
     ``(grad_x, grad_gate, grad_state)``, the first two in the type of ``x``, the
     last ``[..., c]`` in float32.  ``grad_last`` (float32) is the gradient of
     ``last``, None for zeros."""
+    cpp = _cpp()
+    if (cpp is not None
+            and (got := cpp.rows_scan_backward(grad_h, x, gate, states, grad_last, bool(blend), bool(reverse))) is not None):
+        if type(got) is int:
+            _raise("plattice_scan_backward", got, f"x={tuple(x.shape)}")
+        return got
     a, one, many, dev = _scan_common(x, gate, blend, reverse)
     _check_like(grad_h, "grad_h", x.shape, x.dtype, dev)
     _check_like(states, "states", many, torch.float32, dev)
@@ -580,6 +608,11 @@ def log_probs(logits, labels=None, top=0):
     A score of -inf is a class that the row may not have; a row of nothing else
     has log probabilities of -inf and entropy 0.  NaN or +inf in a row make its
     numbers NaN (of the alternatives' classes NaN is the last choice)."""
+    cpp = _cpp()
+    if cpp is not None and type(top) is int and 0 <= top <= _MAX_TOP and (got := cpp.rows_log_probs(logits, labels, top)) is not None:
+        if type(got) is int:
+            _raise("plattice_log_probs", got, f"logits={tuple(logits.shape)} top={top}")
+        return LogProbs._make(got)
     a, lead, dev = _log_probs_common(logits, labels)
     _require(isinstance(top, int) and 0 <= top <= min(_MAX_TOP, a.n), f"top must be in [0, min(n, {_MAX_TOP})]")
     new = lambda *s, dtype=torch.float32: torch.empty(lead + s, dtype=dtype, device=dev)  # noqa: E731
@@ -598,6 +631,13 @@ def log_probs_backward(logits, result, labels=None, grad_logp=None, grad_entropy
     ``result``, the same ``labels`` and the gradients (float32 ``[...]``, None for
     zeros) of ``logp``, ``entropy`` and ``lse``.  The alternatives have none.  A row
     of -inf only has gradient 0."""
+    cpp = _cpp()
+    if (cpp is not None and type(result) is LogProbs
+            and (got := cpp.rows_log_probs_backward(logits, result.stats, result.entropy, labels, grad_logp, grad_entropy,
+                                                    grad_lse)) is not None):
+        if type(got) is int:
+            _raise("plattice_log_probs_backward", got, f"logits={tuple(logits.shape)}")
+        return got
     a, lead, dev = _log_probs_common(logits, labels)
     _require(isinstance(result, LogProbs), "result must be LogProbs")
     _check_like(result.stats, "result.stats", lead + (2,), torch.float32, dev)
