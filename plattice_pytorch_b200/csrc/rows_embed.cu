@@ -3,19 +3,22 @@
 //   y[i] = scale table[id_i]            (0 for an id outside the table)
 //   grad_table[v] = scale sum_{i: id_i = v} grad_y[i]
 //
-// The gradient sorts the positions by label (a stable radix sort, 8 bits of the
-// label a pass), cuts the sorted list into chunks of equal length and adds each
-// chunk's runs of equal labels in registers.  A run inside one chunk is written
-// at once; the parts of a run that crosses chunks go to the workspace and are
-// added in order by a second kernel.  No atomics: the order of the sums depends
-// on the sizes alone.
+// The gradient of a small table (up to kSmallTable labels) is added up in shared
+// memory as the rows come: every warp has a copy of 64 of the table's channels of
+// its own, CTAs' sums are added by a second kernel.  For a larger table the
+// positions are sorted by label (by counting smaller ones, or a stable radix sort,
+// 8 bits of the label a pass), the sorted list is cut into chunks of equal length
+// and each chunk's runs of equal labels are added in registers.  A run inside one
+// chunk is written at once; the parts of a run that crosses chunks go to the
+// workspace and are added in order by another kernel.  The order of the sums
+// depends on the sizes alone: no atomics but counts.
 #include "plattice_runtime.h"
 #include "rows_host.h"
 #include "rows_vec.cuh"
 
 namespace plr {
 
-constexpr int kEmbedUnits = 4;   // accesses a thread makes
+constexpr int kEmbedUnits = 8;   // accesses a thread makes
 
 template <typename T, int V>
 __global__ void __launch_bounds__(256) k_embed(T* __restrict__ y, Labels ids, const T* __restrict__ table, float scale,
@@ -46,12 +49,182 @@ __global__ void __launch_bounds__(256) k_embed(T* __restrict__ y, Labels ids, co
     }
 }
 
+// Stores V values as T, or as `dtype` says where that is another type.
+template <typename T, int V>
+__device__ __forceinline__ void store_out(void* out, int dtype, bool vec, int64_t at, const float (&v)[V]) {
+    if (vec) {
+        Vec<T, V> o;
+        o.from(v);
+        o.store(static_cast<T*>(out) + at);
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) store_param(out, dtype, at + j, v[j]);
+    }
+}
+
+// ----------------------------------------------------------------- small tables
+//
+// A warp goes through rows 32 labels at a time, 8 rows' gradients under way; a lane
+// adds V channels to the label's place in the warp's copy, which is its own place:
+// nothing else reads or writes it.  Where a row has fewer than 32 V channels,
+// several rows go side by side, each group of lanes with a copy.  Warps of a CTA
+// take slabs of 32 V channels first, then rows.  1048576 rows of 64 channels into
+// 21 labels: the sorted way took 210 us.
+
+constexpr int kSmallTable = 96, kTableBytes = 200 * 1024;
+
+struct TableArgs {
+    void* out;                // where one CTA has all rows, else null
+    int out_dtype;
+    float* part;              // [row CTAs][n][c]
+    Labels ids;
+    const void* g;
+    float scale;
+    int64_t count, n;
+    int c, lanes, slabs;      // lanes of a row; slabs of a CTA's warps (blockIdx.y has others)
+    int copies;               // warps a slab
+};
+
+template <typename T, int V, bool kWhole>
+__global__ void __launch_bounds__(1024) k_small_table(const __grid_constant__ TableArgs a) {
+    extern __shared__ float tables[];   // [warp][group][n][lanes V]
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    const int n = (int)a.n, width = a.lanes * V, groups = 32 / a.lanes, each = n * 32 * V;
+    for (int i = threadIdx.x; i < warps * each; i += blockDim.x) tables[i] = 0.f;
+    __syncthreads();
+    const int group = lane / a.lanes, own = lane % a.lanes;
+    const int slab = blockIdx.y * a.slabs + warp % a.slabs, copy = warp / a.slabs;
+    const int col = slab * width + own * V;
+    float* table = tables + warp * each + group * n * width + own * V;
+    const bool here = col < a.c;
+    const T* g = static_cast<const T*>(a.g) + col;
+    const int64_t blocks = (a.count + 31) / 32, step = (int64_t)gridDim.x * a.copies;
+    for (int64_t b = (int64_t)blockIdx.x * a.copies + copy; b < blocks; b += step) {
+        const int64_t row0 = b * 32;
+        const int id = row0 + lane < a.count ? a.ids.at(row0 + lane, a.n) : -1;
+        for (int r = 0; r < 32; r += 8 * groups) {
+            Vec<T, V> v[8];
+            int label[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int at = r + k * groups + group;
+                label[k] = __shfl_sync(0xffffffffu, id, at & 31);
+                if (at > 31 || !here) label[k] = -1;
+                v[k].zero();
+                if (label[k] >= 0) {
+                    const T* from = g + (row0 + at) * a.c;
+                    if constexpr (kWhole) {
+                        v[k].load(from);
+                    } else {
+                        float f[V];
+#pragma unroll
+                        for (int j = 0; j < V; ++j) f[j] = to_f32(from[j]);
+                        v[k].from(f);
+                    }
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (label[k] >= 0) {
+                    float* t = table + label[k] * width;
+#pragma unroll
+                    for (int j = 0; j < V; ++j) t[j] += v[k].at(j);
+                }
+        }
+    }
+    __syncthreads();
+    // The copies of a slab together, in order, for the CTA's channels.
+    const int64_t first = (int64_t)blockIdx.y * a.slabs * width;
+    const int wide = a.c - first < (int64_t)a.slabs * width ? (int)(a.c - first) : a.slabs * width;
+    for (int i = threadIdx.x; i < n * wide; i += blockDim.x) {
+        const int label = i / wide, at = i - label * wide, w = at / width, j = at - w * width;
+        float sum = 0.f;
+        for (int k = 0; k < a.copies; ++k)
+            for (int q = 0; q < groups; ++q) sum += tables[(k * a.slabs + w) * each + (q * n + label) * width + j];
+        const int64_t to = (int64_t)label * a.c + first + at;
+        if (a.out) store_param(a.out, a.out_dtype, to, sum * a.scale);
+        else a.part[(int64_t)blockIdx.x * n * a.c + to] = sum;
+    }
+}
+
+// out[i] = scale times the sum of part[k][i]: 8 groups of 32 threads, each every 8th part.
+__global__ void __launch_bounds__(256) k_small_join(void* out, int dtype, const float* __restrict__ part, int parts, int64_t cells,
+                                                    float scale) {
+    __shared__ float sums[8][32];
+    const int64_t i = (int64_t)blockIdx.x * 32 + threadIdx.x;
+    float s = 0.f;
+    if (i < cells) {
+#pragma unroll 8
+        for (int k = threadIdx.y; k < parts; k += 8) s += part[k * cells + i];
+    }
+    sums[threadIdx.y][threadIdx.x] = s;
+    __syncthreads();
+    if (threadIdx.y == 0 && i < cells) {
+#pragma unroll
+        for (int k = 1; k < 8; ++k) s += sums[k][threadIdx.x];
+        store_param(out, dtype, i, s * scale);
+    }
+}
+
 // --------------------------------------------------------------- sorting labels
 
-constexpr int kTile = 4096;        // entries that a CTA of the sort takes
 constexpr int kDigits = 256;
+constexpr int kRankSorted = 8192;   // as many are sorted by counting
 
 struct Entry { unsigned label, at; };   // at: the position in ids
+
+// A label's place: the labels below it and the equal ones before it.  A CTA has all
+// labels in shared memory and places 64; four threads share a label's comparisons.
+// 8192 labels are 67 M comparisons; the passes below are two launches a digit.
+__global__ void __launch_bounds__(256) k_rank_sort(Entry* __restrict__ out, unsigned* __restrict__ valid, Labels ids, int64_t n,
+                                                   int count) {
+    __shared__ uint4 labels[kRankSorted / 4];
+    __shared__ unsigned places[4][64], sums[8];
+    unsigned* flat = reinterpret_cast<unsigned*>(labels);
+    const int padded = (count + 15) / 16 * 16;
+    unsigned all = 0;
+#pragma unroll 8
+    for (int k = threadIdx.x; k < padded; k += 256) {
+        const unsigned v = k < count ? (unsigned)ids.at(k, n) : 0xffffffffu;   // none: behind all
+        flat[k] = v;
+        all += v != 0xffffffffu;
+    }
+    __syncthreads();
+    const int e = threadIdx.x & 63, i0 = blockIdx.x * 64, i = i0 + e, share = padded / 16;   // fours of a thread
+    const unsigned mine = i < count ? flat[i] : 0xffffffffu;
+    unsigned place = 0;
+    const int from = (threadIdx.x >> 6) * share, to = from + share;
+    // the fours before the CTA's own labels, those around them, those behind
+    const int low = i0 / 4 < from ? from : i0 / 4 < to ? i0 / 4 : to, high = i0 / 4 + 16 < low ? low : i0 / 4 + 16 < to ? i0 / 4 + 16 : to;
+    const unsigned next = mine + 1u;   // equal ones before count
+#pragma unroll 4
+    for (int k = from; k < low; ++k) {
+        const uint4 o = labels[k];
+        place += (o.x < next) + (o.y < next) + (o.z < next) + (o.w < next);
+    }
+    for (int k = low; k < high; ++k) {
+        const uint4 o = labels[k];
+        place += (o.x < mine + (4 * k < i)) + (o.y < mine + (4 * k + 1 < i)) + (o.z < mine + (4 * k + 2 < i)) +
+                 (o.w < mine + (4 * k + 3 < i));
+    }
+#pragma unroll 4
+    for (int k = high; k < to; ++k) {
+        const uint4 o = labels[k];
+        place += (o.x < mine) + (o.y < mine) + (o.z < mine) + (o.w < mine);
+    }
+    places[threadIdx.x >> 6][e] = place;
+    all = __reduce_add_sync(0xffffffffu, all);
+    if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = all;
+    __syncthreads();
+    if (threadIdx.x < 64 && mine != 0xffffffffu)
+        out[places[0][e] + places[1][e] + places[2][e] + places[3][e]] = Entry{mine, (unsigned)i};
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        all = 0;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) all += sums[w];
+        *valid = all;
+    }
+}
 
 // Entries of pass 0 come from the labels themselves (those outside the table
 // are left out), later ones from the pass before.
@@ -76,78 +249,94 @@ struct Source {
     }
 };
 
-// counts [digit][tile]
-__global__ void __launch_bounds__(256) k_sort_count(unsigned* __restrict__ counts, Source src, int shift, int tiles) {
+// counts [tile][digit]; a tile is kItems entries a thread.
+template <int kItems>
+__global__ void __launch_bounds__(256) k_sort_count(unsigned* __restrict__ counts, Source src, int shift) {
     __shared__ unsigned h[kDigits + 1];
     h[threadIdx.x] = 0;
     if (threadIdx.x == 0) h[kDigits] = 0;
     __syncthreads();
-    const int64_t size = src.size(), base = (int64_t)blockIdx.x * kTile;
-    for (int k = 0; k < kTile; k += 256) {
-        Entry e;
-        atomicAdd(&h[src.get(base + k + threadIdx.x, size, shift, e)], 1u);   // counts: any order
-    }
+    const int64_t size = src.size(), base = (int64_t)blockIdx.x * (256 * kItems);
+    Entry e[kItems];
+    int digit[kItems];
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) digit[k] = src.get(base + k * 256 + threadIdx.x, size, shift, e[k]);
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) atomicAdd(&h[digit[k]], 1u);   // counts: any order
     __syncthreads();
-    counts[(int64_t)threadIdx.x * tiles + blockIdx.x] = h[threadIdx.x];
+    counts[(int64_t)blockIdx.x * kDigits + threadIdx.x] = h[threadIdx.x];
 }
 
-// Exclusive sums of m counts by one CTA; the total goes to *valid.
-__global__ void __launch_bounds__(1024) k_sort_sums(unsigned* __restrict__ counts, int64_t m, unsigned* valid) {
-    __shared__ unsigned warps[32];
-    unsigned carry = 0;
+// Exclusive sum over the CTA's 256 threads.
+__device__ __forceinline__ unsigned before_me(unsigned v, unsigned& all) {
+    __shared__ unsigned warps[8];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int64_t base = 0; base < m; base += 1024 * 8) {
-        const int64_t at = base + (int64_t)threadIdx.x * 8;
-        unsigned v[8], sum = 0;
+    unsigned s = v;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            v[i] = at + i < m ? counts[at + i] : 0;
-            sum += v[i];
-        }
-        unsigned s = sum;
+    for (int d = 1; d < 32; d <<= 1) {
+        const unsigned t = __shfl_up_sync(0xffffffffu, s, d);
+        if (lane >= d) s += t;
+    }
+    if (lane == 31) warps[warp] = s;
+    __syncthreads();
+    unsigned o = 0;
+    all = 0;
 #pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const unsigned t = __shfl_up_sync(0xffffffffu, s, d);
-            if (lane >= d) s += t;
-        }
-        if (lane == 31) warps[warp] = s;
-        __syncthreads();
-        unsigned w = warps[lane];
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const unsigned t = __shfl_up_sync(0xffffffffu, w, d);
-            if (lane >= d) w += t;
-        }
-        const unsigned all = __shfl_sync(0xffffffffu, w, 31);
-        const unsigned before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);   // the lanes all take part
-        unsigned o = carry + (warp ? before : 0) + s - sum;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (at + i < m) counts[at + i] = o;
-            o += v[i];
-        }
+    for (int w = 0; w < 8; ++w) {
+        if (w < warp) o += warps[w];
+        all += warps[w];
+    }
+    return o + s - v;
+}
+
+// counts become the number of entries of the digit in the tiles before (many
+// tiles: a CTA a digit); totals [digit].
+__global__ void __launch_bounds__(256) k_sort_sums(unsigned* __restrict__ counts, unsigned* __restrict__ totals, int64_t tiles) {
+    unsigned carry = 0;
+    for (int64_t base = 0; base < tiles; base += 256) {
+        const int64_t t = base + threadIdx.x;
+        unsigned* at = counts + t * kDigits + blockIdx.x;
+        unsigned all;
+        const unsigned o = before_me(t < tiles ? *at : 0u, all);
+        if (t < tiles) *at = carry + o;
         carry += all;
         __syncthreads();
     }
-    if (threadIdx.x == 0) *valid = carry;
+    if (threadIdx.x == 0) totals[blockIdx.x] = carry;
 }
 
-// Stable: a warp takes 512 neighbouring entries of the tile, 32 at a time, and
-// counts equal digits before its own by a match.
-__global__ void __launch_bounds__(256) k_sort_place(Entry* __restrict__ out, const unsigned* __restrict__ offsets,
-                                                    Source src, int shift, int tiles) {
+// Stable: a warp takes neighbouring entries of the tile, 32 at a time, and counts
+// equal digits before its own by a match.  totals null: the tile adds up the
+// counts of all tiles itself.
+template <int kItems>
+__global__ void __launch_bounds__(256) k_sort_place(Entry* __restrict__ out, const unsigned* __restrict__ counts,
+                                                    const unsigned* __restrict__ totals, unsigned* __restrict__ valid, Source src,
+                                                    int shift, int tiles) {
     __shared__ unsigned h[8][kDigits + 1];
     for (int i = threadIdx.x; i < 8 * (kDigits + 1); i += 256) (&h[0][0])[i] = 0;
-    __syncthreads();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t size = src.size(), base = (int64_t)blockIdx.x * kTile + warp * 512;
-    Entry e[16];
-    int digit[16];
-    unsigned rank[16];
+    const int64_t size = src.size(), base = (int64_t)blockIdx.x * (256 * kItems) + warp * (32 * kItems);
+    Entry e[kItems];
+    int digit[kItems];
+    unsigned rank[kItems];
 #pragma unroll
-    for (int k = 0; k < 16; ++k) digit[k] = src.get(base + k * 32 + lane, size, shift, e[k]);
+    for (int k = 0; k < kItems; ++k) digit[k] = src.get(base + k * 32 + lane, size, shift, e[k]);
+    unsigned o = 0, total = 0, all;   // the digit threadIdx.x in the tiles before, and in all
+    if (totals) {
+        o = counts[(int64_t)blockIdx.x * kDigits + threadIdx.x];
+        total = totals[threadIdx.x];
+    } else {
+#pragma unroll 16
+        for (int t = 0; t < tiles; ++t) {
+            const unsigned v = counts[t * kDigits + threadIdx.x];
+            total += v;
+            if (t < (int)blockIdx.x) o += v;
+        }
+    }
+    o += before_me(total, all);   // all threads: h has been cleared behind it
+    if (blockIdx.x == 0 && threadIdx.x == 0) *valid = all;
 #pragma unroll
-    for (int k = 0; k < 16; ++k) {
+    for (int k = 0; k < kItems; ++k) {
         const unsigned same = __match_any_sync(0xffffffffu, digit[k]);
         const unsigned had = h[warp][digit[k]];
         rank[k] = had + __popc(same & ((1u << lane) - 1));
@@ -156,7 +345,6 @@ __global__ void __launch_bounds__(256) k_sort_place(Entry* __restrict__ out, con
         __syncwarp();
     }
     __syncthreads();
-    unsigned o = offsets[(int64_t)threadIdx.x * tiles + blockIdx.x];
 #pragma unroll
     for (int w = 0; w < 8; ++w) {
         const unsigned had = h[w][threadIdx.x];
@@ -165,7 +353,7 @@ __global__ void __launch_bounds__(256) k_sort_place(Entry* __restrict__ out, con
     }
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < 16; ++k)
+    for (int k = 0; k < kItems; ++k)
         if (digit[k] < kDigits) out[h[warp][digit[k]] + rank[k]] = e[k];
 }
 
@@ -180,11 +368,12 @@ struct RunArgs {
     const void* g;
     float scale;
     int c, length;            // length: entries of a chunk
+    bool vec, vec4;           // rows of out, of part: whole accesses
 };
 
 // A thread's V channels of the entries of one chunk.  blockDim: (lanes of a row, chunks of a CTA).
 template <typename T, int V>
-__global__ void __launch_bounds__(256) k_runs(RunArgs a) {
+__global__ void __launch_bounds__(256) k_runs(const __grid_constant__ RunArgs a) {
     const int64_t valid = *a.valid;
     const int64_t chunk = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
     const int64_t begin = chunk * a.length;
@@ -194,18 +383,18 @@ __global__ void __launch_bounds__(256) k_runs(RunArgs a) {
     const T* g = static_cast<const T*>(a.g) + col;
     unsigned label = a.sorted[begin].label;
     bool head = begin > 0 && a.sorted[begin - 1].label == label;
+    const bool tail_at_end = end < valid && a.sorted[end].label == a.sorted[end - 1].label;
     float acc[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) acc[j] = 0.f;
     const auto out = [&](bool tail) {
         if (head || tail) {
-            float* p = a.part + (chunk * 2 + (head ? 0 : 1)) * a.c + col;
-#pragma unroll
-            for (int j = 0; j < V; ++j) p[j] = acc[j];
+            store_out<float, V>(a.part, PLATTICE_F32, a.vec4, (chunk * 2 + (head ? 0 : 1)) * a.c + col, acc);
         } else {
+            float v[V];
 #pragma unroll
-            for (int j = 0; j < V; ++j)
-                store_param(a.out, a.out_dtype, (int64_t)label * a.c + col + j, acc[j] * a.scale);
+            for (int j = 0; j < V; ++j) v[j] = acc[j] * a.scale;
+            store_out<T, V>(a.out, a.out_dtype, a.vec, (int64_t)label * a.c + col, v);
         }
     };
     for (int64_t i = begin; i < end; i += 8) {
@@ -213,13 +402,12 @@ __global__ void __launch_bounds__(256) k_runs(RunArgs a) {
         Vec<T, V> v[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            e[k].label = label;
             if (i + k < end) {
                 e[k] = a.sorted[i + k];
                 v[k].load(g + (int64_t)e[k].at * a.c);
             } else {
                 v[k].zero();
-                if (k) e[k].label = e[k - 1].label;
+                e[k].label = e[k - 1 < 0 ? 0 : k - 1].label;   // i < end: k is above 0
             }
         }
 #pragma unroll
@@ -235,20 +423,21 @@ __global__ void __launch_bounds__(256) k_runs(RunArgs a) {
             for (int j = 0; j < V; ++j) acc[j] += v[k].at(j);
         }
     }
-    out(end < valid && a.sorted[end].label == label);
+    out(tail_at_end);
 }
 
 // The runs that begin in a chunk and go on behind it: its part and those of the
-// chunks up to the run's end, which a search of the sorted list finds.
-// blockDim (32 channels, 8): each of the 8 adds every 8th part, then they are
-// added in order.
-__global__ void __launch_bounds__(256) k_join_runs(RunArgs a) {
-    __shared__ float sums[8][32];
+// chunks up to the run's end, which a search of the sorted list finds.  A CTA a
+// chunk, most have none; `lanes` threads of V channels side by side, the others take
+// every 256 / lanes-th part, and theirs are added in order.
+template <int V>
+__global__ void __launch_bounds__(256) k_join_runs(const __grid_constant__ RunArgs a, int lanes) {
+    __shared__ float sums[256 * V];
     const int64_t valid = *a.valid, chunk = blockIdx.x, end = (chunk + 1) * a.length;
     if (end >= valid) return;
     const unsigned label = a.sorted[end].label;
-    if (a.sorted[end - 1].label != label) return;
     const int64_t begin = chunk * a.length;
+    if (a.sorted[end - 1].label != label) return;
     if (a.sorted[begin].label == label && begin > 0 && a.sorted[begin - 1].label == label) return;   // began earlier
     int64_t lo = end, hi = valid;   // the run ends at the first entry of another label: lo < it <= hi
     while (hi - lo > 1) {
@@ -257,18 +446,43 @@ __global__ void __launch_bounds__(256) k_join_runs(RunArgs a) {
         else hi = mid;
     }
     const int64_t parts = (lo / a.length) - chunk;   // chunks behind this one
-    const int64_t col = (int64_t)blockIdx.y * 32 + threadIdx.x;
-    float s = 0.f;
-    if (col < a.c) {
-        if (threadIdx.y == 0) s = a.part[(chunk * 2 + 1) * a.c + col];
-        for (int64_t j = 1 + threadIdx.y; j <= parts; j += 8) s += a.part[(chunk + j) * 2 * a.c + col];
-    }
-    sums[threadIdx.y][threadIdx.x] = s;
-    __syncthreads();
-    if (threadIdx.y == 0 && col < a.c) {
+    const int lane = threadIdx.x % lanes, group = threadIdx.x / lanes, groups = 256 / lanes;
+    for (int64_t first = 0; first < a.c; first += (int64_t)lanes * V) {
+        const int64_t col = first + lane * V;
+        float s[V];
 #pragma unroll
-        for (int k = 1; k < 8; ++k) s += sums[k][threadIdx.x];
-        store_param(a.out, a.out_dtype, (int64_t)label * a.c + col, s * a.scale);
+        for (int j = 0; j < V; ++j) s[j] = 0.f;
+        if (col < a.c) {
+            if (group == 0) {
+                Vec<float, V> v;
+                v.load(a.part + (chunk * 2 + 1) * a.c + col);
+#pragma unroll
+                for (int j = 0; j < V; ++j) s[j] = v.at(j);
+            }
+            for (int64_t k = 1 + group; k <= parts; k += 8 * groups) {
+                Vec<float, V> v[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    v[u].zero();
+                    if (k + u * groups <= parts) v[u].load(a.part + (chunk + k + u * groups) * 2 * a.c + col);
+                }
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+#pragma unroll
+                    for (int j = 0; j < V; ++j) s[j] += v[u].at(j);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) sums[threadIdx.x * V + j] = s[j];
+        __syncthreads();
+        if (group == 0 && col < a.c) {
+            for (int k = 1; k < groups; ++k)
+#pragma unroll
+                for (int j = 0; j < V; ++j) s[j] += sums[(k * lanes + lane) * V + j];
+#pragma unroll
+            for (int j = 0; j < V; ++j) store_param(a.out, a.out_dtype, (int64_t)label * a.c + col + j, s[j] * a.scale);
+        }
+        __syncthreads();
     }
 }
 
@@ -277,21 +491,46 @@ __global__ void __launch_bounds__(256) k_join_runs(RunArgs a) {
 static int64_t align256(int64_t b) { return (b + 255) / 256 * 256; }
 
 struct EmbedPlan {
-    int passes, tiles, length;
+    bool small;
+    int v, lanes, slabs, warps, ctas, ctas_y;   // small table
+    int passes, items, tiles, length;            // sorted; passes 0: by counting
     int64_t chunks;
-    int64_t valid, counts, first, second, part, bytes;   // offsets in the workspace
+    int64_t valid, totals, counts, first, second, part, bytes;   // offsets in the workspace
 };
+
+constexpr int kOwnSums = 256;   // tiles up to which the tiles add up the counts themselves
 
 static EmbedPlan embed_plan(int64_t count, int64_t n, int c) {
     EmbedPlan p = {};
-    while (p.passes < 4 && (n - 1) >> (8 * p.passes)) ++p.passes;
-    if (p.passes == 0) p.passes = 1;
-    p.tiles = (int)ceil_div(count, kTile);
+    p.small = n <= kSmallTable;
+    if (p.small) {
+        p.v = c % 2 == 0 ? 2 : 1;
+        const int units = c / p.v;
+        p.lanes = 1;
+        while (p.lanes < 32 && p.lanes < units) p.lanes <<= 1;
+        const int all = (int)ceil_div(units, p.lanes), fit = (int)(kTableBytes / (n * 32 * p.v * 4));
+        p.warps = fit < 32 ? fit : 32;
+        p.slabs = all < p.warps ? all : p.warps;
+        p.warps = p.warps / p.slabs * p.slabs;
+        p.ctas_y = (int)ceil_div(all, p.slabs);
+        const int copies = p.warps / p.slabs;
+        // each warp has some blocks of 32 rows, so that its table's way in and out is worth it
+        const int64_t need = ceil_div(count, 32 * 4 * (int64_t)copies), most = p.ctas_y < 148 ? 148 / p.ctas_y : 1;
+        p.ctas = (int)(need < most ? need : most);
+        p.bytes = p.ctas > 1 ? (int64_t)p.ctas * n * c * 4 : 0;
+        return p;
+    }
+    if (count > kRankSorted) {
+        while ((n - 1) >> (8 * p.passes)) ++p.passes;
+        p.items = count <= 262144 ? 4 : 16;
+        p.tiles = (int)ceil_div(count, 256 * p.items);
+    }
     // chunks long enough that few runs cross them, short enough that they fill the device
     const int64_t want = count * ceil_div(c, 8) / (148 * 2048);
     p.length = (int)(want < 16 ? 16 : want > 256 ? 256 : (want + 7) / 8 * 8);
     p.chunks = ceil_div(count, p.length);
-    int64_t at = 256;   // the number of valid entries is in front
+    p.totals = 256;   // the number of valid entries is in front
+    int64_t at = p.totals + kDigits * 4;
     p.counts = at;
     at += align256((int64_t)kDigits * p.tiles * 4);
     p.first = at;
@@ -302,6 +541,55 @@ static EmbedPlan embed_plan(int64_t count, int64_t n, int c) {
     at += align256(p.chunks * 2 * (int64_t)c * 4);
     p.bytes = at;
     return p;
+}
+
+template <typename T, int V, bool kWhole>
+static cudaError_t launch_small(const TableArgs& a, const EmbedPlan& p, cudaStream_t s) {
+    int unused = 0;
+    const cudaError_t e = pl::kernel_once(
+        reinterpret_cast<const void*>(k_small_table<T, V, kWhole>),
+        [](int*) {
+            return cudaFuncSetAttribute(k_small_table<T, V, kWhole>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTableBytes);
+        },
+        &unused);
+    if (e != cudaSuccess) return e;
+    k_small_table<T, V, kWhole><<<dim3(p.ctas, p.ctas_y), p.warps * 32, (size_t)p.warps * a.n * 32 * V * 4, s>>>(a);
+    return cudaGetLastError();
+}
+
+template <typename T>
+static cudaError_t small_table(const TableArgs& a, const EmbedPlan& p, cudaStream_t s) {
+    if (p.v == 1) return launch_small<T, 1, true>(a, p, s);
+    return (uintptr_t)a.g % (2 * sizeof(T)) ? launch_small<T, 2, false>(a, p, s) : launch_small<T, 2, true>(a, p, s);
+}
+
+template <int kItems>
+static void sort_pass(Entry* to, unsigned* counts, unsigned* totals, unsigned* valid, const Source& src, int shift, int tiles,
+                      cudaStream_t s) {
+    k_sort_count<kItems><<<tiles, 256, 0, s>>>(counts, src, shift);
+    const bool own = tiles <= kOwnSums;
+    if (!own) k_sort_sums<<<kDigits, 256, 0, s>>>(counts, totals, tiles);
+    k_sort_place<kItems><<<tiles, 256, 0, s>>>(to, counts, own ? nullptr : totals, valid, src, shift, tiles);
+}
+
+// The labels in order with their positions.
+static const Entry* sort_labels(const EmbedPlan& p, uint8_t* ws, const Labels& ids, int64_t count, int64_t n, cudaStream_t s) {
+    unsigned *valid = reinterpret_cast<unsigned*>(ws), *totals = reinterpret_cast<unsigned*>(ws + p.totals),
+             *counts = reinterpret_cast<unsigned*>(ws + p.counts);
+    Entry *to = reinterpret_cast<Entry*>(ws + p.first), *other = reinterpret_cast<Entry*>(ws + p.second), *from = nullptr;
+    if (p.passes == 0) {
+        k_rank_sort<<<(unsigned)ceil_div(count, 64), 256, 0, s>>>(to, valid, ids, n, (int)count);
+        return to;
+    }
+    for (int pass = 0; pass < p.passes; ++pass) {
+        const Source src{ids, n, count, from, valid};
+        if (p.items == 4) sort_pass<4>(to, counts, totals, valid, src, 8 * pass, p.tiles, s);
+        else sort_pass<16>(to, counts, totals, valid, src, 8 * pass, p.tiles, s);
+        from = to;
+        to = other;
+        other = from;
+    }
+    return from;
 }
 
 template <typename T, int V>
@@ -343,6 +631,15 @@ static cudaError_t launch_runs(int v, const RunArgs& a, int64_t chunks, cudaStre
     return launch_runs<T, 1>(a, chunks, s);
 }
 
+static cudaError_t join_runs(const RunArgs& a, int64_t chunks, cudaStream_t s) {
+    const bool four = a.c % 4 == 0;
+    int lanes = 1;
+    while (lanes < 256 && lanes < a.c / (four ? 4 : 1)) lanes <<= 1;
+    if (four) k_join_runs<4><<<(unsigned)(chunks - 1), 256, 0, s>>>(a, lanes);
+    else k_join_runs<1><<<(unsigned)(chunks - 1), 256, 0, s>>>(a, lanes);
+    return cudaGetLastError();
+}
+
 static bool embed_ok(long long count, long long n, int c) {
     return count >= 0 && n >= 1 && n <= 0x7fffffff && c >= 1 && c <= (1 << 21) && fits(count, c) && fits(n, c);
 }
@@ -381,35 +678,36 @@ int plattice_embed_backward(void* grad_table, int table_dtype, const void* grad_
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (count && (!grad_y || !ids || (uintptr_t)ids % (ids_wide ? 8 : 4))) return PLATTICE_ERR_INVALID;
     const EmbedPlan p = embed_plan(count, n, c);
-    if (count && (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < (size_t)p.bytes))
+    if (count && p.bytes && (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < (size_t)p.bytes))
         return PLATTICE_ERR_WORKSPACE;
-    cudaError_t e = cudaMemsetAsync(grad_table, 0, (size_t)n * c * dtype_size(table_dtype), s);
-    if (count == 0 || e != cudaSuccess) return rows_status(e, "plattice_embed_backward");
+    const Labels labels{ids, ids_wide};
     uint8_t* ws = static_cast<uint8_t*>(workspace);
-    unsigned* valid = reinterpret_cast<unsigned*>(ws);
-    unsigned* counts = reinterpret_cast<unsigned*>(ws + p.counts);
-    Entry *from = nullptr, *to = reinterpret_cast<Entry*>(ws + p.first),
-          *other = reinterpret_cast<Entry*>(ws + p.second);
-    for (int pass = 0; pass < p.passes; ++pass) {
-        const Source src{{ids, ids_wide}, n, count, from, valid};
-        k_sort_count<<<p.tiles, 256, 0, s>>>(counts, src, 8 * pass, p.tiles);
-        k_sort_sums<<<1, 1024, 0, s>>>(counts, (int64_t)kDigits * p.tiles, valid);
-        k_sort_place<<<p.tiles, 256, 0, s>>>(to, counts, src, 8 * pass, p.tiles);
-        from = to;
-        to = other;
-        other = from;
+    cudaError_t e = cudaSuccess;
+    if (count && p.small) {
+        const TableArgs a{p.ctas > 1 ? nullptr : grad_table, table_dtype, reinterpret_cast<float*>(ws), labels, grad_y, scale, count, n, c,
+                          p.lanes, p.slabs, p.warps / p.slabs};
+        e = dtype == PLATTICE_F32    ? small_table<float>(a, p, s)
+            : dtype == PLATTICE_BF16 ? small_table<__nv_bfloat16>(a, p, s)
+                                     : small_table<__half>(a, p, s);
+        if (e == cudaSuccess && p.ctas > 1) {
+            k_small_join<<<(unsigned)ceil_div(n * c, 32), dim3(32, 8), 0, s>>>(grad_table, table_dtype, a.part, p.ctas, n * c, scale);
+            e = cudaGetLastError();
+        }
+        return rows_status(e, "plattice_embed_backward");
     }
+    e = cudaMemsetAsync(grad_table, 0, (size_t)n * c * dtype_size(table_dtype), s);
+    if (count == 0 || e != cudaSuccess) return rows_status(e, "plattice_embed_backward");
+    const Entry* sorted = sort_labels(p, ws, labels, count, n, s);
     e = cudaGetLastError();
     if (e != cudaSuccess) return rows_status(e, "plattice_embed_backward");
-    const RunArgs a{grad_table, table_dtype, reinterpret_cast<float*>(ws + p.part), from, valid, grad_y, scale, c, p.length};
     const int v = widest(c, dtype_size(dtype), (uintptr_t)grad_y);
+    const RunArgs a{grad_table, table_dtype, reinterpret_cast<float*>(ws + p.part), sorted, reinterpret_cast<unsigned*>(ws), grad_y, scale,
+                    c, p.length, table_dtype == dtype && widest(c, dtype_size(dtype), (uintptr_t)grad_table) >= v,
+                    v * (int)sizeof(float) <= 16 ? c % v == 0 : c % 4 == 0};
     e = dtype == PLATTICE_F32    ? launch_runs<float>(v, a, p.chunks, s)
         : dtype == PLATTICE_BF16 ? launch_runs<__nv_bfloat16>(v, a, p.chunks, s)
                                  : launch_runs<__half>(v, a, p.chunks, s);
-    if (e == cudaSuccess && p.chunks > 1) {
-        k_join_runs<<<dim3((unsigned)(p.chunks - 1), (unsigned)ceil_div(c, 32)), dim3(32, 8), 0, s>>>(a);
-        e = cudaGetLastError();
-    }
+    if (e == cudaSuccess && p.chunks > 1) e = join_runs(a, p.chunks, s);
     return rows_status(e, "plattice_embed_backward");
 }
 

@@ -71,7 +71,8 @@ def test_embed_of_nonfinite_rows(dev, R):
 
 EMBED_SIZES = [((1,), 1, 1), ((7,), 5, 3), ((13, 29), 21, 50), ((100,), 1000, 64), ((3, 5, 2), 4, 1030), ((4097,), 33, 8),
                ((9000,), 3, 8), ((20000,), 257, 24), ((5000,), 70000, 16), ((2,), 3, 4096), ((0,), 3, 8), ((40000,), 1, 17),
-               ((70000,), 21, 64), ((300,), 256, 2048)]
+               ((70000,), 21, 64), ((300,), 256, 2048), ((8192,), 97, 2), ((8193,), 300, 4), ((300000,), 96, 6),
+               ((500,), 12, 5000), ((300000,), 200000, 1), ((1200000,), 1000, 1)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
