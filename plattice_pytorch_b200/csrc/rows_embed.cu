@@ -4,7 +4,7 @@
 //   grad_table[v] = scale sum_{i: id_i = v} grad_y[i]
 //
 // The gradient of a small table (up to kSmallTable labels) is added up in shared
-// memory as the rows come: every warp has a copy of 64 of the table's channels of
+// memory as the rows come: every warp has a copy of some of the table's channels of
 // its own, CTAs' sums are added by a second kernel.  For a larger table the
 // positions are sorted by label (by counting smaller ones, or a stable radix sort,
 // 8 bits of the label a pass), the sorted list is cut into chunks of equal length
@@ -18,34 +18,36 @@
 
 namespace plr {
 
-constexpr int kEmbedUnits = 8;   // accesses a thread makes
+// `lanes` (a power of two) threads a row side by side, four rows a thread, so that
+// labels, table rows and stores of four are under way together.
+constexpr int kEmbedRows = 4;
 
 template <typename T, int V>
-__global__ void __launch_bounds__(256) k_embed(T* __restrict__ y, Labels ids, const T* __restrict__ table, float scale,
-                                               int64_t all, int64_t n, unsigned units) {
-    const int64_t base = (int64_t)blockIdx.x * (256 * kEmbedUnits);
-    const GroupAt where(base, units);
-    Vec<T, V> v[kEmbedUnits];
+__global__ void __launch_bounds__(256) k_embed(T* __restrict__ y, Labels ids, const T* __restrict__ table, float scale, int64_t count,
+                                               int64_t n, int units, int shift) {
+    const int lane = threadIdx.x & ((1 << shift) - 1), step = 256 >> shift;
+    const int64_t row0 = (int64_t)blockIdx.x * (step * kEmbedRows) + (threadIdx.x >> shift);
+    int id[kEmbedRows];
 #pragma unroll
-    for (int u = 0; u < kEmbedUnits; ++u) {
-        const unsigned o = u * 256 + threadIdx.x;
-        v[u].zero();
-        if (base + o < all) {
-            int64_t row;
-            unsigned g;
-            where.at(o, row, g);
-            const int id = ids.at(row, n);
-            if (id >= 0) v[u].load(table + ((int64_t)id * units + g) * V);
+    for (int u = 0; u < kEmbedRows; ++u) id[u] = row0 + u * step < count ? ids.at(row0 + u * step, n) : -1;
+    for (int col = lane; col < units; col += 1 << shift) {
+        Vec<T, V> v[kEmbedRows];
+#pragma unroll
+        for (int u = 0; u < kEmbedRows; ++u) {
+            v[u].zero();
+            if (id[u] >= 0) v[u].load(table + ((int64_t)id[u] * units + col) * V);
         }
-    }
+        T* to = y + (row0 * units + col) * V;
+        const int64_t next = (int64_t)step * units * V;
 #pragma unroll
-    for (int u = 0; u < kEmbedUnits; ++u) {
-        const unsigned o = u * 256 + threadIdx.x;
-        float f[V];
+        for (int u = 0; u < kEmbedRows; ++u, to += next)
+            if (row0 + u * step < count) {
+                float f[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) f[i] = v[u].at(i) * scale;
-        v[u].from(f);
-        if (base + o < all) v[u].store(y + (base + o) * V);
+                for (int i = 0; i < V; ++i) f[i] = v[u].at(i) * scale;
+                v[u].from(f);
+                v[u].store(to);
+            }
     }
 }
 
@@ -68,10 +70,11 @@ __device__ __forceinline__ void store_out(void* out, int dtype, bool vec, int64_
 // adds V channels to the label's place in the warp's copy, which is its own place:
 // nothing else reads or writes it.  Where a row has fewer than 32 V channels,
 // several rows go side by side, each group of lanes with a copy.  Warps of a CTA
-// take slabs of 32 V channels first, then rows.  1048576 rows of 64 channels into
+// take slabs of 32 V channels first, then rows.  Four channels a lane where 16 warps'
+// copies of them fit (half the instructions a row), else two.  1048576 rows of 64 channels into
 // 21 labels: the sorted way took 210 us.
 
-constexpr int kSmallTable = 96, kTableBytes = 200 * 1024;
+constexpr int kSmallTable = 96, kWideTable = 24, kTableBytes = 200 * 1024;
 
 struct TableArgs {
     void* out;                // where one CTA has all rows, else null
@@ -86,8 +89,10 @@ struct TableArgs {
 };
 
 template <typename T, int V, bool kWhole>
-__global__ void __launch_bounds__(1024) k_small_table(const __grid_constant__ TableArgs a) {
-    extern __shared__ float tables[];   // [warp][group][n][lanes V]
+__global__ void __launch_bounds__(V == 4 ? 640 : 1024) k_small_table(const __grid_constant__ TableArgs a) {
+    constexpr int kTableRows = sizeof(T) * V > 4 * (V == 4 ? 2 : 1) ? 4 : 8;   // as registers allow
+    extern __shared__ float4 memory[];   // [warp][group][n][lanes V]
+    float* tables = reinterpret_cast<float*>(memory);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     const int n = (int)a.n, width = a.lanes * V, groups = 32 / a.lanes, each = n * 32 * V;
     for (int i = threadIdx.x; i < warps * each; i += blockDim.x) tables[i] = 0.f;
@@ -97,40 +102,67 @@ __global__ void __launch_bounds__(1024) k_small_table(const __grid_constant__ Ta
     const int col = slab * width + own * V;
     float* table = tables + warp * each + group * n * width + own * V;
     const bool here = col < a.c;
-    const T* g = static_cast<const T*>(a.g) + col;
     const int64_t blocks = (a.count + 31) / 32, step = (int64_t)gridDim.x * a.copies;
-    for (int64_t b = (int64_t)blockIdx.x * a.copies + copy; b < blocks; b += step) {
-        const int64_t row0 = b * 32;
-        const int id = row0 + lane < a.count ? a.ids.at(row0 + lane, a.n) : -1;
-        for (int r = 0; r < 32; r += 8 * groups) {
-            Vec<T, V> v[8];
-            int label[8];
+    const auto labels_at = [&](int64_t b) {
+        return b < blocks && b * 32 + lane < a.count ? a.ids.at(b * 32 + lane, a.n) : -1;
+    };
+    struct Rows {
+        Vec<T, V> v[kTableRows];
+        int label[kTableRows];
+    };
+    const int64_t c = a.c, apart = c * groups;
+    const T* g = static_cast<const T*>(a.g) + group * c + col;
+    int64_t b = (int64_t)blockIdx.x * a.copies + copy;
+    int r = 0, id = labels_at(b), id_next = labels_at(b + step);
+    const auto load = [&](Rows& q) {   // rows r.. of block b, whose labels the lanes have; then on to the next
+        const T* from = g + (b * 32 + r) * c;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const int at = r + k * groups + group;
-                label[k] = __shfl_sync(0xffffffffu, id, at & 31);
-                if (at > 31 || !here) label[k] = -1;
-                v[k].zero();
-                if (label[k] >= 0) {
-                    const T* from = g + (row0 + at) * a.c;
-                    if constexpr (kWhole) {
-                        v[k].load(from);
-                    } else {
-                        float f[V];
+        for (int k = 0; k < kTableRows; ++k, from += apart) {
+            const int at = r + k * groups + group, label = __shfl_sync(0xffffffffu, id, at & 31);
+            const bool some = label >= 0 && at < 32 && here;
+            q.label[k] = some ? label : 0;   // a row without a label adds 0 to the first: no branch
+            q.v[k].zero();
+            if (some) {
+                if constexpr (kWhole) {
+                    q.v[k].load(from);
+                } else {
+                    float f[V];
 #pragma unroll
-                        for (int j = 0; j < V; ++j) f[j] = to_f32(from[j]);
-                        v[k].from(f);
-                    }
+                    for (int j = 0; j < V; ++j) f[j] = to_f32(from[j]);
+                    q.v[k].from(f);
                 }
             }
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (label[k] >= 0) {
-                    float* t = table + label[k] * width;
-#pragma unroll
-                    for (int j = 0; j < V; ++j) t[j] += v[k].at(j);
-                }
         }
+        r += kTableRows * groups;
+        if (r >= 32) {
+            r = 0;
+            b += step;
+            id = id_next;
+            id_next = labels_at(b + step);
+        }
+    };
+    const auto add = [&](const Rows& q) {
+#pragma unroll
+        for (int k = 0; k < kTableRows; ++k) {
+            Vec<float, V>* at = reinterpret_cast<Vec<float, V>*>(table + q.label[k] * width);
+            Vec<float, V> t = *at;
+            float f[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) f[j] = t.at(j) + q.v[k].at(j);
+            t.from(f);
+            *at = t;
+        }
+    };
+    Rows odd, even;   // one under way while the other is added
+    load(even);
+    for (bool more = true; more;) {
+        more = b < blocks;
+        load(odd);
+        add(even);
+        if (!more) break;
+        more = b < blocks;
+        load(even);
+        add(odd);
     }
     __syncthreads();
     // The copies of a slab together, in order, for the CTA's channels.
@@ -173,11 +205,26 @@ constexpr int kRankSorted = 8192;   // as many are sorted by counting
 
 struct Entry { unsigned label, at; };   // at: the position in ids
 
+// The table's rows that no label has are 0: all of it is written first, in shares
+// by CTAs that the sort's launches have behind their own (a memory-bound write
+// beside launches that wait for latencies; 16384 labels of a 50000 x 1024 table).
+struct Zeros {
+    uint4* p;
+    int64_t begin, end;   // of this launch, in 16 bytes
+    int ctas;
+    __device__ __forceinline__ void share(int cta) const {
+        const int64_t each = (end - begin + ctas - 1) / ctas, from = begin + cta * each, to = from + each < end ? from + each : end;
+#pragma unroll 4
+        for (int64_t i = from + threadIdx.x; i < to; i += 256) p[i] = make_uint4(0, 0, 0, 0);
+    }
+};
+
 // A label's place: the labels below it and the equal ones before it.  A CTA has all
 // labels in shared memory and places 64; four threads share a label's comparisons.
 // 8192 labels are 67 M comparisons; the passes below are two launches a digit.
-__global__ void __launch_bounds__(256) k_rank_sort(Entry* __restrict__ out, unsigned* __restrict__ valid, Labels ids, int64_t n,
-                                                   int count) {
+__global__ void __launch_bounds__(256) k_rank_sort(Entry* __restrict__ out, unsigned* __restrict__ valid, unsigned* __restrict__ starts, Labels ids, int64_t n,
+                                                   int count, Zeros zeros) {
+    if ((int)blockIdx.x * 64 >= count) return zeros.share(blockIdx.x - (count + 63) / 64);
     __shared__ uint4 labels[kRankSorted / 4];
     __shared__ unsigned places[4][64], sums[8];
     unsigned* flat = reinterpret_cast<unsigned*>(labels);
@@ -223,6 +270,7 @@ __global__ void __launch_bounds__(256) k_rank_sort(Entry* __restrict__ out, unsi
 #pragma unroll
         for (int w = 0; w < 8; ++w) all += sums[w];
         *valid = all;
+        *starts = 0;
     }
 }
 
@@ -251,7 +299,8 @@ struct Source {
 
 // counts [tile][digit]; a tile is kItems entries a thread.
 template <int kItems>
-__global__ void __launch_bounds__(256) k_sort_count(unsigned* __restrict__ counts, Source src, int shift) {
+__global__ void __launch_bounds__(256) k_sort_count(unsigned* __restrict__ counts, Source src, int shift, int tiles, Zeros zeros) {
+    if ((int)blockIdx.x >= tiles) return zeros.share(blockIdx.x - tiles);
     __shared__ unsigned h[kDigits + 1];
     h[threadIdx.x] = 0;
     if (threadIdx.x == 0) h[kDigits] = 0;
@@ -310,8 +359,10 @@ __global__ void __launch_bounds__(256) k_sort_sums(unsigned* __restrict__ counts
 // counts of all tiles itself.
 template <int kItems>
 __global__ void __launch_bounds__(256) k_sort_place(Entry* __restrict__ out, const unsigned* __restrict__ counts,
-                                                    const unsigned* __restrict__ totals, unsigned* __restrict__ valid, Source src,
-                                                    int shift, int tiles) {
+                                                    const unsigned* __restrict__ totals, unsigned* __restrict__ valid,
+                                                    unsigned* __restrict__ starts, Source src,
+                                                    int shift, int tiles, Zeros zeros) {
+    if ((int)blockIdx.x >= tiles) return zeros.share(blockIdx.x - tiles);
     __shared__ unsigned h[8][kDigits + 1];
     for (int i = threadIdx.x; i < 8 * (kDigits + 1); i += 256) (&h[0][0])[i] = 0;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -334,7 +385,7 @@ __global__ void __launch_bounds__(256) k_sort_place(Entry* __restrict__ out, con
         }
     }
     o += before_me(total, all);   // all threads: h has been cleared behind it
-    if (blockIdx.x == 0 && threadIdx.x == 0) *valid = all;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *valid = all, *starts = 0;
 #pragma unroll
     for (int k = 0; k < kItems; ++k) {
         const unsigned same = __match_any_sync(0xffffffffu, digit[k]);
@@ -365,8 +416,10 @@ struct RunArgs {
     float* part;              // [chunks][2][c]: of a run that came from before; that goes on behind
     const Entry* sorted;
     const unsigned* valid;
+    unsigned* starts;         // their number, then the chunks in which a run begins that goes on behind
     const void* g;
     float scale;
+    int64_t count;            // entries that `sorted` has room for
     int c, length;            // length: entries of a chunk
     bool vec, vec4;           // rows of out, of part: whole accesses
 };
@@ -374,15 +427,23 @@ struct RunArgs {
 // A thread's V channels of the entries of one chunk.  blockDim: (lanes of a row, chunks of a CTA).
 template <typename T, int V>
 __global__ void __launch_bounds__(256) k_runs(const __grid_constant__ RunArgs a) {
-    const int64_t valid = *a.valid;
     const int64_t chunk = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
     const int64_t begin = chunk * a.length;
     const int64_t col = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * V;
-    if (begin >= valid || col >= a.c) return;
+    if (begin >= a.count || col >= a.c) return;
+    Entry e[8];   // read ahead of what `valid` allows (there is room for all), used as far as it does
+    const auto entries = [&](int64_t i) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) e[k] = a.sorted[i + k < a.count ? i + k : a.count - 1];
+    };
+    entries(begin);
+    const unsigned before = a.sorted[begin > 0 ? begin - 1 : 0].label;
+    const int64_t valid = *a.valid;
+    if (begin >= valid) return;
     const int64_t end = begin + a.length < valid ? begin + a.length : valid;
     const T* g = static_cast<const T*>(a.g) + col;
-    unsigned label = a.sorted[begin].label;
-    bool head = begin > 0 && a.sorted[begin - 1].label == label;
+    unsigned label = e[0].label;
+    bool head = begin > 0 && before == label;
     const bool tail_at_end = end < valid && a.sorted[end].label == a.sorted[end - 1].label;
     float acc[V];
 #pragma unroll
@@ -398,23 +459,24 @@ __global__ void __launch_bounds__(256) k_runs(const __grid_constant__ RunArgs a)
         }
     };
     for (int64_t i = begin; i < end; i += 8) {
-        Entry e[8];
         Vec<T, V> v[8];
+        unsigned of[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             if (i + k < end) {
-                e[k] = a.sorted[i + k];
+                of[k] = e[k].label;
                 v[k].load(g + (int64_t)e[k].at * a.c);
             } else {
                 v[k].zero();
-                e[k].label = e[k - 1 < 0 ? 0 : k - 1].label;   // i < end: k is above 0
+                of[k] = of[k - 1 < 0 ? 0 : k - 1];   // i < end: k is above 0
             }
         }
+        entries(i + 8);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            if (e[k].label != label) {
+            if (of[k] != label) {
                 out(false);
-                label = e[k].label;
+                label = of[k];
                 head = false;
 #pragma unroll
                 for (int j = 0; j < V; ++j) acc[j] = 0.f;
@@ -424,30 +486,28 @@ __global__ void __launch_bounds__(256) k_runs(const __grid_constant__ RunArgs a)
         }
     }
     out(tail_at_end);
+    if (col == 0 && tail_at_end && !head) a.starts[1 + atomicAdd(a.starts, 1u)] = (unsigned)chunk;   // in any order: runs are apart
 }
 
 // The runs that begin in a chunk and go on behind it: its part and those of the
-// chunks up to the run's end, which a search of the sorted list finds.  A CTA a
-// chunk, most have none; `lanes` threads of V channels side by side, the others take
-// every 256 / lanes-th part, and theirs are added in order.
+// chunks up to the run's end.  `lanes` threads of V channels side by side (blockIdx.y
+// has others), the others take every 256 / lanes-th part, and theirs are added in
+// order.
 template <int V>
 __global__ void __launch_bounds__(256) k_join_runs(const __grid_constant__ RunArgs a, int lanes) {
     __shared__ float sums[256 * V];
-    const int64_t valid = *a.valid, chunk = blockIdx.x, end = (chunk + 1) * a.length;
-    if (end >= valid) return;
-    const unsigned label = a.sorted[end].label;
-    const int64_t begin = chunk * a.length;
-    if (a.sorted[end - 1].label != label) return;
-    if (a.sorted[begin].label == label && begin > 0 && a.sorted[begin - 1].label == label) return;   // began earlier
-    int64_t lo = end, hi = valid;   // the run ends at the first entry of another label: lo < it <= hi
-    while (hi - lo > 1) {
-        const int64_t mid = (lo + hi) >> 1;
-        if (a.sorted[mid].label == label) lo = mid;
-        else hi = mid;
+    const unsigned starts = a.starts[0];
+    const int64_t valid = *a.valid;
+    for (unsigned i = blockIdx.x; i < starts; i += gridDim.x) {
+    const int64_t chunk = a.starts[1 + i];
+    const unsigned label = a.sorted[(chunk + 1) * a.length].label;
+    int64_t parts = 1;   // chunks behind this one that the run reaches: those that begin with its label
+    for (int count = 256; count == 256; parts += count) {
+        const int64_t at = (chunk + 1 + parts + threadIdx.x) * a.length;
+        count = __syncthreads_count(at < valid && a.sorted[at < valid ? at : 0].label == label);
     }
-    const int64_t parts = (lo / a.length) - chunk;   // chunks behind this one
     const int lane = threadIdx.x % lanes, group = threadIdx.x / lanes, groups = 256 / lanes;
-    for (int64_t first = 0; first < a.c; first += (int64_t)lanes * V) {
+    for (int64_t first = (int64_t)blockIdx.y * lanes * V; first < a.c; first += (int64_t)gridDim.y * lanes * V) {
         const int64_t col = first + lane * V;
         float s[V];
 #pragma unroll
@@ -484,6 +544,7 @@ __global__ void __launch_bounds__(256) k_join_runs(const __grid_constant__ RunAr
         }
         __syncthreads();
     }
+    }
 }
 
 // ------------------------------------------------------------------ host side
@@ -495,7 +556,7 @@ struct EmbedPlan {
     int v, lanes, slabs, warps, ctas, ctas_y;   // small table
     int passes, items, tiles, length;            // sorted; passes 0: by counting
     int64_t chunks;
-    int64_t valid, totals, counts, first, second, part, bytes;   // offsets in the workspace
+    int64_t totals, starts, counts, first, second, part, bytes;   // offsets in the workspace
 };
 
 constexpr int kOwnSums = 256;   // tiles up to which the tiles add up the counts themselves
@@ -504,12 +565,12 @@ static EmbedPlan embed_plan(int64_t count, int64_t n, int c) {
     EmbedPlan p = {};
     p.small = n <= kSmallTable;
     if (p.small) {
-        p.v = c % 2 == 0 ? 2 : 1;
+        p.v = c % 4 == 0 && n <= kWideTable ? 4 : c % 2 == 0 ? 2 : 1;
         const int units = c / p.v;
         p.lanes = 1;
         while (p.lanes < 32 && p.lanes < units) p.lanes <<= 1;
         const int all = (int)ceil_div(units, p.lanes), fit = (int)(kTableBytes / (n * 32 * p.v * 4));
-        p.warps = fit < 32 ? fit : 32;
+        p.warps = p.v == 4 ? (fit < 20 ? fit : 20) : fit < 32 ? fit : 32;
         p.slabs = all < p.warps ? all : p.warps;
         p.warps = p.warps / p.slabs * p.slabs;
         p.ctas_y = (int)ceil_div(all, p.slabs);
@@ -531,6 +592,8 @@ static EmbedPlan embed_plan(int64_t count, int64_t n, int c) {
     p.chunks = ceil_div(count, p.length);
     p.totals = 256;   // the number of valid entries is in front
     int64_t at = p.totals + kDigits * 4;
+    p.starts = at;
+    at += align256((p.chunks + 1) * 4);
     p.counts = at;
     at += align256((int64_t)kDigits * p.tiles * 4);
     p.first = at;
@@ -560,31 +623,46 @@ static cudaError_t launch_small(const TableArgs& a, const EmbedPlan& p, cudaStre
 template <typename T>
 static cudaError_t small_table(const TableArgs& a, const EmbedPlan& p, cudaStream_t s) {
     if (p.v == 1) return launch_small<T, 1, true>(a, p, s);
+    if (p.v == 4)
+        return (uintptr_t)a.g % (4 * sizeof(T)) ? launch_small<T, 4, false>(a, p, s) : launch_small<T, 4, true>(a, p, s);
     return (uintptr_t)a.g % (2 * sizeof(T)) ? launch_small<T, 2, false>(a, p, s) : launch_small<T, 2, true>(a, p, s);
 }
 
-template <int kItems>
-static void sort_pass(Entry* to, unsigned* counts, unsigned* totals, unsigned* valid, const Source& src, int shift, int tiles,
-                      cudaStream_t s) {
-    k_sort_count<kItems><<<tiles, 256, 0, s>>>(counts, src, shift);
-    const bool own = tiles <= kOwnSums;
-    if (!own) k_sort_sums<<<kDigits, 256, 0, s>>>(counts, totals, tiles);
-    k_sort_place<kItems><<<tiles, 256, 0, s>>>(to, counts, own ? nullptr : totals, valid, src, shift, tiles);
+// The i-th of `launches` shares of the zeros.
+static Zeros zeros_of(void* table, int64_t bytes, int i, int launches) {
+    const int64_t all = bytes / 16;
+    Zeros z{static_cast<uint4*>(table), all * i / launches, all * (i + 1) / launches, 0};
+    const int64_t need = ceil_div(z.end - z.begin, 256 * 4), most = 2 * (int64_t)sm_count();
+    z.ctas = (int)(need < most ? need : most);
+    return z;
 }
 
-// The labels in order with their positions.
-static const Entry* sort_labels(const EmbedPlan& p, uint8_t* ws, const Labels& ids, int64_t count, int64_t n, cudaStream_t s) {
+template <int kItems>
+static void sort_pass(Entry* to, unsigned* counts, unsigned* totals, unsigned* valid, unsigned* starts, const Source& src, int shift, int tiles,
+                      const Zeros& first, const Zeros& second, cudaStream_t s) {
+    k_sort_count<kItems><<<tiles + first.ctas, 256, 0, s>>>(counts, src, shift, tiles, first);
+    const bool own = tiles <= kOwnSums;
+    if (!own) k_sort_sums<<<kDigits, 256, 0, s>>>(counts, totals, tiles);
+    k_sort_place<kItems><<<tiles + second.ctas, 256, 0, s>>>(to, counts, own ? nullptr : totals, valid, starts, src, shift, tiles, second);
+}
+
+// The labels in order with their positions; `bytes` of the table (a multiple of
+// 16) are zeroed on the way.
+static const Entry* sort_labels(const EmbedPlan& p, uint8_t* ws, const Labels& ids, int64_t count, int64_t n, void* table, int64_t bytes,
+                                cudaStream_t s) {
     unsigned *valid = reinterpret_cast<unsigned*>(ws), *totals = reinterpret_cast<unsigned*>(ws + p.totals),
-             *counts = reinterpret_cast<unsigned*>(ws + p.counts);
+             *starts = reinterpret_cast<unsigned*>(ws + p.starts), *counts = reinterpret_cast<unsigned*>(ws + p.counts);
     Entry *to = reinterpret_cast<Entry*>(ws + p.first), *other = reinterpret_cast<Entry*>(ws + p.second), *from = nullptr;
     if (p.passes == 0) {
-        k_rank_sort<<<(unsigned)ceil_div(count, 64), 256, 0, s>>>(to, valid, ids, n, (int)count);
+        const Zeros z = zeros_of(table, bytes, 0, 1);
+        k_rank_sort<<<(unsigned)ceil_div(count, 64) + z.ctas, 256, 0, s>>>(to, valid, starts, ids, n, (int)count, z);
         return to;
     }
     for (int pass = 0; pass < p.passes; ++pass) {
         const Source src{ids, n, count, from, valid};
-        if (p.items == 4) sort_pass<4>(to, counts, totals, valid, src, 8 * pass, p.tiles, s);
-        else sort_pass<16>(to, counts, totals, valid, src, 8 * pass, p.tiles, s);
+        const Zeros first = zeros_of(table, bytes, 2 * pass, 2 * p.passes), second = zeros_of(table, bytes, 2 * pass + 1, 2 * p.passes);
+        if (p.items == 4) sort_pass<4>(to, counts, totals, valid, starts, src, 8 * pass, p.tiles, first, second, s);
+        else sort_pass<16>(to, counts, totals, valid, starts, src, 8 * pass, p.tiles, first, second, s);
         from = to;
         to = other;
         other = from;
@@ -595,10 +673,12 @@ static const Entry* sort_labels(const EmbedPlan& p, uint8_t* ws, const Labels& i
 template <typename T, int V>
 static cudaError_t launch_embed(void* y, const Labels& ids, const void* table, float scale, int64_t count, int64_t n,
                                 int c, cudaStream_t s) {
-    const int64_t all = count * (c / V), ctas = ceil_div(all, 256 * kEmbedUnits);
+    const int units = c / V;
+    int shift = 0;
+    while (shift < 8 && 1 << shift < units) ++shift;
+    const int64_t ctas = ceil_div(count, (256 >> shift) * kEmbedRows);
     if (ctas > 0x7fffffff) return cudaErrorInvalidValue;
-    k_embed<T, V><<<(unsigned)ctas, 256, 0, s>>>(static_cast<T*>(y), ids, static_cast<const T*>(table), scale, all, n,
-                                                 (unsigned)(c / V));
+    k_embed<T, V><<<(unsigned)ctas, 256, 0, s>>>(static_cast<T*>(y), ids, static_cast<const T*>(table), scale, count, n, units, shift);
     return cudaGetLastError();
 }
 
@@ -633,10 +713,12 @@ static cudaError_t launch_runs(int v, const RunArgs& a, int64_t chunks, cudaStre
 
 static cudaError_t join_runs(const RunArgs& a, int64_t chunks, cudaStream_t s) {
     const bool four = a.c % 4 == 0;
+    const int units = a.c / (four ? 4 : 1);
     int lanes = 1;
-    while (lanes < 256 && lanes < a.c / (four ? 4 : 1)) lanes <<= 1;
-    if (four) k_join_runs<4><<<(unsigned)(chunks - 1), 256, 0, s>>>(a, lanes);
-    else k_join_runs<1><<<(unsigned)(chunks - 1), 256, 0, s>>>(a, lanes);
+    while (lanes < 64 && lanes < units) lanes <<= 1;
+    const dim3 grid((unsigned)(chunks - 1 < 592 ? chunks - 1 : 592), (unsigned)(ceil_div(units, lanes) < 8 ? ceil_div(units, lanes) : 8));
+    if (four) k_join_runs<4><<<grid, 256, 0, s>>>(a, lanes);
+    else k_join_runs<1><<<grid, 256, 0, s>>>(a, lanes);
     return cudaGetLastError();
 }
 
@@ -695,14 +777,16 @@ int plattice_embed_backward(void* grad_table, int table_dtype, const void* grad_
         }
         return rows_status(e, "plattice_embed_backward");
     }
-    e = cudaMemsetAsync(grad_table, 0, (size_t)n * c * dtype_size(table_dtype), s);
+    const size_t bytes = (size_t)n * c * dtype_size(table_dtype), whole = count && aligned16(grad_table) ? bytes / 16 * 16 : 0;
+    if (whole < bytes) e = cudaMemsetAsync(static_cast<uint8_t*>(grad_table) + whole, 0, bytes - whole, s);
     if (count == 0 || e != cudaSuccess) return rows_status(e, "plattice_embed_backward");
-    const Entry* sorted = sort_labels(p, ws, labels, count, n, s);
+    unsigned* starts = reinterpret_cast<unsigned*>(ws + p.starts);
+    const Entry* sorted = sort_labels(p, ws, labels, count, n, grad_table, (int64_t)whole, s);
     e = cudaGetLastError();
     if (e != cudaSuccess) return rows_status(e, "plattice_embed_backward");
     const int v = widest(c, dtype_size(dtype), (uintptr_t)grad_y);
-    const RunArgs a{grad_table, table_dtype, reinterpret_cast<float*>(ws + p.part), sorted, reinterpret_cast<unsigned*>(ws), grad_y, scale,
-                    c, p.length, table_dtype == dtype && widest(c, dtype_size(dtype), (uintptr_t)grad_table) >= v,
+    const RunArgs a{grad_table, table_dtype, reinterpret_cast<float*>(ws + p.part), sorted, reinterpret_cast<unsigned*>(ws), starts, grad_y, scale,
+                    count, c, p.length, table_dtype == dtype && widest(c, dtype_size(dtype), (uintptr_t)grad_table) >= v,
                     v * (int)sizeof(float) <= 16 ? c % v == 0 : c % 4 == 0};
     e = dtype == PLATTICE_F32    ? launch_runs<float>(v, a, p.chunks, s)
         : dtype == PLATTICE_BF16 ? launch_runs<__nv_bfloat16>(v, a, p.chunks, s)
