@@ -66,13 +66,14 @@ __device__ __forceinline__ void store_out(void* out, int dtype, bool vec, int64_
 
 // ----------------------------------------------------------------- small tables
 //
-// A warp goes through rows 32 labels at a time, 8 rows' gradients under way; a lane
-// adds V channels to the label's place in the warp's copy, which is its own place:
-// nothing else reads or writes it.  Where a row has fewer than 32 V channels,
-// several rows go side by side, each group of lanes with a copy.  Warps of a CTA
-// take slabs of 32 V channels first, then rows.  Four channels a lane where 16 warps'
-// copies of them fit (half the instructions a row), else two.  1048576 rows of 64 channels into
-// 21 labels: the sorted way took 210 us.
+// A warp goes through rows 32 at a time; a lane adds V channels to the label's place
+// in the warp's copy, which is its own place: nothing else reads or writes it.
+// Where a row has fewer than 32 V channels, several rows go side by side, each
+// group of lanes with a copy.  Warps of a CTA take slabs of 32 V channels first,
+// then rows.  The rows come by asynchronous copies, two blocks of 32 under way
+// (loads to registers, 16 rows under way, left the warps waiting: 1048576 rows of 64
+// bfloat16 channels into 21 labels 63 us; sorted 210 us).  Rows on no 16-byte
+// boundaries are loaded a block at a time.
 
 constexpr int kSmallTable = 96, kWideTable = 24, kTableBytes = 200 * 1024;
 
@@ -84,95 +85,111 @@ struct TableArgs {
     const void* g;
     float scale;
     int64_t count, n;
-    int c, lanes, slabs;      // lanes of a row; slabs of a CTA's warps (blockIdx.y has others)
+    int c, lane_bits, slabs;  // 2^lane_bits lanes of a row (2..32); slabs of a CTA's warps (blockIdx.y has others)
     int copies;               // warps a slab
 };
 
+__device__ __forceinline__ void copy_async16(void* to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+
 template <typename T, int V, bool kWhole>
-__global__ void __launch_bounds__(V == 4 ? 640 : 1024) k_small_table(const __grid_constant__ TableArgs a) {
-    constexpr int kTableRows = sizeof(T) * V > 4 * (V == 4 ? 2 : 1) ? 4 : 8;   // as registers allow
-    extern __shared__ float4 memory[];   // [warp][group][n][lanes V]
+__global__ void __launch_bounds__(1024) k_small_table(const __grid_constant__ TableArgs a) {
+    // tables [warp][group][n + 1][lanes V], the last row for rows without a label and what
+    // lies behind the rows or channels; then rows [warp][2][32][lanes V] as T
+    extern __shared__ float4 memory[];
     float* tables = reinterpret_cast<float*>(memory);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    const int n = (int)a.n, width = a.lanes * V, groups = 32 / a.lanes, each = n * 32 * V;
+    const int n = (int)a.n, groups = 32 >> a.lane_bits, bits = a.lane_bits + (V == 4 ? 2 : V == 2 ? 1 : 0), width = 1 << bits,
+              each = (n + 1) * 32 * V;
+    T* rows = reinterpret_cast<T*>(tables + warps * each) + warp * 2 * 32 * width;
     for (int i = threadIdx.x; i < warps * each; i += blockDim.x) tables[i] = 0.f;
     __syncthreads();
-    const int group = lane / a.lanes, own = lane % a.lanes;
+    const int group = lane >> a.lane_bits, own = lane & ((1 << a.lane_bits) - 1);
     const int slab = blockIdx.y * a.slabs + warp % a.slabs, copy = warp / a.slabs;
-    const int col = slab * width + own * V;
-    float* table = tables + warp * each + group * n * width + own * V;
-    const bool here = col < a.c;
-    const int64_t blocks = (a.count + 31) / 32, step = (int64_t)gridDim.x * a.copies;
-    const auto labels_at = [&](int64_t b) {
-        return b < blocks && b * 32 + lane < a.count ? a.ids.at(b * 32 + lane, a.n) : -1;
-    };
-    struct Rows {
-        Vec<T, V> v[kTableRows];
-        int label[kTableRows];
-    };
-    const int64_t c = a.c, apart = c * groups;
-    const T* g = static_cast<const T*>(a.g) + group * c + col;
-    int64_t b = (int64_t)blockIdx.x * a.copies + copy;
-    int r = 0, id = labels_at(b), id_next = labels_at(b + step);
-    const auto load = [&](Rows& q) {   // rows r.. of block b, whose labels the lanes have; then on to the next
-        const T* from = g + (b * 32 + r) * c;
-#pragma unroll
-        for (int k = 0; k < kTableRows; ++k, from += apart) {
-            const int at = r + k * groups + group, label = __shfl_sync(0xffffffffu, id, at & 31);
-            const bool some = label >= 0 && at < 32 && here;
-            q.label[k] = some ? label : 0;   // a row without a label adds 0 to the first: no branch
-            q.v[k].zero();
-            if (some) {
-                if constexpr (kWhole) {
-                    q.v[k].load(from);
-                } else {
-                    float f[V];
-#pragma unroll
-                    for (int j = 0; j < V; ++j) f[j] = to_f32(from[j]);
-                    q.v[k].from(f);
-                }
+    float* table = tables + warp * each + group * (n + 1) * width + own * V;
+    const T* g = static_cast<const T*>(a.g) + slab * width;
+    const int wide = a.c - slab * width;   // channels from the slab's first on
+    const int64_t blocks = (a.count + 31) / 32, step = (int64_t)gridDim.x * a.copies, c = a.c;
+    // The rows of block b on their way to a stage; a lane's label of them is the result.
+    const auto bring = [&](int64_t b, T* stage) {
+        const int64_t row0 = b * 32, left = a.count - row0;
+        if (left > 0) {
+            constexpr int kN = kWhole ? 16 / (int)sizeof(T) : 1, kBits = kWhole ? (sizeof(T) == 2 ? 3 : 2) : 0;
+            // a pass of the warp: 32 accesses of kN elements of neighbouring rows (or a part of one)
+            const int per_row = bits - kBits, at = (lane & ((1 << per_row) - 1)) * kN;
+            for (int first = 0; first < (1 << per_row); first += 32) {
+                const int col = at + first * kN;
+                int row = per_row >= 5 ? 0 : lane >> per_row;
+                const int next = per_row >= 5 ? 1 : 32 >> per_row;
+                const T* from = g + (row0 + row) * c + (per_row >= 5 ? (lane + first) * kN : col);
+                T* to = stage + (row << bits) + (per_row >= 5 ? (lane + first) * kN : col);
+                const bool inside = (per_row >= 5 ? (lane + first) * kN : col) < wide;
+                const int most = left < 32 ? (int)left : 32;
+                for (; row < most; row += next, from += next * c, to += next << bits)
+                    if (inside) {
+                        if constexpr (kWhole) copy_async16(to, from);
+                        else *to = *from;
+                    }
             }
         }
-        r += kTableRows * groups;
-        if (r >= 32) {
-            r = 0;
-            b += step;
-            id = id_next;
-            id_next = labels_at(b + step);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        const int id = lane < left ? a.ids.at(row0 + lane, a.n) : -1;
+        return id < 0 ? n : id;
+    };
+    const auto add = [&](const T* stage, int id) {
+        const T* from = stage + (group << bits) + own * V;
+        int at = group;
+#pragma unroll 4
+        for (int r = 0; r < 32; r += 2 * groups, at += 2 * groups, from += (2 * groups) << bits) {
+            // two rows of the group together: of the same label they are added first
+            const int l0 = __shfl_sync(0xffffffffu, id, at), l1 = __shfl_sync(0xffffffffu, id, at + groups);
+            Vec<T, V> v0, v1;
+            v0.load(from);
+            v1.load(from + (groups << bits));
+            Vec<float, V>*p0 = reinterpret_cast<Vec<float, V>*>(table + (l0 << bits)),
+            *p1 = reinterpret_cast<Vec<float, V>*>(table + (l1 << bits));
+            const Vec<float, V> t0 = *p0, t1 = *p1;
+            const bool same = l0 == l1;
+            float f0[V], f1[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float x = v1.at(j);
+                f0[j] = t0.at(j) + (v0.at(j) + (same ? x : 0.f));
+                f1[j] = t1.at(j) + x;
+            }
+            Vec<float, V> o0, o1;
+            o0.from(f0);
+            o1.from(f1);
+            *p0 = o0;
+            if (!same) *p1 = o1;
         }
     };
-    const auto add = [&](const Rows& q) {
-#pragma unroll
-        for (int k = 0; k < kTableRows; ++k) {
-            Vec<float, V>* at = reinterpret_cast<Vec<float, V>*>(table + q.label[k] * width);
-            Vec<float, V> t = *at;
-            float f[V];
-#pragma unroll
-            for (int j = 0; j < V; ++j) f[j] = t.at(j) + q.v[k].at(j);
-            t.from(f);
-            *at = t;
-        }
-    };
-    Rows odd, even;   // one under way while the other is added
-    load(even);
-    for (bool more = true; more;) {
-        more = b < blocks;
-        load(odd);
-        add(even);
-        if (!more) break;
-        more = b < blocks;
-        load(even);
-        add(odd);
+    T *even = rows, *odd = rows + 32 * width;
+    int64_t b = (int64_t)blockIdx.x * a.copies + copy;
+    int id0 = bring(b, even), id1 = bring(b + step, odd);
+    for (; b < blocks; b += 2 * step) {
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        __syncwarp();
+        add(even, id0);
+        __syncwarp();
+        id0 = bring(b + 2 * step, even);
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        __syncwarp();
+        add(odd, id1);
+        __syncwarp();
+        id1 = bring(b + 3 * step, odd);
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
     // The copies of a slab together, in order, for the CTA's channels.
     const int64_t first = (int64_t)blockIdx.y * a.slabs * width;
-    const int wide = a.c - first < (int64_t)a.slabs * width ? (int)(a.c - first) : a.slabs * width;
-    for (int i = threadIdx.x; i < n * wide; i += blockDim.x) {
-        const int label = i / wide, at = i - label * wide, w = at / width, j = at - w * width;
+    const int span = a.c - first < (int64_t)a.slabs * width ? (int)(a.c - first) : a.slabs * width;
+    for (int i = threadIdx.x; i < n * span; i += blockDim.x) {
+        const int label = i / span, at = i - label * span, w = at / width, j = at - w * width;
         float sum = 0.f;
         for (int k = 0; k < a.copies; ++k)
-            for (int q = 0; q < groups; ++q) sum += tables[(k * a.slabs + w) * each + (q * n + label) * width + j];
+            for (int q = 0; q < groups; ++q) sum += tables[(k * a.slabs + w) * each + (q * (n + 1) + label) * width + j];
         const int64_t to = (int64_t)label * a.c + first + at;
         if (a.out) store_param(a.out, a.out_dtype, to, sum * a.scale);
         else a.part[(int64_t)blockIdx.x * n * a.c + to] = sum;
@@ -553,7 +570,7 @@ static int64_t align256(int64_t b) { return (b + 255) / 256 * 256; }
 
 struct EmbedPlan {
     bool small;
-    int v, lanes, slabs, warps, ctas, ctas_y;   // small table
+    int v, lane_bits, slabs, warps, warp_bytes, ctas, ctas_y;   // small table
     int passes, items, tiles, length;            // sorted; passes 0: by counting
     int64_t chunks;
     int64_t totals, starts, counts, first, second, part, bytes;   // offsets in the workspace
@@ -561,16 +578,20 @@ struct EmbedPlan {
 
 constexpr int kOwnSums = 256;   // tiles up to which the tiles add up the counts themselves
 
-static EmbedPlan embed_plan(int64_t count, int64_t n, int c) {
+static EmbedPlan embed_plan(int64_t count, int64_t n, int c, int element) {
     EmbedPlan p = {};
     p.small = n <= kSmallTable;
     if (p.small) {
-        p.v = c % 4 == 0 && n <= kWideTable ? 4 : c % 2 == 0 ? 2 : 1;
+        // 8 bytes a lane (half the instructions a row) where many warps' copies of that fit
+        const int widest_v = element == 4 || n <= kWideTable ? 8 / element : 4 / element;
+        p.v = widest_v;
+        while (c % p.v) p.v >>= 1;
         const int units = c / p.v;
-        p.lanes = 1;
-        while (p.lanes < 32 && p.lanes < units) p.lanes <<= 1;
-        const int all = (int)ceil_div(units, p.lanes), fit = (int)(kTableBytes / (n * 32 * p.v * 4));
-        p.warps = p.v == 4 ? (fit < 20 ? fit : 20) : fit < 32 ? fit : 32;
+        p.lane_bits = 1;
+        while (p.lane_bits < 5 && 1 << p.lane_bits < units) ++p.lane_bits;
+        p.warp_bytes = (int)(n + 1) * 32 * p.v * 4 + 64 * (p.v << p.lane_bits) * element;
+        const int all = (int)ceil_div(units, 1 << p.lane_bits), fit = kTableBytes / p.warp_bytes;
+        p.warps = fit < 32 ? fit : 32;
         p.slabs = all < p.warps ? all : p.warps;
         p.warps = p.warps / p.slabs * p.slabs;
         p.ctas_y = (int)ceil_div(all, p.slabs);
@@ -616,16 +637,17 @@ static cudaError_t launch_small(const TableArgs& a, const EmbedPlan& p, cudaStre
         },
         &unused);
     if (e != cudaSuccess) return e;
-    k_small_table<T, V, kWhole><<<dim3(p.ctas, p.ctas_y), p.warps * 32, (size_t)p.warps * a.n * 32 * V * 4, s>>>(a);
+    k_small_table<T, V, kWhole><<<dim3(p.ctas, p.ctas_y), p.warps * 32, (size_t)p.warps * p.warp_bytes, s>>>(a);
     return cudaGetLastError();
 }
 
 template <typename T>
 static cudaError_t small_table(const TableArgs& a, const EmbedPlan& p, cudaStream_t s) {
-    if (p.v == 1) return launch_small<T, 1, true>(a, p, s);
-    if (p.v == 4)
-        return (uintptr_t)a.g % (4 * sizeof(T)) ? launch_small<T, 4, false>(a, p, s) : launch_small<T, 4, true>(a, p, s);
-    return (uintptr_t)a.g % (2 * sizeof(T)) ? launch_small<T, 2, false>(a, p, s) : launch_small<T, 2, true>(a, p, s);
+    const bool whole = aligned16(a.g) && a.c * sizeof(T) % 16 == 0;
+    if (p.v == 1) return whole ? launch_small<T, 1, true>(a, p, s) : launch_small<T, 1, false>(a, p, s);
+    if (p.v == 2) return whole ? launch_small<T, 2, true>(a, p, s) : launch_small<T, 2, false>(a, p, s);
+    if constexpr (sizeof(T) == 2) return whole ? launch_small<T, 4, true>(a, p, s) : launch_small<T, 4, false>(a, p, s);
+    return cudaErrorInvalidValue;
 }
 
 // The i-th of `launches` shares of the zeros.
@@ -748,7 +770,11 @@ int plattice_embed(void* y, const void* ids, int ids_wide, const void* table, in
 
 int plattice_embed_backward_workspace_size(long long count, long long n, int c, size_t* bytes) {
     if (!bytes || !embed_ok(count, n, c) || count > 0x7fffffff) return PLATTICE_ERR_INVALID;
-    *bytes = count ? (size_t)embed_plan(count, n, c).bytes : 0;
+    *bytes = 0;
+    for (int element = 2; count && element <= 4; element += 2) {   // of gradients of either size
+        const size_t b = (size_t)embed_plan(count, n, c, element).bytes;
+        *bytes = b > *bytes ? b : *bytes;
+    }
     return PLATTICE_OK;
 }
 
@@ -759,7 +785,7 @@ int plattice_embed_backward(void* grad_table, int table_dtype, const void* grad_
         return PLATTICE_ERR_INVALID;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (count && (!grad_y || !ids || (uintptr_t)ids % (ids_wide ? 8 : 4))) return PLATTICE_ERR_INVALID;
-    const EmbedPlan p = embed_plan(count, n, c);
+    const EmbedPlan p = embed_plan(count, n, c, (int)dtype_size(dtype));
     if (count && p.bytes && (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < (size_t)p.bytes))
         return PLATTICE_ERR_WORKSPACE;
     const Labels labels{ids, ids_wide};
@@ -767,7 +793,7 @@ int plattice_embed_backward(void* grad_table, int table_dtype, const void* grad_
     cudaError_t e = cudaSuccess;
     if (count && p.small) {
         const TableArgs a{p.ctas > 1 ? nullptr : grad_table, table_dtype, reinterpret_cast<float*>(ws), labels, grad_y, scale, count, n, c,
-                          p.lanes, p.slabs, p.warps / p.slabs};
+                          p.lane_bits, p.slabs, p.warps / p.slabs};
         e = dtype == PLATTICE_F32    ? small_table<float>(a, p, s)
             : dtype == PLATTICE_BF16 ? small_table<__nv_bfloat16>(a, p, s)
                                      : small_table<__half>(a, p, s);
