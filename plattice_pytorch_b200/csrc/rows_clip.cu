@@ -6,7 +6,9 @@
 // The tensors are cut into pieces of kPiece values; the table of tensors goes
 // with the launch (kernel arguments, no copy to the device), and a CTA finds a
 // piece's tensor by a search of it.  CTAs add their pieces' squares, the second
-// kernel's CTAs each add the CTAs' sums, in the same order, and scale.
+// kernel's CTAs each add the CTAs' sums, in the same order, and scale.  Both are
+// bound by HBM: the gradients are read twice, as far as the L2 does not hold them.
+#include <cooperative_groups.h>
 #include <stdlib.h>
 
 #include <algorithm>
@@ -17,10 +19,11 @@
 
 namespace plr {
 
-constexpr int kPiece = 8192;
-constexpr int kTensors = 256;   // of one launch
+namespace cg = cooperative_groups;
 
-struct Grads {
+constexpr int kPiece = 8192, kUnroll = 4;   // values of a piece: 4 accesses of 8 by each of 256 threads
+
+template <int kTensors> struct Grads {
     const void* g[kTensors];
     void* out[kTensors];
     long long size[kTensors];
@@ -28,9 +31,11 @@ struct Grads {
     uint8_t type[kTensors];       // dtype | out_dtype << 2 | aligned << 4
     int count;
 };
+constexpr int kMost = 256, kSome = 16;   // tensors of one launch; of a small one's table
+constexpr int kResident = 6;             // CTAs of an SM: one round
 
 // The tensor of a piece: the first whose end is above it.
-__device__ __forceinline__ int tensor_of(const Grads& t, long long piece) {
+template <int N> __device__ __forceinline__ int tensor_of(const Grads<N>& t, long long piece) {
     int lo = 0, hi = t.count - 1;
     while (lo < hi) {
         const int mid = (lo + hi) >> 1;
@@ -58,13 +63,29 @@ __device__ __forceinline__ double squares(const float (&v)[8]) {
 }
 
 template <typename T>
-__device__ __forceinline__ double piece_squares(const T* g, long long n, bool aligned) {
+__device__ __forceinline__ double piece_squares(const T* g, int n, bool aligned) {
     double sum = 0.0;
-    for (int i = threadIdx.x * 8; i < n; i += 2048) {
-        float v[8];
-        const int left = (int)(n - i);
-        load8(v, g + i, aligned && left >= 8, left);
-        sum += squares(v);
+    float v[8];
+    if (aligned && n == kPiece) {   // all accesses under way before the first sum
+        Raw8<T> r[kUnroll];
+#pragma unroll
+        for (int k = 0; k < kUnroll; ++k) r[k].load(g + (k * 256 + threadIdx.x) * 8, true, 8);
+#pragma unroll
+        for (int k = 0; k < kUnroll; ++k) {
+            r[k].widen(v);
+            sum += squares(v);
+        }
+    } else if (aligned) {
+        for (int i = threadIdx.x * 8; i < n; i += 2048) {
+            load8(v, g + i, n - i >= 8, n - i);
+            sum += squares(v);
+        }
+    } else {   // neighbouring threads on neighbouring values
+        for (int i = threadIdx.x; i < n; i += 2048) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = i + k * 256 < n ? to_f32(g[i + k * 256]) : 0.f;
+            sum += squares(v);
+        }
     }
     return sum;
 }
@@ -82,19 +103,35 @@ __device__ __forceinline__ double cta_sum(double v) {
     return v;
 }
 
-__global__ void __launch_bounds__(256) k_square_sums(const __grid_constant__ Grads t, double* __restrict__ sums) {
+// Where a piece lies.
+struct At {
+    int tensor, n, dtype;
+    long long first;
+    bool aligned, wide;
+    template <int N> __device__ __forceinline__ At(const Grads<N>& t, long long piece) {
+        tensor = tensor_of(t, piece);
+        first = (piece - (tensor ? t.end[tensor - 1] : 0)) * kPiece;
+        const long long left = t.size[tensor] - first;
+        n = left < kPiece ? (int)left : kPiece;
+        const int type = t.type[tensor];
+        dtype = type & 3;
+        wide = ((type >> 2) & 3) == PLATTICE_F32;
+        aligned = type >> 4;
+    }
+};
+
+template <int N> __device__ __forceinline__ double squares_at(const Grads<N>& t, const At& p) {
+    const void* g = t.g[p.tensor];
+    if (p.dtype == PLATTICE_F32) return piece_squares(static_cast<const float*>(g) + p.first, p.n, p.aligned);
+    if (p.dtype == PLATTICE_BF16) return piece_squares(static_cast<const __nv_bfloat16*>(g) + p.first, p.n, p.aligned);
+    return piece_squares(static_cast<const __half*>(g) + p.first, p.n, p.aligned);
+}
+
+template <int N>
+__global__ void __launch_bounds__(256, kResident) k_square_sums(const __grid_constant__ Grads<N> t, double* __restrict__ sums) {
     double sum = 0.0;
     const long long pieces = t.end[t.count - 1];
-    for (long long p = blockIdx.x; p < pieces; p += gridDim.x) {
-        const int k = tensor_of(t, p);
-        const long long at = (p - (k ? t.end[k - 1] : 0)) * kPiece, left = t.size[k] - at;
-        const long long n = left < kPiece ? left : kPiece;
-        const bool aligned = t.type[k] >> 4;
-        const int dtype = t.type[k] & 3;
-        if (dtype == PLATTICE_F32) sum += piece_squares(static_cast<const float*>(t.g[k]) + at, n, aligned);
-        else if (dtype == PLATTICE_BF16) sum += piece_squares(static_cast<const __nv_bfloat16*>(t.g[k]) + at, n, aligned);
-        else sum += piece_squares(static_cast<const __half*>(t.g[k]) + at, n, aligned);
-    }
+    for (long long p = blockIdx.x; p < pieces; p += gridDim.x) sum += squares_at(t, At(t, p));
     sum = cta_sum(sum);
     if (threadIdx.x == 0) sums[blockIdx.x] = sum;
 }
@@ -120,55 +157,102 @@ __global__ void __launch_bounds__(256) k_norm_only(Norm q) {
     if (threadIdx.x == 0) *q.out = (float)norm;
 }
 
+// Values come and go past the caches' keeping: they are not read again.
 template <typename T, typename O>
-__device__ __forceinline__ void piece_scale(O* out, const T* g, long long n, bool aligned, float f) {
-    for (int i = threadIdx.x * 8; i < n; i += 2048) {
-        float v[8];
-        const int left = (int)(n - i);
-        const bool vec = aligned && left >= 8;
-        load8(v, g + i, vec, left);
+__device__ __forceinline__ void piece_scale(O* out, const T* g, int n, bool aligned, float f) {
+    float v[8];
+    if (aligned && n == kPiece) {
+        Raw8<T> r[kUnroll];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] *= f;
-        store8(out + i, v, vec, left);
+        for (int k = 0; k < kUnroll; ++k) r[k].load(g + (k * 256 + threadIdx.x) * 8, true, 8);
+#pragma unroll
+        for (int k = 0; k < kUnroll; ++k) {
+            r[k].widen(v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] *= f;
+            store8(out + (k * 256 + threadIdx.x) * 8, v, true, 8);
+        }
+    } else if (aligned) {
+        for (int i = threadIdx.x * 8; i < n; i += 2048) {
+            const bool whole = n - i >= 8;
+            load8(v, g + i, whole, n - i);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] *= f;
+            store8(out + i, v, whole, n - i);
+        }
+    } else {
+        for (int i = threadIdx.x; i < n; i += 2048) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = i + k * 256 < n ? to_f32(g[i + k * 256]) : 0.f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (i + k * 256 < n) out[i + k * 256] = from_f32<O>(v[k] * f);
+        }
     }
 }
 
-__global__ void __launch_bounds__(256) k_clip(const __grid_constant__ Grads t, Norm q) {
+template <int N> __device__ __forceinline__ void scale_at(const Grads<N>& t, const At& p, float f) {
+    const void* g = t.g[p.tensor];
+    void* out = t.out[p.tensor];
+    if (f == 1.f && g == out) return;   // in place, as it is
+    if (p.dtype == PLATTICE_F32)
+        piece_scale(static_cast<float*>(out) + p.first, static_cast<const float*>(g) + p.first, p.n, p.aligned, f);
+    else if (p.dtype == PLATTICE_BF16 && p.wide)
+        piece_scale(static_cast<float*>(out) + p.first, static_cast<const __nv_bfloat16*>(g) + p.first, p.n, p.aligned, f);
+    else if (p.dtype == PLATTICE_BF16)
+        piece_scale(static_cast<__nv_bfloat16*>(out) + p.first, static_cast<const __nv_bfloat16*>(g) + p.first, p.n, p.aligned, f);
+    else if (p.wide)
+        piece_scale(static_cast<float*>(out) + p.first, static_cast<const __half*>(g) + p.first, p.n, p.aligned, f);
+    else
+        piece_scale(static_cast<__half*>(out) + p.first, static_cast<const __half*>(g) + p.first, p.n, p.aligned, f);
+}
+
+__device__ __forceinline__ float factor_of(const Norm& q, double norm) {
+    const double f = (double)q.most / (norm + (double)q.eps);
+    return q.most == INFINITY || norm + (double)q.eps == 0.0 ? 1.f : f > 1.0 ? 1.f : (float)f;   // NaN stays
+}
+
+// The pieces that were read last are scaled first: some are still in the L2.
+template <int N>
+__global__ void __launch_bounds__(256, kResident) k_clip(const __grid_constant__ Grads<N> t, Norm q) {
     const double norm = norm_of(q);
     if (blockIdx.x == 0 && threadIdx.x == 0 && q.out) *q.out = (float)norm;
-    const double f64 = (double)q.most / (norm + (double)q.eps);
-    const float f = q.most == INFINITY || norm + (double)q.eps == 0.0 ? 1.f : f64 > 1.0 ? 1.f : (float)f64;   // NaN stays
-    const long long pieces = t.end[t.count - 1];
-    for (long long p = blockIdx.x; p < pieces; p += gridDim.x) {
-        const int k = tensor_of(t, p);
-        if (f == 1.f && t.g[k] == t.out[k]) continue;   // in place, as it is
-        const long long at = (p - (k ? t.end[k - 1] : 0)) * kPiece, left = t.size[k] - at;
-        const long long n = left < kPiece ? left : kPiece;
-        const bool aligned = t.type[k] >> 4;
-        const int dtype = t.type[k] & 3;
-        const bool wide = ((t.type[k] >> 2) & 3) == PLATTICE_F32;
-        if (dtype == PLATTICE_F32)
-            piece_scale(static_cast<float*>(t.out[k]) + at, static_cast<const float*>(t.g[k]) + at, n, aligned, f);
-        else if (dtype == PLATTICE_BF16 && wide)
-            piece_scale(static_cast<float*>(t.out[k]) + at, static_cast<const __nv_bfloat16*>(t.g[k]) + at, n, aligned, f);
-        else if (dtype == PLATTICE_BF16)
-            piece_scale(static_cast<__nv_bfloat16*>(t.out[k]) + at, static_cast<const __nv_bfloat16*>(t.g[k]) + at, n, aligned, f);
-        else if (wide)
-            piece_scale(static_cast<float*>(t.out[k]) + at, static_cast<const __half*>(t.g[k]) + at, n, aligned, f);
-        else
-            piece_scale(static_cast<__half*>(t.out[k]) + at, static_cast<const __half*>(t.g[k]) + at, n, aligned, f);
-    }
+    const float f = factor_of(q, norm);
+    for (long long p = t.end[t.count - 1] - 1 - blockIdx.x; p >= 0; p -= gridDim.x) scale_at(t, At(t, p), f);
+}
+
+// Few pieces: one cluster of kFew CTAs does both, without a second launch.
+constexpr int kFew = 8;
+
+__global__ void __cluster_dims__(kFew) __launch_bounds__(256) k_clip_few(const __grid_constant__ Grads<kSome> t, Norm q) {
+    __shared__ double own;
+    const cg::cluster_group cluster = cg::this_cluster();
+    const long long pieces = t.count ? t.end[t.count - 1] : 0;
+    double sum = 0.0;
+    for (long long p = blockIdx.x; p < pieces; p += kFew) sum += squares_at(t, At(t, p));
+    sum = cta_sum(sum);
+    if (threadIdx.x == 0) own = sum;
+    cluster.sync();
+    sum = 0.0;
+#pragma unroll
+    for (int c = 0; c < kFew; ++c) sum += *cluster.map_shared_rank(&own, c);
+    cluster.sync();   // the others' sums have been read
+    const double norm = sqrt(sum);
+    if (blockIdx.x == 0 && threadIdx.x == 0 && q.out) *q.out = (float)norm;
+    const float f = factor_of(q, norm);
+    if (t.count && t.out[0])
+        for (long long p = blockIdx.x; p < pieces; p += kFew) scale_at(t, At(t, p), f);
 }
 
 // ------------------------------------------------------------------ host side
 
-static int most_ctas() { return 8 * sm_count(); }
+static int most_ctas() { return kResident * sm_count(); }
 
 // Fills a launch's table from grads[first..]; gives the first that did not fit.
-static int fill(Grads& t, const plattice_grad* grads, int first, int count, long long* pieces) {
+template <int N> static int fill(Grads<N>& t, const plattice_grad* grads, int first, int count, long long* pieces) {
     t.count = 0;
     *pieces = 0;
-    for (; first < count && t.count < kTensors; ++first) {
+    for (; first < count && t.count < N; ++first) {
         const plattice_grad& g = grads[first];
         if (g.size == 0) continue;
         const int k = t.count++;
@@ -234,7 +318,7 @@ extern "C" {
 int plattice_clip_grads_workspace_size(const plattice_grad* grads, int count, size_t* bytes) {
     if (!bytes || !grads_ok(grads, count)) return PLATTICE_ERR_INVALID;
     // a sum for each CTA of each launch, whatever the device's SM count (<= 256)
-    *bytes = (size_t)(ceil_div(count, kTensors) + 1) * 2048 * sizeof(double);
+    *bytes = (size_t)(ceil_div(count, kMost) + 1) * 2048 * sizeof(double);
     return PLATTICE_OK;
 }
 
@@ -274,22 +358,27 @@ int plattice_clip_grads(const plattice_grad* grads, int count, float max_norm, f
     plattice_clip_grads_workspace_size(grads, count, &need);
     if (!norm_in && (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < need)) return PLATTICE_ERR_WORKSPACE;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    static thread_local Grads t;
-    double* sums = static_cast<double*>(workspace);
-    int used = 0;
     long long pieces = 0;
+    for (int i = 0; i < count; ++i) pieces += ceil_div(grads[i].size, kPiece);
+    Norm q{norm_in ? nullptr : static_cast<double*>(workspace), 0, norm_in, norm_out, max_norm, eps};
     cudaError_t e = cudaSuccess;
+    if (!norm_in && pieces <= 2 * kFew && tensors <= kSome) {
+        Grads<kSome> t;
+        fill(t, grads, 0, count, &pieces);
+        k_clip_few<<<kFew, 256, 0, s>>>(t, q);
+        return rows_status(cudaGetLastError(), "plattice_clip_grads");
+    }
+    static thread_local Grads<kMost> t;
     if (!norm_in) {
         for (int first = 0; first < count && e == cudaSuccess;) {
             first = fill(t, grads, first, count, &pieces);
             if (!t.count) break;
             const int ctas = ctas_of(pieces);
-            k_square_sums<<<ctas, 256, 0, s>>>(t, sums + used);
-            used += ctas;
+            k_square_sums<<<ctas, 256, 0, s>>>(t, static_cast<double*>(workspace) + q.count);
+            q.count += ctas;
             e = cudaGetLastError();
         }
     }
-    Norm q{norm_in ? nullptr : sums, used, norm_in, norm_out, max_norm, eps};
     if (e == cudaSuccess && outs) {
         for (int first = 0; first < count && e == cudaSuccess;) {
             first = fill(t, grads, first, count, &pieces);
