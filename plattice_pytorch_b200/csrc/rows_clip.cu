@@ -103,13 +103,13 @@ __device__ __forceinline__ double cta_sum(double v) {
     return v;
 }
 
-// Where a piece lies.
+// Where a piece lies; `tensor` where it is known.
 struct At {
     int tensor, n, dtype;
     long long first;
     bool aligned, wide;
-    template <int N> __device__ __forceinline__ At(const Grads<N>& t, long long piece) {
-        tensor = tensor_of(t, piece);
+    template <int N> __device__ __forceinline__ At(const Grads<N>& t, long long piece) : At(t, piece, tensor_of(t, piece)) {}
+    template <int N> __device__ __forceinline__ At(const Grads<N>& t, long long piece, int tensor_) : tensor(tensor_) {
         first = (piece - (tensor ? t.end[tensor - 1] : 0)) * kPiece;
         const long long left = t.size[tensor] - first;
         n = left < kPiece ? (int)left : kPiece;
@@ -117,6 +117,16 @@ struct At {
         dtype = type & 3;
         wide = ((type >> 2) & 3) == PLATTICE_F32;
         aligned = type >> 4;
+    }
+};
+
+// The pieces of a CTA: neighbouring ones, so that it searches for a tensor once.
+struct Share {
+    long long first, end;
+    template <int N> __device__ __forceinline__ explicit Share(const Grads<N>& t) {
+        const long long pieces = t.end[t.count - 1], each = pieces / gridDim.x, more = pieces - each * gridDim.x;
+        first = blockIdx.x * each + (blockIdx.x < more ? blockIdx.x : more);
+        end = first + each + (blockIdx.x < more);
     }
 };
 
@@ -130,8 +140,12 @@ template <int N> __device__ __forceinline__ double squares_at(const Grads<N>& t,
 template <int N>
 __global__ void __launch_bounds__(256, kResident) k_square_sums(const __grid_constant__ Grads<N> t, double* __restrict__ sums) {
     double sum = 0.0;
-    const long long pieces = t.end[t.count - 1];
-    for (long long p = blockIdx.x; p < pieces; p += gridDim.x) sum += squares_at(t, At(t, p));
+    const Share s(t);
+    int tensor = s.first < s.end ? tensor_of(t, s.first) : 0;
+    for (long long p = s.first; p < s.end; ++p) {
+        while (t.end[tensor] <= p) ++tensor;
+        sum += squares_at(t, At(t, p, tensor));
+    }
     sum = cta_sum(sum);
     if (threadIdx.x == 0) sums[blockIdx.x] = sum;
 }
@@ -157,36 +171,48 @@ __global__ void __launch_bounds__(256) k_norm_only(Norm q) {
     if (threadIdx.x == 0) *q.out = (float)norm;
 }
 
-// Values come and go past the caches' keeping: they are not read again.
 template <typename T, typename O>
 __device__ __forceinline__ void piece_scale(O* out, const T* g, int n, bool aligned, float f) {
-    float v[8];
+    // 16 bytes of the wider type a thread: whole sectors of neighbouring threads
+    constexpr int V = 16 / (int)(sizeof(T) > sizeof(O) ? sizeof(T) : sizeof(O)), kPasses = kPiece / (256 * V);
+    float v[V];
     if (aligned && n == kPiece) {
-        Raw8<T> r[kUnroll];
 #pragma unroll
-        for (int k = 0; k < kUnroll; ++k) r[k].load(g + (k * 256 + threadIdx.x) * 8, true, 8);
+        for (int half = 0; half < kPasses; half += 4) {
+            Vec<T, V> r[4];
 #pragma unroll
-        for (int k = 0; k < kUnroll; ++k) {
-            r[k].widen(v);
+            for (int k = 0; k < 4; ++k) r[k].load(g + ((half + k) * 256 + threadIdx.x) * V);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] *= f;
-            store8(out + (k * 256 + threadIdx.x) * 8, v, true, 8);
+            for (int k = 0; k < 4; ++k) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) v[j] = r[k].at(j) * f;
+                Vec<O, V> o;
+                o.from(v);
+                o.store(out + ((half + k) * 256 + threadIdx.x) * V);
+            }
         }
     } else if (aligned) {
-        for (int i = threadIdx.x * 8; i < n; i += 2048) {
-            const bool whole = n - i >= 8;
-            load8(v, g + i, whole, n - i);
+        for (int i = threadIdx.x * V; i < n; i += 256 * V) {
+            if (n - i >= V) {
+                Vec<T, V> r;
+                r.load(g + i);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] *= f;
-            store8(out + i, v, whole, n - i);
+                for (int j = 0; j < V; ++j) v[j] = r.at(j) * f;
+                Vec<O, V> o;
+                o.from(v);
+                o.store(out + i);
+            } else {
+                for (int j = i; j < n; ++j) out[j] = from_f32<O>(to_f32(g[j]) * f);
+            }
         }
     } else {
         for (int i = threadIdx.x; i < n; i += 2048) {
+            float w[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = i + k * 256 < n ? to_f32(g[i + k * 256]) : 0.f;
+            for (int k = 0; k < 8; ++k) w[k] = i + k * 256 < n ? to_f32(g[i + k * 256]) : 0.f;
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-                if (i + k * 256 < n) out[i + k * 256] = from_f32<O>(v[k] * f);
+                if (i + k * 256 < n) out[i + k * 256] = from_f32<O>(w[k] * f);
         }
     }
 }
@@ -212,13 +238,18 @@ __device__ __forceinline__ float factor_of(const Norm& q, double norm) {
     return q.most == INFINITY || norm + (double)q.eps == 0.0 ? 1.f : f > 1.0 ? 1.f : (float)f;   // NaN stays
 }
 
-// The pieces that were read last are scaled first: some are still in the L2.
+// The pieces that a CTA read last are scaled first: some are still in the L2.
 template <int N>
 __global__ void __launch_bounds__(256, kResident) k_clip(const __grid_constant__ Grads<N> t, Norm q) {
     const double norm = norm_of(q);
     if (blockIdx.x == 0 && threadIdx.x == 0 && q.out) *q.out = (float)norm;
     const float f = factor_of(q, norm);
-    for (long long p = t.end[t.count - 1] - 1 - blockIdx.x; p >= 0; p -= gridDim.x) scale_at(t, At(t, p), f);
+    const Share s(t);
+    int tensor = s.first < s.end ? tensor_of(t, s.end - 1) : 0;
+    for (long long p = s.end - 1; p >= s.first; --p) {
+        while (tensor && t.end[tensor - 1] > p) --tensor;
+        scale_at(t, At(t, p, tensor), f);
+    }
 }
 
 // Few pieces: one cluster of kFew CTAs does both, without a second launch.
