@@ -183,12 +183,13 @@ __device__ __forceinline__ void warp_sums(float& a, float& b) {
 // give 0 times infinity) are held at `bound`, 16-bit ones before they are widened:
 // 140 or |m| / 64 below, which their own rounding leaves at least 100.
 template <typename T> struct Exponents {
-    float c, delta;
+    float c, delta, whole;   // whole: 2^-delta
     uint32_t bound;
     bool fast;    // m is far enough from the type's ends (the same for a row)
     __device__ __forceinline__ explicit Exponents(float m) {
         c = -(m * kLog2e);
         delta = fmaf(m, kLog2e, c);
+        whole = exp2_fast(-delta);
         fast = fabsf(m) < 1e38f;
         if constexpr (sizeof(T) == 2) {
             typename Pair<T>::type b;
@@ -231,16 +232,10 @@ struct Sums {
     int equal;
 };
 
-// `own`: the largest of these scores.  The few threads that hold the largest of
-// the row first take it out.
+// The sums of all scores of the pieces, those equal to m with them.
 template <typename T, int K>
-__device__ __forceinline__ void add_up(Sums& s, Piece<T> (&q)[K], float m, float own) {
+__device__ __forceinline__ void add_all(Sums& s, const Piece<T> (&q)[K], const Exponents<T>& x, float m) {
     constexpr int kPairs = Piece<T>::kN / 2;
-    if (own == m) {
-#pragma unroll
-        for (int k = 0; k < K; ++k) s.equal += q[k].take(m);
-    }
-    const Exponents<T> x(m);
     if (x.fast) {
         uint64_t sum = 0ull, weighted = 0ull;
 #pragma unroll
@@ -251,9 +246,9 @@ __device__ __forceinline__ void add_up(Sums& s, Piece<T> (&q)[K], float m, float
                 sum = add2(sum, e);
                 weighted = fma2(e, t, weighted);
             }
-        const float f = exp2_fast(-x.delta), b = both_added(sum) * f;
+        const float b = both_added(sum) * x.whole;
         s.below += b;
-        s.weighted += fmaf(both_added(weighted), f, -x.delta * b);
+        s.weighted += fmaf(both_added(weighted), x.whole, -x.delta * b);
     } else {
         for (int k = 0; k < K; ++k)
 #pragma unroll
@@ -264,6 +259,17 @@ __device__ __forceinline__ void add_up(Sums& s, Piece<T> (&q)[K], float m, float
                 s.weighted = fmaf(e, t, s.weighted);
             }
     }
+}
+
+// `own`: the largest of these scores.  The few threads that hold the largest of
+// the row first take it out.
+template <typename T, int K>
+__device__ __forceinline__ void add_up(Sums& s, Piece<T> (&q)[K], float m, float own) {
+    if (own == m) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) s.equal += q[k].take(m);
+    }
+    add_all(s, q, Exponents<T>(m), m);
 }
 
 // A row's numbers from its sums, written by one thread.
@@ -366,17 +372,17 @@ __device__ __forceinline__ void write_top(const LogpArgs& p, int64_t row, int pl
 
 // ------------------------------------------------------------- a row by a warp
 //
-// Up to 16 neighbouring rows one after the other, the next one's loads under way;
+// Up to 32 neighbouring rows one after the other, the next one's loads under way;
 // lane r keeps row r's sums, and the logarithms, quotients and stores of all of
 // them are made together at the end (one by one they cost more than the
 // exponentials of 256 classes).
 
-constexpr int kWarpRows = 16, kWarpRoom = 64;
+constexpr int kWarpRows = 32, kWarpRoom = 64;
 
 // The best of 16-bit scores: class and score make a key of 32 bits, whose largest
 // of the warp is one instruction; a lane's next largest is that of key - taken
 // (mod 2^32, where those that were taken are smallest).
-template <typename T, int K>
+template <typename T, int K, bool kWhole>
 __device__ __forceinline__ void best_of_16(uint64_t* out, const Piece<T> (&q)[K], int first, int n, int top) {
     typedef typename Pair<T>::type P;
     uint32_t key[8 * K];
@@ -388,10 +394,17 @@ __device__ __forceinline__ void best_of_16(uint64_t* out, const Piece<T> (&q)[K]
             const uint32_t raw = q[k].word(i);
             const P v = __hadd2(*reinterpret_cast<const P*>(&raw), zero);   // -0 as 0
             const uint32_t w = *reinterpret_cast<const uint32_t*>(&v);
-            const uint32_t u = w ^ (((w >> 15) & 0x00010001u) * 0xffffu | 0x80008000u);
+            uint32_t u = w ^ (((w >> 15) & 0x00010001u) * 0xffffu | 0x80008000u);
             const int j = first + k * 256 + 2 * i;
-            key[8 * k + 2 * i] = (unsigned)j < (unsigned)n ? u << 16 | (0xffff - j) : 0u;
-            key[8 * k + 2 * i + 1] = (unsigned)(j + 1) < (unsigned)n ? (u & 0xffff0000u) | (0xfffe - j) : 0u;
+            const uint32_t classes = (uint32_t)(0xfffe - j) << 16 | ((uint32_t)(0xffff - j) & 0xffffu);   // of both
+            if (kWhole) {
+                if (first + k * 256 >= n) u = 0;   // -inf has 0x7f or more
+                key[8 * k + 2 * i] = __byte_perm(u, classes, 0x1054);
+                key[8 * k + 2 * i + 1] = __byte_perm(u, classes, 0x3276);
+            } else {
+                key[8 * k + 2 * i] = (unsigned)j < (unsigned)n ? __byte_perm(u, classes, 0x1054) : 0u;
+                key[8 * k + 2 * i + 1] = (unsigned)(j + 1) < (unsigned)n ? __byte_perm(u, classes, 0x3276) : 0u;
+            }
         }
     uint32_t best = 0, mine = 0;
     const int lane = threadIdx.x & 31;
@@ -477,7 +490,7 @@ __global__ void __launch_bounds__(128) k_logp_warp(const __grid_constant__ LogpA
                 uint64_t* out = best + r * p.top;
                 bool done = false;
                 if (plain) {
-                    if constexpr (sizeof(T) == 2 && K <= 2) best_of_16(out, q, first, n, p.top), done = true;
+                    if constexpr (sizeof(T) == 2 && K <= 2) best_of_16<T, K, kWhole>(out, q, first, n, p.top), done = true;
                     else done = best_by_bound(out, q, first, own, p.top, room[warp], &count[warp]);
                 }
                 if (!done) {
@@ -490,9 +503,18 @@ __global__ void __launch_bounds__(128) k_logp_warp(const __grid_constant__ LogpA
             }
             Sums t = {0.f, 0.f, 0};
             if (plain) {
-                add_up(t, q, m, own);
+                // The largest scores are added with the others; where little is left beside
+                // one of them (the warp agrees), again without.
+                add_all(t, q, Exponents<T>(m), m);
                 warp_sums(t.below, t.weighted);
-                t.equal = (int)__reduce_add_sync(0xffffffffu, (unsigned)t.equal);
+                t.below -= 1.f;
+                t.equal = 1;
+                if (t.below < 0.0625f) {
+                    t = Sums{0.f, 0.f, 0};
+                    add_up(t, q, m, own);
+                    warp_sums(t.below, t.weighted);
+                    t.equal = (int)__reduce_add_sync(0xffffffffu, (unsigned)t.equal);
+                }
             }
             if (lane == r) {
                 most = m;
@@ -1098,19 +1120,23 @@ static cudaError_t launch_ctas(const LogpArgs& a, int64_t nv, int per_row, cudaS
                  : launch_ctas<T, kThreads, kPieces, kAhead, false>(a, nv, per_row, s);
 }
 
-// Rows a warp takes one after the other: few where there are few, so that all SMs work.
-static int rows_each(int64_t rows, int most) {
-    const int64_t want = rows / (sm_count() * 32);
-    return want < 1 ? 1 : want > most ? most : (int)want;
+// Rows a warp takes one after the other: as many as give whole rounds of the CTAs
+// (of 4 warps) that are resident at a time, `most` at most.
+template <typename F> static cudaError_t rows_each(int* each, F* kernel, size_t smem, int64_t rows, int most) {
+    int resident = 0;
+    const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kernel, 128, smem);
+    const int64_t warps = 4 * (int64_t)sm_count() * (resident > 0 ? resident : 1), rounds = ceil_div(rows, warps * most);
+    *each = (int)ceil_div(rows, warps * rounds);
+    return e;
 }
 
 template <typename T, int K, bool kTop>
 static cudaError_t launch_warp(const LogpArgs& a, cudaStream_t s) {
-    const int each = rows_each(a.rows, kWarpRows);
-    const unsigned ctas = grid_of(ceil_div(a.rows, 4 * each));
-    const size_t smem = (size_t)4 * each * a.top * 8;
-    if (whole_rows<T>(a)) k_logp_warp<T, K, kTop, true><<<ctas, 128, smem, s>>>(a, each);
-    else k_logp_warp<T, K, kTop, false><<<ctas, 128, smem, s>>>(a, each);
+    const auto kernel = whole_rows<T>(a) ? k_logp_warp<T, K, kTop, true> : k_logp_warp<T, K, kTop, false>;
+    int each = 0;
+    const cudaError_t e = rows_each(&each, kernel, (size_t)4 * kWarpRows * a.top * 8, a.rows, kWarpRows);
+    if (e != cudaSuccess) return e;
+    kernel<<<grid_of(ceil_div(a.rows, 4 * each)), 128, (size_t)4 * each * a.top * 8, s>>>(a, each);
     return cudaGetLastError();
 }
 template <typename T, int K>
@@ -1153,10 +1179,11 @@ cudaError_t logp_backward(const LogpArgs& a, cudaStream_t s) {
     const int64_t nv = vectors_of<T>(a);
     const bool same = (((uintptr_t)a.x ^ (uintptr_t)a.gx) & 15) == 0;
     if (nv <= 512) {
-        const int each = rows_each(a.rows, 32), pieces = (int)ceil_div(nv, 32);
-        const unsigned ctas = grid_of(ceil_div(a.rows, 4 * each));
-        if (whole_rows<T>(a)) k_logp_grad_warp<T, true><<<ctas, 128, 0, s>>>(a, each, pieces, same);
-        else k_logp_grad_warp<T, false><<<ctas, 128, 0, s>>>(a, each, pieces, same);
+        const auto kernel = whole_rows<T>(a) ? k_logp_grad_warp<T, true> : k_logp_grad_warp<T, false>;
+        int each = 0;
+        const cudaError_t e = rows_each(&each, kernel, 0, a.rows, 32);
+        if (e != cudaSuccess) return e;
+        kernel<<<grid_of(ceil_div(a.rows, 4 * each)), 128, 0, s>>>(a, each, (int)ceil_div(nv, 32), same);
     } else {
         const int64_t shares = ceil_div(nv, 256 * kAtOnce);
         k_logp_grad<T><<<grid_of(a.rows * shares), 256, 0, s>>>(a, shares, same);

@@ -257,16 +257,26 @@ def test_scores_that_are_not_finite(dev, R):
         assert torch.equal(a[0], b[2])
 
 
-def test_confident_answers_keep_their_precision(dev, R):
-    x = torch.tensor([[20.0, 0.0, -1.0], [1e4, 0.0, 0.0], [40.0, 1.0, 2.0]], device=dev)
-    r = R.log_probs(x, torch.zeros(3, dtype=torch.int64, device=dev))
-    below = f64(x)[:, 1:] - f64(x)[:, :1]   # all of them: float64's sum with the 1 would lose exp(-40), too
-    rest = np.exp(below).sum(1)
-    entropy = np.log1p(rest) - (np.exp(below) * below).sum(1) / (1 + rest)
-    assert worst(f64(r.logp), -np.log1p(rest), 40 * U * rest + 2.0 ** -149) <= 1
-    g = f64(R.log_probs_backward(x, r, torch.zeros(3, dtype=torch.int64, device=dev), torch.ones(3, device=dev)))
-    assert worst(g[:, 0], rest / (1 + rest), 60 * U * rest + 2.0 ** -149) <= 1
-    assert worst(f64(r.entropy), entropy, 100 * U * entropy + 2.0 ** -126) <= 1
+@pytest.mark.parametrize("n", [3, 70, 300, 1200, 6000, 40001, 140000])
+def test_confident_answers_keep_their_precision(dev, R, n):
+    """Rows by a thread, a warp, a CTA and a cluster; to the bounds of the exponentials
+    (|d| up to 41 counts, 2 U |d| + 8 U) and of sums of n terms, relative to what is left."""
+    x = torch.tensor([[20.0, 0.0, -1.0], [1e4, 0.0, 0.0], [40.0, 1.0, 2.0]])
+    x = torch.cat([x, torch.full((3, n - 3), -70.0)], 1)
+    for dtype in (torch.float32, torch.bfloat16):
+        v = x.to(dtype).to(dev)
+        labels = torch.zeros(3, dtype=torch.int64, device=dev)
+        r = R.log_probs(v, labels, top=2)
+        below = f64(v)[:, 1:] - f64(v)[:, :1]   # all of them: float64's sum with the 1 would lose exp(-40), too
+        rest = np.exp(below).sum(1)
+        entropy = np.log1p(rest) - (np.exp(below) * below).sum(1) / (1 + rest)
+        e = (2 * 41 + 8 + 10 + n / 32 + 40) * U
+        assert worst(f64(r.logp), -np.log1p(rest), e * rest + 2.0 ** -149) <= 1
+        assert worst(f64(r.top_logp)[:, 0], -np.log1p(rest), e * rest + 2.0 ** -149) <= 1
+        g = f64(R.log_probs_backward(v, r, labels, torch.ones(3, device=dev)))
+        want = rest / (1 + rest)
+        assert worst(g[:, 0], want, (e + half_step(dtype)) * want + 2.0 ** -134) <= 1
+        assert worst(f64(r.entropy), entropy, 2 * e * entropy + 2.0 ** -126) <= 1
 
 
 def test_log_probs_of_unaligned_rows(dev, R):
