@@ -537,45 +537,85 @@ __global__ void __launch_bounds__(128) k_logp_warp(const __grid_constant__ LogpA
 
 // ------------------------------------------------------------- a row by CTAs
 //
-// A CTA of kThreads, or a cluster of per_row of them, goes through rows, kPieces
-// accesses a thread and row.  kLoop false: the accesses of the next two rows are
-// under way as asynchronous copies, to places in shared memory that only the
-// thread itself reads, so that they need no barrier.  kLoop true: rows that no
-// cluster holds; each CTA takes its share in `rounds`, twice.  What is left to do
-// for a row when its sums are known is made for 32 rows at a time.
+// A CTA, or a cluster of per_row of them, goes through rows; each warp has a share
+// of a row, kPieces accesses a lane, and knows no other warp's: it leaves the sums
+// of its share relative to its own largest score, and its best alternatives, in
+// shared memory, and goes on to the next row.  After kBatch rows the CTAs meet, and
+// every row's shares are put together by a warp.  (Meeting twice a row, to share the
+// largest score first, took 115 us for 8192 x 32768 and 281 for 2000 x 100003.)
+//
+// kAhead > 0: the next rows' accesses are under way as asynchronous copies, to
+// places in shared memory that only the thread itself reads, so that they need no
+// barrier.  kAhead 0: rows that no cluster holds; a warp takes its share in rounds.
 
-constexpr int kRoom = 256, kBatch = 32;
+constexpr int kBatch = 32, kTopBatch = 8;
 
 __device__ __forceinline__ void copy16(uint4* to, const void* from) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
 }
 
-struct Batch {
-    float m[kBatch];
-    Sums sums[kBatch];
+// A share's largest score and its sums relative to it.
+struct alignas(16) Share {
+    float m;
+    Sums sums;
+    // Of both: the one with the smaller largest score is scaled to the other.
+    __device__ __forceinline__ void join(const Share& o) {
+        const Share &hi = o.m > m ? o : *this, &lo = o.m > m ? *this : o;
+        Share r = hi;
+        if (lo.m == hi.m) {
+            r.sums.below += lo.sums.below;
+            r.sums.weighted += lo.sums.weighted;
+            r.sums.equal += lo.sums.equal;
+        } else if (lo.m > -INFINITY) {
+            const float t = fmaxf((lo.m - hi.m) * kLog2e, kLowest), e = exp2_fast(t), all = lo.sums.below + (float)lo.sums.equal;
+            r.sums.below = fmaf(all, e, r.sums.below);
+            r.sums.weighted += e * fmaf(t, all, lo.sums.weighted);
+        }
+        r.m = max_nan(m, o.m);
+        *this = r;
+    }
 };
 
+// The sums of a warp's pieces relative to m, its largest score: in all lanes.
+template <typename T, int K>
+__device__ __forceinline__ Sums warp_add_up(Piece<T> (&q)[K], float m, float own) {
+    Sums t = {0.f, 0.f, 0};
+    if (!(m < INFINITY && m > -INFINITY)) return t;
+    // The largest scores are added with the others; where little is left beside one of
+    // them (the warp agrees), again without.
+    add_all(t, q, Exponents<T>(m), m);
+    warp_sums(t.below, t.weighted);
+    t.below -= 1.f;
+    t.equal = 1;
+    if (t.below < 0.0625f) {
+        t = Sums{0.f, 0.f, 0};
+        add_up(t, q, m, own);
+        warp_sums(t.below, t.weighted);
+        t.equal = (int)__reduce_add_sync(0xffffffffu, (unsigned)t.equal);
+    }
+    return t;
+}
+
 template <typename T, int kThreads, int kPieces, int kAhead, bool kTop>
-__global__ void __launch_bounds__(kThreads, kThreads == 512 ? 2 : kThreads == 256 ? 3 : 6) k_logp_ctas(const __grid_constant__ LogpArgs p, int share, int rounds, int per_row) {
+__global__ void __launch_bounds__(kThreads, kThreads == 512 ? 2 : kThreads == 256 ? 3 : 6) k_logp_ctas(
+    const __grid_constant__ LogpArgs p, int share, int rounds, int per_row) {
     constexpr bool kLoop = kAhead == 0;
-    constexpr int kWarps = kThreads / 32, kN = Piece<T>::kN, kSegment = kThreads / 32;   // 32 segments of threads
-    extern __shared__ uint4 ring[];   // [kAhead][kPieces][kThreads], then [kBatch][top] keys
-    __shared__ uint64_t room[2][kRoom], merged[8 * 32];
-    __shared__ int count[2];
-    __shared__ float segment[32], part_m[2][kWarps], cta_m[2], bound_at;
-    __shared__ Sums part[2][kWarps], cta[2];
-    __shared__ Batch batch;
-    uint64_t* best = reinterpret_cast<uint64_t*>(ring + (kLoop ? 0 : kAhead * kPieces * kThreads));
+    constexpr int kWarps = kThreads / 32, kN = Piece<T>::kN, step = 32 * kN, kRows = kTop ? kTopBatch : kBatch;
+    extern __shared__ uint4 ring[];   // [kAhead][kPieces][kThreads], then keys [kRows][kWarps][top]
+    __shared__ uint64_t room[kTop ? kWarps : 1][kWarpRoom];
+    __shared__ int count[kWarps];
+    __shared__ Share shares[kRows][kWarps];
+    uint64_t* lists = reinterpret_cast<uint64_t*>(ring + kAhead * kPieces * kThreads);
     const cg::cluster_group cluster = cg::this_cluster();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rank = per_row > 1 ? (int)cluster.block_rank() : 0;
     const int64_t rows_at = gridDim.x / per_row, row0 = blockIdx.x / per_row;
-    constexpr int step = kThreads * kN;   // a row's classes are fewer than 2^30: offsets in it fit 32 bits
     const auto row_of = [&](int64_t row) { return static_cast<const T*>(p.x) + row * p.n; };
-    const auto start_of = [&](const T* x) {
-        return (rank * share + (int)threadIdx.x) * kN - Piece<T>::shift_of(x);
-    };
-    const auto end_of = [&](const T* x) {   // of this CTA's share of a row
-        const int64_t e = (int64_t)(rank + 1) * share * kN - Piece<T>::shift_of(x);
+    // The warp's share of a row: `share` accesses from a multiple of it on (a row's
+    // classes are fewer than 2^30: offsets in it fit 32 bits).
+    const int64_t begin = (int64_t)(rank * kWarps + warp) * share * kN;
+    const auto start_of = [&](const T* x) { return (int)(begin < p.n + kN ? begin : p.n + kN) + lane * kN - Piece<T>::shift_of(x); };
+    const auto end_of = [&](const T* x) {
+        const int64_t e = begin + (int64_t)share * kN - Piece<T>::shift_of(x);
         return e < p.n ? (int)e : p.n;
     };
     const auto ahead = [&](int64_t row, int stage) {
@@ -586,40 +626,88 @@ __global__ void __launch_bounds__(kThreads, kThreads == 512 ? 2 : kThreads == 25
             if (first >= 0 && first + (kPieces - 1) * step + kN <= end) {
 #pragma unroll
                 for (int k = 0; k < kPieces; ++k) copy16(to + k * kThreads, x + first + k * step);
-            } else
+            } else {
 #pragma unroll 1
-            for (int k = 0; k < kPieces; ++k, to += kThreads) {
-                const int at = first + k * step;
-                if (at >= 0 && at + kN <= end) {
-                    copy16(to, x + at);
-                } else {
-                    Piece<T> q;
-                    q.load(x, at, end, lo_of<T>(p), hi_of<T>(p));
-                    *to = q.q;
+                for (int k = 0; k < kPieces; ++k, to += kThreads) {
+                    const int at = first + k * step;
+                    if (at >= 0 && at + kN <= end) {
+                        copy16(to, x + at);
+                    } else {
+                        Piece<T> q;
+                        q.load(x, at, end, lo_of<T>(p), hi_of<T>(p));
+                        *to = q.q;
+                    }
                 }
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    // The rows of a batch: row0 + (i0 + i) rows_at.
+    const auto meet = [&] {
+        if (per_row > 1) cluster.sync();
+        else __syncthreads();
+    };
+    // The best of a warp's pieces, and (later rounds) of its list so far, to `out`.
+    const auto best = [&](uint64_t* out, const Piece<T>(&q)[kPieces], const T* x, int first, int end, float own, float m) {
+        if (m < INFINITY && m > -INFINITY && best_by_bound(out, q, first, own, p.top, room[warp], &count[warp])) return;
+        uint64_t before = ~0ull;
+        for (int k = 0; k < p.top; ++k) {
+            before = warp_best(best_below(p, x, (int64_t)first, step, end, before));
+            if (lane == 0) out[k] = before;
+        }
+        __syncwarp();
+    };
+    // The rows of a batch, row0 + (i0 + i) rows_at: one a warp of the cluster.
     const auto finish = [&](int64_t i0, int n) {
-        __syncthreads();
-        if (rank == 0 && warp == 0) {
-            const bool here = lane < n;
-            const Sums t = here ? batch.sums[lane] : Sums{0.f, 0.f, 1};
-            const Row mine(here ? batch.m[lane] : 0.f, t.below, t.equal);
-            const int64_t row = row0 + (i0 + lane) * rows_at;
-            if (here) mine.write(p, row, row_of(row), t, p.logp ? label_of(p, row) : -1);
-            for (int i = 0; i < n * p.top; i += 32) {
-                const int e = i + lane, r = p.top ? e / p.top : 0;
-                const float m = __shfl_sync(0xffffffffu, mine.m, r & 31), s = __shfl_sync(0xffffffffu, mine.s, r & 31);
-                if (e < n * p.top) write_top(p, row0 + (i0 + r) * rows_at, e - r * p.top, best[e], m, s);
+        meet();
+        for (int i = warp * per_row + rank; i < n; i += kWarps * per_row) {
+            const int64_t row = row0 + (i0 + i) * rows_at;
+            const int label = p.logp ? label_of(p, row) : -1;
+            Share all = {-INFINITY, {0.f, 0.f, 0}};
+            for (int k = lane; k < kWarps * per_row; k += 32) {
+                const Share* from = &shares[i][k % kWarps];
+                all.join(per_row > 1 ? *cluster.map_shared_rank(from, k / kWarps) : *from);
+            }
+            // The lanes' shares together, each lane with another's.
+#pragma unroll
+            for (int d = 16; d; d >>= 1) {
+                Share o;
+                o.m = __shfl_xor_sync(0xffffffffu, all.m, d);
+                o.sums.below = __shfl_xor_sync(0xffffffffu, all.sums.below, d);
+                o.sums.weighted = __shfl_xor_sync(0xffffffffu, all.sums.weighted, d);
+                o.sums.equal = __shfl_xor_sync(0xffffffffu, all.sums.equal, d);
+                all.join(o);
+            }
+            const Row done(all.m, all.sums.below, all.sums.equal);
+            if (lane == 0) done.write(p, row, row_of(row), all.sums, label);
+            if constexpr (kTop) {
+                // Lists that fall: the best of all is among their heads.
+                const int many = kWarps * per_row;
+                const uint64_t* from[4];
+                uint64_t head[4];
+                int taken[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int k = lane + 32 * u;
+                    from[u] = lists + (i * kWarps + k % kWarps) * p.top;
+                    if (per_row > 1 && k < many) from[u] = cluster.map_shared_rank(from[u], k / kWarps);
+                    head[u] = k < many ? from[u][0] : 0;
+                }
+                uint64_t mine = 0;
+                for (int t = 0; t < p.top; ++t) {
+                    uint64_t b = head[0];
+#pragma unroll
+                    for (int u = 1; u < 4; ++u) b = head[u] > b ? head[u] : b;
+                    b = warp_best(b);
+                    if (lane == t) mine = b;
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)
+                        if (head[u] == b && b) head[u] = ++taken[u] < p.top ? from[u][taken[u]] : 0;   // keys differ: one list
+                }
+                if (lane < p.top) write_top(p, row, lane, mine, done.m, done.s);
             }
         }
-        __syncthreads();
+        meet();
     };
-    if (threadIdx.x < 2) count[threadIdx.x] = 0;
-    __syncthreads();
     if (!kLoop) {
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) ahead(row0 + i * rows_at, i);
@@ -629,17 +717,27 @@ __global__ void __launch_bounds__(kThreads, kThreads == 512 ? 2 : kThreads == 25
     for (int64_t row = row0; row < p.rows; row += rows_at, ++it) {
         const T* x = row_of(row);
         const int start = start_of(x), end = end_of(x);
-        const int buf = (int)(it & 1);
+        uint64_t* out = lists + (held * kWarps + warp) * p.top;
         Piece<T> q[kPieces];
-        const auto load = [&](int round) {
-#pragma unroll
-            for (int k = 0; k < kPieces; ++k) q[k].load(x, start + (round * kPieces + k) * step, end, lo_of<T>(p), hi_of<T>(p));
-        };
-        float own = -INFINITY;
-        if (kLoop) {
+        Share all;
+        if constexpr (kLoop) {
+            all = Share{-INFINITY, {0.f, 0.f, 0}};
             for (int round = 0; round < rounds; ++round) {
-                load(round);
-                own = max_nan(own, Piece<T>::most(q));
+                const int first = start + round * kPieces * step;
+#pragma unroll
+                for (int k = 0; k < kPieces; ++k) q[k].load(x, first + k * step, end, lo_of<T>(p), hi_of<T>(p));
+                const float own = Piece<T>::most(q);
+                Share one;
+                one.m = warp_max(own);
+                one.sums = warp_add_up(q, one.m, own);
+                all.join(one);
+            }
+            if (kTop) {
+                uint64_t before = ~0ull;
+                for (int k = 0; k < p.top; ++k) {
+                    before = warp_best(best_below(p, x, (int64_t)start, step, end, before));
+                    if (lane == 0) out[k] = before;
+                }
             }
         } else {
             constexpr int kSlots = kAhead > 0 ? kAhead : 1;
@@ -648,122 +746,19 @@ __global__ void __launch_bounds__(kThreads, kThreads == 512 ? 2 : kThreads == 25
             const uint4* from = ring + slot * kPieces * kThreads + threadIdx.x;
 #pragma unroll
             for (int k = 0; k < kPieces; ++k) q[k].q = from[k * kThreads];
-            own = Piece<T>::most(q);   // the places have been read
+            const float own = Piece<T>::most(q);   // the places have been read
             ahead(row + kSlots * rows_at, slot);
+            all.m = warp_max(own);
+            if (kTop) best(out, q, x, start, end, own, all.m);
+            all.sums = warp_add_up(q, all.m, own);
         }
-        float m = warp_max(own);
-        if (lane == 0) part_m[buf][warp] = m;
-        if (kTop) {   // the largest of each of 32 neighbouring groups of threads (no NaN there: fmaxf)
-            float v = own;
-#pragma unroll
-            for (int d = 1; d < (kSegment < 32 ? kSegment : 32); d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
-            if (threadIdx.x % kSegment == 0) segment[threadIdx.x / kSegment] = v;
-        }
-        __syncthreads();
-        m = warp_max(part_m[buf][lane % kWarps]);
-        if (per_row > 1) {
-            if (threadIdx.x == 0) cta_m[buf] = m;
-            cluster.sync();
-            m = warp_max(*cluster.map_shared_rank(&cta_m[buf], lane % per_row));
-        }
-        const bool plain = m < INFINITY && m > -INFINITY;
-        if (kTop && threadIdx.x == 0) count[buf ^ 1] = 0;   // of the row before, which all have left
-        bool bounded = false;
-        if (kTop && plain) {   // the same for all threads
-            if (warp == 0) {   // the top-th largest: the largest that as many are not below
-                const float mine = segment[lane];
-                int not_below = 0;
-#pragma unroll
-                for (int i = 0; i < 32; ++i) not_below += segment[i] >= mine;
-                const float bound = warp_max(not_below >= p.top ? mine : -INFINITY);
-                if (lane == 0) bound_at = fmaxf(bound, -3.4028234e38f);   // at least the scores above -inf
-            }
-            __syncthreads();
-            bounded = true;
-        }
-        Sums t = {0.f, 0.f, 0};
-        for (int round = 0; round < (kLoop ? rounds : 1); ++round) {
-            if (kLoop) {
-                load(round);
-                own = Piece<T>::most(q);
-            }
-            if (bounded && own >= bound_at)
-                gather(q, start + round * kPieces * step, step, bound_at, room[buf], &count[buf], kRoom);
-            if (plain) add_up(t, q, m, own);
-        }
-        warp_sums(t.below, t.weighted);
-        t.equal = (int)__reduce_add_sync(0xffffffffu, (unsigned)t.equal);
-        if (lane == 0) part[buf][warp] = t;
-        __syncthreads();
-        uint64_t* out = best + held * p.top;   // of this CTA, where a cluster has several
-        if (kTop) {
-            const int c = count[buf];
-            if (bounded && c <= kRoom && c >= (per_row > 1 && end <= start - threadIdx.x * kN ? 0 : p.top)) {
-                if (warp == 0) {
-                    if (lane < p.top) out[lane] = 0;   // a share may have fewer
-                    __syncwarp();
-                    in_order(out, room[buf], c, p.top);
-                }
-            } else {
-                uint64_t before = ~0ull;
-                for (int k = 0; k < p.top; ++k) {
-                    uint64_t b = best_below(p, x, (int64_t)start, step, end, before);
-                    b = warp_best(b);
-                    __syncthreads();
-                    if (lane == 0) merged[warp] = b;
-                    __syncthreads();
-                    before = warp_best(merged[lane % kWarps]);
-                    if (threadIdx.x == 0) out[k] = before;
-                }
-            }
-        }
-        if (warp == kWarps - 1) {
-            Sums all = lane < kWarps ? part[buf][lane] : Sums{0.f, 0.f, 0};
-            warp_sums(all.below, all.weighted);
-            all.equal = (int)__reduce_add_sync(0xffffffffu, (unsigned)all.equal);
-            if (lane == 0) {
-                if (per_row > 1) {
-                    cta[buf] = all;
-                } else {
-                    batch.m[held] = m;
-                    batch.sums[held] = all;
-                }
-            }
-        }
-        if (per_row > 1) {
-            cluster.sync();
-            if (rank == 0 && warp == 0) {
-                Sums all = lane < per_row ? *cluster.map_shared_rank(&cta[buf], lane % per_row) : Sums{0.f, 0.f, 0};
-                warp_sums(all.below, all.weighted);
-                all.equal = (int)__reduce_add_sync(0xffffffffu, (unsigned)all.equal);
-                if (lane == 0) {
-                    batch.m[held] = m;
-                    batch.sums[held] = all;
-                }
-                if (kTop) {
-                    for (int c = 0; c < per_row; ++c)
-                        if (lane < p.top) merged[c * p.top + lane] = *cluster.map_shared_rank(out + lane, c);
-                    __syncwarp();
-                    int n = 0;   // keys that are there, close together
-                    for (int i = lane; i < (per_row * p.top + 31) / 32 * 32; i += 32) {
-                        const uint64_t v = i < per_row * p.top ? merged[i] : 0;
-                        const unsigned there = __ballot_sync(0xffffffffu, v != 0);
-                        if (v) merged[n + __popc(there & ((1u << lane) - 1))] = v;
-                        n += __popc(there);
-                        __syncwarp();
-                    }
-                    in_order(out, merged, n, p.top);
-                }
-            }
-            if (kTop) cluster.sync();   // the others' lists have been read
-        }
-        if (++held == kBatch) {
+        if (lane == 0) shares[held][warp] = all;
+        if (++held == kRows) {
             finish(it - held + 1, held);
             held = 0;
         }
     }
     if (held) finish(it - held, held);
-    if (per_row > 1) cluster.sync();   // what is shared outlives its readers
 }
 
 // ------------------------------------------------------------- few classes
@@ -1084,14 +1079,14 @@ static unsigned grid_of(int64_t ctas) { return (unsigned)(ctas < (1 << 30) ? cta
 template <typename T, int kThreads, int kPieces, int kAhead, bool kTop>
 static cudaError_t launch_ctas(const LogpArgs& a, int64_t nv, int per_row, cudaStream_t s) {
     const auto kernel = k_logp_ctas<T, kThreads, kPieces, kAhead, kTop>;
-    constexpr int kRing = kAhead * kPieces * kThreads * 16;
-    const int share = (int)ceil_div(nv, per_row);
+    constexpr int kRing = kAhead * kPieces * kThreads * 16, kLists = kTop ? kTopBatch * (kThreads / 32) * 8 : 0;   // keys: times top
+    const int share = (int)ceil_div(ceil_div(nv, per_row * (kThreads / 32)), 32) * 32;   // accesses of a warp
     int resident = 0;
     const cudaError_t e = pl::kernel_once(
         reinterpret_cast<const void*>(kernel),
         [](int* n) {
             const auto k = k_logp_ctas<T, kThreads, kPieces, kAhead, kTop>;
-            const int most = kRing + (kTop ? kBatch * PLATTICE_MAX_TOP * 8 : 0);
+            const int most = kRing + kLists * PLATTICE_MAX_TOP;
             const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
             return e != cudaSuccess ? e : cudaOccupancyMaxActiveBlocksPerMultiprocessor(n, k, kThreads, most);
         },
@@ -1103,7 +1098,7 @@ static cudaError_t launch_ctas(const LogpArgs& a, int64_t nv, int per_row, cudaS
     cudaLaunchConfig_t c = {};
     c.gridDim = dim3((unsigned)(rows * per_row));
     c.blockDim = dim3(kThreads);
-    c.dynamicSmemBytes = kRing + (size_t)kBatch * a.top * 8;
+    c.dynamicSmemBytes = kRing + (size_t)kLists * a.top;
     c.stream = s;
     cudaLaunchAttribute attr = {};
     attr.id = cudaLaunchAttributeClusterDimension;
@@ -1111,7 +1106,7 @@ static cudaError_t launch_ctas(const LogpArgs& a, int64_t nv, int per_row, cudaS
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     c.attrs = &attr;
     c.numAttrs = per_row > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&c, kernel, a, share, (int)ceil_div(share, kPieces * kThreads), per_row);
+    return cudaLaunchKernelEx(&c, kernel, a, share, (int)ceil_div(share, kPieces * 32), per_row);
 }
 
 template <typename T, int kThreads, int kPieces, int kAhead>
