@@ -322,26 +322,97 @@ __device__ __forceinline__ void in_order(uint64_t* out, const uint64_t* keys, in
     }
 }
 
-// The scores that are at least `bound`, anywhere in a thread's pieces (element i of
-// piece k is class first + k step + i), go to `room` in any order: the keys differ.
-template <typename T, int K>
-__device__ __forceinline__ void gather(const Piece<T> (&q)[K], int64_t first, int64_t step, float bound, uint64_t* room, int* count,
-                                       int most) {
-    constexpr int kN = Piece<T>::kN;
+constexpr int kWarpRoom = 96;   // candidates of a warp, and a list so far
+
+// Bits of a lane's scores that are at least `bound` (closed places are not).
+template <typename T, int K> struct Hits {
+    static constexpr int kN = Piece<T>::kN;
+    static_assert(4 * K <= 32, "two masks of 16 words");
+    uint32_t lo = 0, hi = 0;   // 16-bit: words 0-15, 16-31, a bit of each half for either element of a word
+    __device__ __forceinline__ Hits(const Piece<T> (&q)[K], float bound) {
+        if constexpr (sizeof(T) == 2) {
+            typedef typename Pair<T>::type P;
+            P at;
+            pair_from(at, bound, bound);
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-        if (!(q[k].most() >= bound)) continue;
-#pragma unroll
-        for (int i = 0; i < kN; ++i) {
-            const float2 f = q[k].pair(i / 2);
-            const float x = i % 2 ? f.y : f.x;
-            if (x >= bound) {
-                const int at = atomicAdd(count, 1);
-                if (at < most) room[at] = ranked(x, first + k * step + i);
+            for (int w = 0; w < 4 * K; ++w) {
+                const uint32_t v = q[w / 4].word(w % 4);
+                const uint32_t bits = __hge2_mask(*reinterpret_cast<const P*>(&v), at) & (0x10001u << (w & 15));
+                if (w < 16) lo |= bits;
+                else hi |= bits;
             }
+        } else {
+#pragma unroll
+            for (int w = 0; w < 4 * K; ++w) lo |= (__uint_as_float(q[w / 4].word(w % 4)) >= bound ? 1u : 0u) << w;
         }
     }
+    __device__ __forceinline__ bool some() const { return (lo | hi) != 0; }
+    // One of them, taken out: element kN k + i.
+    __device__ __forceinline__ int next() {
+        if constexpr (sizeof(T) == 4) {
+            const int b = __ffs(lo) - 1;
+            lo &= lo - 1;
+            return b;
+        }
+        const bool low = lo != 0;
+        const uint32_t m = low ? lo : hi;
+        const int b = __ffs(m) - 1;
+        if (low) lo &= lo - 1;
+        else hi &= hi - 1;
+        return ((b & 15) + (low ? 0 : 16)) * 2 + (b >> 4);
+    }
+};
+
+// The best by a bound: the scores that are at least the top-th largest of the
+// lanes' largest ones hold them, and mostly they are few more.  With the list so far
+// (null: none) in order to `out`; false where they are too many or too few.
+// fetch(e): the lane's element e; element kN k + i is class first + k step + i.
+template <typename T, int K, typename F>
+__device__ __forceinline__ bool best_by_bound(uint64_t* out, const uint64_t* list, const Piece<T> (&q)[K], int first, int step, float own,
+                                              int top, uint64_t* room, const F& fetch) {
+    constexpr int kN = Piece<T>::kN;
+    const int lane = threadIdx.x & 31;
+    float bound = 0.f, v = own;
+    for (int k = 0; k < top; ++k) {
+        bound = warp_max(v);
+        const unsigned at = __ballot_sync(0xffffffffu, v == bound);
+        if (lane == __ffs(at) - 1) v = -INFINITY;
+    }
+    bound = fmaxf(bound, sizeof(T) == 4 ? -3.4028234e38f : std::is_same<T, __half>::value ? -65504.f : -3.3895314e38f);   // not -inf
+    Hits<T, K> hits(q, bound);
+    int count = 0;
+    for (;;) {
+        const bool some = hits.some();
+        const unsigned at = __ballot_sync(0xffffffffu, some);
+        if (!at || count > kWarpRoom) break;
+        if (some) {
+            const int e = hits.next(), to = count + __popc(at & ((1u << lane) - 1));
+            if (to < kWarpRoom) room[to] = ranked(fetch(e), first + e / kN * step + e % kN);
+        }
+        count += __popc(at);
+    }
+    const int old = list ? top : 0;
+    if (count + old > kWarpRoom || count + old < top) return false;
+    if (lane < old) room[count + lane] = list[lane];
+    __syncwarp();
+    in_order(out, room, count + old, top);
+    __syncwarp();
+    return true;
 }
+
+// A lane's element e out of its registers.
+template <typename T, int K> struct FromRegisters {
+    const Piece<T> (&q)[K];
+    __device__ __forceinline__ float operator()(int e) const {
+        uint32_t w = q[0].word(0);
+        const int at = sizeof(T) == 2 ? e / 2 : e;
+#pragma unroll
+        for (int i = 1; i < 4 * K; ++i) w = at == i ? q[i / 4].word(i % 4) : w;
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w);
+        const uint16_t h = (uint16_t)(e % 2 ? w >> 16 : w);
+        return to_f32(*reinterpret_cast<const T*>(&h));
+    }
+};
 
 // The best key below `before` of the pieces first, first + step, .. < end of a row,
 // read again: for rows whose scores are so alike (or so many -inf) that no bound
@@ -377,11 +448,12 @@ __device__ __forceinline__ void write_top(const LogpArgs& p, int64_t row, int pl
 // them are made together at the end (one by one they cost more than the
 // exponentials of 256 classes).
 
-constexpr int kWarpRows = 32, kWarpRoom = 64;
+constexpr int kWarpRows = 32;
 
 // The best of 16-bit scores: class and score make a key of 32 bits, whose largest
 // of the warp is one instruction; a lane's next largest is that of key - taken
-// (mod 2^32, where those that were taken are smallest).
+// (mod 2^32, where those that were taken are smallest).  Up to two accesses a lane: 262144 x 256, 4 alternatives, 103 us,
+// 120 by the bound above.
 template <typename T, int K, bool kWhole>
 __device__ __forceinline__ void best_of_16(uint64_t* out, const Piece<T> (&q)[K], int first, int n, int top) {
     typedef typename Pair<T>::type P;
@@ -425,34 +497,9 @@ __device__ __forceinline__ void best_of_16(uint64_t* out, const Piece<T> (&q)[K]
     }
 }
 
-// The best by a bound: the scores that are at least the top-th largest of the
-// lanes' largest ones hold them; mostly they are few more.  False where not.
-template <typename T, int K>
-__device__ __forceinline__ bool best_by_bound(uint64_t* out, const Piece<T> (&q)[K], int first, float own, int top, uint64_t* room,
-                                              int* count) {
-    const int lane = threadIdx.x & 31;
-    float bound = 0.f, v = own;
-    for (int k = 0; k < top; ++k) {
-        bound = warp_max(v);
-        const unsigned at = __ballot_sync(0xffffffffu, v == bound);
-        if (lane == __ffs(at) - 1) v = -INFINITY;
-    }
-    bound = fmaxf(bound, -3.4028234e38f);   // at least the scores above -inf
-    if (lane == 0) *count = 0;
-    __syncwarp();
-    if (own >= bound) gather(q, first, 32 * Piece<T>::kN, bound, room, count, kWarpRoom);
-    __syncwarp();
-    const int c = *count;
-    const bool done = c >= top && c <= kWarpRoom;
-    if (done) in_order(out, room, c, top);
-    __syncwarp();
-    return done;
-}
-
 template <typename T, int K, bool kTop, bool kWhole>
 __global__ void __launch_bounds__(128) k_logp_warp(const __grid_constant__ LogpArgs p, int rows_each) {
     __shared__ uint64_t room[4][kWarpRoom];
-    __shared__ int count[4];
     extern __shared__ uint64_t staged[];   // [4][rows_each][top]
     constexpr int kN = Piece<T>::kN;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = p.n;
@@ -488,10 +535,10 @@ __global__ void __launch_bounds__(128) k_logp_warp(const __grid_constant__ LogpA
             const bool plain = m < INFINITY && m > -INFINITY;
             if (kTop) {
                 uint64_t* out = best + r * p.top;
-                bool done = false;
+                bool done = plain;
                 if (plain) {
-                    if constexpr (sizeof(T) == 2 && K <= 2) best_of_16<T, K, kWhole>(out, q, first, n, p.top), done = true;
-                    else done = best_by_bound(out, q, first, own, p.top, room[warp], &count[warp]);
+                    if constexpr (sizeof(T) == 2 && K <= 2) best_of_16<T, K, kWhole>(out, q, first, n, p.top);
+                    else done = best_by_bound(out, nullptr, q, first, 32 * kN, own, p.top, room[warp], FromRegisters<T, K>{q});
                 }
                 if (!done) {
                     uint64_t before = ~0ull;
@@ -603,8 +650,8 @@ __global__ void __launch_bounds__(kThreads, kThreads == 512 ? 2 : kThreads == 25
     constexpr int kWarps = kThreads / 32, kN = Piece<T>::kN, step = 32 * kN, kRows = kTop ? kTopBatch : kBatch;
     extern __shared__ uint4 ring[];   // [kAhead][kPieces][kThreads], then keys [kRows][kWarps][top]
     __shared__ uint64_t room[kTop ? kWarps : 1][kWarpRoom];
-    __shared__ int count[kWarps];
     __shared__ Share shares[kRows][kWarps];
+    __shared__ float2 stats[kTop ? kRows : 1];
     uint64_t* lists = reinterpret_cast<uint64_t*>(ring + kAhead * kPieces * kThreads);
     const cg::cluster_group cluster = cg::this_cluster();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rank = per_row > 1 ? (int)cluster.block_rank() : 0;
@@ -646,9 +693,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 512 ? 2 : kThreads == 25
         if (per_row > 1) cluster.sync();
         else __syncthreads();
     };
-    // The best of a warp's pieces, and (later rounds) of its list so far, to `out`.
-    const auto best = [&](uint64_t* out, const Piece<T>(&q)[kPieces], const T* x, int first, int end, float own, float m) {
-        if (m < INFINITY && m > -INFINITY && best_by_bound(out, q, first, own, p.top, room[warp], &count[warp])) return;
+    const auto best_slowly = [&](uint64_t* out, const T* x, int first, int end) {
         uint64_t before = ~0ull;
         for (int k = 0; k < p.top; ++k) {
             before = warp_best(best_below(p, x, (int64_t)first, step, end, before));
@@ -656,30 +701,43 @@ __global__ void __launch_bounds__(kThreads, kThreads == 512 ? 2 : kThreads == 25
         }
         __syncwarp();
     };
-    // The rows of a batch, row0 + (i0 + i) rows_at: one a warp of the cluster.
+    // The rows of a batch, row0 + (i0 + i) rows_at, every per_row-th of which is this CTA's:
+    // a warp a row where there are enough, else a lane a row.  Then the alternatives, a warp a row.
     const auto finish = [&](int64_t i0, int n) {
         meet();
-        for (int i = warp * per_row + rank; i < n; i += kWarps * per_row) {
-            const int64_t row = row0 + (i0 + i) * rows_at;
-            const int label = p.logp ? label_of(p, row) : -1;
-            Share all = {-INFINITY, {0.f, 0.f, 0}};
-            for (int k = lane; k < kWarps * per_row; k += 32) {
-                const Share* from = &shares[i][k % kWarps];
-                all.join(per_row > 1 ? *cluster.map_shared_rank(from, k / kWarps) : *from);
-            }
-            // The lanes' shares together, each lane with another's.
+        const bool wide = n <= kWarps * per_row;
+        if (wide || warp == 0) {
+            const int i = (wide ? warp : lane) * per_row + rank;
+            if (i < n) {
+                const int64_t row = row0 + (i0 + i) * rows_at;
+                const int label = p.logp ? label_of(p, row) : -1;
+                Share all = {-INFINITY, {0.f, 0.f, 0}};
+#pragma unroll 4
+                for (int k = wide ? lane : 0; k < kWarps * per_row; k += wide ? 32 : 1) {
+                    const Share* from = &shares[i][k % kWarps];
+                    all.join(per_row > 1 ? *cluster.map_shared_rank(from, k / kWarps) : *from);
+                }
+                if (wide) {
 #pragma unroll
-            for (int d = 16; d; d >>= 1) {
-                Share o;
-                o.m = __shfl_xor_sync(0xffffffffu, all.m, d);
-                o.sums.below = __shfl_xor_sync(0xffffffffu, all.sums.below, d);
-                o.sums.weighted = __shfl_xor_sync(0xffffffffu, all.sums.weighted, d);
-                o.sums.equal = __shfl_xor_sync(0xffffffffu, all.sums.equal, d);
-                all.join(o);
+                    for (int d = 16; d; d >>= 1) {
+                        Share o;
+                        o.m = __shfl_xor_sync(0xffffffffu, all.m, d);
+                        o.sums.below = __shfl_xor_sync(0xffffffffu, all.sums.below, d);
+                        o.sums.weighted = __shfl_xor_sync(0xffffffffu, all.sums.weighted, d);
+                        o.sums.equal = __shfl_xor_sync(0xffffffffu, all.sums.equal, d);
+                        all.join(o);
+                    }
+                }
+                const Row done(all.m, all.sums.below, all.sums.equal);
+                if (!wide || lane == 0) {
+                    done.write(p, row, row_of(row), all.sums, label);
+                    if (kTop) stats[i] = make_float2(done.m, done.s);
+                }
             }
-            const Row done(all.m, all.sums.below, all.sums.equal);
-            if (lane == 0) done.write(p, row, row_of(row), all.sums, label);
-            if constexpr (kTop) {
+        }
+        if constexpr (kTop) {
+            __syncthreads();
+            for (int i = warp * per_row + rank; i < n; i += kWarps * per_row) {
                 // Lists that fall: the best of all is among their heads.
                 const int many = kWarps * per_row;
                 const uint64_t* from[4];
@@ -703,7 +761,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 512 ? 2 : kThreads == 25
                     for (int u = 0; u < 4; ++u)
                         if (head[u] == b && b) head[u] = ++taken[u] < p.top ? from[u][taken[u]] : 0;   // keys differ: one list
                 }
-                if (lane < p.top) write_top(p, row, lane, mine, done.m, done.s);
+                if (lane < p.top) write_top(p, row0 + (i0 + i) * rows_at, lane, mine, stats[i].x, stats[i].y);
             }
         }
         meet();
@@ -722,6 +780,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 512 ? 2 : kThreads == 25
         Share all;
         if constexpr (kLoop) {
             all = Share{-INFINITY, {0.f, 0.f, 0}};
+            bool listed = kTop;
             for (int round = 0; round < rounds; ++round) {
                 const int first = start + round * kPieces * step;
 #pragma unroll
@@ -729,16 +788,13 @@ __global__ void __launch_bounds__(kThreads, kThreads == 512 ? 2 : kThreads == 25
                 const float own = Piece<T>::most(q);
                 Share one;
                 one.m = warp_max(own);
+                if (listed && !(round && one.m == -INFINITY))
+                    listed = one.m < INFINITY && best_by_bound(out, round ? out : nullptr, q, first, step, own, p.top, room[warp],
+                                                               FromRegisters<T, kPieces>{q});
                 one.sums = warp_add_up(q, one.m, own);
                 all.join(one);
             }
-            if (kTop) {
-                uint64_t before = ~0ull;
-                for (int k = 0; k < p.top; ++k) {
-                    before = warp_best(best_below(p, x, (int64_t)start, step, end, before));
-                    if (lane == 0) out[k] = before;
-                }
-            }
+            if (kTop && !listed) best_slowly(out, x, start, end);
         } else {
             constexpr int kSlots = kAhead > 0 ? kAhead : 1;
             const int slot = (int)(it % kSlots);
@@ -746,10 +802,15 @@ __global__ void __launch_bounds__(kThreads, kThreads == 512 ? 2 : kThreads == 25
             const uint4* from = ring + slot * kPieces * kThreads + threadIdx.x;
 #pragma unroll
             for (int k = 0; k < kPieces; ++k) q[k].q = from[k * kThreads];
-            const float own = Piece<T>::most(q);   // the places have been read
-            ahead(row + kSlots * rows_at, slot);
+            const float own = Piece<T>::most(q);
             all.m = warp_max(own);
-            if (kTop) best(out, q, x, start, end, own, all.m);
+            if (kTop) {
+                const auto fetch = [&](int e) { return to_f32(reinterpret_cast<const T*>(from + e / kN * kThreads)[e % kN]); };
+                if (!(all.m < INFINITY && all.m > -INFINITY) ||
+                    !best_by_bound(out, nullptr, q, start, step, own, p.top, room[warp], fetch))
+                    best_slowly(out, x, start, end);
+            }
+            ahead(row + kSlots * rows_at, slot);   // the places have been read
             all.sums = warp_add_up(q, all.m, own);
         }
         if (lane == 0) shares[held][warp] = all;
@@ -1081,24 +1142,25 @@ static cudaError_t launch_ctas(const LogpArgs& a, int64_t nv, int per_row, cudaS
     const auto kernel = k_logp_ctas<T, kThreads, kPieces, kAhead, kTop>;
     constexpr int kRing = kAhead * kPieces * kThreads * 16, kLists = kTop ? kTopBatch * (kThreads / 32) * 8 : 0;   // keys: times top
     const int share = (int)ceil_div(ceil_div(nv, per_row * (kThreads / 32)), 32) * 32;   // accesses of a warp
-    int resident = 0;
-    const cudaError_t e = pl::kernel_once(
+    const size_t smem = kRing + (size_t)kLists * a.top;
+    int resident = 1;
+    cudaError_t e = pl::kernel_once(
         reinterpret_cast<const void*>(kernel),
-        [](int* n) {
-            const auto k = k_logp_ctas<T, kThreads, kPieces, kAhead, kTop>;
-            const int most = kRing + kLists * PLATTICE_MAX_TOP;
-            const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
-            return e != cudaSuccess ? e : cudaOccupancyMaxActiveBlocksPerMultiprocessor(n, k, kThreads, most);
+        [](int*) {
+            return cudaFuncSetAttribute(k_logp_ctas<T, kThreads, kPieces, kAhead, kTop>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        kRing + kLists * PLATTICE_MAX_TOP);
         },
         &resident);
+    if (e == cudaSuccess && a.rows * per_row > sm_count())
+        e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kernel, kThreads, smem);
     if (e != cudaSuccess) return e;
-    int64_t rows = (int64_t)(resident > 0 ? resident : 1) * sm_count() / per_row;
+    int64_t rows = (int64_t)(resident > 0 ? resident : 1) * sm_count() / per_row;   // few rows: one CTA an SM, at most
     if (rows < 1) rows = 1;
     if (rows > a.rows) rows = a.rows;
     cudaLaunchConfig_t c = {};
     c.gridDim = dim3((unsigned)(rows * per_row));
     c.blockDim = dim3(kThreads);
-    c.dynamicSmemBytes = kRing + (size_t)kLists * a.top;
+    c.dynamicSmemBytes = smem;
     c.stream = s;
     cudaLaunchAttribute attr = {};
     attr.id = cudaLaunchAttributeClusterDimension;
