@@ -31,7 +31,7 @@ template <int kTensors> struct Grads {
     uint8_t type[kTensors];       // dtype | out_dtype << 2 | aligned << 4
     int count;
 };
-constexpr int kMost = 256, kSome = 16;   // tensors of one launch; of a small one's table
+constexpr int kMost = 256, kSome = 64;   // tensors of one launch; of a small one's table
 constexpr int kResident = 6;             // CTAs of an SM: one round
 
 // The tensor of a piece: the first whose end is above it.
@@ -103,16 +103,16 @@ __device__ __forceinline__ double cta_sum(double v) {
     return v;
 }
 
-// Where a piece lies; `tensor` where it is known.
-struct At {
+// Where a piece of kSize values lies; `tensor` where it is known.
+template <int kSize = kPiece> struct At {
     int tensor, n, dtype;
     long long first;
     bool aligned, wide;
     template <int N> __device__ __forceinline__ At(const Grads<N>& t, long long piece) : At(t, piece, tensor_of(t, piece)) {}
     template <int N> __device__ __forceinline__ At(const Grads<N>& t, long long piece, int tensor_) : tensor(tensor_) {
-        first = (piece - (tensor ? t.end[tensor - 1] : 0)) * kPiece;
+        first = (piece - (tensor ? t.end[tensor - 1] : 0)) * kSize;
         const long long left = t.size[tensor] - first;
-        n = left < kPiece ? (int)left : kPiece;
+        n = left < kSize ? (int)left : kSize;
         const int type = t.type[tensor];
         dtype = type & 3;
         wide = ((type >> 2) & 3) == PLATTICE_F32;
@@ -130,7 +130,7 @@ struct Share {
     }
 };
 
-template <int N> __device__ __forceinline__ double squares_at(const Grads<N>& t, const At& p) {
+template <int N> __device__ __forceinline__ double squares_at(const Grads<N>& t, const At<>& p) {
     const void* g = t.g[p.tensor];
     if (p.dtype == PLATTICE_F32) return piece_squares(static_cast<const float*>(g) + p.first, p.n, p.aligned);
     if (p.dtype == PLATTICE_BF16) return piece_squares(static_cast<const __nv_bfloat16*>(g) + p.first, p.n, p.aligned);
@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(256, kResident) k_square_sums(const __grid_con
     int tensor = s.first < s.end ? tensor_of(t, s.first) : 0;
     for (long long p = s.first; p < s.end; ++p) {
         while (t.end[tensor] <= p) ++tensor;
-        sum += squares_at(t, At(t, p, tensor));
+        sum += squares_at(t, At<>(t, p, tensor));
     }
     sum = cta_sum(sum);
     if (threadIdx.x == 0) sums[blockIdx.x] = sum;
@@ -217,7 +217,7 @@ __device__ __forceinline__ void piece_scale(O* out, const T* g, int n, bool alig
     }
 }
 
-template <int N> __device__ __forceinline__ void scale_at(const Grads<N>& t, const At& p, float f) {
+template <int N> __device__ __forceinline__ void scale_at(const Grads<N>& t, const At<>& p, float f) {
     const void* g = t.g[p.tensor];
     void* out = t.out[p.tensor];
     if (f == 1.f && g == out) return;   // in place, as it is
@@ -248,19 +248,49 @@ __global__ void __launch_bounds__(256, kResident) k_clip(const __grid_constant__
     int tensor = s.first < s.end ? tensor_of(t, s.end - 1) : 0;
     for (long long p = s.end - 1; p >= s.first; --p) {
         while (tensor && t.end[tensor - 1] > p) --tensor;
-        scale_at(t, At(t, p, tensor), f);
+        scale_at(t, At<>(t, p, tensor), f);
     }
 }
 
-// Few pieces: one cluster of kFew CTAs does both, without a second launch.
-constexpr int kFew = 8;
+// Few values: one cluster of kFew CTAs does both, without a second launch, a warp for
+// each piece of kSmallPiece values.
+constexpr int kFew = 8, kSmallPiece = 1024, kFewPieces = 192;
+
+template <typename T>
+__device__ __forceinline__ double warp_squares(const T* g, int n) {
+    double sum = 0.0;
+    for (int i = threadIdx.x & 31; i < n; i += 256) {
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = i + k * 32 < n ? to_f32(g[i + k * 32]) : 0.f;
+        sum += squares(v);
+    }
+    return sum;
+}
+template <typename T, typename O>
+__device__ __forceinline__ void warp_scale(O* out, const T* g, int n, float f) {
+    for (int i = threadIdx.x & 31; i < n; i += 256) {
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = i + k * 32 < n ? to_f32(g[i + k * 32]) : 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (i + k * 32 < n) out[i + k * 32] = from_f32<O>(v[k] * f);
+    }
+}
 
 __global__ void __cluster_dims__(kFew) __launch_bounds__(256) k_clip_few(const __grid_constant__ Grads<kSome> t, Norm q) {
     __shared__ double own;
     const cg::cluster_group cluster = cg::this_cluster();
-    const long long pieces = t.count ? t.end[t.count - 1] : 0;
+    const int pieces = t.count ? (int)t.end[t.count - 1] : 0, first = blockIdx.x + kFew * (threadIdx.x >> 5), step = kFew * 8;
     double sum = 0.0;
-    for (long long p = blockIdx.x; p < pieces; p += kFew) sum += squares_at(t, At(t, p));
+    for (int p = first; p < pieces; p += step) {
+        const At<kSmallPiece> at(t, p);
+        const void* g = t.g[at.tensor];
+        if (at.dtype == PLATTICE_F32) sum += warp_squares(static_cast<const float*>(g) + at.first, at.n);
+        else if (at.dtype == PLATTICE_BF16) sum += warp_squares(static_cast<const __nv_bfloat16*>(g) + at.first, at.n);
+        else sum += warp_squares(static_cast<const __half*>(g) + at.first, at.n);
+    }
     sum = cta_sum(sum);
     if (threadIdx.x == 0) own = sum;
     cluster.sync();
@@ -271,8 +301,20 @@ __global__ void __cluster_dims__(kFew) __launch_bounds__(256) k_clip_few(const _
     const double norm = sqrt(sum);
     if (blockIdx.x == 0 && threadIdx.x == 0 && q.out) *q.out = (float)norm;
     const float f = factor_of(q, norm);
-    if (t.count && t.out[0])
-        for (long long p = blockIdx.x; p < pieces; p += kFew) scale_at(t, At(t, p), f);
+    if (!t.count || !t.out[0]) return;
+    for (int p = first; p < pieces; p += step) {
+        const At<kSmallPiece> at(t, p);
+        const void* g = t.g[at.tensor];
+        void* out = t.out[at.tensor];
+        if (f == 1.f && g == out) continue;   // in place, as it is
+        if (at.dtype == PLATTICE_F32) warp_scale(static_cast<float*>(out) + at.first, static_cast<const float*>(g) + at.first, at.n, f);
+        else if (at.dtype == PLATTICE_BF16 && at.wide)
+            warp_scale(static_cast<float*>(out) + at.first, static_cast<const __nv_bfloat16*>(g) + at.first, at.n, f);
+        else if (at.dtype == PLATTICE_BF16)
+            warp_scale(static_cast<__nv_bfloat16*>(out) + at.first, static_cast<const __nv_bfloat16*>(g) + at.first, at.n, f);
+        else if (at.wide) warp_scale(static_cast<float*>(out) + at.first, static_cast<const __half*>(g) + at.first, at.n, f);
+        else warp_scale(static_cast<__half*>(out) + at.first, static_cast<const __half*>(g) + at.first, at.n, f);
+    }
 }
 
 // ------------------------------------------------------------------ host side
@@ -280,7 +322,7 @@ __global__ void __cluster_dims__(kFew) __launch_bounds__(256) k_clip_few(const _
 static int most_ctas() { return kResident * sm_count(); }
 
 // Fills a launch's table from grads[first..]; gives the first that did not fit.
-template <int N> static int fill(Grads<N>& t, const plattice_grad* grads, int first, int count, long long* pieces) {
+template <int N> static int fill(Grads<N>& t, const plattice_grad* grads, int first, int count, long long* pieces, int size = kPiece) {
     t.count = 0;
     *pieces = 0;
     for (; first < count && t.count < N; ++first) {
@@ -290,7 +332,7 @@ template <int N> static int fill(Grads<N>& t, const plattice_grad* grads, int fi
         t.g[k] = g.g;
         t.out[k] = g.out;
         t.size[k] = g.size;
-        *pieces += ceil_div(g.size, kPiece);
+        *pieces += ceil_div(g.size, size);
         t.end[k] = *pieces;
         t.type[k] = (uint8_t)(g.dtype | g.out_dtype << 2 | (aligned16(g.g) && aligned16(g.out) ? 16 : 0));
     }
@@ -390,12 +432,12 @@ int plattice_clip_grads(const plattice_grad* grads, int count, float max_norm, f
     if (!norm_in && (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < need)) return PLATTICE_ERR_WORKSPACE;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     long long pieces = 0;
-    for (int i = 0; i < count; ++i) pieces += ceil_div(grads[i].size, kPiece);
+    for (int i = 0; i < count; ++i) pieces += ceil_div(grads[i].size, kSmallPiece);
     Norm q{norm_in ? nullptr : static_cast<double*>(workspace), 0, norm_in, norm_out, max_norm, eps};
     cudaError_t e = cudaSuccess;
-    if (!norm_in && pieces <= 2 * kFew && tensors <= kSome) {
+    if (!norm_in && pieces <= kFewPieces && tensors <= kSome) {
         Grads<kSome> t;
-        fill(t, grads, 0, count, &pieces);
+        fill(t, grads, 0, count, &pieces, kSmallPiece);
         k_clip_few<<<kFew, 256, 0, s>>>(t, q);
         return rows_status(cudaGetLastError(), "plattice_clip_grads");
     }

@@ -7,7 +7,7 @@
 // memory as the rows come: every warp has a copy of some of the table's channels of
 // its own, CTAs' sums are added by a second kernel.  For a larger table the
 // positions are sorted by label (by counting smaller ones, or a stable radix sort,
-// 8 bits of the label a pass), the sorted list is cut into chunks of equal length
+// 8 to 10 bits of the label a pass), the sorted list is cut into chunks of equal length
 // and each chunk's runs of equal labels are added in registers.  A run inside one
 // chunk is written at once; the parts of a run that crosses chunks go to the
 // workspace and are added in order by another kernel.  The order of the sums
@@ -48,6 +48,42 @@ __global__ void __launch_bounds__(256) k_embed(T* __restrict__ y, Labels ids, co
                 v[u].from(f);
                 v[u].store(to);
             }
+    }
+}
+
+// Rows that allow no whole accesses: a thread writes 16 bytes of the result, which lies
+// in one stretch, whatever rows they belong to, from table elements one by one
+// (1039280 x 55 bfloat16: 124 us with an element a thread).
+template <typename T>
+__global__ void __launch_bounds__(256) k_embed_flat(T* __restrict__ y, Labels ids, const T* __restrict__ table, float scale, int64_t all,
+                                                    int64_t n, unsigned c) {
+    constexpr int kN = 16 / (int)sizeof(T);
+    const int64_t base = (int64_t)blockIdx.x * (256 * kN);
+    const GroupAt where(base, c);
+    const unsigned o = threadIdx.x * kN;
+    if (base + o >= all) return;
+    int64_t row;
+    unsigned col;
+    where.at(o, row, col);
+    int id = ids.at(row, n);
+    float f[kN];
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+        f[i] = id >= 0 && base + o + i < all ? to_f32(table[(int64_t)id * c + col]) * scale : 0.f;
+        if (++col == c && base + o + i + 1 < all) {
+            col = 0;
+            id = ids.at(++row, n);
+        }
+    }
+    T* to = y + base + o;
+    if (base + o + kN <= all) {
+        Vec<T, kN> v;
+        v.from(f);
+        v.store(to);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kN; ++i)
+            if (base + o + i < all) to[i] = from_f32<T>(f[i]);
     }
 }
 
@@ -217,7 +253,7 @@ __global__ void __launch_bounds__(256) k_small_join(void* out, int dtype, const 
 
 // --------------------------------------------------------------- sorting labels
 
-constexpr int kDigits = 256;
+constexpr int kMostBits = 10;       // of a label, a pass
 constexpr int kRankSorted = 8192;   // as many are sorted by counting
 
 struct Entry { unsigned label, at; };   // at: the position in ids
@@ -232,29 +268,29 @@ struct Zeros {
     __device__ __forceinline__ void share(int cta) const {
         const int64_t each = (end - begin + ctas - 1) / ctas, from = begin + cta * each, to = from + each < end ? from + each : end;
 #pragma unroll 4
-        for (int64_t i = from + threadIdx.x; i < to; i += 256) p[i] = make_uint4(0, 0, 0, 0);
+        for (int64_t i = from + threadIdx.x; i < to; i += blockDim.x) p[i] = make_uint4(0, 0, 0, 0);
     }
 };
 
 // A label's place: the labels below it and the equal ones before it.  A CTA has all
-// labels in shared memory and places 64; four threads share a label's comparisons.
+// labels in shared memory and places 64; sixteen threads share a label's comparisons.
 // 8192 labels are 67 M comparisons; the passes below are two launches a digit.
-__global__ void __launch_bounds__(256) k_rank_sort(Entry* __restrict__ out, unsigned* __restrict__ valid, unsigned* __restrict__ starts, Labels ids, int64_t n,
+__global__ void __launch_bounds__(1024) k_rank_sort(Entry* __restrict__ out, unsigned* __restrict__ valid, unsigned* __restrict__ starts, Labels ids, int64_t n,
                                                    int count, Zeros zeros) {
     if ((int)blockIdx.x * 64 >= count) return zeros.share(blockIdx.x - (count + 63) / 64);
     __shared__ uint4 labels[kRankSorted / 4];
-    __shared__ unsigned places[4][64], sums[8];
+    __shared__ unsigned places[16][64], sums[32];
     unsigned* flat = reinterpret_cast<unsigned*>(labels);
-    const int padded = (count + 15) / 16 * 16;
+    const int padded = (count + 63) / 64 * 64;
     unsigned all = 0;
 #pragma unroll 8
-    for (int k = threadIdx.x; k < padded; k += 256) {
+    for (int k = threadIdx.x; k < padded; k += 1024) {
         const unsigned v = k < count ? (unsigned)ids.at(k, n) : 0xffffffffu;   // none: behind all
         flat[k] = v;
         all += v != 0xffffffffu;
     }
     __syncthreads();
-    const int e = threadIdx.x & 63, i0 = blockIdx.x * 64, i = i0 + e, share = padded / 16;   // fours of a thread
+    const int e = threadIdx.x & 63, i0 = blockIdx.x * 64, i = i0 + e, share = padded / 64;   // fours of a thread
     const unsigned mine = i < count ? flat[i] : 0xffffffffu;
     unsigned place = 0;
     const int from = (threadIdx.x >> 6) * share, to = from + share;
@@ -281,11 +317,16 @@ __global__ void __launch_bounds__(256) k_rank_sort(Entry* __restrict__ out, unsi
     if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = all;
     __syncthreads();
     if (threadIdx.x < 64 && mine != 0xffffffffu)
-        out[places[0][e] + places[1][e] + places[2][e] + places[3][e]] = Entry{mine, (unsigned)i};
+    {
+        place = 0;
+#pragma unroll
+        for (int q = 0; q < 16; ++q) place += places[q][e];
+        out[place] = Entry{mine, (unsigned)i};
+    }
     if (blockIdx.x == 0 && threadIdx.x == 0) {
         all = 0;
 #pragma unroll
-        for (int w = 0; w < 8; ++w) all += sums[w];
+        for (int w = 0; w < 32; ++w) all += sums[w];
         *valid = all;
         *starts = 0;
     }
@@ -300,7 +341,7 @@ struct Source {
     const unsigned* valid;    // entries in `from`
     __device__ __forceinline__ int64_t size() const { return from ? (int64_t)*valid : count; }
     // digit of entry i (kDigits: none) and the entry
-    __device__ __forceinline__ int get(int64_t i, int64_t size, int shift, Entry& e) const {
+    template <int kDigits> __device__ __forceinline__ int get(int64_t i, int64_t size, int shift, Entry& e) const {
         if (i >= size) return kDigits;
         if (from) {
             e = from[i];
@@ -315,22 +356,22 @@ struct Source {
 };
 
 // counts [tile][digit]; a tile is kItems entries a thread.
-template <int kItems>
+template <int kItems, int kDigits>
 __global__ void __launch_bounds__(256) k_sort_count(unsigned* __restrict__ counts, Source src, int shift, int tiles, Zeros zeros) {
     if ((int)blockIdx.x >= tiles) return zeros.share(blockIdx.x - tiles);
     __shared__ unsigned h[kDigits + 1];
-    h[threadIdx.x] = 0;
-    if (threadIdx.x == 0) h[kDigits] = 0;
+    for (int i = threadIdx.x; i <= kDigits; i += 256) h[i] = 0;
     __syncthreads();
     const int64_t size = src.size(), base = (int64_t)blockIdx.x * (256 * kItems);
     Entry e[kItems];
     int digit[kItems];
 #pragma unroll
-    for (int k = 0; k < kItems; ++k) digit[k] = src.get(base + k * 256 + threadIdx.x, size, shift, e[k]);
+    for (int k = 0; k < kItems; ++k) digit[k] = src.get<kDigits>(base + k * 256 + threadIdx.x, size, shift, e[k]);
 #pragma unroll
     for (int k = 0; k < kItems; ++k) atomicAdd(&h[digit[k]], 1u);   // counts: any order
     __syncthreads();
-    counts[(int64_t)blockIdx.x * kDigits + threadIdx.x] = h[threadIdx.x];
+#pragma unroll
+    for (int i = 0; i < kDigits; i += 256) counts[(int64_t)blockIdx.x * kDigits + i + threadIdx.x] = h[i + threadIdx.x];
 }
 
 // Exclusive sum over the CTA's 256 threads.
@@ -361,7 +402,7 @@ __global__ void __launch_bounds__(256) k_sort_sums(unsigned* __restrict__ counts
     unsigned carry = 0;
     for (int64_t base = 0; base < tiles; base += 256) {
         const int64_t t = base + threadIdx.x;
-        unsigned* at = counts + t * kDigits + blockIdx.x;
+        unsigned* at = counts + t * gridDim.x + blockIdx.x;
         unsigned all;
         const unsigned o = before_me(t < tiles ? *at : 0u, all);
         if (t < tiles) *at = carry + o;
@@ -373,13 +414,13 @@ __global__ void __launch_bounds__(256) k_sort_sums(unsigned* __restrict__ counts
 
 // Stable: a warp takes neighbouring entries of the tile, 32 at a time, and counts
 // equal digits before its own by a match.  totals null: the tile adds up the
-// counts of all tiles itself.
-template <int kItems>
+// counts of all tiles itself.  A thread has kEach neighbouring digits.
+template <int kItems, int kDigits>
 __global__ void __launch_bounds__(256) k_sort_place(Entry* __restrict__ out, const unsigned* __restrict__ counts,
                                                     const unsigned* __restrict__ totals, unsigned* __restrict__ valid,
-                                                    unsigned* __restrict__ starts, Source src,
-                                                    int shift, int tiles, Zeros zeros) {
+                                                    unsigned* __restrict__ starts, Source src, int shift, int tiles, Zeros zeros) {
     if ((int)blockIdx.x >= tiles) return zeros.share(blockIdx.x - tiles);
+    constexpr int kEach = kDigits / 256;
     __shared__ unsigned h[8][kDigits + 1];
     for (int i = threadIdx.x; i < 8 * (kDigits + 1); i += 256) (&h[0][0])[i] = 0;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -388,20 +429,35 @@ __global__ void __launch_bounds__(256) k_sort_place(Entry* __restrict__ out, con
     int digit[kItems];
     unsigned rank[kItems];
 #pragma unroll
-    for (int k = 0; k < kItems; ++k) digit[k] = src.get(base + k * 32 + lane, size, shift, e[k]);
-    unsigned o = 0, total = 0, all;   // the digit threadIdx.x in the tiles before, and in all
+    for (int k = 0; k < kItems; ++k) digit[k] = src.get<kDigits>(base + k * 32 + lane, size, shift, e[k]);
+    unsigned o[kEach], total[kEach], sum = 0, all;   // of the thread's digits: in the tiles before, in all
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) o[j] = total[j] = 0;
     if (totals) {
-        o = counts[(int64_t)blockIdx.x * kDigits + threadIdx.x];
-        total = totals[threadIdx.x];
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+            o[j] = counts[(int64_t)blockIdx.x * kDigits + threadIdx.x * kEach + j];
+            total[j] = totals[threadIdx.x * kEach + j];
+        }
     } else {
-#pragma unroll 16
+#pragma unroll 8
         for (int t = 0; t < tiles; ++t) {
-            const unsigned v = counts[t * kDigits + threadIdx.x];
-            total += v;
-            if (t < (int)blockIdx.x) o += v;
+#pragma unroll
+            for (int j = 0; j < kEach; ++j) {
+                const unsigned v = counts[t * kDigits + threadIdx.x * kEach + j];
+                total[j] += v;
+                if (t < (int)blockIdx.x) o[j] += v;
+            }
         }
     }
-    o += before_me(total, all);   // all threads: h has been cleared behind it
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) sum += total[j];
+    unsigned before = before_me(sum, all);   // all threads: h has been cleared behind it
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+        o[j] += before;
+        before += total[j];
+    }
     if (blockIdx.x == 0 && threadIdx.x == 0) *valid = all, *starts = 0;
 #pragma unroll
     for (int k = 0; k < kItems; ++k) {
@@ -414,10 +470,14 @@ __global__ void __launch_bounds__(256) k_sort_place(Entry* __restrict__ out, con
     }
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < 8; ++w) {
-        const unsigned had = h[w][threadIdx.x];
-        h[w][threadIdx.x] = o;
-        o += had;
+    for (int j = 0; j < kEach; ++j) {
+        const int d = threadIdx.x * kEach + j;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) {
+            const unsigned had = h[w][d];
+            h[w][d] = o[j];
+            o[j] += had;
+        }
     }
     __syncthreads();
 #pragma unroll
@@ -507,60 +567,99 @@ __global__ void __launch_bounds__(256) k_runs(const __grid_constant__ RunArgs a)
 }
 
 // The runs that begin in a chunk and go on behind it: its part and those of the
-// chunks up to the run's end.  `lanes` threads of V channels side by side (blockIdx.y
-// has others), the others take every 256 / lanes-th part, and theirs are added in
-// order.
+// chunks up to the run's end, in order.  A warp a run, 32 V channels at a time
+// (blockIdx.y has others); runs of more than kLongRun parts by the CTA: `lanes` threads
+// of V channels side by side, each such group takes every groups-th part, and theirs
+// are added in pairs.
+constexpr int kLongRun = 24, kJoinWarps = 16;
+
 template <int V>
-__global__ void __launch_bounds__(256) k_join_runs(const __grid_constant__ RunArgs a, int lanes) {
-    __shared__ float sums[256 * V];
+__device__ __forceinline__ void add_parts(float (&s)[V], const RunArgs& a, int64_t chunk, int64_t col, int64_t first, int64_t last,
+                                          int64_t step) {
+    for (int64_t k = first; k <= last; k += 8 * step) {
+        Vec<float, V> v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            v[u].zero();
+            if (k + u * step <= last) v[u].load(a.part + (chunk + k + u * step) * 2 * a.c + col);
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+#pragma unroll
+            for (int j = 0; j < V; ++j) s[j] += v[u].at(j);
+    }
+}
+
+template <int V>
+__global__ void __launch_bounds__(32 * kJoinWarps) k_join_runs(const __grid_constant__ RunArgs a, int lanes) {
+    __shared__ float sums[kJoinWarps * 32 * V];
+    __shared__ int64_t long_chunk[kJoinWarps], long_parts[kJoinWarps];
     const unsigned starts = a.starts[0];
     const int64_t valid = *a.valid;
-    for (unsigned i = blockIdx.x; i < starts; i += gridDim.x) {
-    const int64_t chunk = a.starts[1 + i];
-    const unsigned label = a.sorted[(chunk + 1) * a.length].label;
-    int64_t parts = 1;   // chunks behind this one that the run reaches: those that begin with its label
-    for (int count = 256; count == 256; parts += count) {
-        const int64_t at = (chunk + 1 + parts + threadIdx.x) * a.length;
-        count = __syncthreads_count(at < valid && a.sorted[at < valid ? at : 0].label == label);
-    }
-    const int lane = threadIdx.x % lanes, group = threadIdx.x / lanes, groups = 256 / lanes;
-    for (int64_t first = (int64_t)blockIdx.y * lanes * V; first < a.c; first += (int64_t)gridDim.y * lanes * V) {
-        const int64_t col = first + lane * V;
-        float s[V];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t col0 = ((int64_t)blockIdx.y * 32 + lane) * V, next = (int64_t)gridDim.y * 32 * V;
+    const auto tail = [&](float (&s)[V], int64_t chunk, int64_t col) {   // the run's first part
+        Vec<float, V> v;
+        v.load(a.part + (chunk * 2 + 1) * a.c + col);
 #pragma unroll
-        for (int j = 0; j < V; ++j) s[j] = 0.f;
-        if (col < a.c) {
-            if (group == 0) {
-                Vec<float, V> v;
-                v.load(a.part + (chunk * 2 + 1) * a.c + col);
+        for (int j = 0; j < V; ++j) s[j] = v.at(j);
+    };
+    const auto write = [&](float (&s)[V], int64_t chunk, int64_t col) {
+        const int64_t at = (int64_t)a.sorted[(chunk + 1) * a.length].label * a.c + col;
 #pragma unroll
-                for (int j = 0; j < V; ++j) s[j] = v.at(j);
+        for (int j = 0; j < V; ++j) store_param(a.out, a.out_dtype, at + j, s[j] * a.scale);
+    };
+    // runs a CTA takes at a time: few where there are few, so that each has a CTA
+    const unsigned spread = (starts + gridDim.x - 1) / gridDim.x, each = spread < kJoinWarps ? spread : kJoinWarps;
+    for (unsigned i0 = blockIdx.x * each; i0 < starts; i0 += gridDim.x * each) {
+        const unsigned i = warp < each ? i0 + warp : starts;
+        int64_t chunk = 0, parts = 0;   // chunks behind this one that the run reaches: those that begin with its label
+        if (i < starts) {
+            chunk = a.starts[1 + i];
+            const unsigned label = a.sorted[(chunk + 1) * a.length].label;
+            parts = 1;
+            for (int count = 32; count == 32; parts += count) {
+                const int64_t at = (chunk + 1 + parts + lane) * a.length;
+                count = __popc(__ballot_sync(0xffffffffu, at < valid && a.sorted[at < valid ? at : 0].label == label));
             }
-            for (int64_t k = 1 + group; k <= parts; k += 8 * groups) {
-                Vec<float, V> v[8];
-#pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                    v[u].zero();
-                    if (k + u * groups <= parts) v[u].load(a.part + (chunk + k + u * groups) * 2 * a.c + col);
+            if (parts <= kLongRun)
+                for (int64_t col = col0; col < a.c; col += next) {
+                    float s[V];
+                    tail(s, chunk, col);
+                    add_parts(s, a, chunk, col, 1, parts, 1);
+                    write(s, chunk, col);
                 }
+        }
+        if (lane == 0) {
+            long_chunk[warp] = chunk;
+            long_parts[warp] = parts;
+        }
+        __syncthreads();
+        for (int w = 0; w < kJoinWarps; ++w) {
+            if (long_parts[w] <= kLongRun) continue;
+            const int group = threadIdx.x / lanes, groups = 32 * kJoinWarps / lanes, at = threadIdx.x % lanes * V;
+            for (int64_t first = (int64_t)blockIdx.y * lanes * V; first < a.c; first += (int64_t)gridDim.y * lanes * V) {
+                const int64_t col = first + at;
+                float s[V];
 #pragma unroll
-                for (int u = 0; u < 8; ++u)
+                for (int j = 0; j < V; ++j) s[j] = 0.f;
+                if (col < a.c) {
+                    if (group == 0) tail(s, long_chunk[w], col);
+                    add_parts(s, a, long_chunk[w], col, 1 + group, long_parts[w], groups);
+                }
+                for (int d = groups / 2; d; d >>= 1) {
 #pragma unroll
-                    for (int j = 0; j < V; ++j) s[j] += v[u].at(j);
+                    for (int j = 0; j < V; ++j) sums[threadIdx.x * V + j] = s[j];
+                    __syncthreads();
+                    if (group < d)
+#pragma unroll
+                        for (int j = 0; j < V; ++j) s[j] += sums[(threadIdx.x + d * lanes) * V + j];
+                    __syncthreads();
+                }
+                if (group == 0 && col < a.c) write(s, long_chunk[w], col);
             }
         }
-#pragma unroll
-        for (int j = 0; j < V; ++j) sums[threadIdx.x * V + j] = s[j];
         __syncthreads();
-        if (group == 0 && col < a.c) {
-            for (int k = 1; k < groups; ++k)
-#pragma unroll
-                for (int j = 0; j < V; ++j) s[j] += sums[(k * lanes + lane) * V + j];
-#pragma unroll
-            for (int j = 0; j < V; ++j) store_param(a.out, a.out_dtype, (int64_t)label * a.c + col + j, s[j] * a.scale);
-        }
-        __syncthreads();
-    }
     }
 }
 
@@ -571,16 +670,16 @@ static int64_t align256(int64_t b) { return (b + 255) / 256 * 256; }
 struct EmbedPlan {
     bool small;
     int v, lane_bits, slabs, warps, warp_bytes, ctas, ctas_y;   // small table
-    int passes, items, tiles, length;            // sorted; passes 0: by counting
+    int passes, bits, items, tiles, length;      // sorted; passes 0: by counting
     int64_t chunks;
     int64_t totals, starts, counts, first, second, part, bytes;   // offsets in the workspace
 };
 
-constexpr int kOwnSums = 256;   // tiles up to which the tiles add up the counts themselves
+constexpr int kOwnSums = 48;   // tiles up to which the tiles add up the counts themselves
 
 static EmbedPlan embed_plan(int64_t count, int64_t n, int c, int element) {
     EmbedPlan p = {};
-    p.small = n <= kSmallTable;
+    p.small = n <= kSmallTable && count >= 512 * n;   // worth the tables' way in and out (620 of 95 x 98: 85 us, sorted 20)
     if (p.small) {
         // 8 bytes a lane (half the instructions a row) where many warps' copies of that fit
         const int widest_v = element == 4 || n <= kWideTable ? 8 / element : 4 / element;
@@ -603,20 +702,26 @@ static EmbedPlan embed_plan(int64_t count, int64_t n, int c, int element) {
         return p;
     }
     if (count > kRankSorted) {
-        while ((n - 1) >> (8 * p.passes)) ++p.passes;
+        int bits = 1;
+        while ((n - 1) >> bits) ++bits;
+        p.passes = (bits + kMostBits - 1) / kMostBits;
+        p.bits = (bits + p.passes - 1) / p.passes < 8 ? 8 : (bits + p.passes - 1) / p.passes;
         p.items = count <= 262144 ? 4 : 16;
         p.tiles = (int)ceil_div(count, 256 * p.items);
     }
     // chunks long enough that few runs cross them, short enough that they fill the device
     const int64_t want = count * ceil_div(c, 8) / (148 * 2048);
-    p.length = (int)(want < 16 ? 16 : want > 256 ? 256 : (want + 7) / 8 * 8);
+    const int64_t fit = want < 1 ? 8 : want < 16 ? 16 : want > 256 ? 256 : (want + 7) / 8 * 8;
+    // (labels with many entries each: longer ones, so that their runs have fewer parts)
+    const int64_t run = count / n / 16;
+    p.length = (int)(run > fit ? (run < 128 ? run / 8 * 8 : fit > 128 ? fit : 128) : fit);
     p.chunks = ceil_div(count, p.length);
     p.totals = 256;   // the number of valid entries is in front
-    int64_t at = p.totals + kDigits * 4;
+    int64_t at = p.totals + (4 << kMostBits);
     p.starts = at;
     at += align256((p.chunks + 1) * 4);
     p.counts = at;
-    at += align256((int64_t)kDigits * p.tiles * 4);
+    at += align256(((int64_t)4 << p.bits) * p.tiles);
     p.first = at;
     at += align256(count * (int64_t)sizeof(Entry));
     p.second = at;
@@ -659,13 +764,14 @@ static Zeros zeros_of(void* table, int64_t bytes, int i, int launches) {
     return z;
 }
 
-template <int kItems>
-static void sort_pass(Entry* to, unsigned* counts, unsigned* totals, unsigned* valid, unsigned* starts, const Source& src, int shift, int tiles,
-                      const Zeros& first, const Zeros& second, cudaStream_t s) {
-    k_sort_count<kItems><<<tiles + first.ctas, 256, 0, s>>>(counts, src, shift, tiles, first);
+template <int kItems, int kDigits>
+static void sort_pass(Entry* to, unsigned* counts, unsigned* totals, unsigned* valid, unsigned* starts, const Source& src, int shift,
+                      int tiles, const Zeros& first, const Zeros& second, cudaStream_t s) {
+    k_sort_count<kItems, kDigits><<<tiles + first.ctas, 256, 0, s>>>(counts, src, shift, tiles, first);
     const bool own = tiles <= kOwnSums;
     if (!own) k_sort_sums<<<kDigits, 256, 0, s>>>(counts, totals, tiles);
-    k_sort_place<kItems><<<tiles + second.ctas, 256, 0, s>>>(to, counts, own ? nullptr : totals, valid, starts, src, shift, tiles, second);
+    k_sort_place<kItems, kDigits>
+        <<<tiles + second.ctas, 256, 0, s>>>(to, counts, own ? nullptr : totals, valid, starts, src, shift, tiles, second);
 }
 
 // The labels in order with their positions; `bytes` of the table (a multiple of
@@ -677,14 +783,15 @@ static const Entry* sort_labels(const EmbedPlan& p, uint8_t* ws, const Labels& i
     Entry *to = reinterpret_cast<Entry*>(ws + p.first), *other = reinterpret_cast<Entry*>(ws + p.second), *from = nullptr;
     if (p.passes == 0) {
         const Zeros z = zeros_of(table, bytes, 0, 1);
-        k_rank_sort<<<(unsigned)ceil_div(count, 64) + z.ctas, 256, 0, s>>>(to, valid, starts, ids, n, (int)count, z);
+        k_rank_sort<<<(unsigned)ceil_div(count, 64) + z.ctas, 1024, 0, s>>>(to, valid, starts, ids, n, (int)count, z);
         return to;
     }
     for (int pass = 0; pass < p.passes; ++pass) {
         const Source src{ids, n, count, from, valid};
         const Zeros first = zeros_of(table, bytes, 2 * pass, 2 * p.passes), second = zeros_of(table, bytes, 2 * pass + 1, 2 * p.passes);
-        if (p.items == 4) sort_pass<4>(to, counts, totals, valid, starts, src, 8 * pass, p.tiles, first, second, s);
-        else sort_pass<16>(to, counts, totals, valid, starts, src, 8 * pass, p.tiles, first, second, s);
+        const auto run = p.items == 4 ? (p.bits == 8 ? sort_pass<4, 256> : p.bits == 9 ? sort_pass<4, 512> : sort_pass<4, 1024>)
+                                      : (p.bits == 8 ? sort_pass<16, 256> : p.bits == 9 ? sort_pass<16, 512> : sort_pass<16, 1024>);
+        run(to, counts, totals, valid, starts, src, p.bits * pass, p.tiles, first, second, s);
         from = to;
         to = other;
         other = from;
@@ -707,6 +814,12 @@ static cudaError_t launch_embed(void* y, const Labels& ids, const void* table, f
 template <typename T>
 static cudaError_t launch_embed(int v, void* y, const Labels& ids, const void* table, float scale, int64_t count,
                                 int64_t n, int c, cudaStream_t s) {
+    if (v * sizeof(T) < 8 && aligned16(y)) {
+        const int64_t all = count * c, ctas = ceil_div(all, 256 * (16 / (int)sizeof(T)));
+        if (ctas > 0x7fffffff) return cudaErrorInvalidValue;
+        k_embed_flat<T><<<(unsigned)ctas, 256, 0, s>>>(static_cast<T*>(y), ids, static_cast<const T*>(table), scale, all, n, (unsigned)c);
+        return cudaGetLastError();
+    }
     if (v * sizeof(T) == 16) return launch_embed<T, 16 / sizeof(T)>(y, ids, table, scale, count, n, c, s);
     if (v == 4) return launch_embed<T, 4>(y, ids, table, scale, count, n, c, s);
     if (v == 2) return launch_embed<T, 2>(y, ids, table, scale, count, n, c, s);
@@ -715,10 +828,10 @@ static cudaError_t launch_embed(int v, void* y, const Labels& ids, const void* t
 
 template <typename T, int V>
 static cudaError_t launch_runs(const RunArgs& a, int64_t chunks, cudaStream_t s) {
-    const int units = a.c / V;
-    int x = 1;
-    while (x < units && x < 256) x <<= 1;
-    const int y = 256 / x;
+    const int units = a.c / V, x = units < 256 ? units : 256;
+    // chunks of a CTA: fewer where they are few, so that all SMs have some
+    const int64_t spread = ceil_div(chunks, 2 * (int64_t)sm_count());
+    const int y = spread < 256 / x ? (int)spread : 256 / x;
     const dim3 grid((unsigned)ceil_div(chunks, y), (unsigned)ceil_div(units, x));
     if (grid.y > 65535) return cudaErrorInvalidValue;
     k_runs<T, V><<<grid, dim3(x, y), 0, s>>>(a);
@@ -734,13 +847,13 @@ static cudaError_t launch_runs(int v, const RunArgs& a, int64_t chunks, cudaStre
 }
 
 static cudaError_t join_runs(const RunArgs& a, int64_t chunks, cudaStream_t s) {
-    const bool four = a.c % 4 == 0;
-    const int units = a.c / (four ? 4 : 1);
+    const int v = a.c % 4 == 0 ? 4 : 1;
+    const int64_t strips = ceil_div(a.c, 32 * v), x = chunks - 1 < 296 ? chunks - 1 : 296, most = 592 / x;
+    const dim3 grid((unsigned)x, (unsigned)(strips < most ? strips : most));
     int lanes = 1;
-    while (lanes < 64 && lanes < units) lanes <<= 1;
-    const dim3 grid((unsigned)(chunks - 1 < 592 ? chunks - 1 : 592), (unsigned)(ceil_div(units, lanes) < 8 ? ceil_div(units, lanes) : 8));
-    if (four) k_join_runs<4><<<grid, 256, 0, s>>>(a, lanes);
-    else k_join_runs<1><<<grid, 256, 0, s>>>(a, lanes);
+    while (lanes < 32 && lanes * v < a.c) lanes <<= 1;
+    if (v == 4) k_join_runs<4><<<grid, 32 * kJoinWarps, 0, s>>>(a, lanes);
+    else k_join_runs<1><<<grid, 32 * kJoinWarps, 0, s>>>(a, lanes);
     return cudaGetLastError();
 }
 

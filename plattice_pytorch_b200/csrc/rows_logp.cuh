@@ -824,6 +824,8 @@ __global__ void __launch_bounds__(kThreads, kThreads == 512 ? 2 : kThreads == 25
 
 // ------------------------------------------------------------- few classes
 
+// (198959 x 48 in float32 with 20 alternatives, for each of which a thread looks through
+// its row again: 151 us; a warp a row takes 267.)
 constexpr int kFewClasses = 64, kTileRows = 128;
 
 // A tile of rows lies in memory as one stretch: 16 bytes at a time (its start

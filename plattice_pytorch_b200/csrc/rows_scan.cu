@@ -302,6 +302,61 @@ __global__ void __launch_bounds__(kThreads, 4) k_scan_grad(const __grid_constant
         for (int j = 0; j < V; ++j) p.gs[w.line * p.c + w.col + j] = r[j];
 }
 
+// ---------------------------------------------------------------- single steps
+//
+// One step of every line, as where a state is kept between calls: no line to walk,
+// V channels of any line a thread (4679 lines of 792 bfloat16 channels forward and
+// back: 85 us as blocks of a step).
+
+template <typename T, int V, bool kBlend>
+__global__ void __launch_bounds__(256) k_scan_step(const __grid_constant__ ScanArgs p, int64_t units) {
+    const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x, at = u * V;
+    if (u >= units) return;
+    Vec<T, V> x, a;
+    Vec<float, V> s;
+    x.load(static_cast<const T*>(p.x) + at);
+    a.load(static_cast<const T*>(p.a) + at);
+    s.zero();
+    if (p.state) s.load(p.state + at);
+    if (p.states) s.store(p.states + at);
+    float h[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) h[j] = fmaf(a.at(j), s.at(j), input<kBlend>(a.at(j), x.at(j)));
+    Vec<T, V> y;
+    y.from(h);
+    y.store(static_cast<T*>(p.h) + at);
+    s.from(h);
+    if (p.last) s.store(p.last + at);
+}
+
+template <typename T, int V, bool kBlend>
+__global__ void __launch_bounds__(256) k_scan_step_grad(const __grid_constant__ ScanArgs p, int64_t units) {
+    const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x, at = u * V;
+    if (u >= units) return;
+    Vec<T, V> x, a, g, gx, ga;
+    Vec<float, V> s, r;
+    x.load(static_cast<const T*>(p.x) + at);
+    a.load(static_cast<const T*>(p.a) + at);
+    g.load(static_cast<const T*>(p.g) + at);
+    s.load(p.states + at);
+    r.zero();
+    if (p.grad_last) r.load(p.grad_last + at);
+    float fx[V], fa[V], fs[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const float gate = a.at(j), whole = g.at(j) + r.at(j);
+        fx[j] = kBlend ? (1.f - gate) * whole : whole;
+        fa[j] = whole * (kBlend ? s.at(j) - x.at(j) : s.at(j));
+        fs[j] = gate * whole;
+    }
+    gx.from(fx);
+    ga.from(fa);
+    gx.store(static_cast<T*>(p.gx) + at);
+    ga.store(static_cast<T*>(p.ga) + at);
+    r.from(fs);
+    if (p.gs) r.store(p.gs + at);
+}
+
 // ------------------------------------------------------------------ host side
 
 // Threads that fill the device (each has 16 steps of two or three tensors in
@@ -367,6 +422,25 @@ static cudaError_t launch(const ScanArgs& a, const ScanPlan& p, bool blend, bool
     return blend ? launch<T, 1, true>(a, p, grad, s) : launch<T, 1, false>(a, p, grad, s);
 }
 
+template <typename T, int V>
+static cudaError_t launch_step(const ScanArgs& a, bool blend, bool grad, cudaStream_t s) {
+    const int64_t units = a.lines * a.c / V, ctas = ceil_div(units, 256);
+    if (ctas > 0x7fffffff) return cudaErrorInvalidValue;
+    const auto kernel = grad ? (blend ? k_scan_step_grad<T, V, true> : k_scan_step_grad<T, V, false>)
+                             : (blend ? k_scan_step<T, V, true> : k_scan_step<T, V, false>);
+    kernel<<<(unsigned)ctas, 256, 0, s>>>(a, units);
+    return cudaGetLastError();
+}
+
+template <typename T>
+static cudaError_t launch_step(const ScanArgs& a, bool blend, bool grad, cudaStream_t s) {
+    // what is not there has a null pointer, which any access allows
+    const uintptr_t rows = (uintptr_t)a.x | (uintptr_t)a.a | (uintptr_t)a.h | (uintptr_t)a.g | (uintptr_t)a.gx | (uintptr_t)a.ga,
+                    states = (uintptr_t)a.state | (uintptr_t)a.last | (uintptr_t)a.states | (uintptr_t)a.grad_last | (uintptr_t)a.gs;
+    if (a.lines * a.c % 4 == 0 && rows % (4 * sizeof(T)) == 0 && states % 16 == 0) return launch_step<T, 4>(a, blend, grad, s);
+    return launch_step<T, 1>(a, blend, grad, s);
+}
+
 static int run(const plattice_scan_args* q, bool grad, cudaStream_t s, const char* call) {
     const ScanPlan p = scan_plan(q, grad);
     if (p.bytes && (!q->workspace || ((uintptr_t)q->workspace & 255) || q->workspace_bytes < (size_t)p.bytes))
@@ -375,6 +449,16 @@ static int run(const plattice_scan_args* q, bool grad, cudaStream_t s, const cha
     const ScanArgs a{q->x, q->gate, q->state, q->h, q->last, q->states, q->grad_h, q->grad_last, q->grad_x, q->grad_gate,
                      q->grad_state, ws, ws + p.tile_sums / (int64_t)sizeof(float2), q->lines, q->steps,
                      ceil_div(q->steps, kSteps), p.tiles, q->c, q->reverse, p.lanes, p.pieces, p.piece_blocks};
+    if (q->steps == 1) {
+        // pointers of the other direction are not used
+        ScanArgs b = a;
+        if (grad) b.state = nullptr, b.h = nullptr, b.last = nullptr;
+        else b.g = nullptr, b.grad_last = nullptr, b.gx = b.ga = nullptr, b.gs = nullptr;
+        const cudaError_t e = q->dtype == PLATTICE_F32    ? launch_step<float>(b, q->blend, grad, s)
+                              : q->dtype == PLATTICE_BF16 ? launch_step<__nv_bfloat16>(b, q->blend, grad, s)
+                                                          : launch_step<__half>(b, q->blend, grad, s);
+        return rows_status(e, call);
+    }
     const cudaError_t e = q->dtype == PLATTICE_F32    ? launch<float>(a, p, q->blend, grad, s)
                           : q->dtype == PLATTICE_BF16 ? launch<__nv_bfloat16>(a, p, q->blend, grad, s)
                                                       : launch<__half>(a, p, q->blend, grad, s);
