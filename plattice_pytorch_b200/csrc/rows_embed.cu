@@ -170,10 +170,10 @@ __global__ void __launch_bounds__(1024) k_small_table(const __grid_constant__ Ta
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
-        const int id = lane < left ? a.ids.at(row0 + lane, a.n) : -1;
-        return id < 0 ? n : id;
+        return lane < left ? a.ids.raw(row0 + lane) : -1ll;   // not looked at yet: it is on its way, too
     };
-    const auto add = [&](const T* stage, int id) {
+    const auto add = [&](const T* stage, long long label) {
+        const int id = label >= 0 && label < n ? (int)label : n;
         const T* from = stage + (group << bits) + own * V;
         int at = group;
 #pragma unroll 4
@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(1024) k_small_table(const __grid_constant__ Ta
     };
     T *even = rows, *odd = rows + 32 * width;
     int64_t b = (int64_t)blockIdx.x * a.copies + copy;
-    int id0 = bring(b, even), id1 = bring(b + step, odd);
+    long long id0 = bring(b, even), id1 = bring(b + step, odd);
     for (; b < blocks; b += 2 * step) {
         asm volatile("cp.async.wait_group 1;" ::: "memory");
         __syncwarp();

@@ -61,8 +61,11 @@ inline int widest(int64_t c, size_t element, uintptr_t bits) {
 struct Labels {
     const void* p;
     int wide;
+    __device__ __forceinline__ long long raw(int64_t i) const {
+        return wide ? static_cast<const long long*>(p)[i] : (long long)static_cast<const int*>(p)[i];
+    }
     __device__ __forceinline__ int at(int64_t i, int64_t n) const {
-        const int64_t v = wide ? static_cast<const long long*>(p)[i] : (int64_t)static_cast<const int*>(p)[i];
+        const int64_t v = raw(i);
         return v >= 0 && v < n ? (int)v : -1;
     }
 };
