@@ -679,7 +679,9 @@ constexpr int kOwnSums = 48;   // tiles up to which the tiles add up the counts 
 
 static EmbedPlan embed_plan(int64_t count, int64_t n, int c, int element) {
     EmbedPlan p = {};
-    p.small = n <= kSmallTable && count >= 512 * n;   // worth the tables' way in and out (620 of 95 x 98: 85 us, sorted 20)
+    // Worth the tables' way in and out (620 labels of 95 x 98: 85 us, sorted 21), and of rows
+    // that come in whole accesses (118781 x 333 element by element: 275 us).
+    p.small = n <= kSmallTable && count >= 512 * n && c * element % 16 == 0;
     if (p.small) {
         // 8 bytes a lane (half the instructions a row) where many warps' copies of that fit
         const int widest_v = element == 4 || n <= kWideTable ? 8 / element : 4 / element;

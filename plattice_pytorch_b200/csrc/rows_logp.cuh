@@ -826,7 +826,8 @@ __global__ void __launch_bounds__(kThreads, kThreads == 512 ? 2 : kThreads == 25
 
 // (198959 x 48 in float32 with 20 alternatives, for each of which a thread looks through
 // its row again: 151 us; a warp a row takes 267.)
-constexpr int kFewClasses = 64, kTileRows = 128;
+// Up to 256 bytes of classes: 858914 x 73 in float16 with 3 alternatives, a warp a row, 390.
+constexpr int kFewBytes = 256, kTileRows = 128;
 
 // A tile of rows lies in memory as one stretch: 16 bytes at a time (its start
 // allows that when the tensor's does) to shared memory, where rows are `pitch`
@@ -836,10 +837,10 @@ template <typename T> __host__ __device__ inline int pitch_of(int n) {
     return sizeof(T) == 4 ? n | 1 : n % 4 == 0 ? n + 2 : n;
 }
 
-struct Place {   // of an element of a tile: at most 128 x 64 of them, so the quotient is exact
+struct Place {   // of an element of a tile: at most 128 x 128 of them, so the quotient is exact
     int row, j;
     __device__ __forceinline__ Place(int i, int n) {
-        row = (int)(((unsigned)i * ((1u << 20) / (unsigned)n + 1u)) >> 20);
+        row = (int)(((unsigned)i * ((1u << 22) / (unsigned)n + 1u)) >> 22);
         j = i - row * n;
     }
     __device__ __forceinline__ void next(int n) {
@@ -1205,7 +1206,7 @@ static cudaError_t launch_warp(const LogpArgs& a, cudaStream_t s) {
 
 template <typename T>
 cudaError_t logp_forward(const LogpArgs& a, cudaStream_t s) {
-    if (a.n <= kFewClasses) {
+    if (a.n * sizeof(T) <= kFewBytes) {
         k_logp_few<T><<<grid_of(ceil_div(a.rows, kTileRows)), kTileRows, kTileRows * pitch_of<T>(a.n) * sizeof(T), s>>>(
             a, aligned16(a.x));
         return cudaGetLastError();
@@ -1230,7 +1231,7 @@ cudaError_t logp_forward(const LogpArgs& a, cudaStream_t s) {
 
 template <typename T>
 cudaError_t logp_backward(const LogpArgs& a, cudaStream_t s) {
-    if (a.n <= kFewClasses) {
+    if (a.n * sizeof(T) <= kFewBytes) {
         k_logp_few_grad<T><<<grid_of(ceil_div(a.rows, kTileRows)), kTileRows, kTileRows * pitch_of<T>(a.n) * sizeof(T), s>>>(
             a, aligned16(a.x), aligned16(a.gx));
         return cudaGetLastError();

@@ -88,7 +88,7 @@ class LogProbs:
 
     * x - m is within U |d|; its exponential within 2 U |d| + 8 U of itself (the argument's
       product with log2(e), two units for the function); sums of n terms by at least 32
-      lanes (or one lane for up to 64 classes) within (n / 32 + 40) U (n U)
+      lanes (or one lane for up to 128 classes) within (n / 32 + 40) U (n U)
     * s = log(sum) takes the sum's relative error and 4 U of its own
     """
 
@@ -110,7 +110,7 @@ class LogProbs:
             pd2 = np.where(p > 0, p * d * d, 0.0).sum(1)
         self.lse = np.where(empty, -np.inf, (m + s)[:, 0])
         self.top = np.argsort(-x, axis=1, kind="stable")
-        depth = (n if n <= 64 else n / 32 + 40) + 8
+        depth = (n if n <= 128 else n / 32 + 40) + 8
         w = -pd.sum(1)
         self.e_s = U * (depth + 2 * w) + 4 * U * s[:, 0]
         self.e_logp = U * np.where(np.isfinite(d), np.abs(d), 0) + self.e_s[:, None] + 2 * U * np.where(

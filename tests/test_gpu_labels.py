@@ -144,7 +144,7 @@ def _scores(rows, n, dtype, seed, masked=True):
 
 
 LOGP_SIZES = [(1, 1), (5, 2), (40, 3), (33, 21), (257, 32), (9, 33), (20, 100), (3, 255), (70, 256), (12, 1000), (6, 1024),
-              (4, 2050), (5, 5003), (2, 33000), (1, 70001), (150, 4096), (0, 7), (2, 131072), (300, 64), (130, 65), (1, 300001), (200, 40000)]
+              (4, 2050), (5, 5003), (2, 33000), (1, 70001), (150, 4096), (0, 7), (2, 131072), (300, 64), (130, 65), (300, 127), (129, 128), (200, 129), (1, 300001), (200, 40000)]
 
 
 def _check_logp(dev, R, x, top, labels):

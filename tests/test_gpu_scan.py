@@ -42,7 +42,7 @@ def _inputs(lead, t, c, dtype, seed, gates="sigmoid"):
 
 SIZES = [((1,), 1, 1), ((), 1, 4096), ((3,), 2, 5), ((2, 3), 15, 8), ((2,), 16, 33), ((5,), 17, 2), ((1,), 100, 7), ((40,), 64, 64),
          ((3,), 129, 130), ((1,), 5000, 3), ((2,), 2049, 16), ((1,), 20011, 2), ((300,), 33, 24), ((0,), 5, 4), ((2,), 0, 6),
-         ((1,), 9001, 1)]
+         ((1,), 9001, 1), ((3,), 1600, 1), ((2,), 1008, 2), ((5,), 48, 1)]
 
 
 def _rounded(dtype, value):
