@@ -44,7 +44,7 @@ __global__ void __launch_bounds__(256) k_embed(T* __restrict__ y, Labels ids, co
             if (row0 + u * step < count) {
                 float f[V];
 #pragma unroll
-                for (int i = 0; i < V; ++i) f[i] = v[u].at(i) * scale;
+                for (int i = 0; i < V; ++i) f[i] = id[u] >= 0 ? v[u].at(i) * scale : 0.f;
                 v[u].from(f);
                 v[u].store(to);
             }

@@ -185,12 +185,12 @@ __device__ __forceinline__ void warp_sums(float& a, float& b) {
 template <typename T> struct Exponents {
     float c, delta, whole;   // whole: 2^-delta
     uint32_t bound;
-    bool fast;    // m is far enough from the type's ends (the same for a row)
+    bool fast;    // m is small enough for that, and far from the type's lowest (the same for a row)
     __device__ __forceinline__ explicit Exponents(float m) {
         c = -(m * kLog2e);
         delta = fmaf(m, kLog2e, c);
         whole = exp2_fast(-delta);
-        fast = fabsf(m) < 1e38f;
+        fast = fabsf(m) < 1e6f;   // delta is below 2^-24 1.5 |m|
         if constexpr (sizeof(T) == 2) {
             typename Pair<T>::type b;
             const float low = m - fmaxf(140.f, fabsf(m) * (1.f / 64.f));

@@ -69,6 +69,19 @@ def test_embed_of_nonfinite_rows(dev, R):
     assert got[2, 0] == 2 and torch.isposinf(got[2, 1]) and torch.isnan(got[2, 2])
 
 
+@pytest.mark.parametrize("count,n", [(40, 30), (20000, 30), (20000, 3000)])
+def test_gradients_that_are_not_finite(dev, R, count, n):
+    """Reach their own label's row and no other; those of rows without a label reach none."""
+    g = _randn((count, 16), 12)
+    ids = _labels((count,), n, 13, 0.2)
+    ids[0], ids[1], ids[2] = 4, 5, -1
+    g[0, 3], g[1, 7], g[2] = float("inf"), float("nan"), float("nan")
+    got = R.embed_backward(g.to(dev), ids.to(dev), n).cpu()
+    assert torch.isposinf(got[4, 3]) and torch.isnan(got[5, 7])
+    got[4, 3] = got[5, 7] = 0
+    assert torch.isfinite(got).all()
+
+
 EMBED_SIZES = [((1,), 1, 1), ((7,), 5, 3), ((13, 29), 21, 50), ((100,), 1000, 64), ((3, 5, 2), 4, 1030), ((4097,), 33, 8),
                ((9000,), 3, 8), ((20000,), 257, 24), ((5000,), 70000, 16), ((2,), 3, 4096), ((0,), 3, 8), ((40000,), 1, 17),
                ((70000,), 21, 64), ((300,), 256, 2048), ((8192,), 97, 2), ((8193,), 300, 4), ((300000,), 96, 6),
@@ -112,6 +125,12 @@ def test_embed_of_unaligned_rows(dev, R):
         gbase = _randn((1 + 333 * 16,), 9, dtype).to(dev)
         g = gbase[1:].view(333, 16)
         assert torch.equal(R.embed_backward(g, ids, 50), R.embed_backward(g.clone(), ids, 50))
+        gbase = _randn((1 + 30000 * 16,), 9, dtype).to(dev)   # a small table with many labels
+        g, ids = gbase[1:].view(30000, 16), _labels((30000,), 50, 8).to(dev)
+        want, bound = ref.embed_backward(f64(g), ids.cpu().numpy(), 50, 1.0)
+        got = R.embed_backward(g, ids, 50, dtype=torch.float32)
+        assert worst(f64(got), want, _rounded(torch.float32, want) + bound) <= 1
+        assert torch.equal(got, R.embed_backward(g.clone(), ids, 50, dtype=torch.float32))
 
 
 def test_embed_function(dev, R):
@@ -296,6 +315,26 @@ def test_log_probs_of_unaligned_rows(dev, R):
             got = R.log_probs_backward(moved, q, labels, g)
             grad, bound = want.backward(labels.cpu().numpy(), f64(g))
             assert worst(f64(got), grad, bound + _rounded(dtype, grad)) <= 1
+
+
+@pytest.mark.parametrize("n", [7, 100, 900, 5000, 70000])
+@pytest.mark.parametrize("offset", [3e5, 5e6, -2e9, 1e30, -3e38, 60000.0, -65000.0])
+def test_scores_of_any_size(dev, R, offset, n):
+    """Scores around a large one: the exponentials are of the differences (what the type
+    leaves of them), whatever the size; so are the gradients."""
+    for dtype in TYPES:
+        if abs(offset) > torch.finfo(dtype).max:
+            continue
+        x = _randn((4, n), 80, torch.float32, 4.0).double()
+        x = (x + offset).clamp(torch.finfo(dtype).min, torch.finfo(dtype).max).to(dtype)
+        x[1, ::2] = float("-inf")
+        x[2, 3] = offset / 2
+        labels = torch.tensor([1, 1, 3, 5])
+        r, want = _check_logp(dev, R, x, 2, labels)
+        g = [_randn((4,), 81 + i) for i in range(2)]
+        got = R.log_probs_backward(x.to(dev), r, labels.to(dev), *(v.to(dev) for v in g))
+        grad, bound = want.backward(labels.numpy(), *(f64(v) for v in g))
+        assert worst(f64(got), grad, bound + _rounded(dtype, grad)) <= 1
 
 
 def test_log_prob_function(dev, R):
