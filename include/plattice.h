@@ -377,7 +377,8 @@ int plattice_linear_backward(const plattice_linear_args* args, void* stream);
 
 /* Rows from labels: y[i] = scale * table[ids[i]] with table [n][c], both in
  * `dtype`; ids are int64 (ids_wide != 0) or int32.  An id outside 0..n-1 (the
- * "ignored" of label maps) gives a row of zeros.  n < 2^31, c <= 2^21. */
+ * "ignored" of label maps) gives a row of zeros.  n < 2^31, c <= 2^21; scale is
+ * finite. */
 int plattice_embed(void* y, const void* ids, int ids_wide, const void* table, int dtype, float scale,
                    long long count, long long n, int c, void* stream);
 
@@ -397,7 +398,9 @@ int plattice_embed_backward(void* grad_table, int table_dtype, const void* grad_
  * last to the first with reverse.  last [lines][c]: h after the last step taken
  * (NULL: not wanted).  states (NULL: not kept) [lines][ceil(steps / 16)][c]
  * float32: h before every 16th step taken, what the backward starts from.  The
- * recurrence is held in float32; h is its rounding.
+ * recurrence is held in float32; h is its rounding.  Long lines are cut into
+ * pieces whose gates are multiplied together: gates beyond 1 in magnitude have to
+ * leave those products in float32 wherever the state is not 0.
  *
  * Backward, with G[t] = grad_h[t] + gate[t+1] G[t+1] (grad_last, if any, in the
  * place of gate[t+1] G[t+1] after the last step):

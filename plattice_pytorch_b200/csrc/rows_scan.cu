@@ -170,8 +170,12 @@ template <bool kBlend> __device__ __forceinline__ float input(float a, float x) 
 // f s + r.  The second one's CTAs each go through the CTAs before them, then
 // through their own pieces, and know every piece's first state.
 
+// Gates beyond 1 can take a piece's factor f past float32 where no state is: a state
+// of 0 stays r, and a gate of 0 makes the factor 0 (infinity times 0 would be NaN).
+__device__ __forceinline__ float apply(float2 map, float s) { return s == 0.f ? map.y : fmaf(map.x, s, map.y); }
+__device__ __forceinline__ float joined(float f, float g) { return g == 0.f || f == 0.f ? 0.f : f * g; }
 __device__ __forceinline__ float2 then(float2 first, float2 second) {   // the map of both
-    return make_float2(first.x * second.x, fmaf(second.x, first.y, second.y));
+    return make_float2(joined(first.x, second.x), apply(second, first.y));
 }
 
 // Pieces of a backward pass are gone through from the last on.
@@ -201,7 +205,7 @@ __global__ void __launch_bounds__(kThreads) k_scan_sums(const __grid_constant__ 
                     for (int j = 0; j < V; ++j) {
                         const float gate = a.v[t].at(j), v = x.v[t].at(j);
                         r[j] = kGrad ? gate * (v + r[j]) : fmaf(gate, r[j], input<kBlend>(gate, v));
-                        f[j] *= gate;
+                        f[j] = joined(f[j], gate);
                     }
                 }
             }
@@ -256,8 +260,7 @@ __device__ __forceinline__ void first_state(float (&s)[V], const ScanArgs& p, co
         for (int k = 0; k < p.pieces; ++k)
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const float2 m = shared[(k * p.lanes + w.lane) * V + j];
-                s[j] = fmaf(m.x, s[j], m.y);
+                s[j] = apply(shared[(k * p.lanes + w.lane) * V + j], s[j]);
             }
         const float2* sums = p.sums + (w.line * p.tiles + w.tile) * p.pieces * p.c + w.col;
         for (int k = 0; k < (kGrad ? p.pieces - 1 - w.own : w.own); ++k) {
@@ -265,8 +268,7 @@ __device__ __forceinline__ void first_state(float (&s)[V], const ScanArgs& p, co
             if ((w.tile * p.pieces + other) * p.piece_blocks < p.blocks)
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    const float2 m = sums[(int64_t)other * p.c + j];
-                    s[j] = fmaf(m.x, s[j], m.y);
+                    s[j] = apply(sums[(int64_t)other * p.c + j], s[j]);
                 }
         }
     }

@@ -116,6 +116,27 @@ def test_what_is_not_finite_stays_behind_a_later_step(dev, R):
             assert not torch.isfinite(h[0, t // 2:, 0]).any() and not torch.isfinite(last[0, 0])
 
 
+def test_gates_beyond_one_where_nothing_is(dev, R):
+    """Products of the gates pass float32 while the state is 0; a gate of 0 and what comes
+    behind it are as if they had not."""
+    for t in (400, 5000, 30000):
+        x, a = torch.zeros(1, t, 3), torch.full((1, t, 3), 2.0)
+        half = t // 2 + 5
+        a[:, half], a[:, half + 1:] = 0.0, 0.75
+        x[:, half:] = torch.randn(1, t - half, 3, generator=torch.Generator().manual_seed(37))
+        h, eh, last, el = ref.scan(f64(x), f64(a))
+        got, glast, states = R.scan(x.to(dev), a.to(dev), keep=True)
+        assert worst(f64(got), h, eh + _rounded(torch.float32, h)) <= 1 and worst(f64(glast), last, el + 2.0 ** -149) <= 1
+        g = torch.zeros(1, t, 3)   # and backwards: gradients only before the large gates
+        g[:, :20] = 1.0
+        a2 = torch.full((1, t, 3), 0.5)
+        a2[:, 40:] = 2.0
+        _, _, states = R.scan(torch.zeros_like(x).to(dev), a2.to(dev), keep=True)
+        want, bound = ref.scan_backward(f64(g), np.zeros(x.shape), f64(a2))
+        for v, w, b in zip(R.scan_backward(g.to(dev), torch.zeros_like(x).to(dev), a2.to(dev), states), want, bound):
+            assert worst(f64(v), w, b + _rounded(torch.float32, w)) <= 1
+
+
 def test_unaligned_lines(dev, R):
     for dtype in TYPES:
         x, a, s, gy, gl = (v.to(dev) for v in _inputs((3,), 70, 16, dtype, 33))
