@@ -5,18 +5,22 @@
 //
 // The gradient of a small table (up to kSmallTable labels) is added up in shared
 // memory as the rows come: every warp has a copy of some of the table's channels of
-// its own, CTAs' sums are added by a second kernel.  For a larger table the
-// positions are sorted by label (by counting smaller ones, or a stable radix sort,
-// 8 to 10 bits of the label a pass), the sorted list is cut into chunks of equal length
+// its own, CTAs' sums are added by a second kernel.  For a larger table, or fewer
+// labels, the positions are sorted by label (by counting smaller ones, or a stable radix
+// sort, 8 to 10 bits of the label a pass), the sorted list is cut into chunks of equal length
 // and each chunk's runs of equal labels are added in registers.  A run inside one
 // chunk is written at once; the parts of a run that crosses chunks go to the
 // workspace and are added in order by another kernel.  The order of the sums
 // depends on the sizes alone: no atomics but counts.
+#include <cooperative_groups.h>
+
 #include "plattice_runtime.h"
 #include "rows_host.h"
 #include "rows_vec.cuh"
 
 namespace plr {
+
+namespace cg = cooperative_groups;
 
 // `lanes` (a power of two) threads a row side by side, four rows a thread, so that
 // labels, table rows and stores of four are under way together.
@@ -107,9 +111,10 @@ __device__ __forceinline__ void store_out(void* out, int dtype, bool vec, int64_
 // Where a row has fewer than 32 V channels, several rows go side by side, each
 // group of lanes with a copy.  Warps of a CTA take slabs of 32 V channels first,
 // then rows.  The rows come by asynchronous copies, two blocks of 32 under way
-// (loads to registers, 16 rows under way, left the warps waiting: 1048576 rows of 64
-// bfloat16 channels into 21 labels 63 us; sorted 210 us).  Rows on no 16-byte
-// boundaries are loaded a block at a time.
+// (1048576 rows of 64 bfloat16 channels into 21 labels: 51 us, bound by the few warps
+// that the copies of the table leave an SM; from loads to registers 63, sorted 210).
+// Rows on no 16-byte boundaries are loaded a block at a time.  kWideTable: labels up to
+// which a lane takes 8 bytes of 16-bit rows.
 
 constexpr int kSmallTable = 96, kWideTable = 24, kTableBytes = 200 * 1024;
 
@@ -254,7 +259,8 @@ __global__ void __launch_bounds__(256) k_small_join(void* out, int dtype, const 
 // --------------------------------------------------------------- sorting labels
 
 constexpr int kMostBits = 10;       // of a label, a pass
-constexpr int kRankSorted = 8192;   // as many are sorted by counting
+constexpr int kRankSorted = 2048;      // as many are sorted by counting
+constexpr int kClusterSorted = 32768;  // as many by one cluster
 
 struct Entry { unsigned label, at; };   // at: the position in ids
 
@@ -274,7 +280,6 @@ struct Zeros {
 
 // A label's place: the labels below it and the equal ones before it.  A CTA has all
 // labels in shared memory and places 64; sixteen threads share a label's comparisons.
-// 8192 labels are 67 M comparisons; the passes below are two launches a digit.
 __global__ void __launch_bounds__(1024) k_rank_sort(Entry* __restrict__ out, unsigned* __restrict__ valid, unsigned* __restrict__ starts, Labels ids, int64_t n,
                                                    int count, Zeros zeros) {
     if ((int)blockIdx.x * 64 >= count) return zeros.share(blockIdx.x - (count + 63) / 64);
@@ -485,6 +490,102 @@ __global__ void __launch_bounds__(256) k_sort_place(Entry* __restrict__ out, con
         if (digit[k] < kDigits) out[h[warp][digit[k]] + rank[k]] = e[k];
 }
 
+// All passes in one launch, by a cluster: CTA r has entries 4096 r.. of each pass.  The
+// CTAs read each other's counts out of shared memory; the entries go through memory
+// (16384 labels of 50000: 27 us as launches of the kernels above).
+constexpr int kSortCtas = 8, kSortItems = 4;
+
+__global__ void __cluster_dims__(kSortCtas) __launch_bounds__(1024) k_cluster_sort(Entry* first, Entry* second, unsigned* valid,
+                                                                                unsigned* starts, Labels ids, int64_t n, int count,
+                                                                                int passes, int bits, Zeros zeros) {
+    if (blockIdx.x >= kSortCtas) return zeros.share(blockIdx.x - kSortCtas);   // whole clusters
+    extern __shared__ unsigned h[];   // [32][digits + 1], then of the CTA [digits], then where they begin [digits]
+    __shared__ unsigned warps[32];
+    const cg::cluster_group cluster = cg::this_cluster();
+    const int digits = 1 << bits, rank_of = (int)cluster.block_rank(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5,
+              d = threadIdx.x;
+    unsigned *own = h + warp * (digits + 1), *totals = h + 32 * (digits + 1), *begins = totals + digits;
+    int size = count;
+    Entry *from = nullptr, *to = first;
+    for (int pass = 0; pass < passes; ++pass) {
+        for (int i = threadIdx.x; i < 32 * (digits + 1); i += 1024) h[i] = 0;
+        Entry e[kSortItems];
+        int digit[kSortItems];
+        unsigned rank[kSortItems];
+        const int base = rank_of * (1024 * kSortItems) + warp * (32 * kSortItems) + lane;
+#pragma unroll
+        for (int k = 0; k < kSortItems; ++k) {
+            const int i = base + k * 32;
+            digit[k] = digits;
+            if (i < size) {
+                if (from) {   // written by the cluster's other CTAs: not from this SM's cache
+                    const uint2 q = __ldcg(reinterpret_cast<const uint2*>(from) + i);
+                    e[k] = Entry{q.x, q.y};
+                    digit[k] = (e[k].label >> (bits * pass)) & (digits - 1);
+                } else if (const int id = ids.at(i, n); id >= 0) {
+                    e[k] = Entry{(unsigned)id, (unsigned)i};
+                    digit[k] = id & (digits - 1);
+                }
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kSortItems; ++k) {
+            const unsigned same = __match_any_sync(0xffffffffu, digit[k]);
+            const unsigned had = own[digit[k]];
+            rank[k] = had + __popc(same & ((1u << lane) - 1));
+            __syncwarp();
+            if ((same & ((1u << lane) - 1)) == 0) own[digit[k]] = had + __popc(same);
+            __syncwarp();
+        }
+        __syncthreads();
+        if (d < digits) {   // counts of the warps before, and of the CTA
+            unsigned o = 0;
+#pragma unroll 8
+            for (int w = 0; w < 32; ++w) {
+                const unsigned had = h[w * (digits + 1) + d];
+                h[w * (digits + 1) + d] = o;
+                o += had;
+            }
+            totals[d] = o;
+        }
+        cluster.sync();
+        unsigned before = 0, all = 0;
+        if (d < digits)
+#pragma unroll
+            for (int c = 0; c < kSortCtas; ++c) {
+                const unsigned v = *cluster.map_shared_rank(totals + d, c);
+                all += v;
+                if (c < rank_of) before += v;
+            }
+        unsigned s = all;   // exclusive sum over the digits
+#pragma unroll
+        for (int q = 1; q < 32; q <<= 1) {
+            const unsigned t = __shfl_up_sync(0xffffffffu, s, q);
+            if (lane >= q) s += t;
+        }
+        if (lane == 31) warps[warp] = s;
+        __syncthreads();
+        unsigned w = warps[lane];
+#pragma unroll
+        for (int q = 1; q < 32; q <<= 1) {
+            const unsigned t = __shfl_up_sync(0xffffffffu, w, q);
+            if (lane >= q) w += t;
+        }
+        size = (int)__shfl_sync(0xffffffffu, w, 31);
+        const unsigned front = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
+        if (d < digits) begins[d] = (warp ? front : 0u) + s - all + before;
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kSortItems; ++k)
+            if (digit[k] < digits) to[begins[digit[k]] + own[digit[k]] + rank[k]] = e[k];
+        cluster.sync();   // the entries are there, and the counts have been read
+        from = to;
+        to = to == first ? second : first;
+    }
+    if (rank_of == 0 && threadIdx.x == 0) *valid = (unsigned)size, *starts = 0;
+}
+
 // ------------------------------------------------------------------ sums of runs
 
 struct RunArgs {
@@ -618,9 +719,16 @@ __global__ void __launch_bounds__(32 * kJoinWarps) k_join_runs(const __grid_cons
             chunk = a.starts[1 + i];
             const unsigned label = a.sorted[(chunk + 1) * a.length].label;
             parts = 1;
-            for (int count = 32; count == 32; parts += count) {
-                const int64_t at = (chunk + 1 + parts + lane) * a.length;
-                count = __popc(__ballot_sync(0xffffffffu, at < valid && a.sorted[at < valid ? at : 0].label == label));
+            for (int count = 128; count == 128; parts += count) {
+                bool same[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int64_t at = (chunk + 1 + parts + 32 * u + lane) * a.length;
+                    same[u] = at < valid && a.sorted[at < valid ? at : 0].label == label;
+                }
+                count = 0;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) count += __popc(__ballot_sync(0xffffffffu, same[u]));
             }
             if (parts <= kLongRun)
                 for (int64_t col = col0; col < a.c; col += next) {
@@ -709,7 +817,7 @@ static EmbedPlan embed_plan(int64_t count, int64_t n, int c, int element) {
         p.passes = (bits + kMostBits - 1) / kMostBits;
         p.bits = (bits + p.passes - 1) / p.passes < 8 ? 8 : (bits + p.passes - 1) / p.passes;
         p.items = count <= 262144 ? 4 : 16;
-        p.tiles = (int)ceil_div(count, 256 * p.items);
+        p.tiles = count <= kClusterSorted ? 0 : (int)ceil_div(count, 256 * p.items);   // 0: by one cluster
     }
     // chunks long enough that few runs cross them, short enough that they fill the device
     const int64_t want = count * ceil_div(c, 8) / (148 * 2048);
@@ -779,7 +887,7 @@ static void sort_pass(Entry* to, unsigned* counts, unsigned* totals, unsigned* v
 // The labels in order with their positions; `bytes` of the table (a multiple of
 // 16) are zeroed on the way.
 static const Entry* sort_labels(const EmbedPlan& p, uint8_t* ws, const Labels& ids, int64_t count, int64_t n, void* table, int64_t bytes,
-                                cudaStream_t s) {
+                                cudaError_t* error, cudaStream_t s) {
     unsigned *valid = reinterpret_cast<unsigned*>(ws), *totals = reinterpret_cast<unsigned*>(ws + p.totals),
              *starts = reinterpret_cast<unsigned*>(ws + p.starts), *counts = reinterpret_cast<unsigned*>(ws + p.counts);
     Entry *to = reinterpret_cast<Entry*>(ws + p.first), *other = reinterpret_cast<Entry*>(ws + p.second), *from = nullptr;
@@ -787,6 +895,22 @@ static const Entry* sort_labels(const EmbedPlan& p, uint8_t* ws, const Labels& i
         const Zeros z = zeros_of(table, bytes, 0, 1);
         k_rank_sort<<<(unsigned)ceil_div(count, 64) + z.ctas, 1024, 0, s>>>(to, valid, starts, ids, n, (int)count, z);
         return to;
+    }
+    if (p.tiles == 0) {
+        Zeros z = zeros_of(table, bytes, 0, 1);
+        z.ctas = (z.ctas + kSortCtas - 1) / kSortCtas * kSortCtas;
+        int unused = 0;
+        *error = pl::kernel_once(
+            reinterpret_cast<const void*>(k_cluster_sort),
+            [](int*) {
+                return cudaFuncSetAttribute(k_cluster_sort, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                            (32 * ((1 << kMostBits) + 1) + (2 << kMostBits)) * 4);
+            },
+            &unused);
+        const size_t smem = (32 * ((1 << p.bits) + 1) + (2 << p.bits)) * sizeof(unsigned);
+        if (*error == cudaSuccess)
+            k_cluster_sort<<<kSortCtas + z.ctas, 1024, smem, s>>>(to, other, valid, starts, ids, n, (int)count, p.passes, p.bits, z);
+        return p.passes % 2 ? to : other;
     }
     for (int pass = 0; pass < p.passes; ++pass) {
         const Source src{ids, n, count, from, valid};
@@ -850,8 +974,8 @@ static cudaError_t launch_runs(int v, const RunArgs& a, int64_t chunks, cudaStre
 
 static cudaError_t join_runs(const RunArgs& a, int64_t chunks, cudaStream_t s) {
     const int v = a.c % 4 == 0 ? 4 : 1;
-    const int64_t strips = ceil_div(a.c, 32 * v), x = chunks - 1 < 296 ? chunks - 1 : 296, most = 592 / x;
-    const dim3 grid((unsigned)x, (unsigned)(strips < most ? strips : most));
+    const int64_t strips = ceil_div(a.c, 32 * v), x = chunks - 1 < 296 ? chunks - 1 : 296;
+    const dim3 grid((unsigned)x, (unsigned)(strips < 4 ? strips : 4));
     int lanes = 1;
     while (lanes < 32 && lanes * v < a.c) lanes <<= 1;
     if (v == 4) k_join_runs<4><<<grid, 32 * kJoinWarps, 0, s>>>(a, lanes);
@@ -922,8 +1046,8 @@ int plattice_embed_backward(void* grad_table, int table_dtype, const void* grad_
     if (whole < bytes) e = cudaMemsetAsync(static_cast<uint8_t*>(grad_table) + whole, 0, bytes - whole, s);
     if (count == 0 || e != cudaSuccess) return rows_status(e, "plattice_embed_backward");
     unsigned* starts = reinterpret_cast<unsigned*>(ws + p.starts);
-    const Entry* sorted = sort_labels(p, ws, labels, count, n, grad_table, (int64_t)whole, s);
-    e = cudaGetLastError();
+    const Entry* sorted = sort_labels(p, ws, labels, count, n, grad_table, (int64_t)whole, &e, s);
+    if (e == cudaSuccess) e = cudaGetLastError();
     if (e != cudaSuccess) return rows_status(e, "plattice_embed_backward");
     const int v = widest(c, dtype_size(dtype), (uintptr_t)grad_y);
     const RunArgs a{grad_table, table_dtype, reinterpret_cast<float*>(ws + p.part), sorted, reinterpret_cast<unsigned*>(ws), starts, grad_y, scale,

@@ -10,14 +10,14 @@
 // largest score out, so that s = log1p(rest) and the log probability of a
 // confident answer keep their precision.
 //
-// A row is read once and held: few classes by a thread out of shared memory,
-// up to five accesses a lane by a warp in registers, more by a CTA or a
-// cluster of them in registers, and only rows that no cluster holds are read
-// again.  So the largest score is known before the first exponential, which
-// costs a subtraction, a product, a bound, the exponential and two sums (five
-// instructions an element in pairs; the special function unit takes one element
-// in 16 a clock and SM, 60 us for the 268 M of 8192 x 32768, which take 83 us to
-// read).
+// A row is read once and held: few classes by a thread out of shared memory, up to
+// five accesses a lane by a warp in registers, more by the warps of a CTA or a
+// cluster, each with a share of its own; rows that no cluster holds are taken in
+// rounds.  So a thread, a warp or a share knows its largest score before the first
+// exponential, and an element costs a bound, a multiply-add, the exponential and two
+// sums, most of them in pairs.  The special function units take 16 elements a clock
+// and SM, 60 us for the 268 M of 8192 x 32768, which take 83 us to read at the copy
+// rate and 95 here.
 #pragma once
 #include <cooperative_groups.h>
 
@@ -824,9 +824,9 @@ __global__ void __launch_bounds__(kThreads, kThreads == 512 ? 2 : kThreads == 25
 
 // ------------------------------------------------------------- few classes
 
-// (198959 x 48 in float32 with 20 alternatives, for each of which a thread looks through
-// its row again: 151 us; a warp a row takes 267.)
-// Up to 256 bytes of classes: 858914 x 73 in float16 with 3 alternatives, a warp a row, 390.
+// A thread a row, up to 256 bytes of classes: 858914 x 73 in float16 with 3
+// alternatives 140 us, a warp a row 390; 198959 x 48 in float32 with 20, for each of
+// which a thread looks through its row again, 151 us and 267.
 constexpr int kFewBytes = 256, kTileRows = 128;
 
 // A tile of rows lies in memory as one stretch: 16 bytes at a time (its start

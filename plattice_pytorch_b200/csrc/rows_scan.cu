@@ -178,6 +178,27 @@ __device__ __forceinline__ float2 then(float2 first, float2 second) {   // the m
     return make_float2(joined(first.x, second.x), apply(second, first.y));
 }
 
+// The maps of a CTA's pieces (`place`: in the order they are gone through), each after
+// all before it, are left in `shared`: in pairs, so that many pieces of few channels
+// take as many steps as their number has bits (one by one: 169 lines of 2661 x 2, 28 us).
+template <int V>
+__device__ __forceinline__ void scan_maps(float2 (&m)[V], float2* shared, int place, int lane, const ScanArgs& p) {
+    for (int d = 1; d < p.pieces; d <<= 1) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) shared[(place * p.lanes + lane) * V + j] = m[j];
+        __syncthreads();
+        float2 o[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[j] = place >= d ? shared[((place - d) * p.lanes + lane) * V + j] : make_float2(1.f, 0.f);
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < V; ++j) m[j] = then(o[j], m[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) shared[(place * p.lanes + lane) * V + j] = m[j];
+    __syncthreads();
+}
+
 // Pieces of a backward pass are gone through from the last on.
 template <typename T, int V, bool kBlend, bool kGrad>
 __global__ void __launch_bounds__(kThreads) k_scan_sums(const __grid_constant__ ScanArgs p) {
@@ -205,27 +226,27 @@ __global__ void __launch_bounds__(kThreads) k_scan_sums(const __grid_constant__ 
                     for (int j = 0; j < V; ++j) {
                         const float gate = a.v[t].at(j), v = x.v[t].at(j);
                         r[j] = kGrad ? gate * (v + r[j]) : fmaf(gate, r[j], input<kBlend>(gate, v));
-                        f[j] = joined(f[j], gate);
+                        f[j] *= gate;
                     }
                 }
             }
         }
+        // infinity times a gate of 0 (a gate that is itself NaN makes r NaN)
+#pragma unroll
+        for (int j = 0; j < V; ++j) f[j] = f[j] == f[j] ? f[j] : 0.f;
         if (w.first < p.blocks)
 #pragma unroll
             for (int j = 0; j < V; ++j)
                 p.sums[(w.line * p.tiles * p.pieces + w.piece) * p.c + w.col + j] = make_float2(f[j], r[j]);
     }
+    float2 m[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) shared[threadIdx.x * V + j] = make_float2(f[j], r[j]);
-    __syncthreads();
+    for (int j = 0; j < V; ++j) m[j] = make_float2(f[j], r[j]);
+    scan_maps(m, shared, kGrad ? p.pieces - 1 - w.own : w.own, w.lane, p);
     if (w.own == 0 && w.here)
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            float2 all = make_float2(1.f, 0.f);
-            for (int k = 0; k < p.pieces; ++k)
-                all = then(all, shared[((kGrad ? p.pieces - 1 - k : k) * p.lanes + w.lane) * V + j]);
-            p.tile_sums[(w.line * p.tiles + w.tile) * p.c + w.col + j] = all;
-        }
+        for (int j = 0; j < V; ++j)
+            p.tile_sums[(w.line * p.tiles + w.tile) * p.c + w.col + j] = shared[((p.pieces - 1) * p.lanes + w.lane) * V + j];
 }
 
 // The state that the thread's piece starts from: s goes through the maps of the
@@ -253,25 +274,21 @@ __device__ __forceinline__ void first_state(float (&s)[V], const ScanArgs& p, co
                 for (int j = 0; j < V; ++j) all[j] = then(all[j], m[i][j]);
         }
     }
+    // The piece's own map is on its way while the CTAs' are joined.
+    const int place = kGrad ? p.pieces - 1 - w.own : w.own;
+    float2 m[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) shared[threadIdx.x * V + j] = all[j];
+    for (int j = 0; j < V; ++j)
+        m[j] = w.here && w.first < p.blocks ? p.sums[((w.line * p.tiles + w.tile) * p.pieces + w.own) * p.c + w.col + j]
+                                            : make_float2(1.f, 0.f);
+    scan_maps(all, shared, w.own, w.lane, p);
+#pragma unroll
+    for (int j = 0; j < V; ++j) s[j] = apply(shared[((p.pieces - 1) * p.lanes + w.lane) * V + j], s[j]);
     __syncthreads();
-    if (w.here) {
-        for (int k = 0; k < p.pieces; ++k)
+    scan_maps(m, shared, place, w.lane, p);
+    if (place)
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                s[j] = apply(shared[(k * p.lanes + w.lane) * V + j], s[j]);
-            }
-        const float2* sums = p.sums + (w.line * p.tiles + w.tile) * p.pieces * p.c + w.col;
-        for (int k = 0; k < (kGrad ? p.pieces - 1 - w.own : w.own); ++k) {
-            const int other = kGrad ? p.pieces - 1 - k : k;
-            if ((w.tile * p.pieces + other) * p.piece_blocks < p.blocks)
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    s[j] = apply(sums[(int64_t)other * p.c + j], s[j]);
-                }
-        }
-    }
+        for (int j = 0; j < V; ++j) s[j] = apply(shared[((place - 1) * p.lanes + w.lane) * V + j], s[j]);
 }
 
 // ---------------------------------------------------------------- the passes

@@ -84,7 +84,8 @@ def test_gradients_that_are_not_finite(dev, R, count, n):
 
 EMBED_SIZES = [((1,), 1, 1), ((7,), 5, 3), ((13, 29), 21, 50), ((100,), 1000, 64), ((3, 5, 2), 4, 1030), ((4097,), 33, 8),
                ((9000,), 3, 8), ((20000,), 257, 24), ((5000,), 70000, 16), ((2,), 3, 4096), ((0,), 3, 8), ((40000,), 1, 17),
-               ((70000,), 21, 64), ((300,), 256, 2048), ((8192,), 97, 2), ((8193,), 300, 4), ((300000,), 96, 6),
+               ((70000,), 21, 64), ((300,), 256, 2048), ((8192,), 97, 2), ((8193,), 300, 4), ((2049,), 1100, 3), ((32768,), 70000, 2), ((32769,), 2000, 2),
+               ((20011,), 5, 24), ((300000,), 96, 6),
                ((500,), 12, 5000), ((300000,), 200000, 1), ((1200000,), 1000, 1)]
 
 
@@ -163,7 +164,7 @@ def _scores(rows, n, dtype, seed, masked=True):
 
 
 LOGP_SIZES = [(1, 1), (5, 2), (40, 3), (33, 21), (257, 32), (9, 33), (20, 100), (3, 255), (70, 256), (12, 1000), (6, 1024),
-              (4, 2050), (5, 5003), (2, 33000), (1, 70001), (150, 4096), (0, 7), (2, 131072), (300, 64), (130, 65), (300, 127), (129, 128), (200, 129), (1, 300001), (200, 40000)]
+              (4, 2050), (5, 5003), (2, 33000), (1, 70001), (150, 4096), (0, 7), (2, 131072), (300, 64), (130, 65), (300, 127), (129, 128), (200, 129), (1, 300001), (40, 40000)]
 
 
 def _check_logp(dev, R, x, top, labels):
