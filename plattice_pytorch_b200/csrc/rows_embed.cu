@@ -668,8 +668,7 @@ __global__ void __launch_bounds__(256) k_runs(const __grid_constant__ RunArgs a)
 }
 
 // The runs that begin in a chunk and go on behind it: its part and those of the
-// chunks up to the run's end, in order.  A warp a run, 32 V channels at a time
-// (blockIdx.y has others); runs of more than kLongRun parts by the CTA: `lanes` threads
+// chunks up to the run's end, in order.  A warp 32 V channels of a run; runs of more than kLongRun parts by the CTA: `lanes` threads
 // of V channels side by side, each such group takes every groups-th part, and theirs
 // are added in pairs.
 constexpr int kLongRun = 24, kJoinWarps = 16;
@@ -692,13 +691,14 @@ __device__ __forceinline__ void add_parts(float (&s)[V], const RunArgs& a, int64
 }
 
 template <int V>
-__global__ void __launch_bounds__(32 * kJoinWarps) k_join_runs(const __grid_constant__ RunArgs a, int lanes) {
+__global__ void __launch_bounds__(32 * kJoinWarps, 2) k_join_runs(const __grid_constant__ RunArgs a, int lanes) {
     __shared__ float sums[kJoinWarps * 32 * V];
-    __shared__ int64_t long_chunk[kJoinWarps], long_parts[kJoinWarps];
+    __shared__ int64_t long_chunk[kJoinWarps], long_parts[kJoinWarps], long_first[kJoinWarps];
     const unsigned starts = a.starts[0];
     const int64_t valid = *a.valid;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t col0 = ((int64_t)blockIdx.y * 32 + lane) * V, next = (int64_t)gridDim.y * 32 * V;
+    const unsigned strips = (unsigned)((a.c + 32 * V - 1) / (32 * V));
+    const uint64_t items = (uint64_t)starts * strips;
     const auto tail = [&](float (&s)[V], int64_t chunk, int64_t col) {   // the run's first part
         Vec<float, V> v;
         v.load(a.part + (chunk * 2 + 1) * a.c + col);
@@ -710,13 +710,15 @@ __global__ void __launch_bounds__(32 * kJoinWarps) k_join_runs(const __grid_cons
 #pragma unroll
         for (int j = 0; j < V; ++j) store_param(a.out, a.out_dtype, at + j, s[j] * a.scale);
     };
-    // runs a CTA takes at a time: few where there are few, so that each has a CTA
-    const unsigned spread = (starts + gridDim.x - 1) / gridDim.x, each = spread < kJoinWarps ? spread : kJoinWarps;
-    for (unsigned i0 = blockIdx.x * each; i0 < starts; i0 += gridDim.x * each) {
-        const unsigned i = warp < each ? i0 + warp : starts;
+    // items a CTA takes at a time: few where there are few, so that they spread
+    const uint64_t spread = (items + gridDim.x - 1) / gridDim.x;
+    const unsigned each = spread < kJoinWarps ? (unsigned)spread : kJoinWarps;
+    for (uint64_t i0 = (uint64_t)blockIdx.x * each; i0 < items; i0 += (uint64_t)gridDim.x * each) {
+        const uint64_t i = warp < each ? i0 + warp : items;
         int64_t chunk = 0, parts = 0;   // chunks behind this one that the run reaches: those that begin with its label
-        if (i < starts) {
-            chunk = a.starts[1 + i];
+        if (i < items) {
+            const unsigned run = (unsigned)(i / strips), strip = (unsigned)(i - (uint64_t)run * strips);
+            chunk = a.starts[1 + run];
             const unsigned label = a.sorted[(chunk + 1) * a.length].label;
             parts = 1;
             for (int count = 128; count == 128; parts += count) {
@@ -730,13 +732,14 @@ __global__ void __launch_bounds__(32 * kJoinWarps) k_join_runs(const __grid_cons
 #pragma unroll
                 for (int u = 0; u < 4; ++u) count += __popc(__ballot_sync(0xffffffffu, same[u]));
             }
-            if (parts <= kLongRun)
-                for (int64_t col = col0; col < a.c; col += next) {
-                    float s[V];
-                    tail(s, chunk, col);
-                    add_parts(s, a, chunk, col, 1, parts, 1);
-                    write(s, chunk, col);
-                }
+            const int64_t col = ((int64_t)strip * 32 + lane) * V;
+            if (parts <= kLongRun && col < a.c) {
+                float s[V];
+                tail(s, chunk, col);
+                add_parts(s, a, chunk, col, 1, parts, 1);
+                write(s, chunk, col);
+            }
+            if (lane == 0) long_first[warp] = (int64_t)strip * 32 * V;
         }
         if (lane == 0) {
             long_chunk[warp] = chunk;
@@ -746,26 +749,24 @@ __global__ void __launch_bounds__(32 * kJoinWarps) k_join_runs(const __grid_cons
         for (int w = 0; w < kJoinWarps; ++w) {
             if (long_parts[w] <= kLongRun) continue;
             const int group = threadIdx.x / lanes, groups = 32 * kJoinWarps / lanes, at = threadIdx.x % lanes * V;
-            for (int64_t first = (int64_t)blockIdx.y * lanes * V; first < a.c; first += (int64_t)gridDim.y * lanes * V) {
-                const int64_t col = first + at;
-                float s[V];
+            const int64_t col = long_first[w] + at;
+            float s[V];
 #pragma unroll
-                for (int j = 0; j < V; ++j) s[j] = 0.f;
-                if (col < a.c) {
-                    if (group == 0) tail(s, long_chunk[w], col);
-                    add_parts(s, a, long_chunk[w], col, 1 + group, long_parts[w], groups);
-                }
-                for (int d = groups / 2; d; d >>= 1) {
-#pragma unroll
-                    for (int j = 0; j < V; ++j) sums[threadIdx.x * V + j] = s[j];
-                    __syncthreads();
-                    if (group < d)
-#pragma unroll
-                        for (int j = 0; j < V; ++j) s[j] += sums[(threadIdx.x + d * lanes) * V + j];
-                    __syncthreads();
-                }
-                if (group == 0 && col < a.c) write(s, long_chunk[w], col);
+            for (int j = 0; j < V; ++j) s[j] = 0.f;
+            if (col < a.c) {
+                if (group == 0) tail(s, long_chunk[w], col);
+                add_parts(s, a, long_chunk[w], col, 1 + group, long_parts[w], groups);
             }
+            for (int d = groups / 2; d; d >>= 1) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) sums[threadIdx.x * V + j] = s[j];
+                __syncthreads();
+                if (group < d)
+#pragma unroll
+                    for (int j = 0; j < V; ++j) s[j] += sums[(threadIdx.x + d * lanes) * V + j];
+                __syncthreads();
+            }
+            if (group == 0 && col < a.c) write(s, long_chunk[w], col);
         }
         __syncthreads();
     }
@@ -974,8 +975,8 @@ static cudaError_t launch_runs(int v, const RunArgs& a, int64_t chunks, cudaStre
 
 static cudaError_t join_runs(const RunArgs& a, int64_t chunks, cudaStream_t s) {
     const int v = a.c % 4 == 0 ? 4 : 1;
-    const int64_t strips = ceil_div(a.c, 32 * v), x = chunks - 1 < 296 ? chunks - 1 : 296;
-    const dim3 grid((unsigned)x, (unsigned)(strips < 4 ? strips : 4));
+    const int64_t items = (chunks - 1) * ceil_div(a.c, 32 * v);
+    const unsigned grid = (unsigned)(items < 296 ? items : 296);   // one round
     int lanes = 1;
     while (lanes < 32 && lanes * v < a.c) lanes <<= 1;
     if (v == 4) k_join_runs<4><<<grid, 32 * kJoinWarps, 0, s>>>(a, lanes);
