@@ -406,7 +406,8 @@ int plattice_embed_backward(void* grad_table, int table_dtype, const void* grad_
  * place of gate[t+1] G[t+1] after the last step):
  *   grad_x = G, or (1 - gate) G with blend;  grad_gate[t] = G[t] h[t-1], or
  *   G[t] (h[t-1] - x[t]);  grad_state = gate[0] G[0] (NULL: not wanted).
- * h is computed again from states, in float32. */
+ * h is computed again from states, in float32.  The workspaces' sizes depend on
+ * the pointers' alignment: set the tensors before asking for them. */
 #define PLATTICE_SCAN_KEEP 16
 typedef struct plattice_scan_args {
     const void* x;
@@ -471,7 +472,7 @@ int plattice_log_probs_backward(const plattice_log_probs_args* args, void* strea
  *   out = g * min(1, max_norm / (norm + eps)), rounded to out_dtype
  * with out_dtype the tensor's type or PLATTICE_F32, out the tensor itself (in its
  * own type) or memory of its own; memory that any out shares with another tensor
- * is refused (PLATTICE_ERR_INVALID).  Squares are added in float32 by eights (in
+ * or with the norm is refused (PLATTICE_ERR_INVALID).  Squares are added in float32 by eights (in
  * float64 where those would not hold them) and then in float64, in an order that
  * the sizes fix.  norm_in (device, float32) non-NULL: the norm to use, such as
  * one over several processes; the gradients are then read only to be scaled.

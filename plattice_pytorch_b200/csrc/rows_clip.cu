@@ -414,7 +414,7 @@ int plattice_clip_grads(const plattice_grad* grads, int count, float max_norm, f
             if (g.size && ((uintptr_t)g.out % dtype_size(g.out_dtype) || (g.out == g.g && g.out_dtype != g.dtype)))
                 return PLATTICE_ERR_INVALID;
         }
-        Span* v = static_cast<Span*>(malloc(2 * (size_t)tensors * sizeof(Span)));
+        Span* v = static_cast<Span*>(malloc((2 * (size_t)tensors + 2) * sizeof(Span)));
         if (!v) return PLATTICE_ERR_WORKSPACE;
         int n = 0;
         for (int i = 0; i < count; ++i) {
@@ -423,6 +423,9 @@ int plattice_clip_grads(const plattice_grad* grads, int count, float max_norm, f
             v[n++] = {(uintptr_t)g.g, (uintptr_t)g.g + g.size * dtype_size(g.dtype), i, false};
             v[n++] = {(uintptr_t)g.out, (uintptr_t)g.out + g.size * dtype_size(g.out_dtype), i, true};
         }
+        // every CTA reads the norm given, some while others write
+        if (norm_in && norm_in != norm_out) v[n++] = {(uintptr_t)norm_in, (uintptr_t)norm_in + sizeof(float), count, false};
+        if (norm_out) v[n++] = {(uintptr_t)norm_out, (uintptr_t)norm_out + sizeof(float), count + 1, true};
         const bool bad = overlaps(grads, v, n);
         free(v);
         if (bad) return PLATTICE_ERR_INVALID;

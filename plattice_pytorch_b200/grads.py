@@ -81,7 +81,7 @@ def clip_grads(tensors, max_norm, out=None, norm=None, eps=1e-6):
     as one over the gradients of several processes.  ``max_norm`` may be infinite
     (``out`` is then a copy).  A norm that is not finite scales by 0 or NaN, as
     the formula says.  What is written may share no memory with another tensor of
-    either list, nor may a tensor that is scaled in place be listed twice."""
+    either list or with ``norm``, nor may a tensor that is scaled in place be listed twice."""
     if not isinstance(tensors, (list, torch.Tensor)):
         tensors = list(tensors)
     if not isinstance(out, (list, torch.Tensor, type(None))):

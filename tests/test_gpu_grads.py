@@ -140,6 +140,10 @@ def test_shared_memory_is_refused(dev, G):
     h = torch.zeros(100, dtype=torch.bfloat16, device=dev)
     with pytest.raises(RuntimeError, match="memory"):   # float32 over its own 16 bits
         G.clip_grads([whole[:50].view(torch.bfloat16)], 1.0, out=[whole[:100]])
+    one = torch.ones((), device=dev)
+    with pytest.raises(RuntimeError, match="memory"):   # the norm given
+        G.clip_grads([a, one], 1.0, norm=one)
+    G.clip_grads([one], 1.0, out=[torch.empty_like(one)], norm=one)   # only read
     # read twice, written apart: allowed
     out = [torch.empty_like(a), torch.empty_like(a)]
     norm = G.clip_grads([a, a], 1.0, out=out)

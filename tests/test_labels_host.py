@@ -155,15 +155,32 @@ def test_memory_that_clipped_gradients_may_not_share(lib):
         meet = lambda a, b: max(a[0], b[0]) < min(a[1], b[1])  # noqa: E731
         ins = [span(g, s, t) for g, o, s, t, u in items]
         outs = [span(o, s, u) for g, o, s, t, u in items]
+        if not any(s for _, _, s, _, _ in items):
+            continue
+        outs.append(span(FAKE.value, 1, 0))   # the norm
+        items.append((0, FAKE.value, 0, 0, 0))
+        ins.append((0, 0))
         shared = any(meet(outs[i], outs[j]) for i in range(len(items)) for j in range(i))
         shared |= any(meet(outs[i], ins[j]) and not (i == j and items[i][0] == items[i][1])
                       for i in range(len(items)) for j in range(len(items)))
-        if not any(s for _, _, s, _, _ in items):
-            continue
+        items.pop()
         rc = lib.plattice_clip_grads(_grads(*items), len(items), 1.0, 0.0, None, FAKE, None, 0, None)
         assert rc == (_lib.ERR_INVALID if shared else _lib.ERR_WORKSPACE), (items, shared)
         seen.add(shared)
     assert seen == {True, False}
+
+
+def test_the_norm_given_may_not_be_written_over(lib):
+    from plattice_pytorch_b200 import _lib
+    run = lambda norm_in, norm_out, g=4096, out=4096: lib.plattice_clip_grads(  # noqa: E731
+        _grads((g, out, 10, 0, 0), (4200, 4200, 0, 0, 0)), 2, 1.0, 0.0, norm_in, norm_out, None, 0, None)
+    at = ctypes.c_void_p
+    for norm in (4096, 4100, 4132):
+        assert run(at(norm), None) == run(at(norm), at(norm)) == run(None, at(norm)) == _lib.ERR_INVALID, norm
+        # read as a gradient, too: harmless, but not where it is written
+        assert run(None, at(norm), 4096, 8192) == run(at(norm), at(norm), 4096, 8192) == _lib.ERR_INVALID, norm
+    for norm in (4092, 4136):
+        assert run(None, at(norm)) == _lib.ERR_WORKSPACE
 
 
 @pytest.fixture
