@@ -825,8 +825,8 @@ __global__ void __launch_bounds__(kThreads, kThreads == 512 ? 2 : kThreads == 25
 // ------------------------------------------------------------- few classes
 
 // A thread a row, up to 256 bytes of classes: 858914 x 73 in float16 with 3
-// alternatives 140 us, a warp a row 390; 198959 x 48 in float32 with 20, for each of
-// which a thread looks through its row again, 151 us and 267.
+// alternatives 126 us, a warp a row 390; 198959 x 48 in float32 with 20, for each of
+// which a thread looks through its row again, 113 us and 267.
 constexpr int kFewBytes = 256, kTileRows = 128;
 
 // A tile of rows lies in memory as one stretch: 16 bytes at a time (its start
@@ -879,10 +879,11 @@ __device__ __forceinline__ void tile_copy(T* tile, T* x, int count, int n, bool 
 }
 
 // f(x, j) of a row's classes in order; 16-bit ones two at a time where n is even (rows
-// then begin on words).
+// then begin on words).  Four steps' classes are read together.
 template <typename T, typename F> __device__ __forceinline__ void each_class(const T* x, int n, const F& f) {
     if (sizeof(T) == 2 && n % 2 == 0) {
         const uint32_t* w = reinterpret_cast<const uint32_t*>(x);
+#pragma unroll 4
         for (int j = 0; j < n; j += 2, ++w) {
             Vec<T, 2> v;
             v.r.w[0] = *w;
@@ -890,6 +891,7 @@ template <typename T, typename F> __device__ __forceinline__ void each_class(con
             f(v.at(1), j + 1);
         }
     } else {
+#pragma unroll 4
         for (int j = 0; j < n; ++j) f(to_f32(x[j]), j);
     }
 }
@@ -1106,22 +1108,24 @@ __global__ void __launch_bounds__(128) k_logp_grad_warp(const __grid_constant__ 
     }
 }
 
-// A CTA a share of a row: kAtOnce accesses a thread.
+// A CTA a share of a row: kAtOnce accesses a thread (8192 x 32768 in bfloat16: 209 us with
+// 10 CTAs of 128 threads an SM, 216 with 4 of 256).
+constexpr int kShareThreads = 128;
 template <typename T>
-__global__ void __launch_bounds__(256) k_logp_grad(const __grid_constant__ LogpArgs p, int64_t shares, bool same) {
+__global__ void __launch_bounds__(kShareThreads, 10) k_logp_grad(const __grid_constant__ LogpArgs p, int64_t shares, bool same) {
     constexpr int kN = Piece<T>::kN;
     const int64_t all = p.rows * shares;
     for (int64_t share = blockIdx.x; share < all; share += gridDim.x) {
-        const int64_t row = share / shares;
+        const int64_t row = all >> 32 ? share / shares : (unsigned)share / (unsigned)shares;
         const T* x = static_cast<const T*>(p.x) + row * p.n;
-        const int64_t first = ((share - row * shares) * (256 * kAtOnce) + threadIdx.x) * kN - Piece<T>::shift_of(x), n = p.n;
+        const int64_t first = ((share - row * shares) * (kShareThreads * kAtOnce) + threadIdx.x) * kN - Piece<T>::shift_of(x), n = p.n;
         Piece<T> q[kAtOnce];
 #pragma unroll
-        for (int k = 0; k < kAtOnce; ++k) q[k].load(x, first + k * 256 * kN, n, lo_of<T>(p), hi_of<T>(p));
+        for (int k = 0; k < kAtOnce; ++k) q[k].load(x, first + k * kShareThreads * kN, n, lo_of<T>(p), hi_of<T>(p));
         const PieceGrad<T> g(RowGrad(p, row));
 #pragma unroll
         for (int k = 0; k < kAtOnce; ++k) {
-            const int64_t at = first + k * 256 * kN;
+            const int64_t at = first + k * kShareThreads * kN;
             if (at >= n) break;
             float v[kN];
             g.of(v, q[k], at);
@@ -1245,8 +1249,8 @@ cudaError_t logp_backward(const LogpArgs& a, cudaStream_t s) {
         if (e != cudaSuccess) return e;
         kernel<<<grid_of(ceil_div(a.rows, 4 * each)), 128, 0, s>>>(a, each, (int)ceil_div(nv, 32), same);
     } else {
-        const int64_t shares = ceil_div(nv, 256 * kAtOnce);
-        k_logp_grad<T><<<grid_of(a.rows * shares), 256, 0, s>>>(a, shares, same);
+        const int64_t shares = ceil_div(nv, kShareThreads * kAtOnce);
+        k_logp_grad<T><<<grid_of(a.rows * shares), kShareThreads, 0, s>>>(a, shares, same);
     }
     return cudaGetLastError();
 }
