@@ -818,7 +818,9 @@ static EmbedPlan embed_plan(int64_t count, int64_t n, int c, int element) {
         while ((n - 1) >> bits) ++bits;
         p.passes = (bits + kMostBits - 1) / kMostBits;
         p.bits = (bits + p.passes - 1) / p.passes < 8 ? 8 : (bits + p.passes - 1) / p.passes;
-        p.items = count <= 262144 ? 4 : 16;
+        // (510952 labels of 5489: 31, 32 and 39 us a sort with 4, 8 and 16; 1000000 of
+        // 500000: 88, 67 and 69; above, half as many counts to keep)
+        p.items = count <= 262144 ? 4 : count <= 1 << 22 ? 8 : 16;
         p.tiles = count <= kClusterSorted ? 0 : (int)ceil_div(count, 256 * p.items);   // 0: by one cluster
     }
     // chunks long enough that few runs cross them, short enough that they fill the device
@@ -917,8 +919,9 @@ static const Entry* sort_labels(const EmbedPlan& p, uint8_t* ws, const Labels& i
     for (int pass = 0; pass < p.passes; ++pass) {
         const Source src{ids, n, count, from, valid};
         const Zeros first = zeros_of(table, bytes, 2 * pass, 2 * p.passes), second = zeros_of(table, bytes, 2 * pass + 1, 2 * p.passes);
-        const auto run = p.items == 4 ? (p.bits == 8 ? sort_pass<4, 256> : p.bits == 9 ? sort_pass<4, 512> : sort_pass<4, 1024>)
-                                      : (p.bits == 8 ? sort_pass<16, 256> : p.bits == 9 ? sort_pass<16, 512> : sort_pass<16, 1024>);
+        const auto run = p.items == 4   ? (p.bits == 8 ? sort_pass<4, 256> : p.bits == 9 ? sort_pass<4, 512> : sort_pass<4, 1024>)
+                         : p.items == 8 ? (p.bits == 8 ? sort_pass<8, 256> : p.bits == 9 ? sort_pass<8, 512> : sort_pass<8, 1024>)
+                                        : (p.bits == 8 ? sort_pass<16, 256> : p.bits == 9 ? sort_pass<16, 512> : sort_pass<16, 1024>);
         run(to, counts, totals, valid, starts, src, p.bits * pass, p.tiles, first, second, s);
         from = to;
         to = other;
