@@ -773,6 +773,117 @@ __global__ void __launch_bounds__(32 * kJoinWarps, 2) k_join_runs(const __grid_c
     }
 }
 
+// The same for up to 8 V channels: `lanes` threads of V channels a run (a warp a run uses few
+// of its threads: 510952 x 8 of 107924 labels 31 us, so 5).  The longer runs of a round are
+// listed, in any order, and added by a warp or, above kWarpRun parts, by the CTA.
+constexpr int kJoinNarrow = 8, kWarpRun = 512;
+
+template <int V>
+__global__ void __launch_bounds__(32 * kJoinWarps, 2) k_join_narrow(const __grid_constant__ RunArgs a, int bits) {
+    __shared__ float sums[kJoinWarps * 32 * V];
+    __shared__ unsigned long_chunk[kJoinWarps * 32], far_chunk[kJoinWarps * 32], far_parts[kJoinWarps * 32], longs, fars;
+    const unsigned starts = a.starts[0];
+    const int64_t valid = *a.valid;
+    const int lanes = 1 << bits, groups = 32 * kJoinWarps >> bits, group = threadIdx.x >> bits, at = (threadIdx.x & (lanes - 1)) * V;
+    const auto same_label = [&](int64_t chunk, unsigned label) {
+        const int64_t i = chunk * a.length;
+        return i < valid && a.sorted[i < valid ? i : 0].label == label;
+    };
+    const auto tail = [&](float (&s)[V], int64_t chunk) {
+        Vec<float, V> v;
+        v.load(a.part + (chunk * 2 + 1) * a.c + at);
+#pragma unroll
+        for (int j = 0; j < V; ++j) s[j] = v.at(j);
+    };
+    const auto write = [&](float (&s)[V], int64_t chunk) {
+        const int64_t to = (int64_t)a.sorted[(chunk + 1) * a.length].label * a.c + at;
+#pragma unroll
+        for (int j = 0; j < V; ++j) store_param(a.out, a.out_dtype, to + j, s[j] * a.scale);
+    };
+    for (uint64_t r0 = blockIdx.x; r0 < starts; r0 += (uint64_t)gridDim.x * groups) {
+        const uint64_t run = r0 + (uint64_t)group * gridDim.x;
+        if (threadIdx.x == 0) longs = fars = 0;
+        __syncthreads();
+        if (run < starts) {
+            const int64_t chunk = a.starts[1 + run];
+            const unsigned label = a.sorted[(chunk + 1) * a.length].label;
+            int parts = 1;
+            for (int count = 8; count == 8 && parts <= kLongRun; parts += count) {
+                bool same[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) same[u] = same_label(chunk + 1 + parts + u, label);
+                count = 0;
+#pragma unroll
+                for (int u = 0; u < 8; ++u) count += same[u];
+            }
+            if (parts > kLongRun) {
+                if (at == 0) long_chunk[atomicAdd(&longs, 1u)] = (unsigned)chunk;
+            } else if (at < a.c) {
+                float s[V];
+                tail(s, chunk);
+                add_parts(s, a, chunk, at, 1, parts, 1);
+                write(s, chunk);
+            }
+        }
+        __syncthreads();
+        for (unsigned k = threadIdx.x >> 5; k < longs; k += kJoinWarps) {   // a warp a run
+            const int64_t chunk = long_chunk[k];
+            const unsigned label = a.sorted[(chunk + 1) * a.length].label;
+            const int lane = threadIdx.x & 31;
+            int64_t parts = 1;
+            for (int count = 128; count == 128; parts += count) {
+                bool same[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) same[u] = same_label(chunk + 1 + parts + 32 * u + lane, label);
+                count = 0;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) count += __popc(__ballot_sync(0xffffffffu, same[u]));
+            }
+            if (parts > kWarpRun) {
+                if (lane == 0) {
+                    const unsigned i = atomicAdd(&fars, 1u);
+                    far_chunk[i] = (unsigned)chunk;
+                    far_parts[i] = (unsigned)parts;
+                }
+                continue;
+            }
+            float s[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) s[j] = 0.f;
+            if (at < a.c) {
+                if (lane < lanes) tail(s, chunk);
+                add_parts(s, a, chunk, at, 1 + (lane >> bits), parts, 32 >> bits);
+            }
+            for (int d = 16; d >= lanes; d >>= 1)
+#pragma unroll
+                for (int j = 0; j < V; ++j) s[j] += __shfl_down_sync(0xffffffffu, s[j], d);
+            if (lane < lanes && at < a.c) write(s, chunk);
+        }
+        __syncthreads();
+        for (unsigned k = 0; k < fars; ++k) {   // the CTA a run
+            const int64_t chunk = far_chunk[k];
+            float s[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) s[j] = 0.f;
+            if (at < a.c) {
+                if (group == 0) tail(s, chunk);
+                add_parts(s, a, chunk, at, 1 + group, far_parts[k], groups);
+            }
+            for (int d = groups / 2; d; d >>= 1) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) sums[threadIdx.x * V + j] = s[j];
+                __syncthreads();
+                if (group < d)
+#pragma unroll
+                    for (int j = 0; j < V; ++j) s[j] += sums[(threadIdx.x + d * lanes) * V + j];
+                __syncthreads();
+            }
+            if (group == 0 && at < a.c) write(s, chunk);
+        }
+        __syncthreads();
+    }
+}
+
 // ------------------------------------------------------------------ host side
 
 static int64_t align256(int64_t b) { return (b + 255) / 256 * 256; }
@@ -979,12 +1090,15 @@ static cudaError_t launch_runs(int v, const RunArgs& a, int64_t chunks, cudaStre
 
 static cudaError_t join_runs(const RunArgs& a, int64_t chunks, cudaStream_t s) {
     const int v = a.c % 4 == 0 ? 4 : 1;
-    const int64_t items = (chunks - 1) * ceil_div(a.c, 32 * v);
-    const unsigned grid = (unsigned)(items < 296 ? items : 296);   // one round
-    int lanes = 1;
-    while (lanes < 32 && lanes * v < a.c) lanes <<= 1;
-    if (v == 4) k_join_runs<4><<<grid, 32 * kJoinWarps, 0, s>>>(a, lanes);
-    else k_join_runs<1><<<grid, 32 * kJoinWarps, 0, s>>>(a, lanes);
+    const bool narrow = a.c <= kJoinNarrow * v;
+    int bits = 0;   // lanes of a run
+    while (bits < 5 && v << bits < a.c) ++bits;
+    const int64_t items = (chunks - 1) * ceil_div(a.c, 32 * v), need = narrow ? ceil_div(items << bits, 32 * kJoinWarps) : items;
+    const unsigned grid = (unsigned)(need < 296 ? need : 296);   // one round
+    if (v == 4 && narrow) k_join_narrow<4><<<grid, 32 * kJoinWarps, 0, s>>>(a, bits);
+    else if (narrow) k_join_narrow<1><<<grid, 32 * kJoinWarps, 0, s>>>(a, bits);
+    else if (v == 4) k_join_runs<4><<<grid, 32 * kJoinWarps, 0, s>>>(a, 1 << bits);
+    else k_join_runs<1><<<grid, 32 * kJoinWarps, 0, s>>>(a, 1 << bits);
     return cudaGetLastError();
 }
 
