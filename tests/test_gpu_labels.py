@@ -87,7 +87,7 @@ EMBED_SIZES = [((1,), 1, 1), ((7,), 5, 3), ((13, 29), 21, 50), ((100,), 1000, 64
                ((70000,), 21, 64), ((300,), 256, 2048), ((8192,), 97, 2), ((8193,), 300, 4), ((2049,), 1100, 3), ((32768,), 70000, 2), ((32769,), 2000, 2),
                ((20011,), 5, 24), ((300000,), 96, 6),
                ((500,), 12, 5000), ((300000,), 200000, 1), ((1200000,), 1000, 1), ((4200000,), 200, 1), ((4194305,), 1000000, 1),
-               ((4200001,), 60000, 1)]
+               ((4200001,), 60000, 1), ((200000,), 1, 3), ((150000,), 2, 4), ((200000,), 1, 5)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
