@@ -399,8 +399,12 @@ int plattice_embed_backward(void* grad_table, int table_dtype, const void* grad_
  * (NULL: not wanted).  states (NULL: not kept) [lines][ceil(steps / 16)][c]
  * float32: h before every 16th step taken, what the backward starts from.  The
  * recurrence is held in float32; h is its rounding.  Long lines are cut into
- * pieces whose gates are multiplied together: gates beyond 1 in magnitude have to
- * leave those products in float32 wherever the state is not 0.
+ * pieces, whose results are put together as f h + r with f the product of a piece's
+ * gates: h is then within float32's rounding of the recurrence of the magnitudes
+ * (of gate, u and state), as it is step by step, whatever the products come to, and
+ * of 2^-85 where states are below 2^24.
+ * Where the magnitudes themselves leave float32's range and come back, a piece may
+ * hold what a step loses.
  *
  * Backward, with G[t] = grad_h[t] + gate[t+1] G[t+1] (grad_last, if any, in the
  * place of gate[t+1] G[t+1] after the last step):

@@ -18,6 +18,88 @@ namespace plr {
 constexpr int kSteps = PLATTICE_SCAN_KEEP;
 constexpr int kThreads = 128;
 
+// Cut lines: what steps together do to a state, s -> f s + r.  A product of gates leaves
+// float32 long before states do (0.5 for 120 steps and 2 for 200 take a state of 1 to
+// 2^80, and the last 128 steps' product alone is infinite; an infinite state stays
+// infinite however small the product), so f has an exponent of its own: m 2^e, where e
+// is a multiple of 60 and m between 2^-60 and 2^60 (at most 1 with e < 0, at least 1 with
+// e > 0), or m is 0, with e = 0.
+constexpr float kSmall = 0x1p-60f, kLarge = 0x1p60f;
+constexpr int kPart = 60, kFar = kPart << 20;   // e goes no farther: nothing comes back from there
+
+__device__ __forceinline__ bool medium(float v) { return fabsf(v) >= kSmall && fabsf(v) <= kLarge; }
+
+struct Factor {
+    float m;
+    int e;
+    __device__ __forceinline__ void hold() {   // after a product: m is between 2^-120 and 2^120, or 0
+        const bool small = fabsf(m) < kSmall, large = fabsf(m) > kLarge;
+        m *= small ? kLarge : large ? kSmall : 1.f;
+        e += small ? -kPart : large ? kPart : 0;
+        const bool over = e < 0 && fabsf(m) > 1.f, under = e > 0 && fabsf(m) < 1.f;
+        m *= over ? kSmall : under ? kLarge : 1.f;
+        e += over ? kPart : under ? -kPart : 0;
+        e = m == 0.f ? 0 : max(min(e, kFar), -kFar);
+    }
+    __device__ __forceinline__ void times(const Factor& o) {
+        m = m == 0.f ? 0.f : m * o.m;   // the state before a gate of 0 is of no consequence
+        e += o.e;
+        hold();
+    }
+    __device__ __forceinline__ void times(float gate) {   // of any size
+        const float a = fabsf(gate);
+        times(a < kSmall && a > 0.f ? Factor{gate * kLarge * kLarge, -2 * kPart}
+              : a > kLarge          ? Factor{gate * kSmall * kSmall, 2 * kPart}
+                                    : Factor{gate, 0});
+    }
+};
+// Out of line, as it is there for few blocks: gates that leave 2^+-120 within eight steps.
+struct Eight { float g[8]; };
+__device__ __noinline__ Factor times_slowly(Factor f, Eight q) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f.times(q.g[i]);
+    return f;
+}
+
+struct alignas(16) Map {
+    Factor f;
+    float r;
+};
+// A state of 0 stays r, whatever the factor.
+__device__ __forceinline__ float apply(const Map& m, float s) {
+    float v = m.f.m * s;
+    int e = m.f.e;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {   // in parts that float32 has: of more than 6 60 nothing is left, or infinity
+        const int part = max(min(e, 2 * kPart), -2 * kPart);
+        v *= __int_as_float((127 + part) << 23);
+        e -= part;
+    }
+    return s == 0.f ? m.r : v + m.r;
+}
+// The map of both.  Without branches: one for what stays within 2^+-60 took a line of 3000 x 8
+// in bfloat16 0.9 us more, whose 64 pieces soon leave it.
+__device__ __forceinline__ Map then(Map first, const Map& second) {
+    first.f.times(second.f);
+    first.r = apply(second, first.r);
+    return first;
+}
+
+// Nearly all maps are tame: |f| <= 1 and |r| <= 2^24.  Where all of a line's are, and the
+// state it begins with, a map is two numbers of float32: what f loses below 2^-126 is
+// never multiplied up again, and its product with a state, which grows by 2^24 a map at
+// most, is below 2^-85.  f is NaN for a map that is not tame, and so is every product with it;
+// the state is then found from the maps as they are.
+constexpr float kTame = 0x1p24f;
+__device__ __forceinline__ float2 plain(const Map& m) {
+    const bool tame = m.f.e <= 0 && fabsf(m.f.m) <= 1.f && fabsf(m.r) <= kTame;
+    const float f = m.f.e == 0 ? m.f.m : m.f.e == -kPart ? m.f.m * kSmall : m.f.e == -2 * kPart ? m.f.m * kSmall * kSmall : 0.f;
+    return make_float2(tame ? f : __int_as_float(0x7fffffff), m.r);
+}
+__device__ __forceinline__ float2 then(float2 first, float2 second) {
+    return make_float2(first.x * second.x, fmaf(second.x, first.y, second.y));
+}
+
 struct ScanArgs {
     const void *x, *a;
     const float* state;
@@ -27,8 +109,9 @@ struct ScanArgs {
     const float* grad_last;
     void *gx, *ga;
     float* gs;
-    float2* sums;            // cut lines: [line][piece][c] (product of the gates, result from 0)
-    float2* tile_sums;       // [line][tile][c], of a CTA's pieces together
+    Map* sums;               // cut lines: [line][piece][c]
+    Map* tile_sums;          // [line][tile][c], of a CTA's pieces together
+    float2 *plain_sums, *plain_tiles;   // the same as plain()
     int64_t lines, steps, blocks;   // blocks of kSteps in a line
     int64_t tiles;           // CTAs a line's steps are cut over
     int c, reverse;
@@ -90,7 +173,8 @@ template <typename T, int V> struct Block {
     static __device__ __forceinline__ bool stretch(const T* low, int n, bool run) {
         return run && n == kSteps && ((uintptr_t)low & 15) == 0;
     }
-    __device__ __forceinline__ void load(const void* base, int64_t o, int64_t stride, int n, bool run) {
+    // What lies behind the n-th step is 0, or `fill`.
+    __device__ __forceinline__ void load(const void* base, int64_t o, int64_t stride, int n, bool run, float fill = 0.f) {
         const T* p = static_cast<const T*>(base) + o;
         const T* low = stride < 0 ? p + (kSteps - 1) * stride : p;
         if (stretch(low, n, run)) {
@@ -111,8 +195,14 @@ template <typename T, int V> struct Block {
         } else {
 #pragma unroll
             for (int i = 0; i < kSteps; ++i, p += stride) {
-                if (i < n) v[i].load(p);
-                else v[i].zero();
+                if (i < n) {
+                    v[i].load(p);
+                } else {
+                    float all[V];
+#pragma unroll
+                    for (int j = 0; j < V; ++j) all[j] = fill;
+                    v[i].from(all);
+                }
             }
         }
     }
@@ -166,48 +256,46 @@ template <bool kBlend> __device__ __forceinline__ float input(float a, float x) 
 //
 // Lines that do not fill the device by themselves are cut: a thread takes a
 // piece, a CTA `pieces` neighbouring ones of its lanes.  The first kernel gives
-// for each piece and for the CTA's pieces together what it does to a state: s ->
-// f s + r.  The second one's CTAs each go through the CTAs before them, then
-// through their own pieces, and know every piece's first state.
+// for each piece and for the CTA's pieces together what it does to a state.  The
+// second one's CTAs each go through the CTAs before them, then through their own
+// pieces, and know every piece's first state.
 
-// Gates beyond 1 can take a piece's factor f past float32 where no state is: a state
-// of 0 stays r, and a gate of 0 makes the factor 0 (infinity times 0 would be NaN).
-__device__ __forceinline__ float apply(float2 map, float s) { return s == 0.f ? map.y : fmaf(map.x, s, map.y); }
-__device__ __forceinline__ float joined(float f, float g) { return g == 0.f || f == 0.f ? 0.f : f * g; }
-__device__ __forceinline__ float2 then(float2 first, float2 second) {   // the map of both
-    return make_float2(joined(first.x, second.x), apply(second, first.y));
-}
+__device__ __forceinline__ void set_identity(Map& m) { m = Map{{1.f, 0}, 0.f}; }
+__device__ __forceinline__ void set_identity(float2& m) { m = make_float2(1.f, 0.f); }
 
 // The maps of a CTA's pieces (`place`: in the order they are gone through), each after
 // all before it, are left in `shared`: in pairs, so that many pieces of few channels
 // take as many steps as their number has bits (one by one: 169 lines of 2661 x 2, 28 us).
-template <int V>
-__device__ __forceinline__ void scan_maps(float2 (&m)[V], float2* shared, int place, int lane, const ScanArgs& p) {
-    for (int d = 1; d < p.pieces; d <<= 1) {
+// kSets sets of maps, each with places of its own.
+template <typename M, int V, int kSets>
+__device__ __forceinline__ void scan_maps(M (&m)[kSets][V], M (*shared)[kThreads * V], const int (&place)[kSets], int lane,
+                                          const ScanArgs& p) {
+    for (int d = 1;; d <<= 1) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) shared[(place * p.lanes + lane) * V + j] = m[j];
+        for (int q = 0; q < kSets; ++q)
+#pragma unroll
+            for (int j = 0; j < V; ++j) shared[q][(place[q] * p.lanes + lane) * V + j] = m[q][j];
         __syncthreads();
-        float2 o[V];
+        if (d >= p.pieces) return;
 #pragma unroll
-        for (int j = 0; j < V; ++j) o[j] = place >= d ? shared[((place - d) * p.lanes + lane) * V + j] : make_float2(1.f, 0.f);
+        for (int q = 0; q < kSets; ++q)
+            if (place[q] >= d)
+#pragma unroll
+                for (int j = 0; j < V; ++j) m[q][j] = then(shared[q][((place[q] - d) * p.lanes + lane) * V + j], m[q][j]);
         __syncthreads();
-#pragma unroll
-        for (int j = 0; j < V; ++j) m[j] = then(o[j], m[j]);
     }
-#pragma unroll
-    for (int j = 0; j < V; ++j) shared[(place * p.lanes + lane) * V + j] = m[j];
-    __syncthreads();
 }
 
 // Pieces of a backward pass are gone through from the last on.
 template <typename T, int V, bool kBlend, bool kGrad>
 __global__ void __launch_bounds__(kThreads) k_scan_sums(const __grid_constant__ ScanArgs p) {
-    __shared__ float2 shared[kThreads * V];
+    __shared__ Map shared[1][kThreads * V];
     const Work<V, true> w(p, blockIdx.y);
-    float f[V], r[V];
+    Factor f[V];
+    float r[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        f[j] = 1.f;
+        f[j] = Factor{1.f, 0};
         r[j] = 0.f;
     }
     if (w.here) {
@@ -217,84 +305,138 @@ __global__ void __launch_bounds__(kThreads) k_scan_sums(const __grid_constant__ 
             const int n = steps_of(p, b);
             Block<T, V> x, a;
             x.load(kGrad ? p.g : p.x, o, stride, n, p.c == V);
-            a.load(p.a, o, stride, n, p.c == V);
+            a.load(p.a, o, stride, n, p.c == V, 1.f);   // of steps that are not there: r 1 + 0
 #pragma unroll
-            for (int i = 0; i < kSteps; ++i) {
-                const int t = kGrad ? kSteps - 1 - i : i;
-                if (t < n) {
+            for (int j = 0; j < V; ++j) {
+                Factor& q = f[j];
 #pragma unroll
-                    for (int j = 0; j < V; ++j) {
+                for (int first = 0; first < kSteps; first += 8) {
+                    const float m0 = q.m;
+                    float least = INFINITY;
+                    Eight eight;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int t = kGrad ? kSteps - 1 - first - i : first + i;
                         const float gate = a.v[t].at(j), v = x.v[t].at(j);
                         r[j] = kGrad ? gate * (v + r[j]) : fmaf(gate, r[j], input<kBlend>(gate, v));
-                        f[j] *= gate;
+                        q.m *= gate;
+                        least = fminf(least, fabsf(q.m));
+                        eight.g[i] = gate;
+                    }
+                    if (least >= kSmall * kSmall && fabsf(q.m) <= kLarge * kLarge) {
+                        if (q.e != 0 || !medium(q.m)) q.hold();
+                    } else {
+                        bool closed = m0 == 0.f;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) closed |= eight.g[i] == 0.f;
+                        q = closed ? Factor{0.f, 0} : times_slowly(Factor{m0, q.e}, eight);
                     }
                 }
             }
         }
-        // infinity times a gate of 0 (a gate that is itself NaN makes r NaN)
-#pragma unroll
-        for (int j = 0; j < V; ++j) f[j] = f[j] == f[j] ? f[j] : 0.f;
         if (w.first < p.blocks)
 #pragma unroll
-            for (int j = 0; j < V; ++j)
-                p.sums[(w.line * p.tiles * p.pieces + w.piece) * p.c + w.col + j] = make_float2(f[j], r[j]);
+            for (int j = 0; j < V; ++j) {
+                const int64_t at = (w.line * p.tiles * p.pieces + w.piece) * p.c + w.col + j;
+                p.sums[at] = Map{f[j], r[j]};
+                p.plain_sums[at] = plain(Map{f[j], r[j]});
+            }
     }
-    float2 m[V];
+    Map m[1][V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) m[j] = make_float2(f[j], r[j]);
-    scan_maps(m, shared, kGrad ? p.pieces - 1 - w.own : w.own, w.lane, p);
+    for (int j = 0; j < V; ++j) m[0][j] = Map{f[j], r[j]};
+    const int place[1] = {kGrad ? p.pieces - 1 - w.own : w.own};
+    scan_maps<Map, V, 1>(m, shared, place, w.lane, p);
     if (w.own == 0 && w.here)
 #pragma unroll
-        for (int j = 0; j < V; ++j)
-            p.tile_sums[(w.line * p.tiles + w.tile) * p.c + w.col + j] = shared[((p.pieces - 1) * p.lanes + w.lane) * V + j];
+        for (int j = 0; j < V; ++j) {
+            const int64_t at = (w.line * p.tiles + w.tile) * p.c + w.col + j;
+            const Map all = shared[0][((p.pieces - 1) * p.lanes + w.lane) * V + j];
+            p.tile_sums[at] = all;
+            p.plain_tiles[at] = plain(all);
+        }
 }
 
-// The state that the thread's piece starts from: s goes through the maps of the
-// CTAs before, in as many parts as the CTA has pieces, then of its pieces before.
-template <int V, bool kGrad>
-__device__ __forceinline__ void first_state(float (&s)[V], const ScanArgs& p, const Work<V, true>& w) {
-    __shared__ float2 shared[kThreads * V];
+// The maps of all CTAs before, and of the CTA's pieces before the thread's.  Of the first a
+// thread takes a part, one of as many as the CTA has pieces.
+template <typename M, int V, bool kGrad>
+__device__ __forceinline__ void maps_before(M (&tiles)[V], M (&own)[V], const M* tile_sums, const M* sums, M (*shared)[kThreads * V],
+                                            const ScanArgs& p, const Work<V, true>& w) {
+    constexpr int kAtOnce = sizeof(M) == sizeof(float2) ? 8 : 2;
     const int64_t before = kGrad ? p.tiles - 1 - w.tile : w.tile, part = (before + p.pieces - 1) / p.pieces;
-    float2 all[V];
+    M m[2][V];   // of the CTAs; of the piece
 #pragma unroll
-    for (int j = 0; j < V; ++j) all[j] = make_float2(1.f, 0.f);
+    for (int j = 0; j < V; ++j) {
+        set_identity(m[0][j]);
+        set_identity(m[1][j]);
+    }
     if (w.here) {
         const int64_t to = (w.own + 1) * part < before ? (w.own + 1) * part : before;
-        const float2* sums = p.tile_sums + w.line * p.tiles * p.c + w.col;
-        for (int64_t k = w.own * part; k < to; k += 8) {
-            float2 m[8][V];
+        const M* from = tile_sums + w.line * p.tiles * p.c + w.col;
+        for (int64_t k = w.own * part; k < to; k += kAtOnce) {
+            M ahead[kAtOnce][V];
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
+            for (int i = 0; i < kAtOnce; ++i)
 #pragma unroll
-                for (int j = 0; j < V; ++j)
-                    m[i][j] = k + i < to ? sums[(kGrad ? p.tiles - 1 - k - i : k + i) * p.c + j] : make_float2(1.f, 0.f);
+                for (int j = 0; j < V; ++j) {
+                    set_identity(ahead[i][j]);
+                    if (k + i < to) ahead[i][j] = from[(kGrad ? p.tiles - 1 - k - i : k + i) * p.c + j];
+                }
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
+            for (int i = 0; i < kAtOnce; ++i)
 #pragma unroll
-                for (int j = 0; j < V; ++j) all[j] = then(all[j], m[i][j]);
+                for (int j = 0; j < V; ++j) m[0][j] = then(m[0][j], ahead[i][j]);
         }
+        if (w.first < p.blocks)
+#pragma unroll
+            for (int j = 0; j < V; ++j) m[1][j] = sums[((w.line * p.tiles + w.tile) * p.pieces + w.own) * p.c + w.col + j];
     }
-    // The piece's own map is on its way while the CTAs' are joined.
-    const int place = kGrad ? p.pieces - 1 - w.own : w.own;
-    float2 m[V];
+    const int place[2] = {w.own, kGrad ? p.pieces - 1 - w.own : w.own};
+    scan_maps<M, V, 2>(m, shared, place, w.lane, p);
 #pragma unroll
-    for (int j = 0; j < V; ++j)
-        m[j] = w.here && w.first < p.blocks ? p.sums[((w.line * p.tiles + w.tile) * p.pieces + w.own) * p.c + w.col + j]
-                                            : make_float2(1.f, 0.f);
-    scan_maps(all, shared, w.own, w.lane, p);
+    for (int j = 0; j < V; ++j) {
+        tiles[j] = shared[0][((p.pieces - 1) * p.lanes + w.lane) * V + j];
+        if (place[1]) own[j] = shared[1][((place[1] - 1) * p.lanes + w.lane) * V + j];
+        else set_identity(own[j]);
+    }
+}
+
+// The state that the thread's piece starts from, of the line's s: where a map is not tame.
+template <int V> struct States { float s[V]; };
+template <int V, bool kGrad>
+__device__ __noinline__ States<V> first_state_slowly(States<V> s, const ScanArgs& p, int64_t tile) {
+    const Work<V, true> w(p, tile);
+    __shared__ Map shared[2][kThreads * V];
+    Map tiles[V], own[V];
+    maps_before<Map, V, kGrad>(tiles, own, p.tile_sums, p.sums, shared, p, w);
 #pragma unroll
-    for (int j = 0; j < V; ++j) s[j] = apply(shared[((p.pieces - 1) * p.lanes + w.lane) * V + j], s[j]);
-    __syncthreads();
-    scan_maps(m, shared, place, w.lane, p);
-    if (place)
+    for (int j = 0; j < V; ++j) s.s[j] = apply(own[j], apply(tiles[j], s.s[j]));
+    return s;
+}
+template <int V, bool kGrad>
+__device__ __forceinline__ void first_state(float (&s)[V], const ScanArgs& p, const Work<V, true>& w) {
+    __shared__ float2 shared[2][kThreads * V];
+    float2 tiles[V], own[V];
+    maps_before<float2, V, kGrad>(tiles, own, p.plain_tiles, p.plain_sums, shared, p, w);
+    bool tame = true;
+    States<V> line;
 #pragma unroll
-        for (int j = 0; j < V; ++j) s[j] = apply(shared[((place - 1) * p.lanes + w.lane) * V + j], s[j]);
+    for (int j = 0; j < V; ++j) {
+        line.s[j] = s[j];
+        tame &= fabsf(s[j]) <= kTame && tiles[j].x == tiles[j].x && own[j].x == own[j].x;
+        s[j] = fmaf(own[j].x, fmaf(tiles[j].x, s[j], tiles[j].y), own[j].y);
+    }
+    if (__syncthreads_or(!tame)) {
+        line = first_state_slowly<V, kGrad>(line, p, w.tile);
+#pragma unroll
+        for (int j = 0; j < V; ++j) s[j] = line.s[j];
+    }
 }
 
 // ---------------------------------------------------------------- the passes
 
 template <typename T, int V, bool kBlend, bool kCut>
-__global__ void __launch_bounds__(kThreads) k_scan(const __grid_constant__ ScanArgs p) {
+__global__ void __launch_bounds__(kThreads, 6) k_scan(const __grid_constant__ ScanArgs p) {
     const Work<V, kCut> w(p, kCut ? (int64_t)gridDim.y - 1 - blockIdx.y : 0);   // what was read last may still be in the L2
     float h[V];
 #pragma unroll
@@ -445,7 +587,7 @@ constexpr int64_t kEnough = 148 * 512, kEnoughGrad = 148 * 384, kFew = 148 * 192
 
 struct ScanPlan {
     int v, lanes, pieces, piece_blocks;
-    int64_t wide, tiles, tile_sums, bytes;   // wide: CTAs beside one another
+    int64_t wide, tiles, cells, bytes;   // wide: CTAs beside one another; cells: maps of all tiles
     bool cut;
 };
 
@@ -469,9 +611,8 @@ static ScanPlan scan_plan(const plattice_scan_args* q, bool grad) {
     p.pieces = kThreads / p.lanes;
     p.wide = q->lines * ceil_div(units, p.lanes);
     p.tiles = ceil_div(blocks, (int64_t)p.piece_blocks * p.pieces);
-    const int64_t one = q->lines * p.tiles * q->c * (int64_t)sizeof(float2);
-    p.tile_sums = one * p.pieces;
-    p.bytes = one * (p.pieces + 1);
+    p.cells = q->lines * p.tiles * q->c;
+    p.bytes = p.cells * (p.pieces + 1) * (int64_t)(sizeof(Map) + sizeof(float2));
     return p;
 }
 
@@ -525,9 +666,10 @@ static int run(const plattice_scan_args* q, bool grad, cudaStream_t s, const cha
     const ScanPlan p = scan_plan(q, grad);
     if (p.bytes && (!q->workspace || ((uintptr_t)q->workspace & 255) || q->workspace_bytes < (size_t)p.bytes))
         return PLATTICE_ERR_WORKSPACE;
-    float2* ws = static_cast<float2*>(q->workspace);
+    Map *sums = static_cast<Map*>(q->workspace), *tile_sums = sums + p.cells * p.pieces;
+    float2 *plain_sums = reinterpret_cast<float2*>(tile_sums + p.cells), *plain_tiles = plain_sums + p.cells * p.pieces;
     const ScanArgs a{q->x, q->gate, q->state, q->h, q->last, q->states, q->grad_h, q->grad_last, q->grad_x, q->grad_gate,
-                     q->grad_state, ws, ws + p.tile_sums / (int64_t)sizeof(float2), q->lines, q->steps,
+                     q->grad_state, sums, tile_sums, plain_sums, plain_tiles, q->lines, q->steps,
                      ceil_div(q->steps, kSteps), p.tiles, q->c, q->reverse, p.lanes, p.pieces, p.piece_blocks};
     if (q->steps == 1) {
         // pointers of the other direction are not used

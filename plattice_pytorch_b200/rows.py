@@ -526,9 +526,8 @@ def scan(x, gate, state=None, blend=False, reverse=False, keep=False):
     gate[t]) x[t]``, for every line and channel by itself: ``(h, last, states)``.
 
     ``gate`` as ``x`` (0 starts afresh, so that lines of several lengths can lie
-    behind one another; beyond 1 in magnitude, the products of neighbouring gates of
-    a long line have to stay in float32 where they meet a state that is not 0).  ``state [..., c]`` float32: h before the
-    first step (None: zeros).  ``last [..., c]`` float32: h after the last, to go
+    behind one another; beyond 1 in magnitude is allowed, as long as the recurrence
+    stays in float32).  ``state [..., c]`` float32: h before the first step (None: zeros).  ``last [..., c]`` float32: h after the last, to go
     on from (a single step at a time is ``steps`` 1).  ``reverse``: the steps are
     taken from the last to the first.  The recurrence is held in float32, ``h`` is
     its rounding to the type of ``x``.  ``states``: with ``keep`` what
