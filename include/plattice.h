@@ -478,7 +478,7 @@ int plattice_log_probs_backward(const plattice_log_probs_args* args, void* strea
  * own type) or memory of its own; memory that any out shares with another tensor
  * or with the norm is refused (PLATTICE_ERR_INVALID).  Squares are added in float32 by eights (in
  * float64 where those would not hold them) and then in float64, in an order that
- * the sizes fix.  norm_in (device, float32) non-NULL: the norm to use, such as
+ * the sizes fix, and whether each g begins on a 16-byte boundary.  norm_in (device, float32) non-NULL: the norm to use, such as
  * one over several processes; the gradients are then read only to be scaled.
  * norm_out (device, float32; may be norm_in): the norm.  max_norm >= 0, infinite
  * for a copy; without out pointers (all NULL) only the norm is computed.  The

@@ -28,7 +28,7 @@ template <int kTensors> struct Grads {
     void* out[kTensors];
     long long size[kTensors];
     long long end[kTensors];      // pieces up to the tensor's last
-    uint8_t type[kTensors];       // dtype | out_dtype << 2 | aligned << 4
+    uint8_t type[kTensors];       // dtype | out_dtype << 2 | g and out aligned << 4 | g aligned << 5
     int count;
 };
 constexpr int kMost = 256, kSome = 64;   // tensors of one launch; of a small one's table
@@ -107,7 +107,7 @@ __device__ __forceinline__ double cta_sum(double v) {
 template <int kSize = kPiece> struct At {
     int tensor, n, dtype;
     long long first;
-    bool aligned, wide;
+    bool aligned, aligned_g, wide;   // aligned_g: all that the squares' order goes by
     template <int N> __device__ __forceinline__ At(const Grads<N>& t, long long piece) : At(t, piece, tensor_of(t, piece)) {}
     template <int N> __device__ __forceinline__ At(const Grads<N>& t, long long piece, int tensor_) : tensor(tensor_) {
         first = (piece - (tensor ? t.end[tensor - 1] : 0)) * kSize;
@@ -116,7 +116,8 @@ template <int kSize = kPiece> struct At {
         const int type = t.type[tensor];
         dtype = type & 3;
         wide = ((type >> 2) & 3) == PLATTICE_F32;
-        aligned = type >> 4;
+        aligned = type >> 4 & 1;
+        aligned_g = type >> 5;
     }
 };
 
@@ -132,9 +133,9 @@ struct Share {
 
 template <int N> __device__ __forceinline__ double squares_at(const Grads<N>& t, const At<>& p) {
     const void* g = t.g[p.tensor];
-    if (p.dtype == PLATTICE_F32) return piece_squares(static_cast<const float*>(g) + p.first, p.n, p.aligned);
-    if (p.dtype == PLATTICE_BF16) return piece_squares(static_cast<const __nv_bfloat16*>(g) + p.first, p.n, p.aligned);
-    return piece_squares(static_cast<const __half*>(g) + p.first, p.n, p.aligned);
+    if (p.dtype == PLATTICE_F32) return piece_squares(static_cast<const float*>(g) + p.first, p.n, p.aligned_g);
+    if (p.dtype == PLATTICE_BF16) return piece_squares(static_cast<const __nv_bfloat16*>(g) + p.first, p.n, p.aligned_g);
+    return piece_squares(static_cast<const __half*>(g) + p.first, p.n, p.aligned_g);
 }
 
 template <int N>
@@ -334,7 +335,7 @@ template <int N> static int fill(Grads<N>& t, const plattice_grad* grads, int fi
         t.size[k] = g.size;
         *pieces += ceil_div(g.size, size);
         t.end[k] = *pieces;
-        t.type[k] = (uint8_t)(g.dtype | g.out_dtype << 2 | (aligned16(g.g) && aligned16(g.out) ? 16 : 0));
+        t.type[k] = (uint8_t)(g.dtype | g.out_dtype << 2 | (aligned16(g.g) ? aligned16(g.out) ? 48 : 32 : 0));
     }
     return first;
 }
