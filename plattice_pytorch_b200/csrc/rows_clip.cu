@@ -398,7 +398,7 @@ int plattice_clip_grads_workspace_size(const plattice_grad* grads, int count, si
 
 int plattice_clip_grads(const plattice_grad* grads, int count, float max_norm, float eps, const float* norm_in,
                         float* norm_out, void* workspace, size_t workspace_bytes, void* stream) {
-    if (!grads_ok(grads, count)) return PLATTICE_ERR_INVALID;
+    if (!grads_ok(grads, count) || !on_elements(sizeof(float), norm_in, norm_out)) return PLATTICE_ERR_INVALID;
     int outs = 0, tensors = 0;
     for (int i = 0; i < count; ++i)
         if (grads[i].size) {

@@ -1116,7 +1116,8 @@ int plattice_embed(void* y, const void* ids, int ids_wide, const void* table, in
                    long long n, int c, void* stream) {
     if (!dtype_ok(dtype) || !embed_ok(count, n, c)) return PLATTICE_ERR_INVALID;
     if (count == 0) return PLATTICE_OK;
-    if (!y || !ids || !table || (uintptr_t)ids % (ids_wide ? 8 : 4)) return PLATTICE_ERR_INVALID;
+    if (!y || !ids || !table || !on_elements(ids_wide ? 8 : 4, ids) || !on_elements(dtype_size(dtype), y, table))
+        return PLATTICE_ERR_INVALID;
     const int v = widest(c, dtype_size(dtype), (uintptr_t)y | (uintptr_t)table);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const Labels l{ids, ids_wide};
@@ -1139,10 +1140,12 @@ int plattice_embed_backward_workspace_size(long long count, long long n, int c, 
 int plattice_embed_backward(void* grad_table, int table_dtype, const void* grad_y, int dtype, const void* ids,
                             int ids_wide, float scale, void* workspace, size_t workspace_bytes, long long count,
                             long long n, int c, void* stream) {
-    if (!dtype_ok(dtype) || !dtype_ok(table_dtype) || !embed_ok(count, n, c) || count > 0x7fffffff || !grad_table)
+    if (!dtype_ok(dtype) || !dtype_ok(table_dtype) || !embed_ok(count, n, c) || count > 0x7fffffff || !grad_table ||
+        !on_elements(dtype_size(table_dtype), grad_table))
         return PLATTICE_ERR_INVALID;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (count && (!grad_y || !ids || (uintptr_t)ids % (ids_wide ? 8 : 4))) return PLATTICE_ERR_INVALID;
+    if (count && (!grad_y || !ids || !on_elements(ids_wide ? 8 : 4, ids) || !on_elements(dtype_size(dtype), grad_y)))
+        return PLATTICE_ERR_INVALID;
     const EmbedPlan p = embed_plan(count, n, c, (int)dtype_size(dtype));
     if (count && p.bytes && (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < (size_t)p.bytes))
         return PLATTICE_ERR_WORKSPACE;

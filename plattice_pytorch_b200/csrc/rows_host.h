@@ -86,6 +86,8 @@ constexpr int kMaxSmem = 232448;   // shared memory a CTA can have
 
 inline bool dtype_ok(int d) { return d == PLATTICE_F32 || d == PLATTICE_BF16 || d == PLATTICE_F16; }
 inline size_t dtype_size(int d) { return d == PLATTICE_F32 ? 4 : 2; }
+// Whether pointers (null: as good as any) lie on boundaries of `size` bytes.
+template <typename... P> inline bool on_elements(size_t size, const P*... p) { return (((uintptr_t)p | ...) % size) == 0; }
 inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 // Element counts stay below 2^40, far from overflowing the 64-bit offsets.

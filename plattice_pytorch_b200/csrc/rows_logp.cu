@@ -10,7 +10,7 @@ extern "C" {
 static bool logp_ok(const plattice_log_probs_args* q) {
     return q && dtype_ok(q->dtype) && q->rows >= 0 && q->n >= 1 && q->n <= (1 << 30) && q->top >= 0 &&
            q->top <= PLATTICE_MAX_TOP && q->top <= q->n && fits(q->rows, q->n) &&
-           (!q->labels || (uintptr_t)q->labels % (q->labels_wide ? 8 : 4) == 0);
+           on_elements(q->labels_wide ? 8 : 4, q->labels);
 }
 
 static LogpArgs logp_args(const plattice_log_probs_args* q) {
@@ -21,8 +21,9 @@ static LogpArgs logp_args(const plattice_log_probs_args* q) {
 int plattice_log_probs(const plattice_log_probs_args* q, void* stream) {
     if (!logp_ok(q)) return PLATTICE_ERR_INVALID;
     if (q->rows == 0) return PLATTICE_OK;
-    if (!q->logits || (uintptr_t)q->logits % dtype_size(q->dtype) || !q->stats || (uintptr_t)q->stats % 8 ||
-        (q->logp && !q->labels) || (q->top && (!q->top_logp || !q->top_ids)))
+    if (!q->logits || !on_elements(dtype_size(q->dtype), q->logits) || !q->stats || !on_elements(2 * sizeof(float), q->stats) ||
+        !on_elements(sizeof(float), q->logp, q->entropy, q->lse) || (q->logp && !q->labels) ||
+        (q->top && (!q->top_logp || !q->top_ids || !on_elements(sizeof(float), q->top_logp) || !on_elements(8, q->top_ids))))
         return PLATTICE_ERR_INVALID;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const LogpArgs a = logp_args(q);
@@ -35,8 +36,10 @@ int plattice_log_probs(const plattice_log_probs_args* q, void* stream) {
 int plattice_log_probs_backward(const plattice_log_probs_args* q, void* stream) {
     if (!logp_ok(q)) return PLATTICE_ERR_INVALID;
     if (q->rows == 0) return PLATTICE_OK;
-    if (!q->logits || (uintptr_t)q->logits % dtype_size(q->dtype) || !q->stats || (uintptr_t)q->stats % 8 || !q->grad_logits ||
-        (uintptr_t)q->grad_logits % dtype_size(q->dtype) || (q->grad_logp && !q->labels) || (q->grad_entropy && !q->entropy))
+    if (!q->logits || !q->stats || !on_elements(2 * sizeof(float), q->stats) || !q->grad_logits ||
+        !on_elements(dtype_size(q->dtype), q->logits, q->grad_logits) ||
+        !on_elements(sizeof(float), q->grad_logp, q->grad_entropy, q->grad_lse) || (q->grad_logp && !q->labels) ||
+        (q->grad_entropy && (!q->entropy || !on_elements(sizeof(float), q->entropy))))
         return PLATTICE_ERR_INVALID;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const LogpArgs a = logp_args(q);

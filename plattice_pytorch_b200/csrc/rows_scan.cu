@@ -715,7 +715,9 @@ int plattice_scan(const plattice_scan_args* q, void* stream) {
                                     : cudaMemsetAsync(q->last, 0, b, s),
                            "plattice_scan");
     }
-    if (!q->x || !q->gate || !q->h) return PLATTICE_ERR_INVALID;
+    if (!q->x || !q->gate || !q->h || !on_elements(dtype_size(q->dtype), q->x, q->gate, q->h) ||
+        !on_elements(sizeof(float), q->state, q->last, q->states))
+        return PLATTICE_ERR_INVALID;
     return run(q, false, s, "plattice_scan");
 }
 
@@ -736,7 +738,10 @@ int plattice_scan_backward(const plattice_scan_args* q, void* stream) {
                                         : cudaMemsetAsync(q->grad_state, 0, b, s),
                            "plattice_scan_backward");
     }
-    if (!q->x || !q->gate || !q->states || !q->grad_h || !q->grad_x || !q->grad_gate) return PLATTICE_ERR_INVALID;
+    if (!q->x || !q->gate || !q->states || !q->grad_h || !q->grad_x || !q->grad_gate ||
+        !on_elements(dtype_size(q->dtype), q->x, q->gate, q->grad_h, q->grad_x, q->grad_gate) ||
+        !on_elements(sizeof(float), q->states, q->grad_last, q->grad_state))
+        return PLATTICE_ERR_INVALID;
     return run(q, true, s, "plattice_scan_backward");
 }
 
