@@ -481,7 +481,7 @@ int plattice_log_probs_backward(const plattice_log_probs_args* args, void* strea
  * the sizes fix, and whether each g begins on a 16-byte boundary.  norm_in (device, float32) non-NULL: the norm to use, such as
  * one over several processes; the gradients are then read only to be scaled.
  * norm_out (device, float32; may be norm_in): the norm.  max_norm >= 0, infinite
- * for a copy; without out pointers (all NULL) only the norm is computed.  The
+ * for a copy; eps >= 0, finite; without out pointers (all NULL) only the norm is computed.  The
  * arrays are read before the call returns. */
 typedef struct plattice_grad {
     const void* g;

@@ -408,7 +408,7 @@ int plattice_clip_grads(const plattice_grad* grads, int count, float max_norm, f
     if (outs && outs != tensors) return PLATTICE_ERR_INVALID;
     if (!outs && !norm_out) return tensors ? PLATTICE_ERR_INVALID : PLATTICE_OK;
     if (outs) {
-        if (!(max_norm >= 0.f) || !(eps >= 0.f)) return PLATTICE_ERR_INVALID;
+        if (!(max_norm >= 0.f) || !(eps >= 0.f && eps < INFINITY)) return PLATTICE_ERR_INVALID;
         for (int i = 0; i < count; ++i) {
             const plattice_grad& g = grads[i];
             if (!dtype_ok(g.out_dtype) || (g.out_dtype != g.dtype && g.out_dtype != PLATTICE_F32)) return PLATTICE_ERR_INVALID;

@@ -15,6 +15,8 @@
 // no atomics but counts.
 #include <cooperative_groups.h>
 
+#include <cmath>
+
 #include "plattice_runtime.h"
 #include "rows_host.h"
 #include "rows_vec.cuh"
@@ -1114,7 +1116,7 @@ extern "C" {
 
 int plattice_embed(void* y, const void* ids, int ids_wide, const void* table, int dtype, float scale, long long count,
                    long long n, int c, void* stream) {
-    if (!dtype_ok(dtype) || !embed_ok(count, n, c)) return PLATTICE_ERR_INVALID;
+    if (!dtype_ok(dtype) || !embed_ok(count, n, c) || !std::isfinite(scale)) return PLATTICE_ERR_INVALID;
     if (count == 0) return PLATTICE_OK;
     if (!y || !ids || !table || !on_elements(ids_wide ? 8 : 4, ids) || !on_elements(dtype_size(dtype), y, table))
         return PLATTICE_ERR_INVALID;
@@ -1140,7 +1142,7 @@ int plattice_embed_backward_workspace_size(long long count, long long n, int c, 
 int plattice_embed_backward(void* grad_table, int table_dtype, const void* grad_y, int dtype, const void* ids,
                             int ids_wide, float scale, void* workspace, size_t workspace_bytes, long long count,
                             long long n, int c, void* stream) {
-    if (!dtype_ok(dtype) || !dtype_ok(table_dtype) || !embed_ok(count, n, c) || count > 0x7fffffff || !grad_table ||
+    if (!dtype_ok(dtype) || !dtype_ok(table_dtype) || !std::isfinite(scale) || !embed_ok(count, n, c) || count > 0x7fffffff || !grad_table ||
         !on_elements(dtype_size(table_dtype), grad_table))
         return PLATTICE_ERR_INVALID;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -407,7 +407,7 @@ bool is_f32(const at::Tensor* t, at::IntArrayRef sizes, const at::Device& d) {
 py::object rows_embed(const py::object& ids_, const py::object& table_, double scale) {
     const at::Tensor *ids = labels_of(ids_), *table = floating(table_);
     if (!ids || !table || table->dim() != 2 || table->size(0) < 1 || table->size(0) > 0x7fffffff || table->size(1) < 1 ||
-        table->size(1) > (1 << 21) || ids->device() != table->device() || !std::isfinite(scale))
+        table->size(1) > (1 << 21) || ids->device() != table->device() || !std::isfinite((float)scale))
         return py::none();
     const c10::cuda::CUDAGuard guard(table->device());
     c10::SmallVector<int64_t, 8> shape(ids->sizes().begin(), ids->sizes().end());
@@ -422,7 +422,7 @@ py::object rows_embed(const py::object& ids_, const py::object& table_, double s
 py::object rows_embed_backward(const py::object& gy_, const py::object& ids_, int64_t n, double scale, int dtype) {
     const at::Tensor *gy = floating(gy_), *ids = labels_of(ids_);
     if (!rows_tensor(gy) || !ids || gy->size(-1) > (1 << 21) || ids->sizes() != gy->sizes().slice(0, gy->dim() - 1) ||
-        ids->device() != gy->device() || ids->numel() > 0x7fffffff || n < 1 || n > 0x7fffffff || !std::isfinite(scale))
+        ids->device() != gy->device() || ids->numel() > 0x7fffffff || n < 1 || n > 0x7fffffff || !std::isfinite((float)scale))
         return py::none();
     const c10::cuda::CUDAGuard guard(gy->device());
     const int64_t c = gy->size(-1), count = ids->numel();

@@ -16,11 +16,15 @@ import torch
 
 from . import _lib
 from .PLOO import _call, _check_input, _lib_h, _raise, _raw_stream, _require
-from .rows import _DTYPES, _check_like, _cpp
+from .rows import _DTYPES, _MOST, _check_like, _cpp
 
 __all__ = ["grad_norm", "clip_grads"]
 
 _SHARED = "(none may share memory with what is written)"
+
+
+def _fits(max_norm):
+    return 0 <= max_norm <= _MOST or max_norm == float("inf")
 
 
 def _listed(tensors, name):
@@ -87,15 +91,15 @@ def clip_grads(tensors, max_norm, out=None, norm=None, eps=1e-6):
     if not isinstance(out, (list, torch.Tensor, type(None))):
         out = list(out)
     cpp = _cpp()
-    if (cpp is not None and type(tensors) is list and type(max_norm) in (float, int) and max_norm >= 0
-            and type(eps) in (float, int) and 0 <= eps < float("inf")
+    if (cpp is not None and type(tensors) is list and type(max_norm) in (float, int) and _fits(max_norm)
+            and type(eps) in (float, int) and 0 <= eps <= _MOST
             and (got := cpp.clip_grads(tensors, tensors if out is None else out, max_norm, eps, norm)) is not None):
         if type(got) is int:
             _raise("plattice_clip_grads", got, f"{len(tensors)} tensors {_SHARED}")
         return got
     tensors = _listed(tensors, "tensors")
-    _require(isinstance(max_norm, (int, float)) and max_norm >= 0, "max_norm must be a number, at least 0")
-    _require(isinstance(eps, (int, float)) and 0 <= eps < float("inf"), "eps must be a finite number, at least 0")
+    _require(isinstance(max_norm, (int, float)) and _fits(max_norm), "max_norm must be a number of float32, at least 0")
+    _require(isinstance(eps, (int, float)) and 0 <= eps <= _MOST, "eps must be a finite number of float32, at least 0")
     if out is None:
         out = tensors
     else:

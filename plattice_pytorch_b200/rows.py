@@ -31,7 +31,6 @@ No reference counterpart.
 """
 import collections
 import ctypes
-import math
 
 import torch
 
@@ -49,6 +48,7 @@ _MAX_CHANNELS = 1 << 30
 _MAX_EMBED = 1 << 21
 _MAX_TOP = 32
 _SCAN_KEEP = 16   # steps between the states that a scan keeps
+_MOST = torch.finfo(torch.float32).max
 
 
 def _width8(c):
@@ -432,7 +432,7 @@ def _check_labels(t, name, shape, device):
 
 
 def _check_scale(scale):
-    _require(isinstance(scale, (int, float)) and math.isfinite(scale), "scale must be a finite number")
+    _require(isinstance(scale, (int, float)) and abs(scale) <= _MOST, "scale must be a finite number of float32")
 
 
 def embed(ids, table, scale=1.0):
@@ -440,7 +440,7 @@ def embed(ids, table, scale=1.0):
     ``table [n, c]`` (at most 2^21 channels), ``ids [...]`` int64 or int32.  A
     label outside ``0..n-1`` (the "ignored" of label maps) gives a row of zeros."""
     cpp = _cpp()
-    if cpp is not None and type(scale) in (float, int) and (got := cpp.rows_embed(ids, table, scale)) is not None:
+    if cpp is not None and type(scale) in (float, int) and abs(scale) <= _MOST and (got := cpp.rows_embed(ids, table, scale)) is not None:
         if type(got) is int:
             _raise("plattice_embed", got, f"ids={tuple(ids.shape)} table={tuple(table.shape)}")
         return got
@@ -464,7 +464,7 @@ def embed_backward(grad_y, ids, n, scale=1.0, dtype=None):
     ``grad_y``'s), row v the sum of ``scale * grad_y`` over the places where
     ``ids`` is v.  Fewer than 2^31 ids."""
     cpp = _cpp()
-    if (cpp is not None and type(scale) in (float, int) and type(n) is int and (dtype is None or dtype in _DTYPES) and 0 < n < 1 << 31
+    if (cpp is not None and type(scale) in (float, int) and abs(scale) <= _MOST and type(n) is int and (dtype is None or dtype in _DTYPES) and 0 < n < 1 << 31
             and (got := cpp.rows_embed_backward(grad_y, ids, n, scale, -1 if dtype is None else _DTYPES[dtype])) is not None):
         if type(got) is int:
             _raise("plattice_embed_backward", got, f"ids={tuple(ids.shape)} n={n} c={grad_y.shape[-1]}")
