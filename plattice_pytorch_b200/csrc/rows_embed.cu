@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(1024) k_small_table(const __grid_constant__ Ta
     extern __shared__ float4 memory[];
     float* tables = reinterpret_cast<float*>(memory);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    const int n = (int)a.n, groups = 32 >> a.lane_bits, bits = a.lane_bits + (V == 4 ? 2 : V == 2 ? 1 : 0), width = 1 << bits,
+    const int n = (int)a.n, groups = 32 >> a.lane_bits, bits = a.lane_bits + (V == 4 ? 2 : 1), width = 1 << bits,
               each = (n + 1) * 32 * V;
     T* rows = reinterpret_cast<T*>(tables + warps * each) + warp * 2 * 32 * width;
     for (int i = threadIdx.x; i < warps * each; i += blockDim.x) tables[i] = 0.f;
@@ -907,9 +907,7 @@ static EmbedPlan embed_plan(int64_t count, int64_t n, int c, int element) {
     p.small = n <= kSmallTable && count >= 512 * n && c * element % 16 == 0;
     if (p.small) {
         // 8 bytes a lane (half the instructions a row) where many warps' copies of that fit
-        const int widest_v = element == 4 || n <= kWideTable ? 8 / element : 4 / element;
-        p.v = widest_v;
-        while (c % p.v) p.v >>= 1;
+        p.v = element == 4 || n <= kWideTable ? 8 / element : 4 / element;
         const int units = c / p.v;
         p.lane_bits = 1;
         while (p.lane_bits < 5 && 1 << p.lane_bits < units) ++p.lane_bits;
@@ -975,8 +973,7 @@ static cudaError_t launch_small(const TableArgs& a, const EmbedPlan& p, cudaStre
 
 template <typename T>
 static cudaError_t small_table(const TableArgs& a, const EmbedPlan& p, cudaStream_t s) {
-    const bool whole = aligned16(a.g) && a.c * sizeof(T) % 16 == 0;
-    if (p.v == 1) return whole ? launch_small<T, 1, true>(a, p, s) : launch_small<T, 1, false>(a, p, s);
+    const bool whole = aligned16(a.g);   // all rows, then: c is in whole 16 bytes
     if (p.v == 2) return whole ? launch_small<T, 2, true>(a, p, s) : launch_small<T, 2, false>(a, p, s);
     if constexpr (sizeof(T) == 2) return whole ? launch_small<T, 4, true>(a, p, s) : launch_small<T, 4, false>(a, p, s);
     return cudaErrorInvalidValue;
