@@ -114,7 +114,7 @@ __device__ __forceinline__ void store_out(void* out, int dtype, bool vec, int64_
 // Where a row has fewer than 32 V channels, several rows go side by side, each
 // group of lanes with a copy.  Warps of a CTA take slabs of 32 V channels first,
 // then rows.  The rows come by asynchronous copies, two blocks of 32 under way
-// (1048576 rows of 64 bfloat16 channels into 21 labels: 51 us, bound by the few warps
+// (1048576 rows of 64 bfloat16 channels into 21 labels: 55 us, bound by the few warps
 // that the copies of the table leave an SM; from loads to registers 63, sorted 210).
 // Rows on no 16-byte boundaries are loaded a block at a time.  kWideTable: labels up to
 // which a lane takes 8 bytes of 16-bit rows.
@@ -919,7 +919,7 @@ static EmbedPlan embed_plan(int64_t count, int64_t n, int c, int element) {
         p.ctas_y = (int)ceil_div(all, p.slabs);
         const int copies = p.warps / p.slabs;
         // each warp has some blocks of 32 rows, so that its table's way in and out is worth it
-        const int64_t need = ceil_div(count, 32 * 4 * (int64_t)copies), most = p.ctas_y < 148 ? 148 / p.ctas_y : 1;
+        const int64_t need = ceil_div(count, 32 * 4 * (int64_t)copies), most = p.ctas_y < kPlanSms ? kPlanSms / p.ctas_y : 1;
         p.ctas = (int)(need < most ? need : most);
         p.bytes = p.ctas > 1 ? (int64_t)p.ctas * n * c * 4 : 0;
         return p;
@@ -935,7 +935,7 @@ static EmbedPlan embed_plan(int64_t count, int64_t n, int c, int element) {
         p.tiles = count <= kClusterSorted ? 0 : (int)ceil_div(count, 256 * p.items);   // 0: by one cluster
     }
     // chunks long enough that few runs cross them, short enough that they fill the device
-    const int64_t want = count * ceil_div(c, 8) / (148 * 2048);
+    const int64_t want = count * ceil_div(c, 8) / (kPlanSms * 2048);
     const int64_t fit = want < 1 ? 8 : want < 16 ? 16 : want > 256 ? 256 : (want + 7) / 8 * 8;
     // (labels with many entries each: longer ones, so that their runs have fewer parts)
     const int64_t run = count / n / 16;

@@ -79,6 +79,11 @@ int rows_status(cudaError_t e, const char* call);
 // PLATTICE_OK (plattice_poll_status's check).
 int rows_poll(const char* call);
 
+// SMs of a B200.  How work is cut into sums goes by this number, not by the device's own,
+// so that the order of the sums, and their bits, are fixed by the sizes wherever they run
+// (on a part of a device, too); how many CTAs go through the cuts goes by sm_count().
+constexpr int kPlanSms = 148;
+
 // SMs of the current device (148 when it cannot be asked).
 int sm_count();
 

@@ -6,9 +6,11 @@
 //   grad_j = g_l ([j = label] - p_j) - g_e p_j (log p_j + entropy) + g_z p_j
 //
 // m and s are kept apart: their sum would lose s beside a large m (rows whose
-// scores are all the type's lowest value, say).  The sum leaves one 1 of the
-// largest score out, so that s = log1p(rest) and the log probability of a
-// confident answer keep their precision.
+// scores are all the type's lowest value, say).  s is log1p of the sum without one 1 of
+// the largest score.  Where that rest is below 1/16 the 1 is left out from the start, so
+// that confident answers keep their precision; else it is added with the others and taken
+// off again, which is off by about one rounding of the sum (relative to a rest of 1/16,
+// four bits: the log probability is then about -1/16, and off by 2^-24).
 //
 // A row is read once and held: few classes by a thread out of shared memory, up to
 // five accesses a lane by a warp in registers, more by the warps of a CTA or a
@@ -17,7 +19,7 @@
 // exponential, and an element costs a bound, a multiply-add, the exponential and two
 // sums, most of them in pairs.  The special function units take 16 elements a clock
 // and SM, 60 us for the 268 M of 8192 x 32768, which take 83 us to read at the copy
-// rate and 95 here.
+// rate and 100 here (108 to 112 behind a kernel whose writes are still in the L2).
 #pragma once
 #include <cooperative_groups.h>
 
