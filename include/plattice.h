@@ -449,7 +449,8 @@ int plattice_scan_backward(const plattice_scan_args* args, void* stream);
  *   grad_j = grad_logp ([j = label] - p_j) - grad_entropy p_j (log p_j + entropy)
  *            + grad_lse p_j      (lse = m + s),
  * each incoming gradient float32 [rows] or NULL (grad_logp needs labels,
- * grad_entropy the forward's entropy); 0 for a row of -inf only. */
+ * grad_entropy the forward's entropy); 0 for a row of -inf only.  A probability
+ * below 2^-126 counts as 0 (but the label's own in 1 - p). */
 #define PLATTICE_MAX_TOP 32
 typedef struct plattice_log_probs_args {
     const void* logits;

@@ -33,7 +33,7 @@ namespace plr {
 namespace cg = cooperative_groups;
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr float kLowest = -200.f;   // of an exponent of 2: beyond it the exponential is 0
+constexpr float kLowest = -200.f;   // of an exponent of 2: the hardware's exponential is 0 from below -126 on
 
 __device__ __forceinline__ int label_of(const LogpArgs& p, int64_t row) { return Labels{p.labels, p.labels_wide}.at(row, p.n); }
 template <typename T> __device__ __forceinline__ const T* lo_of(const LogpArgs& p) { return static_cast<const T*>(p.x); }

@@ -101,6 +101,25 @@ def test_log_probs_of_two_equal_scores(dev, R):
     assert float((r.entropy.double() - np.log(2.0)).abs().max()) < 4 * U
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,n", [(500, 2), (300, 40), (200, 700), (40, 5000), (3, 100000)])
+def test_gradients_of_probabilities_near_zero(dev, R, dtype, rows, n):
+    """Scores as far apart as 200.  A probability below 2^-126 counts as 0: what it is
+    multiplied by, at most |gl| + |ge| (|log p| + entropy) + |gz|, is added to the bound as often;
+    twice, as p relative to the largest score is cut off, which is up to its own size above it."""
+    g = torch.Generator(device=dev).manual_seed(n)
+    x = (torch.randn(rows, n, generator=g, device=dev) * 30).to(dtype)
+    labels = torch.randint(-1, n + 1, (rows,), generator=g, device=dev)
+    gl, ge, gz = (torch.randn(rows, generator=g, device=dev) for _ in range(3))
+    want = LogProbs(x)
+    r = R.log_probs(x, labels)
+    w, e = want.backward(labels, gl, ge, gz)
+    many = gl.abs()[:, None] + ge.abs()[:, None] * (want.logp.abs() + want.entropy) + gz.abs()[:, None]
+    half = half_step(dtype)
+    assert _within(R.log_probs_backward(x, r, labels, gl, ge, gz), w, e + half * w.abs() + ref.tiny(half) + 2.0 ** -125 * many)
+    assert _within(r.entropy, want.entropy[:, 0], want.e_entropy[:, 0] + 2.0 ** -149)
+
+
 # ---------------------------------------------------------------- small tables
 
 # (labels, n, c): one and several slabs of channels, one and several columns of CTAs, one CTA
